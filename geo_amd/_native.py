@@ -37,6 +37,8 @@ _P = ctypes.c_void_p
 _SZ = ctypes.POINTER(ctypes.c_size_t)
 _D = ctypes.POINTER(ConvDesc)
 _O = ctypes.POINTER(Options)
+_I = ctypes.c_int
+_L = ctypes.c_int64
 C_API = {
     "geo_sc_init": (ctypes.c_int, []),
     "geo_sc_stream_table_copy": (ctypes.c_int, [ctypes.c_int, _P, ctypes.c_size_t, _SZ]),
@@ -81,6 +83,21 @@ C_API = {
     "geo_sc_weight_streams_finish": (ctypes.c_int, [_D, _P, _P]),
     "geo_sc_weight_streams_check": (ctypes.c_int, [_D, _P, _P]),
     "geo_sc_conv2d_add_partial_forward_static": (ctypes.c_int, [_D, _P, _P, _P, _P]),
+    "geo_sc_quantize_rows": (ctypes.c_int, [_P, _I] + [_L] * 3 + [_P, _L, _P, _P, _I, _P]),
+    "geo_sc_rms_norm_q8": (ctypes.c_int, [_P] * 3 + [_I] + [_L] * 4 + [ctypes.c_float, _P, _L] + [_P] * 3 + [_I, _P, _P]),
+    "geo_sc_rms_norm_q8_backward_workspace_size": (ctypes.c_int, [_L, _L, _SZ]),
+    "geo_sc_rms_norm_q8_backward": (ctypes.c_int, [_P, _I, _L, _P, _L, _P, _L, _P, _I, _L, _L, _P, _P, _P, _P,
+                                                   ctypes.c_size_t, _P]),
+    "geo_sc_matmul_q8_workspace_size": (ctypes.c_int, [_L] * 3 + [_SZ]),
+    "geo_sc_matmul_q8": (ctypes.c_int, [_P, _L, _P, _P, _L, _P] + [_L] * 3 + [_P, _I, _P, ctypes.c_size_t, _P]),
+    "geo_sc_matmul_q8_backward_workspace_size": (ctypes.c_int, [_L] * 3 + [_I] * 3 + [_SZ]),
+    "geo_sc_matmul_q8_backward": (ctypes.c_int, [_P, _I, _L, _P, _L, _P, _P, _L, _P] + [_L] * 3 + [_P, _I, _P, _I, _P,
+                                                 ctypes.c_size_t, _P]),
+    "geo_sc_distill_topk_workspace_size": (ctypes.c_int, [_L, _L, _SZ]),
+    "geo_sc_distill_topk": (ctypes.c_int, [_P, _I, _L, _P, _I, _P, _I, _L, _L, _I, ctypes.c_float, _I, _P, _P, _P,
+                                           ctypes.c_size_t, _P]),
+    "geo_sc_distill_topk_backward": (ctypes.c_int, [_P, _I, _P, _I, _L, _P, _I, _P, _I, _L, _L, _I, ctypes.c_float, _P,
+                                                    _P, _P]),
 }
 
 _lib = None
@@ -125,7 +142,7 @@ def probe_lib() -> ctypes.CDLL:
 
 
 def module(name: str):
-    """The PyTorch extension module ``sc_extension_cuda`` or ``sc_extension``."""
+    """The PyTorch extension module ``sc_extension_cuda``, ``sc_extension`` or ``sc_dense``."""
     if name not in _modules:
         path = os.path.join(LIBDIR, name + sysconfig.get_config_var("EXT_SUFFIX"))
         if not os.path.isfile(path):

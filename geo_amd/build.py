@@ -5,6 +5,7 @@
 * ``geo_amd/lib/sc_extension_cuda*.so``   - PyTorch module with the reference's GPU op names
 * ``geo_amd/lib/sc_extension*.so``        - PyTorch module with the reference's CPU op name
                                            (runs the same GPU kernels)
+* ``geo_amd/lib/sc_dense*.so``            - PyTorch module of the dense 8-bit layers and the distillation loss
 """
 from __future__ import annotations
 
@@ -21,9 +22,11 @@ LIBDIR = os.path.join(HERE, "lib")
 OBJDIR = os.path.join(LIBDIR, "obj")
 INCLUDE = os.path.join(ROOT, "include")
 
-HIP_SOURCES = ["sc_streams.hip", "sc_conv_fwd.hip", "sc_conv_bwd.hip", "sc_epilogue.hip", "sc_api.hip"]
+HIP_SOURCES = ["sc_streams.hip", "sc_conv_fwd.hip", "sc_conv_bwd.hip", "sc_epilogue.hip", "sc_rows_q8.hip",
+               "sc_matmul_q8.hip", "sc_distill.hip", "sc_api.hip"]
 PROBE_SOURCE = "sc_probe.hip"   # the benchmark's issue-rate probe: a library of its own, outside the C ABI
-TORCH_MODULES = {"sc_extension_cuda": "sc_extension_cuda.cpp", "sc_extension": "sc_extension.cpp"}
+TORCH_MODULES = {"sc_extension_cuda": "sc_extension_cuda.cpp", "sc_extension": "sc_extension.cpp",
+                 "sc_dense": "sc_dense.cpp"}
 
 # gfx950 only; packed-FP32 instruction selection is switched off for every device pass
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall", "-fvisibility=hidden",
@@ -53,7 +56,7 @@ def build_hip_library() -> str:
     os.makedirs(OBJDIR, exist_ok=True)
     sources = [s for s in HIP_SOURCES if os.path.isfile(os.path.join(CSRC, s))]
     objs = [os.path.join(OBJDIR, s.replace(".hip", ".o")) for s in sources]
-    with ThreadPoolExecutor(max_workers=4) as ex:
+    with ThreadPoolExecutor(max_workers=8) as ex:
         list(ex.map(lambda so: _run(["hipcc", *HIPCC_FLAGS, "-c", os.path.join(CSRC, so[0]), "-o", so[1]]),
                     zip(sources, objs)))
     _run(["hipcc", "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-o", lib_path()])
@@ -82,7 +85,7 @@ def build_torch_modules() -> list:
               "-ltorch_python", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"])
         return out
 
-    with ThreadPoolExecutor(max_workers=2) as ex:
+    with ThreadPoolExecutor(max_workers=3) as ex:
         return list(ex.map(one, TORCH_MODULES.items()))
 
 

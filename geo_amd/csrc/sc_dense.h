@@ -1,0 +1,117 @@
+// Shared device code of the kernels on dense matrices (8-bit rows, norm, 8-bit product, distillation): element types,
+// chunks of eight elements, reductions over a wave and over the threads of a row.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "geo_sc.h"
+
+namespace geo_sc {
+
+using f32 = float;
+using bf16 = __bf16;
+using f16 = _Float16;
+
+inline int dtype_bytes(int dtype) { return dtype == GEO_SC_F32 ? 4 : 2; }
+inline bool dtype_known(int dtype) { return dtype == GEO_SC_F32 || dtype == GEO_SC_BF16 || dtype == GEO_SC_F16; }
+
+// Eight consecutive elements, at any alignment that the element has: gfx950 reads and writes 16 bytes at any byte address,
+// so odd row lengths and strides keep the wide accesses.
+constexpr int kChunk = 8;
+
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* p, float (&v)[kChunk])
+{
+    T raw[kChunk];
+    __builtin_memcpy(raw, p, sizeof raw);
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) v[j] = (float)raw[j];
+}
+// the chunk at column c of a row of `cols` columns; `fill` behind the row's end
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* row, int64_t c, int64_t cols, float fill, float (&v)[kChunk])
+{
+    if (c + kChunk <= cols) {
+        load_chunk(row + c, v);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) v[j] = c + j < cols ? (float)row[c + j] : fill;
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* row, int64_t c, int64_t cols, const float (&v)[kChunk])
+{
+    T raw[kChunk];
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) raw[j] = (T)v[j];
+    if (c + kChunk <= cols) {
+        __builtin_memcpy(row + c, raw, sizeof raw);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j)
+        if (c + j < cols) row[c + j] = raw[j];
+}
+// the same with the type known at run time only (one branch for all lanes)
+__device__ __forceinline__ void store_chunk(void* base, int dtype, int64_t offset, int64_t c, int64_t cols, const float (&v)[kChunk])
+{
+    if (dtype == GEO_SC_F32) store_chunk((f32*)base + offset, c, cols, v);
+    else if (dtype == GEO_SC_BF16) store_chunk((bf16*)base + offset, c, cols, v);
+    else store_chunk((f16*)base + offset, c, cols, v);
+}
+__device__ __forceinline__ void load_chunk(const void* base, int dtype, int64_t offset, int64_t c, int64_t cols, float fill,
+                                           float (&v)[kChunk])
+{
+    if (dtype == GEO_SC_F32) load_chunk((const f32*)base + offset, c, cols, fill, v);
+    else if (dtype == GEO_SC_BF16) load_chunk((const bf16*)base + offset, c, cols, fill, v);
+    else load_chunk((const f16*)base + offset, c, cols, fill, v);
+}
+
+// Bits of |v|: as unsigned integers they order like the magnitudes, with infinity above every number and NaN above infinity,
+// so their maximum is the largest magnitude where all are numbers and says where one is not.
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+constexpr uint32_t kInfinityBits = 0x7f800000u;
+
+// Every lane receives the wave's result; the order of the additions is the same on every run.
+__device__ __forceinline__ float wave_sum(float v)
+{
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v)
+{
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+    return v;
+}
+
+// Sum and maximum over the `waves` waves that share a row, in one exchange through LDS.  `turn` alternates between two
+// sets of slots, so that one barrier per call is enough where calls follow each other.
+struct RowSlots {
+    float sum[2][16];
+    uint32_t most[2][16];
+};
+__device__ __forceinline__ void row_reduce(float& sum, uint32_t& most, int waves, RowSlots& slots, int turn)
+{
+    sum = wave_sum(sum);
+    most = wave_max(most);
+    if (waves == 1) return;
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+        slots.sum[turn & 1][wave] = sum;
+        slots.most[turn & 1][wave] = most;
+    }
+    __syncthreads();
+    float s = 0.f;
+    uint32_t m = 0;
+    for (int k = 0; k < waves; ++k) {
+        s += slots.sum[turn & 1][k];
+        m = max(m, slots.most[turn & 1][k]);
+    }
+    sum = s;
+    most = m;
+}
+
+}  // namespace geo_sc

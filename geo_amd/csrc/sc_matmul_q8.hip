@@ -1,0 +1,705 @@
+// Matrix product in 8-bit integers with a scale for each row of either operand, and its gradients.
+//
+//   y[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k]
+//
+// The sum is an exact 32-bit integer (|x w| <= 2^14, so up to 131071 terms); the two scales come in once, at the end.  Integer
+// sums do not depend on their order, so cutting the inner dimension between waves or workgroups changes no result.
+//
+// Gradients, straight through the rounding of the operands (g: gradient of y):
+//   dx[m][k] = sum_n (g[m][n] w_scale[n]) w[n][k],   dw[n][k] = sum_m (g[m][n] x_scale[m]) x[m][k]
+// The 8-bit operand is exact in bf16; the scaled gradient is held as a sum of bf16 terms, one where g is bf16 (it has no
+// more digits itself), two where it is fp16 and three where it is fp32 (24 bits), which makes the inner dimension as many times
+// as long.  Sums in fp32.
+//
+// Both products run on one kernel: the 16x16 matrix instructions of int8 (64 deep) and bf16 (32 deep) take the same 16 bytes per
+// lane of either operand, so tiles are counted in bytes of the inner dimension.
+#include "sc_dense.h"
+
+namespace geo_sc {
+namespace {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+constexpr int kTile = 128;    // bytes of the inner dimension per step of a tile: a line of a row
+constexpr int kUnits = 256;   // compute units
+
+struct TileArgs {
+    const uint8_t *x, *w;              // rows of `inner` bytes each
+    int64_t x_stride, w_stride;        // bytes
+    int64_t rows, cols, inner;
+    int w_steps;                       // w's inner dimension repeats after this many steps (terms of the gradient)
+    const float *x_scale, *w_scale;    // NULL: 1
+    void* y;
+    int dtype;
+    int steps_per_split;
+    uint32_t* partial;                 // [splits][rows][cols] 32-bit sums, or NULL: one split that writes y
+    int tiles_m, tiles_n;
+};
+
+// One load of 16 bytes per lane straight into LDS, lane after lane from `to` on.  (The host's pass over this file knows no
+// such load, and a kernel that it cannot check gets no stub.)
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t from, uint8_t* to, int offset, int uniform_offset)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (LdsPtr)to, 16, offset, uniform_offset, 0, 0);
+#endif
+}
+
+// 16 bytes of a row from byte k on; zeros behind its end.  A piece that passes the end is the row's last 16 bytes, shifted.
+__device__ __forceinline__ v4i load_piece(const uint8_t* row, int64_t k, int64_t inner)
+{
+    unsigned __int128 v = 0;
+    if (inner < 16) {
+#pragma unroll 1
+        for (int64_t j = inner; j-- > k;) v = v << 8 | row[j];
+        return __builtin_bit_cast(v4i, v);
+    }
+    const int64_t at = k + 16 <= inner ? k : inner - 16, shift = k - at;
+    __builtin_memcpy(&v, row + at, 16);
+    return __builtin_bit_cast(v4i, shift < 16 ? v >> (8 * (int)shift) : (unsigned __int128)0);
+}
+
+template <bool INT8>
+struct Matrix;
+template <>
+struct Matrix<true> {
+    typedef v4i Sum;
+    static __device__ __forceinline__ void add(const v4i& a, const v4i& b, Sum& s) { s = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, s, 0, 0, 0); }
+};
+template <>
+struct Matrix<false> {
+    typedef v4f Sum;
+    static __device__ __forceinline__ void add(const v4i& a, const v4i& b, Sum& s)
+    {
+        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), s, 0, 0, 0);
+    }
+};
+
+// four consecutive columns of a row of y
+__device__ __forceinline__ void store_four(void* y, int dtype, int64_t at, int64_t left, const float (&v)[4])
+{
+    const auto put = [&](auto* p) {
+        using T = std::remove_pointer_t<decltype(p)>;
+        T raw[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+        if (left >= 4) {
+            __builtin_memcpy(p + at, raw, sizeof raw);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (r < left) p[at + r] = raw[r];
+        }
+    };
+    if (dtype == GEO_SC_F32) put((f32*)y);
+    else if (dtype == GEO_SC_BF16) put((bf16*)y);
+    else put((f16*)y);
+}
+
+// Scales and stores four sums of consecutive columns, or hands them to the join as they are.
+template <typename Sum>
+__device__ __forceinline__ void finish_four(const TileArgs& a, int split, int64_t m, int64_t n, const Sum& s, float xs, const float (&ws)[4])
+{
+    const int64_t left = a.cols - n;
+    if (m >= a.rows || left <= 0) return;
+    if (a.partial) {
+        uint32_t* out = a.partial + ((int64_t)split * a.rows + m) * a.cols + n;
+        if (left >= 4) {
+            __builtin_memcpy(out, &s, 16);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const auto one = s[r];   // (a bit cast of the element itself takes the vector's first)
+                if (r < left) out[r] = __builtin_bit_cast(uint32_t, one);
+            }
+        }
+        return;
+    }
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs * ws[r];
+    store_four(a.y, a.dtype, m * a.cols + n, left, v);
+}
+
+__device__ __forceinline__ float scale_at(const float* scale, int64_t i, int64_t count) { return scale && i < count ? scale[i] : 1.f; }
+
+// Tiles of BM rows of x by BN rows of w; WM x WN waves, each with (BM / WM) x (BN / WN) outputs in 16x16 squares.  w is the matrix
+// instruction's first operand, so a lane's four sums are consecutive columns of y.
+//
+// A step stages 128 bytes of every row into LDS, its eight 16-byte pieces at positions piece ^ (row & 7): a wave that reads the
+// same piece of 16 rows then meets every bank once per 8 rows.  Two buffers: while one is multiplied the other is filled.
+// DIRECT: rows start at multiples of 16 bytes and the loads write LDS themselves; otherwise, and for a last step
+// that is not whole, through registers.
+template <int BM, int BN, int WM, int WN, bool INT8, bool DIRECT>
+__global__ __launch_bounds__(WM* WN * 64) void k_tiles(TileArgs a)
+{
+    constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, LX = BM / 8 / W, LW = BN / 8 / W;
+    static_assert(LX * W * 8 == BM && LW * W * 8 == BN, "every wave stages as many rows");
+    typedef typename Matrix<INT8>::Sum Sum;
+    __shared__ __align__(16) uint8_t first[(BM + BN) * kTile];
+    __shared__ __align__(16) uint8_t second[(BM + BN) * kTile];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+
+    // Workgroups go to the eight dies in turn: each die takes a contiguous share of the tiles, so that neighbours share its L2,
+    // in strips of eight tiles of rows.
+    int64_t tile;
+    {
+        const int64_t all = (int64_t)a.tiles_m * a.tiles_n, die = blockIdx.x & 7, at = blockIdx.x >> 3;
+        tile = die * (all / 8) + (die < all % 8 ? die : all % 8) + at;
+    }
+    constexpr int kStrip = 8;
+    const int64_t strip = tile / ((int64_t)kStrip * a.tiles_n), inside = tile - strip * kStrip * a.tiles_n;
+    const int64_t height = a.tiles_m - strip * kStrip < kStrip ? a.tiles_m - strip * kStrip : kStrip;
+    const int64_t m0 = (strip * kStrip + inside % height) * BM, n0 = inside / height * BN;
+    const int wm = wave % WM, wn = wave / WM;
+
+    const int steps = (int)((a.inner + kTile - 1) / kTile);
+    const int begin = blockIdx.y * a.steps_per_split;
+    const int end = begin + a.steps_per_split < steps ? begin + a.steps_per_split : steps;
+    const int whole = (int)(a.inner / kTile);   // steps of 128 bytes
+
+    // rows behind the operand's last are read from its last row; their outputs are not stored
+    const int piece = (lane & 7) ^ (lane >> 3);
+    int x_off[LX], w_off[LW];
+#pragma unroll
+    for (int i = 0; i < LX; ++i) {
+        const int64_t r = (int64_t)(i * W + wave) * 8 + (lane >> 3);
+        x_off[i] = (int)((m0 + r < a.rows ? r : a.rows - 1 - m0) * (DIRECT ? a.x_stride : 1)) + (DIRECT ? piece * 16 : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < LW; ++i) {
+        const int64_t r = (int64_t)(i * W + wave) * 8 + (lane >> 3);
+        w_off[i] = (int)((n0 + r < a.cols ? r : a.cols - 1 - n0) * (DIRECT ? a.w_stride : 1)) + (DIRECT ? piece * 16 : 0);
+    }
+    const uint8_t *x0 = a.x + m0 * a.x_stride, *w0 = a.w + n0 * a.w_stride;
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x0), 0, 0x7fffffff, 0x00020000);
+    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(w0), 0, 0x7fffffff, 0x00020000);
+    const auto w_step = [&](int k) { return k % a.w_steps; };
+
+    // step k by loads that write LDS
+    const auto stage_direct = [&](uint8_t* to, int k) {
+        const int xk = k * kTile, wk = w_step(k) * kTile;
+#pragma unroll
+        for (int i = 0; i < LX; ++i)
+            load_to_lds(xr, to + (i * W + wave) * 1024, x_off[i], xk);
+#pragma unroll
+        for (int i = 0; i < LW; ++i)
+            load_to_lds(wr, to + BM * kTile + (i * W + wave) * 1024, w_off[i], wk);
+    };
+    // the same through registers: any alignment, zeros behind the end of a row
+    const auto fetch = [&](v4i(&v)[LX + LW], int k) {
+        const int64_t xk = (int64_t)k * kTile + piece * 16, wk = (int64_t)w_step(k) * kTile + piece * 16;
+#pragma unroll
+        for (int i = 0; i < LX; ++i) v[i] = load_piece(x0 + (DIRECT ? (int64_t)(x_off[i] - piece * 16) : x_off[i] * a.x_stride), xk, a.inner);
+#pragma unroll
+        for (int i = 0; i < LW; ++i) v[LX + i] = load_piece(w0 + (DIRECT ? (int64_t)(w_off[i] - piece * 16) : w_off[i] * a.w_stride), wk, a.inner);
+    };
+    const auto put = [&](uint8_t* to, const v4i(&v)[LX + LW]) {
+#pragma unroll
+        for (int i = 0; i < LX; ++i) *(v4i*)(to + (i * W + wave) * 1024 + lane * 16) = v[i];
+#pragma unroll
+        for (int i = 0; i < LW; ++i) *(v4i*)(to + BM * kTile + (i * W + wave) * 1024 + lane * 16) = v[LX + i];
+    };
+    Sum sum[TN][TM];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int i = 0; i < TM; ++i) sum[j][i] = Sum{0, 0, 0, 0};
+    const int mine[2] = {(lane & 15) * kTile + (((lane >> 4) ^ (lane & 7)) << 4), (lane & 15) * kTile + (((4 + (lane >> 4)) ^ (lane & 7)) << 4)};
+    const auto multiply = [&](const uint8_t* from) {
+        const uint8_t *xs = from + wm * TM * 16 * kTile, *ws = from + (BM + wn * TN * 16) * kTile;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            v4i fx[TM], fw[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fw[j] = *(const v4i*)(ws + j * 16 * kTile + mine[h]);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) fx[i] = *(const v4i*)(xs + i * 16 * kTile + mine[h]);
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int i = 0; i < TM; ++i) Matrix<INT8>::add(fw[j], fx[i], sum[j][i]);
+        }
+    };
+    // what the other waves read next is in LDS, what they have read may be overwritten
+    const auto arrive = [&]() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    const int stop = DIRECT && end > whole ? whole : end;   // a last step that is not whole comes by itself
+    if constexpr (DIRECT) {
+        if (begin < stop) {
+            stage_direct(first, begin);
+            arrive();
+        }
+        int k = begin;
+        for (; k + 1 < stop; k += 2) {
+            stage_direct(second, k + 1);
+            __builtin_amdgcn_sched_barrier(0);   // (the loads leave before the products, not when they are done)
+            multiply(first);
+            arrive();
+            if (k + 2 < stop) stage_direct(first, k + 2);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(second);
+            arrive();
+        }
+        if (k < stop) multiply(first);
+        if (stop < end) {
+            v4i v[LX + LW];
+            fetch(v, stop);
+            put(second, v);   // (its last readers have passed a barrier since)
+            __syncthreads();
+            multiply(second);
+        }
+    } else {
+        v4i v[LX + LW];
+        fetch(v, begin);
+        put(first, v);
+        __syncthreads();
+        uint8_t *now = first, *next = second;
+        for (int k = begin; k < stop; ++k) {
+            if (k + 1 < stop) fetch(v, k + 1);
+            multiply(now);
+            if (k + 1 < stop) put(next, v);
+            __syncthreads();
+            uint8_t* t = now;
+            now = next;
+            next = t;
+        }
+    }
+
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int64_t n = n0 + (wn * TN + j) * 16 + (lane >> 4) * 4;
+        float ws[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ws[r] = scale_at(a.w_scale, n + r, a.cols);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int64_t m = m0 + (wm * TM + i) * 16 + (lane & 15);
+            finish_four(a, blockIdx.y, m, n, sum[j][i], scale_at(a.x_scale, m, a.rows), ws);
+        }
+    }
+}
+
+// Few rows of x (at most 16 MT): y is bound by the one read of w.  A wave reads 128 bytes of 16 NT rows of w per step, 32 per lane,
+// straight into the registers that the matrix instruction takes, and the same bytes of x; a workgroup's waves, and the
+// grid's second dimension, cut the inner dimension, and the sums meet in LDS.
+constexpr int kFewWaves = 8;
+template <int MT, int NT>
+__global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
+{
+    __shared__ __align__(16) v4i sums[kFewWaves][NT * MT][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t n0 = (int64_t)blockIdx.x * 16 * NT;
+    const int row = lane & 15, at = (lane >> 4) * 32;
+    const uint8_t *xp[MT], *wp[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t m = i * 16 + row;
+        xp[i] = a.x + (m < a.rows ? m : a.rows - 1) * a.x_stride + at;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t n = n0 + j * 16 + row;
+        wp[j] = a.w + (n < a.cols ? n : a.cols - 1) * a.w_stride + at;
+    }
+    v4i sum[NT][MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sum[j][i] = v4i{0, 0, 0, 0};
+    const int steps = (int)((a.inner + kTile - 1) / kTile), whole = (int)(a.inner / kTile);
+    const int begin = blockIdx.y * a.steps_per_split;
+    const int end = begin + a.steps_per_split < steps ? begin + a.steps_per_split : steps;
+    const int end_whole = end < whole ? end : whole;
+    const auto step = [&](const v4i (&w)[NT][2], const v4i (&x)[MT][2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) Matrix<true>::add(w[j][h], x[i][h], sum[j][i]);
+    };
+#pragma unroll 4
+    for (int k = begin + wave; k < end_whole; k += kFewWaves) {
+        v4i w[NT][2], x[MT][2];
+        const int64_t o = (int64_t)k * kTile;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) __builtin_memcpy(w[j], wp[j] + o, 32);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) __builtin_memcpy(x[i], xp[i] + o, 32);
+        step(w, x);
+    }
+    if (end > end_whole && (end_whole - begin) % kFewWaves == wave) {   // the last step, where it is not whole
+        v4i w[NT][2], x[MT][2];
+        const int64_t o = (int64_t)end_whole * kTile;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) w[j][h] = load_piece(wp[j] - at, o + at + h * 16, a.inner);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) x[i][h] = load_piece(xp[i] - at, o + at + h * 16, a.inner);
+        }
+        step(w, x);
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sums[wave][j * MT + i][lane] = sum[j][i];
+    __syncthreads();
+    for (int t = wave; t < NT * MT; t += kFewWaves) {
+        v4i s = sums[0][t][lane];
+#pragma unroll
+        for (int k = 1; k < kFewWaves; ++k) s += sums[k][t][lane];
+        const int64_t m = t % MT * 16 + (lane & 15), n = n0 + t / MT * 16 + (lane >> 4) * 4;
+        float ws[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ws[r] = scale_at(a.w_scale, n + r, a.cols);
+        finish_four(a, blockIdx.y, m, n, s, scale_at(a.x_scale, m, a.rows), ws);
+    }
+}
+
+// y from the sums of the splits
+template <bool INT8>
+__global__ __launch_bounds__(256) void k_join_splits(TileArgs a, int splits)
+{
+    const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    const int64_t m = blockIdx.y + (int64_t)blockIdx.z * 65535;
+    const int64_t left = a.cols - n;
+    if (left <= 0 || m >= a.rows) return;
+    typename Matrix<INT8>::Sum s = {0, 0, 0, 0};
+    for (int k = 0; k < splits; ++k) {
+        const uint32_t* p = a.partial + ((int64_t)k * a.rows + m) * a.cols + n;
+        typename Matrix<INT8>::Sum one = {0, 0, 0, 0};
+        if (left >= 4) {
+            __builtin_memcpy(&one, p, 16);
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (r < left) one[r] = __builtin_bit_cast(std::remove_reference_t<decltype(one[0] + one[0])>, p[r]);
+        }
+        s += one;
+    }
+    const float xs = scale_at(a.x_scale, m, a.rows);
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs * scale_at(a.w_scale, n + r, a.cols);
+    store_four(a.y, a.dtype, m * a.cols + n, left, v);
+}
+
+// ---------------------------------------------------------------- which kernel, and how the inner dimension is cut
+
+struct Plan {
+    int few;       // squares of 16 rows of k_few_rows; 0: k_tiles
+    int tile;      // rows and columns of k_tiles' tile
+    int splits, steps_per_split;
+};
+
+Plan plan_of(int64_t rows, int64_t cols, int64_t inner_bytes, bool int8)
+{
+    Plan p = {};
+    const int64_t steps = (inner_bytes + kTile - 1) / kTile;
+    int64_t groups;
+    int64_t least;   // steps that a split has at least
+    if (int8 && rows <= 64) {
+        p.few = (int)((rows + 15) / 16);
+        groups = (cols + 15) / 16;
+        least = kFewWaves;
+    } else {
+        const auto tiles = [&](int64_t t) { return ((rows + t - 1) / t) * ((cols + t - 1) / t); };
+        p.tile = tiles(256) >= kUnits * 3 / 4 ? 256 : 128;
+        groups = tiles(p.tile);
+        least = 8;
+    }
+    int64_t splits = 1;
+    if (groups < kUnits) {
+        splits = kUnits / groups;
+        if (splits > steps / least) splits = steps / least;
+        if (splits < 1) splits = 1;
+        if (splits > 64) splits = 64;
+    }
+    p.steps_per_split = (int)((steps + splits - 1) / splits);
+    p.splits = (int)((steps + p.steps_per_split - 1) / p.steps_per_split);
+    return p;
+}
+
+size_t partial_bytes(const Plan& p, int64_t rows, int64_t cols) { return p.splits > 1 ? (size_t)p.splits * rows * cols * 4 : 0; }
+
+template <int MT>
+void run_few(const TileArgs& a, const Plan& p, hipStream_t s)
+{
+    k_few_rows<MT, 1><<<dim3((uint32_t)((a.cols + 15) / 16), (uint32_t)p.splits), dim3(kFewWaves * 64), 0, s>>>(a);
+}
+
+template <int B, int WM, int WN, bool INT8>
+void run_tiles(const TileArgs& a, const Plan& p, bool direct, hipStream_t s)
+{
+    const dim3 grid((uint32_t)((int64_t)a.tiles_m * a.tiles_n), (uint32_t)p.splits);
+    if (direct) k_tiles<B, B, WM, WN, INT8, true><<<grid, dim3(WM * WN * 64), 0, s>>>(a);
+    else k_tiles<B, B, WM, WN, INT8, false><<<grid, dim3(WM * WN * 64), 0, s>>>(a);
+}
+
+template <bool INT8>
+int run_product(TileArgs a, void* workspace, hipStream_t s)
+{
+    const Plan p = plan_of(a.rows, a.cols, a.inner, INT8);
+    a.steps_per_split = p.steps_per_split;
+    a.partial = p.splits > 1 ? (uint32_t*)workspace : nullptr;
+    if (p.few) {
+        if (p.few == 1) run_few<1>(a, p, s);
+        else if (p.few == 2) run_few<2>(a, p, s);
+        else if (p.few == 3) run_few<3>(a, p, s);
+        else run_few<4>(a, p, s);
+    } else {
+        a.tiles_m = (int)((a.rows + p.tile - 1) / p.tile);
+        a.tiles_n = (int)((a.cols + p.tile - 1) / p.tile);
+        // loads that write LDS take 16-byte addresses, and offsets of 31 bits from the tile's first row
+        const auto fits = [&](const uint8_t* q, int64_t stride) {
+            return (uintptr_t)q % 16 == 0 && stride % 16 == 0 && stride * p.tile + a.inner < 0x7fffffff;
+        };
+        const bool direct = fits(a.x, a.x_stride) && fits(a.w, a.w_stride);
+        if (p.tile == 256) run_tiles<256, 2, 4, INT8>(a, p, direct, s);
+        else run_tiles<128, 2, 2, INT8>(a, p, direct, s);
+    }
+    if (a.partial) {
+        const uint32_t y = (uint32_t)(a.rows < 65535 ? a.rows : 65535), z = (uint32_t)((a.rows + 65534) / 65535);
+        k_join_splits<INT8><<<dim3((uint32_t)((a.cols + 1023) / 1024), y, z), dim3(256), 0, s>>>(a, p.splits);
+    }
+    return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
+}
+
+// ---------------------------------------------------------------- operands of the gradients
+
+// the terms of v: each the bf16 nearest to what the earlier ones leave
+template <int TERMS>
+__device__ __forceinline__ void split_terms(float v, bf16 (&t)[TERMS])
+{
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i) {
+        t[i] = (bf16)v;
+        v -= (float)t[i];
+        if (!(fabsf(v) < __uint_as_float(kInfinityBits))) v = 0.f;   // of an infinity nothing is left
+    }
+}
+
+// out[m][term][n] = terms of g[m][n] scale[n]; `padded` columns per term, zeros behind the last
+template <int TERMS>
+__global__ __launch_bounds__(256) void k_scaled_grad(const void* g, int dtype, int64_t g_stride, const float* scale, int64_t rows,
+                                                     int64_t cols, int64_t padded, bf16* out)
+{
+    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * kChunk;
+    if (c >= padded) return;
+    float k[kChunk];
+    load_chunk(scale, c, cols, 0.f, k);
+    for (int64_t m = blockIdx.y; m < rows; m += gridDim.y) {
+        float v[kChunk];
+        load_chunk(g, dtype, m * g_stride, c, cols, 0.f, v);
+        bf16 t[TERMS][kChunk];
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+            bf16 one[TERMS];
+            split_terms<TERMS>(v[j] * k[j], one);
+#pragma unroll
+            for (int i = 0; i < TERMS; ++i) t[i][j] = one[i];
+        }
+#pragma unroll
+        for (int i = 0; i < TERMS; ++i) __builtin_memcpy(out + (m * TERMS + i) * padded + c, t[i], sizeof t[i]);
+    }
+}
+
+constexpr int kSide = 64;   // a workgroup transposes 64 x 64 elements through LDS
+
+// out[c][term][r] = terms of g[r][c] scale[r]; `padded` rows per term
+template <int TERMS>
+__global__ __launch_bounds__(256) void k_scaled_grad_t(const void* g, int dtype, int64_t g_stride, const float* scale, int64_t rows,
+                                                       int64_t cols, int64_t padded, bf16* out)
+{
+    __shared__ float tile[kSide][kSide + 1];
+    const int64_t r0 = (int64_t)blockIdx.x * kSide, c0 = (int64_t)blockIdx.y * kSide;
+    for (int i = threadIdx.x; i < kSide * kSide / kChunk; i += 256) {
+        const int r = i / (kSide / kChunk), c = i % (kSide / kChunk) * kChunk;
+        float v[kChunk] = {};
+        if (r0 + r < rows && c0 + c < cols) {
+            load_chunk(g, dtype, (r0 + r) * g_stride, c0 + c, cols, 0.f, v);
+            const float k = scale[r0 + r];
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) v[j] *= k;
+        }
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) tile[r][c + j] = v[j];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kSide * kSide / kChunk; i += 256) {
+        const int c = i / (kSide / kChunk), r = i % (kSide / kChunk) * kChunk;
+        if (c0 + c >= cols) continue;
+        bf16 t[TERMS][kChunk];
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+            bf16 one[TERMS];
+            split_terms<TERMS>(tile[r + j][c], one);
+#pragma unroll
+            for (int q = 0; q < TERMS; ++q) t[q][j] = one[q];
+        }
+#pragma unroll
+        for (int q = 0; q < TERMS; ++q) __builtin_memcpy(out + ((c0 + c) * TERMS + q) * padded + r0 + r, t[q], sizeof t[q]);
+    }
+}
+
+// out[c][r] = q[r][c] in bf16, `padded` rows
+__global__ __launch_bounds__(256) void k_widen_t(const int8_t* q, int64_t q_stride, int64_t rows, int64_t cols, int64_t padded, bf16* out)
+{
+    __shared__ float tile[kSide][kSide + 1];
+    const int64_t r0 = (int64_t)blockIdx.x * kSide, c0 = (int64_t)blockIdx.y * kSide;
+    for (int i = threadIdx.x; i < kSide * kSide / kChunk; i += 256) {
+        const int r = i / (kSide / kChunk), c = i % (kSide / kChunk) * kChunk;
+        float v[kChunk] = {};
+        if (r0 + r < rows && c0 + c < cols) load_chunk(q + (r0 + r) * q_stride, c0 + c, cols, 0.f, v);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) tile[r][c + j] = v[j];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kSide * kSide / kChunk; i += 256) {
+        const int c = i / (kSide / kChunk), r = i % (kSide / kChunk) * kChunk;
+        if (c0 + c >= cols) continue;
+        bf16 t[kChunk];
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) t[j] = (bf16)tile[r + j][c];
+        __builtin_memcpy(out + (c0 + c) * padded + r0 + r, t, sizeof t);
+    }
+}
+
+int terms_of(int grad_dtype) { return grad_dtype == GEO_SC_BF16 ? 1 : grad_dtype == GEO_SC_F16 ? 2 : 3; }
+int64_t padded_to_side(int64_t n) { return (n + kSide - 1) / kSide * kSide; }   // whole steps of 64 bf16 elements
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// what one gradient needs: its two operands and the splits' sums.  `depth` is the dimension summed over.
+struct GradLayout {
+    size_t left, right, partial;
+};
+GradLayout grad_layout(int64_t rows, int64_t cols, int64_t depth, int terms)
+{
+    const int64_t p = padded_to_side(depth);
+    GradLayout l;
+    l.left = align256((size_t)rows * terms * p * 2);
+    l.right = align256((size_t)cols * p * 2);
+    l.partial = align256(partial_bytes(plan_of(rows, cols, terms * p * 2, false), rows, cols));
+    return l;
+}
+
+bool sizes_fit(int64_t rows, int64_t cols, int64_t inner)
+{
+    return rows >= 1 && cols >= 1 && inner >= 1 && rows <= 0x3fffffff && cols <= 0x3fffffff && inner <= 131071;
+}
+
+}  // namespace
+}  // namespace geo_sc
+
+using namespace geo_sc;
+
+extern "C" {
+
+int geo_sc_matmul_q8_workspace_size(int64_t rows, int64_t cols, int64_t inner, size_t* bytes)
+{
+    if (!bytes || !sizes_fit(rows, cols, inner)) return GEO_SC_ERR_INVALID_ARGUMENT;
+    *bytes = partial_bytes(plan_of(rows, cols, inner, true), rows, cols);
+    return GEO_SC_OK;
+}
+
+int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride, const float* w_scale,
+                     int64_t rows, int64_t cols, int64_t inner, void* y, int dtype, void* workspace, size_t workspace_bytes,
+                     geo_sc_stream_t stream)
+{
+    if (!sizes_fit(rows, cols, inner) || !dtype_known(dtype) || x_stride < 0 || w_stride < 0 || !x || !w || !x_scale || !w_scale || !y)
+        return GEO_SC_ERR_INVALID_ARGUMENT;
+    size_t need = 0;
+    geo_sc_matmul_q8_workspace_size(rows, cols, inner, &need);
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return GEO_SC_ERR_WORKSPACE;
+    TileArgs a = {};
+    a.x = (const uint8_t*)x;
+    a.w = (const uint8_t*)w;
+    a.x_stride = x_stride;
+    a.w_stride = w_stride;
+    a.rows = rows;
+    a.cols = cols;
+    a.inner = inner;
+    a.w_steps = 0x7fffffff;
+    a.x_scale = x_scale;
+    a.w_scale = w_scale;
+    a.y = y;
+    a.dtype = dtype;
+    return run_product<true>(a, workspace, (hipStream_t)stream);
+}
+
+int geo_sc_matmul_q8_backward_workspace_size(int64_t rows, int64_t cols, int64_t inner, int grad_dtype, int need_dx, int need_dw,
+                                             size_t* bytes)
+{
+    if (!bytes || !sizes_fit(rows, cols, inner) || cols > 131071 || !dtype_known(grad_dtype)) return GEO_SC_ERR_INVALID_ARGUMENT;
+    const int terms = terms_of(grad_dtype);
+    const GradLayout x = grad_layout(rows, inner, cols, terms), w = grad_layout(cols, inner, rows, terms);
+    const size_t bx = need_dx ? x.left + x.right + x.partial : 0, bw = need_dw ? w.left + w.right + w.partial : 0;
+    *bytes = bx > bw ? bx : bw;   // one after the other in the same memory
+    return GEO_SC_OK;
+}
+
+int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64_t grad_stride, const int8_t* x, int64_t x_stride,
+                              const float* x_scale, const int8_t* w, int64_t w_stride, const float* w_scale, int64_t rows, int64_t cols,
+                              int64_t inner, void* dx, int dx_dtype, void* dw, int dw_dtype, void* workspace, size_t workspace_bytes,
+                              geo_sc_stream_t stream)
+{
+    if (!sizes_fit(rows, cols, inner) || cols > 131071 || !dtype_known(grad_dtype) || (dx && !dtype_known(dx_dtype)) ||
+        (dw && !dtype_known(dw_dtype)) || grad_stride < 0 || x_stride < 0 || w_stride < 0 || !grad || (dx && (!w || !w_scale)) ||
+        (dw && (!x || !x_scale)))
+        return GEO_SC_ERR_INVALID_ARGUMENT;
+    if (!dx && !dw) return GEO_SC_OK;
+    size_t need = 0;
+    geo_sc_matmul_q8_backward_workspace_size(rows, cols, inner, grad_dtype, dx != nullptr, dw != nullptr, &need);
+    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16) return GEO_SC_ERR_WORKSPACE;
+    hipStream_t s = (hipStream_t)stream;
+    const int terms = terms_of(grad_dtype);
+    const auto product = [&](int64_t m, int64_t n, int64_t depth, const GradLayout& l, void* y, int dtype) {
+        const int64_t p = padded_to_side(depth);
+        uint8_t* at = (uint8_t*)workspace;
+        TileArgs a = {};
+        a.x = at;
+        a.w = at + l.left;
+        a.x_stride = terms * p * 2;
+        a.w_stride = p * 2;
+        a.rows = m;
+        a.cols = n;
+        a.inner = terms * p * 2;
+        a.w_steps = (int)(p * 2 / kTile);
+        a.y = y;
+        a.dtype = dtype;
+        return run_product<false>(a, at + l.left + l.right, s);
+    };
+    const auto blocks = [](int64_t n) { return (uint32_t)((n + kSide - 1) / kSide); };
+    if (dx) {
+        const GradLayout l = grad_layout(rows, inner, cols, terms);
+        const int64_t p = padded_to_side(cols);
+        bf16 *left = (bf16*)workspace, *right = (bf16*)((uint8_t*)workspace + l.left);
+        const dim3 grid((uint32_t)((p / kChunk + 255) / 256), (uint32_t)(rows < 2048 ? rows : 2048));
+        if (terms == 1) k_scaled_grad<1><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, w_scale, rows, cols, p, left);
+        else if (terms == 2) k_scaled_grad<2><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, w_scale, rows, cols, p, left);
+        else k_scaled_grad<3><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, w_scale, rows, cols, p, left);
+        k_widen_t<<<dim3(blocks(cols), blocks(inner)), dim3(256), 0, s>>>(w, w_stride, cols, inner, p, right);
+        const int rc = product(rows, inner, cols, l, dx, dx_dtype);
+        if (rc != GEO_SC_OK) return rc;
+    }
+    if (dw) {
+        const GradLayout l = grad_layout(cols, inner, rows, terms);
+        const int64_t p = padded_to_side(rows);
+        bf16 *left = (bf16*)workspace, *right = (bf16*)((uint8_t*)workspace + l.left);
+        const dim3 grid(blocks(rows), blocks(cols));
+        if (terms == 1) k_scaled_grad_t<1><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, x_scale, rows, cols, p, left);
+        else if (terms == 2) k_scaled_grad_t<2><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, x_scale, rows, cols, p, left);
+        else k_scaled_grad_t<3><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, x_scale, rows, cols, p, left);
+        k_widen_t<<<dim3(blocks(rows), blocks(inner)), dim3(256), 0, s>>>(x, x_stride, rows, inner, p, right);
+        const int rc = product(cols, inner, rows, l, dw, dw_dtype);
+        if (rc != GEO_SC_OK) return rc;
+    }
+    return GEO_SC_OK;
+}
+
+}  // extern "C"

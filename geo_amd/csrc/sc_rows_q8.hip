@@ -1,0 +1,426 @@
+// Rows in 8 bits with a scale each, and the root-mean-square norm that ends in them.
+//
+//   a = max_j |n_j|,  scale = a / 127,  q_j = round(n_j * 127 / a)   (half to even; a = 0: scale 0 and q 0)
+//   norm: t = x + residual,  r = 1 / sqrt(mean_j t_j^2 + eps),  n_j = t_j r w_j
+//
+// r is common to a row, so it cancels in q: q_j = round(t_j w_j * 127 / max|t w|) and scale = max|t w| r / 127.  The sum of
+// squares and the maximum then need one pass and one exchange between the row's waves, and the row stays in registers
+// from its only read to its only write.
+//
+// Backward of the norm, straight through the rounding, with g the gradient of the values and h that of the sum:
+//   u = g w,   dt = r (u - t r^2 mean(u t)) + h,   dx = dresidual = dt,   dw = sum over the rows of g t r
+#include "sc_dense.h"
+
+namespace geo_sc {
+namespace {
+
+// Reciprocal and scale of a row from the bits of its largest magnitude.  `unit` multiplies the scale (r of a norm, else 1).
+// A row that holds an infinity or NaN becomes q = 0 with scale NaN: its values are NaN.  Magnitudes below 2^-100 are
+// brought up by 2^100 first, where 127 / a would pass the largest float.
+struct RowScale {
+    float lift, inverse, scale;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t bits, float unit, bool sound)
+{
+    RowScale r;
+    const float a = __uint_as_float(bits);
+    r.lift = a < 0x1p-100f ? 0x1p100f : 1.f;
+    r.inverse = a > 0.f ? 127.f / (a * r.lift) : 0.f;
+    r.scale = a * unit * (1.f / 127.f);
+    if (bits >= kInfinityBits || !sound) {
+        r.inverse = 0.f;
+        r.scale = __uint_as_float(0x7fc00000u);
+    }
+    return r;
+}
+
+struct RowsArgs {
+    const void *x, *residual, *weight;
+    int64_t rows, cols, x_stride, residual_stride, q_stride;
+    float eps;
+    int8_t* q;
+    float *scale, *rstd;
+    void *total, *values;
+    int values_dtype;
+};
+
+template <typename T, bool NORM>
+__device__ __forceinline__ void read_chunk(const RowsArgs& a, int64_t row, int64_t c, float (&t)[kChunk])
+{
+    load_chunk((const T*)a.x + row * a.x_stride, c, a.cols, 0.f, t);
+    if constexpr (NORM) {
+        if (a.residual) {
+            float s[kChunk];
+            load_chunk((const T*)a.residual + row * a.residual_stride, c, a.cols, 0.f, s);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) t[j] += s[j];
+        }
+    }
+}
+
+template <typename T, bool NORM>
+__device__ __forceinline__ void write_chunk(const RowsArgs& a, int64_t row, int64_t c, const RowScale& rs, const float (&n)[kChunk])
+{
+    float v[kChunk];
+    int8_t q[kChunk];
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+        // (a NaN's conversion to an integer is whatever the hardware makes of it: such rows write zeros)
+        const float k = rs.inverse == 0.f ? 0.f : rintf(n[j] * rs.lift * rs.inverse);
+        q[j] = (int8_t)(int)k;
+        v[j] = k * rs.scale;
+    }
+    int8_t* out = a.q + row * a.q_stride;
+    if (c + kChunk <= a.cols) {
+        __builtin_memcpy(out + c, q, sizeof q);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j)
+            if (c + j < a.cols) out[c + j] = q[j];
+    }
+    if (a.values) store_chunk(a.values, a.values_dtype, row * a.cols, c, a.cols, v);
+}
+
+// One row per threadIdx.y; the row's blockDim.x threads hold ITEMS chunks of eight columns each in registers (ITEMS 0: the row
+// does not fit and is read a second time, out of L2, after the reduction).
+template <typename T, bool NORM, int ITEMS>
+__global__ __launch_bounds__(1024) void k_rows(RowsArgs a)
+{
+    __shared__ RowSlots slots;
+    const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const bool live = row < a.rows;   // (blocks of several rows have one wave per row: no barrier)
+    const int threads = blockDim.x, t = threadIdx.x, waves = threads >> 6;
+    constexpr int kHeld = ITEMS > 0 ? ITEMS : 1;
+    float n[kHeld][kChunk];
+    float squares = 0.f;
+    uint32_t most = 0;
+    const auto take = [&](int64_t c, float (&v)[kChunk], bool write_total) {
+        read_chunk<T, NORM>(a, row, c, v);
+        if constexpr (NORM) {
+            if (write_total && a.total && a.residual) store_chunk((T*)a.total + row * a.cols, c, a.cols, v);
+            float w[kChunk];
+            load_chunk((const T*)a.weight, c, a.cols, 0.f, w);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+                squares += v[j] * v[j];
+                v[j] *= w[j];
+            }
+        }
+    };
+    if (live) {
+        if constexpr (ITEMS > 0) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i) {
+                const int64_t c = ((int64_t)i * threads + t) * kChunk;
+                if (c < a.cols) {
+                    take(c, n[i], true);
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(n[i][j]));
+                }
+            }
+        } else {
+            for (int64_t c = (int64_t)t * kChunk; c < a.cols; c += (int64_t)threads * kChunk) {
+                take(c, n[0], true);
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(n[0][j]));
+            }
+        }
+    }
+    row_reduce(squares, most, waves, slots, 0);
+    if (!live) return;
+    float unit = 1.f;
+    bool sound = true;
+    if constexpr (NORM) {
+        unit = 1.f / sqrtf(squares / (float)a.cols + a.eps);
+        sound = squares < __uint_as_float(kInfinityBits);
+    }
+    const RowScale rs = row_scale(most, unit, sound);
+    if (t == 0) {
+        a.scale[row] = rs.scale;
+        if (NORM && a.rstd) a.rstd[row] = unit;
+    }
+    if constexpr (ITEMS > 0) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int64_t c = ((int64_t)i * threads + t) * kChunk;
+            if (c < a.cols) write_chunk<T, NORM>(a, row, c, rs, n[i]);
+        }
+    } else {
+        for (int64_t c = (int64_t)t * kChunk; c < a.cols; c += (int64_t)threads * kChunk) {
+            take(c, n[0], false);
+            write_chunk<T, NORM>(a, row, c, rs, n[0]);
+        }
+    }
+}
+
+template <typename T, bool NORM>
+int run_rows(const RowsArgs& a, hipStream_t s)
+{
+    const int64_t chunks = (a.cols + kChunk - 1) / kChunk;
+    int threads = 64;
+    while (threads < 1024 && threads < chunks) threads *= 2;
+    const int64_t items = (chunks + threads - 1) / threads;
+    const int per_block = threads == 64 ? 4 : 1;
+    const dim3 grid((uint32_t)((a.rows + per_block - 1) / per_block)), block(threads, per_block);
+    if (items <= 1) k_rows<T, NORM, 1><<<grid, block, 0, s>>>(a);
+    else if (items <= 2) k_rows<T, NORM, 2><<<grid, block, 0, s>>>(a);
+    else if (items <= 4) k_rows<T, NORM, 4><<<grid, block, 0, s>>>(a);
+    else k_rows<T, NORM, 0><<<grid, block, 0, s>>>(a);
+    return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
+}
+
+template <bool NORM>
+int run_rows(const RowsArgs& a, int dtype, hipStream_t s)
+{
+    if (dtype == GEO_SC_F32) return run_rows<f32, NORM>(a, s);
+    if (dtype == GEO_SC_BF16) return run_rows<bf16, NORM>(a, s);
+    return run_rows<f16, NORM>(a, s);
+}
+
+// ---------------------------------------------------------------- backward of the norm
+
+struct NormBackArgs {
+    const void *grad_values, *grad_total, *total, *weight;
+    int grad_dtype;
+    int64_t rows, cols, grad_stride, grad_total_stride, total_stride;
+    const float* rstd;
+    void *dx;
+    float* partial;   // [blocks][cols]: sums of the weight's gradient, NULL: not wanted
+};
+
+// A block takes every gridDim.x-th row; its threads keep the weight and their columns' sums of the weight's gradient in
+// registers over all rows of the block.
+template <typename T, int ITEMS>
+__global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs a)
+{
+    __shared__ RowSlots slots;
+    const int threads = blockDim.x, t = threadIdx.x, waves = threads >> 6;
+    float w[ITEMS][kChunk], dw[ITEMS][kChunk];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int64_t c = ((int64_t)i * threads + t) * kChunk;
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) w[i][j] = dw[i][j] = 0.f;
+        if (c < a.cols) load_chunk((const T*)a.weight, c, a.cols, 0.f, w[i]);
+    }
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++turn) {
+        const float r = a.rstd[row];
+        float g[ITEMS][kChunk], v[ITEMS][kChunk], along = 0.f;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int64_t c = ((int64_t)i * threads + t) * kChunk;
+            if (c < a.cols) {
+                load_chunk(a.grad_values, a.grad_dtype, row * a.grad_stride, c, a.cols, 0.f, g[i]);
+                load_chunk((const T*)a.total + row * a.total_stride, c, a.cols, 0.f, v[i]);
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    dw[i][j] += g[i][j] * (v[i][j] * r);
+                    g[i][j] *= w[i][j];
+                    along += g[i][j] * v[i][j];
+                }
+            }
+        }
+        uint32_t none = 0;
+        row_reduce(along, none, waves, slots, turn);
+        const float back = along / (float)a.cols * r * r;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int64_t c = ((int64_t)i * threads + t) * kChunk;
+            if (c < a.cols) {
+                float d[kChunk];
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) d[j] = r * (g[i][j] - v[i][j] * back);
+                if (a.grad_total) {
+                    float h[kChunk];
+                    load_chunk((const T*)a.grad_total + row * a.grad_total_stride, c, a.cols, 0.f, h);
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) d[j] += h[j];
+                }
+                store_chunk((T*)a.dx + row * a.cols, c, a.cols, d);
+            }
+        }
+    }
+    if (a.partial) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int64_t c = ((int64_t)i * threads + t) * kChunk;
+            if (c < a.cols) store_chunk(a.partial + (int64_t)blockIdx.x * a.cols, c, a.cols, dw[i]);
+        }
+    }
+}
+
+// Rows that do not fit into a block's registers: dx row by row, read twice; the weight's gradient by columns, see
+// k_weight_grad_columns.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_norm_back_long(NormBackArgs a)
+{
+    __shared__ RowSlots slots;
+    const int threads = blockDim.x, waves = threads >> 6;
+    const int64_t row = blockIdx.x, first = (int64_t)threadIdx.x * kChunk, step = (int64_t)threads * kChunk;
+    const float r = a.rstd[row];
+    float along = 0.f;
+    float g[kChunk], v[kChunk], w[kChunk];
+    const auto take = [&](int64_t c) {
+        load_chunk(a.grad_values, a.grad_dtype, row * a.grad_stride, c, a.cols, 0.f, g);
+        load_chunk((const T*)a.total + row * a.total_stride, c, a.cols, 0.f, v);
+        load_chunk((const T*)a.weight, c, a.cols, 0.f, w);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) g[j] *= w[j];
+    };
+    for (int64_t c = first; c < a.cols; c += step) {
+        take(c);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) along += g[j] * v[j];
+    }
+    uint32_t none = 0;
+    row_reduce(along, none, waves, slots, 0);
+    const float back = along / (float)a.cols * r * r;
+    for (int64_t c = first; c < a.cols; c += step) {
+        take(c);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) g[j] = r * (g[j] - v[j] * back);
+        if (a.grad_total) {
+            load_chunk((const T*)a.grad_total + row * a.grad_total_stride, c, a.cols, 0.f, w);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) g[j] += w[j];
+        }
+        store_chunk((T*)a.dx + row * a.cols, c, a.cols, g);
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void k_weight_grad_columns(NormBackArgs a)
+{
+    const int64_t c = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * kChunk;
+    if (c >= a.cols) return;
+    float dw[kChunk] = {}, g[kChunk], v[kChunk];
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        load_chunk(a.grad_values, a.grad_dtype, row * a.grad_stride, c, a.cols, 0.f, g);
+        load_chunk((const T*)a.total + row * a.total_stride, c, a.cols, 0.f, v);
+        const float r = a.rstd[row];
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) dw[j] += g[j] * (v[j] * r);
+    }
+    store_chunk(a.partial + (int64_t)blockIdx.y * a.cols, c, a.cols, dw);
+}
+
+// dweight[c] = the sum over the blocks' partial sums: 32 columns by 8 shares of the blocks in a workgroup, joined in a fixed order
+constexpr int kJoinCols = 32, kJoinShares = 8;
+template <typename T>
+__global__ __launch_bounds__(kJoinCols * kJoinShares) void k_join_weight_grad(const float* partial, int64_t blocks, int64_t cols, T* dw)
+{
+    __shared__ float sums[kJoinShares][kJoinCols];
+    const int64_t c = (int64_t)blockIdx.x * kJoinCols + threadIdx.x;
+    float s = 0.f;
+    if (c < cols)
+        for (int64_t b = threadIdx.y; b < blocks; b += kJoinShares) s += partial[b * cols + c];
+    sums[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < cols) {
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < kJoinShares; ++k) s += sums[k][threadIdx.x];
+        dw[c] = (T)s;
+    }
+}
+
+constexpr int64_t kHeldBackCols = 2 * 1024 * kChunk;   // columns that a block's registers hold in the backward
+
+// blocks (= partial sums of the weight's gradient) of the backward
+int64_t norm_back_blocks(int64_t rows, int64_t cols)
+{
+    const int64_t most = cols > kHeldBackCols ? 64 : 512;
+    return rows < most ? rows : most;
+}
+
+template <typename T>
+int run_norm_back(const NormBackArgs& a, T* dw, hipStream_t s)
+{
+    const int64_t chunks = (a.cols + kChunk - 1) / kChunk, blocks = norm_back_blocks(a.rows, a.cols);
+    int threads = 64;
+    while (threads < 1024 && threads < chunks) threads *= 2;
+    if (a.cols > kHeldBackCols) {
+        k_norm_back_long<T><<<dim3((uint32_t)a.rows), dim3(1024), 0, s>>>(a);
+        if (a.partial)
+            k_weight_grad_columns<T><<<dim3((uint32_t)((chunks + 255) / 256), (uint32_t)blocks), dim3(256), 0, s>>>(a);
+    } else if (chunks <= threads) {
+        k_norm_back<T, 1><<<dim3((uint32_t)blocks), dim3(threads), 0, s>>>(a);
+    } else {
+        k_norm_back<T, 2><<<dim3((uint32_t)blocks), dim3(threads), 0, s>>>(a);
+    }
+    if (a.partial)
+        k_join_weight_grad<T><<<dim3((uint32_t)((a.cols + kJoinCols - 1) / kJoinCols)), dim3(kJoinCols, kJoinShares), 0, s>>>(
+            a.partial, blocks, a.cols, dw);
+    return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
+}
+
+bool sizes_fit(int64_t rows, int64_t cols) { return rows >= 0 && cols >= 1 && rows <= 0x7fffffff && cols <= 0x7fffffff; }
+
+}  // namespace
+}  // namespace geo_sc
+
+using namespace geo_sc;
+
+extern "C" {
+
+int geo_sc_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_stride, int8_t* q, int64_t q_stride,
+                         float* scale, void* values, int values_dtype, geo_sc_stream_t stream)
+{
+    if (!sizes_fit(rows, cols) || !dtype_known(dtype) || (values && !dtype_known(values_dtype)) || x_stride < 0 || q_stride < cols)
+        return GEO_SC_ERR_INVALID_ARGUMENT;
+    if (rows == 0) return GEO_SC_OK;
+    if (!x || !q || !scale) return GEO_SC_ERR_INVALID_ARGUMENT;
+    RowsArgs a = {};
+    a.x = x;
+    a.rows = rows;
+    a.cols = cols;
+    a.x_stride = x_stride;
+    a.q_stride = q_stride;
+    a.q = q;
+    a.scale = scale;
+    a.values = values;
+    a.values_dtype = values_dtype;
+    return run_rows<false>(a, dtype, (hipStream_t)stream);
+}
+
+int geo_sc_rms_norm_q8(const void* x, const void* residual, const void* weight, int dtype, int64_t rows, int64_t cols,
+                       int64_t x_stride, int64_t residual_stride, float eps, int8_t* q, int64_t q_stride, float* scale,
+                       void* total, void* values, int values_dtype, float* rstd, geo_sc_stream_t stream)
+{
+    if (!sizes_fit(rows, cols) || !dtype_known(dtype) || (values && !dtype_known(values_dtype)) || x_stride < 0 ||
+        residual_stride < 0 || q_stride < cols || !(eps >= 0.f))
+        return GEO_SC_ERR_INVALID_ARGUMENT;
+    if (rows == 0) return GEO_SC_OK;
+    if (!x || !weight || !q || !scale) return GEO_SC_ERR_INVALID_ARGUMENT;
+    const RowsArgs a = {x, residual, weight, rows, cols, x_stride, residual_stride, q_stride, eps, q, scale, rstd, total, values,
+                        values_dtype};
+    return run_rows<true>(a, dtype, (hipStream_t)stream);
+}
+
+int geo_sc_rms_norm_q8_backward_workspace_size(int64_t rows, int64_t cols, size_t* bytes)
+{
+    if (!bytes || !sizes_fit(rows, cols)) return GEO_SC_ERR_INVALID_ARGUMENT;
+    *bytes = (size_t)norm_back_blocks(rows, cols) * (size_t)cols * sizeof(float);
+    return GEO_SC_OK;
+}
+
+int geo_sc_rms_norm_q8_backward(const void* grad_values, int grad_dtype, int64_t grad_stride, const void* grad_total,
+                                int64_t grad_total_stride, const void* total, int64_t total_stride, const void* weight, int dtype,
+                                int64_t rows, int64_t cols, const float* rstd, void* dx, void* dweight, void* workspace,
+                                size_t workspace_bytes, geo_sc_stream_t stream)
+{
+    if (!sizes_fit(rows, cols) || rows < 1 || !dtype_known(dtype) || !dtype_known(grad_dtype) || grad_stride < 0 ||
+        grad_total_stride < 0 || total_stride < 0 || !grad_values || !total || !weight || !rstd || !dx)
+        return GEO_SC_ERR_INVALID_ARGUMENT;
+    size_t need = 0;
+    geo_sc_rms_norm_q8_backward_workspace_size(rows, cols, &need);
+    if (dweight && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 4)) return GEO_SC_ERR_WORKSPACE;
+    const NormBackArgs a = {grad_values, grad_total, total, weight, grad_dtype, rows, cols, grad_stride, grad_total_stride,
+                            total_stride, rstd, dx, dweight ? (float*)workspace : nullptr};
+    hipStream_t s = (hipStream_t)stream;
+    if (dtype == GEO_SC_F32) return run_norm_back<f32>(a, (f32*)dweight, s);
+    if (dtype == GEO_SC_BF16) return run_norm_back<bf16>(a, (bf16*)dweight, s);
+    return run_norm_back<f16>(a, (f16*)dweight, s);
+}
+
+}  // extern "C"

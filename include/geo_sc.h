@@ -462,6 +462,85 @@ GEO_SC_API int geo_sc_conv2d_add_partial_forward_static(const geo_sc_conv_desc* 
                                                         int32_t* y, geo_sc_stream_t stream);
 GEO_SC_API size_t geo_sc_static_workspace_bytes(void);
 
+/*
+ * Dense layers in 8-bit integers and distillation.  No counterpart in the reference, which keeps its 8-bit operands
+ * (utils_functional.py:28-39) in floats on one fixed scale; here rows have a scale each and products are exact integer
+ * sums, the numbers that the bit streams approximate.  Matrices are row-major with their elements side by side; a stride is
+ * the distance of two rows in elements, where none is asked for rows follow each other.  Rows may start at any
+ * multiple of the element; 16-byte aligned rows are the fast way.
+ */
+enum geo_sc_dtype { GEO_SC_F32 = 0, GEO_SC_BF16 = 1, GEO_SC_F16 = 2 };
+enum geo_sc_reduction { GEO_SC_REDUCE_NONE = 0, GEO_SC_REDUCE_SUM = 1, GEO_SC_REDUCE_MEAN = 2 };
+
+/*
+ * Rows in 8 bits: a = max_j |x[j]|, scale = a * (1 / 127), q[j] = round(x[j] * (127 / a)), half to even, in fp32 operations.  A row
+ * of zeros has scale 0; a row that holds an infinity or NaN has scale NaN and q 0.
+ *   values   NULL, or (rows, cols) of values_dtype: q * scale
+ */
+GEO_SC_API int geo_sc_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t x_stride, int8_t* q,
+                                    int64_t q_stride, float* scale, void* values, int values_dtype, geo_sc_stream_t stream);
+
+/*
+ * Root-mean-square norm of x + residual with 8-bit output: t = x + residual, r = 1 / sqrt(mean_j t[j]^2 + eps),
+ * (q, scale) = rows in 8 bits of t[j] r weight[j].  One pass; fp32 inside, t is rounded for `total` only.
+ *   residual        NULL: none
+ *   total           (rows, cols) of dtype: t; NULL: not wanted (nothing is written without a residual: t is x)
+ *   values          NULL, or (rows, cols) of values_dtype: q * scale
+ *   rstd            NULL, or rows floats: r, for the backward
+ * Backward, straight through the rounding to 8 bits, from g (gradient of the values), `grad_total` (of t; NULL: none):
+ * u = g weight, dx = r (u - t r^2 mean(u t)) + grad_total, the gradient of x and of the residual alike; dweight = sum over
+ * the rows of g t r (NULL: not wanted), in an order that does not change from run to run.  `total` is t as the forward wrote it.
+ * Workspace, 4-byte aligned: geo_sc_rms_norm_q8_backward_workspace_size, needed for dweight.
+ */
+GEO_SC_API int geo_sc_rms_norm_q8(const void* x, const void* residual, const void* weight, int dtype, int64_t rows, int64_t cols,
+                                  int64_t x_stride, int64_t residual_stride, float eps, int8_t* q, int64_t q_stride, float* scale,
+                                  void* total, void* values, int values_dtype, float* rstd, geo_sc_stream_t stream);
+GEO_SC_API int geo_sc_rms_norm_q8_backward_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
+GEO_SC_API int geo_sc_rms_norm_q8_backward(const void* grad_values, int grad_dtype, int64_t grad_stride, const void* grad_total,
+                                           int64_t grad_total_stride, const void* total, int64_t total_stride, const void* weight,
+                                           int dtype, int64_t rows, int64_t cols, const float* rstd, void* dx, void* dweight,
+                                           void* workspace, size_t workspace_bytes, geo_sc_stream_t stream);
+
+/*
+ * y[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] of 8-bit x (rows, inner) and w (cols, inner), y (rows, cols) of
+ * dtype.  The sum is exact; inner at most 131071 (it then cannot pass 32 bits).  Workspace, 16-byte aligned:
+ * geo_sc_matmul_q8_workspace_size, which may be 0.
+ * Backward, straight through the rounding of either operand, from g, the gradient of y: dx = (g w_scale) w of (rows, inner),
+ * dw = (g x_scale)^T x of (cols, inner); either may be NULL.  The 8-bit operand enters exactly, the scaled gradient as one bf16
+ * number where g is bf16, as the sum of two where it is fp16, of three where it is fp32; sums in fp32.  cols at most
+ * 131071.
+ */
+GEO_SC_API int geo_sc_matmul_q8_workspace_size(int64_t rows, int64_t cols, int64_t inner, size_t* bytes);
+GEO_SC_API int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
+                                const float* w_scale, int64_t rows, int64_t cols, int64_t inner, void* y, int dtype, void* workspace,
+                                size_t workspace_bytes, geo_sc_stream_t stream);
+GEO_SC_API int geo_sc_matmul_q8_backward_workspace_size(int64_t rows, int64_t cols, int64_t inner, int grad_dtype, int need_dx,
+                                                        int need_dw, size_t* bytes);
+GEO_SC_API int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64_t grad_stride, const int8_t* x, int64_t x_stride,
+                                         const float* x_scale, const int8_t* w, int64_t w_stride, const float* w_scale, int64_t rows,
+                                         int64_t cols, int64_t inner, void* dx, int dx_dtype, void* dw, int dw_dtype, void* workspace,
+                                         size_t workspace_bytes, geo_sc_stream_t stream);
+
+/*
+ * Distillation from a teacher's top logits at temperature T: per row p = softmax of the entries' top_logits / T, q = softmax of
+ * logits / T over all columns, loss = T^2 sum_k p_k (log p_k - log q[top_index_k]).  top_logits and top_index are (rows, top) without
+ * gaps, top at most 4096, index_bytes 4 or 8; an entry whose index is outside [0, cols) is absent, a column named twice counts
+ * twice.  A row without entries has loss 0 and gradient 0.
+ *   loss     rows floats (GEO_SC_REDUCE_NONE), or one: the rows' sum or mean (all rows count), in a fixed order
+ *   stats    rows * 4 floats for the backward
+ * Backward: grad points to rows floats or one, as loss does; dlogits (rows, cols) of the logits' dtype.
+ * Workspace, 4-byte aligned: geo_sc_distill_topk_workspace_size.
+ */
+GEO_SC_API int geo_sc_distill_topk_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
+GEO_SC_API int geo_sc_distill_topk(const void* logits, int dtype, int64_t logits_stride, const void* top_logits, int top_dtype,
+                                   const void* top_index, int index_bytes, int64_t rows, int64_t cols, int top, float temperature,
+                                   int reduction, float* loss, float* stats, void* workspace, size_t workspace_bytes,
+                                   geo_sc_stream_t stream);
+GEO_SC_API int geo_sc_distill_topk_backward(const float* grad, int reduction, const void* logits, int dtype, int64_t logits_stride,
+                                            const void* top_logits, int top_dtype, const void* top_index, int index_bytes,
+                                            int64_t rows, int64_t cols, int top, float temperature, const float* stats, void* dlogits,
+                                            geo_sc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

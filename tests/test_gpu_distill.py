@@ -1,0 +1,194 @@
+"""The distillation loss from a teacher's top logits and its gradient against their formulas in 64 bits.
+
+Tolerances: U = 2^-24, EPS the half unit of the output's type.  With D the largest |z - max z| / T that has weight, a row's sum of
+exponentials is within (cols / 64 + 64 + 4 D) U of itself (chains of additions, the scaled difference and the exponential)."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+EPS = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}   # 2^-24, 2^-8, 2^-11
+SMALL = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -25}   # (exponentials below 2^-126 are zero)
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def uf():
+    assert torch.cuda.is_available(), "these tests need the GPU"
+    from geo_amd import utils_functional as m
+    return m
+
+
+def inputs(rows, cols, top, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    shared = torch.randn(rows, cols, generator=g) * 2
+    t = (shared + 0.5 * torch.randn(rows, cols, generator=g)).topk(top, dim=1)
+    return (shared + torch.randn(rows, cols, generator=g)).to(dtype).cuda(), t.values.to(dtype).cuda(), t.indices.cuda()
+
+
+def formula(z, t, index, temperature):
+    """rows' losses and their gradients with respect to z, in 64 bits, one row after the other"""
+    z = z.double()
+    loss, grad = torch.zeros(z.shape[0], dtype=torch.float64, device=z.device), torch.zeros_like(z)
+    for r in range(z.shape[0]):
+        there = (index[r] >= 0) & (index[r] < z.shape[1])
+        log_q = torch.log_softmax(z[r] / temperature, 0)
+        values, at = t[r][there].double(), index[r][there].long()
+        if at.numel() == 0 or (values == -torch.inf).all():
+            continue
+        log_p = torch.log_softmax(values / temperature, 0)
+        live = log_p > -torch.inf
+        p = log_p.exp()
+        loss[r] = temperature ** 2 * (p * (log_p - log_q[at]))[live].sum()
+        grad[r] = temperature * (log_q.exp().index_add(0, at, -p))
+    return loss, grad
+
+
+def check(uf, z, t, index, temperature):
+    z = z.detach().requires_grad_(True)
+    dtype, cols = z.dtype, z.shape[1]
+    want, want_z = formula(z.detach(), t, index, temperature)
+    loss = uf.distill_topk(z, t, index, temperature=temperature, reduction="none")
+    spread = ((z.detach().double().amax(1) - z.detach().double().clamp(min=-1e4).amin(1)) / temperature).clamp(max=128.0)
+    rel = (cols / 64 + 64 + 8 * spread) * U
+    assert loss.dtype == torch.float32
+    bad = ((loss.double() - want).abs() > temperature ** 2 * (4 * rel + 8 * U * want.abs() / temperature ** 2)) & want.isfinite()
+    assert not bad.any() and torch.equal(loss.isinf(), want.isinf()), (loss[bad], want[bad])
+    g = torch.linspace(-2, 3, z.shape[0], device="cuda")
+    dz, = torch.autograd.grad(loss, z, g)
+    want_z = want_z * g.double()[:, None]
+    q = torch.softmax(z.detach().double() / temperature, 1)
+    size = (g.double().abs() * temperature)[:, None] * torch.maximum(q, (want_z / (g.double() * temperature + 1e-300)[:, None]).abs() + q)
+    tolerance = EPS[dtype] * want_z.abs() + 4 * rel[:, None] * size + SMALL[dtype] * 4
+    bad = (dz.double() - want_z).abs() > tolerance
+    assert not bad.any(), ((dz.double() - want_z).abs() / tolerance).max().item()
+    return want, want_z
+
+
+# one column; the classes of a small classifier; sizes around a chunk, a wave, a workgroup's stride, a split; long and odd
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1, 1), (256, 10, 5), (5, 63, 63), (3, 513, 7), (70, 1030, 130), (2, 8192, 64), (3, 8193, 1), (1, 100003, 33),
+                                   (1100, 257, 3)])
+@pytest.mark.parametrize("temperature", [1.0, 3.5])
+def test_loss_and_gradient(uf, dtype, shape, temperature):
+    check(uf, *inputs(*shape, dtype), temperature)
+
+
+@pytest.mark.parametrize("index_type", [torch.int32, torch.int64])
+def test_absent_entries_repeated_columns_and_empty_rows(uf, index_type):
+    for cols in (40, 20000):
+        z, t, index = inputs(8, cols, 9, torch.float32, seed=cols)
+        index = index.to(index_type)
+        index[1] = -1                       # no entries
+        index[2, 4:] = -1                   # fewer
+        index[3, 5] = cols                  # outside
+        index[4, 3] = index[4, 0]           # a column twice, and one four times
+        index[5, 4:8] = index[5, 1]
+        t[6, 2] = -torch.inf                # weight zero
+        t[7] = -torch.inf                   # weight zero everywhere
+        want, want_z = check(uf, z, t, index, 2.0)
+        assert want[1] == 0 and want[7] == 0 and (want_z[1] == 0).all() and (want_z[7] == 0).all()
+        z = z.requires_grad_(True)
+        dz, = torch.autograd.grad(uf.distill_topk(z, t, index, temperature=2.0, reduction="sum"), z)
+        assert (dz[1] == 0).all() and (dz[7] == 0).all()
+
+
+def test_masked_columns_and_extreme_logits(uf):
+    for dtype in TYPES:
+        z, t, index = inputs(6, 300, 6, torch.float32, seed=3)
+        keep = torch.zeros(6, 300, dtype=torch.bool, device="cuda").scatter_(1, index, True)
+        z[0].masked_fill_(~keep[0], -torch.inf)                    # columns that the student cannot take
+        z[1].masked_fill_(~keep[1], torch.finfo(dtype).min)        # masked with the type's lowest value
+        z[2, index[2, 0]] = -torch.inf                             # the teacher wants one of them: infinite loss
+        z[3, index[3, 0]] = 1000.0                                 # all weight in one column
+        z[4] = 7.0                                                 # all equal
+        z[5] *= 30
+        check(uf, z.to(dtype), t, index, 1.0)
+    z, t, index = inputs(3, 50, 4, torch.float32, seed=4)
+    z[0, 3] = float("nan")
+    z[1] = -torch.inf
+    z = z.requires_grad_(True)
+    loss = uf.distill_topk(z, t, index, reduction="none")
+    dz, = torch.autograd.grad(loss.sum(), z)
+    assert torch.isnan(loss[:2]).all() and torch.isnan(dz[:2]).all() and torch.isfinite(dz[2]).all()
+
+
+def test_reductions_strides_and_runs(uf):
+    z, t, index = inputs(77, 500, 12, torch.bfloat16, seed=5)
+    z = z.requires_grad_(True)
+    rows = uf.distill_topk(z, t, index, reduction="none")
+    total, mean = uf.distill_topk(z, t, index, reduction="sum"), uf.distill_topk(z, t, index)
+    assert abs(total.item() - rows.double().sum().item()) <= 77 * U * rows.double().abs().sum().item()
+    assert abs(mean.item() - rows.double().mean().item()) <= 78 * U * rows.double().abs().mean().item()
+    scale = torch.tensor(128.0, device="cuda")
+    first, = torch.autograd.grad(mean, z, scale, retain_graph=True)
+    per_row, = torch.autograd.grad(rows, z, torch.full_like(rows, 128.0 / 77))
+    assert (first.double() - per_row.double()).abs().max() <= 2 * EPS[torch.bfloat16] * per_row.double().abs().max()
+    wide = torch.zeros(77, 512, dtype=torch.bfloat16, device="cuda")
+    wide[:, 3:503] = z.detach()
+    part = wide[:, 3:503].requires_grad_(True)
+    loss = uf.distill_topk(part, t, index)
+    dz, = torch.autograd.grad(loss, part, scale)
+    assert torch.equal(loss, mean) and torch.equal(dz, first)
+    for _ in range(3):
+        again = uf.distill_topk(z, t, index)
+        dz, = torch.autograd.grad(again, z, scale)
+        assert torch.equal(again, mean) and torch.equal(dz, first)
+    three = uf.distill_topk(z.detach()[:76].reshape(4, 19, 500), t[:76].reshape(4, 19, 12), index[:76].reshape(4, 19, 12), reduction="none")
+    assert torch.equal(three.reshape(76), rows[:76])
+
+
+def test_gradient_against_differences_of_the_loss(uf):
+    """central differences of the kernel's own loss (fp32: the loss rounds to a few U, a step of 1/64 leaves 1e-4)"""
+    z, t, index = inputs(2, 30, 5, torch.float32, seed=6)
+    z = z.requires_grad_(True)
+    dz, = torch.autograd.grad(uf.distill_topk(z, t, index, temperature=2.0, reduction="sum"), z)
+    step = 2.0 ** -6
+    for c in range(0, 30, 4):
+        e = torch.zeros_like(z)
+        e[:, c] = step
+        with torch.no_grad():
+            up, down = (uf.distill_topk(z + s * e, t, index, temperature=2.0, reduction="none").double() for s in (1, -1))
+        assert ((up - down) / (2 * step) - dz[:, c].double()).abs().max() < 1e-3
+
+
+def test_in_a_graph(uf):
+    z, t, index = inputs(40, 9000, 16, torch.bfloat16, seed=7)
+    z = z.requires_grad_(True)
+    uf.distill_topk(z, t, index).backward()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(uf.distill_topk(z, t, index), z)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = uf.distill_topk(z, t, index)
+        dz, = torch.autograd.grad(loss, z)
+    for seed in range(3):
+        with torch.no_grad():
+            z.copy_(inputs(40, 9000, 16, torch.bfloat16, seed=20 + seed)[0])
+        want = uf.distill_topk(z, t, index)
+        want_z, = torch.autograd.grad(want, z)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(loss, want) and torch.equal(dz, want_z)
+
+
+def test_refusals(uf):
+    z, t, index = inputs(4, 20, 3, torch.float32)
+    bad = [lambda: uf.distill_topk(z.cpu(), t, index), lambda: uf.distill_topk(z.double(), t, index), lambda: uf.distill_topk(z, t[:2], index[:2]),
+           lambda: uf.distill_topk(z, t, index[:, :2]), lambda: uf.distill_topk(z, t, index.short()), lambda: uf.distill_topk(z, t, index, temperature=0.0),
+           lambda: uf.distill_topk(z, t.double(), index), lambda: uf.distill_topk(z[0], t[0], index[0]), lambda: uf.distill_topk(z[:0], t[:0], index[:0]),
+           lambda: uf.distill_topk(z, t[:, :0], index[:, :0]), lambda: uf.distill_topk(z, t.cpu(), index),
+           lambda: uf.distill_topk(z, torch.zeros(4, 4097, device="cuda"), torch.zeros(4, 4097, dtype=torch.int32, device="cuda")),
+           lambda: uf.distill_topk(z, t, index, temperature=float("nan"))]
+    for i, f in enumerate(bad):
+        with pytest.raises(RuntimeError):
+            f()
+            pytest.fail(f"call {i} was not refused")
+    with pytest.raises(ValueError, match="reduction"):
+        uf.distill_topk(z, t, index, reduction="batchmean")
