@@ -23,18 +23,20 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef __bf16 v8b __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* LdsPtr;
 
-constexpr int kTile = 128;    // bytes of the inner dimension per step of a tile: a line of a row
+constexpr int kStage = 64;    // bytes of the inner dimension per stage: one matrix instruction deep
+template <int N>
+using Int = std::integral_constant<int, N>;
 constexpr int kUnits = 256;   // compute units
 
 struct TileArgs {
     const uint8_t *x, *w;              // rows of `inner` bytes each
     int64_t x_stride, w_stride;        // bytes
     int64_t rows, cols, inner;
-    int w_steps;                       // w's inner dimension repeats after this many steps (terms of the gradient)
+    int w_stages;                      // w's inner dimension repeats after this many stages (terms of the gradient)
     const float *x_scale, *w_scale;    // NULL: 1
     void* y;
     int dtype;
-    int steps_per_split;
+    int stages_per_split;
     uint32_t* partial;                 // [splits][rows][cols] 32-bit sums, or NULL: one split that writes y
     int tiles_m, tiles_n;
 };
@@ -68,6 +70,10 @@ template <>
 struct Matrix<true> {
     typedef v4i Sum;
     static __device__ __forceinline__ void add(const v4i& a, const v4i& b, Sum& s) { s = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, s, 0, 0, 0); }
+    static __device__ __forceinline__ void add_in_place(const v4i& a, const v4i& b, Sum& s)
+    {
+        asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(s) : "v"(a), "v"(b));
+    }
 };
 template <>
 struct Matrix<false> {
@@ -75,6 +81,10 @@ struct Matrix<false> {
     static __device__ __forceinline__ void add(const v4i& a, const v4i& b, Sum& s)
     {
         s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), s, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void add_in_place(const v4i& a, const v4i& b, Sum& s)
+    {
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(s) : "v"(a), "v"(b));
     }
 };
 
@@ -127,18 +137,30 @@ __device__ __forceinline__ float scale_at(const float* scale, int64_t i, int64_t
 // Tiles of BM rows of x by BN rows of w; WM x WN waves, each with (BM / WM) x (BN / WN) outputs in 16x16 squares.  w is the matrix
 // instruction's first operand, so a lane's four sums are consecutive columns of y.
 //
-// A step stages 128 bytes of every row into LDS, its eight 16-byte pieces at positions piece ^ (row & 7): a wave that reads the
-// same piece of 16 rows then meets every bank once per 8 rows.  Two buffers: while one is multiplied the other is filled.
-// DIRECT: rows start at multiples of 16 bytes and the loads write LDS themselves; otherwise, and for a last step
-// that is not whole, through registers.
+// A stage is 64 bytes of every row, one matrix instruction deep, in LDS as four 16-byte pieces per row at positions
+// piece ^ (row / 4 & 3): the 16 lanes that read the same piece of 16 rows meet every bank once.
+// DIRECT: rows start at multiples of 16 bytes and the loads write LDS themselves, into a ring of kRing stages: while a wave
+// multiplies stage s out of registers, stage s + 1 moves from LDS to its other registers and the stages up to s + kRing are on their
+// way.  One barrier per stage: it says that every wave's share of stage s + 1 has come and that all have read stage s,
+// whose place stage s + kRing takes.  Otherwise, and for a last stage that is not whole, through registers.
+constexpr int kRing = 4;
+
 template <int BM, int BN, int WM, int WN, bool INT8, bool DIRECT>
 __global__ __launch_bounds__(WM* WN * 64) void k_tiles(TileArgs a)
 {
-    constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, LX = BM / 8 / W, LW = BN / 8 / W;
-    static_assert(LX * W * 8 == BM && LW * W * 8 == BN, "every wave stages as many rows");
+    constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, LX = BM / 16 / W, LW = BN / 16 / W;
+    static_assert(LX * W * 16 == BM && LW * W * 16 == BN, "every wave stages as many rows");
     typedef typename Matrix<INT8>::Sum Sum;
-    __shared__ __align__(16) uint8_t first[(BM + BN) * kTile];
-    __shared__ __align__(16) uint8_t second[(BM + BN) * kTile];
+    // (arrays of their own, not one: the compiler keeps reads of one apart from loads into another)
+    constexpr int kBytes = (BM + BN) * kStage;
+    __shared__ __align__(16) uint8_t ring0[kBytes], ring1[kBytes], ring2[kBytes], ring3[kBytes];
+    const auto place = [&](auto which) -> uint8_t* {
+        constexpr int r = decltype(which)::value % kRing;
+        if constexpr (r == 0) return ring0;
+        else if constexpr (r == 1) return ring1;
+        else if constexpr (r == 2) return ring2;
+        else return ring3;
+    };
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
 
     // Workgroups go to the eight dies in turn: each die takes a contiguous share of the tiles, so that neighbours share its L2,
@@ -154,113 +176,150 @@ __global__ __launch_bounds__(WM* WN * 64) void k_tiles(TileArgs a)
     const int64_t m0 = (strip * kStrip + inside % height) * BM, n0 = inside / height * BN;
     const int wm = wave % WM, wn = wave / WM;
 
-    const int steps = (int)((a.inner + kTile - 1) / kTile);
-    const int begin = blockIdx.y * a.steps_per_split;
-    const int end = begin + a.steps_per_split < steps ? begin + a.steps_per_split : steps;
-    const int whole = (int)(a.inner / kTile);   // steps of 128 bytes
+    const int stages = (int)((a.inner + kStage - 1) / kStage);
+    const int begin = blockIdx.y * a.stages_per_split;
+    const int end = begin + a.stages_per_split < stages ? begin + a.stages_per_split : stages;
+    const int whole = (int)(a.inner / kStage);
 
-    // rows behind the operand's last are read from its last row; their outputs are not stored
-    const int piece = (lane & 7) ^ (lane >> 3);
-    int x_off[LX], w_off[LW];
-#pragma unroll
-    for (int i = 0; i < LX; ++i) {
-        const int64_t r = (int64_t)(i * W + wave) * 8 + (lane >> 3);
-        x_off[i] = (int)((m0 + r < a.rows ? r : a.rows - 1 - m0) * (DIRECT ? a.x_stride : 1)) + (DIRECT ? piece * 16 : 0);
-    }
-#pragma unroll
-    for (int i = 0; i < LW; ++i) {
-        const int64_t r = (int64_t)(i * W + wave) * 8 + (lane >> 3);
-        w_off[i] = (int)((n0 + r < a.cols ? r : a.cols - 1 - n0) * (DIRECT ? a.w_stride : 1)) + (DIRECT ? piece * 16 : 0);
-    }
+    // a wave's loads of a stage: 16 rows each, a lane a piece; rows behind the operand's last are read from its last
+    // row, their outputs are not stored
+    const int piece = (lane & 3) ^ (lane >> 4);
     const uint8_t *x0 = a.x + m0 * a.x_stride, *w0 = a.w + n0 * a.w_stride;
-    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x0), 0, 0x7fffffff, 0x00020000);
-    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(w0), 0, 0x7fffffff, 0x00020000);
-    const auto w_step = [&](int k) { return k % a.w_steps; };
-
-    // step k by loads that write LDS
-    const auto stage_direct = [&](uint8_t* to, int k) {
-        const int xk = k * kTile, wk = w_step(k) * kTile;
-#pragma unroll
-        for (int i = 0; i < LX; ++i)
-            load_to_lds(xr, to + (i * W + wave) * 1024, x_off[i], xk);
-#pragma unroll
-        for (int i = 0; i < LW; ++i)
-            load_to_lds(wr, to + BM * kTile + (i * W + wave) * 1024, w_off[i], wk);
+    const auto row_of = [&](int64_t first, int64_t rows, int i) {
+        const int64_t r = (int64_t)(i * W + wave) * 16 + (lane >> 2);
+        return first + r < rows ? r : rows - 1 - first;
+    };
+    const auto w_stage = [&](int k) {   // (at most three terms)
+        if (k >= a.w_stages) k -= a.w_stages;
+        return k >= a.w_stages ? k - a.w_stages : k;
     };
     // the same through registers: any alignment, zeros behind the end of a row
     const auto fetch = [&](v4i(&v)[LX + LW], int k) {
-        const int64_t xk = (int64_t)k * kTile + piece * 16, wk = (int64_t)w_step(k) * kTile + piece * 16;
+        const int64_t xk = (int64_t)k * kStage + piece * 16, wk = (int64_t)w_stage(k) * kStage + piece * 16;
 #pragma unroll
-        for (int i = 0; i < LX; ++i) v[i] = load_piece(x0 + (DIRECT ? (int64_t)(x_off[i] - piece * 16) : x_off[i] * a.x_stride), xk, a.inner);
+        for (int i = 0; i < LX; ++i) v[i] = load_piece(x0 + row_of(m0, a.rows, i) * a.x_stride, xk, a.inner);
 #pragma unroll
-        for (int i = 0; i < LW; ++i) v[LX + i] = load_piece(w0 + (DIRECT ? (int64_t)(w_off[i] - piece * 16) : w_off[i] * a.w_stride), wk, a.inner);
+        for (int i = 0; i < LW; ++i) v[LX + i] = load_piece(w0 + row_of(n0, a.cols, i) * a.w_stride, wk, a.inner);
     };
     const auto put = [&](uint8_t* to, const v4i(&v)[LX + LW]) {
 #pragma unroll
         for (int i = 0; i < LX; ++i) *(v4i*)(to + (i * W + wave) * 1024 + lane * 16) = v[i];
 #pragma unroll
-        for (int i = 0; i < LW; ++i) *(v4i*)(to + BM * kTile + (i * W + wave) * 1024 + lane * 16) = v[LX + i];
+        for (int i = 0; i < LW; ++i) *(v4i*)(to + BM * kStage + (i * W + wave) * 1024 + lane * 16) = v[LX + i];
     };
     Sum sum[TN][TM];
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int i = 0; i < TM; ++i) sum[j][i] = Sum{0, 0, 0, 0};
-    const int mine[2] = {(lane & 15) * kTile + (((lane >> 4) ^ (lane & 7)) << 4), (lane & 15) * kTile + (((4 + (lane >> 4)) ^ (lane & 7)) << 4)};
-    const auto multiply = [&](const uint8_t* from) {
-        const uint8_t *xs = from + wm * TM * 16 * kTile, *ws = from + (BM + wn * TN * 16) * kTile;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            v4i fx[TM], fw[TN];
-#pragma unroll
-            for (int j = 0; j < TN; ++j) fw[j] = *(const v4i*)(ws + j * 16 * kTile + mine[h]);
-#pragma unroll
-            for (int i = 0; i < TM; ++i) fx[i] = *(const v4i*)(xs + i * 16 * kTile + mine[h]);
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int i = 0; i < TM; ++i) Matrix<INT8>::add(fw[j], fx[i], sum[j][i]);
-        }
+    const int mine = (lane & 15) * kStage + (((lane >> 4) ^ (lane >> 2 & 3)) << 4);
+    const int mine_x = wm * TM * 16 * kStage + mine, mine_w = (BM + wn * TN * 16) * kStage + mine;
+    // fragments: TN of w, then TM of x
+    const auto read_one = [&](v4i(&f)[TM + TN], const uint8_t* from, int t) {
+        f[t] = *(const v4i*)(from + (t < TN ? mine_w + t * 16 * kStage : mine_x + (t - TN) * 16 * kStage));
     };
-    // what the other waves read next is in LDS, what they have read may be overwritten
-    const auto arrive = [&]() {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
+    const auto read = [&](v4i(&f)[TM + TN], const uint8_t* from) {
+#pragma unroll
+        for (int t = 0; t < TM + TN; ++t) read_one(f, from, t);
     };
-    const int stop = DIRECT && end > whole ? whole : end;   // a last step that is not whole comes by itself
+    const auto multiply_one = [&](const v4i(&f)[TM + TN], int t) { Matrix<INT8>::add_in_place(f[t / TM], f[TN + t % TM], sum[t / TM][t % TM]); };
+    const auto multiply = [&](const v4i(&f)[TM + TN]) {
+#pragma unroll
+        for (int t = 0; t < TM * TN; ++t) multiply_one(f, t);
+    };
+    const int stop = DIRECT && end > whole ? whole : end;   // a last stage that is not whole comes by itself
     if constexpr (DIRECT) {
+        int x_off[LX], w_off[LW];
+#pragma unroll
+        for (int i = 0; i < LX; ++i) x_off[i] = (int)(row_of(m0, a.rows, i) * a.x_stride) + piece * 16;
+#pragma unroll
+        for (int i = 0; i < LW; ++i) w_off[i] = (int)(row_of(n0, a.cols, i) * a.w_stride) + piece * 16;
+        const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x0), 0, 0x7fffffff, 0x00020000);
+        const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(w0), 0, 0x7fffffff, 0x00020000);
+        const auto load_one = [&](uint8_t* to, int xk, int wk, int i) {
+            if (i < LX) load_to_lds(xr, to + (i * W + wave) * 1024, x_off[i], xk);
+            else load_to_lds(wr, to + BM * kStage + ((i - LX) * W + wave) * 1024, w_off[i - LX], wk);
+        };
+        // the stage after the next `flying` ones has come, for all waves, and all have what they read before
+        const auto arrive = [&](auto flying) {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(flying)::value * (LX + LW)) : "memory");
+        };
+        // Each die starts at a place of its own in the inner dimension: all at once at the same columns of power-of-two strides
+        // meet in the same channels of the memory.
+        const int turn = stop > begin ? (int)((int64_t)(stop - begin) * (blockIdx.x & 7) / 8) : 0;
+        const auto turned = [&](int k) { return k + turn < stop ? k + turn : k + turn - (stop - begin); };
+        const auto load = [&](uint8_t* to, int k) {
+            const int kk = turned(k), xk = kk * kStage, wk = w_stage(kk) * kStage;
+#pragma unroll
+            for (int i = 0; i < LX + LW; ++i) load_one(to, xk, wk, i);
+        };
+        v4i f[2][TM + TN];
         if (begin < stop) {
-            stage_direct(first, begin);
-            arrive();
+            load(ring0, begin);
+            if (begin + 1 < stop) load(ring1, begin + 1);
+            if (begin + 2 < stop) load(ring2, begin + 2);
+            if (begin + 3 < stop) load(ring3, begin + 3);
+            if (begin + kRing <= stop) arrive(Int<kRing - 1>());
+            else arrive(Int<0>());
+            read(f[0], ring0);
         }
-        int k = begin;
-        for (; k + 1 < stop; k += 2) {
-            stage_direct(second, k + 1);
-            __builtin_amdgcn_sched_barrier(0);   // (the loads leave before the products, not when they are done)
-            multiply(first);
-            arrive();
-            if (k + 2 < stop) stage_direct(first, k + 2);
+        // Multiplies stage k, which is in f[which & 1]; `steady`: at least kRing stages follow.  There the next stage's reads and
+        // the loads stand between the products: a wave issues in order, and products behind a queue of loads would wait for it.
+        constexpr int kReads = TM + TN, kLoads = LX + LW, kProducts = TM * TN, kPer = kProducts / (kReads + kLoads);
+        const auto stage = [&](auto which, int k, auto steady) {
+            constexpr int r = decltype(which)::value;
+            constexpr bool kSteady = decltype(steady)::value;
+            if (kSteady || k + kRing <= stop) arrive(Int<kRing - 2>());
+            else if (k + kRing - 1 <= stop) arrive(Int<kRing - 3>());
+            else arrive(Int<0>());
+            const int kk = turned(k + kRing), xk = kk * kStage, wk = w_stage(kk) * kStage;
+            if (!kSteady && k + kRing < stop) load(place(which), k + kRing);
+#pragma unroll
+            for (int t = 0; t < kReads + kLoads; ++t) {
+                // (behind the last stage the reads bring what nobody uses)
+                if (t < kReads) read_one(f[(r + 1) & 1], place(Int<r + 1>()), t);
+                else if constexpr (kSteady) load_one(place(which), xk, wk, t - kReads);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < kPer; ++u) multiply_one(f[r & 1], t * kPer + u);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int t = (kReads + kLoads) * kPer; t < kProducts; ++t) multiply_one(f[r & 1], t);
             __builtin_amdgcn_sched_barrier(0);
-            multiply(second);
-            arrive();
+        };
+        int k = begin;
+        for (; k + 2 * kRing <= stop; k += kRing) {
+            stage(Int<0>(), k, std::true_type());
+            stage(Int<1>(), k + 1, std::true_type());
+            stage(Int<2>(), k + 2, std::true_type());
+            stage(Int<3>(), k + 3, std::true_type());
         }
-        if (k < stop) multiply(first);
+        for (; k < stop; k += kRing) {
+            stage(Int<0>(), k, std::false_type());
+            if (k + 1 < stop) stage(Int<1>(), k + 1, std::false_type());
+            if (k + 2 < stop) stage(Int<2>(), k + 2, std::false_type());
+            if (k + 3 < stop) stage(Int<3>(), k + 3, std::false_type());
+        }
         if (stop < end) {
             v4i v[LX + LW];
             fetch(v, stop);
-            put(second, v);   // (its last readers have passed a barrier since)
             __syncthreads();
-            multiply(second);
+            put(ring0, v);
+            __syncthreads();
+            read(f[0], ring0);
+            multiply(f[0]);
         }
     } else {
-        v4i v[LX + LW];
+        v4i v[LX + LW], f[TM + TN];
         fetch(v, begin);
-        put(first, v);
+        put(ring0, v);
         __syncthreads();
-        uint8_t *now = first, *next = second;
+        uint8_t *now = ring0, *next = ring1;
         for (int k = begin; k < stop; ++k) {
             if (k + 1 < stop) fetch(v, k + 1);
-            multiply(now);
+            read(f, now);
+            multiply(f);
             if (k + 1 < stop) put(next, v);
             __syncthreads();
             uint8_t* t = now;
@@ -269,24 +328,90 @@ __global__ __launch_bounds__(WM* WN * 64) void k_tiles(TileArgs a)
         }
     }
 
+    // Out through LDS, 64 rows of a wave at a time, each wave in a place of the ring: a lane holds four columns of one row, the
+    // lanes that share a row store 16 bytes each and fill its lines.  Positions of the 16-byte pieces ^ row: no two lanes
+    // of a quarter wave meet in a bank.
+    constexpr int kBatch = 4;
+    static_assert(kBytes >= 16 * kBatch * TN * 64 && W == kRing && TM % kBatch == 0, "a stage holds a wave's rows");
+    float ws[TN][4], xs[TM];   // (all asked for at once: each row's by itself would be waited for by itself)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-        const int64_t n = n0 + (wn * TN + j) * 16 + (lane >> 4) * 4;
-        float ws[4];
+    for (int j = 0; j < TN; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) ws[r] = scale_at(a.w_scale, n + r, a.cols);
+        for (int r = 0; r < 4; ++r) ws[j][r] = 1.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xs[i] = 1.f;
+    if (a.w_scale)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t n = n0 + (wn * TN + j) * 16 + (lane >> 4) * 4 + r;
+                ws[j][r] = a.w_scale[n < a.cols ? n : a.cols - 1];
+            }
+    if (a.x_scale)
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const int64_t m = m0 + (wm * TM + i) * 16 + (lane & 15);
-            finish_four(a, blockIdx.y, m, n, sum[j][i], scale_at(a.x_scale, m, a.rows), ws);
+            xs[i] = a.x_scale[m < a.rows ? m : a.rows - 1];
         }
-    }
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");   // the last products' sums are in their registers
+    __syncthreads();
+    uint8_t* area = wave == 0 ? ring0 : wave == 1 ? ring1 : wave == 2 ? ring2 : ring3;
+    const bool fits = m0 + BM <= a.rows && n0 + BN <= a.cols;
+    const auto finish = [&](auto* y, auto value) {
+        using T = std::remove_pointer_t<decltype(y)>;
+        constexpr int kEach = 16 / (int)sizeof(T), kPieces = TN * 16 / kEach, kAtOnce = 64 / kPieces;   // elements, pieces of a row, rows of a store
+        constexpr int kMix = (kPieces < 16 ? kPieces : 16) - 1;
+        const int row = lane & 15, column = (lane >> 4) * 4;
+#pragma unroll
+        for (int half = 0; half < TM / kBatch; ++half) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) {
+                    Sum s = sum[j][half * kBatch + i];
+                    asm volatile("" : "+v"(s));   // (here, and not for all types at once before the choice of one)
+                    T four[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) four[r] = value(s[r], half * kBatch + i, j, r);
+                    const int at = j * 16 + column, where = (i * 16 + row) * kPieces + ((at / kEach) ^ (row & kMix));
+                    __builtin_memcpy(area + where * 16 + at % kEach * sizeof(T), four, sizeof four);
+                }
+            __builtin_amdgcn_wave_barrier();
+            const int64_t m1 = m0 + (wm * TM + half * kBatch) * 16, n = n0 + wn * TN * 16 + lane % kPieces * kEach;
+#pragma unroll 4
+            for (int h = 0; h < 16 * kBatch; h += kAtOnce) {
+                const int r = h + lane / kPieces;
+                const v4i u = *(const v4i*)(area + (r * kPieces + (lane % kPieces ^ (r & kMix))) * 16);
+                T* to = y + (m1 + r) * a.cols + n;
+                if (fits) {
+                    __builtin_memcpy(to, &u, 16);
+                } else if (m1 + r < a.rows && n < a.cols) {
+                    if (n + kEach <= a.cols) {
+                        __builtin_memcpy(to, &u, 16);
+                    } else {
+                        T raw[kEach];
+                        __builtin_memcpy(raw, &u, 16);
+#pragma unroll
+                        for (int t = 0; t < kEach; ++t)
+                            if (n + t < a.cols) to[t] = raw[t];
+                    }
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    };
+    const auto scaled = [&](auto one, int i, int j, int r) { return (float)one * xs[i] * ws[j][r]; };
+    if (a.partial) finish(a.partial + (int64_t)blockIdx.y * a.rows * a.cols, [&](auto one, int, int, int) { return __builtin_bit_cast(uint32_t, one); });
+    else if (a.dtype == GEO_SC_F32) finish((f32*)a.y, scaled);
+    else if (a.dtype == GEO_SC_BF16) finish((bf16*)a.y, [&](auto one, int i, int j, int r) { return (bf16)scaled(one, i, j, r); });
+    else finish((f16*)a.y, [&](auto one, int i, int j, int r) { return (f16)scaled(one, i, j, r); });
 }
 
 // Few rows of x (at most 16 MT): y is bound by the one read of w.  A wave reads 128 bytes of 16 NT rows of w per step, 32 per lane,
 // straight into the registers that the matrix instruction takes, and the same bytes of x; a workgroup's waves, and the
 // grid's second dimension, cut the inner dimension, and the sums meet in LDS.
-constexpr int kFewWaves = 8;
+constexpr int kFewWaves = 8, kStep = 2 * kStage;
 template <int MT, int NT>
 __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
 {
@@ -310,9 +435,9 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) sum[j][i] = v4i{0, 0, 0, 0};
-    const int steps = (int)((a.inner + kTile - 1) / kTile), whole = (int)(a.inner / kTile);
-    const int begin = blockIdx.y * a.steps_per_split;
-    const int end = begin + a.steps_per_split < steps ? begin + a.steps_per_split : steps;
+    const int steps = (int)((a.inner + kStep - 1) / kStep), whole = (int)(a.inner / kStep);
+    const int begin = blockIdx.y * (a.stages_per_split / 2);
+    const int end = begin + a.stages_per_split / 2 < steps ? begin + a.stages_per_split / 2 : steps;
     const int end_whole = end < whole ? end : whole;
     const auto step = [&](const v4i (&w)[NT][2], const v4i (&x)[MT][2]) {
 #pragma unroll
@@ -325,7 +450,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
 #pragma unroll 4
     for (int k = begin + wave; k < end_whole; k += kFewWaves) {
         v4i w[NT][2], x[MT][2];
-        const int64_t o = (int64_t)k * kTile;
+        const int64_t o = (int64_t)k * kStep;
 #pragma unroll
         for (int j = 0; j < NT; ++j) __builtin_memcpy(w[j], wp[j] + o, 32);
 #pragma unroll
@@ -334,7 +459,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
     }
     if (end > end_whole && (end_whole - begin) % kFewWaves == wave) {   // the last step, where it is not whole
         v4i w[NT][2], x[MT][2];
-        const int64_t o = (int64_t)end_whole * kTile;
+        const int64_t o = (int64_t)end_whole * kStep;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -394,13 +519,13 @@ __global__ __launch_bounds__(256) void k_join_splits(TileArgs a, int splits)
 struct Plan {
     int few;       // squares of 16 rows of k_few_rows; 0: k_tiles
     int tile;      // rows and columns of k_tiles' tile
-    int splits, steps_per_split;
+    int splits, stages_per_split;
 };
 
 Plan plan_of(int64_t rows, int64_t cols, int64_t inner_bytes, bool int8)
 {
     Plan p = {};
-    const int64_t steps = (inner_bytes + kTile - 1) / kTile;
+    const int64_t steps = (inner_bytes + 2 * kStage - 1) / (2 * kStage);   // a split has whole steps of two stages
     int64_t groups;
     int64_t least;   // steps that a split has at least
     if (int8 && rows <= 64) {
@@ -420,8 +545,9 @@ Plan plan_of(int64_t rows, int64_t cols, int64_t inner_bytes, bool int8)
         if (splits < 1) splits = 1;
         if (splits > 64) splits = 64;
     }
-    p.steps_per_split = (int)((steps + splits - 1) / splits);
-    p.splits = (int)((steps + p.steps_per_split - 1) / p.steps_per_split);
+    const int64_t per_split = (steps + splits - 1) / splits;
+    p.stages_per_split = (int)(2 * per_split);
+    p.splits = (int)((steps + per_split - 1) / per_split);
     return p;
 }
 
@@ -445,7 +571,7 @@ template <bool INT8>
 int run_product(TileArgs a, void* workspace, hipStream_t s)
 {
     const Plan p = plan_of(a.rows, a.cols, a.inner, INT8);
-    a.steps_per_split = p.steps_per_split;
+    a.stages_per_split = p.stages_per_split;
     a.partial = p.splits > 1 ? (uint32_t*)workspace : nullptr;
     if (p.few) {
         if (p.few == 1) run_few<1>(a, p, s);
@@ -460,7 +586,7 @@ int run_product(TileArgs a, void* workspace, hipStream_t s)
             return (uintptr_t)q % 16 == 0 && stride % 16 == 0 && stride * p.tile + a.inner < 0x7fffffff;
         };
         const bool direct = fits(a.x, a.x_stride) && fits(a.w, a.w_stride);
-        if (p.tile == 256) run_tiles<256, 2, 4, INT8>(a, p, direct, s);
+        if (p.tile == 256) run_tiles<256, 2, 2, INT8>(a, p, direct, s);
         else run_tiles<128, 2, 2, INT8>(a, p, direct, s);
     }
     if (a.partial) {
@@ -571,7 +697,7 @@ __global__ __launch_bounds__(256) void k_widen_t(const int8_t* q, int64_t q_stri
 }
 
 int terms_of(int grad_dtype) { return grad_dtype == GEO_SC_BF16 ? 1 : grad_dtype == GEO_SC_F16 ? 2 : 3; }
-int64_t padded_to_side(int64_t n) { return (n + kSide - 1) / kSide * kSide; }   // whole steps of 64 bf16 elements
+int64_t padded_to_side(int64_t n) { return (n + kSide - 1) / kSide * kSide; }   // whole stages of bf16 elements
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 // what one gradient needs: its two operands and the splits' sums.  `depth` is the dimension summed over.
@@ -624,7 +750,7 @@ int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, co
     a.rows = rows;
     a.cols = cols;
     a.inner = inner;
-    a.w_steps = 0x7fffffff;
+    a.w_stages = 0x7fffffff;
     a.x_scale = x_scale;
     a.w_scale = w_scale;
     a.y = y;
@@ -669,7 +795,7 @@ int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64_t grad_str
         a.rows = m;
         a.cols = n;
         a.inner = terms * p * 2;
-        a.w_steps = (int)(p * 2 / kTile);
+        a.w_stages = (int)(p * 2 / kStage);
         a.y = y;
         a.dtype = dtype;
         return run_product<false>(a, at + l.left + l.right, s);
