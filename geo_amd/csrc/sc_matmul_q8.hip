@@ -37,8 +37,14 @@ struct TileArgs {
     void* y;
     int dtype;
     int stages_per_split;
+    int splits;
     uint32_t* partial;                 // [splits][rows][cols] 32-bit sums, or NULL: one split that writes y
     int tiles_m, tiles_n;
+};
+// One launch computes up to two products: workgroups from second_at on the second.
+struct TwoProducts {
+    TileArgs first, second;
+    uint32_t second_at;
 };
 
 // One load of 16 bytes per lane straight into LDS, lane after lane from `to` on.  (The host's pass over this file knows no
@@ -146,8 +152,11 @@ __device__ __forceinline__ float scale_at(const float* scale, int64_t i, int64_t
 constexpr int kRing = 4;
 
 template <int BM, int BN, int WM, int WN, bool INT8, bool DIRECT>
-__global__ __launch_bounds__(WM* WN * 64) void k_tiles(TileArgs a)
+__global__ __launch_bounds__(WM* WN * 64) void k_tiles(TwoProducts both)
 {
+    const bool is_second = blockIdx.x >= both.second_at;
+    const TileArgs a = is_second ? both.second : both.first;
+    const uint32_t group = blockIdx.x - (is_second ? both.second_at : 0);
     constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, LX = BM / 16 / W, LW = BN / 16 / W;
     static_assert(LX * W * 16 == BM && LW * W * 16 == BN, "every wave stages as many rows");
     typedef typename Matrix<INT8>::Sum Sum;
@@ -165,19 +174,16 @@ __global__ __launch_bounds__(WM* WN * 64) void k_tiles(TileArgs a)
 
     // Workgroups go to the eight dies in turn: each die takes a contiguous share of the tiles, so that neighbours share its L2,
     // in strips of eight tiles of rows.
-    int64_t tile;
-    {
-        const int64_t all = (int64_t)a.tiles_m * a.tiles_n, die = blockIdx.x & 7, at = blockIdx.x >> 3;
-        tile = die * (all / 8) + (die < all % 8 ? die : all % 8) + at;
-    }
-    constexpr int kStrip = 8;
-    const int64_t strip = tile / ((int64_t)kStrip * a.tiles_n), inside = tile - strip * kStrip * a.tiles_n;
-    const int64_t height = a.tiles_m - strip * kStrip < kStrip ? a.tiles_m - strip * kStrip : kStrip;
-    const int64_t m0 = (strip * kStrip + inside % height) * BM, n0 = inside / height * BN;
+    const uint32_t all = (uint32_t)a.tiles_m * a.tiles_n, split = group / all, die = group % all & 7;
+    const uint32_t tile = die * (all / 8) + (die < all % 8 ? die : all % 8) + (group % all >> 3);
+    constexpr uint32_t kStrip = 8;
+    const uint32_t strip = tile / (kStrip * a.tiles_n), inside = tile - strip * kStrip * a.tiles_n;
+    const uint32_t height = a.tiles_m - strip * kStrip < kStrip ? a.tiles_m - strip * kStrip : kStrip;
+    const int64_t m0 = (int64_t)(strip * kStrip + inside % height) * BM, n0 = (int64_t)(inside / height) * BN;
     const int wm = wave % WM, wn = wave / WM;
 
     const int stages = (int)((a.inner + kStage - 1) / kStage);
-    const int begin = blockIdx.y * a.stages_per_split;
+    const int begin = split * a.stages_per_split;
     const int end = begin + a.stages_per_split < stages ? begin + a.stages_per_split : stages;
     const int whole = (int)(a.inner / kStage);
 
@@ -246,7 +252,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_tiles(TileArgs a)
         };
         // Each die starts at a place of its own in the inner dimension: all at once at the same columns of power-of-two strides
         // meet in the same channels of the memory.
-        const int turn = stop > begin ? (int)((int64_t)(stop - begin) * (blockIdx.x & 7) / 8) : 0;
+        const int turn = stop > begin ? (int)((int64_t)(stop - begin) * die / 8) : 0;
         const auto turned = [&](int k) { return k + turn < stop ? k + turn : k + turn - (stop - begin); };
         const auto load = [&](uint8_t* to, int k) {
             const int kk = turned(k), xk = kk * kStage, wk = w_stage(kk) * kStage;
@@ -331,7 +337,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_tiles(TileArgs a)
     // Out through LDS, 64 rows of a wave at a time, each wave in a place of the ring: a lane holds four columns of one row, the
     // lanes that share a row store 16 bytes each and fill its lines.  Positions of the 16-byte pieces ^ row: no two lanes
     // of a quarter wave meet in a bank.
-    constexpr int kBatch = 4;
+    constexpr int kBatch = TM < 4 ? TM : 4;
     static_assert(kBytes >= 16 * kBatch * TN * 64 && W == kRing && TM % kBatch == 0, "a stage holds a wave's rows");
     float ws[TN][4], xs[TM];   // (all asked for at once: each row's by itself would be waited for by itself)
 #pragma unroll
@@ -402,7 +408,7 @@ __global__ __launch_bounds__(WM* WN * 64) void k_tiles(TileArgs a)
         }
     };
     const auto scaled = [&](auto one, int i, int j, int r) { return (float)one * xs[i] * ws[j][r]; };
-    if (a.partial) finish(a.partial + (int64_t)blockIdx.y * a.rows * a.cols, [&](auto one, int, int, int) { return __builtin_bit_cast(uint32_t, one); });
+    if (a.partial) finish(a.partial + (int64_t)split * a.rows * a.cols, [&](auto one, int, int, int) { return __builtin_bit_cast(uint32_t, one); });
     else if (a.dtype == GEO_SC_F32) finish((f32*)a.y, scaled);
     else if (a.dtype == GEO_SC_BF16) finish((bf16*)a.y, [&](auto one, int i, int j, int r) { return (bf16)scaled(one, i, j, r); });
     else finish((f16*)a.y, [&](auto one, int i, int j, int r) { return (f16)scaled(one, i, j, r); });
@@ -486,26 +492,28 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
     }
 }
 
-// y from the sums of the splits
+// y from the sums of the splits, of both products of a launch
 template <bool INT8>
-__global__ __launch_bounds__(256) void k_join_splits(TileArgs a, int splits)
+__global__ __launch_bounds__(256) void k_join_splits(TwoProducts both)
 {
-    const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    const int64_t m = blockIdx.y + (int64_t)blockIdx.z * 65535;
-    const int64_t left = a.cols - n;
-    if (left <= 0 || m >= a.rows) return;
+    const bool is_second = blockIdx.x >= both.second_at;
+    const TileArgs a = is_second ? both.second : both.first;
+    // (products that are cut have fewer than 2^32 outputs: less than a tile for each compute unit)
+    const uint32_t at = (blockIdx.x - (is_second ? both.second_at : 0)) * 256 + threadIdx.x, fours = (uint32_t)((a.cols + 3) / 4);
+    const int64_t m = at / fours, n = (int64_t)(at % fours) * 4, left = a.cols - n;
+    if (m >= a.rows) return;
     typename Matrix<INT8>::Sum s = {0, 0, 0, 0};
-    for (int k = 0; k < splits; ++k) {
+    for (int k = 0; k < a.splits; ++k) {
         const uint32_t* p = a.partial + ((int64_t)k * a.rows + m) * a.cols + n;
-        typename Matrix<INT8>::Sum one = {0, 0, 0, 0};
+        uint32_t one[4] = {0, 0, 0, 0};
         if (left >= 4) {
-            __builtin_memcpy(&one, p, 16);
+            __builtin_memcpy(one, p, 16);
         } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (r < left) one[r] = __builtin_bit_cast(std::remove_reference_t<decltype(one[0] + one[0])>, p[r]);
+                if (r < left) one[r] = p[r];
         }
-        s += one;
+        s += __builtin_bit_cast(typename Matrix<INT8>::Sum, one);
     }
     const float xs = scale_at(a.x_scale, m, a.rows);
     float v[4];
@@ -516,83 +524,95 @@ __global__ __launch_bounds__(256) void k_join_splits(TileArgs a, int splits)
 
 // ---------------------------------------------------------------- which kernel, and how the inner dimension is cut
 
+struct Shape {
+    int64_t rows, cols, inner;   // bytes of the inner dimension; rows 0: no such product
+    int64_t tiles(int64_t t) const { return ((rows + t - 1) / t) * ((cols + t - 1) / t); }
+    int64_t steps() const { return (inner + 2 * kStage - 1) / (2 * kStage); }   // a split has whole steps of two stages
+};
 struct Plan {
-    int few;       // squares of 16 rows of k_few_rows; 0: k_tiles
-    int tile;      // rows and columns of k_tiles' tile
-    int splits, stages_per_split;
+    int few;        // squares of 16 rows of k_few_rows; 0: k_tiles
+    int tile;       // rows and columns of k_tiles' tile
+    int splits[2], stages_per_split[2];
 };
 
-Plan plan_of(int64_t rows, int64_t cols, int64_t inner_bytes, bool int8)
+void cut(Plan* p, int which, const Shape& s, int64_t groups, int64_t least)
+{
+    const int64_t steps = s.steps();
+    int64_t splits = groups < kUnits ? kUnits / groups : 1;
+    if (splits > steps / least) splits = steps / least;
+    if (splits > 64) splits = 64;
+    if (splits < 1) splits = 1;
+    const int64_t per_split = (steps + splits - 1) / splits;
+    p->stages_per_split[which] = (int)(2 * per_split);
+    p->splits[which] = (int)((steps + per_split - 1) / per_split);
+}
+
+Plan plan_of(const Shape& s, const Shape& t, bool int8)
 {
     Plan p = {};
-    const int64_t steps = (inner_bytes + 2 * kStage - 1) / (2 * kStage);   // a split has whole steps of two stages
-    int64_t groups;
-    int64_t least;   // steps that a split has at least
-    if (int8 && rows <= 64) {
-        p.few = (int)((rows + 15) / 16);
-        groups = (cols + 15) / 16;
-        least = kFewWaves;
-    } else {
-        const auto tiles = [&](int64_t t) { return ((rows + t - 1) / t) * ((cols + t - 1) / t); };
-        p.tile = tiles(256) >= kUnits * 3 / 4 ? 256 : 128;
-        groups = tiles(p.tile);
-        least = 8;
+    if (int8 && s.rows <= 64) {
+        p.few = (int)((s.rows + 15) / 16);
+        cut(&p, 0, s, (s.cols + 15) / 16, kFewWaves);
+        return p;
     }
-    int64_t splits = 1;
-    if (groups < kUnits) {
-        splits = kUnits / groups;
-        if (splits > steps / least) splits = steps / least;
-        if (splits < 1) splits = 1;
-        if (splits > 64) splits = 64;
-    }
-    const int64_t per_split = (steps + splits - 1) / splits;
-    p.stages_per_split = (int)(2 * per_split);
-    p.splits = (int)((steps + per_split - 1) / per_split);
+    const auto tiles = [&](int64_t b) { return s.tiles(b) + (t.rows ? t.tiles(b) : 0); };
+    p.tile = tiles(256) >= kUnits * 3 / 4 ? 256 : tiles(128) >= kUnits ? 128 : 64;
+    cut(&p, 0, s, tiles(p.tile), 8);
+    if (t.rows) cut(&p, 1, t, tiles(p.tile), 8);
     return p;
 }
 
-size_t partial_bytes(const Plan& p, int64_t rows, int64_t cols) { return p.splits > 1 ? (size_t)p.splits * rows * cols * 4 : 0; }
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+size_t partial_bytes(const Plan& p, int which, const Shape& s) { return p.splits[which] > 1 ? align256((size_t)p.splits[which] * s.rows * s.cols * 4) : 0; }
 
 template <int MT>
-void run_few(const TileArgs& a, const Plan& p, hipStream_t s)
+void run_few(const TileArgs& a, hipStream_t s)
 {
-    k_few_rows<MT, 1><<<dim3((uint32_t)((a.cols + 15) / 16), (uint32_t)p.splits), dim3(kFewWaves * 64), 0, s>>>(a);
+    k_few_rows<MT, 1><<<dim3((uint32_t)((a.cols + 15) / 16), (uint32_t)a.splits), dim3(kFewWaves * 64), 0, s>>>(a);
 }
 
-template <int B, int WM, int WN, bool INT8>
-void run_tiles(const TileArgs& a, const Plan& p, bool direct, hipStream_t s)
+template <int B, bool INT8>
+void run_tiles(TwoProducts both, bool direct, hipStream_t s)
 {
-    const dim3 grid((uint32_t)((int64_t)a.tiles_m * a.tiles_n), (uint32_t)p.splits);
-    if (direct) k_tiles<B, B, WM, WN, INT8, true><<<grid, dim3(WM * WN * 64), 0, s>>>(a);
-    else k_tiles<B, B, WM, WN, INT8, false><<<grid, dim3(WM * WN * 64), 0, s>>>(a);
+    const auto groups = [](TileArgs& a) {
+        a.tiles_m = (int)((a.rows + B - 1) / B);
+        a.tiles_n = (int)((a.cols + B - 1) / B);
+        return (uint32_t)a.tiles_m * a.tiles_n * a.splits;
+    };
+    both.second_at = groups(both.first);
+    const dim3 grid(both.second_at + (both.second.rows ? groups(both.second) : 0));
+    if (direct) k_tiles<B, B, 2, 2, INT8, true><<<grid, dim3(256), 0, s>>>(both);
+    else k_tiles<B, B, 2, 2, INT8, false><<<grid, dim3(256), 0, s>>>(both);
 }
 
+// Runs one product, or two in one launch (second.rows 0: one).  The caller has made the plan and the partial sums' memory.
 template <bool INT8>
-int run_product(TileArgs a, void* workspace, hipStream_t s)
+int run_products(TwoProducts both, const Plan& p, hipStream_t s)
 {
-    const Plan p = plan_of(a.rows, a.cols, a.inner, INT8);
-    a.stages_per_split = p.stages_per_split;
-    a.partial = p.splits > 1 ? (uint32_t*)workspace : nullptr;
+    both.first.splits = p.splits[0];
+    both.first.stages_per_split = p.stages_per_split[0];
+    both.second.splits = p.splits[1];
+    both.second.stages_per_split = p.stages_per_split[1];
     if (p.few) {
-        if (p.few == 1) run_few<1>(a, p, s);
-        else if (p.few == 2) run_few<2>(a, p, s);
-        else if (p.few == 3) run_few<3>(a, p, s);
-        else run_few<4>(a, p, s);
+        if (p.few == 1) run_few<1>(both.first, s);
+        else if (p.few == 2) run_few<2>(both.first, s);
+        else if (p.few == 3) run_few<3>(both.first, s);
+        else run_few<4>(both.first, s);
     } else {
-        a.tiles_m = (int)((a.rows + p.tile - 1) / p.tile);
-        a.tiles_n = (int)((a.cols + p.tile - 1) / p.tile);
         // loads that write LDS take 16-byte addresses, and offsets of 31 bits from the tile's first row
-        const auto fits = [&](const uint8_t* q, int64_t stride) {
-            return (uintptr_t)q % 16 == 0 && stride % 16 == 0 && stride * p.tile + a.inner < 0x7fffffff;
+        const auto one_fits = [&](const uint8_t* q, int64_t stride, int64_t inner) {
+            return (uintptr_t)q % 16 == 0 && stride % 16 == 0 && stride * p.tile + inner < 0x7fffffff;
         };
-        const bool direct = fits(a.x, a.x_stride) && fits(a.w, a.w_stride);
-        if (p.tile == 256) run_tiles<256, 2, 2, INT8>(a, p, direct, s);
-        else run_tiles<128, 2, 2, INT8>(a, p, direct, s);
+        const auto fits = [&](const TileArgs& a) { return one_fits(a.x, a.x_stride, a.inner) && one_fits(a.w, a.w_stride, a.inner); };
+        const bool direct = fits(both.first) && (!both.second.rows || fits(both.second));
+        if (p.tile == 256) run_tiles<256, INT8>(both, direct, s);
+        else if (p.tile == 128) run_tiles<128, INT8>(both, direct, s);
+        else run_tiles<64, INT8>(both, direct, s);
     }
-    if (a.partial) {
-        const uint32_t y = (uint32_t)(a.rows < 65535 ? a.rows : 65535), z = (uint32_t)((a.rows + 65534) / 65535);
-        k_join_splits<INT8><<<dim3((uint32_t)((a.cols + 1023) / 1024), y, z), dim3(256), 0, s>>>(a, p.splits);
-    }
+    const auto joins = [](const TileArgs& a) { return a.partial ? (uint32_t)((a.rows * ((a.cols + 3) / 4) + 255) / 256) : 0u; };
+    both.second_at = joins(both.first);
+    const uint32_t all = both.second_at + joins(both.second);
+    if (all) k_join_splits<INT8><<<dim3(all), dim3(256), 0, s>>>(both);
     return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
 }
 
@@ -610,107 +630,147 @@ __device__ __forceinline__ void split_terms(float v, bf16 (&t)[TERMS])
     }
 }
 
-// out[m][term][n] = terms of g[m][n] scale[n]; `padded` columns per term, zeros behind the last
+// The operands of both gradients in one launch, its workgroups in three ranges:
+//   g in tiles of 64 x 64:  dx_left[m][term][n] = terms of g[m][n] w_scale[n],  dw_left[n][term][m] = terms of g[m][n] x_scale[m]
+//   w in tiles of 64 x 128: dx_right[k][n] = w[n][k] in bf16
+//   x in tiles of 64 x 128: dw_right[k][m] = x[m][k] in bf16
+// Rows of an output are padded to whole stages of 64 elements per term, with zeros.
+constexpr int kSide = 64, kWide = 128;
+
+struct OperandArgs {
+    const void* g;
+    int dtype;
+    int64_t g_stride, x_stride, w_stride, rows, cols, inner;
+    const int8_t *x, *w;
+    const float *x_scale, *w_scale;
+    int64_t rows_padded, cols_padded;
+    bf16 *dx_left, *dx_right, *dw_left, *dw_right;   // NULL: that gradient is not wanted
+    uint32_t g_tiles, w_tiles;                       // workgroups of the first two ranges
+};
+
 template <int TERMS>
-__global__ __launch_bounds__(256) void k_scaled_grad(const void* g, int dtype, int64_t g_stride, const float* scale, int64_t rows,
-                                                     int64_t cols, int64_t padded, bf16* out)
+__device__ __forceinline__ void store_terms(const float (&v)[kChunk], bf16* out, int64_t padded)
 {
-    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * kChunk;
-    if (c >= padded) return;
-    float k[kChunk];
-    load_chunk(scale, c, cols, 0.f, k);
-    for (int64_t m = blockIdx.y; m < rows; m += gridDim.y) {
-        float v[kChunk];
-        load_chunk(g, dtype, m * g_stride, c, cols, 0.f, v);
-        bf16 t[TERMS][kChunk];
+    bf16 t[TERMS][kChunk];
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-            bf16 one[TERMS];
-            split_terms<TERMS>(v[j] * k[j], one);
+    for (int j = 0; j < kChunk; ++j) {
+        bf16 one[TERMS];
+        split_terms<TERMS>(v[j], one);
 #pragma unroll
-            for (int i = 0; i < TERMS; ++i) t[i][j] = one[i];
-        }
+        for (int i = 0; i < TERMS; ++i) t[i][j] = one[i];
+    }
 #pragma unroll
-        for (int i = 0; i < TERMS; ++i) __builtin_memcpy(out + (m * TERMS + i) * padded + c, t[i], sizeof t[i]);
+    for (int i = 0; i < TERMS; ++i) __builtin_memcpy(out + i * padded, t[i], sizeof t[i]);
+}
+
+// out[c][r] = q[r][c] in bf16 for a tile of 64 rows and 128 columns.  A thread turns four columns of eight rows: it reads a
+// word of each row (a row of 33 words: no two lanes meet in a bank) and writes eight rows' values of each column.
+__device__ __forceinline__ void widen_tile(const int8_t* q, int64_t stride, int64_t rows, int64_t cols, int64_t padded, uint32_t tile, bf16* out,
+                                           uint32_t* lds)
+{
+    constexpr int kWords = kWide / 4 + 1;
+    const uint32_t across = (uint32_t)((cols + kWide - 1) / kWide);
+    const int64_t r0 = (int64_t)(tile / across) * kSide, c0 = (int64_t)(tile % across) * kWide;
+#pragma unroll
+    for (int i = 0; i < kSide * kWide / 16 / 256; ++i) {
+        const int piece = i * 256 + threadIdx.x, r = piece / (kWide / 16), c = piece % (kWide / 16) * 16;
+        v4i v = {0, 0, 0, 0};
+        if (r0 + r < rows && c0 + c < cols) v = load_piece((const uint8_t*)(q + (r0 + r) * stride), c0 + c, cols);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lds[r * kWords + c / 4 + j] = v[j];
+    }
+    __syncthreads();
+    const int r = threadIdx.x % 8 * 8, c = threadIdx.x / 8 * 4;
+    uint32_t words[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) words[j] = lds[(r + j) * kWords + c / 4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (c0 + c + j >= cols) break;
+        bf16 t[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t[k] = (bf16)(float)(int8_t)(words[k] >> (8 * j));
+        __builtin_memcpy(out + (c0 + c + j) * padded + r0 + r, t, sizeof t);
     }
 }
 
-constexpr int kSide = 64;   // a workgroup transposes 64 x 64 elements through LDS
-
-// out[c][term][r] = terms of g[r][c] scale[r]; `padded` rows per term
 template <int TERMS>
-__global__ __launch_bounds__(256) void k_scaled_grad_t(const void* g, int dtype, int64_t g_stride, const float* scale, int64_t rows,
-                                                       int64_t cols, int64_t padded, bf16* out)
+__global__ __launch_bounds__(256) void k_grad_operands(OperandArgs a)
 {
     __shared__ float tile[kSide][kSide + 1];
-    const int64_t r0 = (int64_t)blockIdx.x * kSide, c0 = (int64_t)blockIdx.y * kSide;
-    for (int i = threadIdx.x; i < kSide * kSide / kChunk; i += 256) {
-        const int r = i / (kSide / kChunk), c = i % (kSide / kChunk) * kChunk;
-        float v[kChunk] = {};
-        if (r0 + r < rows && c0 + c < cols) {
-            load_chunk(g, dtype, (r0 + r) * g_stride, c0 + c, cols, 0.f, v);
-            const float k = scale[r0 + r];
+    static_assert(sizeof tile >= kSide * (kWide + 4), "a tile of 8-bit numbers fits");
+    if (blockIdx.x >= a.g_tiles) {
+        const uint32_t at = blockIdx.x - a.g_tiles;
+        if (at < a.w_tiles) widen_tile(a.w, a.w_stride, a.cols, a.inner, a.cols_padded, at, a.dx_right, (uint32_t*)tile);
+        else widen_tile(a.x, a.x_stride, a.rows, a.inner, a.rows_padded, at - a.w_tiles, a.dw_right, (uint32_t*)tile);
+        return;
+    }
+    const uint32_t across = (uint32_t)(a.cols_padded / kSide);
+    const int64_t r0 = (int64_t)(blockIdx.x / across) * kSide, c0 = (int64_t)(blockIdx.x % across) * kSide;
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) v[j] *= k;
-        }
+    for (int i = 0; i < kSide * kSide / kChunk / 256; ++i) {
+        const int at = i * 256 + threadIdx.x, r = at / (kSide / kChunk), c = at % (kSide / kChunk) * kChunk;
+        float v[kChunk] = {};
+        if (r0 + r < a.rows && c0 + c < a.cols) load_chunk(a.g, a.dtype, (r0 + r) * a.g_stride, c0 + c, a.cols, 0.f, v);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) tile[r][c + j] = v[j];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < kSide * kSide / kChunk; i += 256) {
-        const int c = i / (kSide / kChunk), r = i % (kSide / kChunk) * kChunk;
-        if (c0 + c >= cols) continue;
-        bf16 t[TERMS][kChunk];
+        if (a.dx_left && r0 + r < a.rows) {
+            float k[kChunk] = {};
+            if (c0 + c < a.cols) load_chunk(a.w_scale, c0 + c, a.cols, 0.f, k);
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-            bf16 one[TERMS];
-            split_terms<TERMS>(tile[r + j][c], one);
-#pragma unroll
-            for (int q = 0; q < TERMS; ++q) t[q][j] = one[q];
+            for (int j = 0; j < kChunk; ++j) v[j] *= k[j];
+            store_terms<TERMS>(v, a.dx_left + (r0 + r) * TERMS * a.cols_padded + c0 + c, a.cols_padded);
         }
-#pragma unroll
-        for (int q = 0; q < TERMS; ++q) __builtin_memcpy(out + ((c0 + c) * TERMS + q) * padded + r0 + r, t[q], sizeof t[q]);
     }
-}
-
-// out[c][r] = q[r][c] in bf16, `padded` rows
-__global__ __launch_bounds__(256) void k_widen_t(const int8_t* q, int64_t q_stride, int64_t rows, int64_t cols, int64_t padded, bf16* out)
-{
-    __shared__ float tile[kSide][kSide + 1];
-    const int64_t r0 = (int64_t)blockIdx.x * kSide, c0 = (int64_t)blockIdx.y * kSide;
-    for (int i = threadIdx.x; i < kSide * kSide / kChunk; i += 256) {
-        const int r = i / (kSide / kChunk), c = i % (kSide / kChunk) * kChunk;
-        float v[kChunk] = {};
-        if (r0 + r < rows && c0 + c < cols) load_chunk(q + (r0 + r) * q_stride, c0 + c, cols, 0.f, v);
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) tile[r][c + j] = v[j];
-    }
+    if (!a.dw_left) return;
     __syncthreads();
-    for (int i = threadIdx.x; i < kSide * kSide / kChunk; i += 256) {
-        const int c = i / (kSide / kChunk), r = i % (kSide / kChunk) * kChunk;
-        if (c0 + c >= cols) continue;
-        bf16 t[kChunk];
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) t[j] = (bf16)tile[r + j][c];
-        __builtin_memcpy(out + (c0 + c) * padded + r0 + r, t, sizeof t);
+    for (int i = 0; i < kSide * kSide / kChunk / 256; ++i) {
+        const int at = i * 256 + threadIdx.x, c = at / (kSide / kChunk), r = at % (kSide / kChunk) * kChunk;
+        if (c0 + c >= a.cols) continue;
+        float k[kChunk] = {}, v[kChunk];
+        if (r0 + r < a.rows) load_chunk(a.x_scale, r0 + r, a.rows, 0.f, k);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) v[j] = tile[r + j][c] * k[j];
+        store_terms<TERMS>(v, a.dw_left + (c0 + c) * TERMS * a.rows_padded + r0 + r, a.rows_padded);
     }
 }
 
 int terms_of(int grad_dtype) { return grad_dtype == GEO_SC_BF16 ? 1 : grad_dtype == GEO_SC_F16 ? 2 : 3; }
 int64_t padded_to_side(int64_t n) { return (n + kSide - 1) / kSide * kSide; }   // whole stages of bf16 elements
-size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// what one gradient needs: its two operands and the splits' sums.  `depth` is the dimension summed over.
+// the workspace of the backward: both gradients' operands, then the splits' sums
 struct GradLayout {
-    size_t left, right, partial;
+    Shape dx, dw;
+    Plan plan;   // the first product is dx, or dw where dx is not wanted
+    size_t dx_left, dx_right, dw_left, dw_right, first_partial, second_partial, bytes;
 };
-GradLayout grad_layout(int64_t rows, int64_t cols, int64_t depth, int terms)
+GradLayout grad_layout(int64_t rows, int64_t cols, int64_t inner, int terms, bool need_dx, bool need_dw)
 {
-    const int64_t p = padded_to_side(depth);
-    GradLayout l;
-    l.left = align256((size_t)rows * terms * p * 2);
-    l.right = align256((size_t)cols * p * 2);
-    l.partial = align256(partial_bytes(plan_of(rows, cols, terms * p * 2, false), rows, cols));
+    GradLayout l = {};
+    size_t at = 0;
+    const auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += align256(bytes);
+        return here;
+    };
+    if (need_dx) {
+        const int64_t p = padded_to_side(cols);
+        l.dx = {rows, inner, terms * p * 2};
+        l.dx_left = take((size_t)rows * terms * p * 2);
+        l.dx_right = take((size_t)inner * p * 2);
+    }
+    if (need_dw) {
+        const int64_t p = padded_to_side(rows);
+        l.dw = {cols, inner, terms * p * 2};
+        l.dw_left = take((size_t)cols * terms * p * 2);
+        l.dw_right = take((size_t)inner * p * 2);
+    }
+    const Shape none = {};
+    l.plan = plan_of(need_dx ? l.dx : l.dw, need_dx && need_dw ? l.dw : none, false);
+    l.first_partial = take(partial_bytes(l.plan, 0, need_dx ? l.dx : l.dw));
+    l.second_partial = take(need_dx && need_dw ? partial_bytes(l.plan, 1, l.dw) : 0);
+    l.bytes = at;
     return l;
 }
 
@@ -729,7 +789,8 @@ extern "C" {
 int geo_sc_matmul_q8_workspace_size(int64_t rows, int64_t cols, int64_t inner, size_t* bytes)
 {
     if (!bytes || !sizes_fit(rows, cols, inner)) return GEO_SC_ERR_INVALID_ARGUMENT;
-    *bytes = partial_bytes(plan_of(rows, cols, inner, true), rows, cols);
+    const Shape shape = {rows, cols, inner};
+    *bytes = partial_bytes(plan_of(shape, Shape{}, true), 0, shape);
     return GEO_SC_OK;
 }
 
@@ -739,10 +800,12 @@ int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, co
 {
     if (!sizes_fit(rows, cols, inner) || !dtype_known(dtype) || x_stride < 0 || w_stride < 0 || !x || !w || !x_scale || !w_scale || !y)
         return GEO_SC_ERR_INVALID_ARGUMENT;
-    size_t need = 0;
-    geo_sc_matmul_q8_workspace_size(rows, cols, inner, &need);
+    const Shape shape = {rows, cols, inner};
+    const Plan plan = plan_of(shape, Shape{}, true);
+    const size_t need = partial_bytes(plan, 0, shape);
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return GEO_SC_ERR_WORKSPACE;
-    TileArgs a = {};
+    TwoProducts both = {};
+    TileArgs& a = both.first;
     a.x = (const uint8_t*)x;
     a.w = (const uint8_t*)w;
     a.x_stride = x_stride;
@@ -755,17 +818,15 @@ int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, co
     a.w_scale = w_scale;
     a.y = y;
     a.dtype = dtype;
-    return run_product<true>(a, workspace, (hipStream_t)stream);
+    a.partial = need ? (uint32_t*)workspace : nullptr;
+    return run_products<true>(both, plan, (hipStream_t)stream);
 }
 
 int geo_sc_matmul_q8_backward_workspace_size(int64_t rows, int64_t cols, int64_t inner, int grad_dtype, int need_dx, int need_dw,
                                              size_t* bytes)
 {
     if (!bytes || !sizes_fit(rows, cols, inner) || cols > 131071 || !dtype_known(grad_dtype)) return GEO_SC_ERR_INVALID_ARGUMENT;
-    const int terms = terms_of(grad_dtype);
-    const GradLayout x = grad_layout(rows, inner, cols, terms), w = grad_layout(cols, inner, rows, terms);
-    const size_t bx = need_dx ? x.left + x.right + x.partial : 0, bw = need_dw ? w.left + w.right + w.partial : 0;
-    *bytes = bx > bw ? bx : bw;   // one after the other in the same memory
+    *bytes = need_dx || need_dw ? grad_layout(rows, cols, inner, terms_of(grad_dtype), need_dx, need_dw).bytes : 0;
     return GEO_SC_OK;
 }
 
@@ -779,53 +840,61 @@ int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64_t grad_str
         (dw && (!x || !x_scale)))
         return GEO_SC_ERR_INVALID_ARGUMENT;
     if (!dx && !dw) return GEO_SC_OK;
-    size_t need = 0;
-    geo_sc_matmul_q8_backward_workspace_size(rows, cols, inner, grad_dtype, dx != nullptr, dw != nullptr, &need);
-    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16) return GEO_SC_ERR_WORKSPACE;
-    hipStream_t s = (hipStream_t)stream;
     const int terms = terms_of(grad_dtype);
-    const auto product = [&](int64_t m, int64_t n, int64_t depth, const GradLayout& l, void* y, int dtype) {
-        const int64_t p = padded_to_side(depth);
-        uint8_t* at = (uint8_t*)workspace;
+    const GradLayout l = grad_layout(rows, cols, inner, terms, dx, dw);
+    if (!workspace || workspace_bytes < l.bytes || (uintptr_t)workspace % 16) return GEO_SC_ERR_WORKSPACE;
+    const auto tiles = [](int64_t r, int64_t rs, int64_t c, int64_t cs) { return ((r + rs - 1) / rs) * ((c + cs - 1) / cs); };
+    const int64_t g_tiles = tiles(rows, kSide, cols, kSide), w_tiles = dx ? tiles(cols, kSide, inner, kWide) : 0,
+                  x_tiles = dw ? tiles(rows, kSide, inner, kWide) : 0;
+    if (g_tiles + w_tiles + x_tiles > 0x7fffffff) return GEO_SC_ERR_UNSUPPORTED;
+    hipStream_t s = (hipStream_t)stream;
+    uint8_t* base = (uint8_t*)workspace;
+    OperandArgs o = {};
+    o.g = grad;
+    o.dtype = grad_dtype;
+    o.g_stride = grad_stride;
+    o.x_stride = x_stride;
+    o.w_stride = w_stride;
+    o.rows = rows;
+    o.cols = cols;
+    o.inner = inner;
+    o.x = x;
+    o.w = w;
+    o.x_scale = x_scale;
+    o.w_scale = w_scale;
+    o.rows_padded = padded_to_side(rows);
+    o.cols_padded = padded_to_side(cols);
+    if (dx) o.dx_left = (bf16*)(base + l.dx_left), o.dx_right = (bf16*)(base + l.dx_right);
+    if (dw) o.dw_left = (bf16*)(base + l.dw_left), o.dw_right = (bf16*)(base + l.dw_right);
+    o.g_tiles = (uint32_t)g_tiles;
+    o.w_tiles = (uint32_t)w_tiles;
+    const dim3 grid((uint32_t)(g_tiles + w_tiles + x_tiles));
+    if (terms == 1) k_grad_operands<1><<<grid, dim3(256), 0, s>>>(o);
+    else if (terms == 2) k_grad_operands<2><<<grid, dim3(256), 0, s>>>(o);
+    else k_grad_operands<3><<<grid, dim3(256), 0, s>>>(o);
+    const auto product = [&](const Shape& shape, size_t left, size_t right, bool cut, size_t partial, void* y, int dtype) {
         TileArgs a = {};
-        a.x = at;
-        a.w = at + l.left;
-        a.x_stride = terms * p * 2;
-        a.w_stride = p * 2;
-        a.rows = m;
-        a.cols = n;
-        a.inner = terms * p * 2;
-        a.w_stages = (int)(p * 2 / kStage);
+        a.x = base + left;
+        a.w = base + right;
+        a.x_stride = shape.inner;
+        a.w_stride = shape.inner / terms;
+        a.rows = shape.rows;
+        a.cols = shape.cols;
+        a.inner = shape.inner;
+        a.w_stages = (int)(a.w_stride / kStage);
         a.y = y;
         a.dtype = dtype;
-        return run_product<false>(a, at + l.left + l.right, s);
+        a.partial = cut ? (uint32_t*)(base + partial) : nullptr;
+        return a;
     };
-    const auto blocks = [](int64_t n) { return (uint32_t)((n + kSide - 1) / kSide); };
-    if (dx) {
-        const GradLayout l = grad_layout(rows, inner, cols, terms);
-        const int64_t p = padded_to_side(cols);
-        bf16 *left = (bf16*)workspace, *right = (bf16*)((uint8_t*)workspace + l.left);
-        const dim3 grid((uint32_t)((p / kChunk + 255) / 256), (uint32_t)(rows < 2048 ? rows : 2048));
-        if (terms == 1) k_scaled_grad<1><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, w_scale, rows, cols, p, left);
-        else if (terms == 2) k_scaled_grad<2><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, w_scale, rows, cols, p, left);
-        else k_scaled_grad<3><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, w_scale, rows, cols, p, left);
-        k_widen_t<<<dim3(blocks(cols), blocks(inner)), dim3(256), 0, s>>>(w, w_stride, cols, inner, p, right);
-        const int rc = product(rows, inner, cols, l, dx, dx_dtype);
-        if (rc != GEO_SC_OK) return rc;
-    }
+    TwoProducts both = {};
+    if (dx) both.first = product(l.dx, l.dx_left, l.dx_right, l.plan.splits[0] > 1, l.first_partial, dx, dx_dtype);
     if (dw) {
-        const GradLayout l = grad_layout(cols, inner, rows, terms);
-        const int64_t p = padded_to_side(rows);
-        bf16 *left = (bf16*)workspace, *right = (bf16*)((uint8_t*)workspace + l.left);
-        const dim3 grid(blocks(rows), blocks(cols));
-        if (terms == 1) k_scaled_grad_t<1><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, x_scale, rows, cols, p, left);
-        else if (terms == 2) k_scaled_grad_t<2><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, x_scale, rows, cols, p, left);
-        else k_scaled_grad_t<3><<<grid, dim3(256), 0, s>>>(grad, grad_dtype, grad_stride, x_scale, rows, cols, p, left);
-        k_widen_t<<<dim3(blocks(rows), blocks(inner)), dim3(256), 0, s>>>(x, x_stride, rows, inner, p, right);
-        const int rc = product(cols, inner, rows, l, dw, dw_dtype);
-        if (rc != GEO_SC_OK) return rc;
+        const int which = dx ? 1 : 0;
+        (dx ? both.second : both.first) =
+            product(l.dw, l.dw_left, l.dw_right, l.plan.splits[which] > 1, dx ? l.second_partial : l.first_partial, dw, dw_dtype);
     }
-    return GEO_SC_OK;
+    return run_products<false>(both, l.plan, s);
 }
 
 }  // extern "C"
