@@ -283,15 +283,133 @@ at::Tensor distill_topk_backward(const at::Tensor& grad, const at::Tensor& logit
     return dz;
 }
 
+// ---------------------------------------------------------------- autograd nodes
+//
+// In C++ like the calls themselves: of a training step on small layers the host's time is what counts, and the backward runs in
+// the engine's thread without the interpreter.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
+at::Tensor undefined_or(const MaybeTensor& t) { return t ? *t : at::Tensor(); }
+
+struct LinearQ8 : torch::autograd::Function<LinearQ8> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight)
+    {
+        const auto [q, scale, none] = quantize_rows(x, std::nullopt);
+        const auto [wq, wscale, none2] = quantize_rows(weight, std::nullopt);
+        ctx->save_for_backward({q, scale, wq, wscale});
+        ctx->saved_data["x"] = x.scalar_type();
+        ctx->saved_data["w"] = weight.scalar_type();
+        return matmul_q8(q, scale, wq, wscale, x.scalar_type());
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const auto s = ctx->get_saved_variables();
+        std::optional<at::ScalarType> x, w;
+        if (ctx->needs_input_grad(0)) x = ctx->saved_data["x"].toScalarType();
+        if (ctx->needs_input_grad(1)) w = ctx->saved_data["w"].toScalarType();
+        const auto [dx, dw] = matmul_q8_backward(grads[0], s[0], s[1], s[2], s[3], x, w);
+        return {undefined_or(dx), undefined_or(dw)};
+    }
+};
+
+// (q, scale, values, total); total is an output only where there is a residual
+struct RmsNormQ8 : torch::autograd::Function<RmsNormQ8> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const MaybeTensor& residual, double eps,
+                                 at::ScalarType values_type)
+    {
+        const auto [q, scale, total, values, rstd] = rms_norm_q8(x, weight, residual, eps, values_type, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({total, weight, *rstd});
+        ctx->mark_non_differentiable({q, scale});
+        variable_list out = {q, scale, *values};
+        if (residual) out.push_back(total);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const auto s = ctx->get_saved_variables();
+        const bool residual = grads.size() > 3;
+        const auto [dx, dw] = rms_norm_q8_backward(maybe(grads[2]), residual ? maybe(grads[3]) : MaybeTensor(), s[0], s[1], s[2],
+                                                   ctx->needs_input_grad(1));
+        return {ctx->needs_input_grad(0) ? dx : at::Tensor(), undefined_or(dw), residual && ctx->needs_input_grad(2) ? dx : at::Tensor(),
+                at::Tensor(), at::Tensor()};
+    }
+};
+
+// (y, total); total is an output only where there is a residual
+struct NormLinearQ8 : torch::autograd::Function<NormLinearQ8> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gain, const at::Tensor& weight,
+                                 const MaybeTensor& residual, double eps)
+    {
+        const auto [q, scale, total, none, rstd] = rms_norm_q8(x, gain, residual, eps, std::nullopt, true);
+        const auto [wq, wscale, none2] = quantize_rows(weight, std::nullopt);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, scale, wq, wscale, total, gain, *rstd});
+        ctx->saved_data["w"] = weight.scalar_type();
+        variable_list out = {matmul_q8(q, scale, wq, wscale, x.scalar_type())};
+        if (residual) out.push_back(total);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const auto s = ctx->get_saved_variables();
+        const bool residual = grads.size() > 1, need_gain = ctx->needs_input_grad(1);
+        const bool through = ctx->needs_input_grad(0) || need_gain || (residual && ctx->needs_input_grad(3));
+        MaybeTensor dn, dw, dgain;
+        at::Tensor dx;
+        if (grads[0].defined()) {
+            std::optional<at::ScalarType> x, w;
+            if (through) x = s[4].scalar_type();
+            if (ctx->needs_input_grad(2)) w = ctx->saved_data["w"].toScalarType();
+            std::tie(dn, dw) = matmul_q8_backward(grads[0], s[0], s[1], s[2], s[3], x, w);
+        }
+        if (through) std::tie(dx, dgain) = rms_norm_q8_backward(dn, residual ? maybe(grads[1]) : MaybeTensor(), s[4], s[5], s[6], need_gain);
+        return {ctx->needs_input_grad(0) ? dx : at::Tensor(), undefined_or(dgain), undefined_or(dw),
+                residual && ctx->needs_input_grad(3) ? dx : at::Tensor(), at::Tensor()};
+    }
+};
+
+struct DistillTopK : torch::autograd::Function<DistillTopK> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& top_logits, const at::Tensor& top_index,
+                              double temperature, int64_t reduction)
+    {
+        const auto [loss, stats] = distill_topk(logits, top_logits, top_index, temperature, reduction);
+        ctx->save_for_backward({logits, top_logits, top_index, stats});
+        ctx->saved_data["temperature"] = temperature;
+        ctx->saved_data["reduction"] = reduction;
+        return loss;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const auto s = ctx->get_saved_variables();
+        return {distill_topk_backward(grads[0], s[0], s[1], s[2], ctx->saved_data["temperature"].toDouble(), ctx->saved_data["reduction"].toInt(), s[3]),
+                at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    }
+};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
 {
     m.def("quantize_rows", &quantize_rows, "rows in 8 bits: (q, scale, values or None)");
-    m.def("rms_norm_q8", &rms_norm_q8, "root-mean-square norm with 8-bit output: (q, scale, total, values or None, rstd or None)");
-    m.def("rms_norm_q8_backward", &rms_norm_q8_backward, "(dx, dweight or None)");
+    m.def("rms_norm_q8", [](const at::Tensor& x, const at::Tensor& weight, const MaybeTensor& residual, double eps, std::optional<at::ScalarType> values) {
+        const auto [q, scale, total, v, rstd] = rms_norm_q8(x, weight, residual, eps, values, false);
+        return std::make_tuple(q, scale, total, v);
+    }, "root-mean-square norm with 8-bit output: (q, scale, total, values or None)");
+    m.def("rms_norm_q8_grad", [](const at::Tensor& x, const at::Tensor& weight, const MaybeTensor& residual, double eps, at::ScalarType values) {
+        const variable_list out = RmsNormQ8::apply(x, weight, residual, eps, values);
+        return std::make_tuple(out[0], out[1], residual ? out[3] : x, out[2]);
+    }, "the same, values and total differentiable");
     m.def("matmul_q8", &matmul_q8, "product of 8-bit rows with a scale each");
-    m.def("matmul_q8_backward", &matmul_q8_backward, "(dx or None, dw or None)");
-    m.def("distill_topk", &distill_topk, "divergence from a teacher's top logits: (loss, stats)");
-    m.def("distill_topk_backward", &distill_topk_backward, "gradient of the logits");
+    m.def("linear_q8", [](const at::Tensor& x, const at::Tensor& weight) { return LinearQ8::apply(x, weight); }, "product of x and weight rounded to 8-bit rows");
+    m.def("norm_linear_q8", [](const at::Tensor& x, const at::Tensor& gain, const at::Tensor& weight, const MaybeTensor& residual, double eps) {
+        const variable_list out = NormLinearQ8::apply(x, gain, weight, residual, eps);
+        return std::make_tuple(out[0], residual ? out[1] : x);
+    }, "the norm and the product: (y, total)");
+    m.def("distill_topk", [](const at::Tensor& logits, const at::Tensor& top_logits, const at::Tensor& top_index, double temperature, int64_t reduction) {
+        return DistillTopK::apply(logits, top_logits, top_index, temperature, reduction);
+    }, "divergence from a teacher's top logits");
 }

@@ -14,7 +14,6 @@ reference overwrites its value with the SC result anyway (utils_functional.py:63
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native, capi
 
@@ -175,8 +174,14 @@ def sc_counts(activation, weight, bit_length, padding, forward="1d_bin", load_un
 # fixed scale of ``quantize``.  All take GPU tensors (float32, bfloat16 or float16; rows are the last dimension) and run on PyTorch's
 # current stream.
 
+_dense_module = None
+
+
 def _dense():
-    return _native.module("sc_dense")
+    global _dense_module
+    if _dense_module is None:
+        _dense_module = _native.module("sc_dense")
+    return _dense_module
 
 
 def _wants_grad(*tensors):
@@ -190,27 +195,6 @@ def quantize_rows(x, values=None):
     return _dense().quantize_rows(x, values)
 
 
-class _RMSNormQ8(torch.autograd.Function):
-    """Values and sum of the norm; gradients straight through the rounding to 8 bits."""
-
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps, values):
-        q, scale, total, out, rstd = _dense().rms_norm_q8(x, weight, residual, eps, values, True)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(total, weight, rstd)
-        ctx.residual = residual is not None
-        ctx.mark_non_differentiable(q, scale)
-        return (q, scale, out, total) if ctx.residual else (q, scale, out)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, _q, _scale, grad_values, grad_total=None):
-        total, weight, rstd = ctx.saved_tensors
-        dx, dw = _dense().rms_norm_q8_backward(grad_values, grad_total, total, weight, rstd, ctx.needs_input_grad[1])
-        return (dx if ctx.needs_input_grad[0] else None, dw, dx if ctx.residual and ctx.needs_input_grad[2] else None,
-                None, None)
-
-
 def rms_norm_q8(x, weight, residual=None, eps=1e-6, values=None):
     """Root-mean-square norm of ``x + residual`` with 8-bit output: with ``total = x + residual``, the rows of
     ``total / sqrt(mean(total^2) + eps) * weight`` as ``quantize_rows`` has them.  Returns (q, scale, total, values);
@@ -221,9 +205,8 @@ def rms_norm_q8(x, weight, residual=None, eps=1e-6, values=None):
     if _wants_grad(x, weight, residual):
         if values is None:
             raise ValueError("rms_norm_q8 under autograd needs the type of values, which carry the gradient (or torch.no_grad())")
-        out = _RMSNormQ8.apply(x, weight, residual, float(eps), values)
-        return out[0], out[1], out[3] if residual is not None else x, out[2]
-    return _dense().rms_norm_q8(x, weight, residual, eps, values, False)[:4]
+        return _dense().rms_norm_q8_grad(x, weight, residual, eps, values)
+    return _dense().rms_norm_q8(x, weight, residual, eps, values)
 
 
 def matmul_q8(q, scale, weight_q, weight_scale, dtype=torch.float32):
@@ -233,83 +216,21 @@ def matmul_q8(q, scale, weight_q, weight_scale, dtype=torch.float32):
     return _dense().matmul_q8(q, scale, weight_q, weight_scale, dtype)
 
 
-class _LinearQ8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight):
-        dense = _dense()
-        q, scale, _ = dense.quantize_rows(x, None)
-        wq, wscale, _ = dense.quantize_rows(weight, None)
-        ctx.save_for_backward(q, scale, wq, wscale)
-        ctx.types = x.dtype, weight.dtype
-        return dense.matmul_q8(q, scale, wq, wscale, x.dtype)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        need_x, need_w = ctx.needs_input_grad
-        return _dense().matmul_q8_backward(grad, *ctx.saved_tensors, ctx.types[0] if need_x else None,
-                                           ctx.types[1] if need_w else None)
-
-
 def linear_q8(x, weight):
     """``x @ weight.t()`` with both operands rounded to 8-bit rows first, in ``x``'s type.  The gradients are those of the
     product at the rounded operands, passed straight through the rounding, as ``Conv2d_Add_Partial`` passes its own."""
-    return _LinearQ8.apply(x, weight)
-
-
-class _NormLinearQ8(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, gain, weight, residual, eps):
-        dense = _dense()
-        q, scale, total, _, rstd = dense.rms_norm_q8(x, gain, residual, eps, None, True)
-        wq, wscale, _ = dense.quantize_rows(weight, None)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, scale, wq, wscale, total, gain, rstd)
-        ctx.types, ctx.residual = (x.dtype, weight.dtype), residual is not None
-        y = dense.matmul_q8(q, scale, wq, wscale, x.dtype)
-        return (y, total) if ctx.residual else y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, grad_total=None):
-        q, scale, wq, wscale, total, gain, rstd = ctx.saved_tensors
-        need_x, need_gain, need_w, need_residual, _ = ctx.needs_input_grad
-        through = need_x or need_gain or need_residual
-        dn = dw = dx = dgain = None
-        if grad is not None:
-            dn, dw = _dense().matmul_q8_backward(grad, q, scale, wq, wscale, ctx.types[0] if through else None,
-                                                 ctx.types[1] if need_w else None)
-        if through:
-            dx, dgain = _dense().rms_norm_q8_backward(dn, grad_total, total, gain, rstd, need_gain)
-        return dx if need_x else None, dgain, dw, dx if need_residual else None, None
+    return _dense().linear_q8(x, weight)
 
 
 def norm_linear_q8(x, gain, weight, residual=None, eps=1e-6):
     """The root-mean-square norm of ``x + residual`` with 8-bit output (``rms_norm_q8``, weight ``gain``) and its
     product with ``weight`` rounded to 8-bit rows: (y, x + residual), differentiable in all four tensors."""
-    if residual is None:
-        return _NormLinearQ8.apply(x, gain, weight, None, float(eps)), x
-    return _NormLinearQ8.apply(x, gain, weight, residual, float(eps))
+    return _dense().norm_linear_q8(x, gain, weight, residual, eps)
 
 
 # ---------------------------------------------------------------- distillation
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
-
-
-class _DistillTopK(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, top_logits, top_index, temperature, reduction):
-        loss, stats = _dense().distill_topk(logits, top_logits, top_index, temperature, reduction)
-        ctx.save_for_backward(logits, top_logits, top_index, stats)
-        ctx.how = temperature, reduction
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        logits, top_logits, top_index, stats = ctx.saved_tensors
-        return _dense().distill_topk_backward(grad, logits, top_logits, top_index, *ctx.how, stats), None, None, None, None
 
 
 def distill_topk(logits, top_logits, top_index, temperature=1.0, reduction="mean"):
@@ -322,4 +243,4 @@ def distill_topk(logits, top_logits, top_index, temperature=1.0, reduction="mean
     "none".  The loss is float32; the gradient goes to ``logits`` only (the teacher is fixed)."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
-    return _DistillTopK.apply(logits, top_logits.detach(), top_index, float(temperature), _REDUCTIONS[reduction])
+    return _dense().distill_topk(logits, top_logits, top_index, temperature, _REDUCTIONS[reduction])
