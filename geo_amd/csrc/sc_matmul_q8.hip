@@ -445,35 +445,65 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
     const int begin = blockIdx.y * (a.stages_per_split / 2);
     const int end = begin + a.stages_per_split / 2 < steps ? begin + a.stages_per_split / 2 : steps;
     const int end_whole = end < whole ? end : whole;
-    const auto step = [&](const v4i (&w)[NT][2], const v4i (&x)[MT][2]) {
+    struct Step {
+        v4i w[NT][2], x[MT][2];
+    };
+    const auto multiply = [&](const Step& t) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) Matrix<true>::add(w[j][h], x[i][h], sum[j][i]);
+                for (int i = 0; i < MT; ++i) Matrix<true>::add(t.w[j][h], t.x[i][h], sum[j][i]);
     };
-#pragma unroll 4
-    for (int k = begin + wave; k < end_whole; k += kFewWaves) {
-        v4i w[NT][2], x[MT][2];
+    const auto load = [&](Step& t, int k) {
         const int64_t o = (int64_t)k * kStep;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) __builtin_memcpy(w[j], wp[j] + o, 32);
+        for (int j = 0; j < NT; ++j) __builtin_memcpy(t.w[j], wp[j] + o, 32);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) __builtin_memcpy(x[i], xp[i] + o, 32);
-        step(w, x);
+        for (int i = 0; i < MT; ++i) __builtin_memcpy(t.x[i], xp[i] + o, 32);
+    };
+    // kAhead steps on their way at once, x at the distance of w: loads come back in order.  (The steady part by itself, with
+    // no condition around its loads: behind one, the compiler waits for all of them.)
+    constexpr int kAhead = 16 / (MT + NT);
+    Step ahead[kAhead];
+    int k = begin + wave;
+    if (k + (2 * kAhead - 1) * kFewWaves < end_whole) {
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) load(ahead[d], k + d * kFewWaves);
+        for (; k + (2 * kAhead - 1) * kFewWaves < end_whole; k += kAhead * kFewWaves) {
+#pragma unroll
+            for (int d = 0; d < kAhead; ++d) {
+                multiply(ahead[d]);
+                load(ahead[d], k + (d + kAhead) * kFewWaves);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) multiply(ahead[d]);
+        k += kAhead * kFewWaves;
+    }
+    const int left = k < end_whole ? (end_whole - k + kFewWaves - 1) / kFewWaves : 0;   // fewer than 2 kAhead
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d)
+            if (half * kAhead + d < left) load(ahead[d], k + (half * kAhead + d) * kFewWaves);
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d)
+            if (half * kAhead + d < left) multiply(ahead[d]);
     }
     if (end > end_whole && (end_whole - begin) % kFewWaves == wave) {   // the last step, where it is not whole
-        v4i w[NT][2], x[MT][2];
+        Step t;
         const int64_t o = (int64_t)end_whole * kStep;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) w[j][h] = load_piece(wp[j] - at, o + at + h * 16, a.inner);
+            for (int j = 0; j < NT; ++j) t.w[j][h] = load_piece(wp[j] - at, o + at + h * 16, a.inner);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) x[i][h] = load_piece(xp[i] - at, o + at + h * 16, a.inner);
+            for (int i = 0; i < MT; ++i) t.x[i][h] = load_piece(xp[i] - at, o + at + h * 16, a.inner);
         }
-        step(w, x);
+        multiply(t);
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -490,6 +520,143 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
         for (int r = 0; r < 4; ++r) ws[r] = scale_at(a.w_scale, n + r, a.cols);
         finish_four(a, blockIdx.y, m, n, s, scale_at(a.x_scale, m, a.rows), ws);
     }
+}
+
+// The same for rows that start at multiples of 16 bytes: loads in the
+// order of the matrix instruction's operands give neighbouring lanes different rows, and the memory pipeline takes such a load's
+// lanes one by one (4096 x 16384 bytes of w: 16 us for 16 rows of x, 31 for 48).  Here each wave has a ring of its own in LDS, which
+// the loads fill in lines, and no barrier but where the waves' sums meet.  Workgroups stay: a wave's stages run on from one
+// 16 columns of y to its next, so that w streams.
+template <int MT>
+__global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a)
+{
+    constexpr int kStageBytes = (1 + MT) * 1024, kPlaces = 16384 / kStageBytes;
+    static_assert(kPlaces >= 3 && kPlaces <= 8, "");
+    __shared__ __align__(16) uint8_t p0[kFewWaves][kStageBytes], p1[kFewWaves][kStageBytes], p2[kFewWaves][kStageBytes],
+        p3[kFewWaves][kStageBytes], p4[kFewWaves][kStageBytes], p5[kFewWaves][kStageBytes], p6[kFewWaves][kStageBytes], p7[kFewWaves][kStageBytes];
+    __shared__ __align__(16) v4i sums[kFewWaves][MT][64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const auto place = [&](auto which) -> uint8_t* {
+        constexpr int r = decltype(which)::value % kPlaces;
+        if constexpr (r == 0) return p0[wave];
+        else if constexpr (r == 1) return p1[wave];
+        else if constexpr (r == 2) return p2[wave];
+        else if constexpr (r == 3) return p3[wave];
+        else if constexpr (r == 4) return p4[wave];
+        else if constexpr (r == 5) return p5[wave];
+        else if constexpr (r == 6) return p6[wave];
+        else return p7[wave];
+    };
+    const int whole = (int)(a.inner / kStage), each = (whole - wave + kFewWaves - 1) / kFewWaves;   // a wave's stages of a tile: at least 1
+    const int tiles = (int)((a.cols + 15) / 16), my_tiles = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int total = each * my_tiles;
+
+    // loads: 16 rows of 64 bytes, a lane a piece; the pieces of rows r lie at positions piece ^ (r / 4 & 3)
+    const int piece = ((lane & 3) ^ (lane >> 4)) * 16, load_row = lane >> 2;
+    int x_off[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t m = i * 16 + load_row;
+        x_off[i] = (int)((m < a.rows ? m : a.rows - 1) * a.x_stride) + piece;
+    }
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.x), 0, 0x7fffffff, 0x00020000);
+    int load_tile = blockIdx.x, load_stage = wave;
+    const auto load = [&](uint8_t* to) {   // the wave's next stage
+        const int64_t n0 = (int64_t)load_tile * 16, last = a.cols - 1 - n0;
+        const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.w + n0 * a.w_stride), 0, 0x7fffffff, 0x00020000);
+        const int w_off = (int)((load_row < last ? load_row : last) * a.w_stride) + piece, at = load_stage * kStage;
+        load_to_lds(wr, to, w_off, at);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) load_to_lds(xr, to + (1 + i) * 1024, x_off[i], at);
+        load_stage += kFewWaves;
+        if (load_stage >= whole) {
+            load_stage = wave;
+            load_tile += gridDim.x;
+        }
+    };
+    v4i sum[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sum[i] = v4i{0, 0, 0, 0};
+    const int mine = (lane & 15) * kStage + (((lane >> 4) ^ (lane >> 2 & 3)) << 4);
+    const auto multiply = [&](const uint8_t* from) {
+        const v4i w = *(const v4i*)(from + mine);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) Matrix<true>::add(w, *(const v4i*)(from + (1 + i) * 1024 + mine), sum[i]);
+    };
+    // (of a wave that finishes: its rows of y are the same in every tile)
+    const int64_t m = wave * 16 + (lane & 15);
+    const float xs = wave < MT ? a.x_scale[m < a.rows ? m : a.rows - 1] : 0.f;
+    typedef float Scales __attribute__((ext_vector_type(16), aligned(4)));
+    typedef const Scales __attribute__((address_space(4)))* ConstScales;
+    typedef const float __attribute__((address_space(4)))* ConstFloat;
+    int tile = blockIdx.x, left = each;
+    const auto finish = [&]() {   // the waves' sums of a tile
+        const int64_t n0 = (int64_t)tile * 16;
+        if (whole * kStage < a.inner && wave == kFewWaves - 1) {   // the last stage, where it is not whole
+            const int64_t n = n0 + (lane & 15), k = (int64_t)whole * kStage + (lane >> 4) * 16;
+            const v4i w = load_piece(a.w + (n < a.cols ? n : a.cols - 1) * a.w_stride, k, a.inner);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int64_t r = i * 16 + (lane & 15);
+                Matrix<true>::add(w, load_piece(a.x + (r < a.rows ? r : a.rows - 1) * a.x_stride, k, a.inner), sum[i]);
+            }
+        }
+        // (barriers that leave the loads on their way)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");   // the last tile's sums have been read
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            sums[wave][i][lane] = sum[i];
+            sum[i] = v4i{0, 0, 0, 0};
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (wave < MT) {
+            v4i s = sums[0][wave][lane];
+#pragma unroll
+            for (int k = 1; k < kFewWaves; ++k) s += sums[k][wave][lane];
+            // (sixteen scales by a scalar load: a vector load would be waited for behind all that are on their way)
+            Scales w16;
+            if (n0 + 16 <= a.cols) {
+                w16 = *(ConstScales)(a.w_scale + n0);
+            } else {
+                for (int t = 0; t < 16; ++t) w16[t] = n0 + t < a.cols ? *(ConstFloat)(a.w_scale + n0 + t) : 0.f;
+            }
+            float ws[4], v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ws[r] = lane < 16 ? w16[r] : lane < 32 ? w16[4 + r] : lane < 48 ? w16[8 + r] : w16[12 + r];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs * ws[r];
+            const int64_t n = n0 + (lane >> 4) * 4;
+            if (m < a.rows && n < a.cols) store_four(a.y, a.dtype, m * a.cols + n, a.cols - n, v);
+        }
+        tile += gridDim.x;
+        left = each;
+    };
+    const auto stage = [&](auto which, int at, auto steady) {
+        if (decltype(steady)::value || at + kPlaces <= total) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kPlaces - 1) * (1 + MT)) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        multiply(place(which));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // what was read may be overwritten
+        if (decltype(steady)::value || at + kPlaces < total) load(place(which));
+        if (--left == 0) finish();
+    };
+    const auto for_places = [&](auto f) {
+        [&]<int... R>(std::integer_sequence<int, R...>) { (f(Int<R>()), ...); }
+        (std::make_integer_sequence<int, kPlaces>());
+    };
+    int at = 0;
+    if (total >= 2 * kPlaces) {   // (the steady part by itself, with no condition around its loads: behind one, the compiler waits for all)
+        for_places([&](auto which) { load(place(which)); });
+        for (; at + 2 * kPlaces <= total; at += kPlaces)
+            for_places([&](auto which) { stage(which, at + decltype(which)::value, std::true_type()); });
+    } else {
+        for_places([&](auto which) {
+            if (decltype(which)::value < total) load(place(which));
+        });
+    }
+    for (; at < total; at += kPlaces)
+        for_places([&](auto which) {
+            if (at + decltype(which)::value < total) stage(which, at + decltype(which)::value, std::false_type());
+        });
 }
 
 // y from the sums of the splits, of both products of a launch
@@ -552,7 +719,8 @@ Plan plan_of(const Shape& s, const Shape& t, bool int8)
     Plan p = {};
     if (int8 && s.rows <= 64) {
         p.few = (int)((s.rows + 15) / 16);
-        cut(&p, 0, s, (s.cols + 15) / 16, kFewWaves);
+        // (a split and its join cost 3 us, in which a workgroup goes through 16 KB of its rows)
+        cut(&p, 0, s, (s.cols + 15) / 16, 128);
         return p;
     }
     const auto tiles = [&](int64_t b) { return s.tiles(b) + (t.rows ? t.tiles(b) : 0); };
@@ -565,9 +733,22 @@ Plan plan_of(const Shape& s, const Shape& t, bool int8)
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 size_t partial_bytes(const Plan& p, int which, const Shape& s) { return p.splits[which] > 1 ? align256((size_t)p.splits[which] * s.rows * s.cols * 4) : 0; }
 
+// loads that write LDS take 16-byte addresses, and offsets of 31 bits from a tile's first row
+bool loads_fit(const uint8_t* p, int64_t stride, int64_t rows, int64_t inner)
+{
+    return (uintptr_t)p % 16 == 0 && stride % 16 == 0 && stride * rows + inner < 0x7fffffff;
+}
+
 template <int MT>
 void run_few(const TileArgs& a, hipStream_t s)
 {
+    // Measured, us: 4096 x 4096, k_few_rows / streamed: 1 row 5.0 / 5.2, 4 rows 5.4 / 5.2, 16 rows 6.4 / 5.5; 4096 x 1024: 3.2 / 3.8 for
+    // any; 4096 x 16384: 16 rows 19.1 / 17.1, 48 rows 31 / 22, 64 rows 39 / 25.
+    if (a.splits == 1 && a.rows > 2 && a.inner >= 4 * kFewWaves * kStage && loads_fit(a.x, a.x_stride, 64, a.inner) && loads_fit(a.w, a.w_stride, 16, a.inner)) {
+        const int64_t tiles = (a.cols + 15) / 16;
+        k_few_streamed<MT><<<dim3((uint32_t)(tiles < kUnits ? tiles : kUnits)), dim3(kFewWaves * 64), 0, s>>>(a);
+        return;
+    }
     k_few_rows<MT, 1><<<dim3((uint32_t)((a.cols + 15) / 16), (uint32_t)a.splits), dim3(kFewWaves * 64), 0, s>>>(a);
 }
 
@@ -599,11 +780,7 @@ int run_products(TwoProducts both, const Plan& p, hipStream_t s)
         else if (p.few == 3) run_few<3>(both.first, s);
         else run_few<4>(both.first, s);
     } else {
-        // loads that write LDS take 16-byte addresses, and offsets of 31 bits from the tile's first row
-        const auto one_fits = [&](const uint8_t* q, int64_t stride, int64_t inner) {
-            return (uintptr_t)q % 16 == 0 && stride % 16 == 0 && stride * p.tile + inner < 0x7fffffff;
-        };
-        const auto fits = [&](const TileArgs& a) { return one_fits(a.x, a.x_stride, a.inner) && one_fits(a.w, a.w_stride, a.inner); };
+        const auto fits = [&](const TileArgs& a) { return loads_fit(a.x, a.x_stride, p.tile, a.inner) && loads_fit(a.w, a.w_stride, p.tile, a.inner); };
         const bool direct = fits(both.first) && (!both.second.rows || fits(both.second));
         if (p.tile == 256) run_tiles<256, INT8>(both, direct, s);
         else if (p.tile == 128) run_tiles<128, INT8>(both, direct, s);
