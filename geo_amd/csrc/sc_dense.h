@@ -39,26 +39,42 @@ __device__ __forceinline__ void load_chunk(const T* row, int64_t c, int64_t cols
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) v[j] = c + j < cols ? (float)row[c + j] : fill;
 }
+// `streamed`: past the caches, see streams()
 template <typename T>
-__device__ __forceinline__ void store_chunk(T* row, int64_t c, int64_t cols, const float (&v)[kChunk])
+__device__ __forceinline__ void store_chunk(T* row, int64_t c, int64_t cols, const float (&v)[kChunk], bool streamed = false)
 {
+    typedef int Piece __attribute__((ext_vector_type(4), aligned(2)));
     T raw[kChunk];
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) raw[j] = (T)v[j];
     if (c + kChunk <= cols) {
-        __builtin_memcpy(row + c, raw, sizeof raw);
+        if (streamed) {
+#pragma unroll
+            for (int p = 0; p < (int)sizeof raw / 16; ++p) {
+                Piece u;
+                __builtin_memcpy(&u, (const char*)raw + 16 * p, 16);
+                __builtin_nontemporal_store(u, (Piece*)(row + c) + p);
+            }
+        } else {
+            __builtin_memcpy(row + c, raw, sizeof raw);
+        }
         return;
     }
 #pragma unroll
     for (int j = 0; j < kChunk; ++j)
         if (c + j < cols) row[c + j] = raw[j];
 }
+// Whether a kernel's output goes past the caches.  What passes half of the 256 MB that the memory side caches is not found there by
+// the next kernel anyway, and in them it drives out what is read: 8191 x 4096 bf16 rows normed (134 MB of sum and
+// values) 88 us -> 74, the gradient of 4096 x 32768 logits (268 MB) 126 -> 117.  Smaller outputs stay for their reader.
+inline bool streams(int64_t bytes) { return bytes >= (int64_t)128 << 20; }
 // the same with the type known at run time only (one branch for all lanes)
-__device__ __forceinline__ void store_chunk(void* base, int dtype, int64_t offset, int64_t c, int64_t cols, const float (&v)[kChunk])
+__device__ __forceinline__ void store_chunk(void* base, int dtype, int64_t offset, int64_t c, int64_t cols, const float (&v)[kChunk],
+                                            bool streamed)
 {
-    if (dtype == GEO_SC_F32) store_chunk((f32*)base + offset, c, cols, v);
-    else if (dtype == GEO_SC_BF16) store_chunk((bf16*)base + offset, c, cols, v);
-    else store_chunk((f16*)base + offset, c, cols, v);
+    if (dtype == GEO_SC_F32) store_chunk((f32*)base + offset, c, cols, v, streamed);
+    else if (dtype == GEO_SC_BF16) store_chunk((bf16*)base + offset, c, cols, v, streamed);
+    else store_chunk((f16*)base + offset, c, cols, v, streamed);
 }
 __device__ __forceinline__ void load_chunk(const void* base, int dtype, int64_t offset, int64_t c, int64_t cols, float fill,
                                            float (&v)[kChunk])

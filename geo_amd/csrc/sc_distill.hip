@@ -33,6 +33,7 @@ struct DistillArgs {
     int grad_per_row;
     float factor;        // of the rows' losses in the result
     void* dz;
+    bool streamed;       // dz
 };
 
 __device__ __forceinline__ float exp_scaled(float difference, float c) { return __builtin_amdgcn_exp2f(difference * c); }
@@ -69,32 +70,47 @@ __device__ __forceinline__ float entry_logit(const DistillArgs& a, int64_t row, 
     return (float)((const f16*)a.top_logits)[at];
 }
 
+// A lane's first entry, asked for before the row is read: by itself it is three ways to memory, one after the other.
+struct Entry {
+    int64_t j;
+    float t, z;
+};
+template <typename T>
+__device__ __forceinline__ Entry entry_of(const DistillArgs& a, int64_t row, int k)
+{
+    Entry e = {-1, 0.f, 0.f};
+    if (k < a.top) {
+        e.j = entry_index(a, row, k);
+        e.t = entry_logit(a, row, k);
+        if (e.j >= 0) e.z = (float)((const T*)a.z)[row * a.z_stride + e.j];
+    }
+    return e;
+}
+
 // The row's loss from m and s, by one wave.
 template <typename T>
-__device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, float m, float s)
+__device__ __forceinline__ void finish_row(const DistillArgs& a, int64_t row, float m, float s, const Entry& mine)
 {
     const int lane = threadIdx.x & 63;
     const float c = log2e_over(a.temperature), inverse_t = 1.f / a.temperature;
-    float most = kMinusInfinity;
-    for (int k = lane; k < a.top; k += 64)
+    float most = mine.j >= 0 ? mine.t : kMinusInfinity;
+    for (int k = lane + 64; k < a.top; k += 64)
         if (entry_index(a, row, k) >= 0) most = fmaxf(most, entry_logit(a, row, k));
     most = wave_max_float(most);
     const float base = finite_base(most);
-    float total = 0.f;
-    for (int k = lane; k < a.top; k += 64)
+    float total = mine.j >= 0 ? exp_scaled(mine.t - base, c) : 0.f;
+    for (int k = lane + 64; k < a.top; k += 64)
         if (entry_index(a, row, k) >= 0) total += exp_scaled(entry_logit(a, row, k) - base, c);
     total = wave_sum(total);
     const bool empty = total == 0.f;
     const float inverse = empty ? 0.f : 1.f / total, log_total = logf(total), log_s = logf(s), m0 = finite_base(m);
     float loss = 0.f;
-    for (int k = lane; k < a.top; k += 64) {
-        const int64_t j = entry_index(a, row, k);
-        if (j < 0 || empty) continue;
-        const float t = entry_logit(a, row, k) - base, p = exp_scaled(t, c) * inverse;
-        if (p == 0.f) continue;
-        const float zj = (float)((const T*)a.z)[row * a.z_stride + j] - m0;
-        loss += p * ((t - zj) * inverse_t - log_total + log_s);
-    }
+    const auto add = [&](const Entry& e) {
+        const float t = e.t - base, p = exp_scaled(t, c) * inverse;
+        if (e.j >= 0 && !empty && p != 0.f) loss += p * ((t - (e.z - m0)) * inverse_t - log_total + log_s);
+    };
+    add(mine);
+    for (int k = lane + 64; k < a.top; k += 64) add(entry_of<T>(a, row, k));
     loss = wave_sum(loss) * a.temperature * a.temperature;
     if (lane == 0) {
         a.loss[row] = loss;
@@ -164,9 +180,10 @@ __global__ __launch_bounds__(1024) void k_distill_rows(DistillArgs a)
 {
     const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
     if (row >= a.rows) return;
+    const Entry mine = entry_of<T>(a, row, threadIdx.x < 64 ? (int)threadIdx.x : a.top);
     float m, s;
     scan_row<T>(a, row, 0, a.cols, m, s);
-    if (threadIdx.x < 64) finish_row<T>(a, row, m, s);
+    if (threadIdx.x < 64) finish_row<T>(a, row, m, s, mine);
 }
 
 template <typename T>
@@ -192,8 +209,9 @@ __global__ __launch_bounds__(64) void k_distill_join(DistillArgs a)
         m = p[0];
         s = p[1];
     }
+    const Entry mine = entry_of<T>(a, row, threadIdx.x);
     wave_join(m, s, log2e_over(a.temperature));
-    finish_row<T>(a, row, m, s);
+    finish_row<T>(a, row, m, s, mine);
 }
 
 // the rows' losses in a fixed order
@@ -215,13 +233,17 @@ __global__ __launch_bounds__(1024) void k_sum_losses(const float* rows_loss, int
 template <typename T>
 __global__ __launch_bounds__(1024) void k_distill_back(DistillArgs a)
 {
-    const int64_t row = (int64_t)blockIdx.y * blockDim.y + threadIdx.y, from = (int64_t)blockIdx.x * a.per_split;
+    extern __shared__ int32_t columns[];   // the entries' columns of each row of the block
+    // From the last rows on: what the forward, which commonly ran just before, read last is still in the caches.
+    const int64_t group = gridDim.y - 1 - blockIdx.y, row = group * blockDim.y + threadIdx.y, from = (int64_t)blockIdx.x * a.per_split;
     const int64_t to = from + a.per_split < a.cols ? from + a.per_split : a.cols;
     const bool live = row < a.rows;
     const T* z = (const T*)a.z + row * a.z_stride;
     T* dz = (T*)a.dz + row * a.cols;
+    int32_t* column = columns + threadIdx.y * a.top;
     const float c = log2e_over(a.temperature);
     float m = 0.f, inverse_s = 0.f, top_m = 0.f, top_inverse = 0.f, scale = 0.f;
+    Entry mine = {};
     if (live) {
         const float* st = a.stats + row * kStats;
         m = st[0];
@@ -229,35 +251,48 @@ __global__ __launch_bounds__(1024) void k_distill_back(DistillArgs a)
         top_m = st[2];
         top_inverse = st[3];
         scale = a.grad[a.grad_per_row ? row : 0] * a.factor * a.temperature;
+        mine = entry_of<T>(a, row, threadIdx.x);
+        for (int k = threadIdx.x; k < a.top; k += blockDim.x) column[k] = (int32_t)entry_index(a, row, k);
         const bool empty = top_inverse == 0.f;
         const float k = scale * inverse_s;
         const int64_t step = (int64_t)blockDim.x * kChunk;
-        for (int64_t at = from + (int64_t)threadIdx.x * kChunk; at < to; at += step) {
-            float v[kChunk];
-            load_chunk(z, at, to, 0.f, v);
+        const auto gradient = [&](float(&v)[kChunk]) {
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) v[j] = empty ? 0.f : exp_scaled(v[j] - m, c) * k;
-            store_chunk(dz, at, to, v);
+        };
+        constexpr int kAhead = 8;
+        int64_t at = from + (int64_t)threadIdx.x * kChunk;
+        for (; at + (kAhead - 1) * step + kChunk <= to; at += kAhead * step) {
+            float v[kAhead][kChunk];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) load_chunk(z + at + i * step, v[i]);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                gradient(v[i]);
+                store_chunk(dz, at + i * step, to, v[i], a.streamed);
+            }
+        }
+        for (; at < to; at += step) {
+            float v[kChunk];
+            load_chunk(z, at, to, 0.f, v);
+            gradient(v);
+            store_chunk(dz, at, to, v, a.streamed);
         }
     }
     // The entries' columns are written again, each by one thread: the one of the entry that names the column first,
     // which sums the weights of all that name it.
-    if (blockDim.x > 64) __syncthreads();
+    __syncthreads();
     if (!live || top_inverse == 0.f) return;
     for (int k = threadIdx.x; k < a.top; k += blockDim.x) {
-        const int64_t j = entry_index(a, row, k);
-        if (j < from || j >= to) continue;
+        const Entry e = k == (int)threadIdx.x ? mine : entry_of<T>(a, row, k);
+        if (e.j < from || e.j >= to) continue;
         bool owner = true;
-        float p = 0.f;
-        for (int f = 0; f < a.top; ++f) {
-            if (entry_index(a, row, f) != j) continue;
-            if (f < k) {
-                owner = false;
-                break;
-            }
-            p += exp_scaled(entry_logit(a, row, f) - top_m, c) * top_inverse;
-        }
-        if (owner) dz[j] = (T)(scale * (exp_scaled((float)z[j] - m, c) * inverse_s - p));
+        float p = exp_scaled(e.t - top_m, c) * top_inverse;
+        for (int f = 0; f < k; ++f) owner = owner && column[f] != (int32_t)e.j;
+        if (!owner) continue;
+        for (int f = k + 1; f < a.top; ++f)
+            if (column[f] == (int32_t)e.j) p += exp_scaled(entry_logit(a, row, f) - top_m, c) * top_inverse;
+        dz[e.j] = (T)(scale * (exp_scaled(e.z - m, c) * inverse_s - p));
     }
 }
 
@@ -308,7 +343,8 @@ int run_distill_back(const DistillArgs& a, hipStream_t s)
         b.grad = a.grad + (a.grad_per_row ? r : 0);
         b.top_logits = (const char*)a.top_logits + r * a.top * dtype_bytes(a.top_dtype);
         b.top_index = (const char*)a.top_index + r * a.top * (a.index64 ? 8 : 4);
-        k_distill_back<T><<<dim3((uint32_t)a.splits, (uint32_t)((b.rows + per_block - 1) / per_block)), dim3(threads, per_block), 0, s>>>(b);
+        k_distill_back<T><<<dim3((uint32_t)a.splits, (uint32_t)((b.rows + per_block - 1) / per_block)), dim3(threads, per_block),
+                            (size_t)per_block * a.top * sizeof(int32_t), s>>>(b);
     }
     return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
 }
@@ -396,6 +432,7 @@ int geo_sc_distill_topk_backward(const float* grad, int reduction, const void* l
     a.grad = grad;
     a.grad_per_row = reduction == GEO_SC_REDUCE_NONE;
     a.dz = dlogits;
+    a.streamed = streams(rows * cols * dtype_bytes(dtype));
     cut_rows(a, kGroups);
     hipStream_t s = (hipStream_t)stream;
     if (dtype == GEO_SC_F32) return run_distill_back<f32>(a, s);

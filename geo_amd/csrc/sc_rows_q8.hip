@@ -42,6 +42,7 @@ struct RowsArgs {
     float *scale, *rstd;
     void *total, *values;
     int values_dtype;
+    bool streamed;   // total and values
 };
 
 template <typename T, bool NORM>
@@ -78,94 +79,113 @@ __device__ __forceinline__ void write_chunk(const RowsArgs& a, int64_t row, int6
         for (int j = 0; j < kChunk; ++j)
             if (c + j < a.cols) out[c + j] = q[j];
     }
-    if (a.values) store_chunk(a.values, a.values_dtype, row * a.cols, c, a.cols, v);
+    if (a.values) store_chunk(a.values, a.values_dtype, row * a.cols, c, a.cols, v, a.streamed);
 }
 
-// One row per threadIdx.y; the row's blockDim.x threads hold ITEMS chunks of eight columns each in registers (ITEMS 0: the row
-// does not fit and is read a second time, out of L2, after the reduction).
+__device__ __forceinline__ float row_unit(const RowsArgs& a, float squares) { return 1.f / sqrtf(squares / (float)a.cols + a.eps); }
+
+// One row per threadIdx.y; the row's blockDim.x threads hold ITEMS chunks of eight columns each in registers from the only read to
+// the write.  (Blocks that stay, go on to further rows and ask for the next one ahead took 91 us where these take 84,
+// 8191 x 4096 bf16 with residual, total and values: new blocks hide a row's reduction better.)
 template <typename T, bool NORM, int ITEMS>
 __global__ __launch_bounds__(1024) void k_rows(RowsArgs a)
 {
     __shared__ RowSlots slots;
     const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    const bool live = row < a.rows;   // (blocks of several rows have one wave per row: no barrier)
-    const int threads = blockDim.x, t = threadIdx.x, waves = threads >> 6;
-    constexpr int kHeld = ITEMS > 0 ? ITEMS : 1;
-    float n[kHeld][kChunk];
-    float squares = 0.f;
+    const int threads = blockDim.x, t = threadIdx.x, waves = threads >> 6;   // (blocks of several rows have one wave per row: no barrier)
+    if (row >= a.rows) return;
+    const auto column = [&](int i) { return ((int64_t)i * threads + t) * kChunk; };
+    float n[ITEMS][kChunk], squares = 0.f;
     uint32_t most = 0;
-    const auto take = [&](int64_t c, float (&v)[kChunk], bool write_total) {
-        read_chunk<T, NORM>(a, row, c, v);
-        if constexpr (NORM) {
-            if (write_total && a.total && a.residual) store_chunk((T*)a.total + row * a.cols, c, a.cols, v);
-            float w[kChunk];
-            load_chunk((const T*)a.weight, c, a.cols, 0.f, w);
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                squares += v[j] * v[j];
-                v[j] *= w[j];
-            }
-        }
-    };
-    if (live) {
-        if constexpr (ITEMS > 0) {
+    for (int i = 0; i < ITEMS; ++i)
+        if (column(i) < a.cols) {
+            read_chunk<T, NORM>(a, row, column(i), n[i]);
+            if constexpr (NORM) {
+                if (a.total && a.residual) store_chunk((T*)a.total + row * a.cols, column(i), a.cols, n[i], a.streamed);
+                float w[kChunk];
+                load_chunk((const T*)a.weight, column(i), a.cols, 0.f, w);
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                const int64_t c = ((int64_t)i * threads + t) * kChunk;
-                if (c < a.cols) {
-                    take(c, n[i], true);
-#pragma unroll
-                    for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(n[i][j]));
+                for (int j = 0; j < kChunk; ++j) {
+                    squares += n[i][j] * n[i][j];
+                    n[i][j] *= w[j];
                 }
             }
-        } else {
-            for (int64_t c = (int64_t)t * kChunk; c < a.cols; c += (int64_t)threads * kChunk) {
-                take(c, n[0], true);
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(n[0][j]));
-            }
+            for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(n[i][j]));
         }
-    }
     row_reduce(squares, most, waves, slots, 0);
-    if (!live) return;
-    float unit = 1.f;
-    bool sound = true;
-    if constexpr (NORM) {
-        unit = 1.f / sqrtf(squares / (float)a.cols + a.eps);
-        sound = squares < __uint_as_float(kInfinityBits);
-    }
-    const RowScale rs = row_scale(most, unit, sound);
+    const float unit = NORM ? row_unit(a, squares) : 1.f;
+    const RowScale rs = row_scale(most, unit, !NORM || squares < __uint_as_float(kInfinityBits));
     if (t == 0) {
         a.scale[row] = rs.scale;
         if (NORM && a.rstd) a.rstd[row] = unit;
     }
-    if constexpr (ITEMS > 0) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int64_t c = ((int64_t)i * threads + t) * kChunk;
-            if (c < a.cols) write_chunk<T, NORM>(a, row, c, rs, n[i]);
+    for (int i = 0; i < ITEMS; ++i)
+        if (column(i) < a.cols) write_chunk<T, NORM>(a, row, column(i), rs, n[i]);
+}
+
+// Rows that do not fit into a block's registers: read a second time, out of L2, after the reduction.
+template <typename T, bool NORM>
+__global__ __launch_bounds__(1024) void k_rows_long(RowsArgs a)
+{
+    __shared__ RowSlots slots;
+    const int64_t row = blockIdx.x, first = (int64_t)threadIdx.x * kChunk, step = (int64_t)blockDim.x * kChunk;
+    float n[kChunk], squares = 0.f;
+    uint32_t most = 0;
+    const auto take = [&](int64_t c, bool write_total) {
+        read_chunk<T, NORM>(a, row, c, n);
+        if constexpr (NORM) {
+            if (write_total && a.total && a.residual) store_chunk((T*)a.total + row * a.cols, c, a.cols, n, a.streamed);
+            float w[kChunk];
+            load_chunk((const T*)a.weight, c, a.cols, 0.f, w);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+                squares += n[j] * n[j];
+                n[j] *= w[j];
+            }
         }
-    } else {
-        for (int64_t c = (int64_t)t * kChunk; c < a.cols; c += (int64_t)threads * kChunk) {
-            take(c, n[0], false);
-            write_chunk<T, NORM>(a, row, c, rs, n[0]);
-        }
+    };
+    for (int64_t c = first; c < a.cols; c += step) {
+        take(c, true);
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(n[j]));
+    }
+    row_reduce(squares, most, blockDim.x >> 6, slots, 0);
+    const float unit = NORM ? row_unit(a, squares) : 1.f;
+    const RowScale rs = row_scale(most, unit, !NORM || squares < __uint_as_float(kInfinityBits));
+    if (threadIdx.x == 0) {
+        a.scale[row] = rs.scale;
+        if (NORM && a.rstd) a.rstd[row] = unit;
+    }
+    for (int64_t c = first; c < a.cols; c += step) {
+        take(c, false);
+        write_chunk<T, NORM>(a, row, c, rs, n);
     }
 }
 
-template <typename T, bool NORM>
-int run_rows(const RowsArgs& a, hipStream_t s)
+// Threads of a row with `chunks` chunks: whole waves, at most 1024, of which each has `held` chunks.
+int threads_of_row(int64_t chunks, int held)
 {
+    const int64_t threads = ((chunks + held - 1) / held + 63) / 64 * 64;
+    return threads < 1024 ? (int)threads : 1024;
+}
+
+template <typename T, bool NORM>
+int run_rows(RowsArgs a, hipStream_t s)
+{
+    a.streamed = streams(a.rows * a.cols * ((a.total && a.residual ? (int64_t)sizeof(T) : 0) + (a.values ? dtype_bytes(a.values_dtype) : 0)));
     const int64_t chunks = (a.cols + kChunk - 1) / kChunk;
-    int threads = 64;
-    while (threads < 1024 && threads < chunks) threads *= 2;
+    // Two chunks per thread where there are rows enough to fill the compute units: half as many waves reduce a row.  8191 x 4096
+    // bf16 in 8 bits 29.8 -> 23.5 us, normed 97 -> 88.  Few rows are as fast as their longest thread.
+    const int threads = threads_of_row(chunks, a.rows >= 2048 && chunks > 64 ? 2 : 1), per_block = threads == 64 ? 4 : 1;
     const int64_t items = (chunks + threads - 1) / threads;
-    const int per_block = threads == 64 ? 4 : 1;
     const dim3 grid((uint32_t)((a.rows + per_block - 1) / per_block)), block(threads, per_block);
     if (items <= 1) k_rows<T, NORM, 1><<<grid, block, 0, s>>>(a);
     else if (items <= 2) k_rows<T, NORM, 2><<<grid, block, 0, s>>>(a);
     else if (items <= 4) k_rows<T, NORM, 4><<<grid, block, 0, s>>>(a);
-    else k_rows<T, NORM, 0><<<grid, block, 0, s>>>(a);
+    else k_rows_long<T, NORM><<<dim3((uint32_t)a.rows), dim3(1024), 0, s>>>(a);
     return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
 }
 
@@ -185,12 +205,15 @@ struct NormBackArgs {
     int64_t rows, cols, grad_stride, grad_total_stride, total_stride;
     const float* rstd;
     void *dx;
+    bool streamed;    // dx
     float* partial;   // [blocks][cols]: sums of the weight's gradient, NULL: not wanted
 };
 
+// (Asking for the next row ahead of the exchange took 76 us where this takes 71, 8191 x 4096 bf16 with both gradients: the
+// registers that it needs cost a block per compute unit.)
 // A block takes every gridDim.x-th row; its threads keep the weight and their columns' sums of the weight's gradient in
 // registers over all rows of the block.
-template <typename T, int ITEMS>
+template <typename T, typename G, int ITEMS>
 __global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs a)
 {
     __shared__ RowSlots slots;
@@ -203,43 +226,37 @@ __global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs a)
         for (int j = 0; j < kChunk; ++j) w[i][j] = dw[i][j] = 0.f;
         if (c < a.cols) load_chunk((const T*)a.weight, c, a.cols, 0.f, w[i]);
     }
+    const auto column = [&](int i) { return ((int64_t)i * threads + t) * kChunk; };
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, ++turn) {
-        const float r = a.rstd[row];
-        float g[ITEMS][kChunk], v[ITEMS][kChunk], along = 0.f;
+        const float unit = a.rstd[row];
+        float g[ITEMS][kChunk], v[ITEMS][kChunk], h[ITEMS][kChunk], along = 0.f;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int64_t c = ((int64_t)i * threads + t) * kChunk;
-            if (c < a.cols) {
-                load_chunk(a.grad_values, a.grad_dtype, row * a.grad_stride, c, a.cols, 0.f, g[i]);
-                load_chunk((const T*)a.total + row * a.total_stride, c, a.cols, 0.f, v[i]);
+        for (int i = 0; i < ITEMS; ++i)
+            if (column(i) < a.cols) {
+                load_chunk((const G*)a.grad_values + row * a.grad_stride, column(i), a.cols, 0.f, g[i]);
+                load_chunk((const T*)a.total + row * a.total_stride, column(i), a.cols, 0.f, v[i]);
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) h[i][j] = 0.f;
+                if (a.grad_total) load_chunk((const T*)a.grad_total + row * a.grad_total_stride, column(i), a.cols, 0.f, h[i]);
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
-                    dw[i][j] += g[i][j] * (v[i][j] * r);
+                    dw[i][j] += g[i][j] * (v[i][j] * unit);
                     g[i][j] *= w[i][j];
                     along += g[i][j] * v[i][j];
                 }
             }
-        }
         uint32_t none = 0;
         row_reduce(along, none, waves, slots, turn);
-        const float back = along / (float)a.cols * r * r;
+        const float back = along / (float)a.cols * unit * unit;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i) {
-            const int64_t c = ((int64_t)i * threads + t) * kChunk;
-            if (c < a.cols) {
+        for (int i = 0; i < ITEMS; ++i)
+            if (column(i) < a.cols) {
                 float d[kChunk];
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) d[j] = r * (g[i][j] - v[i][j] * back);
-                if (a.grad_total) {
-                    float h[kChunk];
-                    load_chunk((const T*)a.grad_total + row * a.grad_total_stride, c, a.cols, 0.f, h);
-#pragma unroll
-                    for (int j = 0; j < kChunk; ++j) d[j] += h[j];
-                }
-                store_chunk((T*)a.dx + row * a.cols, c, a.cols, d);
+                for (int j = 0; j < kChunk; ++j) d[j] = unit * (g[i][j] - v[i][j] * back) + h[i][j];
+                store_chunk((T*)a.dx + row * a.cols, column(i), a.cols, d, a.streamed);
             }
-        }
     }
     if (a.partial) {
 #pragma unroll
@@ -285,7 +302,7 @@ __global__ __launch_bounds__(1024) void k_norm_back_long(NormBackArgs a)
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) g[j] += w[j];
         }
-        store_chunk((T*)a.dx + row * a.cols, c, a.cols, g);
+        store_chunk((T*)a.dx + row * a.cols, c, a.cols, g, a.streamed);
     }
 }
 template <typename T>
@@ -304,16 +321,18 @@ __global__ __launch_bounds__(256) void k_weight_grad_columns(NormBackArgs a)
     store_chunk(a.partial + (int64_t)blockIdx.y * a.cols, c, a.cols, dw);
 }
 
-// dweight[c] = the sum over the blocks' partial sums: 32 columns by 8 shares of the blocks in a workgroup, joined in a fixed order
-constexpr int kJoinCols = 32, kJoinShares = 8;
+// dweight[c] = the sum over the blocks' partial sums: 32 columns by 32 shares of the blocks in a workgroup, joined in a fixed order
+constexpr int kJoinCols = 32, kJoinShares = 32;
 template <typename T>
 __global__ __launch_bounds__(kJoinCols * kJoinShares) void k_join_weight_grad(const float* partial, int64_t blocks, int64_t cols, T* dw)
 {
     __shared__ float sums[kJoinShares][kJoinCols];
     const int64_t c = (int64_t)blockIdx.x * kJoinCols + threadIdx.x;
     float s = 0.f;
-    if (c < cols)
+    if (c < cols) {
+#pragma unroll 16
         for (int64_t b = threadIdx.y; b < blocks; b += kJoinShares) s += partial[b * cols + c];
+    }
     sums[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && c < cols) {
@@ -333,20 +352,29 @@ int64_t norm_back_blocks(int64_t rows, int64_t cols)
     return rows < most ? rows : most;
 }
 
+template <typename T, typename G>
+void run_norm_back_held(const NormBackArgs& a, int64_t blocks, hipStream_t s)
+{
+    const int64_t chunks = (a.cols + kChunk - 1) / kChunk;
+    const int threads = threads_of_row(chunks, 1);
+    if (chunks <= threads) k_norm_back<T, G, 1><<<dim3((uint32_t)blocks), dim3(threads), 0, s>>>(a);
+    else k_norm_back<T, G, 2><<<dim3((uint32_t)blocks), dim3(threads), 0, s>>>(a);
+}
+
 template <typename T>
 int run_norm_back(const NormBackArgs& a, T* dw, hipStream_t s)
 {
     const int64_t chunks = (a.cols + kChunk - 1) / kChunk, blocks = norm_back_blocks(a.rows, a.cols);
-    int threads = 64;
-    while (threads < 1024 && threads < chunks) threads *= 2;
     if (a.cols > kHeldBackCols) {
         k_norm_back_long<T><<<dim3((uint32_t)a.rows), dim3(1024), 0, s>>>(a);
         if (a.partial)
             k_weight_grad_columns<T><<<dim3((uint32_t)((chunks + 255) / 256), (uint32_t)blocks), dim3(256), 0, s>>>(a);
-    } else if (chunks <= threads) {
-        k_norm_back<T, 1><<<dim3((uint32_t)blocks), dim3(threads), 0, s>>>(a);
+    } else if (a.grad_dtype == GEO_SC_F32) {
+        run_norm_back_held<T, f32>(a, blocks, s);
+    } else if (a.grad_dtype == GEO_SC_BF16) {
+        run_norm_back_held<T, bf16>(a, blocks, s);
     } else {
-        k_norm_back<T, 2><<<dim3((uint32_t)blocks), dim3(threads), 0, s>>>(a);
+        run_norm_back_held<T, f16>(a, blocks, s);
     }
     if (a.partial)
         k_join_weight_grad<T><<<dim3((uint32_t)((a.cols + kJoinCols - 1) / kJoinCols)), dim3(kJoinCols, kJoinShares), 0, s>>>(
@@ -393,7 +421,7 @@ int geo_sc_rms_norm_q8(const void* x, const void* residual, const void* weight, 
     if (rows == 0) return GEO_SC_OK;
     if (!x || !weight || !q || !scale) return GEO_SC_ERR_INVALID_ARGUMENT;
     const RowsArgs a = {x, residual, weight, rows, cols, x_stride, residual_stride, q_stride, eps, q, scale, rstd, total, values,
-                        values_dtype};
+                        values_dtype, false};
     return run_rows<true>(a, dtype, (hipStream_t)stream);
 }
 
@@ -416,7 +444,7 @@ int geo_sc_rms_norm_q8_backward(const void* grad_values, int grad_dtype, int64_t
     geo_sc_rms_norm_q8_backward_workspace_size(rows, cols, &need);
     if (dweight && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 4)) return GEO_SC_ERR_WORKSPACE;
     const NormBackArgs a = {grad_values, grad_total, total, weight, grad_dtype, rows, cols, grad_stride, grad_total_stride,
-                            total_stride, rstd, dx, dweight ? (float*)workspace : nullptr};
+                            total_stride, rstd, dx, streams(rows * cols * dtype_bytes(dtype)), dweight ? (float*)workspace : nullptr};
     hipStream_t s = (hipStream_t)stream;
     if (dtype == GEO_SC_F32) return run_norm_back<f32>(a, (f32*)dweight, s);
     if (dtype == GEO_SC_BF16) return run_norm_back<bf16>(a, (bf16*)dweight, s);
