@@ -261,6 +261,40 @@ class VGG16_add_partial(nn.Module):
         return self.bnfc1(x)
 
 
+class PatchMLP_q8(nn.Module):
+    """Residual network of dense 8-bit layers on image patches: every patch of ``patch`` x ``patch`` pixels is a row; blocks of
+    norm, widening, relu and narrowing; the rows' mean through a last norm and layer.  All products are exact 8-bit ones
+    (``utils_class.Linear_Q8``), so it serves as the teacher of an SC network (``python -m geo_amd.main_distill``).  Not in
+    the reference."""
+
+    def __init__(self, num_classes=10, c_in=3, patch=4, width=256, hidden=1024, depth=4):
+        super().__init__()
+        self.patch = patch
+        self.embed = utils_class.Linear_Q8(c_in * patch * patch, width)
+        self.up = nn.ModuleList(utils_class.NormLinear_Q8(width, hidden) for _ in range(depth))
+        self.down = nn.ModuleList(utils_class.Linear_Q8(hidden, width) for _ in range(depth))
+        self.head = utils_class.NormLinear_Q8(width, num_classes)
+
+    def prepare(self):
+        """Round all weights for inference (``Linear_Q8.prepare``)."""
+        for layer in self.modules():
+            if isinstance(layer, utils_class.Linear_Q8):
+                layer.prepare()
+
+    def forward(self, images):
+        n, c, h, w = images.shape
+        p = self.patch
+        if h % p or w % p:
+            raise ValueError(f"images of {h} x {w} have no whole patches of {p} x {p}")
+        rows = images.reshape(n, c, h // p, p, w // p, p).permute(0, 2, 4, 1, 3, 5).reshape(n, -1, c * p * p)
+        y, total = self.embed(rows), None
+        for up, down in zip(self.up, self.down):
+            wide, total = up(y, total)
+            y = down(F.relu(wide))
+        logits, _ = self.head((total + y).mean(1))
+        return logits
+
+
 def make_param_copies(model):
     """Full-precision master copies the optimiser updates (main_conv.py:203-213)."""
     return [p.detach().clone().float().requires_grad_(True) for p in model.parameters()]

@@ -217,3 +217,50 @@ def sc_conv_block(conv, bn, input, *, err=7, forward="1d_bin", z_unit=8, load_un
     if quant7 and hardtanh:
         out._geo_q7_version = out._version   # values k / 128, 0 <= k <= 127, until somebody writes to the tensor
     return out
+
+
+class Linear_Q8(nn.Module):
+    """Linear layer without bias whose operands are rounded to 8-bit rows (``utils_functional.linear_q8``): the exact counterpart
+    of an SC layer's product.  In training the weight is rounded on every call and the gradients pass straight through; for
+    inference ``prepare()`` rounds it once, until ``train()`` or ``load_state_dict`` drops the result."""
+
+    def __init__(self, in_features, out_features):
+        super().__init__()
+        self.weight = nn.Parameter(torch.empty(out_features, in_features))
+        nn.init.kaiming_uniform_(self.weight, a=5 ** 0.5)
+        self._q8 = None
+
+    @torch.no_grad()
+    def prepare(self):
+        """Round the weight for inference.  Call again after changing it."""
+        self._q8 = utils_functional.quantize_rows(self.weight)[:2]
+
+    def train(self, mode=True):
+        self._q8 = None
+        return super().train(mode)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._q8 = None
+        super()._load_from_state_dict(*args, **kwargs)
+
+    def forward(self, x):
+        if self._q8 is None or torch.is_grad_enabled():
+            return utils_functional.linear_q8(x, self.weight)
+        q, scale, _ = utils_functional.quantize_rows(x)
+        return utils_functional.matmul_q8(q, scale, *self._q8, dtype=x.dtype)
+
+
+class NormLinear_Q8(Linear_Q8):
+    """Root-mean-square norm of ``x + residual`` with 8-bit output, then the product of ``Linear_Q8``
+    (``utils_functional.norm_linear_q8``).  Returns (y, x + residual)."""
+
+    def __init__(self, in_features, out_features, eps=1e-6):
+        super().__init__(in_features, out_features)
+        self.gain = nn.Parameter(torch.ones(in_features))
+        self.eps = eps
+
+    def forward(self, x, residual=None):
+        if self._q8 is None or torch.is_grad_enabled():
+            return utils_functional.norm_linear_q8(x, self.gain, self.weight, residual=residual, eps=self.eps)
+        q, scale, total, _ = utils_functional.rms_norm_q8(x, self.gain, residual=residual, eps=self.eps)
+        return utils_functional.matmul_q8(q, scale, *self._q8, dtype=x.dtype), total
