@@ -140,29 +140,233 @@ __device__ __forceinline__ void finish_four(const TileArgs& a, int split, int64_
 
 __device__ __forceinline__ float scale_at(const float* scale, int64_t i, int64_t count) { return scale && i < count ? scale[i] : 1.f; }
 
-// Tiles of BM rows of x by BN rows of w; WM x WN waves, each with (BM / WM) x (BN / WN) outputs in 16x16 squares.  w is the matrix
+// ---------------------------------------------------------------- tiles
+//
+// Tiles of B rows of x by B rows of w; four waves, each with a quarter of the outputs in 16x16 squares.  w is the matrix
 // instruction's first operand, so a lane's four sums are consecutive columns of y.
 //
 // A stage is 64 bytes of every row, one matrix instruction deep, in LDS as four 16-byte pieces per row at positions
-// piece ^ (row / 4 & 3): the 16 lanes that read the same piece of 16 rows meet every bank once.
-// DIRECT: rows start at multiples of 16 bytes and the loads write LDS themselves, into a ring of kRing stages: while a wave
-// multiplies stage s out of registers, stage s + 1 moves from LDS to its other registers and the stages up to s + kRing are on their
-// way.  One barrier per stage: it says that every wave's share of stage s + 1 has come and that all have read stage s,
-// whose place stage s + kRing takes.  Otherwise, and for a last stage that is not whole, through registers.
-constexpr int kRing = 4;
+// piece ^ (row / 4 & 2): then no two of the lanes that the LDS serves at once (of its read of 16 bytes, measured: 0 - 3, 12 - 15 and 20 - 27, and so
+// on) meet in a bank.
+constexpr int kRing = 4, kWaves = 4;
 
-template <int BM, int BN, int WM, int WN, bool INT8, bool DIRECT>
-__global__ __launch_bounds__(WM* WN * 64) void k_tiles(TwoProducts both)
-{
-    const bool is_second = blockIdx.x >= both.second_at;
-    const TileArgs a = is_second ? both.second : both.first;
-    const uint32_t group = blockIdx.x - (is_second ? both.second_at : 0);
-    constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, LX = BM / 16 / W, LW = BN / 16 / W;
-    static_assert(LX * W * 16 == BM && LW * W * 16 == BN, "every wave stages as many rows");
+template <int B, bool INT8>
+struct Tiling {
     typedef typename Matrix<INT8>::Sum Sum;
+    static constexpr int T = B / 32;               // squares of a wave in either direction
+    static constexpr int L = B / 16 / kWaves;      // a wave's loads of either operand for a stage, 16 rows each
+    static constexpr int kBytes = 2 * B * kStage;  // of a stage
+    static constexpr int kArea = 16 * T * 64;      // bytes of 16 rows of a wave's sums
+};
+
+// Where a workgroup works: its product's tile and split.
+struct Spot {
+    TileArgs a;
+    int64_t m0, n0;
+    uint32_t split, die;
+    int begin, stop, end;   // stages: whole ones up to stop, one more where the inner dimension ends inside it
+};
+
+// Workgroups go to the eight dies in turn: each die takes a contiguous share of the tiles, so that neighbours share its L2, in
+// strips of four tiles of rows.
+template <int B>
+__device__ __forceinline__ Spot spot_of(const TwoProducts& both, uint32_t work)
+{
+    Spot p;
+    const bool is_second = work >= both.second_at;
+    p.a = is_second ? both.second : both.first;
+    const uint32_t group = work - (is_second ? both.second_at : 0), all = (uint32_t)p.a.tiles_m * p.a.tiles_n;
+    p.split = group / all;
+    p.die = group % all & 7;
+    const uint32_t tile = p.die * (all / 8) + (p.die < all % 8 ? p.die : all % 8) + (group % all >> 3);
+    constexpr uint32_t kStrip = 4;
+    const uint32_t strip = tile / (kStrip * p.a.tiles_n), inside = tile - strip * kStrip * p.a.tiles_n;
+    const uint32_t height = p.a.tiles_m - strip * kStrip < kStrip ? p.a.tiles_m - strip * kStrip : kStrip;
+    p.m0 = (int64_t)(strip * kStrip + inside % height) * B;
+    p.n0 = (int64_t)(inside / height) * B;
+    const int stages = (int)((p.a.inner + kStage - 1) / kStage), whole = (int)(p.a.inner / kStage);
+    p.begin = p.split * p.a.stages_per_split;
+    p.end = p.begin + p.a.stages_per_split < stages ? p.begin + p.a.stages_per_split : stages;
+    p.stop = p.end < whole ? p.end : whole;
+    return p;
+}
+
+__device__ __forceinline__ int w_stage(const TileArgs& a, int k)   // (at most three terms)
+{
+    if (k >= a.w_stages) k -= a.w_stages;
+    return k >= a.w_stages ? k - a.w_stages : k;
+}
+// row that a lane loads for the i-th time, from the tile's first; rows behind the operand's last are its last again, their
+// outputs are not stored
+__device__ __forceinline__ int64_t load_row(int64_t first, int64_t rows, int i, int wave, int lane)
+{
+    const int64_t r = (int64_t)(i * kWaves + wave) * 16 + (lane >> 2);
+    return first + r < rows ? r : rows - 1 - first;
+}
+__device__ __forceinline__ int load_piece_of(int lane) { return (lane & 3) ^ (lane >> 4 & 2); }
+
+// A stage through registers: any alignment, zeros behind the end of a row.
+template <int L>
+__device__ __forceinline__ void fetch_stage(const Spot& p, int k, int wave, int lane, v4i (&v)[2 * L])
+{
+    const int64_t xk = (int64_t)k * kStage + load_piece_of(lane) * 16, wk = (int64_t)w_stage(p.a, k) * kStage + load_piece_of(lane) * 16;
+#pragma unroll
+    for (int i = 0; i < L; ++i) v[i] = load_piece(p.a.x + (p.m0 + load_row(p.m0, p.a.rows, i, wave, lane)) * p.a.x_stride, xk, p.a.inner);
+#pragma unroll
+    for (int i = 0; i < L; ++i) v[L + i] = load_piece(p.a.w + (p.n0 + load_row(p.n0, p.a.cols, i, wave, lane)) * p.a.w_stride, wk, p.a.inner);
+}
+template <int L>
+__device__ __forceinline__ void put_stage(uint8_t* to, int wave, int lane, const v4i (&v)[2 * L])
+{
+#pragma unroll
+    for (int i = 0; i < 2 * L; ++i) *(v4i*)(to + (i * kWaves + wave) * 1024 + lane * 16) = v[i];
+}
+
+// A wave's fragments of a stage: T of w, then T of x.
+template <int B>
+struct Fragments {
+    static constexpr int T = B / 32;
+    int x, w;   // bytes from the stage's begin
+    __device__ Fragments(int wave, int lane)
+    {
+        const int mine = (lane & 15) * kStage + (((lane >> 4) ^ (lane >> 2 & 2)) << 4);
+        x = wave % 2 * T * 16 * kStage + mine;
+        w = (B + wave / 2 * T * 16) * kStage + mine;
+    }
+    __device__ __forceinline__ void read_one(v4i (&f)[2 * T], const uint8_t* from, int t) const
+    {
+        f[t] = *(const v4i*)(from + (t < T ? w + t * 16 * kStage : x + (t - T) * 16 * kStage));
+    }
+    __device__ __forceinline__ void read(v4i (&f)[2 * T], const uint8_t* from) const
+    {
+#pragma unroll
+        for (int t = 0; t < 2 * T; ++t) read_one(f, from, t);
+    }
+};
+template <bool INT8, int T>
+__device__ __forceinline__ void multiply_one(const v4i (&f)[2 * T], typename Matrix<INT8>::Sum (&sum)[T][T], int t)
+{
+    Matrix<INT8>::add_in_place(f[t / T], f[T + t % T], sum[t / T][t % T]);
+}
+template <bool INT8, int T>
+__device__ __forceinline__ void multiply(const v4i (&f)[2 * T], typename Matrix<INT8>::Sum (&sum)[T][T])
+{
+#pragma unroll
+    for (int t = 0; t < T * T; ++t) multiply_one<INT8, T>(f, sum, t);
+}
+
+// The scales of a wave's rows and columns, all asked for at once: each by itself would be waited for by itself.
+template <int T>
+struct TileScales {
+    float x[T], w[T][4];
+    __device__ __forceinline__ void load(const Spot& p, int wave, int lane)
+    {
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+            x[j] = 1.f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[j][r] = 1.f;
+        }
+        if (p.a.w_scale) {
+#pragma unroll
+            for (int j = 0; j < T; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int64_t n = p.n0 + (wave / 2 * T + j) * 16 + (lane >> 4) * 4 + r;
+                    w[j][r] = p.a.w_scale[n < p.a.cols ? n : p.a.cols - 1];
+                }
+        }
+        if (p.a.x_scale) {
+#pragma unroll
+            for (int i = 0; i < T; ++i) {
+                const int64_t m = p.m0 + (wave % 2 * T + i) * 16 + (lane & 15);
+                x[i] = p.a.x_scale[m < p.a.rows ? m : p.a.rows - 1];
+            }
+        }
+    }
+};
+
+template <int B>
+__device__ __forceinline__ bool inside(const Spot& p) { return p.m0 + B <= p.a.rows && p.n0 + B <= p.a.cols; }
+
+// A tile's sums scaled, rounded and stored, or handed to the join as they are.  Out through LDS, each wave in an area of its own: a
+// lane holds four columns of one row, the lanes that share a row store 16 bytes each and fill its lines.  Positions of the
+// 16-byte pieces ^ row: no two lanes of a quarter wave meet in a bank.
+template <int B, bool INT8>
+__device__ __forceinline__ void finish_tile(const Spot& p, typename Matrix<INT8>::Sum (&sum)[B / 32][B / 32], const TileScales<B / 32>& scales,
+                                            uint8_t* area, int wave, int lane)
+{
+    constexpr int T = B / 32;
+    const bool fits = inside<B>(p);
+    const auto finish = [&](auto* y, auto value) {
+        using Y = std::remove_pointer_t<decltype(y)>;
+        constexpr int kEach = 16 / (int)sizeof(Y), kPieces = T * 16 / kEach, kAtOnce = 64 / kPieces;   // elements, pieces of a row, rows of a store
+        constexpr int kMix = (kPieces < 16 ? kPieces : 16) - 1, kBatch = 4 / (int)sizeof(Y);           // squares of rows that the area holds
+        const int row = lane & 15, column = (lane >> 4) * 4;
+#pragma unroll
+        for (int first = 0; first < T; first += kBatch) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+                for (int j = 0; j < T; ++j) {
+                    typename Matrix<INT8>::Sum s = sum[j][first + i];
+                    asm volatile("" : "+v"(s));   // (here, and not for all types at once before the choice of one)
+                    Y four[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) four[r] = value(s[r], first + i, j, r);
+                    const int at = j * 16 + column, where = (i * 16 + row) * kPieces + ((at / kEach) ^ (row & kMix));
+                    __builtin_memcpy(area + where * 16 + at % kEach * sizeof(Y), four, sizeof four);
+                }
+            __builtin_amdgcn_wave_barrier();
+            const int64_t m1 = p.m0 + (wave % 2 * T + first) * 16, n = p.n0 + wave / 2 * T * 16 + lane % kPieces * kEach;
+            v4i u[16 * kBatch / kAtOnce];
+#pragma unroll
+            for (int h = 0; h < 16 * kBatch / kAtOnce; ++h) {
+                const int r = h * kAtOnce + lane / kPieces;
+                u[h] = *(const v4i*)(area + (r * kPieces + (lane % kPieces ^ (r & kMix))) * 16);
+            }
+            if (fits) {
+#pragma unroll
+                for (int h = 0; h < 16 * kBatch / kAtOnce; ++h)
+                    __builtin_memcpy(y + (m1 + h * kAtOnce + lane / kPieces) * p.a.cols + n, &u[h], 16);
+            } else {
+#pragma unroll
+                for (int h = 0; h < 16 * kBatch / kAtOnce; ++h) {
+                    const int64_t m = m1 + h * kAtOnce + lane / kPieces;
+                    Y raw[kEach];
+                    __builtin_memcpy(raw, &u[h], 16);
+                    if (m < p.a.rows && n + kEach <= p.a.cols) {
+                        __builtin_memcpy(y + m * p.a.cols + n, raw, 16);
+                    } else if (m < p.a.rows) {
+#pragma unroll
+                        for (int t = 0; t < kEach; ++t)
+                            if (n + t < p.a.cols) y[m * p.a.cols + n + t] = raw[t];
+                    }
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    };
+    const auto scaled = [&](auto one, int i, int j, int r) { return (float)one * scales.x[i] * scales.w[j][r]; };
+    if (p.a.partial)
+        finish(p.a.partial + (int64_t)p.split * p.a.rows * p.a.cols, [&](auto one, int, int, int) { return __builtin_bit_cast(uint32_t, one); });
+    else if (p.a.dtype == GEO_SC_F32) finish((f32*)p.a.y, scaled);
+    else if (p.a.dtype == GEO_SC_BF16) finish((bf16*)p.a.y, [&](auto one, int i, int j, int r) { return (bf16)scaled(one, i, j, r); });
+    else finish((f16*)p.a.y, [&](auto one, int i, int j, int r) { return (f16)scaled(one, i, j, r); });
+}
+
+// Rows that start at multiples of 16 bytes, and four whole stages of every split.  The loads write LDS themselves, into a ring of
+// kRing stages: while a wave multiplies stage s out of registers, stage s + 1 moves from LDS to its other registers and the stages
+// up to s + kRing are on their way.  One barrier per stage: it says that every wave's share of stage s + 1 has come and
+// that all have read stage s, whose place stage s + kRing takes.
+template <int B, bool INT8>
+__global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)
+{
+    typedef Tiling<B, INT8> G;
+    constexpr int T = G::T, L = G::L;
     // (arrays of their own, not one: the compiler keeps reads of one apart from loads into another)
-    constexpr int kBytes = (BM + BN) * kStage;
-    __shared__ __align__(16) uint8_t ring0[kBytes], ring1[kBytes], ring2[kBytes], ring3[kBytes];
+    __shared__ __align__(16) uint8_t ring0[G::kBytes], ring1[G::kBytes], ring2[G::kBytes], ring3[G::kBytes];
+    __shared__ __align__(16) uint8_t areas[kWaves][G::kArea];
     const auto place = [&](auto which) -> uint8_t* {
         constexpr int r = decltype(which)::value % kRing;
         if constexpr (r == 0) return ring0;
@@ -171,247 +375,148 @@ __global__ __launch_bounds__(WM* WN * 64) void k_tiles(TwoProducts both)
         else return ring3;
     };
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const Fragments<B> fragments(wave, lane);
 
-    // Workgroups go to the eight dies in turn: each die takes a contiguous share of the tiles, so that neighbours share its L2,
-    // in strips of eight tiles of rows.
-    const uint32_t all = (uint32_t)a.tiles_m * a.tiles_n, split = group / all, die = group % all & 7;
-    const uint32_t tile = die * (all / 8) + (die < all % 8 ? die : all % 8) + (group % all >> 3);
-    constexpr uint32_t kStrip = 8;
-    const uint32_t strip = tile / (kStrip * a.tiles_n), inside = tile - strip * kStrip * a.tiles_n;
-    const uint32_t height = a.tiles_m - strip * kStrip < kStrip ? a.tiles_m - strip * kStrip : kStrip;
-    const int64_t m0 = (int64_t)(strip * kStrip + inside % height) * BM, n0 = (int64_t)(inside / height) * BN;
-    const int wm = wave % WM, wn = wave / WM;
-
-    const int stages = (int)((a.inner + kStage - 1) / kStage);
-    const int begin = split * a.stages_per_split;
-    const int end = begin + a.stages_per_split < stages ? begin + a.stages_per_split : stages;
-    const int whole = (int)(a.inner / kStage);
-
-    // a wave's loads of a stage: 16 rows each, a lane a piece; rows behind the operand's last are read from its last
-    // row, their outputs are not stored
-    const int piece = (lane & 3) ^ (lane >> 4);
-    const uint8_t *x0 = a.x + m0 * a.x_stride, *w0 = a.w + n0 * a.w_stride;
-    const auto row_of = [&](int64_t first, int64_t rows, int i) {
-        const int64_t r = (int64_t)(i * W + wave) * 16 + (lane >> 2);
-        return first + r < rows ? r : rows - 1 - first;
+    Spot p;
+    int x_off[L], w_off[L];
+    __amdgpu_buffer_rsrc_t xr, wr;
+    int xk, wk, x_begin, x_end, w_begin, w_end;   // bytes of the inner dimension: next to load; where its turn ends and goes on
+    const auto load_one = [&](uint8_t* to, int i) {
+        if (i < L) load_to_lds(xr, to + (i * kWaves + wave) * 1024, x_off[i], xk);
+        else load_to_lds(wr, to + (i * kWaves + wave) * 1024, w_off[i - L], wk);
     };
-    const auto w_stage = [&](int k) {   // (at most three terms)
-        if (k >= a.w_stages) k -= a.w_stages;
-        return k >= a.w_stages ? k - a.w_stages : k;
+    const auto advance = [&]() {
+        xk += kStage;
+        wk += kStage;
+        wk = xk == x_end ? w_begin : wk == w_end ? 0 : wk;
+        xk = xk == x_end ? x_begin : xk;
     };
-    // the same through registers: any alignment, zeros behind the end of a row
-    const auto fetch = [&](v4i(&v)[LX + LW], int k) {
-        const int64_t xk = (int64_t)k * kStage + piece * 16, wk = (int64_t)w_stage(k) * kStage + piece * 16;
+    const auto load = [&](uint8_t* to) {
 #pragma unroll
-        for (int i = 0; i < LX; ++i) v[i] = load_piece(x0 + row_of(m0, a.rows, i) * a.x_stride, xk, a.inner);
-#pragma unroll
-        for (int i = 0; i < LW; ++i) v[LX + i] = load_piece(w0 + row_of(n0, a.cols, i) * a.w_stride, wk, a.inner);
+        for (int i = 0; i < 2 * L; ++i) load_one(to, i);
+        advance();
     };
-    const auto put = [&](uint8_t* to, const v4i(&v)[LX + LW]) {
+    const auto start = [&](uint32_t work) {
+        p = spot_of<B>(both, work);
 #pragma unroll
-        for (int i = 0; i < LX; ++i) *(v4i*)(to + (i * W + wave) * 1024 + lane * 16) = v[i];
-#pragma unroll
-        for (int i = 0; i < LW; ++i) *(v4i*)(to + BM * kStage + (i * W + wave) * 1024 + lane * 16) = v[LX + i];
-    };
-    Sum sum[TN][TM];
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-#pragma unroll
-        for (int i = 0; i < TM; ++i) sum[j][i] = Sum{0, 0, 0, 0};
-    const int mine = (lane & 15) * kStage + (((lane >> 4) ^ (lane >> 2 & 3)) << 4);
-    const int mine_x = wm * TM * 16 * kStage + mine, mine_w = (BM + wn * TN * 16) * kStage + mine;
-    // fragments: TN of w, then TM of x
-    const auto read_one = [&](v4i(&f)[TM + TN], const uint8_t* from, int t) {
-        f[t] = *(const v4i*)(from + (t < TN ? mine_w + t * 16 * kStage : mine_x + (t - TN) * 16 * kStage));
-    };
-    const auto read = [&](v4i(&f)[TM + TN], const uint8_t* from) {
-#pragma unroll
-        for (int t = 0; t < TM + TN; ++t) read_one(f, from, t);
-    };
-    const auto multiply_one = [&](const v4i(&f)[TM + TN], int t) { Matrix<INT8>::add_in_place(f[t / TM], f[TN + t % TM], sum[t / TM][t % TM]); };
-    const auto multiply = [&](const v4i(&f)[TM + TN]) {
-#pragma unroll
-        for (int t = 0; t < TM * TN; ++t) multiply_one(f, t);
-    };
-    const int stop = DIRECT && end > whole ? whole : end;   // a last stage that is not whole comes by itself
-    if constexpr (DIRECT) {
-        int x_off[LX], w_off[LW];
-#pragma unroll
-        for (int i = 0; i < LX; ++i) x_off[i] = (int)(row_of(m0, a.rows, i) * a.x_stride) + piece * 16;
-#pragma unroll
-        for (int i = 0; i < LW; ++i) w_off[i] = (int)(row_of(n0, a.cols, i) * a.w_stride) + piece * 16;
-        const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(x0), 0, 0x7fffffff, 0x00020000);
-        const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(w0), 0, 0x7fffffff, 0x00020000);
-        const auto load_one = [&](uint8_t* to, int xk, int wk, int i) {
-            if (i < LX) load_to_lds(xr, to + (i * W + wave) * 1024, x_off[i], xk);
-            else load_to_lds(wr, to + BM * kStage + ((i - LX) * W + wave) * 1024, w_off[i - LX], wk);
-        };
-        // the stage after the next `flying` ones has come, for all waves, and all have what they read before
-        const auto arrive = [&](auto flying) {
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(flying)::value * (LX + LW)) : "memory");
-        };
+        for (int i = 0; i < L; ++i) {
+            x_off[i] = (int)(load_row(p.m0, p.a.rows, i, wave, lane) * p.a.x_stride) + load_piece_of(lane) * 16;
+            w_off[i] = (int)(load_row(p.n0, p.a.cols, i, wave, lane) * p.a.w_stride) + load_piece_of(lane) * 16;
+        }
+        xr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a.x + p.m0 * p.a.x_stride), 0, 0x7fffffff, 0x00020000);
+        wr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p.a.w + p.n0 * p.a.w_stride), 0, 0x7fffffff, 0x00020000);
         // Each die starts at a place of its own in the inner dimension: all at once at the same columns of power-of-two strides
-        // meet in the same channels of the memory.
-        const int turn = stop > begin ? (int)((int64_t)(stop - begin) * die / 8) : 0;
-        const auto turned = [&](int k) { return k + turn < stop ? k + turn : k + turn - (stop - begin); };
-        const auto load = [&](uint8_t* to, int k) {
-            const int kk = turned(k), xk = kk * kStage, wk = w_stage(kk) * kStage;
-#pragma unroll
-            for (int i = 0; i < LX + LW; ++i) load_one(to, xk, wk, i);
-        };
-        v4i f[2][TM + TN];
-        if (begin < stop) {
-            load(ring0, begin);
-            if (begin + 1 < stop) load(ring1, begin + 1);
-            if (begin + 2 < stop) load(ring2, begin + 2);
-            if (begin + 3 < stop) load(ring3, begin + 3);
-            if (begin + kRing <= stop) arrive(Int<kRing - 1>());
-            else arrive(Int<0>());
-            read(f[0], ring0);
-        }
-        // Multiplies stage k, which is in f[which & 1]; `steady`: at least kRing stages follow.  There the next stage's reads and
-        // the loads stand between the products: a wave issues in order, and products behind a queue of loads would wait for it.
-        constexpr int kReads = TM + TN, kLoads = LX + LW, kProducts = TM * TN, kPer = kProducts / (kReads + kLoads);
-        const auto stage = [&](auto which, int k, auto steady) {
-            constexpr int r = decltype(which)::value;
-            constexpr bool kSteady = decltype(steady)::value;
-            if (kSteady || k + kRing <= stop) arrive(Int<kRing - 2>());
-            else if (k + kRing - 1 <= stop) arrive(Int<kRing - 3>());
-            else arrive(Int<0>());
-            const int kk = turned(k + kRing), xk = kk * kStage, wk = w_stage(kk) * kStage;
-            if (!kSteady && k + kRing < stop) load(place(which), k + kRing);
-#pragma unroll
-            for (int t = 0; t < kReads + kLoads; ++t) {
-                // (behind the last stage the reads bring what nobody uses)
-                if (t < kReads) read_one(f[(r + 1) & 1], place(Int<r + 1>()), t);
-                else if constexpr (kSteady) load_one(place(which), xk, wk, t - kReads);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int u = 0; u < kPer; ++u) multiply_one(f[r & 1], t * kPer + u);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int t = (kReads + kLoads) * kPer; t < kProducts; ++t) multiply_one(f[r & 1], t);
-            __builtin_amdgcn_sched_barrier(0);
-        };
-        int k = begin;
-        for (; k + 2 * kRing <= stop; k += kRing) {
-            stage(Int<0>(), k, std::true_type());
-            stage(Int<1>(), k + 1, std::true_type());
-            stage(Int<2>(), k + 2, std::true_type());
-            stage(Int<3>(), k + 3, std::true_type());
-        }
-        for (; k < stop; k += kRing) {
-            stage(Int<0>(), k, std::false_type());
-            if (k + 1 < stop) stage(Int<1>(), k + 1, std::false_type());
-            if (k + 2 < stop) stage(Int<2>(), k + 2, std::false_type());
-            if (k + 3 < stop) stage(Int<3>(), k + 3, std::false_type());
-        }
-        if (stop < end) {
-            v4i v[LX + LW];
-            fetch(v, stop);
-            __syncthreads();
-            put(ring0, v);
-            __syncthreads();
-            read(f[0], ring0);
-            multiply(f[0]);
-        }
-    } else {
-        v4i v[LX + LW], f[TM + TN];
-        fetch(v, begin);
-        put(ring0, v);
-        __syncthreads();
-        uint8_t *now = ring0, *next = ring1;
-        for (int k = begin; k < stop; ++k) {
-            if (k + 1 < stop) fetch(v, k + 1);
-            read(f, now);
-            multiply(f);
-            if (k + 1 < stop) put(next, v);
-            __syncthreads();
-            uint8_t* t = now;
-            now = next;
-            next = t;
-        }
-    }
+        // meet in the same channels of the memory (the loads alone of 8192 x 16384 x 4096: 340 us, so 282).
+        const int first = p.begin + (int)((int64_t)(p.stop - p.begin) * p.die / 8);
+        x_begin = p.begin * kStage;
+        x_end = p.stop * kStage;
+        w_begin = w_stage(p.a, p.begin) * kStage;
+        w_end = p.a.w_stages < 0x7fffffff / kStage ? p.a.w_stages * kStage : -1;
+        xk = first * kStage;
+        wk = w_stage(p.a, first) * kStage;
+        load(ring0);
+        load(ring1);
+        load(ring2);
+        load(ring3);
+    };
+    // All but the newest `flying` loads of a wave have come, for all waves, and all have what they read before.
+    const auto arrive = [&](auto flying) { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(decltype(flying)::value) : "memory"); };
 
-    // Out through LDS, 64 rows of a wave at a time, each wave in a place of the ring: a lane holds four columns of one row, the
-    // lanes that share a row store 16 bytes each and fill its lines.  Positions of the 16-byte pieces ^ row: no two lanes
-    // of a quarter wave meet in a bank.
-    constexpr int kBatch = TM < 4 ? TM : 4;
-    static_assert(kBytes >= 16 * kBatch * TN * 64 && W == kRing && TM % kBatch == 0, "a stage holds a wave's rows");
-    float ws[TN][4], xs[TM];   // (all asked for at once: each row's by itself would be waited for by itself)
+    typename G::Sum sum[T][T];
+    v4i f[2][2 * T];
+    // Multiplies stage k, which is in f[which & 1]; `steady`: at least kRing stages follow.  Everything else stands between the
+    // products, little at a time: a wave issues in order, one instruction in four cycles, and a product takes sixteen.  The
+    // next stage's reads in the first half, the loads over all of it, their next place in the second.
+    constexpr int kLoads = 2 * L, kProducts = T * T, kPer = kProducts / kLoads;
+    const auto stage = [&](auto which, int k, auto steady) {
+        constexpr int r = decltype(which)::value;
+        constexpr bool kSteady = decltype(steady)::value;
+        if (kSteady || k + kRing <= p.stop) arrive(Int<(kRing - 2) * kLoads>());
+        else if (k + kRing - 1 <= p.stop) arrive(Int<(kRing - 3) * kLoads>());
+        else arrive(Int<0>());
+        if (!kSteady && k + kRing < p.stop) load(place(which));
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < TN; ++j)
+        for (int u = 0; u < kProducts; ++u) {
+            multiply_one<INT8, T>(f[r & 1], sum, u);
+            __builtin_amdgcn_sched_barrier(0);
+            // (behind the last stage the reads bring what nobody uses)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) ws[j][r] = 1.f;
-#pragma unroll
-    for (int i = 0; i < TM; ++i) xs[i] = 1.f;
-    if (a.w_scale)
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t n = n0 + (wn * TN + j) * 16 + (lane >> 4) * 4 + r;
-                ws[j][r] = a.w_scale[n < a.cols ? n : a.cols - 1];
+            for (int t = 0; t < 2 * T; ++t)
+                if (t * kProducts / (4 * T) == u) fragments.read_one(f[(r + 1) & 1], place(Int<r + 1>()), t);
+            if constexpr (kSteady) {
+                if (u % kPer == kPer / 2) load_one(place(which), u / kPer);
+                if (u == kProducts - 1) advance();
             }
-    if (a.x_scale)
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int64_t m = m0 + (wm * TM + i) * 16 + (lane & 15);
-            xs[i] = a.x_scale[m < a.rows ? m : a.rows - 1];
-        }
-    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");   // the last products' sums are in their registers
-    __syncthreads();
-    uint8_t* area = wave == 0 ? ring0 : wave == 1 ? ring1 : wave == 2 ? ring2 : ring3;
-    const bool fits = m0 + BM <= a.rows && n0 + BN <= a.cols;
-    const auto finish = [&](auto* y, auto value) {
-        using T = std::remove_pointer_t<decltype(y)>;
-        constexpr int kEach = 16 / (int)sizeof(T), kPieces = TN * 16 / kEach, kAtOnce = 64 / kPieces;   // elements, pieces of a row, rows of a store
-        constexpr int kMix = (kPieces < 16 ? kPieces : 16) - 1;
-        const int row = lane & 15, column = (lane >> 4) * 4;
-#pragma unroll
-        for (int half = 0; half < TM / kBatch; ++half) {
-#pragma unroll
-            for (int i = 0; i < kBatch; ++i)
-#pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    Sum s = sum[j][half * kBatch + i];
-                    asm volatile("" : "+v"(s));   // (here, and not for all types at once before the choice of one)
-                    T four[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) four[r] = value(s[r], half * kBatch + i, j, r);
-                    const int at = j * 16 + column, where = (i * 16 + row) * kPieces + ((at / kEach) ^ (row & kMix));
-                    __builtin_memcpy(area + where * 16 + at % kEach * sizeof(T), four, sizeof four);
-                }
-            __builtin_amdgcn_wave_barrier();
-            const int64_t m1 = m0 + (wm * TM + half * kBatch) * 16, n = n0 + wn * TN * 16 + lane % kPieces * kEach;
-#pragma unroll 4
-            for (int h = 0; h < 16 * kBatch; h += kAtOnce) {
-                const int r = h + lane / kPieces;
-                const v4i u = *(const v4i*)(area + (r * kPieces + (lane % kPieces ^ (r & kMix))) * 16);
-                T* to = y + (m1 + r) * a.cols + n;
-                if (fits) {
-                    __builtin_memcpy(to, &u, 16);
-                } else if (m1 + r < a.rows && n < a.cols) {
-                    if (n + kEach <= a.cols) {
-                        __builtin_memcpy(to, &u, 16);
-                    } else {
-                        T raw[kEach];
-                        __builtin_memcpy(raw, &u, 16);
-#pragma unroll
-                        for (int t = 0; t < kEach; ++t)
-                            if (n + t < a.cols) to[t] = raw[t];
-                    }
-                }
-            }
-            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
-    const auto scaled = [&](auto one, int i, int j, int r) { return (float)one * xs[i] * ws[j][r]; };
-    if (a.partial) finish(a.partial + (int64_t)split * a.rows * a.cols, [&](auto one, int, int, int) { return __builtin_bit_cast(uint32_t, one); });
-    else if (a.dtype == GEO_SC_F32) finish((f32*)a.y, scaled);
-    else if (a.dtype == GEO_SC_BF16) finish((bf16*)a.y, [&](auto one, int i, int j, int r) { return (bf16)scaled(one, i, j, r); });
-    else finish((f16*)a.y, [&](auto one, int i, int j, int r) { return (f16)scaled(one, i, j, r); });
+    start(blockIdx.x);
+#pragma unroll
+    for (int j = 0; j < T; ++j)
+#pragma unroll
+        for (int i = 0; i < T; ++i) sum[j][i] = typename G::Sum{0, 0, 0, 0};
+    arrive(Int<(kRing - 1) * kLoads>());
+    fragments.read(f[0], ring0);
+    int k = p.begin;
+    for (; k + 2 * kRing <= p.stop; k += kRing) {
+        stage(Int<0>(), k, std::true_type());
+        stage(Int<1>(), k + 1, std::true_type());
+        stage(Int<2>(), k + 2, std::true_type());
+        stage(Int<3>(), k + 3, std::true_type());
+    }
+    for (; k < p.stop; k += kRing) {
+        stage(Int<0>(), k, std::false_type());
+        if (k + 1 < p.stop) stage(Int<1>(), k + 1, std::false_type());
+        if (k + 2 < p.stop) stage(Int<2>(), k + 2, std::false_type());
+        if (k + 3 < p.stop) stage(Int<3>(), k + 3, std::false_type());
+    }
+    TileScales<T> scales;
+    scales.load(p, wave, lane);
+    if (p.stop < p.end) {   // a last stage that is not whole
+        v4i v[2 * L];
+        fetch_stage<L>(p, p.stop, wave, lane, v);
+        __syncthreads();
+        put_stage<L>(ring0, wave, lane, v);
+        __syncthreads();
+        fragments.read(f[0], ring0);
+        multiply<INT8, T>(f[0], sum);
+    }
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");   // the last products' sums are in their registers
+    finish_tile<B, INT8>(p, sum, scales, areas[wave], wave, lane);
+}
+
+// Any rows: stages through registers, the next one on its way while one is multiplied.
+template <int B, bool INT8>
+__global__ __launch_bounds__(kWaves * 64) void k_tiles_any(TwoProducts both)
+{
+    typedef Tiling<B, INT8> G;
+    constexpr int T = G::T, L = G::L;
+    __shared__ __align__(16) uint8_t buffers[2][G::kBytes];
+    __shared__ __align__(16) uint8_t areas[kWaves][G::kArea];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const Fragments<B> fragments(wave, lane);
+    const Spot p = spot_of<B>(both, blockIdx.x);
+    typename G::Sum sum[T][T];
+#pragma unroll
+    for (int j = 0; j < T; ++j)
+#pragma unroll
+        for (int i = 0; i < T; ++i) sum[j][i] = typename G::Sum{0, 0, 0, 0};
+    v4i v[2 * L], f[2 * T];
+    fetch_stage<L>(p, p.begin, wave, lane, v);
+    put_stage<L>(buffers[0], wave, lane, v);
+    __syncthreads();
+    for (int k = p.begin; k < p.end; ++k) {
+        if (k + 1 < p.end) fetch_stage<L>(p, k + 1, wave, lane, v);
+        fragments.read(f, buffers[(k - p.begin) & 1]);
+        multiply<INT8, T>(f, sum);
+        if (k + 1 < p.end) put_stage<L>(buffers[(k - p.begin + 1) & 1], wave, lane, v);
+        __syncthreads();
+    }
+    TileScales<T> scales;
+    scales.load(p, wave, lane);
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");   // the last products' sums are in their registers
+    finish_tile<B, INT8>(p, sum, scales, areas[wave], wave, lane);
 }
 
 // Few rows of x (at most 16 MT): y is bound by the one read of w.  A wave reads 128 bytes of 16 NT rows of w per step, 32 per lane,
@@ -551,8 +656,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a)
     const int tiles = (int)((a.cols + 15) / 16), my_tiles = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     const int total = each * my_tiles;
 
-    // loads: 16 rows of 64 bytes, a lane a piece; the pieces of rows r lie at positions piece ^ (r / 4 & 3)
-    const int piece = ((lane & 3) ^ (lane >> 4)) * 16, load_row = lane >> 2;
+    // loads: 16 rows of 64 bytes, a lane a piece; the pieces of rows r lie at positions piece ^ (r / 4 & 2)
+    const int piece = ((lane & 3) ^ (lane >> 4 & 2)) * 16, load_row = lane >> 2;
     int x_off[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -577,7 +682,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a)
     v4i sum[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) sum[i] = v4i{0, 0, 0, 0};
-    const int mine = (lane & 15) * kStage + (((lane >> 4) ^ (lane >> 2 & 3)) << 4);
+    const int mine = (lane & 15) * kStage + (((lane >> 4) ^ (lane >> 2 & 2)) << 4);
     const auto multiply = [&](const uint8_t* from) {
         const v4i w = *(const v4i*)(from + mine);
 #pragma unroll
@@ -761,9 +866,9 @@ void run_tiles(TwoProducts both, bool direct, hipStream_t s)
         return (uint32_t)a.tiles_m * a.tiles_n * a.splits;
     };
     both.second_at = groups(both.first);
-    const dim3 grid(both.second_at + (both.second.rows ? groups(both.second) : 0));
-    if (direct) k_tiles<B, B, 2, 2, INT8, true><<<grid, dim3(256), 0, s>>>(both);
-    else k_tiles<B, B, 2, 2, INT8, false><<<grid, dim3(256), 0, s>>>(both);
+    const uint32_t works = both.second_at + (both.second.rows ? groups(both.second) : 0);
+    if (direct) k_tiles<B, INT8><<<dim3(works), dim3(kWaves * 64), 0, s>>>(both);
+    else k_tiles_any<B, INT8><<<dim3(works), dim3(kWaves * 64), 0, s>>>(both);
 }
 
 // Runs one product, or two in one launch (second.rows 0: one).  The caller has made the plan and the partial sums' memory.
@@ -780,7 +885,10 @@ int run_products(TwoProducts both, const Plan& p, hipStream_t s)
         else if (p.few == 3) run_few<3>(both.first, s);
         else run_few<4>(both.first, s);
     } else {
-        const auto fits = [&](const TileArgs& a) { return loads_fit(a.x, a.x_stride, p.tile, a.inner) && loads_fit(a.w, a.w_stride, p.tile, a.inner); };
+        const auto fits = [&](const TileArgs& a) {
+            const int64_t last = a.inner / kStage - (int64_t)(a.splits - 1) * a.stages_per_split;   // whole stages of the last split
+            return last >= kRing && loads_fit(a.x, a.x_stride, p.tile, a.inner) && loads_fit(a.w, a.w_stride, p.tile, a.inner);
+        };
         const bool direct = fits(both.first) && (!both.second.rows || fits(both.second));
         if (p.tile == 256) run_tiles<256, INT8>(both, direct, s);
         else if (p.tile == 128) run_tiles<128, INT8>(both, direct, s);
