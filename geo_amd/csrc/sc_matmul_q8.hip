@@ -807,32 +807,67 @@ struct Plan {
     int splits[2], stages_per_split[2];
 };
 
-void cut(Plan* p, int which, const Shape& s, int64_t groups, int64_t least)
+// Cuts a product's inner dimension into about `splits`, none of fewer than `least` steps, the last of three at least.
+void cut(Plan* p, int which, const Shape& s, int64_t splits, int64_t least)
 {
     const int64_t steps = s.steps();
-    int64_t splits = groups < kUnits ? kUnits / groups : 1;
     if (splits > steps / least) splits = steps / least;
     if (splits > 64) splits = 64;
-    if (splits < 1) splits = 1;
-    const int64_t per_split = (steps + splits - 1) / splits;
+    if (splits < 1 || s.rows * ((s.cols + 3) / 4) > 0x7fffffff) splits = 1;   // (the join counts in 32 bits)
+    int64_t per_split = (steps + splits - 1) / splits;
+    while (per_split < steps && steps - (steps - 1) / per_split * per_split < 3) ++per_split;
     p->stages_per_split[which] = (int)(2 * per_split);
     p->splits[which] = (int)((steps + per_split - 1) / per_split);
 }
 
+// What a tile costs, us, measured: `stage` of a stage where a compute unit has as many workgroups as it holds (and each of them
+// alone no less than `alone`), `rest` of everything else.  int8 and bf16 are within a tenth of each other.
+struct TileCost {
+    int tile, held;
+    double stage, alone, rest;
+};
+constexpr TileCost kTileCosts[] = {{256, 1, .60, .56, 10}, {128, 2, .26, .24, 4}, {64, 4, .115, .08, 3}};
+constexpr int64_t kLeastSteps = 8;
+
+// The tile, and the splits of either product, of the least time by that table: what all compute units do together or what the
+// longest workgroup does, whichever is more, and the join of the splits.  Of 4096 x 4096 x 4096 tiles of 256 take 57 us, of 128 75, of
+// 64 122; of 1009 x 1003 x 1111 29, 11 and 6; the fp32 gradients of 1024 x 4096 x 1024 by 128 take 133 us, cut 93.
 Plan plan_of(const Shape& s, const Shape& t, bool int8)
 {
-    Plan p = {};
+    Plan best = {};
     if (int8 && s.rows <= 64) {
-        p.few = (int)((s.rows + 15) / 16);
+        best.few = (int)((s.rows + 15) / 16);
         // (a split and its join cost 3 us, in which a workgroup goes through 16 KB of its rows)
-        cut(&p, 0, s, (s.cols + 15) / 16, 128);
-        return p;
+        const int64_t groups = (s.cols + 15) / 16;
+        cut(&best, 0, s, groups < kUnits ? kUnits / groups : 1, 128);
+        return best;
     }
-    const auto tiles = [&](int64_t b) { return s.tiles(b) + (t.rows ? t.tiles(b) : 0); };
-    p.tile = tiles(256) >= kUnits * 3 / 4 ? 256 : tiles(128) >= kUnits ? 128 : 64;
-    cut(&p, 0, s, tiles(p.tile), 8);
-    if (t.rows) cut(&p, 1, t, tiles(p.tile), 8);
-    return p;
+    const Shape shapes[2] = {s, t};
+    const int count = t.rows ? 2 : 1;
+    double least = 0;
+    for (const TileCost& c : kTileCosts) {
+        double work = 0;
+        for (int i = 0; i < count; ++i) work += (double)shapes[i].tiles(c.tile) * 2 * shapes[i].steps();
+        const double together = c.stage * work / kUnits;
+        for (int is_cut = 0; is_cut < 2; ++is_cut) {
+            Plan p = {};
+            p.tile = c.tile;
+            double groups = 0, longest = 0, join = 0;
+            for (int i = 0; i < count; ++i) {
+                cut(&p, i, shapes[i], is_cut ? (int64_t)(2 * shapes[i].steps() * c.alone / together) + 1 : 1, kLeastSteps);
+                groups += (double)shapes[i].tiles(c.tile) * p.splits[i];
+                if (p.stages_per_split[i] * c.alone > longest) longest = p.stages_per_split[i] * c.alone;
+                if (p.splits[i] > 1) join += 8e-6 / 4 * p.splits[i] * shapes[i].rows * shapes[i].cols;
+            }
+            const double rounds = (double)((int64_t)groups / (kUnits * c.held) + 1);
+            const double time = (together > longest ? together : longest) + c.rest * rounds + (join > 0 ? 4 + join : 0);
+            if (!best.tile || time < least) {
+                best = p;
+                least = time;
+            }
+        }
+    }
+    return best;
 }
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
