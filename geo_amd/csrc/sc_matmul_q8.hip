@@ -76,6 +76,9 @@ template <>
 struct Matrix<true> {
     typedef v4i Sum;
     static __device__ __forceinline__ void add(const v4i& a, const v4i& b, Sum& s) { s = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, s, 0, 0, 0); }
+    // The same on sums that stay in their accumulation registers: of the builtin's, with as many registers as the tiles need, the
+    // compiler copied three for every product (8192 x 16384 x 4096: 750 us, so 565).  It keeps no distance from these products: what
+    // else reads the sums comes behind settle(), and a test follows the built code for what comes between.
     static __device__ __forceinline__ void add_in_place(const v4i& a, const v4i& b, Sum& s)
     {
         asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(s) : "v"(a), "v"(b));
@@ -243,16 +246,31 @@ struct Fragments {
         for (int t = 0; t < 2 * T; ++t) read_one(f, from, t);
     }
 };
-template <bool INT8, int T>
+// kInPlace: see Matrix::add_in_place
+template <bool INT8, bool kInPlace, int T>
 __device__ __forceinline__ void multiply_one(const v4i (&f)[2 * T], typename Matrix<INT8>::Sum (&sum)[T][T], int t)
 {
-    Matrix<INT8>::add_in_place(f[t / T], f[T + t % T], sum[t / T][t % T]);
+    if constexpr (kInPlace) Matrix<INT8>::add_in_place(f[t / T], f[T + t % T], sum[t / T][t % T]);
+    else Matrix<INT8>::add(f[t / T], f[T + t % T], sum[t / T][t % T]);
 }
-template <bool INT8, int T>
+template <bool INT8, bool kInPlace, int T>
 __device__ __forceinline__ void multiply(const v4i (&f)[2 * T], typename Matrix<INT8>::Sum (&sum)[T][T])
 {
 #pragma unroll
-    for (int t = 0; t < T * T; ++t) multiply_one<INT8, T>(f, sum, t);
+    for (int t = 0; t < T * T; ++t) multiply_one<INT8, kInPlace, T>(f, sum, t);
+}
+
+// The last products' sums are in their registers.  The compiler does not know the products for what they are and keeps no
+// distance; every sum passes through a statement behind the wait, so that no read of one can come before it.
+template <int T, typename Sum>
+__device__ __forceinline__ void settle(Sum (&sum)[T][T])
+{
+    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < T; ++j)
+#pragma unroll
+        for (int i = 0; i < T; i += 2) asm volatile("" : "+a"(sum[j][i]), "+a"(sum[j][i + 1]));
 }
 
 // The scales of a wave's rows and columns, all asked for at once: each by itself would be waited for by itself.
@@ -438,7 +456,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < kProducts; ++u) {
-            multiply_one<INT8, T>(f[r & 1], sum, u);
+            multiply_one<INT8, true, T>(f[r & 1], sum, u);
             __builtin_amdgcn_sched_barrier(0);
             // (behind the last stage the reads bring what nobody uses)
 #pragma unroll
@@ -480,9 +498,9 @@ __global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)
         put_stage<L>(ring0, wave, lane, v);
         __syncthreads();
         fragments.read(f[0], ring0);
-        multiply<INT8, T>(f[0], sum);
+        multiply<INT8, true, T>(f[0], sum);
     }
-    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");   // the last products' sums are in their registers
+    settle(sum);
     finish_tile<B, INT8>(p, sum, scales, areas[wave], wave, lane);
 }
 
@@ -509,13 +527,12 @@ __global__ __launch_bounds__(kWaves * 64) void k_tiles_any(TwoProducts both)
     for (int k = p.begin; k < p.end; ++k) {
         if (k + 1 < p.end) fetch_stage<L>(p, k + 1, wave, lane, v);
         fragments.read(f, buffers[(k - p.begin) & 1]);
-        multiply<INT8, T>(f, sum);
+        multiply<INT8, false, T>(f, sum);
         if (k + 1 < p.end) put_stage<L>(buffers[(k - p.begin + 1) & 1], wave, lane, v);
         __syncthreads();
     }
     TileScales<T> scales;
     scales.load(p, wave, lane);
-    asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");   // the last products' sums are in their registers
     finish_tile<B, INT8>(p, sum, scales, areas[wave], wave, lane);
 }
 

@@ -392,6 +392,46 @@ def test_same_results_on_every_run(uf):
         assert all(torch.equal(a, b) for a, b in zip(first, run()))
 
 
+def test_no_rows(uf):
+    x, w = torch.empty(0, 24, device="cuda", requires_grad=True), rand(10, 24).requires_grad_(True)
+    gain = torch.ones(24, device="cuda", requires_grad=True)
+    q, s, values = uf.quantize_rows(x.detach(), values=torch.bfloat16)
+    assert q.shape == (0, 24) and s.shape == (0,) and values.shape == (0, 24)
+    y = uf.linear_q8(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.empty(0, 10, device="cuda"))
+    assert y.shape == (0, 10) and dx.shape == (0, 24) and (dw == 0).all()
+    _, _, total, values = uf.rms_norm_q8(x, gain, residual=x.detach(), values=torch.float32)
+    dx, dgain = torch.autograd.grad(values, (x, gain), torch.empty(0, 24, device="cuda"))
+    assert dx.shape == (0, 24) and (dgain == 0).all()
+    y, total = uf.norm_linear_q8(x, gain, w, residual=x.detach())
+    assert y.shape == (0, 10) and total.shape == (0, 24)
+
+
+def test_offsets_beyond_32_bits(uf):
+    """matrices of more than 2^32 bytes (and 2^31 elements): their last rows against the same rows by themselves"""
+    rows, cols = 70001, 33000
+    x = torch.randn(rows, 1, generator=torch.Generator().manual_seed(1)).cuda().bfloat16() * torch.linspace(-1, 1, cols, device="cuda").bfloat16()
+    w = torch.ones(cols, dtype=torch.bfloat16, device="cuda")
+    last = x[-3:].clone()
+    q, s, values = uf.quantize_rows(x, values=torch.bfloat16)
+    want = uf.quantize_rows(last, values=torch.bfloat16)
+    assert torch.equal(q[-3:], want[0]) and torch.equal(s[-3:], want[1]) and torch.equal(values[-3:], want[2])
+    del q, values
+    q, s, total, _ = uf.rms_norm_q8(x, w, residual=x)
+    want = uf.rms_norm_q8(last, w, residual=last)
+    assert torch.equal(q[-3:], want[0]) and torch.equal(s[-3:], want[1]) and torch.equal(total[-3:], want[2])
+    del total
+    wq, ws = random_q8(40, cols, 5)
+    y = uf.matmul_q8(q, s, wq, ws)                       # a left operand of more than 2^31 bytes
+    want = product64(q[-3:], s[-3:], wq, ws)
+    close(y[-3:], want, 5 * U * want.abs())
+    del q, x, y
+    (q, s), (wq, ws) = random_q8(rows, 64, 6), random_q8(cols, 64, 7)
+    y = uf.matmul_q8(q, s, wq, ws, dtype=torch.bfloat16)  # a result of more than 2^31 elements
+    want = product64(q[-3:], s[-3:], wq, ws)
+    close(y[-3:], want, (EPS[torch.bfloat16] + 4 * U) * want.abs())
+
+
 def test_refusals(uf):
     x, w = rand(4, 16), rand(8, 16)
     q, s, _ = uf.quantize_rows(x)

@@ -153,6 +153,25 @@ def test_gradient_against_differences_of_the_loss(uf):
         assert ((up - down) / (2 * step) - dz[:, c].double()).abs().max() < 1e-3
 
 
+def test_many_entries_and_large_logits(uf):
+    """as many entries as there may be, most of them repeated or absent; logits of more than 2^32 bytes, by their last rows"""
+    z, _, _ = inputs(5, 600, 1, torch.float32, seed=8)
+    g = torch.Generator().manual_seed(9)
+    check(uf, z, torch.randn(5, 4096, generator=g).cuda(), torch.randint(-50, 650, (5, 4096), generator=g).cuda(), 1.5)
+    rows, cols = 33001, 70001
+    z = torch.randn(rows, 1, generator=g).cuda().bfloat16() * torch.linspace(-3, 3, cols, device="cuda").bfloat16()
+    t, index = torch.randn(rows, 4, generator=g).cuda(), torch.randint(cols, (rows, 4), generator=g).cuda()
+    z = z.requires_grad_(True)
+    loss = uf.distill_topk(z, t, index, reduction="none")
+    dz, = torch.autograd.grad(loss, z, torch.ones_like(loss))
+    last = z.detach()[-3:].clone().requires_grad_(True)
+    # (three rows alone are cut into shares: other sums, within the bounds of the formula's test)
+    want, want_z = formula(last.detach(), t[-3:], index[-3:], 1.0)
+    assert ((loss[-3:].double() - want).abs() <= (cols / 64 + 128) * 4 * U).all()
+    assert ((dz[-3:].double() - want_z).abs() <= EPS[torch.bfloat16] * want_z.abs() + (cols / 64 + 128) * 4 * U * torch.softmax(last.detach().double(), 1)
+            + SMALL[torch.bfloat16]).all()
+
+
 def test_in_a_graph(uf):
     z, t, index = inputs(40, 9000, 16, torch.bfloat16, seed=7)
     z = z.requires_grad_(True)
