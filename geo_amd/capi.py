@@ -81,6 +81,19 @@ def _stream_ptr(stream=None):
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
+def _fork(stream):
+    """Before a call on a stream of its own: what it allocates, result and scratch, is memory of the current stream, where
+    it may still be in use."""
+    if stream is not None:
+        stream.wait_stream(torch.cuda.current_stream())
+
+
+def _join(stream):
+    """Behind such a call: the current stream hands the scratch out again at once, and reads the result."""
+    if stream is not None:
+        torch.cuda.current_stream().wait_stream(stream)
+
+
 def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
 
@@ -126,10 +139,12 @@ def conv2d_add_partial_forward(x, w, bit_length, padding=(0, 0), total_width=7, 
         workspace = torch.empty(workspace_size(desc, options), dtype=torch.uint8, device=x.device)
     if out is None:
         out = torch.empty(output_shape(desc), dtype=torch.int32, device=x.device)
+    _fork(stream)
     _check(_native.lib().geo_sc_conv2d_add_partial_forward_ex(ctypes.byref(desc), _opt_ptr(options), _ptr(x), _ptr(w),
                                                               _ptr(out), _ptr(workspace), workspace.numel(),
                                                               _stream_ptr(stream)),
            "geo_sc_conv2d_add_partial_forward")
+    _join(stream)
     return out
 
 
@@ -140,10 +155,12 @@ def conv2d_add_partial_values(x, w, desc: ConvDesc, bit_length, stream=None):
     _require_gpu_f32(w, "w")
     workspace = torch.empty(workspace_size(desc), dtype=torch.uint8, device=x.device)
     y = torch.empty(output_shape(desc), dtype=torch.float32, device=x.device)
+    _fork(stream)
     lib, y_ptr, stream_ptr = _native.lib(), _ptr(y), _stream_ptr(stream)
     _check(lib.geo_sc_conv2d_add_partial_forward_ex(ctypes.byref(desc), None, _ptr(x), _ptr(w), y_ptr, _ptr(workspace),
                                                     workspace.numel(), stream_ptr), "geo_sc_conv2d_add_partial_forward")
     _check(lib.geo_sc_counts_to_values(y_ptr, y.numel(), int(bit_length), stream_ptr), "geo_sc_counts_to_values")
+    _join(stream)
     return y
 
 
@@ -188,10 +205,12 @@ def conv2d_add_partial_forward_q7(x_q7, w, bit_length, padding=(0, 0), total_wid
         workspace = torch.empty(workspace_size(desc), dtype=torch.uint8, device=w.device)
     if out is None:
         out = torch.empty(output_shape(desc), dtype=torch.int32, device=w.device)
+    _fork(stream)
     _check(_native.lib().geo_sc_conv2d_add_partial_forward_q7(ctypes.byref(desc), _ptr(x_q7), _ptr(w), _ptr(out),
                                                               _ptr(workspace), workspace.numel(),
                                                               _stream_ptr(stream)),
            "geo_sc_conv2d_add_partial_forward_q7")
+    _join(stream)
     return out
 
 
@@ -216,8 +235,10 @@ def layer_epilogue(counts, bit_length, w_n, b_n, relu=False, pool=True, hardtanh
     shape = (n, c, w // 2, h // 2) if pool else (n, c, w, h)
     act = torch.empty(shape, dtype=torch.float32, device=counts.device) if want_act else None
     q7 = torch.empty(shape, dtype=torch.uint8, device=counts.device) if want_q7 else None
+    _fork(stream)
     _check(_native.lib().geo_sc_layer_epilogue(_ptr(counts), n, c, w, h, int(bit_length), _ptr(w_n), _ptr(b_n), flags,
                                                _ptr(act), _ptr(q7), _stream_ptr(stream)), "geo_sc_layer_epilogue")
+    _join(stream)
     return act, q7
 
 
@@ -240,10 +261,12 @@ def layer_tail_backward(counts, grad_out, bit_length, w_n, b_n, mean, invstd, ga
     grad_y = torch.empty((n, c, w, h), dtype=torch.float32, device=dev)
     gg = torch.empty(c, dtype=torch.float32, device=dev)
     gb = torch.empty(c, dtype=torch.float32, device=dev)
+    _fork(stream)
     _check(_native.lib().geo_sc_layer_tail_backward(_ptr(counts), _ptr(grad_out), n, c, w, h, int(bit_length), _ptr(w_n),
                                                     _ptr(b_n), _ptr(mean), _ptr(invstd), _ptr(gamma), flags,
                                                     _ptr(grad_y), _ptr(gg), _ptr(gb), _ptr(ws), ws.numel(),
                                                     _stream_ptr(stream)), "geo_sc_layer_tail_backward")
+    _join(stream)
     return grad_y, gg, gb
 
 
@@ -260,8 +283,10 @@ def count_stats(counts, bit_length, stream=None):
     ws = torch.empty(max(need.value, 8), dtype=torch.uint8, device=counts.device)
     mean = torch.empty(c, dtype=torch.float32, device=counts.device)
     var = torch.empty(c, dtype=torch.float32, device=counts.device)
+    _fork(stream)
     _check(_native.lib().geo_sc_count_stats(_ptr(counts), n, c, w, h, int(bit_length), _ptr(mean), _ptr(var), _ptr(ws),
                                             ws.numel(), _stream_ptr(stream)), "geo_sc_count_stats")
+    _join(stream)
     return mean, var
 
 
@@ -278,10 +303,12 @@ def bn_fixed_affine(mean, var, gamma, beta, eps, elements_per_channel, running_m
     b_n = torch.empty(c, dtype=torch.float32, device=dev)
     invstd = torch.empty(c, dtype=torch.float32, device=dev)
     scale = torch.empty((), dtype=torch.float32, device=dev)
+    _fork(stream)
     _check(_native.lib().geo_sc_bn_fixed_affine(_ptr(mean), _ptr(var), _ptr(gamma), _ptr(beta), c, float(eps),
                                                 float(eps_grad), int(elements_per_channel), _ptr(running_mean),
                                                 _ptr(running_var), _ptr(w_n), _ptr(b_n), _ptr(invstd), _ptr(scale),
                                                 _stream_ptr(stream)), "geo_sc_bn_fixed_affine")
+    _join(stream)
     return w_n, b_n, invstd, scale
 
 
@@ -305,11 +332,13 @@ def bn_fixed_from_counts(counts, bit_length, gamma, beta, eps, running_mean=None
     out = torch.empty((5, c), dtype=torch.float32, device=dev)   # mean, var, w_n, b_n, invstd
     scale = torch.empty((), dtype=torch.float32, device=dev)
     mean, var, w_n, b_n, invstd = out[0], out[1], out[2], out[3], out[4]
+    _fork(stream)
     _check(_native.lib().geo_sc_bn_fixed_from_counts(_ptr(counts), n, c, w, h, int(bit_length), _ptr(gamma), _ptr(beta),
                                                      float(eps), float(eps_grad), _ptr(running_mean),
                                                      _ptr(running_var), _ptr(mean), _ptr(var), _ptr(w_n), _ptr(b_n),
                                                      _ptr(invstd), _ptr(scale), _ptr(ws), ws.numel(),
                                                      _stream_ptr(stream)), "geo_sc_bn_fixed_from_counts")
+    _join(stream)
     return mean, var, w_n, b_n, invstd, scale
 
 
@@ -321,8 +350,10 @@ def bn_eval_weight(var, gamma, eps, stream=None):
                                   and t.numel() == var.numel()):
             raise ValueError("variance and weight must be contiguous float32 tensors of one size on one GPU")
     w = torch.empty(var.numel(), dtype=torch.float32, device=var.device)
+    _fork(stream)
     _check(_native.lib().geo_sc_bn_eval_weight(_ptr(var), _ptr(gamma), var.numel(), float(eps), _ptr(w), _stream_ptr(stream)),
            "geo_sc_bn_eval_weight")
+    _join(stream)
     return w
 
 
@@ -338,9 +369,11 @@ def bn_fixed_eval(x, mean, var, gamma, beta, eps, w_mean=None, out=None, stream=
             raise ValueError("x, statistics and parameters must be contiguous float32 tensors on one GPU")
     y = torch.empty_like(x) if out is None else out
     scale = torch.empty((), dtype=torch.float32, device=x.device)
+    _fork(stream)
     _check(_native.lib().geo_sc_bn_fixed_eval_mean(_ptr(x), n, c, x.numel() // (n * c), _ptr(mean), _ptr(var), _ptr(gamma),
                                                    _ptr(beta), float(eps), _ptr(w_mean), _ptr(y), _ptr(scale),
                                                    _stream_ptr(stream)), "geo_sc_bn_fixed_eval_mean")
+    _join(stream)
     return y, scale
 
 
@@ -351,12 +384,14 @@ def quantize_many(tensors, prec, stream=None):
         _require_gpu_f32(t, "tensor")
     outs = [torch.empty_like(t) for t in tensors]
     n = len(tensors)
+    _fork(stream)
     if n:
         arr = ctypes.c_void_p * n
         sizes = (ctypes.c_size_t * n)(*[t.numel() for t in tensors])
         _check(_native.lib().geo_sc_quantize_many(n, arr(*[t.data_ptr() for t in tensors]),
                                                   arr(*[o.data_ptr() for o in outs]), sizes, int(prec),
                                                   _stream_ptr(stream)), "geo_sc_quantize_many")
+    _join(stream)
     return outs
 
 
@@ -386,8 +421,10 @@ def quantize(x, prec, out=None, stream=None):
         out = torch.empty_like(x)
     elif not (out.is_cuda and out.dtype == torch.float32 and out.is_contiguous() and out.shape == x.shape):
         raise ValueError("out must be a contiguous fp32 GPU tensor of x's shape")
+    _fork(stream)
     _check(_native.lib().geo_sc_quantize(_ptr(x), _ptr(out), x.numel(), int(prec), _stream_ptr(stream)),
            "geo_sc_quantize")
+    _join(stream)
     return out
 
 
@@ -412,7 +449,9 @@ def act_streams(x, desc: ConvDesc, stream=None):
     out = torch.empty(shape, dtype=torch.int32, device=x.device)
     assert out.numel() == n.value
     fn = _native.lib().geo_sc_act_streams_q7 if q7 else _native.lib().geo_sc_act_streams
+    _fork(stream)
     _check(fn(ctypes.byref(desc), _ptr(x), _ptr(out), None, _stream_ptr(stream)), "geo_sc_act_streams")
+    _join(stream)
     return out
 
 
@@ -430,8 +469,10 @@ def weight_streams(w, desc: ConvDesc, stream=None):
     buf = torch.empty(n.value, dtype=torch.int32, device=w.device)
     assert n.value >= classic
     out = buf[:classic].view(shape)
+    _fork(stream)
     _check(_native.lib().geo_sc_weight_streams(ctypes.byref(desc), _ptr(w), _ptr(out), None, _stream_ptr(stream)),
            "geo_sc_weight_streams")
+    _join(stream)
     return out
 
 
@@ -446,8 +487,10 @@ def weight_streams_from_lines(lines, desc: ConvDesc, stream=None):
     buf = torch.empty(n.value, dtype=torch.int32, device=lines.device)
     out = buf[:lines.numel()].view(lines.shape)
     out.copy_(lines)
+    _fork(stream)
     _check(_native.lib().geo_sc_weight_streams_finish(ctypes.byref(desc), _ptr(out), _stream_ptr(stream)),
            "geo_sc_weight_streams_finish")
+    _join(stream)
     return out
 
 
@@ -483,9 +526,11 @@ def conv2d_add_partial_from_streams(act, wgt, desc: ConvDesc, out=None, stream=N
     if wgt.untyped_storage().nbytes() - wgt.storage_offset() * wgt.element_size() < 4 * n.value:
         raise ValueError("weight streams: the buffer behind this tensor is smaller than geo_sc_weight_stream_words "
                          "(take it from weight_streams())")
+    _fork(stream)
     _check(_native.lib().geo_sc_conv2d_add_partial_from_streams(ctypes.byref(desc), _ptr(act), _ptr(wgt), _ptr(out),
                                                                 _stream_ptr(stream)),
            "geo_sc_conv2d_add_partial_from_streams")
+    _join(stream)
     return out
 
 
@@ -512,10 +557,12 @@ def conv2d_add_partial_backward(x, w, grad_y, bit_length=128, padding=(0, 0), ne
         workspace = torch.empty(backward_workspace_size(desc, options), dtype=torch.uint8, device=x.device)
     gx = torch.empty_like(x) if need_grad_x else None
     gw = torch.empty_like(w) if need_grad_w else None
+    _fork(stream)
     _check(_native.lib().geo_sc_conv2d_add_partial_backward_ex(ctypes.byref(desc), _opt_ptr(options), _ptr(x), _ptr(w),
                                                                _ptr(grad_y), _ptr(gx), _ptr(gw), _ptr(workspace),
                                                                workspace.numel(), _stream_ptr(stream)),
            "geo_sc_conv2d_add_partial_backward")
+    _join(stream)
     return gx, gw
 
 
@@ -564,7 +611,9 @@ def probe_mfma_slices(mode, a, b, workgroups, slices, reload_sixteenths=16, out=
     returns the int32 counts (workgroups, 128, 256)."""
     if out is None:
         out = torch.empty((workgroups, PROBE_MFMA_ROWS, PROBE_MFMA_COLS), dtype=torch.int32, device="cuda")
+    _fork(stream)
     _check(_native.probe_lib().geo_sc_probe_mfma_slices(int(mode), int(reload_sixteenths), int(workgroups), int(slices),
                                                         _ptr(a), a.shape[0], _ptr(b), b.shape[0], _ptr(out),
                                                         _stream_ptr(stream)), "geo_sc_probe_mfma_slices")
+    _join(stream)
     return out
