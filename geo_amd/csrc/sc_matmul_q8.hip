@@ -7,11 +7,13 @@
 //
 // Gradients, straight through the rounding of the operands (g: gradient of y):
 //   dx[m][k] = sum_n (g[m][n] w_scale[n]) w[n][k],   dw[n][k] = sum_m (g[m][n] x_scale[m]) x[m][k]
-// The 8-bit operand is exact in bf16; the scaled gradient is held as a sum of bf16 terms, one where g is bf16 (it has no
-// more digits itself), two where it is fp16 and three where it is fp32 (24 bits), which makes the inner dimension as many times
-// as long.  Sums in fp32.
+// The 8-bit operand is exact in fp16; a row of the scaled gradient is brought by a power of two to where its largest magnitude
+// fills fp16's range, and held as a sum of fp16 terms: one where g is bf16 (11 bits for products of 8-bit numbers), two where it is
+// fp16 or fp32 (23 bits; nothing of a term is lost above 2^-39 of the row's largest), which makes the inner dimension twice as
+// long.  Sums in fp32; the power of two comes out at the end, exactly.  (Terms of bf16 need no powers of two, but one rounds the
+// scaled gradient as coarsely as the result is rounded, and fp32 takes three.)
 //
-// Both products run on one kernel: the 16x16 matrix instructions of int8 (64 deep) and bf16 (32 deep) take the same 16 bytes per
+// Both products run on one kernel: the 16x16 matrix instructions of int8 (64 deep) and fp16 (32 deep) take the same 16 bytes per
 // lane of either operand, so tiles are counted in bytes of the inner dimension.
 #include "sc_dense.h"
 
@@ -20,7 +22,7 @@ namespace {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float v4f __attribute__((ext_vector_type(4)));
-typedef __bf16 v8b __attribute__((ext_vector_type(8)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* LdsPtr;
 
 constexpr int kStage = 64;    // bytes of the inner dimension per stage: one matrix instruction deep
@@ -89,11 +91,11 @@ struct Matrix<false> {
     typedef v4f Sum;
     static __device__ __forceinline__ void add(const v4i& a, const v4i& b, Sum& s)
     {
-        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8b, a), __builtin_bit_cast(v8b, b), s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), s, 0, 0, 0);
     }
     static __device__ __forceinline__ void add_in_place(const v4i& a, const v4i& b, Sum& s)
     {
-        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(s) : "v"(a), "v"(b));
+        asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(s) : "v"(a), "v"(b));
     }
 };
 
@@ -838,7 +840,7 @@ void cut(Plan* p, int which, const Shape& s, int64_t splits, int64_t least)
 }
 
 // What a tile costs, us, measured: `stage` of a stage where a compute unit has as many workgroups as it holds (and each of them
-// alone no less than `alone`), `rest` of everything else.  int8 and bf16 are within a tenth of each other.
+// alone no less than `alone`), `rest` of everything else.  int8 and fp16 are within a tenth of each other.
 struct TileCost {
     int tile, held;
     double stage, alone, rest;
@@ -954,25 +956,19 @@ int run_products(TwoProducts both, const Plan& p, hipStream_t s)
 }
 
 // ---------------------------------------------------------------- operands of the gradients
-
-// the terms of v: each the bf16 nearest to what the earlier ones leave
-template <int TERMS>
-__device__ __forceinline__ void split_terms(float v, bf16 (&t)[TERMS])
-{
-#pragma unroll
-    for (int i = 0; i < TERMS; ++i) {
-        t[i] = (bf16)v;
-        v -= (float)t[i];
-        if (!(fabsf(v) < __uint_as_float(kInfinityBits))) v = 0.f;   // of an infinity nothing is left
-    }
-}
-
-// The operands of both gradients in one launch, its workgroups in three ranges:
-//   g in tiles of 64 x 64:  dx_left[m][term][n] = terms of g[m][n] w_scale[n],  dw_left[n][term][m] = terms of g[m][n] x_scale[m]
-//   w in tiles of 64 x 128: dx_right[k][n] = w[n][k] in bf16
-//   x in tiles of 64 x 128: dw_right[k][m] = x[m][k] in bf16
+//
+// Two launches.  k_grad_peaks, in blocks of peak_rows x peak_cols of g: the largest |g[m][n] w_scale[n]| of each row in the block,
+// the largest |g[m][n] x_scale[m]| of each column.  k_grad_operands, its workgroups in three ranges:
+//   g in tiles of 64 x 64: the blocks' maxima joined to powers of two dx_back[m], dw_back[n];
+//     dx_left[m][term][n] = terms of g[m][n] w_scale[n] / dx_back[m],  dw_left[n][term][m] = terms of g[m][n] x_scale[m] / dw_back[n]
+//   w in tiles of 64 x 128: dx_right[k][n] = w[n][k] in fp16
+//   x in tiles of 64 x 128: dw_right[k][m] = x[m][k] in fp16
 // Rows of an output are padded to whole stages of 64 elements per term, with zeros.
 constexpr int kSide = 64, kWide = 128;
+constexpr int kPeakWide = 64 * kChunk;     // columns that a wave looks at
+constexpr int kPeakBatch = 8;              // rows that it asks for at once
+constexpr int kPeakWaves = 16;             // of a workgroup, at most
+constexpr int64_t kMostPeakRows = 2048;    // rows of a block, whose maxima are kept in LDS
 
 struct OperandArgs {
     const void* g;
@@ -980,32 +976,119 @@ struct OperandArgs {
     int64_t g_stride, x_stride, w_stride, rows, cols, inner;
     const int8_t *x, *w;
     const float *x_scale, *w_scale;
-    int64_t rows_padded, cols_padded;
-    bf16 *dx_left, *dx_right, *dw_left, *dw_right;   // NULL: that gradient is not wanted
-    uint32_t g_tiles, w_tiles;                       // workgroups of the first two ranges
+    int64_t rows_padded, cols_padded, peak_rows, peak_cols;
+    uint32_t row_blocks, col_blocks, g_tiles, w_tiles;   // tiles: workgroups of the first two ranges
+    uint32_t *row_peaks, *col_peaks;                 // [col_blocks][rows], [row_blocks][cols]: bits of the maxima
+    float *dx_back, *dw_back;
+    f16 *dx_left, *dx_right, *dw_left, *dw_right;    // NULL, with its peaks: that gradient is not wanted
 };
 
-template <int TERMS>
-__device__ __forceinline__ void store_terms(const float (&v)[kChunk], bf16* out, int64_t padded)
+// The power of two that brings magnitudes up to `peak` to 2^14 .. 2^15, and its inverse.  Of a row with an infinity or NaN, whose
+// every result is one, it leaves the others finite.  The inverse is no denormal, for peaks below 2^-112 either.
+__device__ __forceinline__ float power_for(uint32_t peak, float* back)
 {
-    bf16 t[TERMS][kChunk];
+    const uint32_t e = peak >> 23 & 255, field = e > 15 ? 268 - e : 253;
+    *back = __uint_as_float((254 - field) << 23);
+    return __uint_as_float(field << 23);
+}
+
+// the terms of v: each the fp16 nearest to what the earlier ones leave
+template <int TERMS>
+__device__ __forceinline__ void store_terms(const float (&v)[kChunk], f16* out, int64_t padded)
+{
+    f16 t[TERMS][kChunk];
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
-        bf16 one[TERMS];
-        split_terms<TERMS>(v[j], one);
-#pragma unroll
-        for (int i = 0; i < TERMS; ++i) t[i][j] = one[i];
+        t[0][j] = (f16)v[j];
+        if constexpr (TERMS == 2) {
+            const float left = v[j] - (float)t[0][j];
+            t[1][j] = fabsf(left) < __uint_as_float(kInfinityBits) ? (f16)left : (f16)0.f;   // of an infinity nothing is left
+        }
     }
 #pragma unroll
     for (int i = 0; i < TERMS; ++i) __builtin_memcpy(out + i * padded, t[i], sizeof t[i]);
 }
 
-// out[c][r] = q[r][c] in bf16 for a tile of 64 rows and 128 columns.  A thread turns four columns of eight rows: it reads a
+// A wave takes eight rows of 512 columns at once, a lane eight columns of them; a workgroup's waves pass over its block's rows, then
+// over further columns.  What lies outside is the last row and the last columns once more: a maximum stays what it is.
+// NARROW: g has fewer columns than a lane takes.
+template <typename T, bool NARROW>
+__global__ __launch_bounds__(kPeakWaves * 64) void k_grad_peaks(OperandArgs a)
+{
+    __shared__ uint32_t row_most[kMostPeakRows], col_most[kPeakWaves * kPeakWide];   // (a wave writes its own rows')
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+    const uint32_t across = blockIdx.x / a.row_blocks, down = blockIdx.x % a.row_blocks;
+    const int64_t r0 = down * a.peak_rows, r1 = r0 + a.peak_rows < a.rows ? r0 + a.peak_rows : a.rows;
+    const int64_t c0 = across * a.peak_cols, c1 = c0 + a.peak_cols < a.cols ? c0 + a.peak_cols : a.cols;
+    for (int64_t from = c0; from < c1; from += kPeakWide) {
+        const int64_t own = from + lane * kChunk, c = NARROW || own + kChunk <= a.cols ? own : a.cols - kChunk;
+        float ws[kChunk] = {};
+        uint32_t most[kChunk] = {};
+        if (a.row_peaks) load_chunk(a.w_scale, c, a.cols, 0.f, ws);
+        for (int64_t r = r0 + wave * kPeakBatch; r < r1; r += waves * kPeakBatch) {
+            T raw[kPeakBatch][kChunk];
+#pragma unroll
+            for (int i = 0; i < kPeakBatch; ++i) {
+                const T* row = (const T*)a.g + (r + i < r1 ? r + i : r1 - 1) * a.g_stride;
+                if constexpr (NARROW) {
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) raw[i][j] = c + j < a.cols ? row[c + j] : (T)0.f;
+                } else {
+                    __builtin_memcpy(raw[i], row + c, sizeof raw[i]);
+                }
+            }
+            uint32_t m[kPeakBatch];
+#pragma unroll
+            for (int i = 0; i < kPeakBatch; ++i) {
+                const float xs = a.col_peaks ? fabsf(a.x_scale[r + i < r1 ? r + i : r1 - 1]) : 0.f;
+                m[i] = 0;
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    const float v = fabsf((float)raw[i][j]);
+                    most[j] = max(most[j], __float_as_uint(v * xs));
+                    m[i] = max(m[i], __float_as_uint(v * fabsf(ws[j])));
+                }
+            }
+            if (a.row_peaks) {
+                // lanes trade halves of their rows until each holds one, row lane % 8
+#pragma unroll
+                for (int half = kPeakBatch / 2; half >= 1; half /= 2)
+#pragma unroll
+                    for (int i = 0; i < half; ++i) {
+                        const bool upper = lane & half;
+                        const uint32_t keep = upper ? m[i + half] : m[i], give = upper ? m[i] : m[i + half];
+                        m[i] = max(keep, (uint32_t)__shfl_xor((int)give, half));
+                    }
+#pragma unroll
+                for (int d = 8; d < 64; d *= 2) m[0] = max(m[0], (uint32_t)__shfl_xor((int)m[0], d));
+                const int64_t at = r - r0 + lane;
+                if (lane < kPeakBatch && r + lane < r1) row_most[at] = from > c0 ? max(row_most[at], m[0]) : m[0];
+            }
+        }
+        if (a.col_peaks) {
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) col_most[(wave * kChunk + j) * 64 + lane] = most[j];
+            __syncthreads();
+            for (int k = threadIdx.x; k < kPeakWide; k += blockDim.x) {
+                uint32_t one = 0;
+                for (int v = 0; v < waves; ++v) one = max(one, col_most[v * kPeakWide + k]);
+                const int64_t mine = from + k % 64 * kChunk, n = (NARROW || mine + kChunk <= a.cols ? mine : a.cols - kChunk) + k / 64;
+                if (n < a.cols) a.col_peaks[down * a.cols + n] = one;
+            }
+            __syncthreads();
+        }
+    }
+    if (!a.row_peaks) return;
+    __syncthreads();
+    for (int64_t r = threadIdx.x; r < r1 - r0; r += blockDim.x) a.row_peaks[across * a.rows + r0 + r] = row_most[r];
+}
+
+// out[c][r] = q[r][c] in fp16 for a tile of 64 rows and 128 columns.  A thread turns four columns of eight rows: it reads a
 // word of each row (a row of 33 words: no two lanes meet in a bank) and writes eight rows' values of each column.
-__device__ __forceinline__ void widen_tile(const int8_t* q, int64_t stride, int64_t rows, int64_t cols, int64_t padded, uint32_t tile, bf16* out,
+constexpr int kWideWords = kWide / 4 + 1;
+__device__ __forceinline__ void widen_tile(const int8_t* q, int64_t stride, int64_t rows, int64_t cols, int64_t padded, uint32_t tile, f16* out,
                                            uint32_t* lds)
 {
-    constexpr int kWords = kWide / 4 + 1;
     const uint32_t across = (uint32_t)((cols + kWide - 1) / kWide);
     const int64_t r0 = (int64_t)(tile / across) * kSide, c0 = (int64_t)(tile % across) * kWide;
 #pragma unroll
@@ -1014,19 +1097,19 @@ __device__ __forceinline__ void widen_tile(const int8_t* q, int64_t stride, int6
         v4i v = {0, 0, 0, 0};
         if (r0 + r < rows && c0 + c < cols) v = load_piece((const uint8_t*)(q + (r0 + r) * stride), c0 + c, cols);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) lds[r * kWords + c / 4 + j] = v[j];
+        for (int j = 0; j < 4; ++j) lds[r * kWideWords + c / 4 + j] = v[j];
     }
     __syncthreads();
     const int r = threadIdx.x % 8 * 8, c = threadIdx.x / 8 * 4;
     uint32_t words[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) words[j] = lds[(r + j) * kWords + c / 4];
+    for (int j = 0; j < 8; ++j) words[j] = lds[(r + j) * kWideWords + c / 4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (c0 + c + j >= cols) break;
-        bf16 t[8];
+        f16 t[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) t[k] = (bf16)(float)(int8_t)(words[k] >> (8 * j));
+        for (int k = 0; k < 8; ++k) t[k] = (f16)(float)(int8_t)(words[k] >> (8 * j));
         __builtin_memcpy(out + (c0 + c + j) * padded + r0 + r, t, sizeof t);
     }
 }
@@ -1035,7 +1118,8 @@ template <int TERMS>
 __global__ __launch_bounds__(256) void k_grad_operands(OperandArgs a)
 {
     __shared__ float tile[kSide][kSide + 1];
-    static_assert(sizeof tile >= kSide * (kWide + 4), "a tile of 8-bit numbers fits");
+    __shared__ uint32_t most[2][4][kSide];
+    static_assert(sizeof tile >= kSide * kWideWords * 4, "a tile of 8-bit numbers fits");
     if (blockIdx.x >= a.g_tiles) {
         const uint32_t at = blockIdx.x - a.g_tiles;
         if (at < a.w_tiles) widen_tile(a.w, a.w_stride, a.cols, a.inner, a.cols_padded, at, a.dx_right, (uint32_t*)tile);
@@ -1044,43 +1128,85 @@ __global__ __launch_bounds__(256) void k_grad_operands(OperandArgs a)
     }
     const uint32_t across = (uint32_t)(a.cols_padded / kSide);
     const int64_t r0 = (int64_t)(blockIdx.x / across) * kSide, c0 = (int64_t)(blockIdx.x % across) * kSide;
+    constexpr int kPasses = kSide * kSide / kChunk / 256;
+    float v[kPasses][kChunk];
 #pragma unroll
-    for (int i = 0; i < kSide * kSide / kChunk / 256; ++i) {
+    for (int i = 0; i < kPasses; ++i) {
         const int at = i * 256 + threadIdx.x, r = at / (kSide / kChunk), c = at % (kSide / kChunk) * kChunk;
-        float v[kChunk] = {};
-        if (r0 + r < a.rows && c0 + c < a.cols) load_chunk(a.g, a.dtype, (r0 + r) * a.g_stride, c0 + c, a.cols, 0.f, v);
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) tile[r][c + j] = v[j];
-        if (a.dx_left && r0 + r < a.rows) {
+        for (int j = 0; j < kChunk; ++j) v[i][j] = 0.f;
+        if (r0 + r < a.rows && c0 + c < a.cols) load_chunk(a.g, a.dtype, (r0 + r) * a.g_stride, c0 + c, a.cols, 0.f, v[i]);
+    }
+    // the blocks' maxima of the tile's rows and columns, a quarter of the blocks per wave
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    uint32_t row_most = 0, col_most = 0;
+    if (a.dx_left && r0 + lane < a.rows)
+        for (uint32_t k = wave; k < a.col_blocks; k += 4) row_most = max(row_most, a.row_peaks[k * a.rows + r0 + lane]);
+    if (a.dw_left && c0 + lane < a.cols)
+        for (uint32_t k = wave; k < a.row_blocks; k += 4) col_most = max(col_most, a.col_peaks[k * a.cols + c0 + lane]);
+    most[0][wave][lane] = row_most;
+    most[1][wave][lane] = col_most;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+        const int at = i * 256 + threadIdx.x, r = at / (kSide / kChunk), c = at % (kSide / kChunk) * kChunk;
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) tile[r][c + j] = v[i][j];
+    }
+    __syncthreads();
+    const auto power = [&](int which, int i, float* back) {
+        return power_for(max(max(most[which][0][i], most[which][1][i]), max(most[which][2][i], most[which][3][i])), back);
+    };
+    float back;
+    if (a.dx_left) {
+        if (c0 == 0 && threadIdx.x < kSide && r0 + threadIdx.x < a.rows) {
+            power(0, threadIdx.x, &back);
+            a.dx_back[r0 + threadIdx.x] = back;
+        }
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int at = i * 256 + threadIdx.x, r = at / (kSide / kChunk), c = at % (kSide / kChunk) * kChunk;
+            if (r0 + r >= a.rows) continue;
             float k[kChunk] = {};
             if (c0 + c < a.cols) load_chunk(a.w_scale, c0 + c, a.cols, 0.f, k);
+            const float up = power(0, r, &back);
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) v[j] *= k[j];
-            store_terms<TERMS>(v, a.dx_left + (r0 + r) * TERMS * a.cols_padded + c0 + c, a.cols_padded);
+            for (int j = 0; j < kChunk; ++j) v[i][j] = v[i][j] * k[j] * up;
+            store_terms<TERMS>(v[i], a.dx_left + (r0 + r) * TERMS * a.cols_padded + c0 + c, a.cols_padded);
         }
     }
     if (!a.dw_left) return;
-    __syncthreads();
+    if (r0 == 0 && threadIdx.x < kSide && c0 + threadIdx.x < a.cols) {
+        power(1, threadIdx.x, &back);
+        a.dw_back[c0 + threadIdx.x] = back;
+    }
 #pragma unroll
-    for (int i = 0; i < kSide * kSide / kChunk / 256; ++i) {
+    for (int i = 0; i < kPasses; ++i) {
         const int at = i * 256 + threadIdx.x, c = at / (kSide / kChunk), r = at % (kSide / kChunk) * kChunk;
         if (c0 + c >= a.cols) continue;
-        float k[kChunk] = {}, v[kChunk];
+        float k[kChunk] = {}, t[kChunk];
         if (r0 + r < a.rows) load_chunk(a.x_scale, r0 + r, a.rows, 0.f, k);
+        const float up = power(1, c, &back);
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) v[j] = tile[r + j][c] * k[j];
-        store_terms<TERMS>(v, a.dw_left + (c0 + c) * TERMS * a.rows_padded + r0 + r, a.rows_padded);
+        for (int j = 0; j < kChunk; ++j) t[j] = tile[r + j][c] * k[j] * up;
+        store_terms<TERMS>(t, a.dw_left + (c0 + c) * TERMS * a.rows_padded + r0 + r, a.rows_padded);
     }
 }
 
-int terms_of(int grad_dtype) { return grad_dtype == GEO_SC_BF16 ? 1 : grad_dtype == GEO_SC_F16 ? 2 : 3; }
-int64_t padded_to_side(int64_t n) { return (n + kSide - 1) / kSide * kSide; }   // whole stages of bf16 elements
+int terms_of(int grad_dtype) { return grad_dtype == GEO_SC_BF16 ? 1 : 2; }
+int64_t padded_to_side(int64_t n) { return (n + kSide - 1) / kSide * kSide; }   // whole stages of fp16 elements
+// rows or columns of a block of which one maximum is taken: some 32 blocks where that leaves each `least` at least
+int64_t peak_block(int64_t n, int64_t least, int64_t most)
+{
+    const int64_t block = ((n + 31) / 32 + least - 1) / least * least;
+    return block < most ? block : most;
+}
 
 // the workspace of the backward: both gradients' operands, then the splits' sums
 struct GradLayout {
     Shape dx, dw;
     Plan plan;   // the first product is dx, or dw where dx is not wanted
-    size_t dx_left, dx_right, dw_left, dw_right, first_partial, second_partial, bytes;
+    size_t dx_left, dx_right, dx_back, dw_left, dw_right, dw_back, row_peaks, col_peaks, first_partial, second_partial, bytes;
+    int64_t peak_rows, peak_cols;
 };
 GradLayout grad_layout(int64_t rows, int64_t cols, int64_t inner, int terms, bool need_dx, bool need_dw)
 {
@@ -1091,14 +1217,20 @@ GradLayout grad_layout(int64_t rows, int64_t cols, int64_t inner, int terms, boo
         at += align256(bytes);
         return here;
     };
+    l.peak_rows = peak_block(rows, 32, kMostPeakRows);
+    l.peak_cols = peak_block(cols, kPeakWide, (int64_t)1 << 40);
     if (need_dx) {
         const int64_t p = padded_to_side(cols);
+        l.row_peaks = take((size_t)((cols + l.peak_cols - 1) / l.peak_cols) * rows * 4);
+        l.dx_back = take((size_t)rows * 4);
         l.dx = {rows, inner, terms * p * 2};
         l.dx_left = take((size_t)rows * terms * p * 2);
         l.dx_right = take((size_t)inner * p * 2);
     }
     if (need_dw) {
         const int64_t p = padded_to_side(rows);
+        l.col_peaks = take((size_t)((rows + l.peak_rows - 1) / l.peak_rows) * cols * 4);
+        l.dw_back = take((size_t)cols * 4);
         l.dw = {cols, inner, terms * p * 2};
         l.dw_left = take((size_t)cols * terms * p * 2);
         l.dw_right = take((size_t)inner * p * 2);
@@ -1183,7 +1315,8 @@ int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64_t grad_str
     const auto tiles = [](int64_t r, int64_t rs, int64_t c, int64_t cs) { return ((r + rs - 1) / rs) * ((c + cs - 1) / cs); };
     const int64_t g_tiles = tiles(rows, kSide, cols, kSide), w_tiles = dx ? tiles(cols, kSide, inner, kWide) : 0,
                   x_tiles = dw ? tiles(rows, kSide, inner, kWide) : 0;
-    if (g_tiles + w_tiles + x_tiles > 0x7fffffff) return GEO_SC_ERR_UNSUPPORTED;
+    const int64_t blocks = tiles(rows, l.peak_rows, cols, l.peak_cols);
+    if (g_tiles + w_tiles + x_tiles > 0x7fffffff || blocks > 0x7fffffff) return GEO_SC_ERR_UNSUPPORTED;
     hipStream_t s = (hipStream_t)stream;
     uint8_t* base = (uint8_t*)workspace;
     OperandArgs o = {};
@@ -1201,15 +1334,33 @@ int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64_t grad_str
     o.w_scale = w_scale;
     o.rows_padded = padded_to_side(rows);
     o.cols_padded = padded_to_side(cols);
-    if (dx) o.dx_left = (bf16*)(base + l.dx_left), o.dx_right = (bf16*)(base + l.dx_right);
-    if (dw) o.dw_left = (bf16*)(base + l.dw_left), o.dw_right = (bf16*)(base + l.dw_right);
+    if (dx) {
+        o.dx_left = (f16*)(base + l.dx_left), o.dx_right = (f16*)(base + l.dx_right);
+        o.dx_back = (float*)(base + l.dx_back), o.row_peaks = (uint32_t*)(base + l.row_peaks);
+    }
+    if (dw) {
+        o.dw_left = (f16*)(base + l.dw_left), o.dw_right = (f16*)(base + l.dw_right);
+        o.dw_back = (float*)(base + l.dw_back), o.col_peaks = (uint32_t*)(base + l.col_peaks);
+    }
+    o.peak_rows = l.peak_rows;
+    o.peak_cols = l.peak_cols;
+    o.row_blocks = (uint32_t)((rows + l.peak_rows - 1) / l.peak_rows);
+    o.col_blocks = (uint32_t)((cols + l.peak_cols - 1) / l.peak_cols);
     o.g_tiles = (uint32_t)g_tiles;
     o.w_tiles = (uint32_t)w_tiles;
+    const dim3 peak_threads((uint32_t)((l.peak_rows < kPeakWaves * kPeakBatch ? l.peak_rows / kPeakBatch : kPeakWaves) * 64));
+    const auto peaks = [&](auto one) {
+        using T = decltype(one);
+        if (cols < kChunk) k_grad_peaks<T, true><<<dim3((uint32_t)blocks), peak_threads, 0, s>>>(o);
+        else k_grad_peaks<T, false><<<dim3((uint32_t)blocks), peak_threads, 0, s>>>(o);
+    };
+    if (grad_dtype == GEO_SC_F32) peaks(f32());
+    else if (grad_dtype == GEO_SC_BF16) peaks(bf16());
+    else peaks(f16());
     const dim3 grid((uint32_t)(g_tiles + w_tiles + x_tiles));
     if (terms == 1) k_grad_operands<1><<<grid, dim3(256), 0, s>>>(o);
-    else if (terms == 2) k_grad_operands<2><<<grid, dim3(256), 0, s>>>(o);
-    else k_grad_operands<3><<<grid, dim3(256), 0, s>>>(o);
-    const auto product = [&](const Shape& shape, size_t left, size_t right, bool cut, size_t partial, void* y, int dtype) {
+    else k_grad_operands<2><<<grid, dim3(256), 0, s>>>(o);
+    const auto product = [&](const Shape& shape, size_t left, size_t right, size_t back, bool cut, size_t partial, void* y, int dtype) {
         TileArgs a = {};
         a.x = base + left;
         a.w = base + right;
@@ -1219,17 +1370,18 @@ int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64_t grad_str
         a.cols = shape.cols;
         a.inner = shape.inner;
         a.w_stages = (int)(a.w_stride / kStage);
+        a.x_scale = (const float*)(base + back);
         a.y = y;
         a.dtype = dtype;
         a.partial = cut ? (uint32_t*)(base + partial) : nullptr;
         return a;
     };
     TwoProducts both = {};
-    if (dx) both.first = product(l.dx, l.dx_left, l.dx_right, l.plan.splits[0] > 1, l.first_partial, dx, dx_dtype);
+    if (dx) both.first = product(l.dx, l.dx_left, l.dx_right, l.dx_back, l.plan.splits[0] > 1, l.first_partial, dx, dx_dtype);
     if (dw) {
         const int which = dx ? 1 : 0;
         (dx ? both.second : both.first) =
-            product(l.dw, l.dw_left, l.dw_right, l.plan.splits[which] > 1, dx ? l.second_partial : l.first_partial, dw, dw_dtype);
+            product(l.dw, l.dw_left, l.dw_right, l.dw_back, l.plan.splits[which] > 1, dx ? l.second_partial : l.first_partial, dw, dw_dtype);
     }
     return run_products<false>(both, l.plan, s);
 }

@@ -300,11 +300,52 @@ def test_linear(uf, dtype, shape):
     want = product64(q, s, wq, ws)
     close(y, want, (EPS[dtype] + 4 * U) * want.abs() + subnormal(dtype))
     xr, wr, g64 = q.double() * s.double()[:, None], wq.double() * ws.double()[:, None], g.double()
-    # the scaled gradient: one bf16 number (EPS), two (EPS^2) or three (its fp32 rounding); fp32 sums of all terms
-    terms = {torch.bfloat16: 1, torch.float16: 2, torch.float32: 3}[dtype]
-    kept = EPS[torch.bfloat16] ** terms + U
-    for got, want, size, depth in ((dx, g64 @ wr, g64.abs() @ wr.abs(), n), (dw, g64.t() @ xr, g64.t().abs() @ xr.abs(), m)):
-        close(got, want, EPS[dtype] * want.abs() + (kept + 2 * terms * depth * U) * size + subnormal(dtype))
+    # the scaled gradient: one fp16 number (EPS) or two (EPS^2), the last one's steps 2^-39 of the row's largest; fp32 sums of all terms
+    terms = 1 if dtype == torch.bfloat16 else 2
+    kept = EPS[torch.float16] ** terms + U
+    left_x, left_w = (g64 * ws.double()).abs().amax(1, keepdim=True), (g64 * s.double()[:, None]).abs().amax(0)[:, None]
+    for got, want, size, depth, low in ((dx, g64 @ wr, g64.abs() @ wr.abs(), n, left_x * wq.double().abs().sum(0)),
+                                        (dw, g64.t() @ xr, g64.t().abs() @ xr.abs(), m, left_w * q.double().abs().sum(0))):
+        close(got, want, EPS[dtype] * want.abs() + (kept + 2 * terms * depth * U) * size + 2.0 ** -39 * low + subnormal(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_of_rows_of_any_magnitude(uf, dtype):
+    """a row of a gradient is as exact whatever its magnitude; zeros stay zeros, infinities and NaN stay in their row and column"""
+    m, n, k = 150, 90, 70
+    x, w, g = rand(m, k, dtype=dtype, seed=1), rand(n, k, dtype=dtype, seed=2), rand(m, n, dtype=dtype, seed=3)
+    g = (g.double() * 2.0 ** ((torch.arange(m, device="cuda") * 37 % 181) - 90).double()[:, None]).to(dtype)
+    g[7], g[20, 5], g[40, 60], g[130, 5] = 0, float("inf"), float("nan"), -float("inf")
+    dx, dw = torch.autograd.grad((uf.linear_q8(x.requires_grad_(True), w.requires_grad_(True)),), (x, w), (g,))
+    (q, s, _), (wq, ws, _) = uf.quantize_rows(x.detach()), uf.quantize_rows(w.detach())
+    xr, wr, g64 = q.double() * s.double()[:, None], wq.double() * ws.double()[:, None], g.double()
+    bad_rows, bad_cols = ~torch.isfinite(g64).all(1), ~torch.isfinite(g64).all(0)
+    assert not torch.isfinite(dx[bad_rows]).any() and not torch.isfinite(dw[bad_cols]).any() and (dx[7] == 0).all()
+    terms = 1 if dtype == torch.bfloat16 else 2
+    kept = EPS[torch.float16] ** terms + U
+    a, b = g64[~bad_rows], g64[:, ~bad_cols].t()
+    low = 2.0 ** -39 * (a * ws.double()).abs().amax(1, keepdim=True) * wq.double().abs().sum(0)
+    close(dx[~bad_rows], a @ wr, EPS[dtype] * (a @ wr).abs() + (kept + 2 * terms * n * U) * (a.abs() @ wr.abs()) + low + subnormal(dtype))
+    low = 2.0 ** -39 * (b * s.double()).abs().amax(1, keepdim=True) * q.double().abs().sum(0)
+    close(dw[~bad_cols], b @ xr, EPS[dtype] * (b @ xr).abs() + (kept + 2 * terms * m * U) * (b.abs() @ xr.abs()) + low + subnormal(dtype))
+
+
+@pytest.mark.parametrize("shape", [(70000, 33, 20), (33, 20011, 20), (5000, 1100, 40)])
+def test_gradients_of_long_sides(uf, shape):
+    """maxima joined from many blocks of the gradient, the largest element anywhere"""
+    m, n, k = shape
+    x, w, g = rand(m, k, seed=1), rand(n, k, seed=2), rand(m, n, seed=3)
+    rows, cols = torch.arange(0, m, 97, device="cuda"), torch.arange(0, n, 31, device="cuda")
+    g[rows, rows * 13 % n] = 2.0 ** 40
+    g[cols * 29 % m, cols] = -2.0 ** 50
+    dx, dw = torch.autograd.grad((uf.linear_q8(x.requires_grad_(True), w.requires_grad_(True)),), (x, w), (g,))
+    (q, s, _), (wq, ws, _) = uf.quantize_rows(x.detach()), uf.quantize_rows(w.detach())
+    xr, wr, g64 = q.double() * s.double()[:, None], wq.double() * ws.double()[:, None], g.double()
+    kept = EPS[torch.float16] ** 2 + U
+    low = 2.0 ** -39 * (g64 * ws.double()).abs().amax(1, keepdim=True) * wq.double().abs().sum(0)
+    close(dx, g64 @ wr, U * (g64 @ wr).abs() + (kept + 4 * n * U) * (g64.abs() @ wr.abs()) + low)
+    low = 2.0 ** -39 * (g64 * s.double()[:, None]).abs().amax(0)[:, None] * q.double().abs().sum(0)
+    close(dw, g64.t() @ xr, U * (g64.t() @ xr).abs() + (kept + 4 * m * U) * (g64.t().abs() @ xr.abs()) + low)
 
 
 def test_linear_needs_one_gradient_only(uf):
