@@ -54,8 +54,8 @@ def test_matmul_refuses(lib):
         assert lib.geo_sc_matmul_q8_workspace_size(*sizes, ctypes.byref(size)) == INVALID
         assert lib.geo_sc_matmul_q8_backward_workspace_size(*sizes, 0, 1, 1, ctypes.byref(size)) == INVALID
     # few workgroups and a long inner dimension: cut, with partial sums
-    assert lib.geo_sc_matmul_q8_workspace_size(100, 130, 4096, ctypes.byref(size)) == 0 and size.value >= 2 * 100 * 130 * 4
-    good = [P, 4096, P, P, 4096, P, 100, 130, 4096, P, 1, P, 1 << 30, None]
+    assert lib.geo_sc_matmul_q8_workspace_size(100, 130, 65536, ctypes.byref(size)) == 0 and size.value >= 2 * 100 * 130 * 4
+    good = [P, 4096, P, P, 4096, P, 100, 130, 65536, P, 1, P, 1 << 30, None]
     for at, bad, status in ((0, None, INVALID), (1, -1, INVALID), (2, None, INVALID), (3, None, INVALID), (4, -1, INVALID), (5, None, INVALID),
                             (6, 0, INVALID), (7, 0, INVALID), (8, 131072, INVALID), (9, None, INVALID), (10, 4, INVALID),
                             (11, None, WORKSPACE), (11, P + 4, WORKSPACE), (12, 100, WORKSPACE)):
