@@ -115,33 +115,44 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, MaybeTensor, MaybeTensor> rms_nor
 
 // (dx, dweight)
 std::tuple<at::Tensor, MaybeTensor> rms_norm_q8_backward(const MaybeTensor& grad_values, const MaybeTensor& grad_total,
-                                                         const at::Tensor& total, const at::Tensor& weight, const at::Tensor& rstd,
-                                                         bool need_weight)
+                                                         const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight,
+                                                         const at::Tensor& rstd, bool need_weight)
 {
-    const Rows t = as_rows(total, "total");
-    const c10::hip::HIPGuardMasqueradingAsCUDA guard(total.device());
+    const Rows t = as_rows(x, "x");
+    Rows r = {};
+    if (residual.defined()) r = as_rows(residual, "residual");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     if (!grad_values || t.rows == 0) {   // nothing comes through the norm itself
-        return {grad_total ? grad_total->to(total.scalar_type()) : at::zeros_like(total),
+        return {grad_total ? grad_total->to(x.scalar_type()) : at::zeros_like(x),
                 need_weight ? MaybeTensor(at::zeros_like(weight)) : MaybeTensor()};
     }
     const Rows g = as_rows(*grad_values, "gradient");
     Rows h = {};
-    if (grad_total) h = as_rows(grad_total->to(total.scalar_type()), "gradient");
-    const at::Tensor w = weight.contiguous(), dx = at::empty(total.sizes(), total.options());
+    if (grad_total) h = as_rows(grad_total->to(x.scalar_type()), "gradient");
+    const at::Tensor w = weight.contiguous(), dx = at::empty(x.sizes(), x.options());
     MaybeTensor dw, workspace;
     size_t bytes = 0;
     if (need_weight) {
         dw = at::empty_like(w);
         check_status(geo_sc_rms_norm_q8_backward_workspace_size(t.rows, t.cols, &bytes), "workspace query");
-        workspace = at::empty({(int64_t)bytes}, total.options().dtype(at::kByte));
+        workspace = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
     }
-    const int dtype = dtype_of(total.scalar_type(), "total");
+    const int dtype = dtype_of(x.scalar_type(), "x");
     check_status(geo_sc_rms_norm_q8_backward(g.t.const_data_ptr(), dtype_of(g.t.scalar_type(), "gradient"), g.stride,
                                              grad_total ? h.t.const_data_ptr() : nullptr, h.stride, t.t.const_data_ptr(), t.stride,
-                                             w.const_data_ptr(), dtype, t.rows, t.cols, rstd.const_data_ptr<float>(), dx.data_ptr(),
-                                             data_of(dw), data_of(workspace), bytes, stream_of(total)),
+                                             residual.defined() ? r.t.const_data_ptr() : nullptr, r.stride, w.const_data_ptr(), dtype, t.rows,
+                                             t.cols, rstd.const_data_ptr<float>(), dx.data_ptr(), data_of(dw), data_of(workspace), bytes,
+                                             stream_of(x)),
                  "rms_norm_q8 backward");
     return {dx, dw};
+}
+
+// What the backward forms x + residual from: themselves, because `total` is rounded to their type; where that is fp32, `total`
+// is the sum itself and half the reading.
+std::pair<at::Tensor, at::Tensor> summands(const at::Tensor& x, const MaybeTensor& residual, const at::Tensor& total)
+{
+    if (residual && x.scalar_type() != at::kFloat) return {x, *residual};
+    return {total, at::Tensor()};
 }
 
 // 8-bit rows with a scale each: what the products take
@@ -322,7 +333,8 @@ struct RmsNormQ8 : torch::autograd::Function<RmsNormQ8> {
     {
         const auto [q, scale, total, values, rstd] = rms_norm_q8(x, weight, residual, eps, values_type, true);
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({total, weight, *rstd});
+        const auto [first, second] = summands(x, residual, total);
+        ctx->save_for_backward({first, second, weight, *rstd});
         ctx->mark_non_differentiable({q, scale});
         variable_list out = {q, scale, *values};
         if (residual) out.push_back(total);
@@ -332,7 +344,7 @@ struct RmsNormQ8 : torch::autograd::Function<RmsNormQ8> {
     {
         const auto s = ctx->get_saved_variables();
         const bool residual = grads.size() > 3;
-        const auto [dx, dw] = rms_norm_q8_backward(maybe(grads[2]), residual ? maybe(grads[3]) : MaybeTensor(), s[0], s[1], s[2],
+        const auto [dx, dw] = rms_norm_q8_backward(maybe(grads[2]), residual ? maybe(grads[3]) : MaybeTensor(), s[0], s[1], s[2], s[3],
                                                    ctx->needs_input_grad(1));
         return {ctx->needs_input_grad(0) ? dx : at::Tensor(), undefined_or(dw), residual && ctx->needs_input_grad(2) ? dx : at::Tensor(),
                 at::Tensor(), at::Tensor()};
@@ -347,7 +359,8 @@ struct NormLinearQ8 : torch::autograd::Function<NormLinearQ8> {
         const auto [q, scale, total, none, rstd] = rms_norm_q8(x, gain, residual, eps, std::nullopt, true);
         const auto [wq, wscale, none2] = quantize_rows(weight, std::nullopt);
         ctx->set_materialize_grads(false);
-        ctx->save_for_backward({q, scale, wq, wscale, total, gain, *rstd});
+        const auto [first, second] = summands(x, residual, total);
+        ctx->save_for_backward({q, scale, wq, wscale, first, second, gain, *rstd});
         ctx->saved_data["w"] = weight.scalar_type();
         variable_list out = {matmul_q8(q, scale, wq, wscale, x.scalar_type())};
         if (residual) out.push_back(total);
@@ -366,7 +379,7 @@ struct NormLinearQ8 : torch::autograd::Function<NormLinearQ8> {
             if (ctx->needs_input_grad(2)) w = ctx->saved_data["w"].toScalarType();
             std::tie(dn, dw) = matmul_q8_backward(grads[0], s[0], s[1], s[2], s[3], x, w);
         }
-        if (through) std::tie(dx, dgain) = rms_norm_q8_backward(dn, residual ? maybe(grads[1]) : MaybeTensor(), s[4], s[5], s[6], need_gain);
+        if (through) std::tie(dx, dgain) = rms_norm_q8_backward(dn, residual ? maybe(grads[1]) : MaybeTensor(), s[4], s[5], s[6], s[7], need_gain);
         return {ctx->needs_input_grad(0) ? dx : at::Tensor(), undefined_or(dgain), undefined_or(dw),
                 residual && ctx->needs_input_grad(3) ? dx : at::Tensor(), at::Tensor()};
     }

@@ -39,6 +39,17 @@ __device__ __forceinline__ void load_chunk(const T* row, int64_t c, int64_t cols
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) v[j] = c + j < cols ? (float)row[c + j] : fill;
 }
+// the same as it lies in memory, zeros behind the row's end: what is converted later need not be waited for at the load
+template <typename T>
+__device__ __forceinline__ void fetch_chunk(const T* row, int64_t c, int64_t cols, T (&raw)[kChunk])
+{
+    if (c + kChunk <= cols) {
+        __builtin_memcpy(raw, row + c, sizeof raw);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) raw[j] = c + j < cols ? row[c + j] : (T)0.f;
+}
 // `streamed`: past the caches, see streams()
 template <typename T>
 __device__ __forceinline__ void store_chunk(T* row, int64_t c, int64_t cols, const float (&v)[kChunk], bool streamed = false)

@@ -9,6 +9,8 @@
 //
 // Backward of the norm, straight through the rounding, with g the gradient of the values and h that of the sum:
 //   u = g w,   dt = r (u - t r^2 mean(u t)) + h,   dx = dresidual = dt,   dw = sum over the rows of g t r
+// t is formed again from x and residual: the sum that the forward returns is rounded to their type, which would show in dw
+// (bf16: 2.5e-3 of its size, where its own rounding is 1.7e-3).
 #include "sc_dense.h"
 
 namespace geo_sc {
@@ -200,9 +202,9 @@ int run_rows(const RowsArgs& a, int dtype, hipStream_t s)
 // ---------------------------------------------------------------- backward of the norm
 
 struct NormBackArgs {
-    const void *grad_values, *grad_total, *total, *weight;
+    const void *grad_values, *grad_total, *x, *residual, *weight;   // grad_total, residual: or NULL
     int grad_dtype;
-    int64_t rows, cols, grad_stride, grad_total_stride, total_stride;
+    int64_t rows, cols, grad_stride, grad_total_stride, x_stride, residual_stride;
     const float* rstd;
     void *dx;
     bool streamed;    // dx
@@ -234,13 +236,17 @@ __global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs a)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
             if (column(i) < a.cols) {
-                load_chunk((const G*)a.grad_values + row * a.grad_stride, column(i), a.cols, 0.f, g[i]);
-                load_chunk((const T*)a.total + row * a.total_stride, column(i), a.cols, 0.f, v[i]);
-#pragma unroll
-                for (int j = 0; j < kChunk; ++j) h[i][j] = 0.f;
-                if (a.grad_total) load_chunk((const T*)a.grad_total + row * a.grad_total_stride, column(i), a.cols, 0.f, h[i]);
+                G grad[kChunk];
+                T x[kChunk], residual[kChunk] = {}, also[kChunk] = {};
+                fetch_chunk((const G*)a.grad_values + row * a.grad_stride, column(i), a.cols, grad);
+                fetch_chunk((const T*)a.x + row * a.x_stride, column(i), a.cols, x);
+                if (a.residual) fetch_chunk((const T*)a.residual + row * a.residual_stride, column(i), a.cols, residual);
+                if (a.grad_total) fetch_chunk((const T*)a.grad_total + row * a.grad_total_stride, column(i), a.cols, also);
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
+                    g[i][j] = (float)grad[j];
+                    v[i][j] = (float)x[j] + (float)residual[j];
+                    h[i][j] = (float)also[j];
                     dw[i][j] += g[i][j] * (v[i][j] * unit);
                     g[i][j] *= w[i][j];
                     along += g[i][j] * v[i][j];
@@ -267,6 +273,18 @@ __global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs a)
     }
 }
 
+// a chunk of t = x + residual
+template <typename T>
+__device__ __forceinline__ void load_sum(const NormBackArgs& a, int64_t row, int64_t c, float (&v)[kChunk])
+{
+    load_chunk((const T*)a.x + row * a.x_stride, c, a.cols, 0.f, v);
+    if (!a.residual) return;
+    float r[kChunk];
+    load_chunk((const T*)a.residual + row * a.residual_stride, c, a.cols, 0.f, r);
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) v[j] += r[j];
+}
+
 // Rows that do not fit into a block's registers: dx row by row, read twice; the weight's gradient by columns, see
 // k_weight_grad_columns.
 template <typename T>
@@ -280,7 +298,7 @@ __global__ __launch_bounds__(1024) void k_norm_back_long(NormBackArgs a)
     float g[kChunk], v[kChunk], w[kChunk];
     const auto take = [&](int64_t c) {
         load_chunk(a.grad_values, a.grad_dtype, row * a.grad_stride, c, a.cols, 0.f, g);
-        load_chunk((const T*)a.total + row * a.total_stride, c, a.cols, 0.f, v);
+        load_sum<T>(a, row, c, v);
         load_chunk((const T*)a.weight, c, a.cols, 0.f, w);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) g[j] *= w[j];
@@ -313,7 +331,7 @@ __global__ __launch_bounds__(256) void k_weight_grad_columns(NormBackArgs a)
     float dw[kChunk] = {}, g[kChunk], v[kChunk];
     for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
         load_chunk(a.grad_values, a.grad_dtype, row * a.grad_stride, c, a.cols, 0.f, g);
-        load_chunk((const T*)a.total + row * a.total_stride, c, a.cols, 0.f, v);
+        load_sum<T>(a, row, c, v);
         const float r = a.rstd[row];
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) dw[j] += g[j] * (v[j] * r);
@@ -433,18 +451,18 @@ int geo_sc_rms_norm_q8_backward_workspace_size(int64_t rows, int64_t cols, size_
 }
 
 int geo_sc_rms_norm_q8_backward(const void* grad_values, int grad_dtype, int64_t grad_stride, const void* grad_total,
-                                int64_t grad_total_stride, const void* total, int64_t total_stride, const void* weight, int dtype,
-                                int64_t rows, int64_t cols, const float* rstd, void* dx, void* dweight, void* workspace,
-                                size_t workspace_bytes, geo_sc_stream_t stream)
+                                int64_t grad_total_stride, const void* x, int64_t x_stride, const void* residual,
+                                int64_t residual_stride, const void* weight, int dtype, int64_t rows, int64_t cols, const float* rstd,
+                                void* dx, void* dweight, void* workspace, size_t workspace_bytes, geo_sc_stream_t stream)
 {
     if (!sizes_fit(rows, cols) || rows < 1 || !dtype_known(dtype) || !dtype_known(grad_dtype) || grad_stride < 0 ||
-        grad_total_stride < 0 || total_stride < 0 || !grad_values || !total || !weight || !rstd || !dx)
+        grad_total_stride < 0 || x_stride < 0 || residual_stride < 0 || !grad_values || !x || !weight || !rstd || !dx)
         return GEO_SC_ERR_INVALID_ARGUMENT;
     size_t need = 0;
     geo_sc_rms_norm_q8_backward_workspace_size(rows, cols, &need);
     if (dweight && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 4)) return GEO_SC_ERR_WORKSPACE;
-    const NormBackArgs a = {grad_values, grad_total, total, weight, grad_dtype, rows, cols, grad_stride, grad_total_stride,
-                            total_stride, rstd, dx, streams(rows * cols * dtype_bytes(dtype)), dweight ? (float*)workspace : nullptr};
+    const NormBackArgs a = {grad_values, grad_total, x, residual, weight, grad_dtype, rows, cols, grad_stride, grad_total_stride,
+                            x_stride, residual_stride, rstd, dx, streams(rows * cols * dtype_bytes(dtype)), dweight ? (float*)workspace : nullptr};
     hipStream_t s = (hipStream_t)stream;
     if (dtype == GEO_SC_F32) return run_norm_back<f32>(a, (f32*)dweight, s);
     if (dtype == GEO_SC_BF16) return run_norm_back<bf16>(a, (bf16*)dweight, s);

@@ -489,7 +489,8 @@ GEO_SC_API int geo_sc_quantize_rows(const void* x, int dtype, int64_t rows, int6
  *   rstd            NULL, or rows floats: r, for the backward
  * Backward, straight through the rounding to 8 bits, from g (gradient of the values), `grad_total` (of t; NULL: none):
  * u = g weight, dx = r (u - t r^2 mean(u t)) + grad_total, the gradient of x and of the residual alike; dweight = sum over
- * the rows of g t r (NULL: not wanted), in an order that does not change from run to run.  `total` is t as the forward wrote it.
+ * the rows of g t r (NULL: not wanted), in an order that does not change from run to run.  t is formed again
+ * from x and residual (NULL: none); the forward's `total` of GEO_SC_F32 is t exactly and may stand for x, without a residual.
  * Workspace, 4-byte aligned: geo_sc_rms_norm_q8_backward_workspace_size, needed for dweight.
  */
 GEO_SC_API int geo_sc_rms_norm_q8(const void* x, const void* residual, const void* weight, int dtype, int64_t rows, int64_t cols,
@@ -497,9 +498,10 @@ GEO_SC_API int geo_sc_rms_norm_q8(const void* x, const void* residual, const voi
                                   void* total, void* values, int values_dtype, float* rstd, geo_sc_stream_t stream);
 GEO_SC_API int geo_sc_rms_norm_q8_backward_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
 GEO_SC_API int geo_sc_rms_norm_q8_backward(const void* grad_values, int grad_dtype, int64_t grad_stride, const void* grad_total,
-                                           int64_t grad_total_stride, const void* total, int64_t total_stride, const void* weight,
-                                           int dtype, int64_t rows, int64_t cols, const float* rstd, void* dx, void* dweight,
-                                           void* workspace, size_t workspace_bytes, geo_sc_stream_t stream);
+                                           int64_t grad_total_stride, const void* x, int64_t x_stride, const void* residual,
+                                           int64_t residual_stride, const void* weight, int dtype, int64_t rows, int64_t cols,
+                                           const float* rstd, void* dx, void* dweight, void* workspace, size_t workspace_bytes,
+                                           geo_sc_stream_t stream);
 
 /*
  * y[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] of 8-bit x (rows, inner) and w (cols, inner), y (rows, cols) of

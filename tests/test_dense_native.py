@@ -40,9 +40,10 @@ def test_rms_norm_refuses(lib):
     size = ctypes.c_size_t()
     assert lib.geo_sc_rms_norm_q8_backward_workspace_size(100, 64, ctypes.byref(size)) == 0 and size.value >= 64 * 4
     assert lib.geo_sc_rms_norm_q8_backward_workspace_size(100, 0, ctypes.byref(size)) == INVALID
-    good = [P, 1, 8, None, 0, P, 8, P, 1, 4, 8, P, P, P, P, 1 << 30, None]
-    for at, bad, status in ((0, None, INVALID), (1, 9, INVALID), (2, -1, INVALID), (5, None, INVALID), (7, None, INVALID), (8, 9, INVALID), (9, 0, INVALID),
-                            (10, 0, INVALID), (11, None, INVALID), (12, None, INVALID), (14, None, WORKSPACE), (14, P + 2, WORKSPACE), (15, 3, WORKSPACE)):
+    good = [P, 1, 8, None, 0, P, 8, P, 8, P, 1, 4, 8, P, P, P, P, 1 << 30, None]
+    for at, bad, status in ((0, None, INVALID), (1, 9, INVALID), (2, -1, INVALID), (5, None, INVALID), (6, -1, INVALID), (8, -1, INVALID), (9, None, INVALID),
+                            (10, 9, INVALID), (11, 0, INVALID), (12, 0, INVALID), (13, None, INVALID), (14, None, INVALID), (16, None, WORKSPACE),
+                            (16, P + 2, WORKSPACE), (17, 3, WORKSPACE)):
         args = list(good)
         args[at] = bad
         assert lib.geo_sc_rms_norm_q8_backward(*args) == status, (at, bad)
