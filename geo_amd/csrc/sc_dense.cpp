@@ -194,7 +194,8 @@ at::Tensor matmul_q8(const at::Tensor& q, const at::Tensor& scale, const at::Ten
     const at::Tensor y = at::empty(sizes, q.options().dtype(type));
     if (y.numel() == 0) return y;
     size_t bytes = 0;
-    check_status(geo_sc_matmul_q8_workspace_size(x.r.rows, w.r.rows, x.r.cols, &bytes), "workspace query");
+    check_status(geo_sc_matmul_q8_workspace_size(x.r.t.const_data_ptr<int8_t>(), x.r.stride, w.r.t.const_data_ptr<int8_t>(),
+                                                 w.r.stride, x.r.rows, w.r.rows, x.r.cols, &bytes), "workspace query");
     MaybeTensor workspace;
     if (bytes) workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
     check_status(geo_sc_matmul_q8(x.r.t.const_data_ptr<int8_t>(), x.r.stride, x.scale.const_data_ptr<float>(), w.r.t.const_data_ptr<int8_t>(),

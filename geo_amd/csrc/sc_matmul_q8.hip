@@ -72,6 +72,44 @@ __device__ __forceinline__ v4i load_piece(const uint8_t* row, int64_t k, int64_t
     return __builtin_bit_cast(v4i, shift < 16 ? v >> (8 * (int)shift) : (unsigned __int128)0);
 }
 
+// 16 N bytes from any address.  Loads at odd addresses take the memory pipeline twice and more (4096 x 16384 bytes of w at odd
+// strides, 16 rows of x: 39 us, at multiples of four 18): whole words are loaded, those that hold the first byte to the last,
+// and shifted.
+template <int N>
+struct Shifted {
+    typedef int Four __attribute__((ext_vector_type(4), aligned(4)));
+    const uint8_t* from;
+    int shift, last;
+    Shifted() = default;
+    __device__ __forceinline__ explicit Shifted(const uint8_t* p)
+        : from((const uint8_t*)((uintptr_t)p & ~(uintptr_t)3)), shift((int)((uintptr_t)p & 3)), last(shift ? 16 * N : 16 * N - 4)
+    {
+    }
+    struct Words {
+        Four four[N];
+        uint32_t last;
+    };
+    __device__ __forceinline__ Words load(int64_t offset) const   // a multiple of four
+    {
+        Words t;
+#pragma unroll
+        for (int i = 0; i < N; ++i) t.four[i] = *(const Four*)(from + offset + 16 * i);
+        t.last = *(const uint32_t*)(from + offset + last);
+        return t;
+    }
+    __device__ __forceinline__ v4i piece(const Words& t, int i) const
+    {
+        uint32_t u[5];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = (uint32_t)t.four[i][k];
+        u[4] = i + 1 < N ? (uint32_t)t.four[i + 1 < N ? i + 1 : i][0] : t.last;
+        v4i v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = (int)__builtin_amdgcn_alignbyte(u[k + 1], u[k], (uint32_t)shift);
+        return v;
+    }
+};
+
 template <bool INT8>
 struct Matrix;
 template <>
@@ -506,7 +544,8 @@ __global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)
     finish_tile<B, INT8>(p, sum, scales, areas[wave], wave, lane);
 }
 
-// Any rows: stages through registers, the next one on its way while one is multiplied.
+// Fewer stages than the ring of k_tiles holds, at any alignment: stages through registers, the next one on its way while one is
+// multiplied.  1000 x 1000 x 239: 6.6 us, its launch and one way to memory and back.
 template <int B, bool INT8>
 __global__ __launch_bounds__(kWaves * 64) void k_tiles_any(TwoProducts both)
 {
@@ -538,58 +577,98 @@ __global__ __launch_bounds__(kWaves * 64) void k_tiles_any(TwoProducts both)
     finish_tile<B, INT8>(p, sum, scales, areas[wave], wave, lane);
 }
 
-// Few rows of x (at most 16 MT): y is bound by the one read of w.  A wave reads 128 bytes of 16 NT rows of w per step, 32 per lane,
+// Rows that start anywhere, laid out anew at multiples of 16 bytes for k_tiles: a piece of a row per thread.  What lies behind a
+// row's end up to such a multiple is zero.  (4096 x 4096 x 4095, odd strides: 76 us, of which the copies 10; k_tiles_any on them as
+// they lie 231.  1009 x 1003 x 1111: 10.6 and 16.7.)
+struct AlignArgs {
+    const uint8_t* from[2];   // x, w; NULL: is aligned
+    uint8_t* to[2];
+    int64_t stride[2];
+    uint32_t works[2], pieces;
+    int64_t inner;
+};
+__global__ __launch_bounds__(256) void k_align_rows(AlignArgs a)
+{
+    const uint32_t groups = (a.works[0] + 255) / 256, which = blockIdx.x >= groups;
+    const uint32_t work = (blockIdx.x - (which ? groups : 0)) * 256 + threadIdx.x;
+    if (work >= a.works[which]) return;
+    const int64_t row = work / a.pieces, c = (int64_t)(work % a.pieces) * 16;
+    const uint8_t* from = a.from[which] + row * a.stride[which];
+    v4i v;
+    if (c + 16 <= a.inner) {
+        const Shifted<1> any(from + c);
+        v = any.piece(any.load(0), 0);
+    } else {
+        v = load_piece(from, c, a.inner);
+    }
+    *(v4i*)(a.to[which] + (int64_t)work * 16) = v;
+}
+
+// Few rows of x (at most 16 MT): y is bound by the one read of w.  A wave reads 128 bytes of 16 rows of w per step, 32 per lane,
 // straight into the registers that the matrix instruction takes, and the same bytes of x; a workgroup's waves, and the
-// grid's second dimension, cut the inner dimension, and the sums meet in LDS.
+// grid's second dimension, cut the inner dimension, and the sums meet in LDS.  SHIFTED: rows that start anywhere.
 constexpr int kFewWaves = 8, kStep = 2 * kStage;
-template <int MT, int NT>
+template <int MT, bool SHIFTED>
 __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
 {
-    __shared__ __align__(16) v4i sums[kFewWaves][NT * MT][64];
+    __shared__ __align__(16) v4i sums[kFewWaves][MT][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t n0 = (int64_t)blockIdx.x * 16 * NT;
+    const int64_t n0 = (int64_t)blockIdx.x * 16;
     const int row = lane & 15, at = (lane >> 4) * 32;
-    const uint8_t *xp[MT], *wp[NT];
+    typedef Shifted<2> Any;
+    using Place = std::conditional_t<SHIFTED, Any, const uint8_t*>;
+    Place xp[MT], wp;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const int64_t m = i * 16 + row;
-        xp[i] = a.x + (m < a.rows ? m : a.rows - 1) * a.x_stride + at;
+        xp[i] = Place(a.x + (m < a.rows ? m : a.rows - 1) * a.x_stride + at);
     }
+    const uint8_t* w_row = a.w + (n0 + row < a.cols ? n0 + row : a.cols - 1) * a.w_stride;
+    wp = Place(w_row + at);
+    v4i sum[MT];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int64_t n = n0 + j * 16 + row;
-        wp[j] = a.w + (n < a.cols ? n : a.cols - 1) * a.w_stride + at;
-    }
-    v4i sum[NT][MT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) sum[j][i] = v4i{0, 0, 0, 0};
+    for (int i = 0; i < MT; ++i) sum[i] = v4i{0, 0, 0, 0};
     const int steps = (int)((a.inner + kStep - 1) / kStep), whole = (int)(a.inner / kStep);
     const int begin = blockIdx.y * (a.stages_per_split / 2);
     const int end = begin + a.stages_per_split / 2 < steps ? begin + a.stages_per_split / 2 : steps;
     const int end_whole = end < whole ? end : whole;
+    struct Plain {
+        v4i two[2];
+    };
+    using Bytes = std::conditional_t<SHIFTED, Any::Words, Plain>;   // 32 of a row, as they are loaded
     struct Step {
-        v4i w[NT][2], x[MT][2];
+        Bytes w, x[MT];
+    };
+    const auto load_one = [&](const Place& from, int64_t o) {
+        if constexpr (SHIFTED) {
+            return from.load(o);
+        } else {
+            Plain t;
+            __builtin_memcpy(t.two, from + o, 32);
+            return t;
+        }
+    };
+    const auto half_of = [&](const Place& from, const Bytes& t, int h) {
+        if constexpr (SHIFTED) return from.piece(t, h);
+        else return t.two[h];
     };
     const auto multiply = [&](const Step& t) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+            const v4i w = half_of(wp, t.w, h);
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) Matrix<true>::add(t.w[j][h], t.x[i][h], sum[j][i]);
+            for (int i = 0; i < MT; ++i) Matrix<true>::add(w, half_of(xp[i], t.x[i], h), sum[i]);
+        }
     };
     const auto load = [&](Step& t, int k) {
         const int64_t o = (int64_t)k * kStep;
+        t.w = load_one(wp, o);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) __builtin_memcpy(t.w[j], wp[j] + o, 32);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) __builtin_memcpy(t.x[i], xp[i] + o, 32);
+        for (int i = 0; i < MT; ++i) t.x[i] = load_one(xp[i], o);
     };
     // kAhead steps on their way at once, x at the distance of w: loads come back in order.  (The steady part by itself, with
     // no condition around its loads: behind one, the compiler waits for all of them.)
-    constexpr int kAhead = 16 / (MT + NT);
+    constexpr int kAhead = 16 / (MT + 1);
     Step ahead[kAhead];
     int k = begin + wave;
     if (k + (2 * kAhead - 1) * kFewWaves < end_whole) {
@@ -618,27 +697,25 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
             if (half * kAhead + d < left) multiply(ahead[d]);
     }
     if (end > end_whole && (end_whole - begin) % kFewWaves == wave) {   // the last step, where it is not whole
-        Step t;
-        const int64_t o = (int64_t)end_whole * kStep;
+        const int64_t o = (int64_t)end_whole * kStep + at;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            const v4i w = load_piece(w_row, o + h * 16, a.inner);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) t.w[j][h] = load_piece(wp[j] - at, o + at + h * 16, a.inner);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) t.x[i][h] = load_piece(xp[i] - at, o + at + h * 16, a.inner);
+            for (int i = 0; i < MT; ++i) {
+                const int64_t m = i * 16 + row;
+                Matrix<true>::add(w, load_piece(a.x + (m < a.rows ? m : a.rows - 1) * a.x_stride, o + h * 16, a.inner), sum[i]);
+            }
         }
-        multiply(t);
     }
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) sums[wave][j * MT + i][lane] = sum[j][i];
+    for (int i = 0; i < MT; ++i) sums[wave][i][lane] = sum[i];
     __syncthreads();
-    for (int t = wave; t < NT * MT; t += kFewWaves) {
+    for (int t = wave; t < MT; t += kFewWaves) {
         v4i s = sums[0][t][lane];
 #pragma unroll
         for (int k = 1; k < kFewWaves; ++k) s += sums[k][t][lane];
-        const int64_t m = t % MT * 16 + (lane & 15), n = n0 + t / MT * 16 + (lane >> 4) * 4;
+        const int64_t m = t * 16 + (lane & 15), n = n0 + (lane >> 4) * 4;
         float ws[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) ws[r] = scale_at(a.w_scale, n + r, a.cols);
@@ -850,7 +927,7 @@ constexpr int64_t kLeastSteps = 8;
 
 // The tile, and the splits of either product, of the least time by that table: what all compute units do together or what the
 // longest workgroup does, whichever is more, and the join of the splits.  Of 4096 x 4096 x 4096 tiles of 256 take 57 us, of 128 75, of
-// 64 122; of 1009 x 1003 x 1111 29, 11 and 6; the fp32 gradients of 1024 x 4096 x 1024 by 128 take 133 us, cut 93.
+// 64 122; of 1009 x 1003 x 1111 29, 11 and 6; both fp32 gradients of 1024 x 4096 x 1024 by 128 take 98 us, cut 78.
 Plan plan_of(const Shape& s, const Shape& t, bool int8)
 {
     Plan best = {};
@@ -898,17 +975,44 @@ bool loads_fit(const uint8_t* p, int64_t stride, int64_t rows, int64_t inner)
     return (uintptr_t)p % 16 == 0 && stride % 16 == 0 && stride * rows + inner < 0x7fffffff;
 }
 
+bool is_direct(const TileArgs& a, int tile)
+{
+    const int64_t last = a.inner / kStage - (int64_t)(a.splits - 1) * a.stages_per_split;   // whole stages of the last split
+    return last >= kRing && loads_fit(a.x, a.x_stride, tile, a.inner) && loads_fit(a.w, a.w_stride, tile, a.inner);
+}
+
+// The aligned copies that a product in tiles takes (none where it has fewer stages than k_tiles needs).
+struct Copies {
+    size_t x, w;   // bytes, 0: none
+};
+Copies copies_of(TileArgs a, const Plan& p, int64_t rows, int64_t cols)
+{
+    const int64_t stride = (a.inner + 15) / 16 * 16;
+    a.splits = p.splits[0];
+    a.stages_per_split = p.stages_per_split[0];
+    if (p.few || is_direct(a, p.tile) || rows * (stride / 16) > 0xffffff00 || cols * (stride / 16) > 0xffffff00) return {};
+    const bool x = !loads_fit(a.x, a.x_stride, p.tile, a.inner), w = !loads_fit(a.w, a.w_stride, p.tile, a.inner);
+    if (x) a.x = nullptr, a.x_stride = stride;   // (a place of any alignment)
+    if (w) a.w = nullptr, a.w_stride = stride;
+    if (!is_direct(a, p.tile)) return {};
+    return {x ? align256((size_t)rows * stride) : 0, w ? align256((size_t)cols * stride) : 0};
+}
+
 template <int MT>
 void run_few(const TileArgs& a, hipStream_t s)
 {
     // Measured, us: 4096 x 4096, k_few_rows / streamed: 1 row 5.0 / 5.2, 4 rows 5.4 / 5.2, 16 rows 6.4 / 5.5; 4096 x 1024: 3.2 / 3.8 for
-    // any; 4096 x 16384: 16 rows 19.1 / 17.1, 48 rows 31 / 22, 64 rows 39 / 25.
+    // any; 4096 x 16384: 16 rows 19.1 / 17.1, 48 rows 31 / 22, 64 rows 39 / 25.  Rows at odd addresses, 4096 x 16384: 1 row 18, 16 rows 24,
+    // 48 rows 41 (loaded as they lie 34, 39, 112).
     if (a.splits == 1 && a.rows > 2 && a.inner >= 4 * kFewWaves * kStage && loads_fit(a.x, a.x_stride, 64, a.inner) && loads_fit(a.w, a.w_stride, 16, a.inner)) {
         const int64_t tiles = (a.cols + 15) / 16;
         k_few_streamed<MT><<<dim3((uint32_t)(tiles < kUnits ? tiles : kUnits)), dim3(kFewWaves * 64), 0, s>>>(a);
         return;
     }
-    k_few_rows<MT, 1><<<dim3((uint32_t)((a.cols + 15) / 16), (uint32_t)a.splits), dim3(kFewWaves * 64), 0, s>>>(a);
+    const dim3 grid((uint32_t)((a.cols + 15) / 16), (uint32_t)a.splits);
+    const bool words = ((uintptr_t)a.x | (uintptr_t)a.w | (uint64_t)a.x_stride | (uint64_t)a.w_stride) % 4 == 0;
+    if (words) k_few_rows<MT, false><<<grid, dim3(kFewWaves * 64), 0, s>>>(a);
+    else k_few_rows<MT, true><<<grid, dim3(kFewWaves * 64), 0, s>>>(a);
 }
 
 template <int B, bool INT8>
@@ -939,11 +1043,7 @@ int run_products(TwoProducts both, const Plan& p, hipStream_t s)
         else if (p.few == 3) run_few<3>(both.first, s);
         else run_few<4>(both.first, s);
     } else {
-        const auto fits = [&](const TileArgs& a) {
-            const int64_t last = a.inner / kStage - (int64_t)(a.splits - 1) * a.stages_per_split;   // whole stages of the last split
-            return last >= kRing && loads_fit(a.x, a.x_stride, p.tile, a.inner) && loads_fit(a.w, a.w_stride, p.tile, a.inner);
-        };
-        const bool direct = fits(both.first) && (!both.second.rows || fits(both.second));
+        const bool direct = is_direct(both.first, p.tile) && (!both.second.rows || is_direct(both.second, p.tile));
         if (p.tile == 256) run_tiles<256, INT8>(both, direct, s);
         else if (p.tile == 128) run_tiles<128, INT8>(both, direct, s);
         else run_tiles<64, INT8>(both, direct, s);
@@ -963,7 +1063,8 @@ int run_products(TwoProducts both, const Plan& p, hipStream_t s)
 //     dx_left[m][term][n] = terms of g[m][n] w_scale[n] / dx_back[m],  dw_left[n][term][m] = terms of g[m][n] x_scale[m] / dw_back[n]
 //   w in tiles of 64 x 128: dx_right[k][n] = w[n][k] in fp16
 //   x in tiles of 64 x 128: dw_right[k][m] = x[m][k] in fp16
-// Rows of an output are padded to whole stages of 64 elements per term, with zeros.
+// Rows of an output are padded to whole stages of 64 elements per term, with zeros.  Bound by memory: 4096 x 4096 x 4096 bf16 reads 67
+// MB, writes 134 MB in 45 us (4.5 TB/s).
 constexpr int kSide = 64, kWide = 128;
 constexpr int kPeakWide = 64 * kChunk;     // columns that a wave looks at
 constexpr int kPeakBatch = 8;              // rows that it asks for at once
@@ -1011,6 +1112,7 @@ __device__ __forceinline__ void store_terms(const float (&v)[kChunk], f16* out, 
 
 // A wave takes eight rows of 512 columns at once, a lane eight columns of them; a workgroup's waves pass over its block's rows, then
 // over further columns.  What lies outside is the last row and the last columns once more: a maximum stays what it is.
+// Bound by memory, the block's rows all asked for at once: 4096 x 4096 bf16 in 16 us.
 // NARROW: g has fewer columns than a lane takes.
 template <typename T, bool NARROW>
 __global__ __launch_bounds__(kPeakWaves * 64) void k_grad_peaks(OperandArgs a)
@@ -1243,6 +1345,18 @@ GradLayout grad_layout(int64_t rows, int64_t cols, int64_t inner, int terms, boo
     return l;
 }
 
+Plan forward_plan(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t cols, int64_t inner, TileArgs* a)
+{
+    a->x = (const uint8_t*)x;
+    a->w = (const uint8_t*)w;
+    a->x_stride = x_stride;
+    a->w_stride = w_stride;
+    a->rows = rows;
+    a->cols = cols;
+    a->inner = inner;
+    return plan_of({rows, cols, inner}, Shape{}, true);
+}
+
 bool sizes_fit(int64_t rows, int64_t cols, int64_t inner)
 {
     return rows >= 1 && cols >= 1 && inner >= 1 && rows <= 0x3fffffff && cols <= 0x3fffffff && inner <= 131071;
@@ -1255,11 +1369,14 @@ using namespace geo_sc;
 
 extern "C" {
 
-int geo_sc_matmul_q8_workspace_size(int64_t rows, int64_t cols, int64_t inner, size_t* bytes)
+int geo_sc_matmul_q8_workspace_size(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t cols,
+                                    int64_t inner, size_t* bytes)
 {
-    if (!bytes || !sizes_fit(rows, cols, inner)) return GEO_SC_ERR_INVALID_ARGUMENT;
-    const Shape shape = {rows, cols, inner};
-    *bytes = partial_bytes(plan_of(shape, Shape{}, true), 0, shape);
+    if (!bytes || !sizes_fit(rows, cols, inner) || x_stride < 0 || w_stride < 0) return GEO_SC_ERR_INVALID_ARGUMENT;
+    TileArgs a = {};
+    const Plan plan = forward_plan(x, x_stride, w, w_stride, rows, cols, inner, &a);
+    const Copies copies = copies_of(a, plan, rows, cols);
+    *bytes = partial_bytes(plan, 0, {rows, cols, inner}) + copies.x + copies.w;
     return GEO_SC_OK;
 }
 
@@ -1269,25 +1386,36 @@ int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, co
 {
     if (!sizes_fit(rows, cols, inner) || !dtype_known(dtype) || x_stride < 0 || w_stride < 0 || !x || !w || !x_scale || !w_scale || !y)
         return GEO_SC_ERR_INVALID_ARGUMENT;
-    const Shape shape = {rows, cols, inner};
-    const Plan plan = plan_of(shape, Shape{}, true);
-    const size_t need = partial_bytes(plan, 0, shape);
-    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return GEO_SC_ERR_WORKSPACE;
     TwoProducts both = {};
     TileArgs& a = both.first;
-    a.x = (const uint8_t*)x;
-    a.w = (const uint8_t*)w;
-    a.x_stride = x_stride;
-    a.w_stride = w_stride;
-    a.rows = rows;
-    a.cols = cols;
-    a.inner = inner;
+    const Plan plan = forward_plan(x, x_stride, w, w_stride, rows, cols, inner, &a);
+    const size_t partial = partial_bytes(plan, 0, {rows, cols, inner});
+    const Copies copies = copies_of(a, plan, rows, cols);
+    const size_t need = partial + copies.x + copies.w;
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return GEO_SC_ERR_WORKSPACE;
+    if (copies.x || copies.w) {
+        AlignArgs g = {};
+        uint8_t* to = (uint8_t*)workspace + partial;
+        g.inner = inner;
+        g.pieces = (uint32_t)((inner + 15) / 16);
+        const auto copy = [&](int which, const uint8_t*& from, int64_t& stride, int64_t count, uint8_t* at) {
+            g.from[which] = from;
+            g.stride[which] = stride;
+            g.works[which] = (uint32_t)count * g.pieces;
+            g.to[which] = at;
+            from = at;
+            stride = (int64_t)g.pieces * 16;
+        };
+        if (copies.x) copy(0, a.x, a.x_stride, rows, to);
+        if (copies.w) copy(1, a.w, a.w_stride, cols, to + copies.x);
+        k_align_rows<<<dim3((g.works[0] + 255) / 256 + (g.works[1] + 255) / 256), dim3(256), 0, (hipStream_t)stream>>>(g);
+    }
     a.w_stages = 0x7fffffff;
     a.x_scale = x_scale;
     a.w_scale = w_scale;
     a.y = y;
     a.dtype = dtype;
-    a.partial = need ? (uint32_t*)workspace : nullptr;
+    a.partial = partial ? (uint32_t*)workspace : nullptr;
     return run_products<true>(both, plan, (hipStream_t)stream);
 }
 

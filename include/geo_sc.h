@@ -506,13 +506,15 @@ GEO_SC_API int geo_sc_rms_norm_q8_backward(const void* grad_values, int grad_dty
 /*
  * y[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] of 8-bit x (rows, inner) and w (cols, inner), y (rows, cols) of
  * dtype.  The sum is exact; inner at most 131071 (it then cannot pass 32 bits).  Workspace, 16-byte aligned:
- * geo_sc_matmul_q8_workspace_size, which may be 0.
+ * geo_sc_matmul_q8_workspace_size, which may be 0; of the operands it looks at the alignment only.  Rows at multiples of 16 bytes
+ * are taken as they lie, others are laid out anew in the workspace where more than 64 rows meet them.
  * Backward, straight through the rounding of either operand, from g, the gradient of y: dx = (g w_scale) w of (rows, inner),
- * dw = (g x_scale)^T x of (cols, inner); either may be NULL.  The 8-bit operand enters exactly, the scaled gradient as one bf16
- * number where g is bf16, as the sum of two where it is fp16, of three where it is fp32; sums in fp32.  cols at most
- * 131071.
+ * dw = (g x_scale)^T x of (cols, inner); either may be NULL.  The 8-bit operand enters exactly, the scaled gradient, each of its
+ * rows brought to fp16's range by a power of two, as one fp16 number where g is bf16 and as the sum of two where it is fp16 or
+ * fp32; sums in fp32.  cols at most 131071.
  */
-GEO_SC_API int geo_sc_matmul_q8_workspace_size(int64_t rows, int64_t cols, int64_t inner, size_t* bytes);
+GEO_SC_API int geo_sc_matmul_q8_workspace_size(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows,
+                                               int64_t cols, int64_t inner, size_t* bytes);
 GEO_SC_API int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
                                 const float* w_scale, int64_t rows, int64_t cols, int64_t inner, void* y, int dtype, void* workspace,
                                 size_t workspace_bytes, geo_sc_stream_t stream);

@@ -52,10 +52,16 @@ def test_rms_norm_refuses(lib):
 def test_matmul_refuses(lib):
     size = ctypes.c_size_t()
     for sizes in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1, 1, 131072), (1 << 31, 1, 1)):
-        assert lib.geo_sc_matmul_q8_workspace_size(*sizes, ctypes.byref(size)) == INVALID
+        assert lib.geo_sc_matmul_q8_workspace_size(P, 4096, P, 4096, *sizes, ctypes.byref(size)) == INVALID
         assert lib.geo_sc_matmul_q8_backward_workspace_size(*sizes, 0, 1, 1, ctypes.byref(size)) == INVALID
     # few workgroups and a long inner dimension: cut, with partial sums
-    assert lib.geo_sc_matmul_q8_workspace_size(100, 130, 65536, ctypes.byref(size)) == 0 and size.value >= 2 * 100 * 130 * 4
+    assert lib.geo_sc_matmul_q8_workspace_size(P, 65536, P, 65536, 100, 130, 65536, ctypes.byref(size)) == 0 and size.value >= 2 * 100 * 130 * 4
+    assert lib.geo_sc_matmul_q8_workspace_size(P, -1, P, 4096, 100, 130, 4096, ctypes.byref(size)) == INVALID
+    # rows at odd addresses are laid out anew, but not for few rows
+    cut = size.value
+    assert lib.geo_sc_matmul_q8_workspace_size(P, 65537, P, 65536, 100, 130, 65536, ctypes.byref(size)) == 0 and size.value >= cut + 100 * 65536
+    assert lib.geo_sc_matmul_q8_workspace_size(P, 65536, P + 1, 65536, 100, 130, 65536, ctypes.byref(size)) == 0 and size.value >= cut + 130 * 65536
+    assert lib.geo_sc_matmul_q8_workspace_size(P, 4095, P, 4095, 3, 4096, 4095, ctypes.byref(size)) == 0 and size.value == 0
     good = [P, 4096, P, P, 4096, P, 100, 130, 65536, P, 1, P, 1 << 30, None]
     for at, bad, status in ((0, None, INVALID), (1, -1, INVALID), (2, None, INVALID), (3, None, INVALID), (4, -1, INVALID), (5, None, INVALID),
                             (6, 0, INVALID), (7, 0, INVALID), (8, 131072, INVALID), (9, None, INVALID), (10, 4, INVALID),

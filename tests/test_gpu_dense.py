@@ -272,6 +272,20 @@ def test_product_of_other_strides_and_alignments(uf):
     assert uf.matmul_q8(q[:0], s[:0], wq, ws).shape == (0, 140)
 
 
+@pytest.mark.parametrize("m", [1, 3, 16, 17, 40, 64, 65, 200])
+@pytest.mark.parametrize("lo,hi", [(0, 4099), (1, 4099), (2, 4094), (3, 4096), (0, 2051), (5, 261), (7, 700)])
+def test_product_of_rows_at_odd_addresses(uf, m, lo, hi):
+    """few rows and tiles, either operand alone and both, the memory's first and last bytes among them"""
+    g = torch.Generator().manual_seed(7)
+    q, wq = (torch.randint(-127, 128, (r, 4099), generator=g).to(torch.int8).cuda() for r in (m, 130))
+    s, ws = rand(m, seed=1).abs(), rand(130, seed=2).abs()
+    a, b = q[:, lo:hi], wq[:, lo:hi]
+    aligned = [torch.nn.functional.pad(t, (0, -(hi - lo) % 16))[:, :hi - lo] for t in (a, b)]
+    want = product64(a, s, b, ws)
+    for left, right in ((a, b), (a, aligned[1]), (aligned[0], b), (a.contiguous(), b.contiguous())):
+        close(uf.matmul_q8(left, s, right, ws), want, 5 * U * want.abs())
+
+
 def test_product_of_rows_that_are_no_numbers(uf):
     x = rand(70, 40, seed=1)
     x[3, 4], x[66, 0] = float("nan"), float("inf")
