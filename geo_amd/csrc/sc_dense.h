@@ -20,31 +20,46 @@ inline bool dtype_known(int dtype) { return dtype == GEO_SC_F32 || dtype == GEO_
 // so odd row lengths and strides keep the wide accesses.
 constexpr int kChunk = 8;
 
-template <typename T>
+// ONCE: see reads_once().  (A choice at run time breaks the row of loads: 8191 x 4096 bf16 normed, both passes, 133 us, so 121.)
+template <bool ONCE, typename T>
+__device__ __forceinline__ void fetch_whole(const T* p, T (&raw)[kChunk])
+{
+    typedef int Piece __attribute__((ext_vector_type(4), aligned(2)));
+    if constexpr (ONCE) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof raw / 16; ++i) {
+            const Piece u = __builtin_nontemporal_load((const Piece*)p + i);
+            __builtin_memcpy((char*)raw + 16 * i, &u, 16);
+        }
+    } else {
+        __builtin_memcpy(raw, p, sizeof raw);
+    }
+}
+template <bool ONCE = false, typename T>
 __device__ __forceinline__ void load_chunk(const T* p, float (&v)[kChunk])
 {
     T raw[kChunk];
-    __builtin_memcpy(raw, p, sizeof raw);
+    fetch_whole<ONCE>(p, raw);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) v[j] = (float)raw[j];
 }
 // the chunk at column c of a row of `cols` columns; `fill` behind the row's end
-template <typename T>
+template <bool ONCE = false, typename T>
 __device__ __forceinline__ void load_chunk(const T* row, int64_t c, int64_t cols, float fill, float (&v)[kChunk])
 {
     if (c + kChunk <= cols) {
-        load_chunk(row + c, v);
+        load_chunk<ONCE>(row + c, v);
         return;
     }
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) v[j] = c + j < cols ? (float)row[c + j] : fill;
 }
 // the same as it lies in memory, zeros behind the row's end: what is converted later need not be waited for at the load
-template <typename T>
+template <bool ONCE, typename T>
 __device__ __forceinline__ void fetch_chunk(const T* row, int64_t c, int64_t cols, T (&raw)[kChunk])
 {
     if (c + kChunk <= cols) {
-        __builtin_memcpy(raw, row + c, sizeof raw);
+        fetch_whole<ONCE>(row + c, raw);
         return;
     }
 #pragma unroll
@@ -74,6 +89,13 @@ __device__ __forceinline__ void store_chunk(T* row, int64_t c, int64_t cols, con
 #pragma unroll
     for (int j = 0; j < kChunk; ++j)
         if (c + j < cols) row[c + j] = raw[j];
+}
+// Whether rows that a kernel reads once are read past what the caches hold for others.  8191 x 4096 bf16 normed, both passes, 161 us
+// -> 121, 16384 x 4096 fp32 rows in 8 bits 82 -> 74.  Not where lines are shared by loads that straddle words (8192 x 2047 bf16,
+// 136 -> 145), or by the two loads of a chunk of fp32 at odd places (8192 x 4095, 226 -> 237).
+inline bool reads_once(int dtype, const void* p, int64_t stride)
+{
+    return !(((uintptr_t)p | (uint64_t)(stride * dtype_bytes(dtype))) % (dtype == GEO_SC_F32 ? 16 : 4));
 }
 // Whether a kernel's output goes past the caches.  What passes half of the 256 MB that the memory side caches is not found there by
 // the next kernel anyway, and in them it drives out what is read: 8191 x 4096 bf16 rows normed (134 MB of sum and

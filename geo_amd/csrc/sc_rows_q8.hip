@@ -11,6 +11,8 @@
 //   u = g w,   dt = r (u - t r^2 mean(u t)) + h,   dx = dresidual = dt,   dw = sum over the rows of g t r
 // t is formed again from x and residual: the sum that the forward returns is rounded to their type, which would show in dw
 // (bf16: 2.5e-3 of its size, where its own rounding is 1.7e-3).
+#include <type_traits>
+
 #include "sc_dense.h"
 
 namespace geo_sc {
@@ -47,14 +49,14 @@ struct RowsArgs {
     bool streamed;   // total and values
 };
 
-template <typename T, bool NORM>
+template <typename T, bool NORM, bool ONCE>
 __device__ __forceinline__ void read_chunk(const RowsArgs& a, int64_t row, int64_t c, float (&t)[kChunk])
 {
-    load_chunk((const T*)a.x + row * a.x_stride, c, a.cols, 0.f, t);
+    load_chunk<ONCE>((const T*)a.x + row * a.x_stride, c, a.cols, 0.f, t);
     if constexpr (NORM) {
         if (a.residual) {
             float s[kChunk];
-            load_chunk((const T*)a.residual + row * a.residual_stride, c, a.cols, 0.f, s);
+            load_chunk<ONCE>((const T*)a.residual + row * a.residual_stride, c, a.cols, 0.f, s);
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) t[j] += s[j];
         }
@@ -89,7 +91,7 @@ __device__ __forceinline__ float row_unit(const RowsArgs& a, float squares) { re
 // One row per threadIdx.y; the row's blockDim.x threads hold ITEMS chunks of eight columns each in registers from the only read to
 // the write.  (Blocks that stay, go on to further rows and ask for the next one ahead took 91 us where these take 84,
 // 8191 x 4096 bf16 with residual, total and values: new blocks hide a row's reduction better.)
-template <typename T, bool NORM, int ITEMS>
+template <typename T, bool NORM, int ITEMS, bool ONCE>
 __global__ __launch_bounds__(1024) void k_rows(RowsArgs a)
 {
     __shared__ RowSlots slots;
@@ -102,7 +104,7 @@ __global__ __launch_bounds__(1024) void k_rows(RowsArgs a)
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
         if (column(i) < a.cols) {
-            read_chunk<T, NORM>(a, row, column(i), n[i]);
+            read_chunk<T, NORM, ONCE>(a, row, column(i), n[i]);
             if constexpr (NORM) {
                 if (a.total && a.residual) store_chunk((T*)a.total + row * a.cols, column(i), a.cols, n[i], a.streamed);
                 float w[kChunk];
@@ -137,7 +139,7 @@ __global__ __launch_bounds__(1024) void k_rows_long(RowsArgs a)
     float n[kChunk], squares = 0.f;
     uint32_t most = 0;
     const auto take = [&](int64_t c, bool write_total) {
-        read_chunk<T, NORM>(a, row, c, n);
+        read_chunk<T, NORM, false>(a, row, c, n);
         if constexpr (NORM) {
             if (write_total && a.total && a.residual) store_chunk((T*)a.total + row * a.cols, c, a.cols, n, a.streamed);
             float w[kChunk];
@@ -177,6 +179,8 @@ int threads_of_row(int64_t chunks, int held)
 template <typename T, bool NORM>
 int run_rows(RowsArgs a, hipStream_t s)
 {
+    constexpr int dtype = std::is_same_v<T, f32> ? GEO_SC_F32 : std::is_same_v<T, bf16> ? GEO_SC_BF16 : GEO_SC_F16;
+    const bool once = reads_once(dtype, a.x, a.x_stride) && (!a.residual || reads_once(dtype, a.residual, a.residual_stride));
     a.streamed = streams(a.rows * a.cols * ((a.total && a.residual ? (int64_t)sizeof(T) : 0) + (a.values ? dtype_bytes(a.values_dtype) : 0)));
     const int64_t chunks = (a.cols + kChunk - 1) / kChunk;
     // Two chunks per thread where there are rows enough to fill the compute units: half as many waves reduce a row.  8191 x 4096
@@ -184,9 +188,13 @@ int run_rows(RowsArgs a, hipStream_t s)
     const int threads = threads_of_row(chunks, a.rows >= 2048 && chunks > 64 ? 2 : 1), per_block = threads == 64 ? 4 : 1;
     const int64_t items = (chunks + threads - 1) / threads;
     const dim3 grid((uint32_t)((a.rows + per_block - 1) / per_block)), block(threads, per_block);
-    if (items <= 1) k_rows<T, NORM, 1><<<grid, block, 0, s>>>(a);
-    else if (items <= 2) k_rows<T, NORM, 2><<<grid, block, 0, s>>>(a);
-    else if (items <= 4) k_rows<T, NORM, 4><<<grid, block, 0, s>>>(a);
+    const auto held = [&](auto count) {
+        if (once) k_rows<T, NORM, count(), true><<<grid, block, 0, s>>>(a);
+        else k_rows<T, NORM, count(), false><<<grid, block, 0, s>>>(a);
+    };
+    if (items <= 1) held(std::integral_constant<int, 1>());
+    else if (items <= 2) held(std::integral_constant<int, 2>());
+    else if (items <= 4) held(std::integral_constant<int, 4>());
     else k_rows_long<T, NORM><<<dim3((uint32_t)a.rows), dim3(1024), 0, s>>>(a);
     return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
 }
@@ -208,6 +216,7 @@ struct NormBackArgs {
     const float* rstd;
     void *dx;
     bool streamed;    // dx
+    bool once;        // what is read
     float* partial;   // [blocks][cols]: sums of the weight's gradient, NULL: not wanted
 };
 
@@ -215,7 +224,7 @@ struct NormBackArgs {
 // registers that it needs cost a block per compute unit.)
 // A block takes every gridDim.x-th row; its threads keep the weight and their columns' sums of the weight's gradient in
 // registers over all rows of the block.
-template <typename T, typename G, int ITEMS>
+template <typename T, typename G, int ITEMS, bool ONCE>
 __global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs a)
 {
     __shared__ RowSlots slots;
@@ -238,10 +247,10 @@ __global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs a)
             if (column(i) < a.cols) {
                 G grad[kChunk];
                 T x[kChunk], residual[kChunk] = {}, also[kChunk] = {};
-                fetch_chunk((const G*)a.grad_values + row * a.grad_stride, column(i), a.cols, grad);
-                fetch_chunk((const T*)a.x + row * a.x_stride, column(i), a.cols, x);
-                if (a.residual) fetch_chunk((const T*)a.residual + row * a.residual_stride, column(i), a.cols, residual);
-                if (a.grad_total) fetch_chunk((const T*)a.grad_total + row * a.grad_total_stride, column(i), a.cols, also);
+                fetch_chunk<ONCE>((const G*)a.grad_values + row * a.grad_stride, column(i), a.cols, grad);
+                fetch_chunk<ONCE>((const T*)a.x + row * a.x_stride, column(i), a.cols, x);
+                if (a.residual) fetch_chunk<ONCE>((const T*)a.residual + row * a.residual_stride, column(i), a.cols, residual);
+                if (a.grad_total) fetch_chunk<ONCE>((const T*)a.grad_total + row * a.grad_total_stride, column(i), a.cols, also);
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
                     g[i][j] = (float)grad[j];
@@ -375,8 +384,12 @@ void run_norm_back_held(const NormBackArgs& a, int64_t blocks, hipStream_t s)
 {
     const int64_t chunks = (a.cols + kChunk - 1) / kChunk;
     const int threads = threads_of_row(chunks, 1);
-    if (chunks <= threads) k_norm_back<T, G, 1><<<dim3((uint32_t)blocks), dim3(threads), 0, s>>>(a);
-    else k_norm_back<T, G, 2><<<dim3((uint32_t)blocks), dim3(threads), 0, s>>>(a);
+    const auto held = [&](auto count) {
+        if (a.once) k_norm_back<T, G, count(), true><<<dim3((uint32_t)blocks), dim3(threads), 0, s>>>(a);
+        else k_norm_back<T, G, count(), false><<<dim3((uint32_t)blocks), dim3(threads), 0, s>>>(a);
+    };
+    if (chunks <= threads) held(std::integral_constant<int, 1>());
+    else held(std::integral_constant<int, 2>());
 }
 
 template <typename T>
@@ -461,8 +474,11 @@ int geo_sc_rms_norm_q8_backward(const void* grad_values, int grad_dtype, int64_t
     size_t need = 0;
     geo_sc_rms_norm_q8_backward_workspace_size(rows, cols, &need);
     if (dweight && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 4)) return GEO_SC_ERR_WORKSPACE;
+    const bool once = reads_once(dtype, x, x_stride) && (!residual || reads_once(dtype, residual, residual_stride)) &&
+                      reads_once(grad_dtype, grad_values, grad_stride) && (!grad_total || reads_once(dtype, grad_total, grad_total_stride));
     const NormBackArgs a = {grad_values, grad_total, x, residual, weight, grad_dtype, rows, cols, grad_stride, grad_total_stride,
-                            x_stride, residual_stride, rstd, dx, streams(rows * cols * dtype_bytes(dtype)), dweight ? (float*)workspace : nullptr};
+                            x_stride, residual_stride, rstd, dx, streams(rows * cols * dtype_bytes(dtype)), once,
+                            dweight ? (float*)workspace : nullptr};
     hipStream_t s = (hipStream_t)stream;
     if (dtype == GEO_SC_F32) return run_norm_back<f32>(a, (f32*)dweight, s);
     if (dtype == GEO_SC_BF16) return run_norm_back<bf16>(a, (bf16*)dweight, s);
