@@ -417,6 +417,8 @@ __device__ __forceinline__ void finish_tile(const Spot& p, typename Matrix<INT8>
 // kRing stages: while a wave multiplies stage s out of registers, stage s + 1 moves from LDS to its other registers and the stages
 // up to s + kRing are on their way.  One barrier per stage: it says that every wave's share of stage s + 1 has come and
 // that all have read stage s, whose place stage s + kRing takes.
+// Bound by power: 8192 x 16384 x 4096 in 448 us (2.46 POP/s) at 1.95 GHz, where the products alone run at 2.17; both gradients of
+// 4096 x 4096 x 4096 bf16 in 200 us (1.37 PFLOP/s).
 template <int B, bool INT8>
 __global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)
 {
@@ -727,7 +729,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
 // order of the matrix instruction's operands give neighbouring lanes different rows, and the memory pipeline takes such a load's
 // lanes one by one (4096 x 16384 bytes of w: 16 us for 16 rows of x, 31 for 48).  Here each wave has a ring of its own in LDS, which
 // the loads fill in lines, and no barrier but where the waves' sums meet.  Workgroups stay: a wave's stages run on from one
-// 16 columns of y to its next, so that w streams.
+// 16 columns of y to its next, so that w streams.  48 rows by 4096 x 16384 in 21.5 us: 3.1 TB/s of w, and x three times as much out of L2.
 template <int MT>
 __global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a)
 {
@@ -860,7 +862,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a)
         });
 }
 
-// y from the sums of the splits, of both products of a launch
+// y from the sums of the splits, of both products of a launch: memory, and 3 us at the least
 template <bool INT8>
 __global__ __launch_bounds__(256) void k_join_splits(TwoProducts both)
 {
