@@ -5,10 +5,12 @@
 //
 // r is common to a row, so it cancels in q: q_j = round(t_j w_j * 127 / max|t w|) and scale = max|t w| r / 127.  The sum of
 // squares and the maximum then need one pass and one exchange between the row's waves, and the row stays in registers
-// from its only read to its only write.
+// from its only read to its only write.  Where the squares or the products pass the range of fp32 the row is read again and taken
+// times a power of two, which cancels in q alike (in_range, scaled_row).
 //
 // Backward of the norm, straight through the rounding, with g the gradient of the values and h that of the sum:
-//   u = g w,   dt = r (u - t r^2 mean(u t)) + h,   dx = dresidual = dt,   dw = sum over the rows of g t r
+//   u = g w,   dt = r (u - t r mean(u t r)) + h,   dx = dresidual = dt,   dw = sum over the rows of g t r
+// (t r is at most the root of the columns: no product with it passes the range that u has.)
 // t is formed again from x and residual: the sum that the forward returns is rounded to their type, which would show in dw
 // (bf16: 2.5e-3 of its size, where its own rounding is 1.7e-3).
 #include <type_traits>
@@ -88,6 +90,32 @@ __device__ __forceinline__ void write_chunk(const RowsArgs& a, int64_t row, int6
 
 __device__ __forceinline__ float row_unit(const RowsArgs& a, float squares) { return 1.f / sqrtf(squares / (float)a.cols + a.eps); }
 
+// Whether sums of squares and products with the weight, formed as they are, lost nothing to infinity or to zero.  (A row of zeros
+// counts as outside: it looks like one whose squares and products vanished.)
+__device__ __forceinline__ bool in_range(const RowsArgs& a, float squares, uint32_t most)
+{
+    return squares < __uint_as_float(kInfinityBits) && squares + a.eps * (float)a.cols > 0x1p-64f && most < kInfinityBits &&
+           most >= __float_as_uint(0x1p-100f);
+}
+// The power of two that brings the largest magnitude, which is a number and not zero, to 1 .. 4 (denormals less far).
+__device__ __forceinline__ float power_up(uint32_t peak)
+{
+    const int field = 254 - (int)(peak >> 23);
+    return __uint_as_float((uint32_t)(field < 1 ? 1 : field > 253 ? 253 : field) << 23);
+}
+// r of a row, and r / up, the factor of t up, from the sum of the squares of t up.  Where eps up^2 is beyond all squares r is eps's alone.
+__device__ __forceinline__ void scaled_units(const RowsArgs& a, float squares, float up, float& unit, float& factor)
+{
+    const float eps = a.eps * up * up;
+    if (eps < 0x1p100f) {
+        factor = 1.f / sqrtf(squares / (float)a.cols + eps);
+        unit = factor * up;
+    } else {
+        unit = 1.f / sqrtf(a.eps);
+        factor = unit * (1.f / up);
+    }
+}
+
 // One row per threadIdx.y; the row's blockDim.x threads hold ITEMS chunks of eight columns each in registers from the only read to
 // the write.  Bound by memory: 16384 x 4096 fp32 to q and bf16 values 403 MB in 73 us, 8191 x 4096 bf16 with residual to q, sum and
 // values 302 MB in 59 (5.5 and 5.1 TB/s).  (Blocks that stay, go on to further rows and ask for the next one ahead: 91 us for
@@ -120,8 +148,43 @@ __global__ __launch_bounds__(1024) void k_rows(RowsArgs a)
             for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(n[i][j]));
         }
     row_reduce(squares, most, waves, slots, 0);
-    const float unit = NORM ? row_unit(a, squares) : 1.f;
-    const RowScale rs = row_scale(most, unit, !NORM || squares < __uint_as_float(kInfinityBits));
+    float unit = NORM ? row_unit(a, squares) : 1.f, factor = unit;
+    bool sound = true;
+    if (NORM && __builtin_expect(!in_range(a, squares, most), false)) {   // (all threads of a row alike)
+        uint32_t peak = 0;
+        float none = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < ITEMS; ++i)
+            if (column(i) < a.cols) {
+                read_chunk<T, NORM, false>(a, row, column(i), n[0]);
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) peak = max(peak, magnitude_bits(n[0][j]));
+            }
+        row_reduce(none, peak, waves, slots, 1);
+        sound = peak < kInfinityBits;
+        if (sound && peak) {
+            const float up = power_up(peak);
+            squares = 0.f;
+            most = 0;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (column(i) < a.cols) {
+                    read_chunk<T, NORM, false>(a, row, column(i), n[i]);
+                    float w[kChunk];
+                    load_chunk((const T*)a.weight, column(i), a.cols, 0.f, w);
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) {
+                        n[i][j] *= up;
+                        squares += n[i][j] * n[i][j];
+                        n[i][j] *= w[j];
+                        most = max(most, magnitude_bits(n[i][j]));
+                    }
+                }
+            row_reduce(squares, most, waves, slots, 0);
+            scaled_units(a, squares, up, unit, factor);
+        }
+    }
+    const RowScale rs = row_scale(most, factor, sound);
     if (t == 0) {
         a.scale[row] = rs.scale;
         if (NORM && a.rstd) a.rstd[row] = unit;
@@ -138,7 +201,7 @@ __global__ __launch_bounds__(1024) void k_rows_long(RowsArgs a)
 {
     __shared__ RowSlots slots;
     const int64_t row = blockIdx.x, first = (int64_t)threadIdx.x * kChunk, step = (int64_t)blockDim.x * kChunk;
-    float n[kChunk], squares = 0.f;
+    float n[kChunk], squares = 0.f, up = 1.f;
     uint32_t most = 0;
     const auto take = [&](int64_t c, bool write_total) {
         read_chunk<T, NORM, false>(a, row, c, n);
@@ -148,19 +211,42 @@ __global__ __launch_bounds__(1024) void k_rows_long(RowsArgs a)
             load_chunk((const T*)a.weight, c, a.cols, 0.f, w);
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
+                n[j] *= up;
                 squares += n[j] * n[j];
                 n[j] *= w[j];
             }
         }
     };
-    for (int64_t c = first; c < a.cols; c += step) {
-        take(c, true);
+    const auto scan = [&](bool write_total) {
+        squares = 0.f;
+        most = 0;
+        for (int64_t c = first; c < a.cols; c += step) {
+            take(c, write_total);
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(n[j]));
+            for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(n[j]));
+        }
+        row_reduce(squares, most, blockDim.x >> 6, slots, 0);
+    };
+    scan(true);
+    float unit = NORM ? row_unit(a, squares) : 1.f, factor = unit;
+    bool sound = true;
+    if (NORM && __builtin_expect(!in_range(a, squares, most), false)) {
+        uint32_t peak = 0;
+        float none = 0.f;
+        for (int64_t c = first; c < a.cols; c += step) {
+            read_chunk<T, NORM, false>(a, row, c, n);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) peak = max(peak, magnitude_bits(n[j]));
+        }
+        row_reduce(none, peak, blockDim.x >> 6, slots, 1);
+        sound = peak < kInfinityBits;
+        if (sound && peak) {
+            up = power_up(peak);
+            scan(false);
+            scaled_units(a, squares, up, unit, factor);
+        }
     }
-    row_reduce(squares, most, blockDim.x >> 6, slots, 0);
-    const float unit = NORM ? row_unit(a, squares) : 1.f;
-    const RowScale rs = row_scale(most, unit, !NORM || squares < __uint_as_float(kInfinityBits));
+    const RowScale rs = row_scale(most, factor, sound);
     if (threadIdx.x == 0) {
         a.scale[row] = rs.scale;
         if (NORM && a.rstd) a.rstd[row] = unit;
@@ -256,16 +342,16 @@ __global__ __launch_bounds__(1024) void k_norm_back(NormBackArgs a)
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
                     g[i][j] = (float)grad[j];
-                    v[i][j] = (float)x[j] + (float)residual[j];
+                    v[i][j] = ((float)x[j] + (float)residual[j]) * unit;
                     h[i][j] = (float)also[j];
-                    dw[i][j] += g[i][j] * (v[i][j] * unit);
+                    dw[i][j] += g[i][j] * v[i][j];
                     g[i][j] *= w[i][j];
                     along += g[i][j] * v[i][j];
                 }
             }
         uint32_t none = 0;
         row_reduce(along, none, waves, slots, turn);
-        const float back = along / (float)a.cols * unit * unit;
+        const float back = along / (float)a.cols;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
             if (column(i) < a.cols) {
@@ -312,7 +398,10 @@ __global__ __launch_bounds__(1024) void k_norm_back_long(NormBackArgs a)
         load_sum<T>(a, row, c, v);
         load_chunk((const T*)a.weight, c, a.cols, 0.f, w);
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) g[j] *= w[j];
+        for (int j = 0; j < kChunk; ++j) {
+            v[j] *= r;
+            g[j] *= w[j];
+        }
     };
     for (int64_t c = first; c < a.cols; c += step) {
         take(c);
@@ -321,7 +410,7 @@ __global__ __launch_bounds__(1024) void k_norm_back_long(NormBackArgs a)
     }
     uint32_t none = 0;
     row_reduce(along, none, waves, slots, 0);
-    const float back = along / (float)a.cols * r * r;
+    const float back = along / (float)a.cols;
     for (int64_t c = first; c < a.cols; c += step) {
         take(c);
 #pragma unroll

@@ -483,6 +483,7 @@ GEO_SC_API int geo_sc_quantize_rows(const void* x, int dtype, int64_t rows, int6
 /*
  * Root-mean-square norm of x + residual with 8-bit output: t = x + residual, r = 1 / sqrt(mean_j t[j]^2 + eps),
  * (q, scale) = rows in 8 bits of t[j] r weight[j].  One pass; fp32 inside, t is rounded for `total` only.
+ * Rows of any finite t: where squares or t weight pass fp32's range they are formed from t times a power of two.
  *   residual        NULL: none
  *   total           (rows, cols) of dtype: t; NULL: not wanted (nothing is written without a residual: t is x)
  *   values          NULL, or (rows, cols) of values_dtype: q * scale
