@@ -117,6 +117,15 @@ __device__ __forceinline__ void load_chunk(const void* base, int dtype, int64_t 
     else load_chunk((const f16*)base + offset, c, cols, fill, v);
 }
 
+// Calls launch(first, count) for consecutive shares of `groups` workgroups of `threads`: a launch counts its threads in 32 bits, and
+// one of more starts what the count leaves of them, without an error.
+template <typename F>
+void in_launches(int64_t groups, int threads, F launch)
+{
+    const int64_t most = 0xffffffffll / threads;
+    for (int64_t first = 0; first < groups; first += most) launch(first, (uint32_t)(groups - first < most ? groups - first : most));
+}
+
 // Bits of |v|: as unsigned integers they order like the magnitudes, with infinity above every number and NaN above infinity,
 // so their maximum is the largest magnitude where all are numbers and says where one is not.
 __device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }

@@ -324,16 +324,32 @@ int threads_of(int64_t cols)
     return threads;
 }
 
+// the rows from `first` on, of what forward and backward have in common
 template <typename T>
-int run_distill(DistillArgs a, int reduction, float* result, hipStream_t s)
+DistillArgs rows_from(DistillArgs a, int64_t first)
+{
+    a.rows -= first;
+    a.z = (const T*)a.z + first * a.z_stride;
+    a.stats += first * kStats;
+    a.top_logits = (const char*)a.top_logits + first * a.top * dtype_bytes(a.top_dtype);
+    a.top_index = (const char*)a.top_index + first * a.top * (a.index64 ? 8 : 4);
+    return a;
+}
+
+template <typename T>
+int run_distill(const DistillArgs& a, int reduction, float* result, hipStream_t s)
 {
     const int threads = threads_of(a.per_split), per_block = threads == 64 ? 4 : 1;
     if (a.splits == 1) {
-        // (fp32 gains nothing: 4096 x 32768 with the gradient 339 us, read like any other 329)
-        const dim3 grid((uint32_t)((a.rows + per_block - 1) / per_block)), block(threads, per_block);
-        if constexpr (std::is_same_v<T, f32>) k_distill_rows<T, false><<<grid, block, 0, s>>>(a);
-        else if (reads_once(GEO_SC_BF16, a.z, a.z_stride)) k_distill_rows<T, true><<<grid, block, 0, s>>>(a);
-        else k_distill_rows<T, false><<<grid, block, 0, s>>>(a);
+        const dim3 block(threads, per_block);
+        in_launches((a.rows + per_block - 1) / per_block, threads, [&](int64_t first, uint32_t grid) {
+            DistillArgs b = rows_from<T>(a, first * per_block);
+            b.loss = a.loss + first * per_block;
+            // (fp32 gains nothing: 4096 x 32768 with the gradient 339 us, read like any other 329)
+            if constexpr (std::is_same_v<T, f32>) k_distill_rows<T, false><<<grid, block, 0, s>>>(b);
+            else if (reads_once(GEO_SC_BF16, a.z, a.z_stride)) k_distill_rows<T, true><<<grid, block, 0, s>>>(b);
+            else k_distill_rows<T, false><<<grid, block, 0, s>>>(b);
+        });
     } else {
         k_distill_split<T><<<dim3((uint32_t)a.splits, (uint32_t)a.rows), dim3(threads), 0, s>>>(a);
         k_distill_join<T><<<dim3((uint32_t)a.rows), dim3(64), 0, s>>>(a);
@@ -347,14 +363,10 @@ int run_distill_back(const DistillArgs& a, hipStream_t s)
 {
     const int threads = threads_of(a.per_split), per_block = threads == 64 ? 4 : 1;
     for (int64_t r = 0; r < a.rows; r += 65535 * (int64_t)per_block) {   // rows are the grid's second dimension
-        DistillArgs b = a;
-        b.rows = a.rows - r < 65535 * (int64_t)per_block ? a.rows - r : 65535 * (int64_t)per_block;
-        b.z = (const T*)a.z + r * a.z_stride;
+        DistillArgs b = rows_from<T>(a, r);
+        if (b.rows > 65535 * (int64_t)per_block) b.rows = 65535 * (int64_t)per_block;
         b.dz = (T*)a.dz + r * a.cols;
-        b.stats = a.stats + r * kStats;
         b.grad = a.grad + (a.grad_per_row ? r : 0);
-        b.top_logits = (const char*)a.top_logits + r * a.top * dtype_bytes(a.top_dtype);
-        b.top_index = (const char*)a.top_index + r * a.top * (a.index64 ? 8 : 4);
         k_distill_back<T><<<dim3((uint32_t)a.splits, (uint32_t)((b.rows + per_block - 1) / per_block)), dim3(threads, per_block),
                             (size_t)per_block * a.top * sizeof(int32_t), s>>>(b);
     }

@@ -29,6 +29,7 @@ constexpr int kStage = 64;    // bytes of the inner dimension per stage: one mat
 template <int N>
 using Int = std::integral_constant<int, N>;
 constexpr int kUnits = 256;   // compute units
+constexpr int64_t kMostGroups = 0xfffffe;   // workgroups of 256 threads in a launch, which counts threads in 32 bits
 
 struct TileArgs {
     const uint8_t *x, *w;              // rows of `inner` bytes each
@@ -611,11 +612,11 @@ __global__ __launch_bounds__(256) void k_align_rows(AlignArgs a)
 // grid's second dimension, cut the inner dimension, and the sums meet in LDS.  SHIFTED: rows that start anywhere.
 constexpr int kFewWaves = 8, kStep = 2 * kStage;
 template <int MT, bool SHIFTED>
-__global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a)
+__global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a, uint32_t first_tile)
 {
     __shared__ __align__(16) v4i sums[kFewWaves][MT][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t n0 = (int64_t)blockIdx.x * 16;
+    const int64_t n0 = ((int64_t)first_tile + blockIdx.x) * 16;
     const int row = lane & 15, at = (lane >> 4) * 32;
     typedef Shifted<2> Any;
     using Place = std::conditional_t<SHIFTED, Any, const uint8_t*>;
@@ -992,7 +993,7 @@ Copies copies_of(TileArgs a, const Plan& p, int64_t rows, int64_t cols)
     const int64_t stride = (a.inner + 15) / 16 * 16;
     a.splits = p.splits[0];
     a.stages_per_split = p.stages_per_split[0];
-    if (p.few || is_direct(a, p.tile) || rows * (stride / 16) > 0xffffff00 || cols * (stride / 16) > 0xffffff00) return {};
+    if (p.few || is_direct(a, p.tile) || (rows + cols) * (stride / 16) > kMostGroups * 256) return {};   // (one launch)
     const bool x = !loads_fit(a.x, a.x_stride, p.tile, a.inner), w = !loads_fit(a.w, a.w_stride, p.tile, a.inner);
     if (x) a.x = nullptr, a.x_stride = stride;   // (a place of any alignment)
     if (w) a.w = nullptr, a.w_stride = stride;
@@ -1011,24 +1012,28 @@ void run_few(const TileArgs& a, hipStream_t s)
         k_few_streamed<MT><<<dim3((uint32_t)(tiles < kUnits ? tiles : kUnits)), dim3(kFewWaves * 64), 0, s>>>(a);
         return;
     }
-    const dim3 grid((uint32_t)((a.cols + 15) / 16), (uint32_t)a.splits);
     const bool words = ((uintptr_t)a.x | (uintptr_t)a.w | (uint64_t)a.x_stride | (uint64_t)a.w_stride) % 4 == 0;
-    if (words) k_few_rows<MT, false><<<grid, dim3(kFewWaves * 64), 0, s>>>(a);
-    else k_few_rows<MT, true><<<grid, dim3(kFewWaves * 64), 0, s>>>(a);
+    in_launches((a.cols + 15) / 16, kFewWaves * 64, [&](int64_t first, uint32_t tiles) {
+        const dim3 grid(tiles, (uint32_t)a.splits);
+        if (words) k_few_rows<MT, false><<<grid, dim3(kFewWaves * 64), 0, s>>>(a, (uint32_t)first);
+        else k_few_rows<MT, true><<<grid, dim3(kFewWaves * 64), 0, s>>>(a, (uint32_t)first);
+    });
 }
 
 template <int B, bool INT8>
-void run_tiles(TwoProducts both, bool direct, hipStream_t s)
+bool run_tiles(TwoProducts both, bool direct, hipStream_t s)
 {
     const auto groups = [](TileArgs& a) {
         a.tiles_m = (int)((a.rows + B - 1) / B);
         a.tiles_n = (int)((a.cols + B - 1) / B);
-        return (uint32_t)a.tiles_m * a.tiles_n * a.splits;
+        return (int64_t)a.tiles_m * a.tiles_n * a.splits;
     };
-    both.second_at = groups(both.first);
-    const uint32_t works = both.second_at + (both.second.rows ? groups(both.second) : 0);
-    if (direct) k_tiles<B, INT8><<<dim3(works), dim3(kWaves * 64), 0, s>>>(both);
-    else k_tiles_any<B, INT8><<<dim3(works), dim3(kWaves * 64), 0, s>>>(both);
+    const int64_t first = groups(both.first), works = first + (both.second.rows ? groups(both.second) : 0);
+    if (works > kMostGroups) return false;   // (more outputs than the memory holds, but for products of less than a tile's height)
+    both.second_at = (uint32_t)first;
+    if (direct) k_tiles<B, INT8><<<dim3((uint32_t)works), dim3(kWaves * 64), 0, s>>>(both);
+    else k_tiles_any<B, INT8><<<dim3((uint32_t)works), dim3(kWaves * 64), 0, s>>>(both);
+    return true;
 }
 
 // Runs one product, or two in one launch (second.rows 0: one).  The caller has made the plan and the partial sums' memory.
@@ -1046,9 +1051,10 @@ int run_products(TwoProducts both, const Plan& p, hipStream_t s)
         else run_few<4>(both.first, s);
     } else {
         const bool direct = is_direct(both.first, p.tile) && (!both.second.rows || is_direct(both.second, p.tile));
-        if (p.tile == 256) run_tiles<256, INT8>(both, direct, s);
-        else if (p.tile == 128) run_tiles<128, INT8>(both, direct, s);
-        else run_tiles<64, INT8>(both, direct, s);
+        const bool fits = p.tile == 256   ? run_tiles<256, INT8>(both, direct, s)
+                          : p.tile == 128 ? run_tiles<128, INT8>(both, direct, s)
+                                          : run_tiles<64, INT8>(both, direct, s);
+        if (!fits) return GEO_SC_ERR_UNSUPPORTED;
     }
     const auto joins = [](const TileArgs& a) { return a.partial ? (uint32_t)((a.rows * ((a.cols + 3) / 4) + 255) / 256) : 0u; };
     both.second_at = joins(both.first);
@@ -1446,7 +1452,7 @@ int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64_t grad_str
     const int64_t g_tiles = tiles(rows, kSide, cols, kSide), w_tiles = dx ? tiles(cols, kSide, inner, kWide) : 0,
                   x_tiles = dw ? tiles(rows, kSide, inner, kWide) : 0;
     const int64_t blocks = tiles(rows, l.peak_rows, cols, l.peak_cols);
-    if (g_tiles + w_tiles + x_tiles > 0x7fffffff || blocks > 0x7fffffff) return GEO_SC_ERR_UNSUPPORTED;
+    if (g_tiles + w_tiles + x_tiles > kMostGroups || blocks > kMostGroups / (kPeakWaves * 64 / 256)) return GEO_SC_ERR_UNSUPPORTED;
     hipStream_t s = (hipStream_t)stream;
     uint8_t* base = (uint8_t*)workspace;
     OperandArgs o = {};

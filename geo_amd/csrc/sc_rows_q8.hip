@@ -264,6 +264,21 @@ int threads_of_row(int64_t chunks, int held)
     return threads < 1024 ? (int)threads : 1024;
 }
 
+// the rows from `first` on
+template <typename T>
+RowsArgs rows_from(RowsArgs a, int64_t first)
+{
+    a.x = (const T*)a.x + first * a.x_stride;
+    if (a.residual) a.residual = (const T*)a.residual + first * a.residual_stride;
+    a.q += first * a.q_stride;
+    a.scale += first;
+    if (a.rstd) a.rstd += first;
+    if (a.total) a.total = (T*)a.total + first * a.cols;
+    if (a.values) a.values = (char*)a.values + first * a.cols * dtype_bytes(a.values_dtype);
+    a.rows -= first;
+    return a;
+}
+
 template <typename T, bool NORM>
 int run_rows(RowsArgs a, hipStream_t s)
 {
@@ -275,15 +290,18 @@ int run_rows(RowsArgs a, hipStream_t s)
     // bf16 in 8 bits 23.5 us, with one 29.8.  Few rows are as fast as their longest thread.
     const int threads = threads_of_row(chunks, a.rows >= 2048 && chunks > 64 ? 2 : 1), per_block = threads == 64 ? 4 : 1;
     const int64_t items = (chunks + threads - 1) / threads;
-    const dim3 grid((uint32_t)((a.rows + per_block - 1) / per_block)), block(threads, per_block);
-    const auto held = [&](auto count) {
-        if (once) k_rows<T, NORM, count(), true><<<grid, block, 0, s>>>(a);
-        else k_rows<T, NORM, count(), false><<<grid, block, 0, s>>>(a);
-    };
-    if (items <= 1) held(std::integral_constant<int, 1>());
-    else if (items <= 2) held(std::integral_constant<int, 2>());
-    else if (items <= 4) held(std::integral_constant<int, 4>());
-    else k_rows_long<T, NORM><<<dim3((uint32_t)a.rows), dim3(1024), 0, s>>>(a);
+    const dim3 block(threads, per_block);
+    in_launches((a.rows + per_block - 1) / per_block, threads, [&](int64_t first, uint32_t grid) {
+        const RowsArgs b = rows_from<T>(a, first * per_block);
+        const auto held = [&](auto count) {
+            if (once) k_rows<T, NORM, count(), true><<<grid, block, 0, s>>>(b);
+            else k_rows<T, NORM, count(), false><<<grid, block, 0, s>>>(b);
+        };
+        if (items <= 1) held(std::integral_constant<int, 1>());
+        else if (items <= 2) held(std::integral_constant<int, 2>());
+        else if (items <= 4) held(std::integral_constant<int, 4>());
+        else k_rows_long<T, NORM><<<grid, block, 0, s>>>(b);
+    });
     return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
 }
 
@@ -306,6 +324,7 @@ struct NormBackArgs {
     bool streamed;    // dx
     bool once;        // what is read
     float* partial;   // [blocks][cols]: sums of the weight's gradient, NULL: not wanted
+    int64_t first_row;   // of a launch of k_norm_back_long
 };
 
 // A block takes every gridDim.x-th row; its threads keep the weight and their columns' sums of the weight's gradient in
@@ -389,7 +408,7 @@ __global__ __launch_bounds__(1024) void k_norm_back_long(NormBackArgs a)
 {
     __shared__ RowSlots slots;
     const int threads = blockDim.x, waves = threads >> 6;
-    const int64_t row = blockIdx.x, first = (int64_t)threadIdx.x * kChunk, step = (int64_t)threads * kChunk;
+    const int64_t row = a.first_row + blockIdx.x, first = (int64_t)threadIdx.x * kChunk, step = (int64_t)threads * kChunk;
     const float r = a.rstd[row];
     float along = 0.f;
     float g[kChunk], v[kChunk], w[kChunk];
@@ -490,7 +509,11 @@ int run_norm_back(const NormBackArgs& a, T* dw, hipStream_t s)
 {
     const int64_t chunks = (a.cols + kChunk - 1) / kChunk, blocks = norm_back_blocks(a.rows, a.cols);
     if (a.cols > kHeldBackCols) {
-        k_norm_back_long<T><<<dim3((uint32_t)a.rows), dim3(1024), 0, s>>>(a);
+        in_launches(a.rows, 1024, [&](int64_t first, uint32_t count) {
+            NormBackArgs b = a;
+            b.first_row = first;
+            k_norm_back_long<T><<<dim3(count), dim3(1024), 0, s>>>(b);
+        });
         if (a.partial)
             k_weight_grad_columns<T><<<dim3((uint32_t)((chunks + 255) / 256), (uint32_t)blocks), dim3(256), 0, s>>>(a);
     } else if (a.grad_dtype == GEO_SC_F32) {
@@ -571,7 +594,7 @@ int geo_sc_rms_norm_q8_backward(const void* grad_values, int grad_dtype, int64_t
                       reads_once(grad_dtype, grad_values, grad_stride) && (!grad_total || reads_once(dtype, grad_total, grad_total_stride));
     const NormBackArgs a = {grad_values, grad_total, x, residual, weight, grad_dtype, rows, cols, grad_stride, grad_total_stride,
                             x_stride, residual_stride, rstd, dx, streams(rows * cols * dtype_bytes(dtype)), once,
-                            dweight ? (float*)workspace : nullptr};
+                            dweight ? (float*)workspace : nullptr, 0};
     hipStream_t s = (hipStream_t)stream;
     if (dtype == GEO_SC_F32) return run_norm_back<f32>(a, (f32*)dweight, s);
     if (dtype == GEO_SC_BF16) return run_norm_back<bf16>(a, (bf16*)dweight, s);
