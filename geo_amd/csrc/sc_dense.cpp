@@ -23,6 +23,7 @@ void on_gpu(const at::Tensor& t, const char* what)
 {
     TORCH_CHECK(t.is_cuda(), what, " must be on the GPU");
     TORCH_CHECK(t.layout() == at::kStrided && !t.is_neg(), what, " must be an ordinary dense tensor");
+    TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), what, " carries a forward-mode tangent, which these operators have no rule for");
 }
 void with(const at::Tensor& t, const char* what, const at::Tensor& other, const char* other_what)
 {

@@ -1,0 +1,43 @@
+"""What the dense operators and the loss have no rule for is refused, not answered with something else: forward-mode tangents, second
+derivatives, recording of the calls as operations."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from tests.test_gpu_dense import rand, uf  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def operands():
+    g = torch.Generator().manual_seed(7)
+    index = torch.stack([torch.randperm(24, generator=g)[:5] for _ in range(12)]).cuda()
+    return dict(x=rand(12, 24, seed=1), gain=1 + rand(24, seed=2, scale=0.1), w=rand(16, 24, seed=3), residual=rand(12, 24, seed=4), t=rand(12, 5, seed=5),
+                index=index)
+
+
+CALLS = {"linear": lambda uf, o: uf.linear_q8(o["x"], o["w"]),
+         "norm_linear": lambda uf, o: uf.norm_linear_q8(o["x"], o["gain"], o["w"], residual=o["residual"])[0],
+         "norm": lambda uf, o: uf.rms_norm_q8(o["x"], o["gain"], residual=o["residual"], values=torch.float32)[3],
+         "loss": lambda uf, o: uf.distill_topk(o["x"], o["t"], o["index"])}
+
+
+@pytest.mark.parametrize("call", list(CALLS) + ["rows", "product"])
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_tangents_are_refused(uf, call, grad_mode):
+    """a tangent that is dropped would be a derivative of zero"""
+    o = operands()
+    q, s, _ = uf.quantize_rows(o["x"])
+    wq, ws, _ = uf.quantize_rows(o["w"])
+    run = {**CALLS, "rows": lambda uf, o: uf.quantize_rows(o["x"], values=torch.float32)[2],
+           "product": lambda uf, o: uf.matmul_q8(q, o["s"], wq, ws)}[call]
+    o["s"] = s
+    run(uf, o)
+    for name in ("x", "gain", "w", "residual", "t", "s"):
+        used = {"linear": "xw", "rows": "x", "product": "s", "loss": "xt"}.get(call, ["x", "gain", "residual"] + ["w"] * (call == "norm_linear"))
+        if name not in used:
+            continue
+        with torch.set_grad_enabled(grad_mode), forward_ad.dual_level():
+            dual = dict(o, **{name: forward_ad.make_dual(o[name], torch.ones_like(o[name]))})
+            with pytest.raises(RuntimeError, match="tangent|jvp"):
+                run(uf, dual)
