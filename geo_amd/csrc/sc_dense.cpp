@@ -3,6 +3,8 @@
 // token's call is bound by its host time.
 #include "sc_torch_common.h"
 
+#include <torch/csrc/autograd/functions/utils.h>
+
 using namespace geo_sc_torch;
 
 namespace {
@@ -51,6 +53,29 @@ Rows as_rows(const at::Tensor& t, const char* what)
     if (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= 0) return {t, t.size(0), cols, t.size(0) > 1 ? t.stride(0) : cols};
     const at::Tensor c = t.contiguous();
     return {c, c.numel() / cols, cols, cols};
+}
+
+// A gradient that a kernel wrote.  Under create_graph it needs a graph of its own, or a second derivative would come out as zero: here
+// a node that raises, on the way to all that the gradient depends on (what the node being evaluated leads to, and `upstream`).
+struct Once : torch::autograd::Node {
+    torch::autograd::variable_list apply(torch::autograd::variable_list&&) override
+    {
+        TORCH_CHECK(false, "the dense 8-bit layers and the distillation loss can be differentiated once only");
+    }
+    std::string name() const override { return "DifferentiableOnce"; }
+};
+at::Tensor once(const at::Tensor& g, std::initializer_list<at::Tensor> upstream)
+{
+    if (!at::GradMode::is_enabled()) return g;
+    const auto current = torch::autograd::get_current_node();
+    torch::autograd::edge_list edges;
+    if (current) edges = current->next_edges();
+    for (const at::Tensor& u : upstream)
+        if (u.defined() && u.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(u));
+    const auto node = std::make_shared<Once>();
+    node->set_next_edges(std::move(edges));
+    torch::autograd::set_history(g, node);
+    return g;
 }
 
 // 8-bit rows that start at multiples of 16 bytes: what the product's fast way takes
@@ -145,7 +170,9 @@ std::tuple<at::Tensor, MaybeTensor> rms_norm_q8_backward(const MaybeTensor& grad
                                              t.cols, rstd.const_data_ptr<float>(), dx.data_ptr(), data_of(dw), data_of(workspace), bytes,
                                              stream_of(x)),
                  "rms_norm_q8 backward");
-    return {dx, dw};
+    const at::Tensor sum_grad = grad_total ? *grad_total : at::Tensor();
+    if (dw) once(*dw, {*grad_values});
+    return {once(dx, {*grad_values, sum_grad}), dw};
 }
 
 // What the backward forms x + residual from: themselves, because `total` is rounded to their type; where that is fp32, `total`
@@ -232,6 +259,8 @@ std::tuple<MaybeTensor, MaybeTensor> matmul_q8_backward(const at::Tensor& grad, 
                                            dx ? dtype_of(*dx_type, "dx") : 0, data_of(dw), dw ? dtype_of(*dw_type, "dw") : 0,
                                            workspace.data_ptr(), bytes, stream_of(q)),
                  "matmul_q8 backward");
+    if (dx) once(*dx, {grad});
+    if (dw) once(*dw, {grad});
     return {dx, dw};
 }
 
@@ -293,7 +322,7 @@ at::Tensor distill_topk_backward(const at::Tensor& grad, const at::Tensor& logit
                                               top.index.const_data_ptr(), top.index_bytes, z.rows, z.cols, top.top, (float)temperature,
                                               stats.const_data_ptr<float>(), dz.data_ptr(), stream_of(logits)),
                  "distill_topk backward");
-    return dz;
+    return once(dz, {grad});
 }
 
 // ---------------------------------------------------------------- autograd nodes

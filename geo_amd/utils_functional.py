@@ -172,7 +172,7 @@ def sc_counts(activation, weight, bit_length, padding, forward="1d_bin", load_un
 #
 # The SC layers approximate products of 8-bit operands; these compute them exactly, with a scale per row in place of the one
 # fixed scale of ``quantize``.  All take GPU tensors (float32, bfloat16 or float16; rows are the last dimension) and run on PyTorch's
-# current stream.
+# current stream.  The gradients can be taken once: a second derivative raises, as does a forward-mode tangent.
 
 _dense_module = None
 
@@ -224,7 +224,7 @@ def linear_q8(x, weight):
 
 def norm_linear_q8(x, gain, weight, residual=None, eps=1e-6):
     """The root-mean-square norm of ``x + residual`` with 8-bit output (``rms_norm_q8``, weight ``gain``) and its
-    product with ``weight`` rounded to 8-bit rows: (y, x + residual), differentiable in all four tensors."""
+    product with ``weight`` rounded to 8-bit rows: (y, x + residual), differentiable (once) in all four tensors."""
     return _dense().norm_linear_q8(x, gain, weight, residual, eps)
 
 
@@ -240,7 +240,8 @@ def distill_topk(logits, top_logits, top_index, temperature=1.0, reduction="mean
 
     ``top_logits`` and ``top_index`` (int32 or int64) are (rows, entries), at most 4096 entries; an index outside the columns (-1)
     marks an absent entry, and a row without entries has loss and gradient 0.  ``reduction``: "mean" over all rows, "sum" or
-    "none".  The loss is float32; the gradient goes to ``logits`` only (the teacher is fixed)."""
+    "none".  The loss is float32; the gradient, which can be taken once, goes to ``logits`` only (the teacher is
+    fixed)."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     return _dense().distill_topk(logits, top_logits, top_index, temperature, _REDUCTIONS[reduction])

@@ -41,3 +41,31 @@ def test_tangents_are_refused(uf, call, grad_mode):
             dual = dict(o, **{name: forward_ad.make_dual(o[name], torch.ones_like(o[name]))})
             with pytest.raises(RuntimeError, match="tangent|jvp"):
                 run(uf, dual)
+
+
+@pytest.mark.parametrize("call", list(CALLS))
+def test_second_derivatives_are_refused(uf, call):
+    """a penalty on a gradient would add nothing to the result"""
+    for name in {"linear": "xw", "loss": "x"}.get(call, ("x", "gain", "residual") + ("w",) * (call == "norm_linear")):
+        o = operands()
+        o[name].requires_grad_(True)
+        first, = torch.autograd.grad(CALLS[call](uf, o).sum(), o[name])
+        again, = torch.autograd.grad(CALLS[call](uf, o).sum(), o[name], create_graph=True)
+        assert torch.equal(first, again.detach()) and again.requires_grad   # asked for and not used: the value is there
+        with pytest.raises(RuntimeError, match="once only"):
+            again.square().sum().backward()
+        # beside a term that has a second derivative too
+        total = CALLS[call](uf, o).sum() + o[name].pow(3).sum()
+        both, = torch.autograd.grad(total, o[name], create_graph=True)
+        with pytest.raises(RuntimeError, match="once only"):
+            torch.autograd.grad(both.sum(), o[name])
+
+
+def test_gradient_of_the_sum_alone_has_a_second_derivative(uf):
+    """what passes by the norm, x + residual, is linear"""
+    o = operands()
+    x = o["x"].requires_grad_(True)
+    _, _, total, _ = uf.rms_norm_q8(x, o["gain"], residual=o["residual"], values=torch.float32)
+    g, = torch.autograd.grad(total.pow(3).sum(), x, create_graph=True)
+    second, = torch.autograd.grad(g.sum(), x)
+    assert torch.equal(g, 3 * total.square()) and torch.allclose(second, 6 * total, rtol=1e-6)
