@@ -3,7 +3,9 @@
 // token's call is bound by its host time.
 #include "sc_torch_common.h"
 
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 using namespace geo_sc_torch;
 
@@ -31,6 +33,14 @@ void with(const at::Tensor& t, const char* what, const at::Tensor& other, const 
 {
     on_gpu(t, what);
     TORCH_CHECK(t.device() == other.device(), what, " and ", other_what, " are on different devices");
+}
+
+// Whoever records a program's operations to run them again sees the allocation of the outputs, and not what fills them.
+void not_recorded()
+{
+    TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                    !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                "the dense 8-bit layers and the distillation loss cannot be traced");
 }
 
 geo_sc_stream_t stream_of(const at::Tensor& t)
@@ -94,6 +104,7 @@ void* data_of(const MaybeTensor& t) { return t ? t->data_ptr() : nullptr; }
 
 std::tuple<at::Tensor, at::Tensor, MaybeTensor> quantize_rows(const at::Tensor& x, std::optional<at::ScalarType> values_type)
 {
+    not_recorded();
     const Rows r = as_rows(x, "x");
     const int dtype = dtype_of(x.scalar_type(), "x"), vtype = values_type ? dtype_of(*values_type, "values") : 0;
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
@@ -112,6 +123,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, MaybeTensor, MaybeTensor> rms_nor
                                                                                    std::optional<at::ScalarType> values_type,
                                                                                    bool for_backward)
 {
+    not_recorded();
     const Rows r = as_rows(x, "x");
     const int dtype = dtype_of(x.scalar_type(), "x"), vtype = values_type ? dtype_of(*values_type, "values") : 0;
     with(weight, "weight", x, "x");
@@ -144,6 +156,7 @@ std::tuple<at::Tensor, MaybeTensor> rms_norm_q8_backward(const MaybeTensor& grad
                                                          const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight,
                                                          const at::Tensor& rstd, bool need_weight)
 {
+    not_recorded();
     const Rows t = as_rows(x, "x");
     Rows r = {};
     if (residual.defined()) r = as_rows(residual, "residual");
@@ -210,6 +223,7 @@ Q8 as_q8(const at::Tensor& q, const at::Tensor& scale, const char* what)
 
 at::Tensor matmul_q8(const at::Tensor& q, const at::Tensor& scale, const at::Tensor& wq, const at::Tensor& wscale, at::ScalarType type)
 {
+    not_recorded();
     const Q8 x = as_q8(q, scale, "q"), w = as_q8(wq, wscale, "weight_q");
     const int dtype = dtype_of(type, "dtype");
     with(wq, "weight_q", q, "q");
@@ -237,6 +251,7 @@ std::tuple<MaybeTensor, MaybeTensor> matmul_q8_backward(const at::Tensor& grad, 
                                                         const at::Tensor& wq, const at::Tensor& wscale,
                                                         std::optional<at::ScalarType> dx_type, std::optional<at::ScalarType> dw_type)
 {
+    not_recorded();
     const Q8 x = as_q8(q, scale, "q"), w = as_q8(wq, wscale, "weight_q");
     const Rows g = as_rows(grad, "gradient");
     with(grad, "gradient", q, "q");
@@ -287,6 +302,7 @@ Top as_top(const Rows& z, const at::Tensor& logits, const at::Tensor& top_logits
 std::tuple<at::Tensor, at::Tensor> distill_topk(const at::Tensor& logits, const at::Tensor& top_logits, const at::Tensor& top_index,
                                                 double temperature, int64_t reduction)
 {
+    not_recorded();
     const Rows z = as_rows(logits, "logits");
     const int dtype = dtype_of(logits.scalar_type(), "logits");
     TORCH_CHECK(logits.dim() >= 2, "logits must be (rows, columns)");
@@ -309,6 +325,7 @@ std::tuple<at::Tensor, at::Tensor> distill_topk(const at::Tensor& logits, const 
 at::Tensor distill_topk_backward(const at::Tensor& grad, const at::Tensor& logits, const at::Tensor& top_logits, const at::Tensor& top_index,
                                  double temperature, int64_t reduction, const at::Tensor& stats)
 {
+    not_recorded();
     const Rows z = as_rows(logits, "logits");
     const Top top = as_top(z, logits, top_logits, top_index);
     with(grad, "gradient", logits, "logits");

@@ -69,3 +69,32 @@ def test_gradient_of_the_sum_alone_has_a_second_derivative(uf):
     g, = torch.autograd.grad(total.pow(3).sum(), x, create_graph=True)
     second, = torch.autograd.grad(g.sum(), x)
     assert torch.equal(g, 3 * total.square()) and torch.allclose(second, 6 * total, rtol=1e-6)
+
+
+@pytest.mark.parametrize("call", list(CALLS))
+@pytest.mark.filterwarnings("ignore")
+def test_recording_is_refused(uf, call):
+    """what would be recorded is the outputs' allocation: the replay would return the allocator's memory"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    o = operands()
+
+    def run(x):
+        return CALLS[call](uf, dict(o, x=x))
+
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(run, o["x"], check_trace=False)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(run)(o["x"])
+    leaf = o["x"].requires_grad_(True)
+    out = run(leaf).sum()
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(lambda g: torch.autograd.grad(out, leaf, g, retain_graph=True)[0])(torch.ones_like(out))
+    torch.autograd.grad(out, leaf)   # neither leaves anything behind
+
+
+def test_modules_are_not_traced_either(uf):
+    from geo_amd import utils_class
+    layer = utils_class.Linear_Q8(24, 16).cuda().eval()
+    layer.prepare()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(layer, torch.ones(3, 24, device="cuda"), check_trace=False)
