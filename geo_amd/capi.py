@@ -5,6 +5,7 @@ C call.  These are what the GPU parity tests and the benchmark drive.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -81,17 +82,28 @@ def _stream_ptr(stream=None):
     return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
 
 
-def _fork(stream):
-    """Before a call on a stream of its own: what it allocates, result and scratch, is memory of the current stream, where
-    it may still be in use."""
-    if stream is not None:
-        stream.wait_stream(torch.cuda.current_stream())
+_HERE = contextlib.nullcontext()
 
 
-def _join(stream):
-    """Behind such a call: the current stream hands the scratch out again at once, and reads the result."""
-    if stream is not None:
-        torch.cuda.current_stream().wait_stream(stream)
+def _on(stream):
+    """Where a call on a stream of its own allocates and converts: in that stream's order and memory.  (The inputs are the
+    caller's to have ready on that stream, as everywhere in PyTorch.)"""
+    return _HERE if stream is None else torch.cuda.stream(stream)
+
+
+def _hand_over(stream, *results):
+    """Behind such a call, for the results that it allocated: the current stream, where they are used, waits for the call, and
+    their memory is not handed out again before what the current stream does with them.  Results in the caller's tensors
+    need neither, so that calls on several streams overlap; nor does the next call's stream wait for the current one."""
+    if stream is None:
+        return
+    current = torch.cuda.current_stream(stream.device)
+    if current == stream:
+        return
+    current.wait_stream(stream)
+    for t in results:
+        if t is not None:
+            t.record_stream(current)
 
 
 def _ptr(t):
@@ -135,16 +147,18 @@ def conv2d_add_partial_forward(x, w, bit_length, padding=(0, 0), total_width=7, 
     if desc is None:
         desc = make_desc(x.shape, w.shape, bit_length, padding, total_width, load_width, load_wait_w, load_wait_a,
                          accumulate, z_unit, generator, seed)
-    if workspace is None:
-        workspace = torch.empty(workspace_size(desc, options), dtype=torch.uint8, device=x.device)
-    if out is None:
-        out = torch.empty(output_shape(desc), dtype=torch.int32, device=x.device)
-    _fork(stream)
+    given = out is not None
+    with _on(stream):
+        if workspace is None:
+            workspace = torch.empty(workspace_size(desc, options), dtype=torch.uint8, device=x.device)
+        if not given:
+            out = torch.empty(output_shape(desc), dtype=torch.int32, device=x.device)
     _check(_native.lib().geo_sc_conv2d_add_partial_forward_ex(ctypes.byref(desc), _opt_ptr(options), _ptr(x), _ptr(w),
                                                               _ptr(out), _ptr(workspace), workspace.numel(),
                                                               _stream_ptr(stream)),
            "geo_sc_conv2d_add_partial_forward")
-    _join(stream)
+    if not given:
+        _hand_over(stream, out)
     return out
 
 
@@ -153,14 +167,14 @@ def conv2d_add_partial_values(x, w, desc: ConvDesc, bit_length, stream=None):
     (geo_sc_counts_to_values)."""
     _require_gpu_f32(x, "x")
     _require_gpu_f32(w, "w")
-    workspace = torch.empty(workspace_size(desc), dtype=torch.uint8, device=x.device)
-    y = torch.empty(output_shape(desc), dtype=torch.float32, device=x.device)
-    _fork(stream)
+    with _on(stream):
+        workspace = torch.empty(workspace_size(desc), dtype=torch.uint8, device=x.device)
+        y = torch.empty(output_shape(desc), dtype=torch.float32, device=x.device)
     lib, y_ptr, stream_ptr = _native.lib(), _ptr(y), _stream_ptr(stream)
     _check(lib.geo_sc_conv2d_add_partial_forward_ex(ctypes.byref(desc), None, _ptr(x), _ptr(w), y_ptr, _ptr(workspace),
                                                     workspace.numel(), stream_ptr), "geo_sc_conv2d_add_partial_forward")
     _check(lib.geo_sc_counts_to_values(y_ptr, y.numel(), int(bit_length), stream_ptr), "geo_sc_counts_to_values")
-    _join(stream)
+    _hand_over(stream, y)
     return y
 
 
@@ -201,16 +215,18 @@ def conv2d_add_partial_forward_q7(x_q7, w, bit_length, padding=(0, 0), total_wid
     _require_gpu_f32(w, "w")
     desc = make_desc(x_q7.shape, w.shape, bit_length, padding, total_width, load_width, load_wait_w, load_wait_a,
                      accumulate, z_unit)
-    if workspace is None:
-        workspace = torch.empty(workspace_size(desc), dtype=torch.uint8, device=w.device)
-    if out is None:
-        out = torch.empty(output_shape(desc), dtype=torch.int32, device=w.device)
-    _fork(stream)
+    given = out is not None
+    with _on(stream):
+        if workspace is None:
+            workspace = torch.empty(workspace_size(desc), dtype=torch.uint8, device=w.device)
+        if not given:
+            out = torch.empty(output_shape(desc), dtype=torch.int32, device=w.device)
     _check(_native.lib().geo_sc_conv2d_add_partial_forward_q7(ctypes.byref(desc), _ptr(x_q7), _ptr(w), _ptr(out),
                                                               _ptr(workspace), workspace.numel(),
                                                               _stream_ptr(stream)),
            "geo_sc_conv2d_add_partial_forward_q7")
-    _join(stream)
+    if not given:
+        _hand_over(stream, out)
     return out
 
 
@@ -226,19 +242,20 @@ def layer_epilogue(counts, bit_length, w_n, b_n, relu=False, pool=True, hardtanh
     if not (counts.is_cuda and counts.dtype == torch.int32 and counts.is_contiguous() and counts.dim() == 4):
         raise ValueError("counts must be a contiguous int32 GPU tensor (N, C, W, H)")
     n, c, w, h = counts.shape
-    w_n = w_n.to(counts.device, torch.float32).contiguous()
-    b_n = b_n.to(counts.device, torch.float32).contiguous()
+    with _on(stream):
+        w_n = w_n.to(counts.device, torch.float32).contiguous()
+        b_n = b_n.to(counts.device, torch.float32).contiguous()
     if w_n.numel() != c or b_n.numel() != c:
         raise ValueError("w_n and b_n need one entry per channel")
     flags = (EPI_RELU if relu else 0) | (EPI_POOL2 if pool else 0) | (EPI_HARDTANH01 if hardtanh else 0) | \
         (EPI_QUANT7 if quant7 else 0)
     shape = (n, c, w // 2, h // 2) if pool else (n, c, w, h)
-    act = torch.empty(shape, dtype=torch.float32, device=counts.device) if want_act else None
-    q7 = torch.empty(shape, dtype=torch.uint8, device=counts.device) if want_q7 else None
-    _fork(stream)
+    with _on(stream):
+        act = torch.empty(shape, dtype=torch.float32, device=counts.device) if want_act else None
+        q7 = torch.empty(shape, dtype=torch.uint8, device=counts.device) if want_q7 else None
     _check(_native.lib().geo_sc_layer_epilogue(_ptr(counts), n, c, w, h, int(bit_length), _ptr(w_n), _ptr(b_n), flags,
                                                _ptr(act), _ptr(q7), _stream_ptr(stream)), "geo_sc_layer_epilogue")
-    _join(stream)
+    _hand_over(stream, act, q7)
     return act, q7
 
 
@@ -249,24 +266,25 @@ def layer_tail_backward(counts, grad_out, bit_length, w_n, b_n, mean, invstd, ga
     n, c, w, h = counts.shape
     dev = counts.device
     f = lambda t: t.to(dev, torch.float32).contiguous()
-    grad_out, w_n, b_n, mean, invstd = f(grad_out), f(w_n), f(b_n), f(mean), f(invstd)
-    gamma = None if gamma is None else f(gamma)
+    with _on(stream):
+        grad_out, w_n, b_n, mean, invstd = f(grad_out), f(w_n), f(b_n), f(mean), f(invstd)
+        gamma = None if gamma is None else f(gamma)
     exp = (n, c, w // 2, h // 2) if pool else (n, c, w, h)
     if tuple(grad_out.shape) != exp:
         raise ValueError(f"grad_out has shape {tuple(grad_out.shape)}, expected {exp}")
     flags = (EPI_RELU if relu else 0) | (EPI_POOL2 if pool else 0) | (EPI_HARDTANH01 if hardtanh else 0)
     nbytes = ctypes.c_size_t(0)
     _check(_native.lib().geo_sc_layer_tail_backward_workspace_size(n, c, w, h, ctypes.byref(nbytes)), "tail workspace")
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-    grad_y = torch.empty((n, c, w, h), dtype=torch.float32, device=dev)
-    gg = torch.empty(c, dtype=torch.float32, device=dev)
-    gb = torch.empty(c, dtype=torch.float32, device=dev)
-    _fork(stream)
+    with _on(stream):
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+        grad_y = torch.empty((n, c, w, h), dtype=torch.float32, device=dev)
+        gg = torch.empty(c, dtype=torch.float32, device=dev)
+        gb = torch.empty(c, dtype=torch.float32, device=dev)
     _check(_native.lib().geo_sc_layer_tail_backward(_ptr(counts), _ptr(grad_out), n, c, w, h, int(bit_length), _ptr(w_n),
                                                     _ptr(b_n), _ptr(mean), _ptr(invstd), _ptr(gamma), flags,
                                                     _ptr(grad_y), _ptr(gg), _ptr(gb), _ptr(ws), ws.numel(),
                                                     _stream_ptr(stream)), "geo_sc_layer_tail_backward")
-    _join(stream)
+    _hand_over(stream, grad_y, gg, gb)
     return grad_y, gg, gb
 
 
@@ -280,13 +298,13 @@ def count_stats(counts, bit_length, stream=None):
     need = ctypes.c_size_t()
     _check(_native.lib().geo_sc_count_stats_workspace_size(n, c, w, h, ctypes.byref(need)),
            "geo_sc_count_stats_workspace_size")
-    ws = torch.empty(max(need.value, 8), dtype=torch.uint8, device=counts.device)
-    mean = torch.empty(c, dtype=torch.float32, device=counts.device)
-    var = torch.empty(c, dtype=torch.float32, device=counts.device)
-    _fork(stream)
+    with _on(stream):
+        ws = torch.empty(max(need.value, 8), dtype=torch.uint8, device=counts.device)
+        mean = torch.empty(c, dtype=torch.float32, device=counts.device)
+        var = torch.empty(c, dtype=torch.float32, device=counts.device)
     _check(_native.lib().geo_sc_count_stats(_ptr(counts), n, c, w, h, int(bit_length), _ptr(mean), _ptr(var), _ptr(ws),
                                             ws.numel(), _stream_ptr(stream)), "geo_sc_count_stats")
-    _join(stream)
+    _hand_over(stream, mean, var)
     return mean, var
 
 
@@ -299,16 +317,16 @@ def bn_fixed_affine(mean, var, gamma, beta, eps, elements_per_channel, running_m
     for t in (mean, var, gamma, beta, running_mean, running_var):
         if t is not None and not (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.numel() == c):
             raise ValueError("statistics and parameters must be contiguous float32 GPU tensors of one size")
-    w_n = torch.empty(c, dtype=torch.float32, device=dev)
-    b_n = torch.empty(c, dtype=torch.float32, device=dev)
-    invstd = torch.empty(c, dtype=torch.float32, device=dev)
-    scale = torch.empty((), dtype=torch.float32, device=dev)
-    _fork(stream)
+    with _on(stream):
+        w_n = torch.empty(c, dtype=torch.float32, device=dev)
+        b_n = torch.empty(c, dtype=torch.float32, device=dev)
+        invstd = torch.empty(c, dtype=torch.float32, device=dev)
+        scale = torch.empty((), dtype=torch.float32, device=dev)
     _check(_native.lib().geo_sc_bn_fixed_affine(_ptr(mean), _ptr(var), _ptr(gamma), _ptr(beta), c, float(eps),
                                                 float(eps_grad), int(elements_per_channel), _ptr(running_mean),
                                                 _ptr(running_var), _ptr(w_n), _ptr(b_n), _ptr(invstd), _ptr(scale),
                                                 _stream_ptr(stream)), "geo_sc_bn_fixed_affine")
-    _join(stream)
+    _hand_over(stream, w_n, b_n, invstd, scale)
     return w_n, b_n, invstd, scale
 
 
@@ -328,17 +346,17 @@ def bn_fixed_from_counts(counts, bit_length, gamma, beta, eps, running_mean=None
     need = ctypes.c_size_t()
     _check(_native.lib().geo_sc_count_stats_workspace_size(n, c, w, h, ctypes.byref(need)),
            "geo_sc_count_stats_workspace_size")
-    ws = torch.empty(max(need.value, 8), dtype=torch.uint8, device=dev)
-    out = torch.empty((5, c), dtype=torch.float32, device=dev)   # mean, var, w_n, b_n, invstd
-    scale = torch.empty((), dtype=torch.float32, device=dev)
+    with _on(stream):
+        ws = torch.empty(max(need.value, 8), dtype=torch.uint8, device=dev)
+        out = torch.empty((5, c), dtype=torch.float32, device=dev)   # mean, var, w_n, b_n, invstd
+        scale = torch.empty((), dtype=torch.float32, device=dev)
     mean, var, w_n, b_n, invstd = out[0], out[1], out[2], out[3], out[4]
-    _fork(stream)
     _check(_native.lib().geo_sc_bn_fixed_from_counts(_ptr(counts), n, c, w, h, int(bit_length), _ptr(gamma), _ptr(beta),
                                                      float(eps), float(eps_grad), _ptr(running_mean),
                                                      _ptr(running_var), _ptr(mean), _ptr(var), _ptr(w_n), _ptr(b_n),
                                                      _ptr(invstd), _ptr(scale), _ptr(ws), ws.numel(),
                                                      _stream_ptr(stream)), "geo_sc_bn_fixed_from_counts")
-    _join(stream)
+    _hand_over(stream, out, scale)
     return mean, var, w_n, b_n, invstd, scale
 
 
@@ -349,11 +367,11 @@ def bn_eval_weight(var, gamma, eps, stream=None):
         if t is not None and not (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.device == var.device
                                   and t.numel() == var.numel()):
             raise ValueError("variance and weight must be contiguous float32 tensors of one size on one GPU")
-    w = torch.empty(var.numel(), dtype=torch.float32, device=var.device)
-    _fork(stream)
+    with _on(stream):
+        w = torch.empty(var.numel(), dtype=torch.float32, device=var.device)
     _check(_native.lib().geo_sc_bn_eval_weight(_ptr(var), _ptr(gamma), var.numel(), float(eps), _ptr(w), _stream_ptr(stream)),
            "geo_sc_bn_eval_weight")
-    _join(stream)
+    _hand_over(stream, w)
     return w
 
 
@@ -367,13 +385,13 @@ def bn_fixed_eval(x, mean, var, gamma, beta, eps, w_mean=None, out=None, stream=
         if t is not None and not (t.is_cuda and t.dtype == torch.float32 and t.is_contiguous() and t.device == x.device
                                   and t.numel() == size):
             raise ValueError("x, statistics and parameters must be contiguous float32 tensors on one GPU")
-    y = torch.empty_like(x) if out is None else out
-    scale = torch.empty((), dtype=torch.float32, device=x.device)
-    _fork(stream)
+    with _on(stream):
+        y = torch.empty_like(x) if out is None else out
+        scale = torch.empty((), dtype=torch.float32, device=x.device)
     _check(_native.lib().geo_sc_bn_fixed_eval_mean(_ptr(x), n, c, x.numel() // (n * c), _ptr(mean), _ptr(var), _ptr(gamma),
                                                    _ptr(beta), float(eps), _ptr(w_mean), _ptr(y), _ptr(scale),
                                                    _stream_ptr(stream)), "geo_sc_bn_fixed_eval_mean")
-    _join(stream)
+    _hand_over(stream, y, scale)
     return y, scale
 
 
@@ -382,16 +400,16 @@ def quantize_many(tensors, prec, stream=None):
     returns the new tensors."""
     for t in tensors:
         _require_gpu_f32(t, "tensor")
-    outs = [torch.empty_like(t) for t in tensors]
+    with _on(stream):
+        outs = [torch.empty_like(t) for t in tensors]
     n = len(tensors)
-    _fork(stream)
     if n:
         arr = ctypes.c_void_p * n
         sizes = (ctypes.c_size_t * n)(*[t.numel() for t in tensors])
         _check(_native.lib().geo_sc_quantize_many(n, arr(*[t.data_ptr() for t in tensors]),
                                                   arr(*[o.data_ptr() for o in outs]), sizes, int(prec),
                                                   _stream_ptr(stream)), "geo_sc_quantize_many")
-    _join(stream)
+    _hand_over(stream, *outs)
     return outs
 
 
@@ -417,14 +435,16 @@ def quantize(x, prec, out=None, stream=None):
     """geo_sc_quantize: round(x * 2^prec) clamped to +-(2^prec - 1), over 2^prec, in one launch.
     ``x`` is a contiguous fp32 GPU tensor; ``out`` may be ``x`` itself."""
     _require_gpu_f32(x, "x")
-    if out is None:
-        out = torch.empty_like(x)
+    given = out is not None
+    if not given:
+        with _on(stream):
+            out = torch.empty_like(x)
     elif not (out.is_cuda and out.dtype == torch.float32 and out.is_contiguous() and out.shape == x.shape):
         raise ValueError("out must be a contiguous fp32 GPU tensor of x's shape")
-    _fork(stream)
     _check(_native.lib().geo_sc_quantize(_ptr(x), _ptr(out), x.numel(), int(prec), _stream_ptr(stream)),
            "geo_sc_quantize")
-    _join(stream)
+    if not given:
+        _hand_over(stream, out)
     return out
 
 
@@ -446,12 +466,12 @@ def act_streams(x, desc: ConvDesc, stream=None):
     inner = ctypes.c_int(0)
     _check(_native.lib().geo_sc_act_stream_layout(ctypes.byref(desc), ctypes.byref(inner)), "act layout")
     shape = (packs, desc.c_in, wi, hi, desc.n) if inner.value else (desc.n, packs, desc.c_in, wi, hi)
-    out = torch.empty(shape, dtype=torch.int32, device=x.device)
+    with _on(stream):
+        out = torch.empty(shape, dtype=torch.int32, device=x.device)
     assert out.numel() == n.value
     fn = _native.lib().geo_sc_act_streams_q7 if q7 else _native.lib().geo_sc_act_streams
-    _fork(stream)
     _check(fn(ctypes.byref(desc), _ptr(x), _ptr(out), None, _stream_ptr(stream)), "geo_sc_act_streams")
-    _join(stream)
+    _hand_over(stream, out)
     return out
 
 
@@ -466,13 +486,13 @@ def weight_streams(w, desc: ConvDesc, stream=None):
     classic = packs * desc.h_k * desc.c_in * desc.w_k * ((desc.c_out + 15) // 16) * 32
     # the buffer may continue behind the two-rail lines (rail-packed copy for large y-mode launches);
     # the returned view shows the lines and keeps the whole buffer alive
-    buf = torch.empty(n.value, dtype=torch.int32, device=w.device)
+    with _on(stream):
+        buf = torch.empty(n.value, dtype=torch.int32, device=w.device)
     assert n.value >= classic
     out = buf[:classic].view(shape)
-    _fork(stream)
     _check(_native.lib().geo_sc_weight_streams(ctypes.byref(desc), _ptr(w), _ptr(out), None, _stream_ptr(stream)),
            "geo_sc_weight_streams")
-    _join(stream)
+    _hand_over(stream, out)
     return out
 
 
@@ -484,13 +504,13 @@ def weight_streams_from_lines(lines, desc: ConvDesc, stream=None):
     _check(_native.lib().geo_sc_weight_stream_words(ctypes.byref(desc), ctypes.byref(n)), "weight words")
     if not (lines.is_cuda and lines.dtype == torch.int32 and lines.is_contiguous()) or lines.numel() > n.value:
         raise ValueError("lines must be a contiguous int32 GPU tensor of the two-rail layout")
-    buf = torch.empty(n.value, dtype=torch.int32, device=lines.device)
-    out = buf[:lines.numel()].view(lines.shape)
-    out.copy_(lines)
-    _fork(stream)
+    with _on(stream):
+        buf = torch.empty(n.value, dtype=torch.int32, device=lines.device)
+        out = buf[:lines.numel()].view(lines.shape)
+        out.copy_(lines)
     _check(_native.lib().geo_sc_weight_streams_finish(ctypes.byref(desc), _ptr(out), _stream_ptr(stream)),
            "geo_sc_weight_streams_finish")
-    _join(stream)
+    _hand_over(stream, out)
     return out
 
 
@@ -519,18 +539,20 @@ def skips_zero_rail(desc: ConvDesc) -> bool:
 
 def conv2d_add_partial_from_streams(act, wgt, desc: ConvDesc, out=None, stream=None):
     """The AND/OR/popcount kernel alone on pre-generated streams (int32-typed words)."""
-    if out is None:
-        out = torch.empty(output_shape(desc), dtype=torch.int32, device=act.device)
+    given = out is not None
+    if not given:
+        with _on(stream):
+            out = torch.empty(output_shape(desc), dtype=torch.int32, device=act.device)
     n = ctypes.c_size_t(0)
     _check(_native.lib().geo_sc_weight_stream_words(ctypes.byref(desc), ctypes.byref(n)), "weight words")
     if wgt.untyped_storage().nbytes() - wgt.storage_offset() * wgt.element_size() < 4 * n.value:
         raise ValueError("weight streams: the buffer behind this tensor is smaller than geo_sc_weight_stream_words "
                          "(take it from weight_streams())")
-    _fork(stream)
     _check(_native.lib().geo_sc_conv2d_add_partial_from_streams(ctypes.byref(desc), _ptr(act), _ptr(wgt), _ptr(out),
                                                                 _stream_ptr(stream)),
            "geo_sc_conv2d_add_partial_from_streams")
-    _join(stream)
+    if not given:
+        _hand_over(stream, out)
     return out
 
 
@@ -553,16 +575,16 @@ def conv2d_add_partial_backward(x, w, grad_y, bit_length=128, padding=(0, 0), ne
         desc = make_desc(x.shape, w.shape, bit_length, padding, accumulate=accumulate, z_unit=z_unit)
     if tuple(grad_y.shape) != output_shape(desc):
         raise ValueError(f"grad_y has shape {tuple(grad_y.shape)}, expected {output_shape(desc)}")
-    if workspace is None:
-        workspace = torch.empty(backward_workspace_size(desc, options), dtype=torch.uint8, device=x.device)
-    gx = torch.empty_like(x) if need_grad_x else None
-    gw = torch.empty_like(w) if need_grad_w else None
-    _fork(stream)
+    with _on(stream):
+        if workspace is None:
+            workspace = torch.empty(backward_workspace_size(desc, options), dtype=torch.uint8, device=x.device)
+        gx = torch.empty_like(x) if need_grad_x else None
+        gw = torch.empty_like(w) if need_grad_w else None
     _check(_native.lib().geo_sc_conv2d_add_partial_backward_ex(ctypes.byref(desc), _opt_ptr(options), _ptr(x), _ptr(w),
                                                                _ptr(grad_y), _ptr(gx), _ptr(gw), _ptr(workspace),
                                                                workspace.numel(), _stream_ptr(stream)),
            "geo_sc_conv2d_add_partial_backward")
-    _join(stream)
+    _hand_over(stream, gx, gw)
     return gx, gw
 
 
@@ -609,11 +631,13 @@ def probe_mfma_operands(n_a, n_b, seed=0, p_a=1 / 8, p_b=1 / 16):
 def probe_mfma_slices(mode, a, b, workgroups, slices, reload_sixteenths=16, out=None, stream=None):
     """geo_sc_probe_mfma_slices: `slices` (cycle, kernel row) slices of the forward as fp4 GEMM tiles per workgroup;
     returns the int32 counts (workgroups, 128, 256)."""
-    if out is None:
-        out = torch.empty((workgroups, PROBE_MFMA_ROWS, PROBE_MFMA_COLS), dtype=torch.int32, device="cuda")
-    _fork(stream)
+    given = out is not None
+    if not given:
+        with _on(stream):
+            out = torch.empty((workgroups, PROBE_MFMA_ROWS, PROBE_MFMA_COLS), dtype=torch.int32, device="cuda")
     _check(_native.probe_lib().geo_sc_probe_mfma_slices(int(mode), int(reload_sixteenths), int(workgroups), int(slices),
                                                         _ptr(a), a.shape[0], _ptr(b), b.shape[0], _ptr(out),
                                                         _stream_ptr(stream)), "geo_sc_probe_mfma_slices")
-    _join(stream)
+    if not given:
+        _hand_over(stream, out)
     return out
