@@ -22,15 +22,19 @@ def periodic(t):
     return bool((t == t[:1]).all())
 
 
+def all_are(t, value):   # (a comparison in an assert would be shown, element by element, should it fail)
+    return bool((t == value).all())
+
+
 def test_rows_of_one_column(uf):
     x = (1 + torch.arange(64, device="cuda", dtype=torch.bfloat16)).repeat(ROWS // 64)[:, None]
     q, scale, values = uf.quantize_rows(x, values=torch.bfloat16)
-    assert (q == 127).all() and periodic(scale) and torch.equal(values, x)
+    assert all_are(q, 127) and periodic(scale) and all_are(values, x)
     close(scale[:64], x[:64, 0].double() / 127, 3 * U * x[:64, 0].double() / 127)
     del q, scale, values
     one = torch.ones(1, dtype=torch.bfloat16, device="cuda")
     q, scale, total, values = uf.rms_norm_q8(x, one, residual=x, eps=0.0, values=torch.bfloat16)
-    assert (q == 127).all() and periodic(scale) and torch.equal(total, 2 * x) and (values == 1).all()
+    assert all_are(q, 127) and periodic(scale) and all_are(total, 2 * x) and all_are(values, 1)
 
 
 def test_loss_of_two_columns(uf):
