@@ -1,6 +1,8 @@
 """SC layer modules with the reference's interface (utils_class.py)."""
 from __future__ import annotations
 
+import warnings
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
@@ -221,8 +223,9 @@ def sc_conv_block(conv, bn, input, *, err=7, forward="1d_bin", z_unit=8, load_un
 
 class Linear_Q8(nn.Module):
     """Linear layer without bias whose operands are rounded to 8-bit rows (``utils_functional.linear_q8``): the exact counterpart
-    of an SC layer's product.  In training the weight is rounded on every call and the gradients pass straight through; for
-    inference ``prepare()`` rounds it once, until ``train()`` or ``load_state_dict`` drops the result."""
+    of an SC layer's product.  In training the weight is rounded on every call and the gradients pass straight through.  For
+    inference ``prepare()`` rounds it once, and calls without gradients take that result until ``train()``, ``load_state_dict`` or
+    a move to another device or type drops it; ``eval()`` keeps it.  A weight that has been written to since is said so in a warning."""
 
     def __init__(self, in_features, out_features):
         super().__init__()
@@ -230,24 +233,55 @@ class Linear_Q8(nn.Module):
         nn.init.kaiming_uniform_(self.weight, a=5 ** 0.5)
         self._q8 = None
 
+    def _weight_now(self):
+        w = self.weight
+        return w.data_ptr(), None if w.is_inference() else w._version, w.device, w.dtype   # (inference tensors count no writes)
+
     @torch.no_grad()
     def prepare(self):
         """Round the weight for inference.  Call again after changing it."""
         self._q8 = utils_functional.quantize_rows(self.weight)[:2]
+        self._q8_of = self._weight_now()
 
     def train(self, mode=True):
-        self._q8 = None
+        if mode:
+            self._q8 = None
         return super().train(mode)
 
     def _load_from_state_dict(self, *args, **kwargs):
         self._q8 = None
         super()._load_from_state_dict(*args, **kwargs)
 
+    def _apply(self, *args, **kwargs):
+        before = self.weight.data_ptr(), self.weight.device, self.weight.dtype
+        super()._apply(*args, **kwargs)
+        if before != (self.weight.data_ptr(), self.weight.device, self.weight.dtype):
+            self._q8 = None
+        return self
+
+    def __getstate__(self):
+        state = dict(self.__dict__)
+        if state["_q8"] is not None and self._q8_of != self._weight_now():
+            state["_q8"] = None
+        return state
+
+    def __setstate__(self, state):   # of a copy: another weight, of the same values
+        super().__setstate__(state)
+        if self._q8 is not None:
+            self._q8_of = self._weight_now()
+
+    def _prepared(self):
+        """The rounded weight for a call without gradients, or None."""
+        if self._q8 is not None and self._q8_of != self._weight_now() and not torch.is_grad_enabled():
+            warnings.warn("the weight has changed since prepare(), whose result this call takes: prepare() again", stacklevel=3)
+        return None if torch.is_grad_enabled() else self._q8
+
     def forward(self, x):
-        if self._q8 is None or torch.is_grad_enabled():
+        weight = self._prepared()
+        if weight is None:
             return utils_functional.linear_q8(x, self.weight)
         q, scale, _ = utils_functional.quantize_rows(x)
-        return utils_functional.matmul_q8(q, scale, *self._q8, dtype=x.dtype)
+        return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype)
 
 
 class NormLinear_Q8(Linear_Q8):
@@ -260,7 +294,8 @@ class NormLinear_Q8(Linear_Q8):
         self.eps = eps
 
     def forward(self, x, residual=None):
-        if self._q8 is None or torch.is_grad_enabled():
+        weight = self._prepared()
+        if weight is None:
             return utils_functional.norm_linear_q8(x, self.gain, self.weight, residual=residual, eps=self.eps)
         q, scale, total, _ = utils_functional.rms_norm_q8(x, self.gain, residual=residual, eps=self.eps)
-        return utils_functional.matmul_q8(q, scale, *self._q8, dtype=x.dtype), total
+        return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype), total
