@@ -253,10 +253,10 @@ std::tuple<MaybeTensor, MaybeTensor> matmul_q8_backward(const at::Tensor& grad, 
 {
     not_recorded();
     const Q8 x = as_q8(q, scale, "q"), w = as_q8(wq, wscale, "weight_q");
-    const Rows g = as_rows(grad, "gradient");
+    Rows g = as_rows(grad, "gradient");
+    if (g.rows > 1 && g.stride && g.stride < g.cols) g = as_rows(grad.contiguous(), "gradient");   // (rows that overlap)
     with(grad, "gradient", q, "q");
     TORCH_CHECK(x.r.cols == w.r.cols && g.rows == x.r.rows && g.cols == w.r.rows, "gradient must have the shape of the product");
-    TORCH_CHECK(g.cols <= 131071, "at most 131071 rows of weight_q in the backward");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
     MaybeTensor dx, dw;
     if (dx_type) dx = at::empty(q.sizes(), q.options().dtype(*dx_type));

@@ -1430,7 +1430,7 @@ int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, co
 int geo_sc_matmul_q8_backward_workspace_size(int64_t rows, int64_t cols, int64_t inner, int grad_dtype, int need_dx, int need_dw,
                                              size_t* bytes)
 {
-    if (!bytes || !sizes_fit(rows, cols, inner) || cols > 131071 || !dtype_known(grad_dtype)) return GEO_SC_ERR_INVALID_ARGUMENT;
+    if (!bytes || !sizes_fit(rows, cols, inner) || !dtype_known(grad_dtype)) return GEO_SC_ERR_INVALID_ARGUMENT;
     *bytes = need_dx || need_dw ? grad_layout(rows, cols, inner, terms_of(grad_dtype), need_dx, need_dw).bytes : 0;
     return GEO_SC_OK;
 }
@@ -1440,8 +1440,8 @@ int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64_t grad_str
                               int64_t inner, void* dx, int dx_dtype, void* dw, int dw_dtype, void* workspace, size_t workspace_bytes,
                               geo_sc_stream_t stream)
 {
-    if (!sizes_fit(rows, cols, inner) || cols > 131071 || !dtype_known(grad_dtype) || (dx && !dtype_known(dx_dtype)) ||
-        (dw && !dtype_known(dw_dtype)) || grad_stride < 0 || x_stride < 0 || w_stride < 0 || !grad || (dx && (!w || !w_scale)) ||
+    if (!sizes_fit(rows, cols, inner) || !dtype_known(grad_dtype) || (dx && !dtype_known(dx_dtype)) || (dw && !dtype_known(dw_dtype)) ||
+        grad_stride < 0 || (grad_stride && rows > 1 && grad_stride < cols) || x_stride < 0 || w_stride < 0 || !grad || (dx && (!w || !w_scale)) ||
         (dw && (!x || !x_scale)))
         return GEO_SC_ERR_INVALID_ARGUMENT;
     if (!dx && !dw) return GEO_SC_OK;

@@ -512,7 +512,8 @@ GEO_SC_API int geo_sc_rms_norm_q8_backward(const void* grad_values, int grad_dty
  * Backward, straight through the rounding of either operand, from g, the gradient of y: dx = (g w_scale) w of (rows, inner),
  * dw = (g x_scale)^T x of (cols, inner); either may be NULL.  The 8-bit operand enters exactly, the scaled gradient, each of its
  * rows brought to fp16's range by a power of two, as one fp16 number where g is bf16 and as the sum of two where it is fp16 or
- * fp32; sums in fp32.  cols at most 131071.
+ * fp32; sums in fp32, so that neither rows nor cols have a bound of their own.  The rows of g may be one and the same (grad_stride 0) but
+ * not overlap.
  */
 GEO_SC_API int geo_sc_matmul_q8_workspace_size(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows,
                                                int64_t cols, int64_t inner, size_t* bytes);
