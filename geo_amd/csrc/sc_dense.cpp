@@ -253,6 +253,11 @@ std::tuple<MaybeTensor, MaybeTensor> matmul_q8_backward(const at::Tensor& grad, 
 {
     not_recorded();
     const Q8 x = as_q8(q, scale, "q"), w = as_q8(wq, wscale, "weight_q");
+    if (w.r.rows == 0 && grad.numel() == 0) {   // no columns: sums of nothing
+        on_gpu(grad, "gradient");
+        return {dx_type ? MaybeTensor(at::zeros(q.sizes(), q.options().dtype(*dx_type))) : MaybeTensor(),
+                dw_type ? MaybeTensor(at::empty(wq.sizes(), q.options().dtype(*dw_type))) : MaybeTensor()};
+    }
     Rows g = as_rows(grad, "gradient");
     if (g.rows > 1 && g.stride && g.stride < g.cols) g = as_rows(grad.contiguous(), "gradient");   // (rows that overlap)
     with(grad, "gradient", q, "q");

@@ -38,3 +38,17 @@ def test_gradients_with_rows_that_overlap_or_are_one(uf):
         got = torch.autograd.grad(uf.linear_q8(x, w), (x, w), g)
         want = torch.autograd.grad(uf.linear_q8(x, w), (x, w), g.contiguous().clone())
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_no_columns_at_all(uf, dtype):
+    """sums of nothing"""
+    x, w = rand(5, 24, dtype=dtype, seed=1).requires_grad_(True), torch.empty(0, 24, dtype=dtype, device="cuda", requires_grad=True)
+    gain = torch.ones(24, dtype=dtype, device="cuda", requires_grad=True)
+    y = uf.linear_q8(x, w)
+    dx, dw = torch.autograd.grad(y.sum(), (x, w))
+    assert y.shape == (5, 0) and dx.shape == (5, 24) and dx.dtype == dtype and (dx == 0).all() and dw.shape == (0, 24)
+    y, total = uf.norm_linear_q8(x, gain, w, residual=x.detach())
+    h = rand(5, 24, dtype=dtype, seed=2)
+    dx, dgain, dw = torch.autograd.grad((y, total), (x, gain, w), (torch.empty_like(y), h))
+    assert torch.equal(dx, h) and (dgain == 0).all() and dw.shape == (0, 24)
