@@ -311,7 +311,8 @@ std::tuple<at::Tensor, at::Tensor> distill_topk(const at::Tensor& logits, const 
     const Rows z = as_rows(logits, "logits");
     const int dtype = dtype_of(logits.scalar_type(), "logits");
     TORCH_CHECK(logits.dim() >= 2, "logits must be (rows, columns)");
-    TORCH_CHECK(temperature > 0, "temperature must be positive");
+    TORCH_CHECK((float)temperature > 0 && (float)temperature * (float)temperature > 0 && std::isfinite((float)temperature * (float)temperature),
+                "temperature must be positive, its square a float that is neither 0 nor infinite");
     TORCH_CHECK(z.rows >= 1, "logits have no rows");
     const Top top = as_top(z, logits, top_logits, top_index);
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());

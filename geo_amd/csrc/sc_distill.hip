@@ -377,6 +377,8 @@ bool distill_sizes_fit(int64_t rows, int64_t cols, int top)
 {
     return rows >= 1 && rows <= 0x3fffffff && cols >= 1 && cols <= 0x7fffffff && top >= 1 && top <= kMaxTop;
 }
+// The loss takes T^2 as a factor; where that is a number above zero, so are 1 / T and log2(e) / T.
+bool temperature_fits(float t) { return t > 0.f && t * t > 0.f && t * t <= 3.402823466e38f; }
 constexpr int64_t kGroups = 1024;   // workgroups that few long rows are cut into
 float factor_of(int reduction, int64_t rows) { return reduction == GEO_SC_REDUCE_MEAN ? 1.f / (float)rows : 1.f; }
 
@@ -403,7 +405,7 @@ int geo_sc_distill_topk(const void* logits, int dtype, int64_t logits_stride, co
                         float* loss, float* stats, void* workspace, size_t workspace_bytes, geo_sc_stream_t stream)
 {
     if (!distill_sizes_fit(rows, cols, top) || !dtype_known(dtype) || !dtype_known(top_dtype) || (index_bytes != 4 && index_bytes != 8) ||
-        logits_stride < 0 || !(temperature > 0.f) || reduction < GEO_SC_REDUCE_NONE || reduction > GEO_SC_REDUCE_MEAN || !logits ||
+        logits_stride < 0 || !temperature_fits(temperature) || reduction < GEO_SC_REDUCE_NONE || reduction > GEO_SC_REDUCE_MEAN || !logits ||
         !top_logits || !top_index || !loss || !stats)
         return GEO_SC_ERR_INVALID_ARGUMENT;
     DistillArgs a = {};
@@ -437,7 +439,7 @@ int geo_sc_distill_topk_backward(const float* grad, int reduction, const void* l
                                  int64_t cols, int top, float temperature, const float* stats, void* dlogits, geo_sc_stream_t stream)
 {
     if (!distill_sizes_fit(rows, cols, top) || !dtype_known(dtype) || !dtype_known(top_dtype) || (index_bytes != 4 && index_bytes != 8) ||
-        logits_stride < 0 || !(temperature > 0.f) || reduction < GEO_SC_REDUCE_NONE || reduction > GEO_SC_REDUCE_MEAN || !grad ||
+        logits_stride < 0 || !temperature_fits(temperature) || reduction < GEO_SC_REDUCE_NONE || reduction > GEO_SC_REDUCE_MEAN || !grad ||
         !logits || !top_logits || !top_index || !stats || !dlogits)
         return GEO_SC_ERR_INVALID_ARGUMENT;
     DistillArgs a = {};

@@ -531,7 +531,7 @@ GEO_SC_API int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64
  * Distillation from a teacher's top logits at temperature T: per row p = softmax of the entries' top_logits / T, q = softmax of
  * logits / T over all columns, loss = T^2 sum_k p_k (log p_k - log q[top_index_k]).  top_logits and top_index are (rows, top) without
  * gaps, top at most 4096, index_bytes 4 or 8; an entry whose index is outside [0, cols) is absent, a column named twice counts
- * twice.  A row without entries has loss 0 and gradient 0.
+ * twice.  A row without entries has loss 0 and gradient 0.  T^2 must be a float that is neither 0 nor infinite.
  *   loss     rows floats (GEO_SC_REDUCE_NONE), or one: the rows' sum or mean (all rows count), in a fixed order
  *   stats    rows * 4 floats for the backward
  * Backward: grad points to rows floats or one, as loss does; dlogits (rows, cols) of the logits' dtype.
