@@ -286,12 +286,12 @@ class PatchMLP_q8(nn.Module):
         p = self.patch
         if h % p or w % p:
             raise ValueError(f"images of {h} x {w} have no whole patches of {p} x {p}")
-        rows = images.reshape(n, c, h // p, p, w // p, p).permute(0, 2, 4, 1, 3, 5).reshape(n, -1, c * p * p)
+        rows = images.reshape(n, c, h // p, p, w // p, p).permute(0, 2, 4, 1, 3, 5).reshape(n, h // p * (w // p), c * p * p)
         y, total = self.embed(rows), None
         for up, down in zip(self.up, self.down):
             wide, total = up(y, total)
             y = down(F.relu(wide))
-        logits, _ = self.head((total + y).mean(1))
+        logits, _ = self.head((y if total is None else total + y).mean(1))
         return logits
 
 
