@@ -306,7 +306,8 @@ __global__ __launch_bounds__(1024) void k_distill_back(DistillArgs a)
 
 constexpr int64_t kSplitLeast = 8192;   // columns that a split of a row has at least
 
-// Long rows, when there are few, are cut: enough workgroups for the compute units, at most 64 shares (the join is one wave).
+// Long rows, when there are few (fewer than `groups`, so that they fit the grid's second dimension), are cut: enough workgroups for the
+// compute units, at most 64 shares (the join is one wave).
 void cut_rows(DistillArgs& a, int64_t groups)
 {
     int64_t splits = (groups + a.rows - 1) / a.rows;
@@ -421,7 +422,6 @@ int geo_sc_distill_topk(const void* logits, int dtype, int64_t logits_stride, co
     a.temperature = temperature;
     a.factor = factor_of(reduction, rows);
     cut_rows(a, kGroups);
-    if (a.splits > 1 && rows > 65535) return GEO_SC_ERR_UNSUPPORTED;   // (cannot be: so many rows are not cut)
     size_t need = 0;
     geo_sc_distill_topk_workspace_size(rows, cols, &need);
     if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 4) return GEO_SC_ERR_WORKSPACE;

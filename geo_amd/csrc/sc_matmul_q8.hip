@@ -235,11 +235,7 @@ __device__ __forceinline__ Spot spot_of(const TwoProducts& both, uint32_t work)
     return p;
 }
 
-__device__ __forceinline__ int w_stage(const TileArgs& a, int k)   // (at most three terms)
-{
-    if (k >= a.w_stages) k -= a.w_stages;
-    return k >= a.w_stages ? k - a.w_stages : k;
-}
+__device__ __forceinline__ int w_stage(const TileArgs& a, int k) { return k >= a.w_stages ? k - a.w_stages : k; }   // (at most two terms)
 // row that a lane loads for the i-th time, from the tile's first; rows behind the operand's last are its last again, their
 // outputs are not stored
 __device__ __forceinline__ int64_t load_row(int64_t first, int64_t rows, int i, int wave, int lane)
