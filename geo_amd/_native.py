@@ -89,6 +89,7 @@ C_API = {
     "geo_sc_rms_norm_q8_backward": (ctypes.c_int, [_P, _I, _L, _P, _L, _P, _L, _P, _L, _P, _I, _L, _L, _P, _P, _P, _P,
                                                    ctypes.c_size_t, _P]),
     "geo_sc_matmul_q8_workspace_size": (ctypes.c_int, [_P, _L, _P, _L] + [_L] * 3 + [_SZ]),
+    "geo_sc_matmul_q8_plan": (ctypes.c_int, [_P, _L, _P, _L] + [_L] * 3 + [ctypes.POINTER(_I)] * 3),
     "geo_sc_matmul_q8": (ctypes.c_int, [_P, _L, _P, _P, _L, _P] + [_L] * 3 + [_P, _I, _P, ctypes.c_size_t, _P]),
     "geo_sc_matmul_q8_backward_workspace_size": (ctypes.c_int, [_L] * 3 + [_I] * 3 + [_SZ]),
     "geo_sc_matmul_q8_backward": (ctypes.c_int, [_P, _I, _L, _P, _L, _P, _P, _L, _P] + [_L] * 3 + [_P, _I, _P, _I, _P,

@@ -997,13 +997,19 @@ Copies copies_of(TileArgs a, const Plan& p, int64_t rows, int64_t cols)
     return {x ? align256((size_t)rows * stride) : 0, w ? align256((size_t)cols * stride) : 0};
 }
 
+// Measured, us: 4096 x 4096, k_few_rows / streamed: 1 row 5.0 / 5.2, 4 rows 5.4 / 5.2, 16 rows 6.4 / 5.5; 4096 x 1024: 3.2 / 3.8 for
+// any; 4096 x 16384: 16 rows 19.1 / 17.1, 48 rows 31 / 22, 64 rows 39 / 25.  Rows at odd addresses, 4096 x 16384: 1 row 18, 16 rows 24,
+// 48 rows 41 (loaded as they lie 34, 39, 112).
+bool is_streamed(const TileArgs& a)
+{
+    return a.splits == 1 && a.rows > 2 && a.inner >= 4 * kFewWaves * kStage && loads_fit(a.x, a.x_stride, 64, a.inner) &&
+           loads_fit(a.w, a.w_stride, 16, a.inner);
+}
+
 template <int MT>
 void run_few(const TileArgs& a, hipStream_t s)
 {
-    // Measured, us: 4096 x 4096, k_few_rows / streamed: 1 row 5.0 / 5.2, 4 rows 5.4 / 5.2, 16 rows 6.4 / 5.5; 4096 x 1024: 3.2 / 3.8 for
-    // any; 4096 x 16384: 16 rows 19.1 / 17.1, 48 rows 31 / 22, 64 rows 39 / 25.  Rows at odd addresses, 4096 x 16384: 1 row 18, 16 rows 24,
-    // 48 rows 41 (loaded as they lie 34, 39, 112).
-    if (a.splits == 1 && a.rows > 2 && a.inner >= 4 * kFewWaves * kStage && loads_fit(a.x, a.x_stride, 64, a.inner) && loads_fit(a.w, a.w_stride, 16, a.inner)) {
+    if (is_streamed(a)) {
         const int64_t tiles = (a.cols + 15) / 16;
         k_few_streamed<MT><<<dim3((uint32_t)(tiles < kUnits ? tiles : kUnits)), dim3(kFewWaves * 64), 0, s>>>(a);
         return;
@@ -1381,6 +1387,22 @@ int geo_sc_matmul_q8_workspace_size(const int8_t* x, int64_t x_stride, const int
     const Plan plan = forward_plan(x, x_stride, w, w_stride, rows, cols, inner, &a);
     const Copies copies = copies_of(a, plan, rows, cols);
     *bytes = partial_bytes(plan, 0, {rows, cols, inner}) + copies.x + copies.w;
+    return GEO_SC_OK;
+}
+
+int geo_sc_matmul_q8_plan(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t cols, int64_t inner,
+                          int* kernel, int* tile, int* splits)
+{
+    if (!kernel || !tile || !splits || !sizes_fit(rows, cols, inner) || x_stride < 0 || w_stride < 0) return GEO_SC_ERR_INVALID_ARGUMENT;
+    TileArgs a = {};
+    const Plan plan = forward_plan(x, x_stride, w, w_stride, rows, cols, inner, &a);
+    const Copies copies = copies_of(a, plan, rows, cols);
+    a.splits = plan.splits[0];
+    a.stages_per_split = plan.stages_per_split[0];
+    if (plan.few) *kernel = is_streamed(a) ? GEO_SC_Q8_FEW_STREAMED : GEO_SC_Q8_FEW_ROWS;
+    else *kernel = is_direct(a, plan.tile) || copies.x || copies.w ? GEO_SC_Q8_TILES : GEO_SC_Q8_TILES_ANY;
+    *tile = plan.few ? 16 * plan.few : plan.tile;
+    *splits = plan.splits[0];
     return GEO_SC_OK;
 }
 

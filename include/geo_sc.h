@@ -517,6 +517,10 @@ GEO_SC_API int geo_sc_rms_norm_q8_backward(const void* grad_values, int grad_dty
  */
 GEO_SC_API int geo_sc_matmul_q8_workspace_size(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows,
                                                int64_t cols, int64_t inner, size_t* bytes);
+/* What geo_sc_matmul_q8 does with such operands: the kernel, the rows of x that it takes at once, the cuts of the inner dimension. */
+enum geo_sc_q8_kernel { GEO_SC_Q8_FEW_ROWS = 0, GEO_SC_Q8_FEW_STREAMED = 1, GEO_SC_Q8_TILES = 2, GEO_SC_Q8_TILES_ANY = 3 };
+GEO_SC_API int geo_sc_matmul_q8_plan(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t cols,
+                                     int64_t inner, int* kernel, int* tile, int* splits);
 GEO_SC_API int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
                                 const float* w_scale, int64_t rows, int64_t cols, int64_t inner, void* y, int dtype, void* workspace,
                                 size_t workspace_bytes, geo_sc_stream_t stream);
