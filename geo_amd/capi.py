@@ -1,7 +1,9 @@
 """Python callers of the C ABI in ``include/geo_sc.h`` (ctypes, raw device pointers).
 
 torch is used for device memory and the current stream only; every function below is one
-C call.  These are what the GPU parity tests and the benchmark drive.
+C call.  These are what the GPU parity tests and the benchmark drive.  Where a function takes
+``stream``, the inputs have to be ready on it; results that the function allocates may be used on
+the current stream right away, results in the caller's ``out`` once that stream is through.
 """
 from __future__ import annotations
 

@@ -414,7 +414,7 @@ __device__ __forceinline__ void finish_tile(const Spot& p, typename Matrix<INT8>
 // kRing stages: while a wave multiplies stage s out of registers, stage s + 1 moves from LDS to its other registers and the stages
 // up to s + kRing are on their way.  One barrier per stage: it says that every wave's share of stage s + 1 has come and
 // that all have read stage s, whose place stage s + kRing takes.
-// Bound by power: 8192 x 16384 x 4096 in 448 us (2.46 POP/s) at 1.95 GHz, where the products alone run at 2.17; both gradients of
+// Bound by power: 8192 x 16384 x 4096 in 446 - 452 us (2.43 - 2.46 POP/s) at 1.95 GHz, where the products alone run at 2.17; both gradients of
 // 4096 x 4096 x 4096 bf16 in 200 us (1.37 PFLOP/s).
 template <int B, bool INT8>
 __global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)

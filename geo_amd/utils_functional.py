@@ -218,7 +218,8 @@ def matmul_q8(q, scale, weight_q, weight_scale, dtype=torch.float32):
 
 def linear_q8(x, weight):
     """``x @ weight.t()`` with both operands rounded to 8-bit rows first, in ``x``'s type.  The gradients are those of the
-    product at the rounded operands, passed straight through the rounding, as ``Conv2d_Add_Partial`` passes its own."""
+    product at the rounded operands, passed straight through the rounding, as ``Conv2d_Add_Partial`` passes its own.  The upstream
+    gradient, times a scale, enters them with 11 bits where it is bfloat16 and with 23 where it is float16 or float32."""
     return _dense().linear_q8(x, weight)
 
 
