@@ -32,6 +32,19 @@ class Options(ctypes.Structure):
                 ("backward_operand_bits", ctypes.c_int32)]
 
 
+class AdamWTensor(ctypes.Structure):
+    """geo_sc_adamw_tensor of include/geo_sc.h"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "avg_scale", "sq_scale", "copy", "clamped")] + \
+               [("elements", ctypes.c_int64)]
+
+
+class AdamWOptions(ctypes.Structure):
+    """geo_sc_adamw_options of include/geo_sc.h"""
+    _fields_ = [("struct_bytes", ctypes.c_size_t)] + [(n, ctypes.c_int32) for n in ("param_dtype", "grad_dtype", "copy_dtype", "state_bits")] + \
+               [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "grad_scale")] + \
+               [("lo", ctypes.c_float), ("hi", ctypes.c_float), ("step", ctypes.c_int64), ("device_step", ctypes.c_void_p)]
+
+
 # every symbol include/geo_sc.h declares: name -> (restype, argtypes)
 _P = ctypes.c_void_p
 _SZ = ctypes.POINTER(ctypes.c_size_t)
@@ -99,6 +112,7 @@ C_API = {
                                            ctypes.c_size_t, _P]),
     "geo_sc_distill_topk_backward": (ctypes.c_int, [_P, _I, _P, _I, _L, _P, _I, _P, _I, _L, _L, _I, ctypes.c_float, _P,
                                                     _P, _P]),
+    "geo_sc_adamw": (ctypes.c_int, [_I, ctypes.POINTER(AdamWTensor), ctypes.POINTER(AdamWOptions), _P, ctypes.c_size_t, _P]),
 }
 
 _lib = None

@@ -1,4 +1,4 @@
-// PyTorch module `sc_dense`: the dense 8-bit layers and the distillation loss of libgeo_sc.so on tensors.  Checks, outputs
+// PyTorch module `sc_dense`: the dense 8-bit layers, the distillation loss and the AdamW step of libgeo_sc.so on tensors.  Checks, outputs
 // and workspaces from the caching allocator, launch on PyTorch's current HIP stream.  In C++ because a single
 // token's call is bound by its host time.
 #include "sc_torch_common.h"
@@ -6,6 +6,10 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
+
+#include <array>
+#include <map>
+#include <unordered_set>
 
 using namespace geo_sc_torch;
 
@@ -40,7 +44,7 @@ void not_recorded()
 {
     TORCH_CHECK(!torch::jit::tracer::isTracing() &&
                     !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
-                "the dense 8-bit layers and the distillation loss cannot be traced");
+                "the dense 8-bit layers, the distillation loss and the AdamW step cannot be traced");
 }
 
 geo_sc_stream_t stream_of(const at::Tensor& t)
@@ -348,6 +352,116 @@ at::Tensor distill_topk_backward(const at::Tensor& grad, const at::Tensor& logit
     return once(dz, {grad});
 }
 
+// ---------------------------------------------------------------- AdamW
+
+using Tensors = std::vector<at::Tensor>;
+using MaybeTensors = std::optional<Tensors>;
+
+// What one of the lists of a step must be: on the GPU of the first parameter, side by side, of the parameter's element count (of its
+// blocks'), of the type or types named.
+void in_step(const at::Tensor& t, const char* what, const at::Tensor& first, int64_t elements, std::initializer_list<at::ScalarType> types)
+{
+    with(t, what, first, "params");
+    TORCH_CHECK(t.is_contiguous(), what, " must be contiguous");
+    TORCH_CHECK(t.numel() == elements, what, " must have ", elements, " elements, got ", t.numel());
+    for (const at::ScalarType type : types)
+        if (t.scalar_type() == type) return;
+    TORCH_CHECK(false, what, " must not be ", t.scalar_type());
+}
+
+constexpr int64_t kStateBlock = 256;
+
+void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_avg, const Tensors& exp_avg_sq, int64_t step,
+                const MaybeTensor& device_step, double lr, double beta1, double beta2, double eps, double weight_decay, double grad_scale,
+                const MaybeTensors& avg_scales, const MaybeTensors& sq_scales, const MaybeTensors& copies,
+                const std::optional<std::vector<MaybeTensor>>& clamped, double lo, double hi)
+{
+    not_recorded();
+    const size_t n = params.size();
+    TORCH_CHECK(grads.size() == n && exp_avg.size() == n && exp_avg_sq.size() == n && (!avg_scales || avg_scales->size() == n) &&
+                    (!sq_scales || sq_scales->size() == n) && (!copies || copies->size() == n) && (!clamped || clamped->size() == n),
+                "the lists of a step must be of one length");
+    TORCH_CHECK(lr >= 0 && eps >= 0 && weight_decay >= 0 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && lo <= hi,
+                "lr, eps and weight_decay must not be negative, the betas must be in [0, 1), the bounds in order");
+    TORCH_CHECK(device_step || step >= 1, "the number of a step is 1 or more");
+    if (!n) return;
+    const at::Tensor& first = params[0];
+    const bool eight = avg_scales.has_value();
+    if (device_step) in_step(*device_step, "step", first, 1, {at::kLong});
+    // Tensors of the same types go into one call; no writer meets another.
+    typedef std::array<int, 3> Types;
+    std::map<Types, std::vector<geo_sc_adamw_tensor>> calls;
+    std::unordered_set<const void*> written;
+    const auto write = [&](const at::Tensor& t, const char* what) {
+        TORCH_CHECK(t.numel() == 0 || written.insert(t.data_ptr()).second, what, ": a step writes no tensor twice");
+        return t.data_ptr();
+    };
+    for (size_t i = 0; i < n; ++i) {
+        const int64_t elements = params[i].numel(), blocks = (elements + kStateBlock - 1) / kStateBlock;
+        geo_sc_adamw_tensor t = {};
+        t.elements = elements;
+        in_step(params[i], "params", first, elements, {at::kFloat, at::kBFloat16, at::kHalf});
+        in_step(grads[i], "grads", first, elements, {at::kFloat, at::kBFloat16, at::kHalf});
+        t.param = write(params[i], "params");
+        t.grad = grads[i].const_data_ptr();
+        for (const auto& [state, scales, what, codes, scale] : {std::make_tuple(&exp_avg, &avg_scales, "exp_avg", &t.exp_avg, &t.avg_scale),
+                                                                std::make_tuple(&exp_avg_sq, &sq_scales, "exp_avg_sq", &t.exp_avg_sq, &t.sq_scale)}) {
+            in_step((*state)[i], what, first, elements, {eight ? at::kFloat8_e4m3fn : at::kFloat});
+            *codes = write((*state)[i], what);
+            if (!eight) continue;
+            in_step((**scales)[i], "scales", first, blocks, {at::kFloat8_e8m0fnu});
+            *scale = (uint8_t*)write((**scales)[i], "scales");
+        }
+        if (copies) {
+            in_step((*copies)[i], "copies", first, elements, {at::kFloat, at::kBFloat16, at::kHalf});
+            t.copy = write((*copies)[i], "copies");
+        }
+        if (clamped && (*clamped)[i]) {
+            in_step(*(*clamped)[i], "clamped", first, elements, {at::kFloat});
+            t.clamped = (float*)write(*(*clamped)[i], "clamped");
+        }
+        calls[{dtype_of(params[i].scalar_type(), "params"), dtype_of(grads[i].scalar_type(), "grads"),
+               copies ? dtype_of((*copies)[i].scalar_type(), "copies") : 0}]
+            .push_back(t);
+    }
+    TORCH_CHECK(!device_step || calls.size() == 1, "a step that is counted on the GPU takes tensors of the same types");
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(first.device());
+    at::Tensor workspace;
+    if (device_step) workspace = at::empty({16}, first.options().dtype(at::kByte));
+    for (const auto& [types, tensors] : calls) {
+        geo_sc_adamw_options o = {};
+        o.struct_bytes = sizeof o;
+        o.param_dtype = types[0];
+        o.grad_dtype = types[1];
+        o.copy_dtype = types[2];
+        o.state_bits = eight ? 8 : 32;
+        o.lr = lr;
+        o.beta1 = beta1;
+        o.beta2 = beta2;
+        o.eps = eps;
+        o.weight_decay = weight_decay;
+        o.grad_scale = grad_scale;
+        o.lo = (float)lo;
+        o.hi = (float)hi;
+        o.step = step;
+        o.device_step = device_step ? device_step->data_ptr<int64_t>() : nullptr;
+        check_status(geo_sc_adamw((int)tensors.size(), tensors.data(), &o, device_step ? workspace.data_ptr() : nullptr, device_step ? 16 : 0,
+                                  stream_of(first)),
+                     "adamw_step");
+    }
+    // (for whoever watches a tensor's version: autograd, prepared weights)
+    const auto changed = [](const at::Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); };
+    for (const Tensors* list : {&params, &exp_avg, &exp_avg_sq})
+        for (const at::Tensor& t : *list) changed(t);
+    for (const MaybeTensors* list : {&avg_scales, &sq_scales, &copies})
+        if (*list)
+            for (const at::Tensor& t : **list) changed(t);
+    if (clamped)
+        for (const MaybeTensor& t : *clamped)
+            if (t) changed(*t);
+    if (device_step) changed(*device_step);
+}
+
 // ---------------------------------------------------------------- autograd nodes
 //
 // In C++ like the calls themselves: of a training step on small layers the host's time is what counts, and the backward runs in
@@ -476,6 +590,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         const variable_list out = NormLinearQ8::apply(x, gain, weight, residual, eps);
         return std::make_tuple(out[0], residual ? out[1] : x);
     }, "the norm and the product: (y, total)");
+    m.def("adamw_step", &adamw_step, "one AdamW step on lists of tensors");
     m.def("distill_topk", [](const at::Tensor& logits, const at::Tensor& top_logits, const at::Tensor& top_index, double temperature, int64_t reduction) {
         return DistillTopK::apply(logits, top_logits, top_index, temperature, reduction);
     }, "divergence from a teacher's top logits");

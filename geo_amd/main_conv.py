@@ -31,7 +31,7 @@ def build_parser():
     p.add_argument("--dataset", default="CIFAR10", type=str, help="CIFAR10, SVHN or SYNTHETIC")
     p.add_argument("--seed", default=0, type=int)
     p.add_argument("--device", default=0, type=int, help="GPU id (this build has no CPU path: -1 is refused)")
-    p.add_argument("--optim", default="Adam", type=str, help="Adam, RMSprop or SGD")
+    p.add_argument("--optim", default="Adam", type=str, help="Adam, AdamW, AdamW8 (states in 8 bits), RMSprop or SGD")
     p.add_argument("--lr", default=2e-3, type=float)
     p.add_argument("--err", default="7777", type=str, help="stream length per layer as 2**digit")
     p.add_argument("--z_unit", default="3344", type=str, help="channels per OR group per layer as 2**digit (yz_bin)")
@@ -136,12 +136,14 @@ def main(argv=None):
     param_copy = [p.clone().cuda(args.device).float().detach().requires_grad_(True) for p in net.parameters()]
     if args.optim == "Adam":
         optimizer = optim.Adam(param_copy, lr=args.lr, weight_decay=0)
+    elif args.optim in ("AdamW", "AdamW8"):   # (all tensors of the step in one kernel; states in 32 bits or in 8)
+        optimizer = network.AdamW(param_copy, lr=args.lr, weight_decay=0, state_bits=8 if args.optim == "AdamW8" else 32)
     elif args.optim == "RMSprop":
         optimizer = optim.RMSprop(param_copy, lr=args.lr, weight_decay=0)
     elif args.optim == "SGD":
         optimizer = optim.SGD(param_copy, lr=args.lr, weight_decay=0, momentum=0.01)
     else:
-        raise SystemExit(f"unknown optimiser {args.optim!r}: Adam, RMSprop or SGD")
+        raise SystemExit(f"unknown optimiser {args.optim!r}: Adam, AdamW, AdamW8, RMSprop or SGD")
     scheduler = optim.lr_scheduler.ReduceLROnPlateau(optimizer=optimizer, factor=0.3, patience=150, threshold=0.05)
     best = -1.0
     history = []

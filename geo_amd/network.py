@@ -300,6 +300,102 @@ def make_param_copies(model):
     return [p.detach().clone().float().requires_grad_(True) for p in model.parameters()]
 
 
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) with all tensors of a step in one kernel (``utils_functional.adamw_step``), states in 32 bits or in
+    8.  Parameters are contiguous GPU tensors of float32, bfloat16 or float16; gradients of any of these types.
+
+    ``capturable=True`` counts the steps on the GPU, for steps that are recorded into a graph (``GraphedTrainStep``), where the learning rate
+    is recorded with them.  ``apply_update`` hands it the unscaling of the gradients and the copies into the parameters as well."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, capturable=False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas)):
+            raise ValueError("lr, eps and weight_decay must not be negative, betas in [0, 1)")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      capturable=capturable))
+
+    def _fresh(self, p, group, step):
+        like = lambda n, dtype: torch.zeros(n, dtype=dtype, device=p.device)   # noqa: E731
+        state = dict(step=step)
+        if group["state_bits"] == 8:
+            blocks = (p.numel() + 255) // 256
+            state.update(exp_avg=like(p.shape, torch.float8_e4m3fn), exp_avg_sq=like(p.shape, torch.float8_e4m3fn),
+                         avg_scale=like(blocks, torch.float8_e8m0fnu), sq_scale=like(blocks, torch.float8_e8m0fnu))
+        else:
+            state.update(exp_avg=like(p.shape, torch.float32), exp_avg_sq=like(p.shape, torch.float32))
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_scale=1.0, grads=None, copies=None, clamped=None, bounds=(-1.0, 0.999)):
+        """One step.  ``grads``, ``copies``, ``clamped``: dicts from parameters to tensors; a gradient that is not among them is the
+        parameter's own, a parameter without one stays as it is."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        from . import utils_functional as uf
+        for group in self.param_groups:
+            # parameters that have made the same number of steps; those counted on the GPU, that are counted together
+            rows, counter = {}, None
+            for p in group["params"]:
+                g = (grads or {}).get(p, p.grad)
+                if g is None:
+                    continue
+                if g.is_sparse:
+                    raise RuntimeError("AdamW takes no sparse gradients")
+                state = self.state[p]
+                if not state:
+                    if group["capturable"]:
+                        counter = torch.zeros((), dtype=torch.int64, device=p.device) if counter is None else counter
+                    state.update(self._fresh(p, group, counter if group["capturable"] else 0))
+                if not group["capturable"]:
+                    state["step"] += 1
+                step = state["step"]
+                copy = None if copies is None else copies.get(p)
+                # one call per device, number of steps and set of types (those that are not counted on the GPU may mix them)
+                types = (p.dtype, g.dtype) if group["capturable"] else None
+                key = (p.device, id(step) if group["capturable"] else step, types, None if copy is None else copy.dtype)
+                rows.setdefault(key, (step, []))[1].append((p, g.contiguous(), state, copy))
+            counted = [step for step, _ in rows.values()]
+            if group["capturable"] and len({id(s) for s in counted}) < len(counted):
+                raise RuntimeError("AdamW(capturable=True) takes parameters, gradients and copies of one type each in a group")
+            for step, row in rows.values():
+                states = [state for _, _, state, _ in row]
+                uf.adamw_step([p for p, _, _, _ in row], [g for _, g, _, _ in row], [s["exp_avg"] for s in states],
+                              [s["exp_avg_sq"] for s in states], step, group["lr"], group["betas"], group["eps"], group["weight_decay"],
+                              grad_scale, scales=([s["avg_scale"] for s in states], [s["sq_scale"] for s in states])
+                              if group["state_bits"] == 8 else None,
+                              copies=None if row[0][3] is None else [c for _, _, _, c in row],
+                              clamped=None if clamped is None else [clamped.get(p) for p, _, _, _ in row], bounds=bounds)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """States come back in their own types (the base class would bring them to the parameters'); steps counted on the GPU are
+        counted together again where they are equal."""
+        super().load_state_dict(state_dict)
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, (p, group) in zip(saved, ((p, group) for group in self.param_groups for p in group["params"])):
+            if i not in state_dict["state"]:
+                continue
+            state = self._fresh(p, group, 0)
+            for k, v in state_dict["state"][i].items():
+                if k == "step":
+                    v = int(v)
+                elif v.dtype != state[k].dtype or v.numel() != state[k].numel():
+                    raise ValueError(f"{k} of a parameter of {tuple(p.shape)} does not fit states of {group['state_bits']} bits")
+                else:
+                    v = v.to(p.device, copy=True)
+                state[k] = v
+            self.state[p] = state
+        for group in self.param_groups:
+            together = {}
+            for p in group["params"] if group["capturable"] else ():
+                if self.state.get(p):
+                    step = self.state[p]["step"]
+                    self.state[p]["step"] = together.setdefault((p.device, step), torch.full((), step, dtype=torch.int64, device=p.device))
+
+
 def apply_update(model, optimizer, param_copy):
     """The part of the reference's step that follows ``loss.backward()`` (utils_own.py:98-114): restore
     the full-precision weights, hand the gradients to the master copies and un-scale them, optimiser
@@ -307,6 +403,11 @@ def apply_update(model, optimizer, param_copy):
     # (the reference first copies weight_org back into weight.data; the copy-back from the master copies below
     # overwrites every parameter before anything reads it, so that copy changes nothing and is not launched)
     params = list(model.parameters())
+    orgs = {id(m.weight): m.weight_org for m in model.modules() if hasattr(m, "weight_org")}
+    if isinstance(optimizer, AdamW) and all(p.is_cuda and p.data.is_contiguous() for p in params) and \
+            all(o.dtype == torch.float32 and o.is_contiguous() for o in orgs.values()):
+        _apply_adamw(params, orgs, optimizer, param_copy)
+        return
     # the per-parameter loops of the reference as multi-tensor calls: one kernel for all gradients,
     # one for all copies
     with_grad = [(master, p) for master, p in zip(param_copy, params) if p.grad is not None]
@@ -317,7 +418,6 @@ def apply_update(model, optimizer, param_copy):
         for (master, _), g in zip(with_grad, scaled):
             master.grad = g
     optimizer.step()
-    orgs = {id(m.weight): m.weight_org for m in model.modules() if hasattr(m, "weight_org")}
     if all(p.is_cuda and p.dtype == torch.float32 and p.data.is_contiguous() for p in params):
         # copy back and refresh weight_org, all parameters in one launch
         from . import capi
@@ -326,6 +426,22 @@ def apply_update(model, optimizer, param_copy):
     else:
         torch._foreach_copy_([p.data for p in params], [master.data for master in param_copy])
         for p in params:
+            if id(p) in orgs:
+                torch.clamp(p.data, -1, 0.999, out=orgs[id(p)])
+    optimizer.zero_grad()
+
+
+def _apply_adamw(params, orgs, optimizer, param_copy):
+    """``apply_update`` with the unscaling, the copies back and ``weight_org`` in the optimiser's kernel."""
+    stepped = [(master, p) for master, p in zip(param_copy, params) if p.grad is not None]
+    for master in param_copy:
+        master.grad = None
+    optimizer.step(grads={master: p.grad for master, p in stepped}, grad_scale=1 / SCALE_FACTOR,
+                   copies={master: p.data for master, p in stepped},
+                   clamped={master: orgs[id(p)] for master, p in stepped if id(p) in orgs}, bounds=(-1, 0.999))
+    for master, p in zip(param_copy, params):   # (what has no gradient is copied back all the same: the layers have quantised it)
+        if p.grad is None:
+            p.data.copy_(master.data)
             if id(p) in orgs:
                 torch.clamp(p.data, -1, 0.999, out=orgs[id(p)])
     optimizer.zero_grad()

@@ -246,3 +246,26 @@ def distill_topk(logits, top_logits, top_index, temperature=1.0, reduction="mean
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     return _dense().distill_topk(logits, top_logits, top_index, temperature, _REDUCTIONS[reduction])
+
+
+# ---------------------------------------------------------------- optimiser step
+
+def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, grad_scale=1.0, scales=None,
+               copies=None, clamped=None, bounds=(-1.0, 0.999)):
+    """One AdamW step on lists of contiguous GPU tensors, in place, in fp32 operations whatever their types: with t = ``step`` and
+    g = ``grads * grad_scale``::
+
+        m = beta1 m + (1 - beta1) g;   v = beta2 v + (1 - beta2) g^2
+        params = params (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+
+    ``params`` and ``grads`` are float32, bfloat16 or float16.  States of 32 bits: ``exp_avg`` and ``exp_avg_sq`` hold m and v
+    (float32).  States of 8 bits, where ``scales`` is a pair of lists: ``exp_avg`` holds m, ``exp_avg_sq`` the root of v, both
+    as ``torch.float8_e4m3fn`` numbers times a power of two (``torch.float8_e8m0fnu``) for each 256 elements of the flattened tensor; numbers
+    between two codes go up or down so that the mean over steps is right.  All-zero states (scales too) are those of no step.
+
+    ``step`` is the number of this step, from 1 on, or an int64 GPU tensor of one element that holds the number of steps done, which
+    the call counts up: that is the form to record in a graph.  ``copies``: tensors that receive the new parameters, before their rounding, in a
+    type of their own.  ``clamped``: float32 tensors (or None) that receive them clamped to ``bounds``."""
+    counted = step if torch.is_tensor(step) else None
+    _dense().adamw_step(params, grads, exp_avg, exp_avg_sq, 0 if counted is not None else step, counted, lr, betas[0], betas[1], eps,
+                        weight_decay, grad_scale, scales[0] if scales else None, scales[1] if scales else None, copies, clamped, *bounds)

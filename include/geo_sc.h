@@ -551,6 +551,48 @@ GEO_SC_API int geo_sc_distill_topk_backward(const float* grad, int reduction, co
                                             int64_t rows, int64_t cols, int top, float temperature, const float* stats, void* dlogits,
                                             geo_sc_stream_t stream);
 
+/*
+ * One AdamW step on many tensors, of any element counts, none of them named twice: in fp32 operations on each element, with t the
+ * number of this step (from 1 on) and g = grad * grad_scale:
+ *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2,
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * rounded once to the type of param.  Elements of a tensor lie side by side, at any multiple of the element.
+ *   state_bits 32   exp_avg and exp_avg_sq are m and v in fp32
+ *   state_bits 8    exp_avg is m and exp_avg_sq the ROOT of v as 8-bit floats (4 bits of exponent from 2^-6, 3 of mantissa, largest
+ *                   448), times a power of two for each 256 elements of the tensor: avg_scale and sq_scale hold, one byte each,
+ *                   its exponent plus 127.  It brings the largest finite number of the 256 to 128 .. 256.  A number between
+ *                   two codes goes up or down by a fixed sequence over steps and places that fills the interval evenly, so
+ *                   that changes of less than half a code add up; a root above zero is no code of zero; infinities and NaN become
+ *                   NaN and leave the others of the 256 alone.
+ *   copy            NULL, or the new param, before its rounding, in copy_dtype
+ *   clamped         NULL, or the new param, before its rounding, clamped to [lo, hi] in fp32 (NaN stays NaN)
+ *   device_step     NULL: the number of this step is `step`.  Else a device pointer to the number of steps done: the call adds
+ *                   one and takes that (so that the call can be recorded in a graph and replayed), through the workspace (16
+ *                   bytes, 8-byte aligned); `step` is not read
+ * The arrays `tensors` and `options` are read during the call.
+ */
+typedef struct geo_sc_adamw_tensor {
+    void* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    uint8_t* avg_scale;
+    uint8_t* sq_scale;
+    void* copy;
+    float* clamped;
+    int64_t elements;
+} geo_sc_adamw_tensor;
+typedef struct geo_sc_adamw_options {
+    size_t struct_bytes; /* sizeof(geo_sc_adamw_options) */
+    int32_t param_dtype, grad_dtype, copy_dtype, state_bits;
+    double lr, beta1, beta2, eps, weight_decay, grad_scale;
+    float lo, hi;
+    int64_t step;
+    int64_t* device_step;
+} geo_sc_adamw_options;
+GEO_SC_API int geo_sc_adamw(int count, const geo_sc_adamw_tensor* tensors, const geo_sc_adamw_options* options, void* workspace,
+                            size_t workspace_bytes, geo_sc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
