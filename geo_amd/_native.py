@@ -45,6 +45,14 @@ class AdamWOptions(ctypes.Structure):
                [("lo", ctypes.c_float), ("hi", ctypes.c_float), ("step", ctypes.c_int64), ("device_step", ctypes.c_void_p)]
 
 
+class GatedNormDesc(ctypes.Structure):
+    """geo_sc_gated_norm_desc of include/geo_sc.h"""
+    _fields_ = [("struct_bytes", ctypes.c_size_t)] + \
+               [(n, ctypes.c_void_p) for n in ("x", "residual", "weight", "post_weight", "gate", "residual_scale")] + \
+               [(n, ctypes.c_int64) for n in ("rows", "cols", "x_stride", "residual_stride", "rows_per_gate")] + \
+               [("eps", ctypes.c_float), ("dtype", ctypes.c_int32)]
+
+
 # every symbol include/geo_sc.h declares: name -> (restype, argtypes)
 _P = ctypes.c_void_p
 _SZ = ctypes.POINTER(ctypes.c_size_t)
@@ -112,6 +120,10 @@ C_API = {
                                            ctypes.c_size_t, _P]),
     "geo_sc_distill_topk_backward": (ctypes.c_int, [_P, _I, _P, _I, _L, _P, _I, _P, _I, _L, _L, _I, ctypes.c_float, _P,
                                                     _P, _P]),
+    "geo_sc_gated_norm": (ctypes.c_int, [ctypes.POINTER(GatedNormDesc)] + [_P] * 4),
+    "geo_sc_gated_norm_q8": (ctypes.c_int, [ctypes.POINTER(GatedNormDesc), _P, _L] + [_P] * 3 + [_I, _P]),
+    "geo_sc_gated_norm_backward_workspace_size": (ctypes.c_int, [_L, _L, _SZ]),
+    "geo_sc_gated_norm_backward": (ctypes.c_int, [ctypes.POINTER(GatedNormDesc), _P, _L, _P, _L] + [_P] * 8 + [ctypes.c_size_t, _P]),
     "geo_sc_adamw": (ctypes.c_int, [_I, ctypes.POINTER(AdamWTensor), ctypes.POINTER(AdamWOptions), _P, ctypes.c_size_t, _P]),
 }
 

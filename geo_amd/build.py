@@ -23,7 +23,7 @@ OBJDIR = os.path.join(LIBDIR, "obj")
 INCLUDE = os.path.join(ROOT, "include")
 
 HIP_SOURCES = ["sc_streams.hip", "sc_conv_fwd.hip", "sc_conv_bwd.hip", "sc_epilogue.hip", "sc_rows_q8.hip",
-               "sc_matmul_q8.hip", "sc_distill.hip", "sc_adamw.hip", "sc_api.hip"]
+               "sc_matmul_q8.hip", "sc_distill.hip", "sc_adamw.hip", "sc_gated_norm.hip", "sc_api.hip"]
 PROBE_SOURCE = "sc_probe.hip"   # the benchmark's issue-rate probe: a library of its own, outside the C ABI
 TORCH_MODULES = {"sc_extension_cuda": "sc_extension_cuda.cpp", "sc_extension": "sc_extension.cpp",
                  "sc_dense": "sc_dense.cpp"}

@@ -192,6 +192,137 @@ std::tuple<at::Tensor, MaybeTensor> rms_norm_q8_backward(const MaybeTensor& grad
     return {once(dx, {*grad_values, sum_grad}), dw};
 }
 
+// ---------------------------------------------------------------- gated norm
+
+// The description of a call, and the tensors that it points into.
+struct Gated {
+    Rows x, residual;
+    at::Tensor weight;
+    MaybeTensor post, gate, scale;
+    geo_sc_gated_norm_desc desc;
+};
+Gated as_gated(const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight, const MaybeTensor& post, const MaybeTensor& gate,
+               const MaybeTensor& scale, double eps)
+{
+    Gated g;
+    g.x = as_rows(x, "x");
+    const int dtype = dtype_of(x.scalar_type(), "x");
+    with(residual, "residual", x, "x");
+    TORCH_CHECK(residual.sizes() == x.sizes() && residual.scalar_type() == x.scalar_type(), "residual must have the shape and type of x");
+    g.residual = as_rows(residual, "residual");
+    const auto per_channel = [&](const at::Tensor& t, const char* what) {
+        with(t, what, x, "x");
+        TORCH_CHECK(t.dim() == 1 && t.size(0) == g.x.cols, what, " must have the ", g.x.cols, " elements of a row of x");
+        TORCH_CHECK(t.scalar_type() == x.scalar_type(), what, " must have the type of x");
+        return t.contiguous();
+    };
+    g.weight = per_channel(weight, "weight");
+    if (post) g.post = per_channel(*post, "post_weight");
+    if (scale) g.scale = per_channel(*scale, "residual_scale");
+    TORCH_CHECK(eps >= 0, "eps must not be negative");
+    g.desc = {};
+    g.desc.rows_per_gate = 1;
+    if (gate && gate->dim() == 1) {
+        g.gate = per_channel(*gate, "gate");
+        g.desc.rows_per_gate = g.x.rows > 0 ? g.x.rows : 1;
+    } else if (gate) {
+        with(*gate, "gate", x, "x");
+        TORCH_CHECK(gate->scalar_type() == x.scalar_type(), "gate must have the type of x");
+        TORCH_CHECK(gate->dim() == x.dim() && gate->size(-1) == g.x.cols, "gate must have the ", g.x.cols,
+                    " elements of a row of x, or the dimensions of x");
+        // x's leading dimensions, then ones: rows that share a gate follow each other
+        int64_t d = x.dim() - 2, shared = 1;
+        for (; d >= 0 && gate->size(d) == 1; --d) shared *= x.size(d);
+        for (; d >= 0; --d) TORCH_CHECK(gate->size(d) == x.size(d), "gate must have x's leading dimensions, then ones");
+        g.gate = gate->contiguous();
+        g.desc.rows_per_gate = shared > 0 ? shared : 1;
+    }
+    g.desc.struct_bytes = sizeof g.desc;
+    g.desc.x = g.x.t.const_data_ptr();
+    g.desc.residual = g.residual.t.const_data_ptr();
+    g.desc.weight = g.weight.const_data_ptr();
+    g.desc.post_weight = g.post ? g.post->const_data_ptr() : nullptr;
+    g.desc.gate = g.gate ? g.gate->const_data_ptr() : nullptr;
+    g.desc.residual_scale = g.scale ? g.scale->const_data_ptr() : nullptr;
+    g.desc.rows = g.x.rows;
+    g.desc.cols = g.x.cols;
+    g.desc.x_stride = g.x.stride;
+    g.desc.residual_stride = g.residual.stride;
+    g.desc.eps = (float)eps;
+    g.desc.dtype = dtype;
+    return g;
+}
+
+// (out, total, rstd)
+std::tuple<at::Tensor, at::Tensor, MaybeTensor> gated_norm(const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight,
+                                                           const MaybeTensor& post, const MaybeTensor& gate, const MaybeTensor& scale, double eps,
+                                                           bool for_backward)
+{
+    not_recorded();
+    const Gated g = as_gated(x, residual, weight, post, gate, scale, eps);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    const at::Tensor out = at::empty(x.sizes(), x.options()), total = at::empty(x.sizes(), x.options());
+    MaybeTensor rstd;
+    if (for_backward) rstd = at::empty({g.x.rows, 2}, x.options().dtype(at::kFloat));
+    check_status(geo_sc_gated_norm(&g.desc, out.data_ptr(), total.data_ptr(), (float*)data_of(rstd), stream_of(x)), "gated_norm");
+    return {out, total, rstd};
+}
+
+// (q, scale, total, values)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, MaybeTensor> gated_norm_q8(const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight,
+                                                                          const MaybeTensor& post, const MaybeTensor& gate, const MaybeTensor& scale,
+                                                                          double eps, std::optional<at::ScalarType> values_type)
+{
+    not_recorded();
+    const Gated g = as_gated(x, residual, weight, post, gate, scale, eps);
+    const int vtype = values_type ? dtype_of(*values_type, "values") : 0;
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    const at::Tensor q = empty_q(x.sizes(), x.options()), q_scale = row_scalars(x), total = at::empty(x.sizes(), x.options());
+    MaybeTensor values;
+    if (values_type) values = at::empty(x.sizes(), x.options().dtype(*values_type));
+    check_status(geo_sc_gated_norm_q8(&g.desc, q.data_ptr<int8_t>(), (g.x.cols + 15) / 16 * 16, q_scale.data_ptr<float>(), total.data_ptr(),
+                                      data_of(values), vtype, stream_of(x)),
+                 "gated_norm_q8");
+    return {q, q_scale, total, values};
+}
+
+struct GatedGradients {
+    at::Tensor x, residual;
+    MaybeTensor weight, post, gate, scale;
+};
+// `wanted`: of weight, post, gate, scale
+GatedGradients gated_norm_backward(const at::Tensor& grad_out, const at::Tensor& grad_total, const at::Tensor& x, const at::Tensor& residual,
+                                   const at::Tensor& weight, const MaybeTensor& post, const MaybeTensor& gate, const MaybeTensor& scale,
+                                   double eps, const at::Tensor& rstd, const std::array<bool, 4>& wanted)
+{
+    not_recorded();
+    const Gated g = as_gated(x, residual, weight, post, gate, scale, eps);
+    const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
+    GatedGradients d;
+    const auto like = [](const at::Tensor& t, bool zero) { return zero ? at::zeros(t.sizes(), t.options()) : at::empty(t.sizes(), t.options()); };
+    const bool none = g.x.rows == 0 || (!grad_out.defined() && !grad_total.defined());
+    d.x = like(x, none);
+    d.residual = like(residual, none);
+    if (wanted[0]) d.weight = like(g.weight, none);
+    if (wanted[1] && g.post) d.post = like(*g.post, none);
+    if (wanted[2] && g.gate) d.gate = like(*g.gate, none);
+    if (wanted[3] && g.scale) d.scale = like(*g.scale, none);
+    if (none) return d;
+    Rows out = {}, total = {};
+    out = as_rows(grad_out.defined() ? grad_out.to(x.scalar_type()) : at::zeros(x.sizes(), x.options()), "gradient");
+    if (grad_total.defined()) total = as_rows(grad_total.to(x.scalar_type()), "gradient");
+    size_t bytes = 0;
+    check_status(geo_sc_gated_norm_backward_workspace_size(g.x.rows, g.x.cols, &bytes), "workspace query");
+    const at::Tensor workspace = at::empty({(int64_t)bytes}, x.options().dtype(at::kByte));
+    check_status(geo_sc_gated_norm_backward(&g.desc, out.t.const_data_ptr(), out.stride, grad_total.defined() ? total.t.const_data_ptr() : nullptr,
+                                            total.stride, rstd.const_data_ptr<float>(), d.x.data_ptr(), d.residual.data_ptr(), data_of(d.weight),
+                                            data_of(d.post), data_of(d.gate), data_of(d.scale), workspace.data_ptr(), bytes, stream_of(x)),
+                 "gated_norm backward");
+    for (const MaybeTensor& t : {MaybeTensor(d.x), MaybeTensor(d.residual), d.weight, d.post, d.gate, d.scale})
+        if (t) once(*t, {grad_out, grad_total});
+    return d;
+}
+
 // What the backward forms x + residual from: themselves, because `total` is rounded to their type; where that is fp32, `total`
 // is the sum itself and half the reading.
 std::pair<at::Tensor, at::Tensor> summands(const at::Tensor& x, const MaybeTensor& residual, const at::Tensor& total)
@@ -553,6 +684,31 @@ struct NormLinearQ8 : torch::autograd::Function<NormLinearQ8> {
     }
 };
 
+// (out, total)
+struct GatedNorm : torch::autograd::Function<GatedNorm> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight,
+                                 const MaybeTensor& post, const MaybeTensor& gate, const MaybeTensor& scale, double eps)
+    {
+        const auto [out, total, rstd] = gated_norm(x, residual, weight, post, gate, scale, eps, true);
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({x, residual, weight, undefined_or(post), undefined_or(gate), undefined_or(scale), *rstd});
+        ctx->saved_data["eps"] = eps;
+        return {out, total};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const auto s = ctx->get_saved_variables();
+        // (inputs are counted without those that are None)
+        std::array<bool, 4> wanted = {ctx->needs_input_grad(2), false, false, false};
+        for (size_t i = 0, at = 3; i < 3; ++i)
+            if (s[3 + i].defined()) wanted[1 + i] = ctx->needs_input_grad(at++);
+        const GatedGradients d = gated_norm_backward(grads[0], grads[1], s[0], s[1], s[2], maybe(s[3]), maybe(s[4]), maybe(s[5]),
+                                                     ctx->saved_data["eps"].toDouble(), s[6], wanted);
+        return {ctx->needs_input_grad(0) ? d.x : at::Tensor(), ctx->needs_input_grad(1) ? d.residual : at::Tensor(), undefined_or(d.weight),
+                undefined_or(d.post), undefined_or(d.gate), undefined_or(d.scale), at::Tensor()};
+    }
+};
+
 struct DistillTopK : torch::autograd::Function<DistillTopK> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& top_logits, const at::Tensor& top_index,
                               double temperature, int64_t reduction)
@@ -590,6 +746,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         const variable_list out = NormLinearQ8::apply(x, gain, weight, residual, eps);
         return std::make_tuple(out[0], residual ? out[1] : x);
     }, "the norm and the product: (y, total)");
+    m.def("gated_norm", [](const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight, const MaybeTensor& post, const MaybeTensor& gate,
+                           const MaybeTensor& scale, double eps, bool differentiable) {
+        if (differentiable) {
+            const variable_list out = GatedNorm::apply(x, residual, weight, post, gate, scale, eps);
+            return std::make_tuple(out[0], out[1]);
+        }
+        const auto [out, total, none] = gated_norm(x, residual, weight, post, gate, scale, eps, false);
+        return std::make_tuple(out, total);
+    }, "norm behind a block, gate, scaled residual and the next norm: (out, total)");
+    m.def("gated_norm_q8", &gated_norm_q8, "the same with 8-bit output: (q, scale, total, values or None)");
     m.def("adamw_step", &adamw_step, "one AdamW step on lists of tensors");
     m.def("distill_topk", [](const at::Tensor& logits, const at::Tensor& top_logits, const at::Tensor& top_index, double temperature, int64_t reduction) {
         return DistillTopK::apply(logits, top_logits, top_index, temperature, reduction);

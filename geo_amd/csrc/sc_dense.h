@@ -1,4 +1,4 @@
-// Shared device code of the kernels on dense matrices (8-bit rows, norm, 8-bit product, distillation): element types,
+// Shared device code of the kernels on dense matrices (8-bit rows, norms, 8-bit product, distillation, AdamW): element types,
 // chunks of eight elements, reductions over a wave and over the threads of a row.
 #pragma once
 
@@ -170,6 +170,59 @@ __device__ __forceinline__ void row_reduce(float& sum, uint32_t& most, int waves
     }
     sum = s;
     most = m;
+}
+
+// Reciprocal and scale of a row from the bits of its largest magnitude.  `unit` multiplies the scale (r of a norm, else 1).
+// A row that holds an infinity or NaN becomes q = 0 with scale NaN: its values are NaN.  Magnitudes below 2^-100 are
+// brought up by 2^100 first, where 127 / a would pass the largest float.
+struct RowScale {
+    float lift, inverse, scale;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t bits, float unit, bool sound)
+{
+    RowScale r;
+    const float a = __uint_as_float(bits);
+    r.lift = a < 0x1p-100f ? 0x1p100f : 1.f;
+    r.inverse = a > 0.f ? 127.f / (a * r.lift) : 0.f;
+    r.scale = a * unit * (1.f / 127.f);
+    if (bits >= kInfinityBits || !sound) {
+        r.inverse = 0.f;
+        r.scale = __uint_as_float(0x7fc00000u);
+    }
+    return r;
+}
+
+// The chunk at column c of a row in 8 bits, and the values v that it then stands for.
+__device__ __forceinline__ void store_eight(int8_t* row, int64_t c, int64_t cols, const RowScale& rs, const float (&n)[kChunk], float (&v)[kChunk])
+{
+    int8_t q[kChunk];
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+        // (a NaN's conversion to an integer is whatever the hardware makes of it: such rows write zeros)
+        const float k = rs.inverse == 0.f ? 0.f : rintf(n[j] * rs.lift * rs.inverse);
+        q[j] = (int8_t)(int)k;
+        v[j] = k * rs.scale;
+    }
+    if (c + kChunk <= cols) {
+        __builtin_memcpy(row + c, q, sizeof q);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j)
+            if (c + j < cols) row[c + j] = q[j];
+    }
+}
+
+// The power of two that brings the largest magnitude, which is a number and not zero, to 1 .. 4 (denormals less far).
+__device__ __forceinline__ float power_up(uint32_t peak)
+{
+    const int field = 254 - (int)(peak >> 23);
+    return __uint_as_float((uint32_t)(field < 1 ? 1 : field > 253 ? 253 : field) << 23);
+}
+// Threads of a row with `chunks` chunks: whole waves, at most 1024, of which each has `held` chunks.
+inline int threads_of_row(int64_t chunks, int held)
+{
+    const int64_t threads = ((chunks + held - 1) / held + 63) / 64 * 64;
+    return threads < 1024 ? (int)threads : 1024;
 }
 
 }  // namespace geo_sc

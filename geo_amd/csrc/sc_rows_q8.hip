@@ -20,26 +20,6 @@
 namespace geo_sc {
 namespace {
 
-// Reciprocal and scale of a row from the bits of its largest magnitude.  `unit` multiplies the scale (r of a norm, else 1).
-// A row that holds an infinity or NaN becomes q = 0 with scale NaN: its values are NaN.  Magnitudes below 2^-100 are
-// brought up by 2^100 first, where 127 / a would pass the largest float.
-struct RowScale {
-    float lift, inverse, scale;
-};
-__device__ __forceinline__ RowScale row_scale(uint32_t bits, float unit, bool sound)
-{
-    RowScale r;
-    const float a = __uint_as_float(bits);
-    r.lift = a < 0x1p-100f ? 0x1p100f : 1.f;
-    r.inverse = a > 0.f ? 127.f / (a * r.lift) : 0.f;
-    r.scale = a * unit * (1.f / 127.f);
-    if (bits >= kInfinityBits || !sound) {
-        r.inverse = 0.f;
-        r.scale = __uint_as_float(0x7fc00000u);
-    }
-    return r;
-}
-
 struct RowsArgs {
     const void *x, *residual, *weight;
     int64_t rows, cols, x_stride, residual_stride, q_stride;
@@ -69,22 +49,7 @@ template <typename T, bool NORM>
 __device__ __forceinline__ void write_chunk(const RowsArgs& a, int64_t row, int64_t c, const RowScale& rs, const float (&n)[kChunk])
 {
     float v[kChunk];
-    int8_t q[kChunk];
-#pragma unroll
-    for (int j = 0; j < kChunk; ++j) {
-        // (a NaN's conversion to an integer is whatever the hardware makes of it: such rows write zeros)
-        const float k = rs.inverse == 0.f ? 0.f : rintf(n[j] * rs.lift * rs.inverse);
-        q[j] = (int8_t)(int)k;
-        v[j] = k * rs.scale;
-    }
-    int8_t* out = a.q + row * a.q_stride;
-    if (c + kChunk <= a.cols) {
-        __builtin_memcpy(out + c, q, sizeof q);
-    } else {
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j)
-            if (c + j < a.cols) out[c + j] = q[j];
-    }
+    store_eight(a.q + row * a.q_stride, c, a.cols, rs, n, v);
     if (a.values) store_chunk(a.values, a.values_dtype, row * a.cols, c, a.cols, v, a.streamed);
 }
 
@@ -96,12 +61,6 @@ __device__ __forceinline__ bool in_range(const RowsArgs& a, float squares, uint3
 {
     return squares < __uint_as_float(kInfinityBits) && squares + a.eps * (float)a.cols > 0x1p-64f && most < kInfinityBits &&
            most >= __float_as_uint(0x1p-100f);
-}
-// The power of two that brings the largest magnitude, which is a number and not zero, to 1 .. 4 (denormals less far).
-__device__ __forceinline__ float power_up(uint32_t peak)
-{
-    const int field = 254 - (int)(peak >> 23);
-    return __uint_as_float((uint32_t)(field < 1 ? 1 : field > 253 ? 253 : field) << 23);
 }
 // r of a row, and r / up, the factor of t up, from the sum of the squares of t up.  Where eps up^2 is beyond all squares r is eps's alone.
 __device__ __forceinline__ void scaled_units(const RowsArgs& a, float squares, float up, float& unit, float& factor)
@@ -255,13 +214,6 @@ __global__ __launch_bounds__(1024) void k_rows_long(RowsArgs a)
         take(c, false);
         write_chunk<T, NORM>(a, row, c, rs, n);
     }
-}
-
-// Threads of a row with `chunks` chunks: whole waves, at most 1024, of which each has `held` chunks.
-int threads_of_row(int64_t chunks, int held)
-{
-    const int64_t threads = ((chunks + held - 1) / held + 63) / 64 * 64;
-    return threads < 1024 ? (int)threads : 1024;
 }
 
 // the rows from `first` on

@@ -248,6 +248,31 @@ def distill_topk(logits, top_logits, top_index, temperature=1.0, reduction="mean
     return _dense().distill_topk(logits, top_logits, top_index, temperature, _REDUCTIONS[reduction])
 
 
+# ---------------------------------------------------------------- between two blocks
+
+def gated_norm(x, residual, weight, post_weight=None, gate=None, residual_scale=None, eps=1e-6):
+    """The norm behind a block, its gate, the scaled residual and the norm in front of the next block, in one pass: for a block's output
+    ``x`` and the stream ``residual`` beside it, with ``rms(v) = sqrt(mean(v^2) + eps)`` over the last dimension::
+
+        m = x / rms(x) * post_weight                    (without post_weight: m = x)
+        total = residual_scale * residual + gate * m    (each 1 where it is None)
+        out = total / rms(total) * weight
+
+    Returns (out, total) in ``x``'s type, which all tensors have; sums and factors are float32.  ``weight``, ``post_weight`` and
+    ``residual_scale`` are (columns,), ``gate`` (columns,) or of x's dimensions with ones behind the leading ones that it has: (samples,
+    1, columns) for x of (samples, tokens, columns).  Differentiable (once) in all of them."""
+    return _dense().gated_norm(x, residual, weight, post_weight, gate, residual_scale, eps,
+                               _wants_grad(x, residual, weight, post_weight, gate, residual_scale))
+
+
+def gated_norm_q8(x, residual, weight, post_weight=None, gate=None, residual_scale=None, eps=1e-6, values=None):
+    """``gated_norm`` with its ``out`` as ``quantize_rows`` has it, for the 8-bit products of a served network: (q, scale, total,
+    values), ``values`` None unless a type is named.  No gradients: train with ``gated_norm`` and ``linear_q8``."""
+    if _wants_grad(x, residual, weight, post_weight, gate, residual_scale):
+        raise ValueError("gated_norm_q8 has no gradients: take gated_norm (or torch.no_grad())")
+    return _dense().gated_norm_q8(x, residual, weight, post_weight, gate, residual_scale, eps, values)
+
+
 # ---------------------------------------------------------------- optimiser step
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, grad_scale=1.0, scales=None,

@@ -552,6 +552,40 @@ GEO_SC_API int geo_sc_distill_topk_backward(const float* grad, int reduction, co
                                             geo_sc_stream_t stream);
 
 /*
+ * The norm behind a block, its gate, the scaled residual and the norm in front of the next block: per row of x (the block's output)
+ * and residual, with m = x / sqrt(mean_j x[j]^2 + eps) post_weight (post_weight NULL: m = x),
+ *   t = residual_scale residual + gate m,   out = t / sqrt(mean_j t[j]^2 + eps) weight
+ * in fp32; t is rounded for `total` only.  Rows of any finite x and t.  weight, post_weight and residual_scale are `cols` elements,
+ * gate is (rows / rows_per_gate, cols): one for each run of rows_per_gate consecutive rows, which must divide rows.  post_weight, gate and
+ * residual_scale may be NULL.  All are of `dtype`.
+ * geo_sc_gated_norm: out and total, (rows, cols) of dtype; rstd NULL, or rows * 2 floats for the backward (both norms' factors).
+ * geo_sc_gated_norm_q8: instead of out its rows in 8 bits (geo_sc_quantize_rows), values NULL or what they stand for in values_dtype.
+ * Backward, from the gradients of out and of total (NULL: none), both of dtype: dx and dresidual (rows, cols), and dweight,
+ * dpost, dscale (cols) and dgate (of the gate's shape), each NULL where it is not wanted, summed over rows in an order that does not
+ * change from run to run.  Workspace, 4-byte aligned: geo_sc_gated_norm_backward_workspace_size.
+ */
+typedef struct geo_sc_gated_norm_desc {
+    size_t struct_bytes; /* sizeof(geo_sc_gated_norm_desc) */
+    const void* x;
+    const void* residual;
+    const void* weight;
+    const void* post_weight;
+    const void* gate;
+    const void* residual_scale;
+    int64_t rows, cols, x_stride, residual_stride, rows_per_gate;
+    float eps;
+    int32_t dtype;
+} geo_sc_gated_norm_desc;
+GEO_SC_API int geo_sc_gated_norm(const geo_sc_gated_norm_desc* desc, void* out, void* total, float* rstd, geo_sc_stream_t stream);
+GEO_SC_API int geo_sc_gated_norm_q8(const geo_sc_gated_norm_desc* desc, int8_t* q, int64_t q_stride, float* scale, void* total, void* values,
+                                    int values_dtype, geo_sc_stream_t stream);
+GEO_SC_API int geo_sc_gated_norm_backward_workspace_size(int64_t rows, int64_t cols, size_t* bytes);
+GEO_SC_API int geo_sc_gated_norm_backward(const geo_sc_gated_norm_desc* desc, const void* grad, int64_t grad_stride, const void* grad_total,
+                                          int64_t grad_total_stride, const float* rstd, void* dx, void* dresidual, void* dweight,
+                                          void* dpost, void* dgate, void* dscale, void* workspace, size_t workspace_bytes,
+                                          geo_sc_stream_t stream);
+
+/*
  * One AdamW step on many tensors, of any element counts, none of them named twice: in fp32 operations on each element, with t the
  * number of this step (from 1 on) and g = grad * grad_scale:
  *   m = beta1 m + (1 - beta1) g,   v = beta2 v + (1 - beta2) g^2,
