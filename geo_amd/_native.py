@@ -53,6 +53,12 @@ class GatedNormDesc(ctypes.Structure):
                [("eps", ctypes.c_float), ("dtype", ctypes.c_int32)]
 
 
+class Q8Epilogue(ctypes.Structure):
+    """geo_sc_q8_epilogue of include/geo_sc.h"""
+    _fields_ = [("struct_bytes", ctypes.c_size_t)] + [(n, ctypes.c_void_p) for n in ("bias", "residual", "slope")] + \
+               [("residual_stride", ctypes.c_int64), ("bias_dtype", ctypes.c_int32), ("slope_dtype", ctypes.c_int32), ("activation", ctypes.c_int32)]
+
+
 # every symbol include/geo_sc.h declares: name -> (restype, argtypes)
 _P = ctypes.c_void_p
 _SZ = ctypes.POINTER(ctypes.c_size_t)
@@ -120,6 +126,10 @@ C_API = {
                                            ctypes.c_size_t, _P]),
     "geo_sc_distill_topk_backward": (ctypes.c_int, [_P, _I, _P, _I, _L, _P, _I, _P, _I, _L, _L, _I, ctypes.c_float, _P,
                                                     _P, _P]),
+    "geo_sc_matmul_q8_epilogue": (ctypes.c_int, [_P, _L, _P, _P, _L, _P] + [_L] * 3 + [ctypes.POINTER(Q8Epilogue), _P, _I, _P, ctypes.c_size_t, _P]),
+    "geo_sc_matmul_q8_epilogue_backward_workspace_size": (ctypes.c_int, [_L] * 3 + [_I] * 4 + [_SZ]),
+    "geo_sc_matmul_q8_epilogue_backward": (ctypes.c_int, [_P, _I, _L, _P, _I, _P, _L, _P, _P, _L, _P] + [_L] * 3 + [_P, _I, _P, _I, _P, _I, _P,
+                                                          ctypes.c_size_t, _P]),
     "geo_sc_gated_norm": (ctypes.c_int, [ctypes.POINTER(GatedNormDesc)] + [_P] * 4),
     "geo_sc_gated_norm_q8": (ctypes.c_int, [ctypes.POINTER(GatedNormDesc), _P, _L] + [_P] * 3 + [_I, _P]),
     "geo_sc_gated_norm_backward_workspace_size": (ctypes.c_int, [_L, _L, _SZ]),

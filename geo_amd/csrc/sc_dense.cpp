@@ -356,7 +356,24 @@ Q8 as_q8(const at::Tensor& q, const at::Tensor& scale, const char* what)
     return v;
 }
 
-at::Tensor matmul_q8(const at::Tensor& q, const at::Tensor& scale, const at::Tensor& wq, const at::Tensor& wscale, at::ScalarType type)
+// What follows a product: bias, activation, residual, and whether the backward will ask for the activation's slope.
+struct After {
+    MaybeTensor bias, residual;
+    int activation = GEO_SC_ACT_NONE;
+    bool keep_slope = false;
+    at::Tensor slope;   // what came of it
+    bool any() const { return bias || residual || activation != GEO_SC_ACT_NONE; }
+};
+int activation_of(const std::optional<std::string>& name)
+{
+    if (!name) return GEO_SC_ACT_NONE;
+    if (*name == "relu") return GEO_SC_ACT_RELU;
+    if (*name == "gelu") return GEO_SC_ACT_GELU;
+    if (*name == "silu") return GEO_SC_ACT_SILU;
+    TORCH_CHECK(false, "activation must be None, 'relu', 'gelu' or 'silu', got '", *name, "'");
+}
+
+at::Tensor matmul_q8(const at::Tensor& q, const at::Tensor& scale, const at::Tensor& wq, const at::Tensor& wscale, at::ScalarType type, After& after)
 {
     not_recorded();
     const Q8 x = as_q8(q, scale, "q"), w = as_q8(wq, wscale, "weight_q");
@@ -367,56 +384,108 @@ at::Tensor matmul_q8(const at::Tensor& q, const at::Tensor& scale, const at::Ten
     TORCH_CHECK(x.r.cols <= 131071, "at most 131071 elements per row");
     std::vector<int64_t> sizes(q.sizes().begin(), q.sizes().end());
     sizes.back() = w.r.rows;
+    geo_sc_q8_epilogue e = {};
+    at::Tensor bias;
+    Rows residual;
+    if (after.bias) {
+        with(*after.bias, "bias", q, "q");
+        TORCH_CHECK(after.bias->dim() == 1 && after.bias->size(0) == w.r.rows, "bias must have the ", w.r.rows, " elements of a row of the product");
+        e.bias_dtype = dtype_of(after.bias->scalar_type(), "bias");
+        bias = after.bias->contiguous();
+        e.bias = bias.const_data_ptr();
+    }
+    if (after.residual) {
+        with(*after.residual, "residual", q, "q");
+        TORCH_CHECK(after.residual->sizes() == at::IntArrayRef(sizes) && after.residual->scalar_type() == type,
+                    "residual must have the shape and type of the product");
+    }
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
     const at::Tensor y = at::empty(sizes, q.options().dtype(type));
+    if (after.keep_slope) {
+        // fp16 holds a relu's slope exactly, and any to an eighth of what bf16 rounds by; beside fp16's own rounding it would show
+        // (gradients of 4000 x 500 fp16 1.5 times as far off)
+        const bool half = type == at::kBFloat16 || after.activation == GEO_SC_ACT_RELU;
+        after.slope = at::empty({x.r.rows, w.r.rows}, q.options().dtype(half ? at::kHalf : at::kFloat));
+        e.slope_dtype = half ? GEO_SC_F16 : GEO_SC_F32;
+    }
     if (y.numel() == 0) return y;
+    if (after.residual) {
+        residual = as_rows(*after.residual, "residual");
+        e.residual = residual.t.const_data_ptr();
+        e.residual_stride = residual.stride;
+    }
     size_t bytes = 0;
     check_status(geo_sc_matmul_q8_workspace_size(x.r.t.const_data_ptr<int8_t>(), x.r.stride, w.r.t.const_data_ptr<int8_t>(),
                                                  w.r.stride, x.r.rows, w.r.rows, x.r.cols, &bytes), "workspace query");
     MaybeTensor workspace;
     if (bytes) workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    if (after.any()) {
+        e.struct_bytes = sizeof e;
+        e.activation = after.activation;
+        e.slope = after.keep_slope ? after.slope.data_ptr() : nullptr;
+        check_status(geo_sc_matmul_q8_epilogue(x.r.t.const_data_ptr<int8_t>(), x.r.stride, x.scale.const_data_ptr<float>(),
+                                               w.r.t.const_data_ptr<int8_t>(), w.r.stride, w.scale.const_data_ptr<float>(), x.r.rows, w.r.rows,
+                                               x.r.cols, &e, y.data_ptr(), dtype, data_of(workspace), bytes, stream_of(q)),
+                     "matmul_q8");
+        return y;
+    }
     check_status(geo_sc_matmul_q8(x.r.t.const_data_ptr<int8_t>(), x.r.stride, x.scale.const_data_ptr<float>(), w.r.t.const_data_ptr<int8_t>(),
                                   w.r.stride, w.scale.const_data_ptr<float>(), x.r.rows, w.r.rows, x.r.cols, y.data_ptr(), dtype,
                                   data_of(workspace), bytes, stream_of(q)),
                  "matmul_q8");
     return y;
 }
+at::Tensor matmul_q8(const at::Tensor& q, const at::Tensor& scale, const at::Tensor& wq, const at::Tensor& wscale, at::ScalarType type)
+{
+    After none;
+    return matmul_q8(q, scale, wq, wscale, type, none);
+}
 
-std::tuple<MaybeTensor, MaybeTensor> matmul_q8_backward(const at::Tensor& grad, const at::Tensor& q, const at::Tensor& scale,
-                                                        const at::Tensor& wq, const at::Tensor& wscale,
-                                                        std::optional<at::ScalarType> dx_type, std::optional<at::ScalarType> dw_type)
+struct ProductGradients {
+    MaybeTensor x, w, bias;
+};
+// `slope`: of the activation, or undefined; y_type is the product's type then
+ProductGradients matmul_q8_backward(const at::Tensor& grad, const at::Tensor& q, const at::Tensor& scale, const at::Tensor& wq,
+                                    const at::Tensor& wscale, std::optional<at::ScalarType> dx_type, std::optional<at::ScalarType> dw_type,
+                                    const at::Tensor& slope = {}, std::optional<at::ScalarType> dbias_type = std::nullopt)
 {
     not_recorded();
     const Q8 x = as_q8(q, scale, "q"), w = as_q8(wq, wscale, "weight_q");
     if (w.r.rows == 0 && grad.numel() == 0) {   // no columns: sums of nothing
         on_gpu(grad, "gradient");
         return {dx_type ? MaybeTensor(at::zeros(q.sizes(), q.options().dtype(*dx_type))) : MaybeTensor(),
-                dw_type ? MaybeTensor(at::empty(wq.sizes(), q.options().dtype(*dw_type))) : MaybeTensor()};
+                dw_type ? MaybeTensor(at::empty(wq.sizes(), q.options().dtype(*dw_type))) : MaybeTensor(),
+                dbias_type ? MaybeTensor(at::empty({0}, q.options().dtype(*dbias_type))) : MaybeTensor()};
     }
     Rows g = as_rows(grad, "gradient");
     if (g.rows > 1 && g.stride && g.stride < g.cols) g = as_rows(grad.contiguous(), "gradient");   // (rows that overlap)
     with(grad, "gradient", q, "q");
     TORCH_CHECK(x.r.cols == w.r.cols && g.rows == x.r.rows && g.cols == w.r.rows, "gradient must have the shape of the product");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
-    MaybeTensor dx, dw;
+    MaybeTensor dx, dw, dbias;
     if (dx_type) dx = at::empty(q.sizes(), q.options().dtype(*dx_type));
     if (dw_type) dw = at::empty(wq.sizes(), q.options().dtype(*dw_type));
+    if (dbias_type) dbias = at::empty({g.cols}, q.options().dtype(*dbias_type));
     if (g.rows == 0 && dw) dw->zero_();
-    if (g.rows == 0 || (!dx && !dw)) return {dx, dw};
+    if (g.rows == 0 && dbias) dbias->zero_();
+    if (g.rows == 0 || (!dx && !dw && !dbias)) return {dx, dw, dbias};
     const int grad_type = dtype_of(g.t.scalar_type(), "gradient");
     size_t bytes = 0;
-    check_status(geo_sc_matmul_q8_backward_workspace_size(g.rows, g.cols, x.r.cols, grad_type, dx.has_value(), dw.has_value(), &bytes),
+    check_status(geo_sc_matmul_q8_epilogue_backward_workspace_size(g.rows, g.cols, x.r.cols, grad_type, dx.has_value(), dw.has_value(),
+                                                                   dbias.has_value(), &bytes),
                  "workspace query");
     const at::Tensor workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-    check_status(geo_sc_matmul_q8_backward(g.t.const_data_ptr(), grad_type, g.stride, x.r.t.const_data_ptr<int8_t>(), x.r.stride,
-                                           x.scale.const_data_ptr<float>(), w.r.t.const_data_ptr<int8_t>(), w.r.stride,
-                                           w.scale.const_data_ptr<float>(), g.rows, g.cols, x.r.cols, data_of(dx),
-                                           dx ? dtype_of(*dx_type, "dx") : 0, data_of(dw), dw ? dtype_of(*dw_type, "dw") : 0,
-                                           workspace.data_ptr(), bytes, stream_of(q)),
+    check_status(geo_sc_matmul_q8_epilogue_backward(g.t.const_data_ptr(), grad_type, g.stride, slope.defined() ? slope.const_data_ptr() : nullptr,
+                                                    slope.defined() && slope.scalar_type() == at::kHalf ? GEO_SC_F16 : GEO_SC_F32,
+                                                    x.r.t.const_data_ptr<int8_t>(), x.r.stride, x.scale.const_data_ptr<float>(),
+                                                    w.r.t.const_data_ptr<int8_t>(), w.r.stride, w.scale.const_data_ptr<float>(), g.rows, g.cols,
+                                                    x.r.cols, data_of(dx), dx ? dtype_of(*dx_type, "dx") : 0, data_of(dw),
+                                                    dw ? dtype_of(*dw_type, "dw") : 0, data_of(dbias), dbias ? dtype_of(*dbias_type, "dbias") : 0,
+                                                    workspace.data_ptr(), bytes, stream_of(q)),
                  "matmul_q8 backward");
-    if (dx) once(*dx, {grad});
-    if (dw) once(*dw, {grad});
-    return {dx, dw};
+    for (const MaybeTensor& d : {dx, dw, dbias})
+        if (d) once(*d, {grad});
+    return {dx, dw, dbias};
 }
 
 // the teacher's entries of the rows of `logits`
@@ -620,8 +689,43 @@ struct LinearQ8 : torch::autograd::Function<LinearQ8> {
         std::optional<at::ScalarType> x, w;
         if (ctx->needs_input_grad(0)) x = ctx->saved_data["x"].toScalarType();
         if (ctx->needs_input_grad(1)) w = ctx->saved_data["w"].toScalarType();
-        const auto [dx, dw] = matmul_q8_backward(grads[0], s[0], s[1], s[2], s[3], x, w);
-        return {undefined_or(dx), undefined_or(dw)};
+        const ProductGradients d = matmul_q8_backward(grads[0], s[0], s[1], s[2], s[3], x, w);
+        return {undefined_or(d.x), undefined_or(d.w)};
+    }
+};
+
+// the same with an epilogue
+struct LinearQ8Epilogue : torch::autograd::Function<LinearQ8Epilogue> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight, const MaybeTensor& bias, const MaybeTensor& residual,
+                              int64_t activation, bool keep_slope)
+    {
+        const auto [q, scale, none] = quantize_rows(x, std::nullopt);
+        const auto [wq, wscale, none2] = quantize_rows(weight, std::nullopt);
+        After after;
+        after.bias = bias;
+        after.residual = residual;
+        after.activation = (int)activation;
+        after.keep_slope = keep_slope;
+        const at::Tensor y = matmul_q8(q, scale, wq, wscale, x.scalar_type(), after);
+        ctx->save_for_backward({q, scale, wq, wscale, after.slope});
+        ctx->saved_data["x"] = x.scalar_type();
+        ctx->saved_data["w"] = weight.scalar_type();
+        if (bias) ctx->saved_data["bias"] = bias->scalar_type();
+        ctx->saved_data["residual"] = residual.has_value();
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const auto s = ctx->get_saved_variables();
+        const bool has_bias = ctx->saved_data.count("bias");
+        std::optional<at::ScalarType> x, w, bias;
+        if (ctx->needs_input_grad(0)) x = ctx->saved_data["x"].toScalarType();
+        if (ctx->needs_input_grad(1)) w = ctx->saved_data["w"].toScalarType();
+        if (has_bias && ctx->needs_input_grad(2)) bias = ctx->saved_data["bias"].toScalarType();
+        ProductGradients d;
+        if (x || w || bias) d = matmul_q8_backward(grads[0], s[0], s[1], s[2], s[3], x, w, s[4], bias);
+        return {undefined_or(d.x), undefined_or(d.w), undefined_or(d.bias), ctx->saved_data["residual"].toBool() ? grads[0] : at::Tensor(),
+                at::Tensor(), at::Tensor()};
     }
 };
 
@@ -653,15 +757,20 @@ struct RmsNormQ8 : torch::autograd::Function<RmsNormQ8> {
 // (y, total); total is an output only where there is a residual
 struct NormLinearQ8 : torch::autograd::Function<NormLinearQ8> {
     static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& gain, const at::Tensor& weight,
-                                 const MaybeTensor& residual, double eps)
+                                 const MaybeTensor& residual, double eps, const MaybeTensor& bias, int64_t activation, bool keep_slope)
     {
         const auto [q, scale, total, none, rstd] = rms_norm_q8(x, gain, residual, eps, std::nullopt, true);
         const auto [wq, wscale, none2] = quantize_rows(weight, std::nullopt);
         ctx->set_materialize_grads(false);
         const auto [first, second] = summands(x, residual, total);
-        ctx->save_for_backward({q, scale, wq, wscale, first, second, gain, *rstd});
+        After after;
+        after.bias = bias;
+        after.activation = (int)activation;
+        after.keep_slope = keep_slope;
+        variable_list out = {matmul_q8(q, scale, wq, wscale, x.scalar_type(), after)};
+        ctx->save_for_backward({q, scale, wq, wscale, first, second, gain, *rstd, after.slope});
         ctx->saved_data["w"] = weight.scalar_type();
-        variable_list out = {matmul_q8(q, scale, wq, wscale, x.scalar_type())};
+        if (bias) ctx->saved_data["bias"] = bias->scalar_type();
         if (residual) out.push_back(total);
         return out;
     }
@@ -670,17 +779,20 @@ struct NormLinearQ8 : torch::autograd::Function<NormLinearQ8> {
         const auto s = ctx->get_saved_variables();
         const bool residual = grads.size() > 1, need_gain = ctx->needs_input_grad(1);
         const bool through = ctx->needs_input_grad(0) || need_gain || (residual && ctx->needs_input_grad(3));
-        MaybeTensor dn, dw, dgain;
+        const bool need_bias = ctx->saved_data.count("bias") && ctx->needs_input_grad(3 + residual);
+        ProductGradients d;
+        MaybeTensor dgain;
         at::Tensor dx;
         if (grads[0].defined()) {
-            std::optional<at::ScalarType> x, w;
+            std::optional<at::ScalarType> x, w, bias;
             if (through) x = s[4].scalar_type();
             if (ctx->needs_input_grad(2)) w = ctx->saved_data["w"].toScalarType();
-            std::tie(dn, dw) = matmul_q8_backward(grads[0], s[0], s[1], s[2], s[3], x, w);
+            if (need_bias) bias = ctx->saved_data["bias"].toScalarType();
+            d = matmul_q8_backward(grads[0], s[0], s[1], s[2], s[3], x, w, s[8], bias);
         }
-        if (through) std::tie(dx, dgain) = rms_norm_q8_backward(dn, residual ? maybe(grads[1]) : MaybeTensor(), s[4], s[5], s[6], s[7], need_gain);
-        return {ctx->needs_input_grad(0) ? dx : at::Tensor(), undefined_or(dgain), undefined_or(dw),
-                residual && ctx->needs_input_grad(3) ? dx : at::Tensor(), at::Tensor()};
+        if (through) std::tie(dx, dgain) = rms_norm_q8_backward(d.x, residual ? maybe(grads[1]) : MaybeTensor(), s[4], s[5], s[6], s[7], need_gain);
+        return {ctx->needs_input_grad(0) ? dx : at::Tensor(), undefined_or(dgain), undefined_or(d.w),
+                residual && ctx->needs_input_grad(3) ? dx : at::Tensor(), at::Tensor(), undefined_or(d.bias), at::Tensor(), at::Tensor()};
     }
 };
 
@@ -740,10 +852,32 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         const variable_list out = RmsNormQ8::apply(x, weight, residual, eps, values);
         return std::make_tuple(out[0], out[1], residual ? out[3] : x, out[2]);
     }, "the same, values and total differentiable");
-    m.def("matmul_q8", &matmul_q8, "product of 8-bit rows with a scale each");
+    m.def("matmul_q8", py::overload_cast<const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, at::ScalarType>(&matmul_q8),
+          "product of 8-bit rows with a scale each");
+    m.def("matmul_q8_epilogue", [](const at::Tensor& q, const at::Tensor& scale, const at::Tensor& wq, const at::Tensor& wscale, at::ScalarType type,
+                                   const MaybeTensor& bias, const std::optional<std::string>& activation, const MaybeTensor& residual) {
+        After after;
+        after.bias = bias;
+        after.residual = residual;
+        after.activation = activation_of(activation);
+        return matmul_q8(q, scale, wq, wscale, type, after);
+    }, "the same with bias, activation and residual");
+    m.def("linear_q8_epilogue", [](const at::Tensor& x, const at::Tensor& weight, const MaybeTensor& bias, const std::optional<std::string>& activation,
+                                   const MaybeTensor& residual) {
+        const int kind = activation_of(activation);
+        // (the slope is for the gradients of all but the residual)
+        const bool keep = kind != GEO_SC_ACT_NONE && at::GradMode::is_enabled() &&
+                          (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()));
+        return LinearQ8Epilogue::apply(x, weight, bias, residual, kind, keep);
+    }, "product of x and weight rounded to 8-bit rows, with bias, activation and residual");
     m.def("linear_q8", [](const at::Tensor& x, const at::Tensor& weight) { return LinearQ8::apply(x, weight); }, "product of x and weight rounded to 8-bit rows");
-    m.def("norm_linear_q8", [](const at::Tensor& x, const at::Tensor& gain, const at::Tensor& weight, const MaybeTensor& residual, double eps) {
-        const variable_list out = NormLinearQ8::apply(x, gain, weight, residual, eps);
+    m.def("norm_linear_q8", [](const at::Tensor& x, const at::Tensor& gain, const at::Tensor& weight, const MaybeTensor& residual, double eps,
+                               const MaybeTensor& bias, const std::optional<std::string>& activation) {
+        const int kind = activation_of(activation);
+        const bool keep = kind != GEO_SC_ACT_NONE && at::GradMode::is_enabled() &&
+                          (x.requires_grad() || gain.requires_grad() || weight.requires_grad() || (residual && residual->requires_grad()) ||
+                           (bias && bias->requires_grad()));
+        const variable_list out = NormLinearQ8::apply(x, gain, weight, residual, eps, bias, kind, keep);
         return std::make_tuple(out[0], residual ? out[1] : x);
     }, "the norm and the product: (y, total)");
     m.def("gated_norm", [](const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight, const MaybeTensor& post, const MaybeTensor& gate,

@@ -184,6 +184,128 @@ __device__ __forceinline__ void finish_four(const TileArgs& a, int split, int64_
 
 __device__ __forceinline__ float scale_at(const float* scale, int64_t i, int64_t count) { return scale && i < count ? scale[i] : 1.f; }
 
+// ---------------------------------------------------------------- epilogue
+//
+//   z = x_scale w_scale sum + bias,   y = act(z) + residual;   for the backward slope = act'(z)
+// In fp32, y rounded once.  The slope and not z is kept: z in 16 bits would be off by up to a 2048th of itself, the slope in fp16 is off by
+// as much of a number that is 1.13 at most, whatever z is.
+
+struct Epilogue {
+    const void *bias, *residual;   // or NULL; the residual's type is y's
+    void* slope;                   // [rows][cols]; or NULL
+    int64_t residual_stride;
+    int bias_dtype, slope_dtype, activation;
+};
+bool slope_type_known(int dtype) { return dtype == GEO_SC_F32 || dtype == GEO_SC_F16; }
+
+// z becomes act(z), d its slope.  NaN stays; of the lowest floats on, z times a probability of zero is zero.
+template <int N>
+__device__ __forceinline__ void activate(int kind, float (&z)[N], float (&d)[N])
+{
+    if (kind == GEO_SC_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            d[j] = z[j] > 0.f ? 1.f : 0.f;
+            z[j] = z[j] < 0.f ? 0.f : z[j];
+        }
+    } else if (kind == GEO_SC_ACT_GELU) {   // z times the normal distribution's share below z
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float below = 0.5f + 0.5f * erff(z[j] * 0.70710678f);
+            d[j] = below + z[j] * expf(-0.5f * z[j] * z[j]) * 0.39894228f;
+            z[j] *= below;
+        }
+    } else if (kind == GEO_SC_ACT_SILU) {   // z times its logistic function
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float s = 1.f / (1.f + expf(-z[j]));
+            d[j] = s + z[j] * s * (1.f - s);
+            z[j] *= s;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) d[j] = 1.f;
+    }
+}
+
+// N consecutive columns of a row, of which `left` are there
+template <int N, typename T>
+__device__ __forceinline__ void load_columns(const T* p, int64_t left, float (&v)[N])
+{
+    if (left >= N) {
+        T raw[N];
+        __builtin_memcpy(raw, p, sizeof raw);
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = (float)raw[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = j < left ? (float)p[j] : 0.f;
+    }
+}
+template <int N>
+__device__ __forceinline__ void load_columns(const void* p, int dtype, int64_t at, int64_t left, float (&v)[N])
+{
+    if (dtype == GEO_SC_F32) load_columns((const f32*)p + at, left, v);
+    else if (dtype == GEO_SC_BF16) load_columns((const bf16*)p + at, left, v);
+    else load_columns((const f16*)p + at, left, v);
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_columns(T* p, int64_t left, const float (&v)[N])
+{
+    T raw[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) raw[j] = (T)v[j];
+    if (left >= N) {
+        __builtin_memcpy(p, raw, sizeof raw);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < left) p[j] = raw[j];
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_columns(void* p, int dtype, int64_t at, int64_t left, const float (&v)[N])
+{
+    if (dtype == GEO_SC_F32) store_columns((f32*)p + at, left, v);
+    else if (dtype == GEO_SC_BF16) store_columns((bf16*)p + at, left, v);
+    else store_columns((f16*)p + at, left, v);
+}
+template <int N>
+__device__ __forceinline__ void load_bias(const Epilogue& e, int64_t n, int64_t cols, float (&v)[N])
+{
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = 0.f;
+    if (e.bias && n < cols) load_columns(e.bias, e.bias_dtype, n, cols - n, v);
+}
+// N columns from n on of row m: their sums scaled and the bias added come in as z
+template <int N>
+__device__ __forceinline__ void finish_columns(const TileArgs& a, const Epilogue& e, int64_t m, int64_t n, float (&z)[N])
+{
+    const int64_t left = a.cols - n;
+    if (m >= a.rows || left <= 0) return;
+    float d[N];
+    activate(e.activation, z, d);
+    if (e.slope) {
+        if (e.slope_dtype == GEO_SC_F32) store_columns((f32*)e.slope + m * a.cols + n, left, d);
+        else store_columns((f16*)e.slope + m * a.cols + n, left, d);
+    }
+    if (e.residual) {
+        load_columns(e.residual, a.dtype, m * e.residual_stride + n, left, d);
+#pragma unroll
+        for (int j = 0; j < N; ++j) z[j] += d[j];
+    }
+    store_columns(a.y, a.dtype, m * a.cols + n, left, z);
+}
+// the same from four sums and their scales
+__device__ __forceinline__ void finish_four(const TileArgs& a, const Epilogue& e, int64_t m, int64_t n, const v4i& s, float xs, const float (&ws)[4])
+{
+    float z[4], bias[4];
+    load_bias(e, n, a.cols, bias);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) z[r] = (float)s[r] * xs * ws[r] + bias[r];
+    finish_columns(a, e, m, n, z);
+}
+
 // ---------------------------------------------------------------- tiles
 //
 // Tiles of B rows of x by B rows of w; four waves, each with a quarter of the outputs in 16x16 squares.  w is the matrix
@@ -410,20 +532,59 @@ __device__ __forceinline__ void finish_tile(const Spot& p, typename Matrix<INT8>
     else finish((f16*)p.a.y, [&](auto one, int i, int j, int r) { return (f16)scaled(one, i, j, r); });
 }
 
+// The same through the epilogue: the sums as they are into LDS, ROWS of a wave's rows at a time, and out of it a lane eight columns of a row.
+template <int B, int ROWS>
+__device__ __forceinline__ void finish_tile(const Spot& p, const Epilogue& e, v4i (&sum)[B / 32][B / 32], uint8_t* area, int wave, int lane)
+{
+    constexpr int T = B / 32, kCols = T * 16, kPieces = kCols / 4, kMix = (kPieces < 16 ? kPieces : 16) - 1;
+    constexpr int kLanes = kCols / kChunk, kAtOnce = 64 / kLanes;   // lanes of a row, rows at once
+    static_assert(ROWS % 16 == 0 && kCols % ROWS == 0 && ROWS % kAtOnce == 0, "");
+    const int64_t n = p.n0 + wave / 2 * kCols + lane % kLanes * kChunk;
+    float ws[kChunk] = {}, bias[kChunk];
+    if (n < p.a.cols) load_columns(p.a.w_scale + n, p.a.cols - n, ws);
+    load_bias(e, n, p.a.cols, bias);
+#pragma unroll
+    for (int first = 0; first < kCols; first += ROWS) {
+#pragma unroll
+        for (int i = 0; i < ROWS / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < T; ++j) {
+                const int row = i * 16 + (lane & 15), piece = j * 4 + (lane >> 4);
+                *(v4i*)(area + (row * kPieces + (piece ^ (row & kMix))) * 16) = sum[j][first / 16 + i];
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int r = lane / kLanes; r < ROWS; r += kAtOnce) {
+            const int64_t m = p.m0 + wave % 2 * kCols + first + r;
+            if (m >= p.a.rows || n >= p.a.cols) continue;
+            const float xs = p.a.x_scale[m];
+            float z[kChunk];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const v4i s = *(const v4i*)(area + (r * kPieces + ((lane % kLanes * 2 + h) ^ (r & kMix))) * 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) z[h * 4 + j] = (float)s[j] * xs * ws[h * 4 + j] + bias[h * 4 + j];
+            }
+            finish_columns(p.a, e, m, n, z);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 // Rows that start at multiples of 16 bytes, and four whole stages of every split.  The loads write LDS themselves, into a ring of
 // kRing stages: while a wave multiplies stage s out of registers, stage s + 1 moves from LDS to its other registers and the stages
 // up to s + kRing are on their way.  One barrier per stage: it says that every wave's share of stage s + 1 has come and
 // that all have read stage s, whose place stage s + kRing takes.
 // Bound by power: 8192 x 16384 x 4096 in 446 - 452 us (2.43 - 2.46 POP/s) at 1.95 GHz, where the products alone run at 2.17; both gradients of
 // 4096 x 4096 x 4096 bf16 in 200 us (1.37 PFLOP/s).
-template <int B, bool INT8>
-__global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)
+// finish(p, sum, ring, wave, lane) stores the sums of a tile; `ring` gives the place of a stage, kBytes each, which is free then.
+template <int B, bool INT8, typename Finish>
+__device__ __forceinline__ void tiles_body(const TwoProducts& both, Finish finish)
 {
     typedef Tiling<B, INT8> G;
     constexpr int T = G::T, L = G::L;
     // (arrays of their own, not one: the compiler keeps reads of one apart from loads into another)
     __shared__ __align__(16) uint8_t ring0[G::kBytes], ring1[G::kBytes], ring2[G::kBytes], ring3[G::kBytes];
-    __shared__ __align__(16) uint8_t areas[kWaves][G::kArea];
     const auto place = [&](auto which) -> uint8_t* {
         constexpr int r = decltype(which)::value % kRing;
         if constexpr (r == 0) return ring0;
@@ -528,8 +689,7 @@ __global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)
         if (k + 2 < p.stop) stage(Int<2>(), k + 2, std::false_type());
         if (k + 3 < p.stop) stage(Int<3>(), k + 3, std::false_type());
     }
-    TileScales<T> scales;
-    scales.load(p, wave, lane);
+    finish.ask(p, wave, lane);
     if (p.stop < p.end) {   // a last stage that is not whole
         v4i v[2 * L];
         fetch_stage<L>(p, p.stop, wave, lane, v);
@@ -540,18 +700,49 @@ __global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)
         multiply<INT8, true, T>(f[0], sum);
     }
     settle(sum);
-    finish_tile<B, INT8>(p, sum, scales, areas[wave], wave, lane);
+    finish(p, sum, wave == 0 ? ring0 : wave == 1 ? ring1 : wave == 2 ? ring2 : ring3, wave, lane);
+}
+template <int B, bool INT8>
+__global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)
+{
+    __shared__ __align__(16) uint8_t areas[kWaves][Tiling<B, INT8>::kArea];
+    struct Finish {
+        uint8_t (*areas)[Tiling<B, INT8>::kArea];
+        TileScales<B / 32> scales;
+        __device__ __forceinline__ void ask(const Spot& p, int wave, int lane) { scales.load(p, wave, lane); }
+        __device__ __forceinline__ void operator()(const Spot& p, typename Matrix<INT8>::Sum (&sum)[B / 32][B / 32], uint8_t*, int wave, int lane)
+        {
+            finish_tile<B, INT8>(p, sum, scales, areas[wave], wave, lane);
+        }
+    };
+    tiles_body<B, INT8>(both, Finish{areas, {}});
+}
+// (the ring takes the sums on their way out: 128 KB of LDS for the largest tile)
+template <int B>
+__global__ __launch_bounds__(kWaves * 64) void k_tiles_epilogue(TwoProducts both, Epilogue e)
+{
+    struct Finish {
+        const Epilogue& e;
+        __device__ __forceinline__ void ask(const Spot&, int, int) {}
+        __device__ __forceinline__ void operator()(const Spot& p, v4i (&sum)[B / 32][B / 32], uint8_t* place, int wave, int lane)
+        {
+            __syncthreads();   // all have read the last stage
+            finish_tile<B, B / 2 < 64 ? B / 2 : 64>(p, e, sum, place, wave, lane);
+        }
+    };
+    tiles_body<B, true>(both, Finish{e});
 }
 
 // Fewer stages than the ring of k_tiles holds, at any alignment: stages through registers, the next one on its way while one is
 // multiplied.  1000 x 1000 x 239: 6.6 us, its launch and one way to memory and back.
-template <int B, bool INT8>
-__global__ __launch_bounds__(kWaves * 64) void k_tiles_any(TwoProducts both)
+template <int B, bool INT8, bool EPILOGUE>
+__global__ __launch_bounds__(kWaves * 64) void k_tiles_any(TwoProducts both, Epilogue e)
 {
     typedef Tiling<B, INT8> G;
     constexpr int T = G::T, L = G::L;
+    constexpr int kArea = EPILOGUE ? 32 * T * 64 : G::kArea;   // (32 rows of sums)
     __shared__ __align__(16) uint8_t buffers[2][G::kBytes];
-    __shared__ __align__(16) uint8_t areas[kWaves][G::kArea];
+    __shared__ __align__(16) uint8_t areas[kWaves][kArea];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const Fragments<B> fragments(wave, lane);
     const Spot p = spot_of<B>(both, blockIdx.x);
@@ -571,9 +762,13 @@ __global__ __launch_bounds__(kWaves * 64) void k_tiles_any(TwoProducts both)
         if (k + 1 < p.end) put_stage<L>(buffers[(k - p.begin + 1) & 1], wave, lane, v);
         __syncthreads();
     }
-    TileScales<T> scales;
-    scales.load(p, wave, lane);
-    finish_tile<B, INT8>(p, sum, scales, areas[wave], wave, lane);
+    if constexpr (EPILOGUE) {
+        finish_tile<B, 32>(p, e, sum, areas[wave], wave, lane);
+    } else {
+        TileScales<T> scales;
+        scales.load(p, wave, lane);
+        finish_tile<B, INT8>(p, sum, scales, areas[wave], wave, lane);
+    }
 }
 
 // Rows that start anywhere, laid out anew at multiples of 16 bytes for k_tiles: a piece of a row per thread.  What lies behind a
@@ -607,8 +802,8 @@ __global__ __launch_bounds__(256) void k_align_rows(AlignArgs a)
 // straight into the registers that the matrix instruction takes, and the same bytes of x; a workgroup's waves, and the
 // grid's second dimension, cut the inner dimension, and the sums meet in LDS.  SHIFTED: rows that start anywhere.
 constexpr int kFewWaves = 8, kStep = 2 * kStage;
-template <int MT, bool SHIFTED>
-__global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a, uint32_t first_tile)
+template <int MT, bool SHIFTED, bool EPILOGUE>
+__global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a, uint32_t first_tile, Epilogue e)
 {
     __shared__ __align__(16) v4i sums[kFewWaves][MT][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -718,7 +913,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a, uint32_
         float ws[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) ws[r] = scale_at(a.w_scale, n + r, a.cols);
-        finish_four(a, blockIdx.y, m, n, s, scale_at(a.x_scale, m, a.rows), ws);
+        if constexpr (EPILOGUE) finish_four(a, e, m, n, s, scale_at(a.x_scale, m, a.rows), ws);
+        else finish_four(a, blockIdx.y, m, n, s, scale_at(a.x_scale, m, a.rows), ws);
     }
 }
 
@@ -727,8 +923,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(TileArgs a, uint32_
 // lanes one by one (4096 x 16384 bytes of w: 16 us for 16 rows of x, 31 for 48).  Here each wave has a ring of its own in LDS, which
 // the loads fill in lines, and no barrier but where the waves' sums meet.  Workgroups stay: a wave's stages run on from one
 // 16 columns of y to its next, so that w streams.  48 rows by 4096 x 16384 in 21.5 us: 3.1 TB/s of w, and x three times as much out of L2.
-template <int MT>
-__global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a)
+template <int MT, bool EPILOGUE>
+__global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a, Epilogue e)
 {
     constexpr int kStageBytes = (1 + MT) * 1024, kPlaces = 16384 / kStageBytes;
     static_assert(kPlaces >= 3 && kPlaces <= 8, "");
@@ -790,6 +986,21 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a)
     typedef const Scales __attribute__((address_space(4)))* ConstScales;
     typedef const float __attribute__((address_space(4)))* ConstFloat;
     int tile = blockIdx.x, left = each;
+    // An epilogue comes later, at one place for all stages: in every one of them its code would be there as often as there are places.
+    // (A tile has as many stages at least as there are places: no two are held at once.)
+    float held[4];
+    int64_t held_n = 0;
+    bool holds = false;
+    const auto finish_held = [&]() {
+        if (!EPILOGUE || !holds) return;
+        holds = false;
+        if (wave >= MT) return;
+        float bias[4];
+        load_bias(e, held_n, a.cols, bias);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) held[r] += bias[r];
+        finish_columns(a, e, m, held_n, held);
+    };
     const auto finish = [&]() {   // the waves' sums of a tile
         const int64_t n0 = (int64_t)tile * 16;
         if (whole * kStage < a.inner && wave == kFewWaves - 1) {   // the last stage, where it is not whole
@@ -826,8 +1037,15 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a)
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs * ws[r];
             const int64_t n = n0 + (lane >> 4) * 4;
-            if (m < a.rows && n < a.cols) store_four(a.y, a.dtype, m * a.cols + n, a.cols - n, v);
+            if constexpr (EPILOGUE) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) held[r] = v[r];
+                held_n = n;
+            } else {
+                if (m < a.rows && n < a.cols) store_four(a.y, a.dtype, m * a.cols + n, a.cols - n, v);
+            }
         }
+        holds = EPILOGUE;
         tile += gridDim.x;
         left = each;
     };
@@ -846,22 +1064,27 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a)
     int at = 0;
     if (total >= 2 * kPlaces) {   // (the steady part by itself, with no condition around its loads: behind one, the compiler waits for all)
         for_places([&](auto which) { load(place(which)); });
-        for (; at + 2 * kPlaces <= total; at += kPlaces)
+        for (; at + 2 * kPlaces <= total; at += kPlaces) {
+            finish_held();
             for_places([&](auto which) { stage(which, at + decltype(which)::value, std::true_type()); });
+        }
     } else {
         for_places([&](auto which) {
             if (decltype(which)::value < total) load(place(which));
         });
     }
-    for (; at < total; at += kPlaces)
+    for (; at < total; at += kPlaces) {
+        finish_held();
         for_places([&](auto which) {
             if (at + decltype(which)::value < total) stage(which, at + decltype(which)::value, std::false_type());
         });
+    }
+    finish_held();
 }
 
 // y from the sums of the splits, of both products of a launch: memory, and 3 us at the least
-template <bool INT8>
-__global__ __launch_bounds__(256) void k_join_splits(TwoProducts both)
+template <bool INT8, bool EPILOGUE>
+__global__ __launch_bounds__(256) void k_join_splits(TwoProducts both, Epilogue e)
 {
     const bool is_second = blockIdx.x >= both.second_at;
     const TileArgs a = is_second ? both.second : both.first;
@@ -883,6 +1106,13 @@ __global__ __launch_bounds__(256) void k_join_splits(TwoProducts both)
         s += __builtin_bit_cast(typename Matrix<INT8>::Sum, one);
     }
     const float xs = scale_at(a.x_scale, m, a.rows);
+    if constexpr (EPILOGUE) {
+        float ws[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ws[r] = scale_at(a.w_scale, n + r, a.cols);
+        finish_four(a, e, m, n, s, xs, ws);
+        return;
+    }
     float v[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs * scale_at(a.w_scale, n + r, a.cols);
@@ -1006,24 +1236,32 @@ bool is_streamed(const TileArgs& a)
            loads_fit(a.w, a.w_stride, 16, a.inner);
 }
 
+// `e`: the epilogue, or NULL
 template <int MT>
-void run_few(const TileArgs& a, hipStream_t s)
+void run_few(const TileArgs& a, const Epilogue* e, hipStream_t s)
 {
-    if (is_streamed(a)) {
+    constexpr int kPlaces = 16384 / ((1 + MT) * 1024);   // (an epilogue: as many stages of a tile for each wave)
+    if (is_streamed(a) && (!e || a.inner / kStage / kFewWaves >= kPlaces)) {
         const int64_t tiles = (a.cols + 15) / 16;
-        k_few_streamed<MT><<<dim3((uint32_t)(tiles < kUnits ? tiles : kUnits)), dim3(kFewWaves * 64), 0, s>>>(a);
+        const dim3 grid((uint32_t)(tiles < kUnits ? tiles : kUnits)), block(kFewWaves * 64);
+        if (e) k_few_streamed<MT, true><<<grid, block, 0, s>>>(a, *e);
+        else k_few_streamed<MT, false><<<grid, block, 0, s>>>(a, {});
         return;
     }
     const bool words = ((uintptr_t)a.x | (uintptr_t)a.w | (uint64_t)a.x_stride | (uint64_t)a.w_stride) % 4 == 0;
     in_launches((a.cols + 15) / 16, kFewWaves * 64, [&](int64_t first, uint32_t tiles) {
-        const dim3 grid(tiles, (uint32_t)a.splits);
-        if (words) k_few_rows<MT, false><<<grid, dim3(kFewWaves * 64), 0, s>>>(a, (uint32_t)first);
-        else k_few_rows<MT, true><<<grid, dim3(kFewWaves * 64), 0, s>>>(a, (uint32_t)first);
+        const dim3 grid(tiles, (uint32_t)a.splits), block(kFewWaves * 64);
+        const auto run = [&](auto shifted) {
+            if (e) k_few_rows<MT, shifted(), true><<<grid, block, 0, s>>>(a, (uint32_t)first, *e);
+            else k_few_rows<MT, shifted(), false><<<grid, block, 0, s>>>(a, (uint32_t)first, {});
+        };
+        if (words) run(std::false_type());
+        else run(std::true_type());
     });
 }
 
 template <int B, bool INT8>
-bool run_tiles(TwoProducts both, bool direct, hipStream_t s)
+bool run_tiles(TwoProducts both, const Epilogue* e, bool direct, hipStream_t s)
 {
     const auto groups = [](TileArgs& a) {
         a.tiles_m = (int)((a.rows + B - 1) / B);
@@ -1033,35 +1271,52 @@ bool run_tiles(TwoProducts both, bool direct, hipStream_t s)
     const int64_t first = groups(both.first), works = first + (both.second.rows ? groups(both.second) : 0);
     if (works > kMostGroups) return false;   // (more outputs than the memory holds, but for products of less than a tile's height)
     both.second_at = (uint32_t)first;
-    if (direct) k_tiles<B, INT8><<<dim3((uint32_t)works), dim3(kWaves * 64), 0, s>>>(both);
-    else k_tiles_any<B, INT8><<<dim3((uint32_t)works), dim3(kWaves * 64), 0, s>>>(both);
+    const dim3 grid((uint32_t)works), block(kWaves * 64);
+    if constexpr (INT8) {
+        if (e) {
+            if (direct) k_tiles_epilogue<B><<<grid, block, 0, s>>>(both, *e);
+            else k_tiles_any<B, true, true><<<grid, block, 0, s>>>(both, *e);
+            return true;
+        }
+    }
+    if (direct) k_tiles<B, INT8><<<grid, block, 0, s>>>(both);
+    else k_tiles_any<B, INT8, false><<<grid, block, 0, s>>>(both, {});
     return true;
 }
 
 // Runs one product, or two in one launch (second.rows 0: one).  The caller has made the plan and the partial sums' memory.
+// `e`: the epilogue of the one product, or NULL; where the inner dimension is cut, the join has it.
 template <bool INT8>
-int run_products(TwoProducts both, const Plan& p, hipStream_t s)
+int run_products(TwoProducts both, const Epilogue* e, const Plan& p, hipStream_t s)
 {
+    const Epilogue* const now = both.first.partial ? nullptr : e;
     both.first.splits = p.splits[0];
     both.first.stages_per_split = p.stages_per_split[0];
     both.second.splits = p.splits[1];
     both.second.stages_per_split = p.stages_per_split[1];
     if (p.few) {
-        if (p.few == 1) run_few<1>(both.first, s);
-        else if (p.few == 2) run_few<2>(both.first, s);
-        else if (p.few == 3) run_few<3>(both.first, s);
-        else run_few<4>(both.first, s);
+        if (p.few == 1) run_few<1>(both.first, now, s);
+        else if (p.few == 2) run_few<2>(both.first, now, s);
+        else if (p.few == 3) run_few<3>(both.first, now, s);
+        else run_few<4>(both.first, now, s);
     } else {
         const bool direct = is_direct(both.first, p.tile) && (!both.second.rows || is_direct(both.second, p.tile));
-        const bool fits = p.tile == 256   ? run_tiles<256, INT8>(both, direct, s)
-                          : p.tile == 128 ? run_tiles<128, INT8>(both, direct, s)
-                                          : run_tiles<64, INT8>(both, direct, s);
+        const bool fits = p.tile == 256   ? run_tiles<256, INT8>(both, now, direct, s)
+                          : p.tile == 128 ? run_tiles<128, INT8>(both, now, direct, s)
+                                          : run_tiles<64, INT8>(both, now, direct, s);
         if (!fits) return GEO_SC_ERR_UNSUPPORTED;
     }
     const auto joins = [](const TileArgs& a) { return a.partial ? (uint32_t)((a.rows * ((a.cols + 3) / 4) + 255) / 256) : 0u; };
     both.second_at = joins(both.first);
     const uint32_t all = both.second_at + joins(both.second);
-    if (all) k_join_splits<INT8><<<dim3(all), dim3(256), 0, s>>>(both);
+    if (all) {
+        if constexpr (INT8) {
+            if (e) k_join_splits<true, true><<<dim3(all), dim3(256), 0, s>>>(both, *e);
+            else k_join_splits<true, false><<<dim3(all), dim3(256), 0, s>>>(both, {});
+        } else {
+            k_join_splits<false, false><<<dim3(all), dim3(256), 0, s>>>(both, {});
+        }
+    }
     return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
 }
 
@@ -1090,6 +1345,11 @@ struct OperandArgs {
     int64_t rows_padded, cols_padded, peak_rows, peak_cols;
     uint32_t row_blocks, col_blocks, g_tiles, w_tiles;   // tiles: workgroups of the first two ranges
     uint32_t *row_peaks, *col_peaks;                 // [col_blocks][rows], [row_blocks][cols]: bits of the maxima
+    const void* slope;                               // [rows][cols] that g is multiplied by on its way in, or NULL
+    int slope_dtype;
+    float* col_sums;                                 // [row_blocks][cols] of g slope, or NULL
+    void* dbias;
+    int dbias_dtype;
     float *dx_back, *dw_back;
     f16 *dx_left, *dx_right, *dw_left, *dw_right;    // NULL, with its peaks: that gradient is not wanted
 };
@@ -1102,6 +1362,9 @@ __device__ __forceinline__ float power_for(uint32_t peak, float* back)
     *back = __uint_as_float((254 - field) << 23);
     return __uint_as_float(field << 23);
 }
+
+// (where the slope is zero nothing comes through, no infinity either)
+__device__ __forceinline__ float through_slope(float g, float slope) { return slope == 0.f ? 0.f : g * slope; }
 
 // the terms of v: each the fp16 nearest to what the earlier ones leave
 template <int TERMS>
@@ -1123,10 +1386,12 @@ __device__ __forceinline__ void store_terms(const float (&v)[kChunk], f16* out, 
 // A wave takes eight rows of 512 columns at once, a lane eight columns of them; a workgroup's waves pass over its block's rows, then
 // over further columns.  What lies outside is the last row and the last columns once more: a maximum stays what it is.
 // Bound by memory, the block's rows all asked for at once: 4096 x 4096 bf16 in 16 us.
-// NARROW: g has fewer columns than a lane takes.
-template <typename T, bool NARROW>
+// NARROW: g has fewer columns than a lane takes.  SLOPE: g is multiplied by a slope of type S on its way in.  SUMS: the columns' sums too, where
+// they are asked for.  Either takes four rows at once: the registers for eight are more than a wave of such workgroups has.
+template <typename T, bool NARROW, bool SUMS, bool SLOPE, typename S>
 __global__ __launch_bounds__(kPeakWaves * 64) void k_grad_peaks(OperandArgs a)
 {
+    constexpr int kBatch = SLOPE || SUMS ? 4 : kPeakBatch;
     __shared__ uint32_t row_most[kMostPeakRows], col_most[kPeakWaves * kPeakWide];   // (a wave writes its own rows')
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const uint32_t across = blockIdx.x / a.row_blocks, down = blockIdx.x % a.row_blocks;
@@ -1136,11 +1401,12 @@ __global__ __launch_bounds__(kPeakWaves * 64) void k_grad_peaks(OperandArgs a)
         const int64_t own = from + lane * kChunk, c = NARROW || own + kChunk <= a.cols ? own : a.cols - kChunk;
         float ws[kChunk] = {};
         uint32_t most[kChunk] = {};
+        float sums[kChunk] = {};
         if (a.row_peaks) load_chunk(a.w_scale, c, a.cols, 0.f, ws);
-        for (int64_t r = r0 + wave * kPeakBatch; r < r1; r += waves * kPeakBatch) {
-            T raw[kPeakBatch][kChunk];
+        for (int64_t r = r0 + wave * kBatch; r < r1; r += waves * kBatch) {
+            T raw[kBatch][kChunk];
 #pragma unroll
-            for (int i = 0; i < kPeakBatch; ++i) {
+            for (int i = 0; i < kBatch; ++i) {
                 const T* row = (const T*)a.g + (r + i < r1 ? r + i : r1 - 1) * a.g_stride;
                 if constexpr (NARROW) {
 #pragma unroll
@@ -1149,22 +1415,38 @@ __global__ __launch_bounds__(kPeakWaves * 64) void k_grad_peaks(OperandArgs a)
                     __builtin_memcpy(raw[i], row + c, sizeof raw[i]);
                 }
             }
-            uint32_t m[kPeakBatch];
+            S slope[SLOPE ? kBatch : 1][kChunk];
+            if constexpr (SLOPE) {
 #pragma unroll
-            for (int i = 0; i < kPeakBatch; ++i) {
+                for (int i = 0; i < kBatch; ++i) {
+                    const S* row = (const S*)a.slope + (r + i < r1 ? r + i : r1 - 1) * a.cols;
+                    if constexpr (NARROW) {
+#pragma unroll
+                        for (int j = 0; j < kChunk; ++j) slope[i][j] = c + j < a.cols ? row[c + j] : (S)0.f;
+                    } else {
+                        __builtin_memcpy(slope[i], row + c, sizeof slope[i]);
+                    }
+                }
+            }
+            uint32_t m[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
                 const float xs = a.col_peaks ? fabsf(a.x_scale[r + i < r1 ? r + i : r1 - 1]) : 0.f;
                 m[i] = 0;
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
-                    const float v = fabsf((float)raw[i][j]);
+                    float v = (float)raw[i][j];
+                    if constexpr (SLOPE) v = through_slope(v, (float)slope[i][j]);
+                    if constexpr (SUMS) sums[j] += r + i < r1 ? v : 0.f;
+                    v = fabsf(v);
                     most[j] = max(most[j], __float_as_uint(v * xs));
                     m[i] = max(m[i], __float_as_uint(v * fabsf(ws[j])));
                 }
             }
             if (a.row_peaks) {
-                // lanes trade halves of their rows until each holds one, row lane % 8
+                // lanes trade halves of their rows until each holds one, row lane % kBatch
 #pragma unroll
-                for (int half = kPeakBatch / 2; half >= 1; half /= 2)
+                for (int half = kBatch / 2; half >= 1; half /= 2)
 #pragma unroll
                     for (int i = 0; i < half; ++i) {
                         const bool upper = lane & half;
@@ -1172,9 +1454,9 @@ __global__ __launch_bounds__(kPeakWaves * 64) void k_grad_peaks(OperandArgs a)
                         m[i] = max(keep, (uint32_t)__shfl_xor((int)give, half));
                     }
 #pragma unroll
-                for (int d = 8; d < 64; d *= 2) m[0] = max(m[0], (uint32_t)__shfl_xor((int)m[0], d));
+                for (int d = kBatch; d < 64; d *= 2) m[0] = max(m[0], (uint32_t)__shfl_xor((int)m[0], d));
                 const int64_t at = r - r0 + lane;
-                if (lane < kPeakBatch && r + lane < r1) row_most[at] = from > c0 ? max(row_most[at], m[0]) : m[0];
+                if (lane < kBatch && r + lane < r1) row_most[at] = from > c0 ? max(row_most[at], m[0]) : m[0];
             }
         }
         if (a.col_peaks) {
@@ -1186,6 +1468,18 @@ __global__ __launch_bounds__(kPeakWaves * 64) void k_grad_peaks(OperandArgs a)
                 for (int v = 0; v < waves; ++v) one = max(one, col_most[v * kPeakWide + k]);
                 const int64_t mine = from + k % 64 * kChunk, n = (NARROW || mine + kChunk <= a.cols ? mine : a.cols - kChunk) + k / 64;
                 if (n < a.cols) a.col_peaks[down * a.cols + n] = one;
+            }
+            __syncthreads();
+        }
+        if (SUMS && a.col_sums) {
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) col_most[(wave * kChunk + j) * 64 + lane] = __float_as_uint(sums[j]);
+            __syncthreads();
+            for (int k = threadIdx.x; k < kPeakWide; k += blockDim.x) {
+                float one = 0.f;
+                for (int v = 0; v < waves; ++v) one += __uint_as_float(col_most[v * kPeakWide + k]);
+                const int64_t mine = from + k % 64 * kChunk, n = (NARROW || mine + kChunk <= a.cols ? mine : a.cols - kChunk) + k / 64;
+                if (n < a.cols) a.col_sums[down * a.cols + n] = one;
             }
             __syncthreads();
         }
@@ -1247,7 +1541,22 @@ __global__ __launch_bounds__(256) void k_grad_operands(OperandArgs a)
         const int at = i * 256 + threadIdx.x, r = at / (kSide / kChunk), c = at % (kSide / kChunk) * kChunk;
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) v[i][j] = 0.f;
-        if (r0 + r < a.rows && c0 + c < a.cols) load_chunk(a.g, a.dtype, (r0 + r) * a.g_stride, c0 + c, a.cols, 0.f, v[i]);
+        if (r0 + r < a.rows && c0 + c < a.cols) {
+            load_chunk(a.g, a.dtype, (r0 + r) * a.g_stride, c0 + c, a.cols, 0.f, v[i]);
+            if (a.slope) {
+                float slope[kChunk];
+                load_chunk(a.slope, a.slope_dtype, (r0 + r) * a.cols, c0 + c, a.cols, 0.f, slope);
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) v[i][j] = through_slope(v[i][j], slope[j]);
+            }
+        }
+    }
+    if (a.dbias && r0 == 0 && threadIdx.x < kSide && c0 + threadIdx.x < a.cols) {
+        float sum = 0.f;
+        for (uint32_t k = 0; k < a.row_blocks; ++k) sum += a.col_sums[k * a.cols + c0 + threadIdx.x];
+        if (a.dbias_dtype == GEO_SC_F32) ((f32*)a.dbias)[c0 + threadIdx.x] = sum;
+        else if (a.dbias_dtype == GEO_SC_BF16) ((bf16*)a.dbias)[c0 + threadIdx.x] = (bf16)sum;
+        else ((f16*)a.dbias)[c0 + threadIdx.x] = (f16)sum;
     }
     // the blocks' maxima of the tile's rows and columns, a quarter of the blocks per wave
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -1317,10 +1626,10 @@ int64_t peak_block(int64_t n, int64_t least, int64_t most)
 struct GradLayout {
     Shape dx, dw;
     Plan plan;   // the first product is dx, or dw where dx is not wanted
-    size_t dx_left, dx_right, dx_back, dw_left, dw_right, dw_back, row_peaks, col_peaks, first_partial, second_partial, bytes;
+    size_t dx_left, dx_right, dx_back, dw_left, dw_right, dw_back, row_peaks, col_peaks, col_sums, first_partial, second_partial, bytes;
     int64_t peak_rows, peak_cols;
 };
-GradLayout grad_layout(int64_t rows, int64_t cols, int64_t inner, int terms, bool need_dx, bool need_dw)
+GradLayout grad_layout(int64_t rows, int64_t cols, int64_t inner, int terms, bool need_dx, bool need_dw, bool need_dbias)
 {
     GradLayout l = {};
     size_t at = 0;
@@ -1348,9 +1657,10 @@ GradLayout grad_layout(int64_t rows, int64_t cols, int64_t inner, int terms, boo
         l.dw_right = take((size_t)inner * p * 2);
     }
     const Shape none = {};
-    l.plan = plan_of(need_dx ? l.dx : l.dw, need_dx && need_dw ? l.dw : none, false);
+    if (need_dx || need_dw) l.plan = plan_of(need_dx ? l.dx : l.dw, need_dx && need_dw ? l.dw : none, false);
     l.first_partial = take(partial_bytes(l.plan, 0, need_dx ? l.dx : l.dw));
     l.second_partial = take(need_dx && need_dw ? partial_bytes(l.plan, 1, l.dw) : 0);
+    if (need_dbias) l.col_sums = take((size_t)((rows + l.peak_rows - 1) / l.peak_rows) * cols * 4);
     l.bytes = at;
     return l;
 }
@@ -1370,6 +1680,148 @@ Plan forward_plan(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_
 bool sizes_fit(int64_t rows, int64_t cols, int64_t inner)
 {
     return rows >= 1 && cols >= 1 && inner >= 1 && rows <= 0x3fffffff && cols <= 0x3fffffff && inner <= 131071;
+}
+
+int forward(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride, const float* w_scale, int64_t rows,
+            int64_t cols, int64_t inner, void* y, int dtype, const Epilogue* e, void* workspace, size_t workspace_bytes, hipStream_t stream)
+{
+    if (!sizes_fit(rows, cols, inner) || !dtype_known(dtype) || x_stride < 0 || w_stride < 0 || !x || !w || !x_scale || !w_scale || !y)
+        return GEO_SC_ERR_INVALID_ARGUMENT;
+    TwoProducts both = {};
+    TileArgs& a = both.first;
+    const Plan plan = forward_plan(x, x_stride, w, w_stride, rows, cols, inner, &a);
+    const size_t partial = partial_bytes(plan, 0, {rows, cols, inner});
+    const Copies copies = copies_of(a, plan, rows, cols);
+    const size_t need = partial + copies.x + copies.w;
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return GEO_SC_ERR_WORKSPACE;
+    if (copies.x || copies.w) {
+        AlignArgs g = {};
+        uint8_t* to = (uint8_t*)workspace + partial;
+        g.inner = inner;
+        g.pieces = (uint32_t)((inner + 15) / 16);
+        const auto copy = [&](int which, const uint8_t*& from, int64_t& stride, int64_t count, uint8_t* at) {
+            g.from[which] = from;
+            g.stride[which] = stride;
+            g.works[which] = (uint32_t)count * g.pieces;
+            g.to[which] = at;
+            from = at;
+            stride = (int64_t)g.pieces * 16;
+        };
+        if (copies.x) copy(0, a.x, a.x_stride, rows, to);
+        if (copies.w) copy(1, a.w, a.w_stride, cols, to + copies.x);
+        k_align_rows<<<dim3((g.works[0] + 255) / 256 + (g.works[1] + 255) / 256), dim3(256), 0, stream>>>(g);
+    }
+    a.w_stages = 0x7fffffff;
+    a.x_scale = x_scale;
+    a.w_scale = w_scale;
+    a.y = y;
+    a.dtype = dtype;
+    a.partial = partial ? (uint32_t*)workspace : nullptr;
+    return run_products<true>(both, e, plan, stream);
+}
+
+int backward(const void* grad, int grad_dtype, int64_t grad_stride, const void* slope, int slope_type, const int8_t* x, int64_t x_stride,
+             const float* x_scale, const int8_t* w, int64_t w_stride, const float* w_scale, int64_t rows, int64_t cols, int64_t inner, void* dx,
+             int dx_dtype, void* dw, int dw_dtype, void* dbias, int dbias_dtype, void* workspace, size_t workspace_bytes, hipStream_t s)
+{
+    if (!sizes_fit(rows, cols, inner) || !dtype_known(grad_dtype) || (dx && !dtype_known(dx_dtype)) || (dw && !dtype_known(dw_dtype)) ||
+        (dbias && !dtype_known(dbias_dtype)) || (slope && !slope_type_known(slope_type)) ||
+        grad_stride < 0 || (grad_stride && rows > 1 && grad_stride < cols) || x_stride < 0 || w_stride < 0 || !grad || (dx && (!w || !w_scale)) ||
+        (dw && (!x || !x_scale)))
+        return GEO_SC_ERR_INVALID_ARGUMENT;
+    if (!dx && !dw && !dbias) return GEO_SC_OK;
+    const int terms = terms_of(grad_dtype);
+    const GradLayout l = grad_layout(rows, cols, inner, terms, dx, dw, dbias);
+    if (!workspace || workspace_bytes < l.bytes || (uintptr_t)workspace % 16) return GEO_SC_ERR_WORKSPACE;
+    const auto tiles = [](int64_t r, int64_t rs, int64_t c, int64_t cs) { return ((r + rs - 1) / rs) * ((c + cs - 1) / cs); };
+    const bool products = dx || dw;   // (for the bias alone: the first row of tiles)
+    const int64_t g_tiles = tiles(products ? rows : 1, kSide, cols, kSide), w_tiles = dx ? tiles(cols, kSide, inner, kWide) : 0,
+                  x_tiles = dw ? tiles(rows, kSide, inner, kWide) : 0;
+    const int64_t blocks = tiles(rows, l.peak_rows, cols, l.peak_cols);
+    if (g_tiles + w_tiles + x_tiles > kMostGroups || blocks > kMostGroups / (kPeakWaves * 64 / 256)) return GEO_SC_ERR_UNSUPPORTED;
+    uint8_t* base = (uint8_t*)workspace;
+    OperandArgs o = {};
+    o.g = grad;
+    o.dtype = grad_dtype;
+    o.g_stride = grad_stride;
+    o.x_stride = x_stride;
+    o.w_stride = w_stride;
+    o.rows = rows;
+    o.cols = cols;
+    o.inner = inner;
+    o.x = x;
+    o.w = w;
+    o.x_scale = x_scale;
+    o.w_scale = w_scale;
+    o.rows_padded = padded_to_side(rows);
+    o.cols_padded = padded_to_side(cols);
+    if (dx) {
+        o.dx_left = (f16*)(base + l.dx_left), o.dx_right = (f16*)(base + l.dx_right);
+        o.dx_back = (float*)(base + l.dx_back), o.row_peaks = (uint32_t*)(base + l.row_peaks);
+    }
+    if (dw) {
+        o.dw_left = (f16*)(base + l.dw_left), o.dw_right = (f16*)(base + l.dw_right);
+        o.dw_back = (float*)(base + l.dw_back), o.col_peaks = (uint32_t*)(base + l.col_peaks);
+    }
+    o.slope = slope;
+    o.slope_dtype = slope_type;
+    if (dbias) {
+        o.col_sums = (float*)(base + l.col_sums);
+        o.dbias = dbias;
+        o.dbias_dtype = dbias_dtype;
+    }
+    o.peak_rows = l.peak_rows;
+    o.peak_cols = l.peak_cols;
+    o.row_blocks = (uint32_t)((rows + l.peak_rows - 1) / l.peak_rows);
+    o.col_blocks = (uint32_t)((cols + l.peak_cols - 1) / l.peak_cols);
+    o.g_tiles = (uint32_t)g_tiles;
+    o.w_tiles = (uint32_t)w_tiles;
+    const dim3 peak_threads((uint32_t)((l.peak_rows < kPeakWaves * kPeakBatch ? l.peak_rows / kPeakBatch : kPeakWaves) * 64));
+    const auto peaks_of = [&](auto one, auto with_sums, auto with_slope, auto of_slope) {
+        using T = decltype(one);
+        using S = decltype(of_slope);
+        if (cols < kChunk) k_grad_peaks<T, true, with_sums(), with_slope(), S><<<dim3((uint32_t)blocks), peak_threads, 0, s>>>(o);
+        else k_grad_peaks<T, false, with_sums(), with_slope(), S><<<dim3((uint32_t)blocks), peak_threads, 0, s>>>(o);
+    };
+    const auto peaks = [&](auto one) {
+        const std::true_type yes;
+        const std::false_type no;
+        if (!slope && !dbias) peaks_of(one, no, no, one);
+        else if (!slope) peaks_of(one, yes, no, one);
+        else if (slope_type == GEO_SC_F32) peaks_of(one, yes, yes, f32());
+        else peaks_of(one, yes, yes, f16());
+    };
+    if (grad_dtype == GEO_SC_F32) peaks(f32());
+    else if (grad_dtype == GEO_SC_BF16) peaks(bf16());
+    else peaks(f16());
+    const dim3 grid((uint32_t)(g_tiles + w_tiles + x_tiles));
+    if (terms == 1) k_grad_operands<1><<<grid, dim3(256), 0, s>>>(o);
+    else k_grad_operands<2><<<grid, dim3(256), 0, s>>>(o);
+    if (!products) return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
+    const auto product = [&](const Shape& shape, size_t left, size_t right, size_t back, bool cut, size_t partial, void* y, int dtype) {
+        TileArgs a = {};
+        a.x = base + left;
+        a.w = base + right;
+        a.x_stride = shape.inner;
+        a.w_stride = shape.inner / terms;
+        a.rows = shape.rows;
+        a.cols = shape.cols;
+        a.inner = shape.inner;
+        a.w_stages = (int)(a.w_stride / kStage);
+        a.x_scale = (const float*)(base + back);
+        a.y = y;
+        a.dtype = dtype;
+        a.partial = cut ? (uint32_t*)(base + partial) : nullptr;
+        return a;
+    };
+    TwoProducts both = {};
+    if (dx) both.first = product(l.dx, l.dx_left, l.dx_right, l.dx_back, l.plan.splits[0] > 1, l.first_partial, dx, dx_dtype);
+    if (dw) {
+        const int which = dx ? 1 : 0;
+        (dx ? both.second : both.first) =
+            product(l.dw, l.dw_left, l.dw_right, l.dw_back, l.plan.splits[which] > 1, dx ? l.second_partial : l.first_partial, dw, dw_dtype);
+    }
+    return run_products<false>(both, nullptr, l.plan, s);
 }
 
 }  // namespace
@@ -1410,46 +1862,35 @@ int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, co
                      int64_t rows, int64_t cols, int64_t inner, void* y, int dtype, void* workspace, size_t workspace_bytes,
                      geo_sc_stream_t stream)
 {
-    if (!sizes_fit(rows, cols, inner) || !dtype_known(dtype) || x_stride < 0 || w_stride < 0 || !x || !w || !x_scale || !w_scale || !y)
+    return forward(x, x_stride, x_scale, w, w_stride, w_scale, rows, cols, inner, y, dtype, nullptr, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int geo_sc_matmul_q8_epilogue(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride, const float* w_scale,
+                              int64_t rows, int64_t cols, int64_t inner, const geo_sc_q8_epilogue* epilogue, void* y, int dtype,
+                              void* workspace, size_t workspace_bytes, geo_sc_stream_t stream)
+{
+    if (!epilogue || epilogue->struct_bytes != sizeof *epilogue || epilogue->activation < GEO_SC_ACT_NONE || epilogue->activation > GEO_SC_ACT_SILU ||
+        (epilogue->bias && !dtype_known(epilogue->bias_dtype)) || epilogue->residual_stride < 0 ||
+        (epilogue->slope && !slope_type_known(epilogue->slope_dtype)))
         return GEO_SC_ERR_INVALID_ARGUMENT;
-    TwoProducts both = {};
-    TileArgs& a = both.first;
-    const Plan plan = forward_plan(x, x_stride, w, w_stride, rows, cols, inner, &a);
-    const size_t partial = partial_bytes(plan, 0, {rows, cols, inner});
-    const Copies copies = copies_of(a, plan, rows, cols);
-    const size_t need = partial + copies.x + copies.w;
-    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return GEO_SC_ERR_WORKSPACE;
-    if (copies.x || copies.w) {
-        AlignArgs g = {};
-        uint8_t* to = (uint8_t*)workspace + partial;
-        g.inner = inner;
-        g.pieces = (uint32_t)((inner + 15) / 16);
-        const auto copy = [&](int which, const uint8_t*& from, int64_t& stride, int64_t count, uint8_t* at) {
-            g.from[which] = from;
-            g.stride[which] = stride;
-            g.works[which] = (uint32_t)count * g.pieces;
-            g.to[which] = at;
-            from = at;
-            stride = (int64_t)g.pieces * 16;
-        };
-        if (copies.x) copy(0, a.x, a.x_stride, rows, to);
-        if (copies.w) copy(1, a.w, a.w_stride, cols, to + copies.x);
-        k_align_rows<<<dim3((g.works[0] + 255) / 256 + (g.works[1] + 255) / 256), dim3(256), 0, (hipStream_t)stream>>>(g);
-    }
-    a.w_stages = 0x7fffffff;
-    a.x_scale = x_scale;
-    a.w_scale = w_scale;
-    a.y = y;
-    a.dtype = dtype;
-    a.partial = partial ? (uint32_t*)workspace : nullptr;
-    return run_products<true>(both, plan, (hipStream_t)stream);
+    const Epilogue e = {epilogue->bias,       epilogue->residual,    epilogue->slope,     epilogue->residual_stride,
+                        epilogue->bias_dtype, epilogue->slope_dtype, epilogue->activation};
+    return forward(x, x_stride, x_scale, w, w_stride, w_scale, rows, cols, inner, y, dtype, &e, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 int geo_sc_matmul_q8_backward_workspace_size(int64_t rows, int64_t cols, int64_t inner, int grad_dtype, int need_dx, int need_dw,
                                              size_t* bytes)
 {
     if (!bytes || !sizes_fit(rows, cols, inner) || !dtype_known(grad_dtype)) return GEO_SC_ERR_INVALID_ARGUMENT;
-    *bytes = need_dx || need_dw ? grad_layout(rows, cols, inner, terms_of(grad_dtype), need_dx, need_dw).bytes : 0;
+    *bytes = need_dx || need_dw ? grad_layout(rows, cols, inner, terms_of(grad_dtype), need_dx, need_dw, false).bytes : 0;
+    return GEO_SC_OK;
+}
+
+int geo_sc_matmul_q8_epilogue_backward_workspace_size(int64_t rows, int64_t cols, int64_t inner, int grad_dtype, int need_dx, int need_dw,
+                                                      int need_dbias, size_t* bytes)
+{
+    if (!bytes || !sizes_fit(rows, cols, inner) || !dtype_known(grad_dtype)) return GEO_SC_ERR_INVALID_ARGUMENT;
+    *bytes = grad_layout(rows, cols, inner, terms_of(grad_dtype), need_dx, need_dw, need_dbias).bytes;
     return GEO_SC_OK;
 }
 
@@ -1458,86 +1899,17 @@ int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64_t grad_str
                               int64_t inner, void* dx, int dx_dtype, void* dw, int dw_dtype, void* workspace, size_t workspace_bytes,
                               geo_sc_stream_t stream)
 {
-    if (!sizes_fit(rows, cols, inner) || !dtype_known(grad_dtype) || (dx && !dtype_known(dx_dtype)) || (dw && !dtype_known(dw_dtype)) ||
-        grad_stride < 0 || (grad_stride && rows > 1 && grad_stride < cols) || x_stride < 0 || w_stride < 0 || !grad || (dx && (!w || !w_scale)) ||
-        (dw && (!x || !x_scale)))
-        return GEO_SC_ERR_INVALID_ARGUMENT;
-    if (!dx && !dw) return GEO_SC_OK;
-    const int terms = terms_of(grad_dtype);
-    const GradLayout l = grad_layout(rows, cols, inner, terms, dx, dw);
-    if (!workspace || workspace_bytes < l.bytes || (uintptr_t)workspace % 16) return GEO_SC_ERR_WORKSPACE;
-    const auto tiles = [](int64_t r, int64_t rs, int64_t c, int64_t cs) { return ((r + rs - 1) / rs) * ((c + cs - 1) / cs); };
-    const int64_t g_tiles = tiles(rows, kSide, cols, kSide), w_tiles = dx ? tiles(cols, kSide, inner, kWide) : 0,
-                  x_tiles = dw ? tiles(rows, kSide, inner, kWide) : 0;
-    const int64_t blocks = tiles(rows, l.peak_rows, cols, l.peak_cols);
-    if (g_tiles + w_tiles + x_tiles > kMostGroups || blocks > kMostGroups / (kPeakWaves * 64 / 256)) return GEO_SC_ERR_UNSUPPORTED;
-    hipStream_t s = (hipStream_t)stream;
-    uint8_t* base = (uint8_t*)workspace;
-    OperandArgs o = {};
-    o.g = grad;
-    o.dtype = grad_dtype;
-    o.g_stride = grad_stride;
-    o.x_stride = x_stride;
-    o.w_stride = w_stride;
-    o.rows = rows;
-    o.cols = cols;
-    o.inner = inner;
-    o.x = x;
-    o.w = w;
-    o.x_scale = x_scale;
-    o.w_scale = w_scale;
-    o.rows_padded = padded_to_side(rows);
-    o.cols_padded = padded_to_side(cols);
-    if (dx) {
-        o.dx_left = (f16*)(base + l.dx_left), o.dx_right = (f16*)(base + l.dx_right);
-        o.dx_back = (float*)(base + l.dx_back), o.row_peaks = (uint32_t*)(base + l.row_peaks);
-    }
-    if (dw) {
-        o.dw_left = (f16*)(base + l.dw_left), o.dw_right = (f16*)(base + l.dw_right);
-        o.dw_back = (float*)(base + l.dw_back), o.col_peaks = (uint32_t*)(base + l.col_peaks);
-    }
-    o.peak_rows = l.peak_rows;
-    o.peak_cols = l.peak_cols;
-    o.row_blocks = (uint32_t)((rows + l.peak_rows - 1) / l.peak_rows);
-    o.col_blocks = (uint32_t)((cols + l.peak_cols - 1) / l.peak_cols);
-    o.g_tiles = (uint32_t)g_tiles;
-    o.w_tiles = (uint32_t)w_tiles;
-    const dim3 peak_threads((uint32_t)((l.peak_rows < kPeakWaves * kPeakBatch ? l.peak_rows / kPeakBatch : kPeakWaves) * 64));
-    const auto peaks = [&](auto one) {
-        using T = decltype(one);
-        if (cols < kChunk) k_grad_peaks<T, true><<<dim3((uint32_t)blocks), peak_threads, 0, s>>>(o);
-        else k_grad_peaks<T, false><<<dim3((uint32_t)blocks), peak_threads, 0, s>>>(o);
-    };
-    if (grad_dtype == GEO_SC_F32) peaks(f32());
-    else if (grad_dtype == GEO_SC_BF16) peaks(bf16());
-    else peaks(f16());
-    const dim3 grid((uint32_t)(g_tiles + w_tiles + x_tiles));
-    if (terms == 1) k_grad_operands<1><<<grid, dim3(256), 0, s>>>(o);
-    else k_grad_operands<2><<<grid, dim3(256), 0, s>>>(o);
-    const auto product = [&](const Shape& shape, size_t left, size_t right, size_t back, bool cut, size_t partial, void* y, int dtype) {
-        TileArgs a = {};
-        a.x = base + left;
-        a.w = base + right;
-        a.x_stride = shape.inner;
-        a.w_stride = shape.inner / terms;
-        a.rows = shape.rows;
-        a.cols = shape.cols;
-        a.inner = shape.inner;
-        a.w_stages = (int)(a.w_stride / kStage);
-        a.x_scale = (const float*)(base + back);
-        a.y = y;
-        a.dtype = dtype;
-        a.partial = cut ? (uint32_t*)(base + partial) : nullptr;
-        return a;
-    };
-    TwoProducts both = {};
-    if (dx) both.first = product(l.dx, l.dx_left, l.dx_right, l.dx_back, l.plan.splits[0] > 1, l.first_partial, dx, dx_dtype);
-    if (dw) {
-        const int which = dx ? 1 : 0;
-        (dx ? both.second : both.first) =
-            product(l.dw, l.dw_left, l.dw_right, l.dw_back, l.plan.splits[which] > 1, dx ? l.second_partial : l.first_partial, dw, dw_dtype);
-    }
-    return run_products<false>(both, l.plan, s);
+    return backward(grad, grad_dtype, grad_stride, nullptr, 0, x, x_stride, x_scale, w, w_stride, w_scale, rows, cols, inner, dx, dx_dtype, dw,
+                    dw_dtype, nullptr, 0, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int geo_sc_matmul_q8_epilogue_backward(const void* grad, int grad_dtype, int64_t grad_stride, const void* slope, int slope_dtype, const int8_t* x,
+                                       int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride, const float* w_scale, int64_t rows,
+                                       int64_t cols, int64_t inner, void* dx, int dx_dtype, void* dw, int dw_dtype, void* dbias, int dbias_dtype,
+                                       void* workspace, size_t workspace_bytes, geo_sc_stream_t stream)
+{
+    return backward(grad, grad_dtype, grad_stride, slope, slope_dtype, x, x_stride, x_scale, w, w_stride, w_scale, rows, cols, inner, dx,
+                    dx_dtype, dw, dw_dtype, dbias, dbias_dtype, workspace, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -19,6 +19,8 @@ def build_parser():
     p.description = "SC CNN trained from an 8-bit teacher's top logits on MI355X"
     p.add_argument("--teacher_epochs", default=10, type=int)
     p.add_argument("--teacher_lr", default=1e-3, type=float)
+    p.add_argument("--teacher_optim", default="Adam", choices=("Adam", "AdamW", "AdamW8"), help="AdamW8: states in 8 bits")
+    p.add_argument("--teacher_gated", default=0, type=int, help="1: the teacher's blocks are normed and gated behind too, with gelu and biases")
     p.add_argument("--top", default=5, type=int, help="the teacher's logits that the student sees per image")
     p.add_argument("--temperature", default=4.0, type=float)
     p.add_argument("--alpha", default=0.9, type=float, help="weight of the divergence; 1 - alpha: of the labels' cross entropy")
@@ -32,9 +34,13 @@ def _batches(loader, iterations):
         yield inputs.cuda(non_blocking=True), target.cuda(non_blocking=True)
 
 
-def train_teacher(teacher, loader, epochs, lr, iterations=None):
-    """Returns the mean loss of each epoch."""
-    optimizer, criterion, losses = optim.Adam(teacher.parameters(), lr=lr), nn.CrossEntropyLoss(), []
+def train_teacher(teacher, loader, epochs, lr, iterations=None, optimizer="Adam"):
+    """Returns the mean loss of each epoch.  ``optimizer``: "Adam" (PyTorch's), "AdamW" or "AdamW8" (``network.AdamW``)."""
+    if optimizer == "Adam":
+        optimizer = optim.Adam(teacher.parameters(), lr=lr)
+    else:
+        optimizer = network.AdamW(teacher.parameters(), lr=lr, state_bits=8 if optimizer == "AdamW8" else 32)
+    criterion, losses = nn.CrossEntropyLoss(), []
     teacher.train()
     for _ in range(epochs):
         mean = utils_own.AverageMeter()
@@ -75,8 +81,8 @@ def main(argv=None):
         raise SystemExit("this build runs on the GPU only: --device must be >= 0 and a GPU must be visible")
     torch.cuda.set_device(args.device)
     trainloader, testloader = main_conv._loaders(args)
-    teacher = network.PatchMLP_q8().cuda()
-    teacher_losses = train_teacher(teacher, trainloader, args.teacher_epochs, args.teacher_lr, args.iterations)
+    teacher = network.PatchMLP_q8(**(dict(activation="gelu", gated=True, bias=True) if args.teacher_gated else {})).cuda()
+    teacher_losses = train_teacher(teacher, trainloader, args.teacher_epochs, args.teacher_lr, args.iterations, args.teacher_optim)
     teacher.eval()
     teacher.prepare()
     print("Teacher: loss per epoch " + " ".join(f"{v:.4f}" for v in teacher_losses))

@@ -263,16 +263,20 @@ class VGG16_add_partial(nn.Module):
 
 class PatchMLP_q8(nn.Module):
     """Residual network of dense 8-bit layers on image patches: every patch of ``patch`` x ``patch`` pixels is a row; blocks of
-    norm, widening, relu and narrowing; the rows' mean through a last norm and layer.  All products are exact 8-bit ones
-    (``utils_class.Linear_Q8``), so it serves as the teacher of an SC network (``python -m geo_amd.main_distill``).  Not in
+    norm, widening, activation and narrowing; the rows' mean through a last norm and layer.  All products are exact 8-bit ones
+    (``utils_class.Linear_Q8``), so it serves as the teacher of an SC network (``python -m geo_amd.main_distill``).  ``gated``: each block's
+    output is normed and gated before it joins the stream (``utils_class.GatedNormLinear_Q8``); ``bias``: the blocks' layers have one.  Not in
     the reference."""
 
-    def __init__(self, num_classes=10, c_in=3, patch=4, width=256, hidden=1024, depth=4):
+    def __init__(self, num_classes=10, c_in=3, patch=4, width=256, hidden=1024, depth=4, activation="relu", gated=False, bias=False):
         super().__init__()
         self.patch = patch
+        self.gated = gated
         self.embed = utils_class.Linear_Q8(c_in * patch * patch, width)
-        self.up = nn.ModuleList(utils_class.NormLinear_Q8(width, hidden) for _ in range(depth))
-        self.down = nn.ModuleList(utils_class.Linear_Q8(hidden, width) for _ in range(depth))
+        inner = dict(bias=bias, activation=activation)
+        self.up = nn.ModuleList((utils_class.GatedNormLinear_Q8 if gated and i else utils_class.NormLinear_Q8)(width, hidden, **inner)
+                                for i in range(depth))
+        self.down = nn.ModuleList(utils_class.Linear_Q8(hidden, width, bias=bias) for _ in range(depth))
         self.head = utils_class.NormLinear_Q8(width, num_classes)
 
     def prepare(self):
@@ -290,7 +294,7 @@ class PatchMLP_q8(nn.Module):
         y, total = self.embed(rows), None
         for up, down in zip(self.up, self.down):
             wide, total = up(y, total)
-            y = down(F.relu(wide))
+            y = down(wide)
         logits, _ = self.head((y if total is None else total + y).mean(1))
         return logits
 

@@ -222,15 +222,17 @@ def sc_conv_block(conv, bn, input, *, err=7, forward="1d_bin", z_unit=8, load_un
 
 
 class Linear_Q8(nn.Module):
-    """Linear layer without bias whose operands are rounded to 8-bit rows (``utils_functional.linear_q8``): the exact counterpart
-    of an SC layer's product.  In training the weight is rounded on every call and the gradients pass straight through.  For
+    """Linear layer whose operands are rounded to 8-bit rows (``utils_functional.linear_q8``): the exact counterpart
+    of an SC layer's product; with ``bias``, ``activation`` (None, "relu", "gelu", "silu") and a residual in the product's kernel.  In training the weight is rounded on every call and the gradients pass straight through.  For
     inference ``prepare()`` rounds it once, and calls without gradients take that result until ``train()``, ``load_state_dict`` or
     a move to another device or type drops it; ``eval()`` keeps it.  A weight that has been written to since is said so in a warning."""
 
-    def __init__(self, in_features, out_features):
+    def __init__(self, in_features, out_features, bias=False, activation=None):
         super().__init__()
         self.weight = nn.Parameter(torch.empty(out_features, in_features))
         nn.init.kaiming_uniform_(self.weight, a=5 ** 0.5)
+        self.register_parameter("bias", nn.Parameter(torch.zeros(out_features)) if bias else None)
+        self.activation = activation
         self._q8 = None
 
     def _weight_now(self):
@@ -276,26 +278,50 @@ class Linear_Q8(nn.Module):
             warnings.warn("the weight has changed since prepare(), whose result this call takes: prepare() again", stacklevel=3)
         return None if torch.is_grad_enabled() else self._q8
 
-    def forward(self, x):
+    def forward(self, x, residual=None):
         weight = self._prepared()
+        epilogue = dict(bias=self.bias, activation=self.activation)
         if weight is None:
-            return utils_functional.linear_q8(x, self.weight)
+            return utils_functional.linear_q8(x, self.weight, residual=residual, **epilogue)
         q, scale, _ = utils_functional.quantize_rows(x)
-        return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype)
+        return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype, residual=residual, **epilogue)
 
 
 class NormLinear_Q8(Linear_Q8):
     """Root-mean-square norm of ``x + residual`` with 8-bit output, then the product of ``Linear_Q8``
     (``utils_functional.norm_linear_q8``).  Returns (y, x + residual)."""
 
-    def __init__(self, in_features, out_features, eps=1e-6):
-        super().__init__(in_features, out_features)
+    def __init__(self, in_features, out_features, eps=1e-6, bias=False, activation=None):
+        super().__init__(in_features, out_features, bias, activation)
         self.gain = nn.Parameter(torch.ones(in_features))
         self.eps = eps
 
     def forward(self, x, residual=None):
         weight = self._prepared()
+        epilogue = dict(bias=self.bias, activation=self.activation)
         if weight is None:
-            return utils_functional.norm_linear_q8(x, self.gain, self.weight, residual=residual, eps=self.eps)
+            return utils_functional.norm_linear_q8(x, self.gain, self.weight, residual=residual, eps=self.eps, **epilogue)
         q, scale, total, _ = utils_functional.rms_norm_q8(x, self.gain, residual=residual, eps=self.eps)
-        return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype), total
+        return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype, **epilogue), total
+
+
+class GatedNormLinear_Q8(NormLinear_Q8):
+    """``NormLinear_Q8`` behind a block whose output ``x`` is normed and gated before it joins the stream ``residual``
+    (``utils_functional.gated_norm``, its 8-bit form once the weight is prepared), then the product.  Parameters: ``gain`` (in front of
+    the product), ``post_gain`` and ``gate`` (of the block's output, per channel), ``residual_scale``.  Returns (y, the new stream)."""
+
+    def __init__(self, in_features, out_features, eps=1e-6, bias=False, activation=None, gate=1.0):
+        super().__init__(in_features, out_features, eps, bias, activation)
+        self.post_gain = nn.Parameter(torch.ones(in_features))
+        self.gate = nn.Parameter(torch.full((in_features,), float(gate)))
+        self.residual_scale = nn.Parameter(torch.ones(in_features))
+
+    def forward(self, x, residual):
+        weight = self._prepared()
+        around = dict(post_weight=self.post_gain, gate=self.gate, residual_scale=self.residual_scale, eps=self.eps)
+        epilogue = dict(bias=self.bias, activation=self.activation)
+        if weight is None:
+            normed, total = utils_functional.gated_norm(x, residual, self.gain, **around)
+            return utils_functional.linear_q8(normed, self.weight, **epilogue), total
+        q, scale, total, _ = utils_functional.gated_norm_q8(x, residual, self.gain, **around)
+        return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype, **epilogue), total

@@ -209,24 +209,35 @@ def rms_norm_q8(x, weight, residual=None, eps=1e-6, values=None):
     return _dense().rms_norm_q8(x, weight, residual, eps, values)
 
 
-def matmul_q8(q, scale, weight_q, weight_scale, dtype=torch.float32):
-    """``y[..., n] = scale[...] * weight_scale[n] * sum_k q[..., k] * weight_q[n, k]`` for 8-bit rows with a scale each
-    (``quantize_rows``, ``rms_norm_q8``); the integer sum is exact (at most 131071 terms).  ``y`` is of ``dtype``.  No
-    gradients: see ``linear_q8``."""
-    return _dense().matmul_q8(q, scale, weight_q, weight_scale, dtype)
+def matmul_q8(q, scale, weight_q, weight_scale, dtype=torch.float32, bias=None, activation=None, residual=None):
+    """``y[..., n] = act(scale[...] * weight_scale[n] * sum_k q[..., k] * weight_q[n, k] + bias[n]) + residual[..., n]`` for 8-bit rows with a
+    scale each (``quantize_rows``, ``rms_norm_q8``, ``gated_norm_q8``); the integer sum is exact (at most 131071 terms), what follows is
+    float32, ``y``, rounded once, of ``dtype``.  ``bias``: (columns,) of any of the three types; ``activation``: None, "relu", "gelu" (z times
+    the normal distribution's share below z) or "silu" (z / (1 + exp(-z))); ``residual``: of y's shape and type.  No gradients: see
+    ``linear_q8``."""
+    if bias is None and activation is None and residual is None:
+        return _dense().matmul_q8(q, scale, weight_q, weight_scale, dtype)
+    if _wants_grad(bias, residual):
+        raise ValueError("matmul_q8 has no gradients: take linear_q8 (or torch.no_grad())")
+    return _dense().matmul_q8_epilogue(q, scale, weight_q, weight_scale, dtype, bias, activation, residual)
 
 
-def linear_q8(x, weight):
-    """``x @ weight.t()`` with both operands rounded to 8-bit rows first, in ``x``'s type.  The gradients are those of the
-    product at the rounded operands, passed straight through the rounding, as ``Conv2d_Add_Partial`` passes its own.  The upstream
-    gradient, times a scale, enters them with 11 bits where it is bfloat16 and with 23 where it is float16 or float32."""
-    return _dense().linear_q8(x, weight)
+def linear_q8(x, weight, bias=None, activation=None, residual=None):
+    """``act(x @ weight.t() + bias) + residual`` with both operands of the product rounded to 8-bit rows first, in ``x``'s type
+    (``matmul_q8`` says what the epilogue takes).  The gradients are those of the product at the rounded operands, passed straight
+    through the rounding, as ``Conv2d_Add_Partial`` passes its own.  The upstream gradient, times a scale and the activation's slope, enters them
+    with 11 bits where it is bfloat16 and with 23 where it is float16 or float32; the slope of gelu and silu is kept with 11 bits for bfloat16, with
+    24 otherwise."""
+    if bias is None and activation is None and residual is None:
+        return _dense().linear_q8(x, weight)
+    return _dense().linear_q8_epilogue(x, weight, bias, activation, residual)
 
 
-def norm_linear_q8(x, gain, weight, residual=None, eps=1e-6):
+def norm_linear_q8(x, gain, weight, residual=None, eps=1e-6, bias=None, activation=None):
     """The root-mean-square norm of ``x + residual`` with 8-bit output (``rms_norm_q8``, weight ``gain``) and its
-    product with ``weight`` rounded to 8-bit rows: (y, x + residual), differentiable (once) in all four tensors."""
-    return _dense().norm_linear_q8(x, gain, weight, residual, eps)
+    product with ``weight`` rounded to 8-bit rows, with bias and activation (``matmul_q8``): (y, x + residual), differentiable (once)
+    in all tensors."""
+    return _dense().norm_linear_q8(x, gain, weight, residual, eps, bias, activation)
 
 
 # ---------------------------------------------------------------- distillation

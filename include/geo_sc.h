@@ -532,6 +532,36 @@ GEO_SC_API int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64
                                          size_t workspace_bytes, geo_sc_stream_t stream);
 
 /*
+ * The same product with an epilogue: with z = x_scale[m] w_scale[n] sum + bias[n] in fp32, y = act(z) + residual, rounded once.
+ * Activations: relu; gelu, z times the normal distribution's share below z; silu, z / (1 + exp(-z)).
+ *   bias, residual   NULL: none; `cols` elements of bias_dtype, (rows, cols) of y's dtype with residual_stride between its rows
+ *   slope            NULL, or (rows, cols), without gaps, for the backward: act'(z) in slope_dtype, GEO_SC_F16 or GEO_SC_F32
+ * Workspace: geo_sc_matmul_q8_workspace_size.
+ * Backward, from g (gradient of y): with dz = g slope (0 where the slope is 0; slope NULL: dz = g), dx and dw as
+ * geo_sc_matmul_q8_backward has them from dz, dbias[n] = sum_m dz[m][n] in an order that does not change from run to run; each of the three may be
+ * NULL.  The residual's gradient is g.
+ */
+enum geo_sc_activation { GEO_SC_ACT_NONE = 0, GEO_SC_ACT_RELU = 1, GEO_SC_ACT_GELU = 2, GEO_SC_ACT_SILU = 3 };
+typedef struct geo_sc_q8_epilogue {
+    size_t struct_bytes; /* sizeof(geo_sc_q8_epilogue) */
+    const void* bias;
+    const void* residual;
+    void* slope;
+    int64_t residual_stride;
+    int32_t bias_dtype, slope_dtype, activation;
+} geo_sc_q8_epilogue;
+GEO_SC_API int geo_sc_matmul_q8_epilogue(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
+                                         const float* w_scale, int64_t rows, int64_t cols, int64_t inner, const geo_sc_q8_epilogue* epilogue,
+                                         void* y, int dtype, void* workspace, size_t workspace_bytes, geo_sc_stream_t stream);
+GEO_SC_API int geo_sc_matmul_q8_epilogue_backward_workspace_size(int64_t rows, int64_t cols, int64_t inner, int grad_dtype, int need_dx,
+                                                                 int need_dw, int need_dbias, size_t* bytes);
+GEO_SC_API int geo_sc_matmul_q8_epilogue_backward(const void* grad, int grad_dtype, int64_t grad_stride, const void* slope, int slope_dtype,
+                                                  const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
+                                                  const float* w_scale, int64_t rows, int64_t cols, int64_t inner, void* dx, int dx_dtype,
+                                                  void* dw, int dw_dtype, void* dbias, int dbias_dtype, void* workspace,
+                                                  size_t workspace_bytes, geo_sc_stream_t stream);
+
+/*
  * Distillation from a teacher's top logits at temperature T: per row p = softmax of the entries' top_logits / T, q = softmax of
  * logits / T over all columns, loss = T^2 sum_k p_k (log p_k - log q[top_index_k]).  top_logits and top_index are (rows, top) without
  * gaps, top at most 4096, index_bytes 4 or 8; an entry whose index is outside [0, cols) is absent, a column named twice counts
