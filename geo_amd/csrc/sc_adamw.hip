@@ -53,6 +53,7 @@ struct Share {
     Tensor tensors[kTensors];
 };
 static_assert(sizeof(Share) <= 4096, "the arguments of a launch");
+static_assert(kTensors <= 64, "a lane for each tensor");
 
 __host__ __device__ inline Steps steps_at(double lr, double b1, double b2, int64_t t)
 {
@@ -74,17 +75,22 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v)
 }
 // A scale's byte is the exponent field of a float; 0 is half of the smallest normal one, 255 no number.
 __device__ __forceinline__ float scale_of(uint8_t byte) { return __uint_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : (uint32_t)byte << 23); }
-__device__ __forceinline__ float decode(uint32_t code)
+__device__ __forceinline__ void decode(const uint8_t (&codes)[kChunk], float (&v)[kChunk])
 {
-    // (the code's fields as those of a float: exponents below 2^-6 - 120 are denormals there as here)
-    const float v = __uint_as_float((code & 0x7f) << 20) * 0x1p120f;
-    const float size = (code & 0x7f) == 0x7f ? __uint_as_float(0x7fc00000u) : v;
-    return code & 0x80 ? -size : size;
+#ifdef __HIP_DEVICE_COMPILE__
+    uint32_t words[2];
+    __builtin_memcpy(words, codes, sizeof words);
+#pragma unroll
+    for (int j = 0; j < kChunk; j += 2) {
+        const auto two = j & 2 ? __builtin_amdgcn_cvt_pk_f32_fp8((int)words[j / 4], true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)words[j / 4], false);
+        v[j] = two[0];
+        v[j + 1] = two[1];
+    }
+#endif
 }
-// The code of v >= 0, up to 256, or of no number; `dither` of 2^32 is the fraction of a step from which on it goes up.
+// The code of v >= 0, up to 256; `dither` of 2^32 is the fraction of a step from which on it goes up.
 __device__ __forceinline__ uint32_t encode(float v, uint32_t dither)
 {
-    if (!(v < __uint_as_float(kInfinityBits))) return 0x7f;
     const bool tiny = v < 0x1p-6f;   // steps of 2^-9: those that 2^-6 .. 2^-5 has
     const uint32_t up = __float_as_uint(tiny ? v + 0x1p-6f : v) + (dither >> 12);
     return (up >> 20) - (tiny ? 121 * 8 : 120 * 8);
@@ -128,21 +134,27 @@ struct States<8> {
         codes(t.sq, c, t.elements, s);
         const bool there = c < t.elements;
         const float up = there ? scale_of(t.avg_scale[c / kBlock]) : 0.f, root_up = there ? scale_of(t.sq_scale[c / kBlock]) : 0.f;
+        decode(a, m);
+        decode(s, v);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
-            m[j] = decode(a[j]) * up;
-            const float root = decode(s[j]) * root_up;
-            v[j] = root * root;
+            m[j] *= up;
+            v[j] *= root_up;
+            v[j] *= v[j];
         }
     }
     template <bool ROOT>
     static __device__ __forceinline__ void put(void* to, uint8_t* scale, int64_t c, int64_t n, const float (&x)[kChunk], uint32_t first)
     {
+        // (behind the tensor's end x is zero)
         uint32_t most = 0;
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-            const uint32_t bits = c + j < n ? magnitude_bits(x[j]) : 0;
-            most = max(most, bits < kInfinityBits ? bits : 0);
+        for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(x[j]));
+        const bool numbers = !__any(most >= kInfinityBits);   // of the wave's chunks: nearly always
+        if (!numbers) {
+            most = 0;
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) most = max(most, magnitude_bits(x[j]) < kInfinityBits ? magnitude_bits(x[j]) : 0);
         }
         most = block_max(most) >> 23;
         const uint32_t field = most > 8 ? most - 7 : 1;
@@ -151,6 +163,7 @@ struct States<8> {
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
             uint32_t code = encode(fabsf(x[j]) * down, first + (uint32_t)j * 0x9E3779B1u);
+            if (!numbers && magnitude_bits(x[j]) >= kInfinityBits) code = 0x7f;
             if (ROOT) code = x[j] > 0.f ? max(code, 1u) : code;
             else code |= __float_as_uint(x[j]) >> 31 << 7;
             raw[j] = (uint8_t)code;
@@ -178,8 +191,10 @@ struct States<8> {
 template <typename P, typename G, int BITS>
 __global__ __launch_bounds__(kThreads) void k_adamw(Share s)
 {
-    int i = 0;
-    for (int k = 1; k < s.count; ++k) i += s.first[k] <= blockIdx.x;
+    // the tensor: each lane looks at the first workgroup of one
+    const int lane = threadIdx.x & 63;
+    const bool begun = lane < s.count && s.first[lane < kTensors ? lane : 0] <= blockIdx.x;
+    const int i = __popcll(__ballot(begun)) - 1;
     const Tensor& t = s.tensors[i];
     const Constants& k = s.c;
     const Steps steps = k.device_steps ? *k.device_steps : k.steps;

@@ -35,7 +35,7 @@ struct NormArgs {
     int64_t first_row;   // of a launch
 };
 
-// Sum and largest over a row's lanes: LANES 32 (two rows in a wave) or 64, then over its waves.
+// Sum, or sum and largest, over a row's lanes: LANES 32 (two rows in a wave) or 64, then over its waves.
 template <int LANES>
 __device__ __forceinline__ void reduce_row(float& sum, uint32_t& most, int waves, RowSlots& slots, int& turn)
 {
@@ -52,9 +52,18 @@ __device__ __forceinline__ void reduce_row(float& sum, uint32_t& most, int waves
 template <int LANES>
 __device__ __forceinline__ void reduce_row(float& sum, int waves, RowSlots& slots, int& turn)
 {
-    uint32_t none = 0;
-    reduce_row<LANES>(sum, none, waves, slots, turn);
+#pragma unroll
+    for (int d = LANES / 2; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
+    if (LANES == 32 || waves == 1) return;
+    if ((threadIdx.x & 63) == 0) slots.sum[turn & 1][threadIdx.x >> 6] = sum;
+    __syncthreads();
+    sum = 0.f;
+    for (int k = 0; k < waves; ++k) sum += slots.sum[turn & 1][k];
+    ++turn;
 }
+
+// (rows are counted in 31 bits; a division of 64 takes as long as a row's sums)
+__device__ __forceinline__ int64_t run_of(int64_t row, int64_t run) { return (uint32_t)row / (uint32_t)run; }
 
 // The factor of a norm: n = v up factor, r = unit.  `up` is 1 but where the squares of v pass fp32's range.
 struct Root {
@@ -82,7 +91,58 @@ __device__ __forceinline__ Root root_of_scaled(float squares, float up, int64_t 
     return {up, r * (1.f / up), r};
 }
 
-// One row per threadIdx.y: a row's blockDim.x threads hold ITEMS chunks of eight columns each.
+// A chunk as it lies in memory.  (An array of 16-bit elements takes a register for each of them.)  keep(): what is formed from it is
+// formed behind this, not ahead into registers of its own.
+template <typename T>
+struct Raw {
+    uint32_t words[kChunk * sizeof(T) / 4];
+    template <bool ONCE>
+    __device__ __forceinline__ void fetch(const void* row, int64_t c, int64_t cols)
+    {
+        T v[kChunk];
+        if (c + kChunk <= cols) {   // (either way into whole registers by itself)
+            fetch_whole<ONCE>((const T*)row + c, v);
+            __builtin_memcpy(words, v, sizeof words);
+            return;
+        }
+        fetch_chunk<ONCE>((const T*)row, c, cols, v);
+        __builtin_memcpy(words, v, sizeof words);
+        keep();
+    }
+    __device__ __forceinline__ void set(float v)
+    {
+        T one[kChunk];
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) one[j] = (T)v;
+        __builtin_memcpy(words, one, sizeof words);
+    }
+    __device__ __forceinline__ void fetch_or_ones(const void* row, int64_t c, int64_t cols)
+    {
+        if (row) fetch<false>(row, c, cols);
+        else set(1.f);
+    }
+    __device__ __forceinline__ void keep()
+    {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof words / 4); ++i) asm volatile("" : "+v"(words[i]));
+    }
+    __device__ __forceinline__ float operator[](int j) const
+    {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(words[j]);
+        else if constexpr (std::is_same_v<T, bf16>) return __uint_as_float(j & 1 ? words[j / 2] & 0xffff0000u : words[j / 2] << 16);
+        else return (float)__builtin_bit_cast(f16, (uint16_t)(words[j / 2] >> (16 * (j & 1))));
+    }
+};
+
+// fp32 numbers from here on.  (A multiply-add whose result goes into fp16 is one instruction with one rounding, where the compiler takes it.)
+__device__ __forceinline__ void rounded(float (&v)[kChunk])
+{
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) asm volatile("" : "+v"(v[j]));
+}
+
+// One row per threadIdx.y: a row's blockDim.x threads hold ITEMS chunks of eight columns each.  (Fused multiply-adds by name: the compiler's choice
+// is another in every instance, and totals are the same bits in all of them.)
 template <typename T, int ITEMS, int LANES, bool ONCE, bool EIGHT>
 __global__ __launch_bounds__(1024) void k_gated_norm(NormArgs a)
 {
@@ -98,7 +158,7 @@ __global__ __launch_bounds__(1024) void k_gated_norm(NormArgs a)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) squares += v[i][j] * v[i][j];
+            for (int j = 0; j < kChunk; ++j) squares = fmaf(v[i][j], v[i][j], squares);
         reduce_row<LANES>(squares, waves, slots, turn);
         if (__builtin_expect(in_range(squares, a.cols, a.eps), true)) return root_of(squares, a.cols, a.eps);
         uint32_t peak = 0;
@@ -114,48 +174,71 @@ __global__ __launch_bounds__(1024) void k_gated_norm(NormArgs a)
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) squares += v[i][j] * up * (v[i][j] * up);
+            for (int j = 0; j < kChunk; ++j) squares = fmaf(v[i][j] * up, v[i][j] * up, squares);
         reduce_row<LANES>(squares, waves, slots, turn);
         return root_of_scaled(squares, up, a.cols, a.eps);
     };
-    T raw[ITEMS][kChunk], also[ITEMS][kChunk];
+    Raw<T> raw[ITEMS], also[ITEMS];
     float v[ITEMS][kChunk];
+    const T* gate = a.gate ? (const T*)a.gate + run_of(row, a.run) * a.cols : nullptr;
+    // What belongs to the channels is asked for together with the row, where the registers are there for it, and not behind an exchange.
+    constexpr bool kAhead = sizeof(T) == 2 ? ITEMS <= 2 : ITEMS == 1;
+    struct Held {
+        Raw<T> post, gate, scale, weight;
+    };
+    Held held[kAhead ? ITEMS : 1];
+    const auto channels = [&](int i, const T* from, Raw<T> Held::*which, float (&f)[kChunk]) {
+        if constexpr (kAhead) {
+            (held[i].*which).keep();
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) f[j] = (held[i].*which)[j];
+        } else {
+            load_chunk(from, column(i), a.cols, 0.f, f);
+        }
+    };
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         if (column(i) < a.cols) {
-            fetch_chunk<ONCE>((const T*)a.x + row * a.x_stride, column(i), a.cols, raw[i]);
-            fetch_chunk<ONCE>((const T*)a.residual + row * a.residual_stride, column(i), a.cols, also[i]);
+            raw[i].template fetch<ONCE>((const T*)a.x + row * a.x_stride, column(i), a.cols);
+            also[i].template fetch<ONCE>((const T*)a.residual + row * a.residual_stride, column(i), a.cols);
+            if constexpr (kAhead) {
+                if (a.post) held[i].post.template fetch<false>(a.post, column(i), a.cols);
+                if (gate) held[i].gate.template fetch<false>(gate, column(i), a.cols);
+                if (a.scale) held[i].scale.template fetch<false>(a.scale, column(i), a.cols);
+                held[i].weight.template fetch<false>(a.weight, column(i), a.cols);
+            }
         } else {
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) raw[i][j] = also[i][j] = (T)0.f;
+            raw[i].set(0.f);
+            also[i].set(0.f);
         }
     }
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) v[i][j] = (float)raw[i][j];
+        for (int j = 0; j < kChunk; ++j) v[i][j] = raw[i][j];
     Root first = {1.f, 1.f, 1.f};
     if (a.post) first = root_of_row(v);
-    const T* gate = a.gate ? (const T*)a.gate + row / a.run * a.cols : nullptr;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
         if (column(i) < a.cols) {
             float f[kChunk];
             if (a.post) {
-                load_chunk((const T*)a.post, column(i), a.cols, 0.f, f);
+                channels(i, (const T*)a.post, &Held::post, f);
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) v[i][j] = v[i][j] * first.up * first.factor * f[j];
             }
             if (gate) {
-                load_chunk(gate, column(i), a.cols, 0.f, f);
+                channels(i, gate, &Held::gate, f);
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) v[i][j] *= f[j];
             }
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) f[j] = 1.f;
-            if (a.scale) load_chunk((const T*)a.scale, column(i), a.cols, 0.f, f);
+            if (a.scale) channels(i, (const T*)a.scale, &Held::scale, f);
+            also[i].keep();
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) v[i][j] += f[j] * (float)also[i][j];
+            for (int j = 0; j < kChunk; ++j) v[i][j] = fmaf(f[j], also[i][j], v[i][j]);
+            rounded(v[i]);
             store_chunk((T*)a.total + row * a.cols, column(i), a.cols, v[i], a.streamed);
         }
     const Root second = root_of_row(v);
@@ -168,7 +251,7 @@ __global__ __launch_bounds__(1024) void k_gated_norm(NormArgs a)
     for (int i = 0; i < ITEMS; ++i)
         if (column(i) < a.cols) {
             float w[kChunk];
-            load_chunk((const T*)a.weight, column(i), a.cols, 0.f, w);
+            channels(i, (const T*)a.weight, &Held::weight, w);
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
                 v[i][j] = v[i][j] * second.up * second.factor * w[j];
@@ -203,7 +286,7 @@ __device__ __forceinline__ void form_total(const NormArgs& a, int64_t row, int64
         for (int j = 0; j < kChunk; ++j) t[j] = t[j] * first.up * first.factor * f[j];
     }
     if (a.gate) {
-        load_chunk((const T*)a.gate + row / a.run * a.cols, c, a.cols, 0.f, f);
+        load_chunk((const T*)a.gate + run_of(row, a.run) * a.cols, c, a.cols, 0.f, f);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) t[j] *= f[j];
     }
@@ -213,7 +296,8 @@ __device__ __forceinline__ void form_total(const NormArgs& a, int64_t row, int64
     float r[kChunk];
     load_chunk((const T*)a.residual + row * a.residual_stride, c, a.cols, 0.f, r);
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) t[j] += f[j] * r[j];
+    for (int j = 0; j < kChunk; ++j) t[j] = fmaf(f[j], r[j], t[j]);
+    rounded(t);
 }
 
 // Rows that do not fit into a workgroup's registers: read again, out of L2, after each exchange.
@@ -230,7 +314,7 @@ __global__ __launch_bounds__(1024) void k_gated_norm_long(NormArgs a)
         for (int64_t c = begin; c < a.cols; c += step) {
             take(c);
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) squares += v[j] * v[j];
+            for (int j = 0; j < kChunk; ++j) squares = fmaf(v[j], v[j], squares);
         }
         reduce_row<64>(squares, waves, slots, turn);
         if (__builtin_expect(in_range(squares, a.cols, a.eps), true)) return root_of(squares, a.cols, a.eps);
@@ -248,7 +332,7 @@ __global__ __launch_bounds__(1024) void k_gated_norm_long(NormArgs a)
         for (int64_t c = begin; c < a.cols; c += step) {
             take(c);
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) squares += v[j] * up * (v[j] * up);
+            for (int j = 0; j < kChunk; ++j) squares = fmaf(v[j] * up, v[j] * up, squares);
         }
         reduce_row<64>(squares, waves, slots, turn);
         return root_of_scaled(squares, up, a.cols, a.eps);
@@ -358,8 +442,11 @@ __device__ __forceinline__ void load_or_ones(const void* p, int64_t c, int64_t c
     }
 }
 
+// The row and two of the channels' numbers are held as they lie in memory and formed anew on either side of an exchange; gate and post
+// come as their product only, and of their two sums over rows one is kept, sum dt n1 over a run, which post and the run's gate multiply where
+// the run ends.  That leaves two waves on a SIMD with two chunks a thread: 8192 x 4096 in workgroups of 256, two on a compute unit.
 template <typename T, int ITEMS, int LANES, bool ONCE>
-__global__ __launch_bounds__(512) void k_gated_back(BackArgs a)
+__global__ __launch_bounds__(512, 2) void k_gated_back(BackArgs a)
 {
     __shared__ RowSlots slots;
     const NormArgs& n = a.n;
@@ -368,23 +455,49 @@ __global__ __launch_bounds__(512) void k_gated_back(BackArgs a)
     const int64_t last = first + a.each < n.rows ? first + a.each : n.rows;
     if (unit >= a.units) return;
     const auto column = [&](int i) { return ((int64_t)i * threads + t) * kChunk; };
-    float weight[ITEMS][kChunk], post[ITEMS][kChunk], scale[ITEMS][kChunk], gate[ITEMS][kChunk];
-    float dweight[ITEMS][kChunk], dpost[ITEMS][kChunk], dscale[ITEMS][kChunk], dgate[ITEMS][kChunk];
-    int64_t run = n.gate ? first / n.run : 0, run_end = n.gate ? (run + 1) * n.run : n.rows;
-    const auto take_gate = [&](int i) {
-        load_or_ones<T>(n.gate ? (const T*)n.gate + run * n.cols : nullptr, column(i), n.cols, gate[i]);
+    Raw<T> weight[ITEMS], scale[ITEMS];
+    float branch[ITEMS][kChunk];   // gate post
+    float dweight[ITEMS][kChunk], dscale[ITEMS][kChunk], sum[ITEMS][kChunk];   // sum: of dt n1 over a run
+    int64_t run = n.gate ? run_of(first, n.run) : 0, run_end = n.gate ? (run + 1) * n.run : n.rows;
+    const auto gate_of_run = [&]() { return n.gate ? (const T*)n.gate + run * n.cols : nullptr; };
+    const auto begin_run = [&](int i) {
+        float gate[kChunk];
+        load_or_ones<T>(n.post, column(i), n.cols, branch[i]);
+        load_or_ones<T>(gate_of_run(), column(i), n.cols, gate);
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) dgate[i][j] = 0.f;
+        for (int j = 0; j < kChunk; ++j) {
+            branch[i][j] *= gate[j];
+            sum[i][j] = 0.f;
+        }
+    };
+    bool some = false;   // runs of this unit have ended
+    const auto end_run = [&](int i) {
+        float v[kChunk], d[kChunk];
+        if (a.dgate) {
+            load_or_ones<T>(n.post, column(i), n.cols, v);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) d[j] = sum[i][j] * v[j];
+            put_gate<T>(a, unit, first, last, run, column(i), d);
+        }
+        if (a.dpost) {
+            float* to = a.partial + (unit * kSums + kPost) * n.cols;
+            load_or_ones<T>(gate_of_run(), column(i), n.cols, v);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) d[j] = 0.f;
+            if (some) load_chunk(to, column(i), n.cols, 0.f, d);
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) d[j] += sum[i][j] * v[j];
+            store_chunk(to, column(i), n.cols, d);
+        }
     };
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) dweight[i][j] = dpost[i][j] = dscale[i][j] = 0.f;
+        for (int j = 0; j < kChunk; ++j) dweight[i][j] = dscale[i][j] = 0.f;
         if (column(i) < n.cols) {
-            load_chunk((const T*)n.weight, column(i), n.cols, 0.f, weight[i]);
-            load_or_ones<T>(n.post, column(i), n.cols, post[i]);
-            load_or_ones<T>(n.scale, column(i), n.cols, scale[i]);
-            take_gate(i);
+            weight[i].fetch_or_ones(n.weight, column(i), n.cols);
+            scale[i].fetch_or_ones(n.scale, column(i), n.cols);
+            begin_run(i);
         }
     }
     int turn = 0;
@@ -392,55 +505,56 @@ __global__ __launch_bounds__(512) void k_gated_back(BackArgs a)
         if (row == run_end) {
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
-                if (column(i) < n.cols) put_gate<T>(a, unit, first, last, run, column(i), dgate[i]);
+                if (column(i) < n.cols) end_run(i);
+            some = true;
             ++run;
             run_end += n.run;
 #pragma unroll
             for (int i = 0; i < ITEMS; ++i)
-                if (column(i) < n.cols) take_gate(i);
+                if (column(i) < n.cols) begin_run(i);
         }
         const float r1 = n.rstd[2 * row], r2 = n.rstd[2 * row + 1];
-        T residual[ITEMS][kChunk], also[ITEMS][kChunk];
-        float n1[ITEMS][kChunk], n2[ITEMS][kChunk], u[ITEMS][kChunk], along = 0.f;
+        Raw<T> x[ITEMS], residual[ITEMS], g[ITEMS], also[ITEMS];
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
             if (column(i) < n.cols) {
-                T x[kChunk], g[kChunk];
-                fetch_chunk<ONCE>((const T*)n.x + row * n.x_stride, column(i), n.cols, x);
-                fetch_chunk<ONCE>((const T*)n.residual + row * n.residual_stride, column(i), n.cols, residual[i]);
-                fetch_chunk<ONCE>((const T*)a.grad + row * a.grad_stride, column(i), n.cols, g);
-                if (a.grad_total) {
-                    fetch_chunk<ONCE>((const T*)a.grad_total + row * a.grad_total_stride, column(i), n.cols, also[i]);
-                } else {
+                x[i].template fetch<ONCE>((const T*)n.x + row * n.x_stride, column(i), n.cols);
+                residual[i].template fetch<ONCE>((const T*)n.residual + row * n.residual_stride, column(i), n.cols);
+                g[i].template fetch<ONCE>((const T*)a.grad + row * a.grad_stride, column(i), n.cols);
+                if (a.grad_total) also[i].template fetch<ONCE>((const T*)a.grad_total + row * a.grad_total_stride, column(i), n.cols);
+                else also[i].set(0.f);
+            }
+        const auto keep_all = [&](int i) { x[i].keep(), residual[i].keep(), g[i].keep(), also[i].keep(), weight[i].keep(), scale[i].keep(); };
+        const auto form_n2 = [&](int i, int j, float n1) { return (scale[i][j] * residual[i][j] + branch[i][j] * n1) * r2; };
+        float along = 0.f;
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) also[i][j] = (T)0.f;
-                }
+        for (int i = 0; i < ITEMS; ++i)
+            if (column(i) < n.cols) {
+                keep_all(i);
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
-                    n1[i][j] = (float)x[j] * r1;
-                    n2[i][j] = (scale[i][j] * (float)residual[i][j] + gate[i][j] * (n1[i][j] * post[i][j])) * r2;
-                    u[i][j] = (float)g[j] * weight[i][j];
-                    dweight[i][j] += (float)g[j] * n2[i][j];
-                    along += u[i][j] * n2[i][j];
+                    const float n2 = form_n2(i, j, x[i][j] * r1);
+                    dweight[i][j] += g[i][j] * n2;
+                    along += g[i][j] * weight[i][j] * n2;
                 }
             }
         reduce_row<LANES>(along, waves, slots, turn);
         const float back = along / (float)n.cols;
+        float s[ITEMS][kChunk];
         along = 0.f;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i)
             if (column(i) < n.cols) {
-                float dt[kChunk], d[kChunk];
+                float d[kChunk];
+                keep_all(i);
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) {
-                    dt[j] = r2 * (u[i][j] - n2[i][j] * back) + (float)also[i][j];
-                    d[j] = dt[j] * scale[i][j];
-                    dscale[i][j] += dt[j] * (float)residual[i][j];
-                    dgate[i][j] += dt[j] * (n1[i][j] * post[i][j]);
-                    const float e = dt[j] * gate[i][j];
-                    dpost[i][j] += e * n1[i][j];
-                    u[i][j] = e * post[i][j];
-                    along += u[i][j] * n1[i][j];
+                    const float n1 = x[i][j] * r1, dt = r2 * (g[i][j] * weight[i][j] - form_n2(i, j, n1) * back) + also[i][j];
+                    d[j] = dt * scale[i][j];
+                    dscale[i][j] += dt * residual[i][j];
+                    sum[i][j] += dt * n1;
+                    s[i][j] = dt * branch[i][j];
+                    along += s[i][j] * n1;
                 }
                 store_chunk((T*)a.dresidual + row * n.cols, column(i), n.cols, d, a.streamed);
             }
@@ -454,7 +568,7 @@ __global__ __launch_bounds__(512) void k_gated_back(BackArgs a)
             if (column(i) < n.cols) {
                 float d[kChunk];
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) d[j] = n.post ? r1 * (u[i][j] - n1[i][j] * through) : u[i][j];
+                for (int j = 0; j < kChunk; ++j) d[j] = n.post ? r1 * (s[i][j] - x[i][j] * r1 * through) : s[i][j];
                 store_chunk((T*)a.dx + row * n.cols, column(i), n.cols, d, a.streamed);
             }
     }
@@ -464,9 +578,8 @@ __global__ __launch_bounds__(512) void k_gated_back(BackArgs a)
         if (column(i) < n.cols) {
             float* to = a.partial + unit * kSums * n.cols;
             if (a.dweight) store_chunk(to + kWeight * n.cols, column(i), n.cols, dweight[i]);
-            if (a.dpost) store_chunk(to + kPost * n.cols, column(i), n.cols, dpost[i]);
             if (a.dscale) store_chunk(to + kScale * n.cols, column(i), n.cols, dscale[i]);
-            put_gate<T>(a, unit, first, last, run, column(i), dgate[i]);
+            end_run(i);
         }
 }
 
@@ -483,7 +596,7 @@ struct Terms {
         load_chunk((const T*)n.weight, c, n.cols, 0.f, weight);
         load_or_ones<T>(n.post, c, n.cols, post);
         load_or_ones<T>(n.scale, c, n.cols, scale);
-        load_or_ones<T>(n.gate ? (const T*)n.gate + row / n.run * n.cols : nullptr, c, n.cols, gate);
+        load_or_ones<T>(n.gate ? (const T*)n.gate + run_of(row, n.run) * n.cols : nullptr, c, n.cols, gate);
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) {
             n1[j] = x[j] * r1;
@@ -559,7 +672,7 @@ __global__ __launch_bounds__(256) void k_gated_back_columns(BackArgs a)
     const int64_t last = first + a.each < n.rows ? first + a.each : n.rows;
     if (c >= n.cols) return;
     float dweight[kChunk] = {}, dpost[kChunk] = {}, dscale[kChunk] = {}, dgate[kChunk] = {};
-    int64_t run = n.gate ? first / n.run : 0, run_end = n.gate ? (run + 1) * n.run : n.rows;
+    int64_t run = n.gate ? run_of(first, n.run) : 0, run_end = n.gate ? (run + 1) * n.run : n.rows;
     for (int64_t row = first; row < last; ++row) {
         if (row == run_end) {
             put_gate<T>(a, unit, first, last, run, c, dgate);
@@ -586,14 +699,13 @@ __global__ __launch_bounds__(256) void k_gated_back_columns(BackArgs a)
     put_gate<T>(a, unit, first, last, run, c, dgate);
 }
 
-// The sums over the units: 32 columns by 32 shares of the units in a workgroup.  blockIdx.y: dweight, dpost, dscale, then the runs that may
+// The sums over the units: COLS columns by SHARES shares of the units in a workgroup.  blockIdx.y: dweight, dpost, dscale, then the runs that may
 // be cut: all of them, or one for each border between units where those are fewer.
-constexpr int kJoinCols = 32, kJoinShares = 32;
-template <typename T>
-__global__ __launch_bounds__(kJoinCols * kJoinShares) void k_join(BackArgs a, bool by_border)
+template <typename T, int COLS, int SHARES>
+__global__ __launch_bounds__(COLS * SHARES) void k_join(BackArgs a, bool by_border)
 {
-    __shared__ float sums[kJoinShares][kJoinCols];
-    const int64_t cols = a.n.cols, c = (int64_t)blockIdx.x * kJoinCols + threadIdx.x;
+    __shared__ float sums[SHARES][COLS];
+    const int64_t cols = a.n.cols, c = (int64_t)blockIdx.x * COLS + threadIdx.x;
     float s = 0.f;
     T* to;
     if (blockIdx.y < kSums) {
@@ -601,7 +713,7 @@ __global__ __launch_bounds__(kJoinCols * kJoinShares) void k_join(BackArgs a, bo
         if (!to) return;
         if (c < cols) {
 #pragma unroll 16
-            for (int64_t u = threadIdx.y; u < a.units; u += kJoinShares) s += a.partial[(u * kSums + blockIdx.y) * cols + c];
+            for (int64_t u = threadIdx.y; u < a.units; u += SHARES) s += a.partial[(u * kSums + blockIdx.y) * cols + c];
         }
     } else {
         if (!a.dgate) return;
@@ -616,14 +728,14 @@ __global__ __launch_bounds__(kJoinCols * kJoinShares) void k_join(BackArgs a, bo
         if (from == to_unit) return;   // written by its unit
         to = (T*)a.dgate + run * cols;
         if (c < cols)
-            for (int64_t u = from + threadIdx.y; u <= to_unit; u += kJoinShares) s += gate_part(a, u, u * a.each / a.n.run == run ? 0 : 1)[c];
+            for (int64_t u = from + threadIdx.y; u <= to_unit; u += SHARES) s += gate_part(a, u, u * a.each / a.n.run == run ? 0 : 1)[c];
     }
     sums[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && c < cols) {
         s = 0.f;
-#pragma unroll
-        for (int k = 0; k < kJoinShares; ++k) s += sums[k][threadIdx.x];
+#pragma unroll 16
+        for (int k = 0; k < SHARES; ++k) s += sums[k][threadIdx.x];
         to[c] = (T)s;
     }
 }
@@ -631,12 +743,20 @@ __global__ __launch_bounds__(kJoinCols * kJoinShares) void k_join(BackArgs a, bo
 constexpr int kBackThreads = 512;
 constexpr int64_t kHeldBackCols = 2 * kBackThreads * kChunk;   // columns that a workgroup's registers hold in the backward
 
+// threads of a row: two chunks each where they are more than a wave has
+int back_threads(int64_t cols)
+{
+    const int64_t chunks = (cols + kChunk - 1) / kChunk;
+    return chunks <= 32 ? 32 : threads_of_row(chunks, chunks > 64 ? 2 : 1);
+}
+
+// Rows go to as many units as are on the GPU at once, eight waves of them on a compute unit.
 struct Units {
     int64_t count, each;
 };
 Units units_of(int64_t rows, int64_t cols)
 {
-    const int64_t most = cols > kHeldBackCols ? 64 : cols <= 64 * kChunk ? 2048 : 512;
+    const int64_t most = cols > kHeldBackCols ? 64 : (int64_t)256 * kBackThreads / back_threads(cols);
     const int64_t each = (rows + most - 1) / most;
     return {(rows + each - 1) / each, each};
 }
@@ -658,7 +778,7 @@ int run_back(BackArgs a, int dtype, hipStream_t s)
     } else {
         const bool once = reads_once(dtype, n.x, n.x_stride) && reads_once(dtype, n.residual, n.residual_stride) &&
                           reads_once(dtype, a.grad, a.grad_stride) && (!a.grad_total || reads_once(dtype, a.grad_total, a.grad_total_stride));
-        const int threads = chunks <= 32 ? 32 : chunks <= kBackThreads ? threads_of_row(chunks, 1) : kBackThreads;
+        const int threads = back_threads(n.cols);
         const int per_block = threads <= 64 ? 256 / threads : 1;
         const dim3 block(threads, per_block), grid((uint32_t)((a.units + per_block - 1) / per_block));
         const auto held = [&](auto count, auto lanes) {
@@ -673,8 +793,12 @@ int run_back(BackArgs a, int dtype, hipStream_t s)
     if (a.partial) {
         const int64_t runs = a.dgate ? n.rows / n.run : 0;
         const bool by_border = runs > a.units - 1;
-        k_join<T><<<dim3((uint32_t)((n.cols + kJoinCols - 1) / kJoinCols), (uint32_t)(kSums + (by_border ? a.units - 1 : runs))),
-                    dim3(kJoinCols, kJoinShares), 0, s>>>(a, by_border);
+        const auto join = [&](auto columns, auto shares) {
+            const dim3 grid((uint32_t)((n.cols + columns() - 1) / columns()), (uint32_t)(kSums + (by_border ? a.units - 1 : runs)));
+            k_join<T, columns(), shares()><<<grid, dim3(columns(), shares()), 0, s>>>(a, by_border);
+        };
+        if (n.cols <= 1024) join(std::integral_constant<int, 8>(), std::integral_constant<int, 128>());
+        else join(std::integral_constant<int, 32>(), std::integral_constant<int, 16>());
     }
     return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
 }

@@ -198,7 +198,11 @@ struct Epilogue {
 };
 bool slope_type_known(int dtype) { return dtype == GEO_SC_F32 || dtype == GEO_SC_F16; }
 
-// z becomes act(z), d its slope.  NaN stays; of the lowest floats on, z times a probability of zero is zero.
+// z becomes act(z), d its slope.  NaN stays NaN.
+// gelu: z P(z) with P(z) = 1 - Q(z) the normal distribution's share below z, its slope P + z p.  With x = |z| / sqrt 2 and u = 1 / (1 + 0.3275911 x),
+// 2 Q(|z|) = (a1 u + .. + a5 u^5) exp(-x^2) to 1.5e-7 (Abramowitz and Stegun 7.1.26), from the exponential that the density p takes anyway.
+// The hardware's exponential and reciprocal are within a unit each.  A wave of a large tile is alone on its SIMD and does 256
+// numbers a lane, four cycles an instruction (the transcendental ones sixteen).
 template <int N>
 __device__ __forceinline__ void activate(int kind, float (&z)[N], float (&d)[N])
 {
@@ -208,19 +212,22 @@ __device__ __forceinline__ void activate(int kind, float (&z)[N], float (&d)[N])
             d[j] = z[j] > 0.f ? 1.f : 0.f;
             z[j] = z[j] < 0.f ? 0.f : z[j];
         }
-    } else if (kind == GEO_SC_ACT_GELU) {   // z times the normal distribution's share below z
+    } else if (kind == GEO_SC_ACT_GELU) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const float below = 0.5f + 0.5f * erff(z[j] * 0.70710678f);
-            d[j] = below + z[j] * expf(-0.5f * z[j] * z[j]) * 0.39894228f;
+            const float u = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678f * fabsf(z[j]));
+            const float e = __builtin_amdgcn_exp2f(z[j] * z[j] * (-0.5f * 1.44269504f));
+            const float series = u * (0.254829592f + u * (-0.284496736f + u * (1.421413741f + u * (-1.453152027f + u * 1.061405429f))));
+            const float tail = 0.5f * series * e, below = z[j] < 0.f ? tail : 1.f - tail;
+            d[j] = below + z[j] * e * 0.39894228f;
             z[j] *= below;
         }
-    } else if (kind == GEO_SC_ACT_SILU) {   // z times its logistic function
+    } else if (kind == GEO_SC_ACT_SILU) {   // z times s = 1 / (1 + exp(-z)); slope s + z s (1 - s)
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            const float s = 1.f / (1.f + expf(-z[j]));
-            d[j] = s + z[j] * s * (1.f - s);
+            const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[j] * -1.44269504f));
             z[j] *= s;
+            d[j] = s + z[j] * (1.f - s);
         }
     } else {
 #pragma unroll
@@ -325,6 +332,10 @@ struct Tiling {
     static constexpr int kArea = 16 * T * 64;      // bytes of 16 rows of a wave's sums
 };
 
+// Quotients are computed in vector registers; of the whole wave's they say so here, or descriptors that are formed from them are taken for
+// the lanes' own, and every load goes through a loop over them.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
 // Where a workgroup works: its product's tile and split.
 struct Spot {
     TileArgs a;
@@ -342,14 +353,14 @@ __device__ __forceinline__ Spot spot_of(const TwoProducts& both, uint32_t work)
     const bool is_second = work >= both.second_at;
     p.a = is_second ? both.second : both.first;
     const uint32_t group = work - (is_second ? both.second_at : 0), all = (uint32_t)p.a.tiles_m * p.a.tiles_n;
-    p.split = group / all;
-    p.die = group % all & 7;
+    p.split = uniform(group / all);
+    p.die = uniform(group % all & 7);
     const uint32_t tile = p.die * (all / 8) + (p.die < all % 8 ? p.die : all % 8) + (group % all >> 3);
     constexpr uint32_t kStrip = 4;
-    const uint32_t strip = tile / (kStrip * p.a.tiles_n), inside = tile - strip * kStrip * p.a.tiles_n;
+    const uint32_t strip = uniform(tile / (kStrip * p.a.tiles_n)), inside = tile - strip * kStrip * p.a.tiles_n;
     const uint32_t height = p.a.tiles_m - strip * kStrip < kStrip ? p.a.tiles_m - strip * kStrip : kStrip;
-    p.m0 = (int64_t)(strip * kStrip + inside % height) * B;
-    p.n0 = (int64_t)(inside / height) * B;
+    p.m0 = (int64_t)(strip * kStrip + uniform(inside % height)) * B;
+    p.n0 = (int64_t)uniform(inside / height) * B;
     const int stages = (int)((p.a.inner + kStage - 1) / kStage), whole = (int)(p.a.inner / kStage);
     p.begin = p.split * p.a.stages_per_split;
     p.end = p.begin + p.a.stages_per_split < stages ? p.begin + p.a.stages_per_split : stages;
@@ -532,44 +543,120 @@ __device__ __forceinline__ void finish_tile(const Spot& p, typename Matrix<INT8>
     else finish((f16*)p.a.y, [&](auto one, int i, int j, int r) { return (f16)scaled(one, i, j, r); });
 }
 
-// The same through the epilogue: the sums as they are into LDS, ROWS of a wave's rows at a time, and out of it a lane eight columns of a row.
+// The same through the epilogue: the sums times their rows' scales into LDS, ROWS of a wave's rows at a time, and out of it a lane eight
+// columns of a row.  A wave of a large tile is alone on its SIMD, so nothing is waited for where it is used: the sums out of LDS and the
+// residual's rows are asked for kBatch rows at a time, a batch ahead.
 template <int B, int ROWS>
-__device__ __forceinline__ void finish_tile(const Spot& p, const Epilogue& e, v4i (&sum)[B / 32][B / 32], uint8_t* area, int wave, int lane)
-{
-    constexpr int T = B / 32, kCols = T * 16, kPieces = kCols / 4, kMix = (kPieces < 16 ? kPieces : 16) - 1;
-    constexpr int kLanes = kCols / kChunk, kAtOnce = 64 / kLanes;   // lanes of a row, rows at once
-    static_assert(ROWS % 16 == 0 && kCols % ROWS == 0 && ROWS % kAtOnce == 0, "");
-    const int64_t n = p.n0 + wave / 2 * kCols + lane % kLanes * kChunk;
-    float ws[kChunk] = {}, bias[kChunk];
-    if (n < p.a.cols) load_columns(p.a.w_scale + n, p.a.cols - n, ws);
-    load_bias(e, n, p.a.cols, bias);
+struct EpilogueTile {
+    static constexpr int T = B / 32, kCols = T * 16, kPieces = kCols / 4, kMix = (kPieces < 16 ? kPieces : 16) - 1;
+    static constexpr int kLanes = kCols / kChunk, kAtOnce = 64 / kLanes;   // lanes of a row, rows at once
+    static constexpr int kPasses = ROWS / kAtOnce, kBatch = B == 256 ? 4 : 2, kStep = kBatch * kAtOnce;
+    static_assert(ROWS % 16 == 0 && kCols % ROWS == 0 && kPasses % kBatch == 0, "");
+    const Epilogue& e;
+    float ws[kChunk], bias[kChunk], xs[T];
+
+    __device__ __forceinline__ int64_t column(const Spot& p, int wave, int lane) const { return p.n0 + wave / 2 * kCols + lane % kLanes * kChunk; }
+    // asks for the scales and the bias
+    __device__ __forceinline__ void ask(const Spot& p, int wave, int lane)
+    {
+        const int64_t n = column(p, wave, lane);
 #pragma unroll
-    for (int first = 0; first < kCols; first += ROWS) {
+        for (int j = 0; j < kChunk; ++j) ws[j] = 0.f;
+        if (n < p.a.cols) load_columns(p.a.w_scale + n, p.a.cols - n, ws);
+        load_bias(e, n, p.a.cols, bias);
 #pragma unroll
-        for (int i = 0; i < ROWS / 16; ++i)
-#pragma unroll
-            for (int j = 0; j < T; ++j) {
-                const int row = i * 16 + (lane & 15), piece = j * 4 + (lane >> 4);
-                *(v4i*)(area + (row * kPieces + (piece ^ (row & kMix))) * 16) = sum[j][first / 16 + i];
-            }
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-        for (int r = lane / kLanes; r < ROWS; r += kAtOnce) {
-            const int64_t m = p.m0 + wave % 2 * kCols + first + r;
-            if (m >= p.a.rows || n >= p.a.cols) continue;
-            const float xs = p.a.x_scale[m];
-            float z[kChunk];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const v4i s = *(const v4i*)(area + (r * kPieces + ((lane % kLanes * 2 + h) ^ (r & kMix))) * 16);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) z[h * 4 + j] = (float)s[j] * xs * ws[h * 4 + j] + bias[h * 4 + j];
-            }
-            finish_columns(p.a, e, m, n, z);
+        for (int i = 0; i < T; ++i) {
+            const int64_t m = p.m0 + wave % 2 * kCols + i * 16 + (lane & 15);
+            xs[i] = p.a.x_scale[m < p.a.rows ? m : p.a.rows - 1];
         }
-        __builtin_amdgcn_wave_barrier();
     }
-}
+    // WHOLE: the tile lies inside the product
+    template <typename Y, bool WHOLE>
+    __device__ __forceinline__ void rows(const Spot& p, v4i (&sum)[T][T], uint8_t* area, int wave, int lane) const
+    {
+        const int64_t cols = p.a.cols, n = column(p, wave, lane), left = cols - n, m0 = p.m0 + wave % 2 * kCols + lane / kLanes;
+        const int mine = lane / kLanes, piece = lane % kLanes * 2;
+        const auto ask_residual = [&](Y (&raw)[kBatch][kChunk], int r) {
+            if (!e.residual || (!WHOLE && left <= 0)) return;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int64_t m = m0 + r + i * kAtOnce;
+                const Y* row = (const Y*)e.residual + (m < p.a.rows ? m : p.a.rows - 1) * e.residual_stride;   // (behind the last row that row once more)
+                if constexpr (WHOLE) fetch_whole<false>(row + n, raw[i]);
+                else fetch_chunk<false>(row, n, cols, raw[i]);
+            }
+        };
+        const auto ask_sums = [&](float (&v)[kBatch][kChunk], int r) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int row = (r + i * kAtOnce + mine) % ROWS;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) __builtin_memcpy(v[i] + 4 * h, area + (row * kPieces + ((piece + h) ^ (row & kMix))) * 16, 16);
+            }
+        };
+        Y residual_ahead[kBatch][kChunk] = {};
+        float sums_ahead[kBatch][kChunk];
+        ask_residual(residual_ahead, 0);
+        int64_t at = m0 * cols + n;
+#pragma unroll
+        for (int first = 0; first < kCols; first += ROWS) {
+#pragma unroll
+            for (int i = 0; i < ROWS / 16; ++i)
+#pragma unroll
+                for (int j = 0; j < T; ++j) {
+                    const int row = i * 16 + (lane & 15), to = j * 4 + (lane >> 4);
+                    v4i s = sum[j][first / 16 + i];
+                    asm volatile("" : "+v"(s));   // (out of its accumulation registers here)
+                    float v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs[first / 16 + i];
+                    __builtin_memcpy(area + (row * kPieces + (to ^ (row & kMix))) * 16, v, 16);
+                }
+            __builtin_amdgcn_wave_barrier();
+            ask_sums(sums_ahead, 0);
+#pragma unroll 1
+            for (int r = 0; r < ROWS; r += kStep) {
+                Y residual[kBatch][kChunk];
+                float z[kBatch][kChunk];
+                __builtin_memcpy(residual, residual_ahead, sizeof residual);
+                __builtin_memcpy(z, sums_ahead, sizeof z);
+                ask_sums(sums_ahead, r + kStep);   // (behind the last ones the first once more)
+                ask_residual(residual_ahead, first + r + kStep);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i, at += kAtOnce * cols) {
+                    float d[kChunk];
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) z[i][j] = z[i][j] * ws[j] + bias[j];
+                    activate(e.activation, z[i], d);
+                    if (!WHOLE && (m0 + first + r + i * kAtOnce >= p.a.rows || left <= 0)) continue;
+                    const int64_t there = WHOLE ? kChunk : left;
+                    if (e.slope) {
+                        if (e.slope_dtype == GEO_SC_F32) store_columns((f32*)e.slope + at, there, d);
+                        else store_columns((f16*)e.slope + at, there, d);
+                    }
+                    if (e.residual) {
+#pragma unroll
+                        for (int j = 0; j < kChunk; ++j) z[i][j] += (float)residual[i][j];
+                    }
+                    store_columns((Y*)p.a.y + at, there, z[i]);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+    }
+    template <typename Y>
+    __device__ __forceinline__ void rows(const Spot& p, v4i (&sum)[T][T], uint8_t* area, int wave, int lane) const
+    {
+        if (inside<B>(p)) rows<Y, true>(p, sum, area, wave, lane);
+        else rows<Y, false>(p, sum, area, wave, lane);
+    }
+    __device__ __forceinline__ void finish(const Spot& p, v4i (&sum)[T][T], uint8_t* area, int wave, int lane) const
+    {
+        if (p.a.dtype == GEO_SC_F32) rows<f32>(p, sum, area, wave, lane);
+        else if (p.a.dtype == GEO_SC_BF16) rows<bf16>(p, sum, area, wave, lane);
+        else rows<f16>(p, sum, area, wave, lane);
+    }
+};
 
 // Rows that start at multiples of 16 bytes, and four whole stages of every split.  The loads write LDS themselves, into a ring of
 // kRing stages: while a wave multiplies stage s out of registers, stage s + 1 moves from LDS to its other registers and the stages
@@ -719,18 +806,18 @@ __global__ __launch_bounds__(kWaves * 64) void k_tiles(TwoProducts both)
 }
 // (the ring takes the sums on their way out: 128 KB of LDS for the largest tile)
 template <int B>
-__global__ __launch_bounds__(kWaves * 64) void k_tiles_epilogue(TwoProducts both, Epilogue e)
+__global__ __launch_bounds__(kWaves * 64, 256 / B) void k_tiles_epilogue(TwoProducts both, Epilogue e)
 {
     struct Finish {
-        const Epilogue& e;
-        __device__ __forceinline__ void ask(const Spot&, int, int) {}
+        EpilogueTile<B, B / 2 < 64 ? B / 2 : 64> tile;
+        __device__ __forceinline__ void ask(const Spot& p, int wave, int lane) { tile.ask(p, wave, lane); }
         __device__ __forceinline__ void operator()(const Spot& p, v4i (&sum)[B / 32][B / 32], uint8_t* place, int wave, int lane)
         {
             __syncthreads();   // all have read the last stage
-            finish_tile<B, B / 2 < 64 ? B / 2 : 64>(p, e, sum, place, wave, lane);
+            tile.finish(p, sum, place, wave, lane);
         }
     };
-    tiles_body<B, true>(both, Finish{e});
+    tiles_body<B, true>(both, Finish{{e}});
 }
 
 // Fewer stages than the ring of k_tiles holds, at any alignment: stages through registers, the next one on its way while one is
@@ -763,7 +850,9 @@ __global__ __launch_bounds__(kWaves * 64) void k_tiles_any(TwoProducts both, Epi
         __syncthreads();
     }
     if constexpr (EPILOGUE) {
-        finish_tile<B, 32>(p, e, sum, areas[wave], wave, lane);
+        EpilogueTile<B, 32> tile = {e};
+        tile.ask(p, wave, lane);
+        tile.finish(p, sum, areas[wave], wave, lane);
     } else {
         TileScales<T> scales;
         scales.load(p, wave, lane);
