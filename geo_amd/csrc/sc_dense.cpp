@@ -402,11 +402,11 @@ at::Tensor matmul_q8(const at::Tensor& q, const at::Tensor& scale, const at::Ten
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
     const at::Tensor y = at::empty(sizes, q.options().dtype(type));
     if (after.keep_slope) {
-        // fp16 holds a relu's slope exactly, and any to an eighth of what bf16 rounds by; beside fp16's own rounding it would show
-        // (gradients of 4000 x 500 fp16 1.5 times as far off)
-        const bool half = type == at::kBFloat16 || after.activation == GEO_SC_ACT_RELU;
-        after.slope = at::empty({x.r.rows, w.r.rows}, q.options().dtype(half ? at::kHalf : at::kFloat));
-        e.slope_dtype = half ? GEO_SC_F16 : GEO_SC_F32;
+        // a relu's slope is 0 or 1; others in fp16 are off by an eighth of what bf16 rounds by, and beside fp16's own rounding that would
+        // show (gradients of 4000 x 500 fp16 1.5 times as far off)
+        const at::ScalarType kept = after.activation == GEO_SC_ACT_RELU ? at::kByte : type == at::kBFloat16 ? at::kHalf : at::kFloat;
+        after.slope = at::empty({x.r.rows, w.r.rows}, q.options().dtype(kept));
+        e.slope_dtype = kept == at::kByte ? GEO_SC_U8 : dtype_of(kept, "slope");
     }
     if (y.numel() == 0) return y;
     if (after.residual) {
@@ -476,7 +476,7 @@ ProductGradients matmul_q8_backward(const at::Tensor& grad, const at::Tensor& q,
                  "workspace query");
     const at::Tensor workspace = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
     check_status(geo_sc_matmul_q8_epilogue_backward(g.t.const_data_ptr(), grad_type, g.stride, slope.defined() ? slope.const_data_ptr() : nullptr,
-                                                    slope.defined() && slope.scalar_type() == at::kHalf ? GEO_SC_F16 : GEO_SC_F32,
+                                                    !slope.defined() ? 0 : slope.scalar_type() == at::kByte ? GEO_SC_U8 : dtype_of(slope.scalar_type(), "slope"),
                                                     x.r.t.const_data_ptr<int8_t>(), x.r.stride, x.scale.const_data_ptr<float>(),
                                                     w.r.t.const_data_ptr<int8_t>(), w.r.stride, w.scale.const_data_ptr<float>(), g.rows, g.cols,
                                                     x.r.cols, data_of(dx), dx ? dtype_of(*dx_type, "dx") : 0, data_of(dw),

@@ -38,6 +38,7 @@ struct TileArgs {
     int w_stages;                      // w's inner dimension repeats after this many stages (terms of the gradient)
     const float *x_scale, *w_scale;    // NULL: 1
     void* y;
+    int64_t y_stride;                  // elements
     int dtype;
     int stages_per_split;
     int splits;
@@ -179,7 +180,7 @@ __device__ __forceinline__ void finish_four(const TileArgs& a, int split, int64_
     float v[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs * ws[r];
-    store_four(a.y, a.dtype, m * a.cols + n, left, v);
+    store_four(a.y, a.dtype, m * a.y_stride + n, left, v);
 }
 
 __device__ __forceinline__ float scale_at(const float* scale, int64_t i, int64_t count) { return scale && i < count ? scale[i] : 1.f; }
@@ -196,7 +197,7 @@ struct Epilogue {
     int64_t residual_stride;
     int bias_dtype, slope_dtype, activation;
 };
-bool slope_type_known(int dtype) { return dtype == GEO_SC_F32 || dtype == GEO_SC_F16; }
+bool slope_type_known(int dtype) { return dtype == GEO_SC_F32 || dtype == GEO_SC_F16 || dtype == GEO_SC_U8; }
 
 // z becomes act(z), d its slope.  NaN stays NaN.
 // gelu: z P(z) with P(z) = 1 - Q(z) the normal distribution's share below z, its slope P + z p.  With x = |z| / sqrt 2 and u = 1 / (1 + 0.3275911 x),
@@ -284,6 +285,13 @@ __device__ __forceinline__ void load_bias(const Epilogue& e, int64_t n, int64_t 
     for (int j = 0; j < N; ++j) v[j] = 0.f;
     if (e.bias && n < cols) load_columns(e.bias, e.bias_dtype, n, cols - n, v);
 }
+template <int N>
+__device__ __forceinline__ void store_slope(const Epilogue& e, int64_t at, int64_t left, const float (&d)[N])
+{
+    if (e.slope_dtype == GEO_SC_F32) store_columns((f32*)e.slope + at, left, d);
+    else if (e.slope_dtype == GEO_SC_F16) store_columns((f16*)e.slope + at, left, d);
+    else store_columns((uint8_t*)e.slope + at, left, d);
+}
 // N columns from n on of row m: their sums scaled and the bias added come in as z
 template <int N>
 __device__ __forceinline__ void finish_columns(const TileArgs& a, const Epilogue& e, int64_t m, int64_t n, float (&z)[N])
@@ -292,16 +300,13 @@ __device__ __forceinline__ void finish_columns(const TileArgs& a, const Epilogue
     if (m >= a.rows || left <= 0) return;
     float d[N];
     activate(e.activation, z, d);
-    if (e.slope) {
-        if (e.slope_dtype == GEO_SC_F32) store_columns((f32*)e.slope + m * a.cols + n, left, d);
-        else store_columns((f16*)e.slope + m * a.cols + n, left, d);
-    }
+    if (e.slope) store_slope(e, m * a.y_stride + n, left, d);
     if (e.residual) {
         load_columns(e.residual, a.dtype, m * e.residual_stride + n, left, d);
 #pragma unroll
         for (int j = 0; j < N; ++j) z[j] += d[j];
     }
-    store_columns(a.y, a.dtype, m * a.cols + n, left, z);
+    store_columns(a.y, a.dtype, m * a.y_stride + n, left, z);
 }
 // the same from four sums and their scales
 __device__ __forceinline__ void finish_four(const TileArgs& a, const Epilogue& e, int64_t m, int64_t n, const v4i& s, float xs, const float (&ws)[4])
@@ -486,7 +491,7 @@ __device__ __forceinline__ void finish_tile(const Spot& p, typename Matrix<INT8>
 {
     constexpr int T = B / 32;
     const bool fits = inside<B>(p);
-    const auto finish = [&](auto* y, auto value) {
+    const auto finish = [&](auto* y, int64_t stride, auto value) {
         using Y = std::remove_pointer_t<decltype(y)>;
         constexpr int kEach = 16 / (int)sizeof(Y), kPieces = T * 16 / kEach, kAtOnce = 64 / kPieces;   // elements, pieces of a row, rows of a store
         constexpr int kMix = (kPieces < 16 ? kPieces : 16) - 1, kBatch = 4 / (int)sizeof(Y);           // squares of rows that the area holds
@@ -516,7 +521,7 @@ __device__ __forceinline__ void finish_tile(const Spot& p, typename Matrix<INT8>
             if (fits) {
 #pragma unroll
                 for (int h = 0; h < 16 * kBatch / kAtOnce; ++h)
-                    __builtin_memcpy(y + (m1 + h * kAtOnce + lane / kPieces) * p.a.cols + n, &u[h], 16);
+                    __builtin_memcpy(y + (m1 + h * kAtOnce + lane / kPieces) * stride + n, &u[h], 16);
             } else {
 #pragma unroll
                 for (int h = 0; h < 16 * kBatch / kAtOnce; ++h) {
@@ -524,11 +529,11 @@ __device__ __forceinline__ void finish_tile(const Spot& p, typename Matrix<INT8>
                     Y raw[kEach];
                     __builtin_memcpy(raw, &u[h], 16);
                     if (m < p.a.rows && n + kEach <= p.a.cols) {
-                        __builtin_memcpy(y + m * p.a.cols + n, raw, 16);
+                        __builtin_memcpy(y + m * stride + n, raw, 16);
                     } else if (m < p.a.rows) {
 #pragma unroll
                         for (int t = 0; t < kEach; ++t)
-                            if (n + t < p.a.cols) y[m * p.a.cols + n + t] = raw[t];
+                            if (n + t < p.a.cols) y[m * stride + n + t] = raw[t];
                     }
                 }
             }
@@ -537,10 +542,10 @@ __device__ __forceinline__ void finish_tile(const Spot& p, typename Matrix<INT8>
     };
     const auto scaled = [&](auto one, int i, int j, int r) { return (float)one * scales.x[i] * scales.w[j][r]; };
     if (p.a.partial)
-        finish(p.a.partial + (int64_t)p.split * p.a.rows * p.a.cols, [&](auto one, int, int, int) { return __builtin_bit_cast(uint32_t, one); });
-    else if (p.a.dtype == GEO_SC_F32) finish((f32*)p.a.y, scaled);
-    else if (p.a.dtype == GEO_SC_BF16) finish((bf16*)p.a.y, [&](auto one, int i, int j, int r) { return (bf16)scaled(one, i, j, r); });
-    else finish((f16*)p.a.y, [&](auto one, int i, int j, int r) { return (f16)scaled(one, i, j, r); });
+        finish(p.a.partial + (int64_t)p.split * p.a.rows * p.a.cols, p.a.cols, [&](auto one, int, int, int) { return __builtin_bit_cast(uint32_t, one); });
+    else if (p.a.dtype == GEO_SC_F32) finish((f32*)p.a.y, p.a.y_stride, scaled);
+    else if (p.a.dtype == GEO_SC_BF16) finish((bf16*)p.a.y, p.a.y_stride, [&](auto one, int i, int j, int r) { return (bf16)scaled(one, i, j, r); });
+    else finish((f16*)p.a.y, p.a.y_stride, [&](auto one, int i, int j, int r) { return (f16)scaled(one, i, j, r); });
 }
 
 // The same through the epilogue: the sums times their rows' scales into LDS, ROWS of a wave's rows at a time, and out of it a lane eight
@@ -574,7 +579,7 @@ struct EpilogueTile {
     template <typename Y, bool WHOLE>
     __device__ __forceinline__ void rows(const Spot& p, v4i (&sum)[T][T], uint8_t* area, int wave, int lane) const
     {
-        const int64_t cols = p.a.cols, n = column(p, wave, lane), left = cols - n, m0 = p.m0 + wave % 2 * kCols + lane / kLanes;
+        const int64_t cols = p.a.cols, stride = p.a.y_stride, n = column(p, wave, lane), left = cols - n, m0 = p.m0 + wave % 2 * kCols + lane / kLanes;
         const int mine = lane / kLanes, piece = lane % kLanes * 2;
         const auto ask_residual = [&](Y (&raw)[kBatch][kChunk], int r) {
             if (!e.residual || (!WHOLE && left <= 0)) return;
@@ -597,7 +602,7 @@ struct EpilogueTile {
         Y residual_ahead[kBatch][kChunk] = {};
         float sums_ahead[kBatch][kChunk];
         ask_residual(residual_ahead, 0);
-        int64_t at = m0 * cols + n;
+        int64_t at = m0 * stride + n;
 #pragma unroll
         for (int first = 0; first < kCols; first += ROWS) {
 #pragma unroll
@@ -623,17 +628,14 @@ struct EpilogueTile {
                 ask_sums(sums_ahead, r + kStep);   // (behind the last ones the first once more)
                 ask_residual(residual_ahead, first + r + kStep);
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i, at += kAtOnce * cols) {
+                for (int i = 0; i < kBatch; ++i, at += kAtOnce * stride) {
                     float d[kChunk];
 #pragma unroll
                     for (int j = 0; j < kChunk; ++j) z[i][j] = z[i][j] * ws[j] + bias[j];
                     activate(e.activation, z[i], d);
                     if (!WHOLE && (m0 + first + r + i * kAtOnce >= p.a.rows || left <= 0)) continue;
                     const int64_t there = WHOLE ? kChunk : left;
-                    if (e.slope) {
-                        if (e.slope_dtype == GEO_SC_F32) store_columns((f32*)e.slope + at, there, d);
-                        else store_columns((f16*)e.slope + at, there, d);
-                    }
+                    if (e.slope) store_slope(e, at, there, d);
                     if (e.residual) {
 #pragma unroll
                         for (int j = 0; j < kChunk; ++j) z[i][j] += (float)residual[i][j];
@@ -1131,7 +1133,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_streamed(TileArgs a, Epi
                 for (int r = 0; r < 4; ++r) held[r] = v[r];
                 held_n = n;
             } else {
-                if (m < a.rows && n < a.cols) store_four(a.y, a.dtype, m * a.cols + n, a.cols - n, v);
+                if (m < a.rows && n < a.cols) store_four(a.y, a.dtype, m * a.y_stride + n, a.cols - n, v);
             }
         }
         holds = EPILOGUE;
@@ -1205,7 +1207,7 @@ __global__ __launch_bounds__(256) void k_join_splits(TwoProducts both, Epilogue 
     float v[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs * scale_at(a.w_scale, n + r, a.cols);
-    store_four(a.y, a.dtype, m * a.cols + n, left, v);
+    store_four(a.y, a.dtype, m * a.y_stride + n, left, v);
 }
 
 // ---------------------------------------------------------------- which kernel, and how the inner dimension is cut
@@ -1373,6 +1375,54 @@ bool run_tiles(TwoProducts both, const Epilogue* e, bool direct, hipStream_t s)
     return true;
 }
 
+// The rows and columns of a product that its last tiles are for, if they are no more than 64 in a direction, as products of their own
+// in tiles of 64: 4096 x 4099 takes 272 tiles of 256, a second round of the compute units for 48 rows of w's.
+constexpr int64_t kMostStrip = 64;
+struct Strips {
+    TileArgs main, down, right;   // all but the last rows and columns; the last rows; the last columns of the others (rows 0: none)
+    Epilogue down_epilogue, right_epilogue;
+};
+Strips cut_strips(const TileArgs& a, int tile, const Epilogue* e)
+{
+    Strips s = {};
+    s.main = a;
+    const int64_t last_rows = a.rows % tile, last_cols = a.cols % tile;
+    const bool down = last_rows && last_rows <= kMostStrip && a.rows > tile, right = last_cols && last_cols <= kMostStrip && a.cols > tile;
+    const int y_bytes = dtype_bytes(a.dtype);
+    const auto shift = [&](TileArgs& t, Epilogue& f, int64_t row, int64_t col) {
+        const int64_t at = row * a.y_stride + col;
+        t.x += row * a.x_stride;
+        t.w += col * a.w_stride;
+        if (t.x_scale) t.x_scale += row;
+        if (t.w_scale) t.w_scale += col;
+        t.y = (char*)t.y + at * y_bytes;
+        if (!e) return;
+        f = *e;
+        if (f.bias) f.bias = (const char*)f.bias + col * dtype_bytes(f.bias_dtype);
+        if (f.residual) f.residual = (const char*)f.residual + (row * f.residual_stride + col) * y_bytes;
+        if (f.slope) f.slope = (char*)f.slope + at * (f.slope_dtype == GEO_SC_F32 ? 4 : f.slope_dtype == GEO_SC_F16 ? 2 : 1);
+    };
+    if (down) {
+        s.main.rows -= last_rows;
+        s.down = a;
+        s.down.rows = last_rows;
+        shift(s.down, s.down_epilogue, s.main.rows, 0);
+    }
+    if (right) {
+        s.main.cols -= last_cols;
+        s.right = s.main;
+        s.right.cols = last_cols;
+        shift(s.right, s.right_epilogue, 0, s.main.cols);
+    }
+    return s;
+}
+int64_t rounds_of(const TileArgs& a, const TileArgs& b, int tile)
+{
+    const auto tiles = [&](const TileArgs& t) { return ((t.rows + tile - 1) / tile) * ((t.cols + tile - 1) / tile); };
+    const int64_t at_once = kUnits * (tile == 256 ? 1 : 2);
+    return (tiles(a) + (b.rows ? tiles(b) : 0) + at_once - 1) / at_once;
+}
+
 // Runs one product, or two in one launch (second.rows 0: one).  The caller has made the plan and the partial sums' memory.
 // `e`: the epilogue of the one product, or NULL; where the inner dimension is cut, the join has it.
 template <bool INT8>
@@ -1390,6 +1440,21 @@ int run_products(TwoProducts both, const Epilogue* e, const Plan& p, hipStream_t
         else run_few<4>(both.first, now, s);
     } else {
         const bool direct = is_direct(both.first, p.tile) && (!both.second.rows || is_direct(both.second, p.tile));
+        if (direct && p.tile > 64 && p.splits[0] == 1 && (!both.second.rows || p.splits[1] == 1)) {
+            const Strips first = cut_strips(both.first, p.tile, now), second = cut_strips(both.second, p.tile, nullptr);
+            if (rounds_of(first.main, second.main, p.tile) < rounds_of(both.first, both.second, p.tile)) {
+                const auto strip = [&](const TileArgs& a, const Epilogue& e) {
+                    TwoProducts one = {};
+                    one.first = a;
+                    return !a.rows || run_tiles<64, INT8>(one, now ? &e : nullptr, true, s);
+                };
+                if (!strip(first.down, first.down_epilogue) || !strip(first.right, first.right_epilogue) || !strip(second.down, {}) ||
+                    !strip(second.right, {}))
+                    return GEO_SC_ERR_UNSUPPORTED;
+                both.first = first.main;
+                both.second = second.main;
+            }
+        }
         const bool fits = p.tile == 256   ? run_tiles<256, INT8>(both, now, direct, s)
                           : p.tile == 128 ? run_tiles<128, INT8>(both, now, direct, s)
                                           : run_tiles<64, INT8>(both, now, direct, s);
@@ -1511,7 +1576,7 @@ __global__ __launch_bounds__(kPeakWaves * 64) void k_grad_peaks(OperandArgs a)
                     const S* row = (const S*)a.slope + (r + i < r1 ? r + i : r1 - 1) * a.cols;
                     if constexpr (NARROW) {
 #pragma unroll
-                        for (int j = 0; j < kChunk; ++j) slope[i][j] = c + j < a.cols ? row[c + j] : (S)0.f;
+                        for (int j = 0; j < kChunk; ++j) slope[i][j] = c + j < a.cols ? row[c + j] : (S)0;
                     } else {
                         __builtin_memcpy(slope[i], row + c, sizeof slope[i]);
                     }
@@ -1634,7 +1699,8 @@ __global__ __launch_bounds__(256) void k_grad_operands(OperandArgs a)
             load_chunk(a.g, a.dtype, (r0 + r) * a.g_stride, c0 + c, a.cols, 0.f, v[i]);
             if (a.slope) {
                 float slope[kChunk];
-                load_chunk(a.slope, a.slope_dtype, (r0 + r) * a.cols, c0 + c, a.cols, 0.f, slope);
+                if (a.slope_dtype == GEO_SC_U8) load_columns((const uint8_t*)a.slope + (r0 + r) * a.cols + c0 + c, a.cols - c0 - c, slope);
+                else load_chunk(a.slope, a.slope_dtype, (r0 + r) * a.cols, c0 + c, a.cols, 0.f, slope);
 #pragma unroll
                 for (int j = 0; j < kChunk; ++j) v[i][j] = through_slope(v[i][j], slope[j]);
             }
@@ -1653,6 +1719,7 @@ __global__ __launch_bounds__(256) void k_grad_operands(OperandArgs a)
     if (a.dx_left && r0 + lane < a.rows)
         for (uint32_t k = wave; k < a.col_blocks; k += 4) row_most = max(row_most, a.row_peaks[k * a.rows + r0 + lane]);
     if (a.dw_left && c0 + lane < a.cols)
+#pragma unroll 8
         for (uint32_t k = wave; k < a.row_blocks; k += 4) col_most = max(col_most, a.col_peaks[k * a.cols + c0 + lane]);
     most[0][wave][lane] = row_most;
     most[1][wave][lane] = col_most;
@@ -1704,10 +1771,10 @@ __global__ __launch_bounds__(256) void k_grad_operands(OperandArgs a)
 
 int terms_of(int grad_dtype) { return grad_dtype == GEO_SC_BF16 ? 1 : 2; }
 int64_t padded_to_side(int64_t n) { return (n + kSide - 1) / kSide * kSide; }   // whole stages of fp16 elements
-// rows or columns of a block of which one maximum is taken: some 32 blocks where that leaves each `least` at least
-int64_t peak_block(int64_t n, int64_t least, int64_t most)
+// rows or columns of a block of which one maximum is taken: some `count` blocks where that leaves each `least` at least
+int64_t peak_block(int64_t n, int64_t count, int64_t least, int64_t most)
 {
-    const int64_t block = ((n + 31) / 32 + least - 1) / least * least;
+    const int64_t block = ((n + count - 1) / count + least - 1) / least * least;
     return block < most ? block : most;
 }
 
@@ -1727,8 +1794,10 @@ GradLayout grad_layout(int64_t rows, int64_t cols, int64_t inner, int terms, boo
         at += align256(bytes);
         return here;
     };
-    l.peak_rows = peak_block(rows, 32, kMostPeakRows);
-    l.peak_cols = peak_block(cols, kPeakWide, (int64_t)1 << 40);
+    l.peak_cols = peak_block(cols, 32, kPeakWide, (int64_t)1 << 40);
+    // (a workgroup for each compute unit, but no more than 128 maxima of a column to join: 16384 x 1024 in 64 blocks 32 us)
+    const int64_t across = (cols + l.peak_cols - 1) / l.peak_cols;
+    l.peak_rows = peak_block(rows, across >= 8 ? 32 : across >= 2 ? 256 / across : 128, 32, kMostPeakRows);
     if (need_dx) {
         const int64_t p = padded_to_side(cols);
         l.row_peaks = take((size_t)((cols + l.peak_cols - 1) / l.peak_cols) * rows * 4);
@@ -1804,6 +1873,7 @@ int forward(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_
     a.x_scale = x_scale;
     a.w_scale = w_scale;
     a.y = y;
+    a.y_stride = cols;
     a.dtype = dtype;
     a.partial = partial ? (uint32_t*)workspace : nullptr;
     return run_products<true>(both, e, plan, stream);
@@ -1878,6 +1948,7 @@ int backward(const void* grad, int grad_dtype, int64_t grad_stride, const void* 
         if (!slope && !dbias) peaks_of(one, no, no, one);
         else if (!slope) peaks_of(one, yes, no, one);
         else if (slope_type == GEO_SC_F32) peaks_of(one, yes, yes, f32());
+        else if (slope_type == GEO_SC_U8) peaks_of(one, yes, yes, uint8_t());
         else peaks_of(one, yes, yes, f16());
     };
     if (grad_dtype == GEO_SC_F32) peaks(f32());
@@ -1899,6 +1970,7 @@ int backward(const void* grad, int grad_dtype, int64_t grad_stride, const void* 
         a.w_stages = (int)(a.w_stride / kStage);
         a.x_scale = (const float*)(base + back);
         a.y = y;
+        a.y_stride = shape.cols;
         a.dtype = dtype;
         a.partial = cut ? (uint32_t*)(base + partial) : nullptr;
         return a;
@@ -1960,7 +2032,8 @@ int geo_sc_matmul_q8_epilogue(const int8_t* x, int64_t x_stride, const float* x_
 {
     if (!epilogue || epilogue->struct_bytes != sizeof *epilogue || epilogue->activation < GEO_SC_ACT_NONE || epilogue->activation > GEO_SC_ACT_SILU ||
         (epilogue->bias && !dtype_known(epilogue->bias_dtype)) || epilogue->residual_stride < 0 ||
-        (epilogue->slope && !slope_type_known(epilogue->slope_dtype)))
+        (epilogue->slope && (!slope_type_known(epilogue->slope_dtype) ||
+                             (epilogue->slope_dtype == GEO_SC_U8 && epilogue->activation > GEO_SC_ACT_RELU))))
         return GEO_SC_ERR_INVALID_ARGUMENT;
     const Epilogue e = {epilogue->bias,       epilogue->residual,    epilogue->slope,     epilogue->residual_stride,
                         epilogue->bias_dtype, epilogue->slope_dtype, epilogue->activation};

@@ -469,7 +469,7 @@ GEO_SC_API size_t geo_sc_static_workspace_bytes(void);
  * the distance of two rows in elements, where none is asked for rows follow each other.  Rows may start at any
  * multiple of the element; 16-byte aligned rows are the fast way.
  */
-enum geo_sc_dtype { GEO_SC_F32 = 0, GEO_SC_BF16 = 1, GEO_SC_F16 = 2 };
+enum geo_sc_dtype { GEO_SC_F32 = 0, GEO_SC_BF16 = 1, GEO_SC_F16 = 2, GEO_SC_U8 = 3 /* slopes of a relu only */ };
 enum geo_sc_reduction { GEO_SC_REDUCE_NONE = 0, GEO_SC_REDUCE_SUM = 1, GEO_SC_REDUCE_MEAN = 2 };
 
 /*
@@ -535,7 +535,8 @@ GEO_SC_API int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64
  * The same product with an epilogue: with z = x_scale[m] w_scale[n] sum + bias[n] in fp32, y = act(z) + residual, rounded once.
  * Activations: relu; gelu, z times the normal distribution's share below z; silu, z / (1 + exp(-z)).
  *   bias, residual   NULL: none; `cols` elements of bias_dtype, (rows, cols) of y's dtype with residual_stride between its rows
- *   slope            NULL, or (rows, cols), without gaps, for the backward: act'(z) in slope_dtype, GEO_SC_F16 or GEO_SC_F32
+ *   slope            NULL, or (rows, cols), without gaps, for the backward: act'(z) in slope_dtype, GEO_SC_F16, GEO_SC_F32 or, of a
+ *                    relu (or no activation), GEO_SC_U8
  * Workspace: geo_sc_matmul_q8_workspace_size.
  * Backward, from g (gradient of y): with dz = g slope (0 where the slope is 0; slope NULL: dz = g), dx and dw as
  * geo_sc_matmul_q8_backward has them from dz, dbias[n] = sum_m dz[m][n] in an order that does not change from run to run; each of the three may be

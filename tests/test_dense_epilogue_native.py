@@ -34,7 +34,7 @@ def test_forward_refuses(lib):
         args = list(good)
         args[at] = bad
         assert lib.geo_sc_matmul_q8_epilogue(*args) == status, (at, bad)
-    for bad in (dict(struct_bytes=8), dict(bias_dtype=3), dict(activation=4), dict(activation=-1), dict(residual_stride=-1), dict(slope_dtype=1), dict(slope_dtype=3)):
+    for bad in (dict(struct_bytes=8), dict(bias_dtype=3), dict(activation=4), dict(activation=-1), dict(residual_stride=-1), dict(slope_dtype=1), dict(slope_dtype=4), dict(slope_dtype=3)):
         args = list(good)
         args[9] = epilogue(**bad)
         assert lib.geo_sc_matmul_q8_epilogue(*args) == INVALID, bad
@@ -51,7 +51,7 @@ def test_backward_refuses(lib):
     assert query(100, 130, 4096, 1, 1, 1, 1, ctypes.byref(size)) == 0 and size.value > plain.value
     assert query(100, 130, 4096, 1, 0, 0, 1, ctypes.byref(size)) == 0 and size.value >= 130 * 4
     good = [P, 1, 130, P, 2, P, 4096, P, P, 4096, P, 100, 130, 4096, P, 1, P, 1, P, 1, P, 1 << 40, None]
-    for at, bad, status in ((0, None, INVALID), (1, 5, INVALID), (2, -1, INVALID), (2, 7, INVALID), (4, 3, INVALID), (4, 1, INVALID), (5, None, INVALID), (7, None, INVALID),
+    for at, bad, status in ((0, None, INVALID), (1, 5, INVALID), (2, -1, INVALID), (2, 7, INVALID), (4, 4, INVALID), (4, 1, INVALID), (5, None, INVALID), (7, None, INVALID),
                             (8, None, INVALID), (10, None, INVALID), (11, 0, INVALID), (12, 0, INVALID), (13, 131072, INVALID), (15, 5, INVALID),
                             (17, 5, INVALID), (19, 5, INVALID), (20, None, WORKSPACE), (20, P + 8, WORKSPACE), (21, 100, WORKSPACE)):
         args = list(good)

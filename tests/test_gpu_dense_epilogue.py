@@ -61,6 +61,35 @@ def test_kernels(uf, shape):
         check(uf, q, s, wq, ws, dtype, kind, bias, residual)
 
 
+# rows and columns just beyond whole tiles, where the tiles are just beyond what all compute units do at once: strips of their own
+STRIPS = [(4096, 4099, 300), (4100, 4096, 300), (4111, 4160, 300), (4160, 8192 - 255, 260), (2049, 2051 * 4, 270)]
+
+
+@pytest.mark.parametrize("shape", STRIPS)
+def test_strips(uf, shape):
+    m, n, k = shape
+    (q, s), (wq, ws) = random_q8(m, k, 1), random_q8(n, k, 2)
+    q, wq, ws = aligned(q), aligned(wq), ws / (k ** 0.5 * 40)
+    for dtype in TYPES:
+        want = product64(q, s, wq, ws)
+        close(uf.matmul_q8(q, s, wq, ws, dtype=dtype), want, (EPS[dtype] + 4 * U) * want.abs() + subnormal(dtype))
+        check(uf, q, s, wq, ws, dtype, "gelu", rand(n, dtype=dtype, seed=3), rand(m, n, dtype=dtype, seed=4))
+    # gradients of the same sizes: either product's rows and columns
+    g = rand(m, n, dtype=torch.bfloat16, seed=5)
+    x, w = rand(m, k, dtype=torch.bfloat16, seed=6), rand(n, k, dtype=torch.bfloat16, seed=7)
+    bias = rand(n, seed=8)
+    _, (dx, dw, dbias) = gradients(uf, x, w, bias, None, g, "silu")
+    (q, s, _), (wq, ws, _) = uf.quantize_rows(x.detach()), uf.quantize_rows(w.detach())
+    _, _, slope, slope_off, _ = epilogue64(product64(q, s, wq, ws), bias.detach(), "silu", None, torch.bfloat16)
+    dz, dz_off = g.double() * slope, g.double().abs() * (slope_off + U * slope.abs())
+    xr, wr = q.double() * s.double()[:, None], wq.double() * ws.double()[:, None]
+    kept = EPS[torch.float16] + U
+    for got, want, size, off, depth in ((dx, dz @ wr, dz.abs() @ wr.abs(), dz_off @ wr.abs(), n),
+                                        (dw, dz.t() @ xr, dz.t().abs() @ xr.abs(), dz_off.t() @ xr.abs(), m)):
+        close(got, want, EPS[torch.bfloat16] * want.abs() + (kept + 2 * depth * U) * size + off + 1e-9)
+    close(dbias, dz.sum(0), U * dz.sum(0).abs() + m * U * dz.abs().sum(0) + dz_off.sum(0))
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(1, 100, 300), (5, 77, 4200), (33, 130, 4097), (40, 100, 40000), (65, 129, 127), (130, 300, 700), (700, 515, 2049)])
