@@ -555,12 +555,20 @@ template <int B, int ROWS>
 struct EpilogueTile {
     static constexpr int T = B / 32, kCols = T * 16, kPieces = kCols / 4, kMix = (kPieces < 16 ? kPieces : 16) - 1;
     static constexpr int kLanes = kCols / kChunk, kAtOnce = 64 / kLanes;   // lanes of a row, rows at once
-    static constexpr int kPasses = ROWS / kAtOnce, kBatch = B == 256 ? 4 : 2, kStep = kBatch * kAtOnce;
-    static_assert(ROWS % 16 == 0 && kCols % ROWS == 0 && kPasses % kBatch == 0, "");
+    static constexpr int kPasses = ROWS / kAtOnce;
+    static_assert(ROWS % 16 == 0 && kCols % ROWS == 0 && kPasses % (B == 256 ? 4 : 2) == 0, "");
     const Epilogue& e;
     float ws[kChunk], bias[kChunk], xs[T];
 
-    __device__ __forceinline__ int64_t column(const Spot& p, int wave, int lane) const { return p.n0 + wave / 2 * kCols + lane % kLanes * kChunk; }
+    // A wave whose columns end inside a chunk has that chunk begin earlier: its lane, and those behind it, form the last eight columns
+    // once more, the same numbers as the lane before, and nothing depends on a lane.  (Masked loads cannot be asked for ahead: the tiles
+    // of the last rows of 4095 x 4099 with a residual took 25 us more.)  One that has fewer than eight columns is masked.
+    static __device__ __forceinline__ int64_t begin(const Spot& p, int wave) { return p.n0 + wave / 2 * kCols; }
+    static __device__ __forceinline__ int64_t column(const Spot& p, int wave, int lane)
+    {
+        const int64_t n = begin(p, wave) + lane % kLanes * kChunk, last = p.a.cols - kChunk;
+        return n > last && last >= begin(p, wave) ? last : n;
+    }
     // asks for the scales and the bias
     __device__ __forceinline__ void ask(const Spot& p, int wave, int lane)
     {
@@ -575,28 +583,37 @@ struct EpilogueTile {
             xs[i] = p.a.x_scale[m < p.a.rows ? m : p.a.rows - 1];
         }
     }
-    // WHOLE: the tile lies inside the product
-    template <typename Y, bool WHOLE>
+    enum Way { kWhole, kOverlap, kMasked };
+    template <typename Y, Way WAY>
     __device__ __forceinline__ void rows(const Spot& p, v4i (&sum)[T][T], uint8_t* area, int wave, int lane) const
     {
+        constexpr int kBatch = B == 256 && sizeof(Y) == 2 ? 4 : 2, kStep = kBatch * kAtOnce;   // (what the registers hold)
         const int64_t cols = p.a.cols, stride = p.a.y_stride, n = column(p, wave, lane), left = cols - n, m0 = p.m0 + wave % 2 * kCols + lane / kLanes;
-        const int mine = lane / kLanes, piece = lane % kLanes * 2;
+        const int mine = lane / kLanes, piece = lane % kLanes * 2, from = (int)(n - begin(p, wave));
         const auto ask_residual = [&](Y (&raw)[kBatch][kChunk], int r) {
-            if (!e.residual || (!WHOLE && left <= 0)) return;
+            if (!e.residual || (WAY == kMasked && left <= 0)) return;
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
                 const int64_t m = m0 + r + i * kAtOnce;
                 const Y* row = (const Y*)e.residual + (m < p.a.rows ? m : p.a.rows - 1) * e.residual_stride;   // (behind the last row that row once more)
-                if constexpr (WHOLE) fetch_whole<false>(row + n, raw[i]);
-                else fetch_chunk<false>(row, n, cols, raw[i]);
+                if constexpr (WAY == kMasked) fetch_chunk<false>(row, n, cols, raw[i]);
+                else fetch_whole<false>(row + n, raw[i]);
             }
         };
         const auto ask_sums = [&](float (&v)[kBatch][kChunk], int r) {
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
                 const int row = (r + i * kAtOnce + mine) % ROWS;
+                if constexpr (WAY == kOverlap) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) __builtin_memcpy(v[i] + 4 * h, area + (row * kPieces + ((piece + h) ^ (row & kMix))) * 16, 16);
+                    for (int j = 0; j < kChunk; ++j) {
+                        const int c = from + j;
+                        v[i][j] = *(const float*)(area + (row * kPieces + ((c >> 2) ^ (row & kMix))) * 16 + (c & 3) * 4);
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) __builtin_memcpy(v[i] + 4 * h, area + (row * kPieces + ((piece + h) ^ (row & kMix))) * 16, 16);
+                }
             }
         };
         Y residual_ahead[kBatch][kChunk] = {};
@@ -633,8 +650,8 @@ struct EpilogueTile {
 #pragma unroll
                     for (int j = 0; j < kChunk; ++j) z[i][j] = z[i][j] * ws[j] + bias[j];
                     activate(e.activation, z[i], d);
-                    if (!WHOLE && (m0 + first + r + i * kAtOnce >= p.a.rows || left <= 0)) continue;
-                    const int64_t there = WHOLE ? kChunk : left;
+                    if (m0 + first + r + i * kAtOnce >= p.a.rows || (WAY == kMasked && left <= 0)) continue;
+                    const int64_t there = WAY == kMasked ? left : kChunk;
                     if (e.slope) store_slope(e, at, there, d);
                     if (e.residual) {
 #pragma unroll
@@ -649,8 +666,10 @@ struct EpilogueTile {
     template <typename Y>
     __device__ __forceinline__ void rows(const Spot& p, v4i (&sum)[T][T], uint8_t* area, int wave, int lane) const
     {
-        if (inside<B>(p)) rows<Y, true>(p, sum, area, wave, lane);
-        else rows<Y, false>(p, sum, area, wave, lane);
+        const int64_t there = p.a.cols - begin(p, wave);
+        if (there >= kCols) rows<Y, kWhole>(p, sum, area, wave, lane);
+        else if (there >= kChunk) rows<Y, kOverlap>(p, sum, area, wave, lane);
+        else if (there > 0) rows<Y, kMasked>(p, sum, area, wave, lane);
     }
     __device__ __forceinline__ void finish(const Spot& p, v4i (&sum)[T][T], uint8_t* area, int wave, int lane) const
     {
@@ -1643,6 +1662,36 @@ __global__ __launch_bounds__(kPeakWaves * 64) void k_grad_peaks(OperandArgs a)
     for (int64_t r = threadIdx.x; r < r1 - r0; r += blockDim.x) a.row_peaks[across * a.rows + r0 + r] = row_most[r];
 }
 
+// The maxima and sums of more than kMostJoined blocks of rows, into the first block's place: every tile of k_grad_operands would
+// read them all (16384 x 1024 in 128 blocks: 50 us, so 37 and 4).
+constexpr uint32_t kMostJoined = 32;
+__global__ __launch_bounds__(256) void k_join_peaks(OperandArgs a)
+{
+    const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+    const uint32_t share = threadIdx.x >> 6;
+    __shared__ uint32_t most[4][64];
+    __shared__ float sums[4][64];
+    uint32_t m = 0;
+    float s = 0.f;
+    if (c < a.cols) {
+        if (a.col_peaks) {
+#pragma unroll 16
+            for (uint32_t k = share; k < a.row_blocks; k += 4) m = max(m, a.col_peaks[k * a.cols + c]);
+        }
+        if (a.col_sums) {
+#pragma unroll 16
+            for (uint32_t k = share; k < a.row_blocks; k += 4) s += a.col_sums[k * a.cols + c];
+        }
+    }
+    most[share][threadIdx.x & 63] = m;
+    sums[share][threadIdx.x & 63] = s;
+    __syncthreads();   // (all have read: a column is one workgroup's)
+    if (share || c >= a.cols) return;
+    const int i = threadIdx.x;
+    if (a.col_peaks) a.col_peaks[c] = max(max(most[0][i], most[1][i]), max(most[2][i], most[3][i]));
+    if (a.col_sums) a.col_sums[c] = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
+}
+
 // out[c][r] = q[r][c] in fp16 for a tile of 64 rows and 128 columns.  A thread turns four columns of eight rows: it reads a
 // word of each row (a row of 33 words: no two lanes meet in a bank) and writes eight rows' values of each column.
 constexpr int kWideWords = kWide / 4 + 1;
@@ -1795,7 +1844,7 @@ GradLayout grad_layout(int64_t rows, int64_t cols, int64_t inner, int terms, boo
         return here;
     };
     l.peak_cols = peak_block(cols, 32, kPeakWide, (int64_t)1 << 40);
-    // (a workgroup for each compute unit, but no more than 128 maxima of a column to join: 16384 x 1024 in 64 blocks 32 us)
+    // (a workgroup for each compute unit: 16384 x 1024 in 256 blocks 16 us, in 64 32)
     const int64_t across = (cols + l.peak_cols - 1) / l.peak_cols;
     l.peak_rows = peak_block(rows, across >= 8 ? 32 : across >= 2 ? 256 / across : 128, 32, kMostPeakRows);
     if (need_dx) {
@@ -1935,7 +1984,9 @@ int backward(const void* grad, int grad_dtype, int64_t grad_stride, const void* 
     o.col_blocks = (uint32_t)((cols + l.peak_cols - 1) / l.peak_cols);
     o.g_tiles = (uint32_t)g_tiles;
     o.w_tiles = (uint32_t)w_tiles;
-    const dim3 peak_threads((uint32_t)((l.peak_rows < kPeakWaves * kPeakBatch ? l.peak_rows / kPeakBatch : kPeakWaves) * 64));
+    // (with a slope or sums, half as many waves: two workgroups on a compute unit, where one would leave the last few a round of their own)
+    const int most_waves = slope || dbias ? kPeakWaves / 2 : kPeakWaves;
+    const dim3 peak_threads((uint32_t)((l.peak_rows < most_waves * kPeakBatch ? l.peak_rows / kPeakBatch : most_waves) * 64));
     const auto peaks_of = [&](auto one, auto with_sums, auto with_slope, auto of_slope) {
         using T = decltype(one);
         using S = decltype(of_slope);
@@ -1954,6 +2005,10 @@ int backward(const void* grad, int grad_dtype, int64_t grad_stride, const void* 
     if (grad_dtype == GEO_SC_F32) peaks(f32());
     else if (grad_dtype == GEO_SC_BF16) peaks(bf16());
     else peaks(f16());
+    if (o.row_blocks > kMostJoined && (o.col_peaks || o.col_sums)) {
+        k_join_peaks<<<dim3((uint32_t)((cols + 63) / 64)), dim3(256), 0, s>>>(o);
+        o.row_blocks = 1;
+    }
     const dim3 grid((uint32_t)(g_tiles + w_tiles + x_tiles));
     if (terms == 1) k_grad_operands<1><<<grid, dim3(256), 0, s>>>(o);
     else k_grad_operands<2><<<grid, dim3(256), 0, s>>>(o);

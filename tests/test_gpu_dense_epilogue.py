@@ -90,6 +90,26 @@ def test_strips(uf, shape):
     close(dbias, dz.sum(0), U * dz.sum(0).abs() + m * U * dz.abs().sum(0) + dz_off.sum(0))
 
 
+# columns that end inside a chunk of a tile's first and second half, with fewer than eight of them there, and exactly at their ends
+@pytest.mark.parametrize("cols", [1, 7, 8, 9, 31, 32, 33, 39, 40, 41, 63, 64, 65, 100, 127, 128, 129, 200, 257, 263, 264, 385, 391, 392, 500])
+@pytest.mark.parametrize("rows,inner", [(66, 260), (129, 70), (1000, 2100)])
+def test_columns_that_end_anywhere(uf, rows, cols, inner):
+    (q, s), (wq, ws) = random_q8(rows, inner, 1), random_q8(cols, inner, 2)
+    q, wq, ws = aligned(q), aligned(wq), ws / (inner ** 0.5 * 40)
+    for dtype in TYPES:
+        check(uf, q, s, wq, ws, dtype, "gelu", rand(cols, dtype=dtype, seed=3), rand(rows, cols, dtype=dtype, seed=4))
+
+
+# the same where the tiles are large
+@pytest.mark.parametrize("cols", [4100, 4103, 4107, 4200, 4223, 4225, 4230, 4300])
+def test_columns_that_end_anywhere_in_large_tiles(uf, cols):
+    rows, inner = 4090, 600
+    (q, s), (wq, ws) = random_q8(rows, inner, 1), random_q8(cols, inner, 2)
+    q, wq, ws = aligned(q), aligned(wq), ws / (inner ** 0.5 * 40)
+    for dtype in TYPES:
+        check(uf, q, s, wq, ws, dtype, "silu", rand(cols, dtype=dtype, seed=3), rand(rows, cols, dtype=dtype, seed=4))
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape", [(1, 100, 300), (5, 77, 4200), (33, 130, 4097), (40, 100, 40000), (65, 129, 127), (130, 300, 700), (700, 515, 2049)])
