@@ -141,136 +141,171 @@ __device__ __forceinline__ void rounded(float (&v)[kChunk])
     for (int j = 0; j < kChunk; ++j) asm volatile("" : "+v"(v[j]));
 }
 
-// One row per threadIdx.y: a row's blockDim.x threads hold ITEMS chunks of eight columns each.  (Fused multiply-adds by name: the compiler's choice
-// is another in every instance, and totals are the same bits in all of them.)
-template <typename T, int ITEMS, int LANES, bool ONCE, bool EIGHT>
+// ROWS rows per threadIdx.y: their blockDim.x threads hold ITEMS chunks of eight columns of each.  Two rows at once read what belongs to
+// the channels once, four vectors of a row's length out of L2 beside a row's four, and share the exchanges.  (Fused multiply-adds by name: the
+// compiler's choice is another in every instance, and totals are the same bits in all of them.)
+template <int ROWS>
+struct ManySlots {
+    float sum[2][ROWS][16];
+};
+template <typename T, int ROWS, int ITEMS, int LANES, bool ONCE, bool EIGHT>
 __global__ __launch_bounds__(1024) void k_gated_norm(NormArgs a)
 {
     __shared__ RowSlots slots;
-    const int64_t row = a.first_row + (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    __shared__ ManySlots<ROWS> many;
     const int threads = blockDim.x, t = threadIdx.x, waves = threads >> 6;   // (blocks of several rows have no more than a wave per row: no barrier)
-    if (row >= a.rows) return;
+    const int64_t row0 = a.first_row + ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * ROWS;
+    if (row0 >= a.rows) return;
+    const auto row_of = [&](int q) { return row0 + q < a.rows ? row0 + q : a.rows - 1; };   // (one too many is the last one again, and not stored)
     int turn = 0;
     const auto column = [&](int i) { return ((int64_t)i * threads + t) * kChunk; };
-    // the sum of squares of what is held, and its root; again from v times a power of two where that is needed
-    const auto root_of_row = [&](const float (&v)[ITEMS][kChunk]) {
-        float squares = 0.f;
+    const auto reduce_all = [&](float (&sum)[ROWS]) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
+        for (int q = 0; q < ROWS; ++q)
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) squares = fmaf(v[i][j], v[i][j], squares);
-        reduce_row<LANES>(squares, waves, slots, turn);
-        if (__builtin_expect(in_range(squares, a.cols, a.eps), true)) return root_of(squares, a.cols, a.eps);
-        uint32_t peak = 0;
-        float none = 0.f;
+            for (int d = LANES / 2; d >= 1; d >>= 1) sum[q] += __shfl_xor(sum[q], d);
+        if (LANES == 32 || waves == 1) return;
+        if ((t & 63) == 0)
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
+            for (int q = 0; q < ROWS; ++q) many.sum[turn & 1][q][t >> 6] = sum[q];
+        __syncthreads();
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) peak = max(peak, magnitude_bits(v[i][j]));
-        reduce_row<LANES>(none, peak, waves, slots, turn);
-        if (peak == 0 || peak >= kInfinityBits) return root_of(squares, a.cols, a.eps);
-        const float up = power_up(peak);
-        squares = 0.f;
-#pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) squares = fmaf(v[i][j] * up, v[i][j] * up, squares);
-        reduce_row<LANES>(squares, waves, slots, turn);
-        return root_of_scaled(squares, up, a.cols, a.eps);
+        for (int q = 0; q < ROWS; ++q) {
+            sum[q] = 0.f;
+            for (int k = 0; k < waves; ++k) sum[q] += many.sum[turn & 1][q][k];
+        }
+        ++turn;
     };
-    Raw<T> raw[ITEMS], also[ITEMS];
-    float v[ITEMS][kChunk];
-    const T* gate = a.gate ? (const T*)a.gate + run_of(row, a.run) * a.cols : nullptr;
-    // What belongs to the channels is asked for together with the row, where the registers are there for it, and not behind an exchange.
-    constexpr bool kAhead = sizeof(T) == 2 ? ITEMS <= 2 : ITEMS == 1;
-    struct Held {
-        Raw<T> post, gate, scale, weight;
-    };
-    Held held[kAhead ? ITEMS : 1];
-    const auto channels = [&](int i, const T* from, Raw<T> Held::*which, float (&f)[kChunk]) {
-        if constexpr (kAhead) {
-            (held[i].*which).keep();
+    // the sums of squares of what is held, and their roots; again from v times a power of two where that is needed
+    const auto roots_of = [&](const float (&v)[ROWS][ITEMS][kChunk], Root (&root)[ROWS]) {
+        float squares[ROWS];
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) f[j] = (held[i].*which)[j];
-        } else {
-            load_chunk(from, column(i), a.cols, 0.f, f);
+        for (int q = 0; q < ROWS; ++q) {
+            squares[q] = 0.f;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) squares[q] = fmaf(v[q][i][j], v[q][i][j], squares[q]);
+        }
+        reduce_all(squares);
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q) {
+            root[q] = root_of(squares[q], a.cols, a.eps);
+            if (__builtin_expect(in_range(squares[q], a.cols, a.eps), true)) continue;   // (all threads of a row alike)
+            uint32_t peak = 0;
+            float none = 0.f;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) peak = max(peak, magnitude_bits(v[q][i][j]));
+            reduce_row<LANES>(none, peak, waves, slots, turn);
+            if (peak == 0 || peak >= kInfinityBits) continue;
+            const float up = power_up(peak);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) sum = fmaf(v[q][i][j] * up, v[q][i][j] * up, sum);
+            reduce_row<LANES>(sum, waves, slots, turn);
+            root[q] = root_of_scaled(sum, up, a.cols, a.eps);
         }
     };
+    Raw<T> raw[ROWS][ITEMS], also[ROWS][ITEMS];
+    float v[ROWS][ITEMS][kChunk];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-        if (column(i) < a.cols) {
-            raw[i].template fetch<ONCE>((const T*)a.x + row * a.x_stride, column(i), a.cols);
-            also[i].template fetch<ONCE>((const T*)a.residual + row * a.residual_stride, column(i), a.cols);
-            if constexpr (kAhead) {
-                if (a.post) held[i].post.template fetch<false>(a.post, column(i), a.cols);
-                if (gate) held[i].gate.template fetch<false>(gate, column(i), a.cols);
-                if (a.scale) held[i].scale.template fetch<false>(a.scale, column(i), a.cols);
-                held[i].weight.template fetch<false>(a.weight, column(i), a.cols);
+    for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            if (column(i) < a.cols) {
+                raw[q][i].template fetch<ONCE>((const T*)a.x + row_of(q) * a.x_stride, column(i), a.cols);
+                also[q][i].template fetch<ONCE>((const T*)a.residual + row_of(q) * a.residual_stride, column(i), a.cols);
+            } else {
+                raw[q][i].set(0.f);
+                also[q][i].set(0.f);
             }
-        } else {
-            raw[i].set(0.f);
-            also[i].set(0.f);
         }
-    }
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i)
+    for (int q = 0; q < ROWS; ++q)
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) v[i][j] = raw[i][j];
-    Root first = {1.f, 1.f, 1.f};
-    if (a.post) first = root_of_row(v);
+        for (int i = 0; i < ITEMS; ++i)
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) v[q][i][j] = raw[q][i][j];
+    Root first[ROWS], second[ROWS];
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) first[q] = {1.f, 1.f, 1.f};
+    if (a.post) roots_of(v, first);
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
         if (column(i) < a.cols) {
             float f[kChunk];
             if (a.post) {
-                channels(i, (const T*)a.post, &Held::post, f);
+                load_chunk((const T*)a.post, column(i), a.cols, 0.f, f);
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) v[i][j] = v[i][j] * first.up * first.factor * f[j];
+                for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) v[q][i][j] = v[q][i][j] * first[q].up * first[q].factor * f[j];
             }
-            if (gate) {
-                channels(i, gate, &Held::gate, f);
+            if (a.gate) {
 #pragma unroll
-                for (int j = 0; j < kChunk; ++j) v[i][j] *= f[j];
+                for (int q = 0; q < ROWS; ++q) {
+                    load_chunk((const T*)a.gate + run_of(row_of(q), a.run) * a.cols, column(i), a.cols, 0.f, f);
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) v[q][i][j] *= f[j];
+                }
             }
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) f[j] = 1.f;
-            if (a.scale) channels(i, (const T*)a.scale, &Held::scale, f);
-            also[i].keep();
+            if (a.scale) load_chunk((const T*)a.scale, column(i), a.cols, 0.f, f);
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) v[i][j] = fmaf(f[j], also[i][j], v[i][j]);
-            rounded(v[i]);
-            store_chunk((T*)a.total + row * a.cols, column(i), a.cols, v[i], a.streamed);
+            for (int q = 0; q < ROWS; ++q) {
+                also[q][i].keep();
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) v[q][i][j] = fmaf(f[j], also[q][i][j], v[q][i][j]);
+                rounded(v[q][i]);
+                if (row0 + q < a.rows) store_chunk((T*)a.total + (row0 + q) * a.cols, column(i), a.cols, v[q][i], a.streamed);
+            }
         }
-    const Root second = root_of_row(v);
-    if (t == 0 && a.rstd) {
-        a.rstd[2 * row] = first.unit;
-        a.rstd[2 * row + 1] = second.unit;
-    }
-    uint32_t most = 0;
+    roots_of(v, second);
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q)
+        if (t == 0 && a.rstd && row0 + q < a.rows) {
+            a.rstd[2 * (row0 + q)] = first[q].unit;
+            a.rstd[2 * (row0 + q) + 1] = second[q].unit;
+        }
+    uint32_t most[ROWS] = {};
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i)
         if (column(i) < a.cols) {
             float w[kChunk];
-            channels(i, (const T*)a.weight, &Held::weight, w);
+            load_chunk((const T*)a.weight, column(i), a.cols, 0.f, w);
 #pragma unroll
-            for (int j = 0; j < kChunk; ++j) {
-                v[i][j] = v[i][j] * second.up * second.factor * w[j];
-                most = max(most, magnitude_bits(v[i][j]));
+            for (int q = 0; q < ROWS; ++q) {
+#pragma unroll
+                for (int j = 0; j < kChunk; ++j) {
+                    v[q][i][j] = v[q][i][j] * second[q].up * second[q].factor * w[j];
+                    most[q] = max(most[q], magnitude_bits(v[q][i][j]));
+                }
+                if constexpr (!EIGHT)
+                    if (row0 + q < a.rows) store_chunk((T*)a.out + (row0 + q) * a.cols, column(i), a.cols, v[q][i], a.streamed);
             }
-            if constexpr (!EIGHT) store_chunk((T*)a.out + row * a.cols, column(i), a.cols, v[i], a.streamed);
         }
     if constexpr (EIGHT) {
-        float none = 0.f;
-        reduce_row<LANES>(none, most, waves, slots, turn);
-        const RowScale rs = row_scale(most, 1.f, true);
-        if (t == 0) a.q_scale[row] = rs.scale;
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (column(i) < a.cols) {
-                float values[kChunk];
-                store_eight(a.q + row * a.q_stride, column(i), a.cols, rs, v[i], values);
-                if (a.values) store_chunk(a.values, a.values_dtype, row * a.cols, column(i), a.cols, values, a.streamed);
-            }
+        for (int q = 0; q < ROWS; ++q) {
+            float none = 0.f;
+            reduce_row<LANES>(none, most[q], waves, slots, turn);
+            if (row0 + q >= a.rows) continue;
+            const int64_t row = row0 + q;
+            const RowScale rs = row_scale(most[q], 1.f, true);
+            if (t == 0) a.q_scale[row] = rs.scale;
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (column(i) < a.cols) {
+                    float values[kChunk];
+                    store_eight(a.q + row * a.q_stride, column(i), a.cols, rs, v[q][i], values);
+                    if (a.values) store_chunk(a.values, a.values_dtype, row * a.cols, column(i), a.cols, values, a.streamed);
+                }
+        }
     }
 }
 
@@ -380,20 +415,24 @@ int run_norm(NormArgs a, int dtype, hipStream_t s)
     a.streamed = streams(a.rows * a.cols * ((int64_t)sizeof(T) + (EIGHT ? a.values ? dtype_bytes(a.values_dtype) : 0 : (int64_t)sizeof(T))));
     const int64_t chunks = (a.cols + kChunk - 1) / kChunk;
     const int threads = chunks <= 32 ? 32 : threads_of_row(chunks, a.rows >= 2048 && chunks > 64 ? 2 : 1);
-    const int per_block = threads <= 64 ? 256 / threads : 1;
     const int64_t items = (chunks + threads - 1) / threads;
+    const bool two = sizeof(T) == 2 && a.rows >= 2048 && items == 2;
+    const int per_block = threads <= 64 ? 256 / threads : 1, rows_per_block = per_block * (two ? 2 : 1);
     const dim3 block(threads, per_block);
-    in_launches((a.rows + per_block - 1) / per_block, threads * per_block, [&](int64_t first, uint32_t grid) {
-        a.first_row = first * per_block;
-        const auto held = [&](auto count, auto lanes) {
-            if (once) k_gated_norm<T, count(), lanes(), true, EIGHT><<<grid, block, 0, s>>>(a);
-            else k_gated_norm<T, count(), lanes(), false, EIGHT><<<grid, block, 0, s>>>(a);
+    in_launches((a.rows + rows_per_block - 1) / rows_per_block, threads * per_block, [&](int64_t first, uint32_t grid) {
+        a.first_row = first * rows_per_block;
+        const auto held = [&](auto rows, auto count, auto lanes) {
+            if (once) k_gated_norm<T, rows(), count(), lanes(), true, EIGHT><<<grid, block, 0, s>>>(a);
+            else k_gated_norm<T, rows(), count(), lanes(), false, EIGHT><<<grid, block, 0, s>>>(a);
         };
         const std::integral_constant<int, 64> wave;
-        if (threads == 32) held(std::integral_constant<int, 1>(), std::integral_constant<int, 32>());
-        else if (items <= 1) held(std::integral_constant<int, 1>(), wave);
-        else if (items <= 2) held(std::integral_constant<int, 2>(), wave);
-        else if (items <= 4) held(std::integral_constant<int, 4>(), wave);
+        const std::integral_constant<int, 1> one;
+        const std::integral_constant<int, 2> pair;
+        if (threads == 32) held(one, one, std::integral_constant<int, 32>());
+        else if (items <= 1) held(one, one, wave);
+        else if (two) held(pair, pair, wave);
+        else if (items <= 2) held(one, pair, wave);
+        else if (items <= 4) held(one, std::integral_constant<int, 4>(), wave);
         else k_gated_norm_long<T, EIGHT><<<grid, block, 0, s>>>(a);
     });
     return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
@@ -501,6 +540,20 @@ __global__ __launch_bounds__(512, 2) void k_gated_back(BackArgs a)
         }
     }
     int turn = 0;
+    // (the next row is on its way while one is worked on)
+    Raw<T> x_next[ITEMS], residual_next[ITEMS], g_next[ITEMS], also_next[ITEMS];
+    const auto ask = [&](int64_t row) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i)
+            if (column(i) < n.cols) {
+                x_next[i].template fetch<ONCE>((const T*)n.x + row * n.x_stride, column(i), n.cols);
+                residual_next[i].template fetch<ONCE>((const T*)n.residual + row * n.residual_stride, column(i), n.cols);
+                g_next[i].template fetch<ONCE>((const T*)a.grad + row * a.grad_stride, column(i), n.cols);
+                if (a.grad_total) also_next[i].template fetch<ONCE>((const T*)a.grad_total + row * a.grad_total_stride, column(i), n.cols);
+                else also_next[i].set(0.f);
+            }
+    };
+    ask(first);
     for (int64_t row = first; row < last; ++row) {
         if (row == run_end) {
 #pragma unroll
@@ -516,14 +569,8 @@ __global__ __launch_bounds__(512, 2) void k_gated_back(BackArgs a)
         const float r1 = n.rstd[2 * row], r2 = n.rstd[2 * row + 1];
         Raw<T> x[ITEMS], residual[ITEMS], g[ITEMS], also[ITEMS];
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
-            if (column(i) < n.cols) {
-                x[i].template fetch<ONCE>((const T*)n.x + row * n.x_stride, column(i), n.cols);
-                residual[i].template fetch<ONCE>((const T*)n.residual + row * n.residual_stride, column(i), n.cols);
-                g[i].template fetch<ONCE>((const T*)a.grad + row * a.grad_stride, column(i), n.cols);
-                if (a.grad_total) also[i].template fetch<ONCE>((const T*)a.grad_total + row * a.grad_total_stride, column(i), n.cols);
-                else also[i].set(0.f);
-            }
+        for (int i = 0; i < ITEMS; ++i) x[i] = x_next[i], residual[i] = residual_next[i], g[i] = g_next[i], also[i] = also_next[i];
+        ask(row + 1 < last ? row + 1 : row);
         const auto keep_all = [&](int i) { x[i].keep(), residual[i].keep(), g[i].keep(), also[i].keep(), weight[i].keep(), scale[i].keep(); };
         const auto form_n2 = [&](int i, int j, float n1) { return (scale[i][j] * residual[i][j] + branch[i][j] * n1) * r2; };
         float along = 0.f;
