@@ -35,6 +35,14 @@ struct NormArgs {
     int64_t first_row;   // of a launch
 };
 
+// threadIdx.y: of a row of whole waves it is the wave's, and so are the row's addresses and factors.
+template <int LANES>
+__device__ __forceinline__ uint32_t row_in_block()
+{
+    if constexpr (LANES == 64) return (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.y);
+    else return threadIdx.y;
+}
+
 // Sum, or sum and largest, over a row's lanes: LANES 32 (two rows in a wave) or 64, then over its waves.
 template <int LANES>
 __device__ __forceinline__ void reduce_row(float& sum, uint32_t& most, int waves, RowSlots& slots, int& turn)
@@ -154,7 +162,7 @@ __global__ __launch_bounds__(1024) void k_gated_norm(NormArgs a)
     __shared__ RowSlots slots;
     __shared__ ManySlots<ROWS> many;
     const int threads = blockDim.x, t = threadIdx.x, waves = threads >> 6;   // (blocks of several rows have no more than a wave per row: no barrier)
-    const int64_t row0 = a.first_row + ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * ROWS;
+    const int64_t row0 = a.first_row + ((int64_t)blockIdx.x * blockDim.y + row_in_block<LANES>()) * ROWS;
     if (row0 >= a.rows) return;
     const auto row_of = [&](int q) { return row0 + q < a.rows ? row0 + q : a.rows - 1; };   // (one too many is the last one again, and not stored)
     int turn = 0;
@@ -490,7 +498,7 @@ __global__ __launch_bounds__(512, 2) void k_gated_back(BackArgs a)
     __shared__ RowSlots slots;
     const NormArgs& n = a.n;
     const int threads = blockDim.x, t = threadIdx.x, waves = threads >> 6;
-    const int64_t unit = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, first = unit * a.each;
+    const int64_t unit = (int64_t)blockIdx.x * blockDim.y + row_in_block<LANES>(), first = unit * a.each;
     const int64_t last = first + a.each < n.rows ? first + a.each : n.rows;
     if (unit >= a.units) return;
     const auto column = [&](int i) { return ((int64_t)i * threads + t) * kChunk; };
