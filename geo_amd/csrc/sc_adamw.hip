@@ -17,6 +17,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #pragma clang fp contract(off)
 
 namespace geo_sc {
@@ -36,6 +38,7 @@ struct Constants {
     int copy_dtype;
     Steps steps;
     const Steps* device_steps;   // or NULL
+    bool streamed;               // what is written
 };
 struct Tensor {
     void* param;
@@ -102,16 +105,17 @@ struct States;
 template <>
 struct States<32> {
     float m[kChunk], v[kChunk];
+    template <bool ONCE>
     __device__ __forceinline__ void load(const Tensor& t, int64_t c)
     {
-        load_chunk((const float*)t.avg, c, t.elements, 0.f, m);
-        load_chunk((const float*)t.sq, c, t.elements, 0.f, v);
+        load_chunk<ONCE>((const float*)t.avg, c, t.elements, 0.f, m);
+        load_chunk<ONCE>((const float*)t.sq, c, t.elements, 0.f, v);
     }
-    __device__ __forceinline__ void store(const Tensor& t, int64_t c, const float (&)[kChunk], uint32_t)
+    __device__ __forceinline__ void store(const Tensor& t, int64_t c, const float (&)[kChunk], uint32_t, bool streamed)
     {
         if (c >= t.elements) return;
-        store_chunk((float*)t.avg, c, t.elements, m);
-        store_chunk((float*)t.sq, c, t.elements, v);
+        store_chunk((float*)t.avg, c, t.elements, m, streamed);
+        store_chunk((float*)t.sq, c, t.elements, v, streamed);
     }
 };
 template <>
@@ -127,6 +131,7 @@ struct States<8> {
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) raw[j] = c + j < n ? p[c + j] : 0;
     }
+    template <bool ONCE>
     __device__ __forceinline__ void load(const Tensor& t, int64_t c)
     {
         uint8_t a[kChunk], s[kChunk];
@@ -179,7 +184,7 @@ struct States<8> {
         for (int j = 0; j < kChunk; ++j)
             if (c + j < n) p[c + j] = raw[j];
     }
-    __device__ __forceinline__ void store(const Tensor& t, int64_t c, const float (&root)[kChunk], uint32_t number)
+    __device__ __forceinline__ void store(const Tensor& t, int64_t c, const float (&root)[kChunk], uint32_t number, bool)
     {
         const uint32_t first = (uint32_t)(c % kBlock) * 0x9E3779B1u + number * 0x6A09E667u;
         put<false>(t.avg, t.avg_scale, c, t.elements, m, first);
@@ -187,8 +192,8 @@ struct States<8> {
     }
 };
 
-// A workgroup takes 2048 elements of one tensor, a thread eight side by side.
-template <typename P, typename G, int BITS>
+// A workgroup takes 2048 elements of one tensor, a thread eight side by side.  ONCE: past the caches, see reads_once().
+template <typename P, typename G, int BITS, bool ONCE>
 __global__ __launch_bounds__(kThreads) void k_adamw(Share s)
 {
     // the tensor: each lane looks at the first workgroup of one
@@ -202,9 +207,9 @@ __global__ __launch_bounds__(kThreads) void k_adamw(Share s)
     float p[kChunk], g[kChunk], root[kChunk];
     States<BITS> states;
     // (lanes behind the tensor's end go on: their block's largest number is asked of all)
-    load_chunk((const P*)t.param, c, n, 0.f, p);
-    load_chunk((const G*)t.grad, c, n, 0.f, g);
-    states.load(t, c);
+    load_chunk<ONCE>((const P*)t.param, c, n, 0.f, p);
+    load_chunk<ONCE>((const G*)t.grad, c, n, 0.f, g);
+    states.template load<ONCE>(t, c);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) {
         const float grad = g[j] * k.scale;
@@ -213,23 +218,27 @@ __global__ __launch_bounds__(kThreads) void k_adamw(Share s)
         root[j] = sqrtf(states.v[j]);
         p[j] = p[j] * k.keep - (states.m[j] * steps.size) / (root[j] * steps.inverse_root + k.eps);
     }
-    states.store(t, c, root, steps.number);
+    states.store(t, c, root, steps.number, k.streamed);
     if (c >= n) return;
-    store_chunk((P*)t.param, c, n, p);
-    if (t.copy) store_chunk(t.copy, k.copy_dtype, 0, c, n, p, false);
+    store_chunk((P*)t.param, c, n, p, k.streamed);
+    if (t.copy) store_chunk(t.copy, k.copy_dtype, 0, c, n, p, k.streamed);
     if (t.clamped) {
         float v[kChunk];
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) v[j] = p[j] < k.lo ? k.lo : p[j] > k.hi ? k.hi : p[j];
-        store_chunk(t.clamped, c, n, v);
+        store_chunk(t.clamped, c, n, v, k.streamed);
     }
 }
 
 template <typename P, typename G>
 void run(const Share& s, uint32_t groups, int bits, hipStream_t stream)
 {
-    if (bits == 8) k_adamw<P, G, 8><<<dim3(groups), dim3(kThreads), 0, stream>>>(s);
-    else k_adamw<P, G, 32><<<dim3(groups), dim3(kThreads), 0, stream>>>(s);
+    const auto go = [&](auto width) {
+        if (s.c.streamed) k_adamw<P, G, width(), true><<<dim3(groups), dim3(kThreads), 0, stream>>>(s);
+        else k_adamw<P, G, width(), false><<<dim3(groups), dim3(kThreads), 0, stream>>>(s);
+    };
+    if (bits == 8) go(std::integral_constant<int, 8>());
+    else go(std::integral_constant<int, 32>());
 }
 template <typename P>
 void run(const Share& s, uint32_t groups, int grad_dtype, int bits, hipStream_t stream)
@@ -282,6 +291,15 @@ extern "C" int geo_sc_adamw(int count, const geo_sc_adamw_tensor* tensors, const
     } else {
         c.steps = steps_at(o->lr, o->beta1, o->beta2, o->step);
     }
+    // Past the caches where what is written fills them, and everything lies at whole lines' parts.
+    int64_t written = 0;
+    uint64_t places = 0;
+    for (int i = 0; i < count; ++i) {
+        const geo_sc_adamw_tensor& t = tensors[i];
+        written += t.elements * (dtype_bytes(o->param_dtype) + (eight ? 2 : 8) + (t.copy ? dtype_bytes(o->copy_dtype) : 0));
+        if (t.elements) places |= (uintptr_t)t.param | (uintptr_t)t.grad | (eight ? 0 : (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq);
+    }
+    c.streamed = streams(written) && places % 16 == 0;
     uint32_t groups = 0;
     bool launched = o->device_step;
     const auto launch = [&]() {

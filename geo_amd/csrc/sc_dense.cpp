@@ -7,9 +7,8 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
 #include <array>
-#include <map>
-#include <unordered_set>
 
 using namespace geo_sc_torch;
 
@@ -590,11 +589,13 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
     if (device_step) in_step(*device_step, "step", first, 1, {at::kLong});
     // Tensors of the same types go into one call; no writer meets another.
     typedef std::array<int, 3> Types;
-    std::map<Types, std::vector<geo_sc_adamw_tensor>> calls;
-    std::unordered_set<const void*> written;
-    const auto write = [&](const at::Tensor& t, const char* what) {
-        TORCH_CHECK(t.numel() == 0 || written.insert(t.data_ptr()).second, what, ": a step writes no tensor twice");
-        return t.data_ptr();
+    std::vector<std::pair<Types, std::vector<geo_sc_adamw_tensor>>> calls;
+    std::vector<void*> written;
+    written.reserve(n * 7);
+    const auto write = [&](const at::Tensor& t) {
+        void* p = t.data_ptr();
+        if (t.numel()) written.push_back(p);
+        return p;
     };
     for (size_t i = 0; i < n; ++i) {
         const int64_t elements = params[i].numel(), blocks = (elements + kStateBlock - 1) / kStateBlock;
@@ -602,28 +603,36 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
         t.elements = elements;
         in_step(params[i], "params", first, elements, {at::kFloat, at::kBFloat16, at::kHalf});
         in_step(grads[i], "grads", first, elements, {at::kFloat, at::kBFloat16, at::kHalf});
-        t.param = write(params[i], "params");
+        t.param = write(params[i]);
         t.grad = grads[i].const_data_ptr();
         for (const auto& [state, scales, what, codes, scale] : {std::make_tuple(&exp_avg, &avg_scales, "exp_avg", &t.exp_avg, &t.avg_scale),
                                                                 std::make_tuple(&exp_avg_sq, &sq_scales, "exp_avg_sq", &t.exp_avg_sq, &t.sq_scale)}) {
             in_step((*state)[i], what, first, elements, {eight ? at::kFloat8_e4m3fn : at::kFloat});
-            *codes = write((*state)[i], what);
+            *codes = write((*state)[i]);
             if (!eight) continue;
             in_step((**scales)[i], "scales", first, blocks, {at::kFloat8_e8m0fnu});
-            *scale = (uint8_t*)write((**scales)[i], "scales");
+            *scale = (uint8_t*)write((**scales)[i]);
         }
         if (copies) {
             in_step((*copies)[i], "copies", first, elements, {at::kFloat, at::kBFloat16, at::kHalf});
-            t.copy = write((*copies)[i], "copies");
+            t.copy = write((*copies)[i]);
         }
         if (clamped && (*clamped)[i]) {
             in_step(*(*clamped)[i], "clamped", first, elements, {at::kFloat});
-            t.clamped = (float*)write(*(*clamped)[i], "clamped");
+            t.clamped = (float*)write(*(*clamped)[i]);
         }
-        calls[{dtype_of(params[i].scalar_type(), "params"), dtype_of(grads[i].scalar_type(), "grads"),
-               copies ? dtype_of((*copies)[i].scalar_type(), "copies") : 0}]
-            .push_back(t);
+        const Types types = {dtype_of(params[i].scalar_type(), "params"), dtype_of(grads[i].scalar_type(), "grads"),
+                             copies ? dtype_of((*copies)[i].scalar_type(), "copies") : 0};
+        size_t k = 0;
+        while (k < calls.size() && calls[k].first != types) ++k;
+        if (k == calls.size()) {
+            calls.emplace_back(types, std::vector<geo_sc_adamw_tensor>());
+            calls[k].second.reserve(n - i);
+        }
+        calls[k].second.push_back(t);
     }
+    std::sort(written.begin(), written.end());
+    TORCH_CHECK(std::adjacent_find(written.begin(), written.end()) == written.end(), "a step writes no tensor twice");
     TORCH_CHECK(!device_step || calls.size() == 1, "a step that is counted on the GPU takes tensors of the same types");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(first.device());
     at::Tensor workspace;
