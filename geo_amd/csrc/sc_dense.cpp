@@ -590,11 +590,12 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
     // Tensors of the same types go into one call; no writer meets another.
     typedef std::array<int, 3> Types;
     std::vector<std::pair<Types, std::vector<geo_sc_adamw_tensor>>> calls;
-    std::vector<void*> written;
+    std::vector<std::pair<const char*, const char*>> written;   // begin, end
     written.reserve(n * 7);
     const auto write = [&](const at::Tensor& t) {
+        TORCH_CHECK(!t.is_inference() || c10::InferenceMode::is_enabled(), "an inference tensor is written to in inference mode only");
         void* p = t.data_ptr();
-        if (t.numel()) written.push_back(p);
+        if (t.numel()) written.emplace_back((const char*)p, (const char*)p + t.nbytes());
         return p;
     };
     for (size_t i = 0; i < n; ++i) {
@@ -632,7 +633,7 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
         calls[k].second.push_back(t);
     }
     std::sort(written.begin(), written.end());
-    TORCH_CHECK(std::adjacent_find(written.begin(), written.end()) == written.end(), "a step writes no tensor twice");
+    for (size_t i = 1; i < written.size(); ++i) TORCH_CHECK(written[i - 1].second <= written[i].first, "a step writes no memory twice");
     TORCH_CHECK(!device_step || calls.size() == 1, "a step that is counted on the GPU takes tensors of the same types");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(first.device());
     at::Tensor workspace;

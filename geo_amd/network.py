@@ -339,6 +339,8 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         from . import utils_functional as uf
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing() and not all(g["capturable"] for g in self.param_groups):
+            raise RuntimeError("AdamW(capturable=True) is the one whose steps can be recorded: others count them on the host")
         for group in self.param_groups:
             # parameters that have made the same number of steps; those counted on the GPU, that are counted together
             rows, counter = {}, None
@@ -437,14 +439,16 @@ def apply_update(model, optimizer, param_copy):
 
 def _apply_adamw(params, orgs, optimizer, param_copy):
     """``apply_update`` with the unscaling, the copies back and ``weight_org`` in the optimiser's kernel."""
-    stepped = [(master, p) for master, p in zip(param_copy, params) if p.grad is not None]
+    known = {id(p) for group in optimizer.param_groups for p in group["params"]}
+    stepped = [(master, p) for master, p in zip(param_copy, params) if p.grad is not None and id(master) in known]
     for master in param_copy:
         master.grad = None
     optimizer.step(grads={master: p.grad for master, p in stepped}, grad_scale=1 / SCALE_FACTOR,
                    copies={master: p.data for master, p in stepped},
                    clamped={master: orgs[id(p)] for master, p in stepped if id(p) in orgs}, bounds=(-1, 0.999))
-    for master, p in zip(param_copy, params):   # (what has no gradient is copied back all the same: the layers have quantised it)
-        if p.grad is None:
+    done = {id(p) for _, p in stepped}
+    for master, p in zip(param_copy, params):   # (what is not stepped is copied back all the same: the layers have quantised it)
+        if id(p) not in done:
             p.data.copy_(master.data)
             if id(p) in orgs:
                 torch.clamp(p.data, -1, 0.999, out=orgs[id(p)])

@@ -269,6 +269,8 @@ class Linear_Q8(nn.Module):
 
     def __setstate__(self, state):   # of a copy: another weight, of the same values
         super().__setstate__(state)
+        self.__dict__.setdefault("activation", None)   # (pickled before there were any)
+        self._parameters.setdefault("bias", None)
         if self._q8 is not None:
             self._q8_of = self._weight_now()
 

@@ -268,6 +268,7 @@ def test_refusals(uf):
             (lambda: step([x, x], [y(), y()], [y(), y()], [y(), y()]), "twice"),
             (lambda: step([x], [y()], [x], [y()]), "twice"),
             (lambda: step([x], [y()], [y()], [y()], copies=[x]), "twice"),
+            (lambda: step([x[:300], x[299:]], [y()[:300], y()[:213]], [y()[:300], y()[:213]], [y()[:300], y()[:213]]), "twice"),
             (lambda: step([x.reshape(16, 32).t()], [y()], [y()], [y()]), "contiguous"),
             (lambda: step([x], [torch.zeros(1024, device="cuda")[::2]], [y()], [y()]), "contiguous"),
             (lambda: step([x], [y()[:511]], [y()], [y()]), "elements"),
@@ -403,3 +404,69 @@ def test_command_line(uf, tmp_path):
         got = main_conv.main(["--dataset", "SYNTHETIC", "--err", "5555", "--epochs", "1", "--iterations", "2", "--synthetic_size", "256", "--optim", name,
                               "--save_dir", str(tmp_path / name), "--load_unit", "2222", "--load_wait", "2222"])
         assert math.isfinite(got["history"][0]["train_loss"])
+
+
+def test_step_on_the_host_is_not_recorded(uf):
+    """its number would be in the graph, the same in every replay"""
+    from geo_amd import network
+    p = torch.ones(10, device="cuda", requires_grad=True)
+    p.grad = torch.ones(10, device="cuda")
+    opt = network.AdamW([p])
+    opt.step()
+    with pytest.raises(RuntimeError, match="capturable"):
+        graph_of(opt.step)
+    torch.cuda.synchronize()
+    assert opt.state[p]["step"] == 1
+
+
+def test_inference_tensors(uf):
+    with torch.inference_mode():
+        x, m, v = (torch.zeros(10, device="cuda") for _ in range(3))
+        uf.adamw_step([x], [torch.ones(10, device="cuda")], [m], [v], 1, 0.1, weight_decay=0.0)
+    assert (x + 0.1).abs().max() < 1e-6
+    with pytest.raises(RuntimeError, match="inference"):
+        uf.adamw_step([x], [torch.ones(10, device="cuda")], [m], [v], 2, 0.1)
+    assert (x + 0.1).abs().max() < 1e-6   # nothing written
+
+
+def test_masters_that_the_optimiser_does_not_have_are_copied_back(uf):
+    from geo_amd import network
+    model = small_model()
+    masters = network.make_param_copies(model)
+    opt = network.AdamW(masters[:2], lr=0.1, weight_decay=0.0)
+    for p in model.parameters():
+        p.grad = torch.full_like(p, 128.0)
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(5.0)   # as a layer's quantisation: the step brings the masters' values back
+    network.apply_update(model, opt, masters)
+    for i, (master, p) in enumerate(zip(masters, model.parameters())):
+        assert torch.equal(master, p) and (master.grad is None)
+    assert sum(bool(opt.state[m]) for m in masters[:2]) == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_goes_through_a_file(uf, bits, tmp_path):
+    from geo_amd import network
+    a, b = small_model(0), small_model(0)
+    first, second = network.AdamW(a.parameters(), state_bits=bits), network.AdamW(b.parameters(), state_bits=bits)
+    run_steps(a, first, 2)
+    b.load_state_dict(a.state_dict())
+    torch.save(first.state_dict(), tmp_path / "state.pt")
+    second.load_state_dict(torch.load(tmp_path / "state.pt", weights_only=True))
+    run_steps(a, first, 2, seed=3)
+    run_steps(b, second, 2, seed=3)
+    assert all(torch.equal(x, y) for x, y in zip(a.parameters(), b.parameters()))
+
+
+def test_several_groups_and_types(uf):
+    """groups of their own rates and states; parameters of several types in one"""
+    from geo_amd import network
+    p = [torch.ones(300, device="cuda", dtype=t, requires_grad=True) for t in (torch.float32, torch.bfloat16, torch.float16, torch.float32)]
+    opt = network.AdamW([dict(params=p[:3], lr=0.5), dict(params=p[3:], lr=0.25, state_bits=8)], weight_decay=0.0)
+    for t in p:
+        t.grad = torch.full_like(t, 0.5)
+    opt.step()
+    for t, want in zip(p, (0.5, 0.5, 0.5, 0.75)):
+        assert (t.float() - want).abs().max() <= 2 ** -8
+    assert opt.state[p[3]]["exp_avg"].dtype == torch.float8_e4m3fn and opt.state[p[1]]["exp_avg"].dtype == torch.float32
