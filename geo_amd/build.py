@@ -5,7 +5,8 @@
 * ``geo_amd/lib/sc_extension_cuda*.so``   - PyTorch module with the reference's GPU op names
 * ``geo_amd/lib/sc_extension*.so``        - PyTorch module with the reference's CPU op name
                                            (runs the same GPU kernels)
-* ``geo_amd/lib/sc_dense*.so``            - PyTorch module of the dense 8-bit layers and the distillation loss
+* ``geo_amd/lib/sc_dense*.so``            - PyTorch module of the dense 8-bit layers, the gated norm, the distillation
+                                           loss and the AdamW step
 """
 from __future__ import annotations
 

@@ -4,7 +4,9 @@
 //   p = p (1 - lr wd) - (m lr / (1 - b1^t)) / (r / sqrt(1 - b2^t) + eps)
 //
 // Everything in fp32, each operation rounded by itself (no fused multiply-add), so that a program of elementary operations has the
-// same bits.  Bound by memory: each element is read and written once.
+// same bits.  Bound by memory, each element is read and written once: 139.6M fp32 masters with bf16 gradients and copies, 3.9 GB, in 764 us
+// (5.1 TB/s), 120M of them with 8-bit states, 1.9 GB, in 370 (5.2 TB/s; decoding, root, quotient and rounding are some 110 instructions an element
+// there, 0.9 of that time by themselves).  15 tensors of 2.1M elements in all with 8-bit states 11.4 us, 12 small ones 5.9.
 //
 // States of 8 bits: m and r as floats of 4 exponent and 3 mantissa bits, times a power of two per block of 256 elements.  The root and
 // not v, which would need twice the exponents.  A power of two, because codes then stay what they are when a

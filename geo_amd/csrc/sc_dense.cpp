@@ -1,4 +1,4 @@
-// PyTorch module `sc_dense`: the dense 8-bit layers, the distillation loss and the AdamW step of libgeo_sc.so on tensors.  Checks, outputs
+// PyTorch module `sc_dense`: the dense 8-bit layers, the gated norm, the distillation loss and the AdamW step of libgeo_sc.so on tensors.  Checks, outputs
 // and workspaces from the caching allocator, launch on PyTorch's current HIP stream.  In C++ because a single
 // token's call is bound by its host time.
 #include "sc_torch_common.h"

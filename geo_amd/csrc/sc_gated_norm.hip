@@ -4,7 +4,9 @@
 //   t = scale residual + gate m;   n2 = t r2,  r2 = 1 / sqrt(mean t^2 + eps);   out = weight n2
 //
 // Per channel: weight, post, scale; gate per channel of a run of consecutive rows (a sample's).  A row's threads hold it in registers from
-// its only read to its only write, with two exchanges between its waves.  Sums and factors in fp32; t is rounded for `total` only.
+// its only read to its only write, with two exchanges between its waves.  8192 x 4096 bf16, a gate per sample: 268 MB in 73 us (3.7 TB/s; 49
+// without post, gate and scale, whose loads stand behind the first exchange; asked for ahead of it, their registers cost more than the
+// wait, 85 - 115).  Sums and factors in fp32; t is rounded for `total` only.
 // Rows of any finite magnitude: where squares pass the range of fp32 they are taken of the row times a power of two.
 //
 // Backward, from g (gradient of out) and h (of t), means over a row:
@@ -491,7 +493,8 @@ __device__ __forceinline__ void load_or_ones(const void* p, int64_t c, int64_t c
 
 // The row and two of the channels' numbers are held as they lie in memory and formed anew on either side of an exchange; gate and post
 // come as their product only, and of their two sums over rows one is kept, sum dt n1 over a run, which post and the run's gate multiply where
-// the run ends.  That leaves two waves on a SIMD with two chunks a thread: 8192 x 4096 in workgroups of 256, two on a compute unit.
+// the run ends.  That leaves two waves on a SIMD with two chunks a thread: 8192 x 4096 in workgroups of 256, two on a compute unit.  402 MB
+// and 25 MB of partial sums in 105 us (4.1 TB/s), joined in 9.
 template <typename T, int ITEMS, int LANES, bool ONCE>
 __global__ __launch_bounds__(512, 2) void k_gated_back(BackArgs a)
 {
