@@ -634,6 +634,12 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
     }
     std::sort(written.begin(), written.end());
     for (size_t i = 1; i < written.size(); ++i) TORCH_CHECK(written[i - 1].second <= written[i].first, "a step writes no memory twice");
+    for (const at::Tensor& g : grads) {   // (one gradient may serve several parameters, but not be written over on the way)
+        const char* begin = (const char*)g.const_data_ptr();
+        const auto above = std::lower_bound(written.begin(), written.end(), begin + g.nbytes(),
+                                            [](const auto& range, const char* end) { return range.first < end; });   // the first range behind it
+        TORCH_CHECK(g.numel() == 0 || above == written.begin() || (above - 1)->second <= begin, "a step writes none of its gradients");
+    }
     TORCH_CHECK(!device_step || calls.size() == 1, "a step that is counted on the GPU takes tensors of the same types");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(first.device());
     at::Tensor workspace;

@@ -586,21 +586,40 @@ struct EpilogueTile {
     }
     enum Way { kWhole, kOverlap, kMasked };
     template <typename Y, Way WAY>
-    __device__ __forceinline__ void rows(const Spot& p, v4i (&sum)[T][T], uint8_t* area, int wave, int lane) const
-    {
-        constexpr int kBatch = B == 256 && sizeof(Y) == 2 ? 4 : 2, kStep = kBatch * kAtOnce;   // (what the registers hold)
-        const int64_t cols = p.a.cols, stride = p.a.y_stride, n = column(p, wave, lane), left = cols - n, m0 = p.m0 + wave % 2 * kCols + lane / kLanes;
-        const int mine = lane / kLanes, piece = lane % kLanes * 2, from = (int)(n - begin(p, wave));
-        const auto ask_residual = [&](Y (&raw)[kBatch][kChunk], int r) {
-            if (!e.residual || (WAY == kMasked && left <= 0)) return;
+    struct Batch {   // of rows: what the registers hold, and in the rarer ways less code
+        static constexpr int kRows = B == 256 && sizeof(Y) == 2 && WAY == kWhole ? 4 : 2, kStep = kRows * kAtOnce, kWords = kChunk * (int)sizeof(Y) / 4;
+        static __device__ __forceinline__ float element(const uint32_t (&words)[kWords], int j)
+        {
+            if constexpr (sizeof(Y) == 4) return __uint_as_float(words[j]);
+            else return (float)__builtin_bit_cast(Y, (uint16_t)(words[j / 2] >> (16 * (j & 1))));
+        }
+        // the residual from row m on, as it lies in memory
+        static __device__ __forceinline__ void ask(const Spot& p, const Epilogue& e, int64_t m, int64_t n, uint32_t (&words)[16])
+        {
+            if (!e.residual) return;
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int64_t m = m0 + r + i * kAtOnce;
-                const Y* row = (const Y*)e.residual + (m < p.a.rows ? m : p.a.rows - 1) * e.residual_stride;   // (behind the last row that row once more)
-                if constexpr (WAY == kMasked) fetch_chunk<false>(row, n, cols, raw[i]);
-                else fetch_whole<false>(row + n, raw[i]);
+            for (int i = 0; i < kRows; ++i) {
+                const int64_t mine = m + i * kAtOnce;
+                const Y* row = (const Y*)e.residual + (mine < p.a.rows ? mine : p.a.rows - 1) * e.residual_stride;   // (behind the last row that row once more)
+                if constexpr (WAY == kMasked) {   // (and behind the last column that one)
+                    Y one[kChunk];
+#pragma unroll
+                    for (int j = 0; j < kChunk; ++j) one[j] = row[n + j < p.a.cols ? n + j : p.a.cols - 1];
+                    __builtin_memcpy(words + i * kWords, one, sizeof one);
+                } else {
+                    __builtin_memcpy(words + i * kWords, row + n, kWords * 4);
+                }
             }
-        };
+        }
+    };
+    // What is written out of `area`: ROWS rows from `first` of the wave's on.  `ahead`: the residual of the first batch.
+    template <typename Y, Way WAY>
+    __device__ __forceinline__ void rows(const Spot& p, const uint8_t* area, int wave, int lane, int first, uint32_t (&ahead)[16]) const
+    {
+        typedef Batch<Y, WAY> Of;
+        constexpr int kBatch = Of::kRows, kStep = Of::kStep;
+        const int64_t stride = p.a.y_stride, n = column(p, wave, lane), left = p.a.cols - n, m0 = p.m0 + wave % 2 * kCols + first + lane / kLanes;
+        const int mine = lane / kLanes, piece = lane % kLanes * 2, from = (int)(n - begin(p, wave));
         const auto ask_sums = [&](float (&v)[kBatch][kChunk], int r) {
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
@@ -617,66 +636,89 @@ struct EpilogueTile {
                 }
             }
         };
-        Y residual_ahead[kBatch][kChunk] = {};
         float sums_ahead[kBatch][kChunk];
-        ask_residual(residual_ahead, 0);
+        ask_sums(sums_ahead, 0);
         int64_t at = m0 * stride + n;
-#pragma unroll
-        for (int first = 0; first < kCols; first += ROWS) {
-#pragma unroll
-            for (int i = 0; i < ROWS / 16; ++i)
-#pragma unroll
-                for (int j = 0; j < T; ++j) {
-                    const int row = i * 16 + (lane & 15), to = j * 4 + (lane >> 4);
-                    v4i s = sum[j][first / 16 + i];
-                    asm volatile("" : "+v"(s));   // (out of its accumulation registers here)
-                    float v[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs[first / 16 + i];
-                    __builtin_memcpy(area + (row * kPieces + (to ^ (row & kMix))) * 16, v, 16);
-                }
-            __builtin_amdgcn_wave_barrier();
-            ask_sums(sums_ahead, 0);
 #pragma unroll 1
-            for (int r = 0; r < ROWS; r += kStep) {
-                Y residual[kBatch][kChunk];
-                float z[kBatch][kChunk];
-                __builtin_memcpy(residual, residual_ahead, sizeof residual);
-                __builtin_memcpy(z, sums_ahead, sizeof z);
-                ask_sums(sums_ahead, r + kStep);   // (behind the last ones the first once more)
-                ask_residual(residual_ahead, first + r + kStep);
+        for (int r = 0; r < ROWS; r += kStep) {
+            uint32_t residual[kBatch][Of::kWords];
+            float z[kBatch][kChunk];
+            __builtin_memcpy(residual, ahead, sizeof residual);
+            __builtin_memcpy(z, sums_ahead, sizeof z);
+            ask_sums(sums_ahead, r + kStep);   // (behind the last ones the first once more)
+            if (r + kStep < ROWS) Of::ask(p, e, m0 + r + kStep, n, ahead);
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i, at += kAtOnce * stride) {
-                    float d[kChunk];
+            for (int i = 0; i < kBatch; ++i, at += kAtOnce * stride) {
+                float d[kChunk];
 #pragma unroll
-                    for (int j = 0; j < kChunk; ++j) z[i][j] = z[i][j] * ws[j] + bias[j];
-                    activate(e.activation, z[i], d);
-                    if (m0 + first + r + i * kAtOnce >= p.a.rows || (WAY == kMasked && left <= 0)) continue;
-                    const int64_t there = WAY == kMasked ? left : kChunk;
-                    if (e.slope) store_slope(e, at, there, d);
-                    if (e.residual) {
+                for (int j = 0; j < kChunk; ++j) z[i][j] = z[i][j] * ws[j] + bias[j];
+                activate(e.activation, z[i], d);
+                if (m0 + r + i * kAtOnce >= p.a.rows || (WAY == kMasked && left <= 0)) continue;
+                const int64_t there = WAY == kMasked ? left : kChunk;
+                if (e.slope) store_slope(e, at, there, d);
+                if (e.residual) {
 #pragma unroll
-                        for (int j = 0; j < kChunk; ++j) z[i][j] += (float)residual[i][j];
-                    }
-                    store_columns((Y*)p.a.y + at, there, z[i]);
+                    for (int j = 0; j < kChunk; ++j) z[i][j] += Of::element(residual[i], j);
                 }
+                store_columns((Y*)p.a.y + at, there, z[i]);
             }
-            __builtin_amdgcn_wave_barrier();
         }
     }
-    template <typename Y>
-    __device__ __forceinline__ void rows(const Spot& p, v4i (&sum)[T][T], uint8_t* area, int wave, int lane) const
+    // ROWS of the wave's rows, from FIRST on, into `area`
+    template <int FIRST>
+    __device__ __forceinline__ void put(v4i (&sum)[T][T], uint8_t* area, int lane) const
     {
-        const int64_t there = p.a.cols - begin(p, wave);
-        if (there >= kCols) rows<Y, kWhole>(p, sum, area, wave, lane);
-        else if (there >= kChunk) rows<Y, kOverlap>(p, sum, area, wave, lane);
-        else if (there > 0) rows<Y, kMasked>(p, sum, area, wave, lane);
+#pragma unroll
+        for (int i = 0; i < ROWS / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < T; ++j) {
+                const int row = i * 16 + (lane & 15), to = j * 4 + (lane >> 4);
+                v4i s = sum[j][FIRST / 16 + i];
+                asm volatile("" : "+v"(s));   // (out of its accumulation registers here)
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = (float)s[r] * xs[FIRST / 16 + i];
+                __builtin_memcpy(area + (row * kPieces + (to ^ (row & kMix))) * 16, v, 16);
+            }
     }
+    // A loop over the shares of ROWS rows, with the types and ways inside it: each of them has its code once, and no branch of a kernel has to
+    // go further than an instruction can say (128 KB).
     __device__ __forceinline__ void finish(const Spot& p, v4i (&sum)[T][T], uint8_t* area, int wave, int lane) const
     {
-        if (p.a.dtype == GEO_SC_F32) rows<f32>(p, sum, area, wave, lane);
-        else if (p.a.dtype == GEO_SC_BF16) rows<bf16>(p, sum, area, wave, lane);
-        else rows<f16>(p, sum, area, wave, lane);
+        const int64_t there = p.a.cols - begin(p, wave), n = column(p, wave, lane), m0 = p.m0 + wave % 2 * kCols + lane / kLanes;
+        if (there <= 0) return;
+        const auto of_kind = [&](auto work) {
+            const auto of_way = [&](auto y) {
+                if (there >= kCols) work(y, std::integral_constant<Way, kWhole>());
+                else if (there >= kChunk) work(y, std::integral_constant<Way, kOverlap>());
+                else work(y, std::integral_constant<Way, kMasked>());
+            };
+            if (p.a.dtype == GEO_SC_F32) of_way(f32());
+            else if (p.a.dtype == GEO_SC_BF16) of_way(bf16());
+            else of_way(f16());
+        };
+        uint32_t ahead[16] = {};
+        const auto ask_first = [&](int first) {
+            of_kind([&](auto y, auto way) { Batch<decltype(y), way()>::ask(p, e, m0 + first, n, ahead); });
+        };
+        ask_first(0);
+        put<0>(sum, area, lane);   // (in front of the loop: their registers are free from here on)
+#pragma unroll 1
+        for (int first = 0;;) {
+            __builtin_amdgcn_wave_barrier();
+            of_kind([&](auto y, auto way) { rows<decltype(y), way()>(p, area, wave, lane, first, ahead); });
+            __builtin_amdgcn_wave_barrier();
+            first += ROWS;
+            if (first >= kCols) break;
+            ask_first(first);
+            static_assert(kCols <= 2 * ROWS || kCols == 4 * ROWS, "");
+            if constexpr (kCols > ROWS)
+                if (first == ROWS) put<ROWS>(sum, area, lane);
+            if constexpr (kCols > 2 * ROWS) {
+                if (first == 2 * ROWS) put<2 * ROWS>(sum, area, lane);
+                if (first == 3 * ROWS) put<3 * ROWS>(sum, area, lane);
+            }
+        }
     }
 };
 

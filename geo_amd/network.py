@@ -279,6 +279,13 @@ class PatchMLP_q8(nn.Module):
         self.down = nn.ModuleList(utils_class.Linear_Q8(hidden, width, bias=bias) for _ in range(depth))
         self.head = utils_class.NormLinear_Q8(width, num_classes)
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "gated" not in state:   # pickled when the relu was the network's own
+            self.gated = False
+            for up in self.up:
+                up.activation = "relu"
+
     def prepare(self):
         """Round all weights for inference (``Linear_Q8.prepare``)."""
         for layer in self.modules():
@@ -309,15 +316,20 @@ class AdamW(torch.optim.Optimizer):
     8.  Parameters are contiguous GPU tensors of float32, bfloat16 or float16; gradients of any of these types.
 
     ``capturable=True`` counts the steps on the GPU, for steps that are recorded into a graph (``GraphedTrainStep``), where the learning rate
-    is recorded with them.  ``apply_update`` hands it the unscaling of the gradients and the copies into the parameters as well."""
+    is recorded with them; parameters whose first step was the same are counted together, also in a step that has no gradient for one of
+    them.  ``apply_update`` hands it the unscaling of the gradients and the copies into the parameters as well."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, capturable=False):
-        if state_bits not in (8, 32):
-            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
-        if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas)):
-            raise ValueError("lr, eps and weight_decay must not be negative, betas in [0, 1)")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       capturable=capturable))
+
+    def add_param_group(self, param_group):
+        options = {**self.defaults, **param_group}
+        if options["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {options['state_bits']}")
+        if not (options["lr"] >= 0 and options["eps"] >= 0 and options["weight_decay"] >= 0 and all(0 <= b < 1 for b in options["betas"])):
+            raise ValueError("lr, eps and weight_decay must not be negative, betas in [0, 1)")
+        super().add_param_group(param_group)
 
     def _fresh(self, p, group, step):
         like = lambda n, dtype: torch.zeros(n, dtype=dtype, device=p.device)   # noqa: E731
@@ -339,11 +351,12 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         from . import utils_functional as uf
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing() and not all(g["capturable"] for g in self.param_groups):
+        recorded = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        if recorded and not all(g["capturable"] for g in self.param_groups):
             raise RuntimeError("AdamW(capturable=True) is the one whose steps can be recorded: others count them on the host")
         for group in self.param_groups:
             # parameters that have made the same number of steps; those counted on the GPU, that are counted together
-            rows, counter = {}, None
+            rows, counters = {}, {}
             for p in group["params"]:
                 g = (grads or {}).get(p, p.grad)
                 if g is None:
@@ -352,12 +365,12 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("AdamW takes no sparse gradients")
                 state = self.state[p]
                 if not state:
-                    if group["capturable"]:
-                        counter = torch.zeros((), dtype=torch.int64, device=p.device) if counter is None else counter
-                    state.update(self._fresh(p, group, counter if group["capturable"] else 0))
-                if not group["capturable"]:
-                    state["step"] += 1
-                step = state["step"]
+                    if recorded:   # (every replay would begin anew)
+                        raise RuntimeError("the first step of a parameter, which makes its states, cannot be recorded: do one before")
+                    if group["capturable"] and p.device not in counters:
+                        counters[p.device] = torch.zeros((), dtype=torch.int64, device=p.device)
+                    state.update(self._fresh(p, group, counters[p.device] if group["capturable"] else 0))
+                step = state["step"] if group["capturable"] else state["step"] + 1
                 copy = None if copies is None else copies.get(p)
                 # one call per device, number of steps and set of types (those that are not counted on the GPU may mix them)
                 types = (p.dtype, g.dtype) if group["capturable"] else None
@@ -374,6 +387,9 @@ class AdamW(torch.optim.Optimizer):
                               if group["state_bits"] == 8 else None,
                               copies=None if row[0][3] is None else [c for _, _, _, c in row],
                               clamped=None if clamped is None else [clamped.get(p) for p, _, _, _ in row], bounds=bounds)
+                if not group["capturable"]:
+                    for state in states:
+                        state["step"] = step
         return loss
 
     def load_state_dict(self, state_dict):

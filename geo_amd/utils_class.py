@@ -223,9 +223,10 @@ def sc_conv_block(conv, bn, input, *, err=7, forward="1d_bin", z_unit=8, load_un
 
 class Linear_Q8(nn.Module):
     """Linear layer whose operands are rounded to 8-bit rows (``utils_functional.linear_q8``): the exact counterpart
-    of an SC layer's product; with ``bias``, ``activation`` (None, "relu", "gelu", "silu") and a residual in the product's kernel.  In training the weight is rounded on every call and the gradients pass straight through.  For
-    inference ``prepare()`` rounds it once, and calls without gradients take that result until ``train()``, ``load_state_dict`` or
-    a move to another device or type drops it; ``eval()`` keeps it.  A weight that has been written to since is said so in a warning."""
+    of an SC layer's product; with ``bias``, ``activation`` (None, "relu", "gelu", "silu") and a residual in the product's kernel.  In
+    training the weight is rounded on every call and the gradients pass straight through.  For inference ``prepare()`` rounds it once, and
+    calls without gradients take that result until ``train()``, ``load_state_dict`` or a move to another device or type drops it; ``eval()``
+    keeps it.  A weight that has been written to since is said so in a warning."""
 
     def __init__(self, in_features, out_features, bias=False, activation=None):
         super().__init__()

@@ -537,7 +537,8 @@ GEO_SC_API int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64
  *   bias, residual   NULL: none; `cols` elements of bias_dtype, (rows, cols) of y's dtype with residual_stride between its rows
  *   slope            NULL, or (rows, cols), without gaps, for the backward: act'(z) in slope_dtype, GEO_SC_F16, GEO_SC_F32 or, of a
  *                    relu (or no activation), GEO_SC_U8
- * y and slope overlap nothing that is read.  Workspace: geo_sc_matmul_q8_workspace_size.
+ * y and slope overlap nothing that is read.  Workspace: geo_sc_matmul_q8_workspace_size.  Kernels are those of geo_sc_matmul_q8_plan, but
+ * that rows of w of less than 4096 bytes (with 17 to 64 rows of x, 2560 to 1536) go to GEO_SC_Q8_FEW_ROWS where the product alone streams.
  * Backward, from g (gradient of y): with dz = g slope (0 where the slope is 0; slope NULL: dz = g), dx and dw as
  * geo_sc_matmul_q8_backward has them from dz, dbias[n] = sum_m dz[m][n] in an order that does not change from run to run; each of the three may be
  * NULL.  The residual's gradient is g.

@@ -73,3 +73,5 @@ def test_optimiser_refuses():
     for bad in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(weight_decay=-0.1)):
         with pytest.raises(ValueError):
             network.AdamW(p, **bad)
+        with pytest.raises(ValueError):
+            network.AdamW([dict(params=p, **bad)])

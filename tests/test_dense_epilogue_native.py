@@ -84,3 +84,17 @@ def test_distances_around_the_products_of_the_tile_kernels(tmp_path):
         products, bad = violations(code)
         assert products >= 8, name
         assert not bad, (name, [(code[i], code[j]) for i, j in bad[:3]])
+
+
+def test_teacher_pickled_before_its_layers_had_activations():
+    """the relu was the network's own then"""
+    import copy
+    from geo_amd import network
+    net = network.PatchMLP_q8(width=16, hidden=32, depth=2)
+    del net.__dict__["gated"]
+    for layer in (*net.up, *net.down, net.head, net.embed):
+        del layer.__dict__["activation"]
+        del layer._parameters["bias"]
+    again = copy.deepcopy(net)
+    assert not again.gated and [up.activation for up in again.up] == ["relu", "relu"]
+    assert all(layer.activation is None and layer.bias is None for layer in (*again.down, again.head, again.embed))

@@ -419,6 +419,46 @@ def test_step_on_the_host_is_not_recorded(uf):
     assert opt.state[p]["step"] == 1
 
 
+def test_first_step_is_not_recorded(uf):
+    """it makes the states, which every replay would clear"""
+    from geo_amd import network
+    p = torch.ones(10, device="cuda", requires_grad=True)
+    p.grad = torch.ones(10, device="cuda")
+    opt = network.AdamW([p], capturable=True)
+    with pytest.raises(RuntimeError, match="first step"):
+        graph_of(opt.step)
+    torch.cuda.synchronize()
+    opt.step()
+    graph = graph_of(opt.step)   # (records a step, does not make it)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert opt.state[p]["step"].item() == 4
+
+
+def test_refused_step_is_not_counted(uf):
+    from geo_amd import network
+    p = torch.ones(10, device="cuda", requires_grad=True)
+    p.grad = torch.ones(10, device="cuda")
+    opt = network.AdamW([p])
+    opt.step()
+    with pytest.raises(RuntimeError, match="copies"):
+        opt.step(copies={p: torch.ones(9, device="cuda")})
+    assert opt.state[p]["step"] == 1
+
+
+def test_gradients_that_would_be_written_over(uf):
+    memory = torch.ones(64, device="cuda")
+    m, v = torch.zeros(16, device="cuda"), torch.zeros(16, device="cuda")
+    for begin in (0, 8, 15):
+        with pytest.raises(RuntimeError, match="none of its gradients"):
+            uf.adamw_step([memory[15:31]], [memory[begin:begin + 16]], [m], [v], 1, 0.1)
+    for begin in (31, 32, 48):   # beside the parameter, and one gradient for two
+        uf.adamw_step([memory[15:31]], [memory[begin:begin + 16]], [m], [v], 1, 0.1)
+    other = [torch.zeros(16, device="cuda") for _ in range(5)]
+    uf.adamw_step([memory[15:31], other[0]], [memory[32:48]] * 2, [m, other[1]], [v, other[2]], 1, 0.1)
+
+
 def test_inference_tensors(uf):
     with torch.inference_mode():
         x, m, v = (torch.zeros(10, device="cuda") for _ in range(3))
