@@ -210,7 +210,7 @@ __device__ __forceinline__ void activate(int kind, float (&z)[N], float (&d)[N])
     if (kind == GEO_SC_ACT_RELU) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
-            d[j] = z[j] > 0.f ? 1.f : 0.f;
+            d[j] = z[j] <= 0.f ? 0.f : 1.f;   // (what comes back to a NaN goes on, as behind torch's relu)
             z[j] = z[j] < 0.f ? 0.f : z[j];
         }
     } else if (kind == GEO_SC_ACT_GELU) {
