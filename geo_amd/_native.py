@@ -50,7 +50,7 @@ class GatedNormDesc(ctypes.Structure):
     _fields_ = [("struct_bytes", ctypes.c_size_t)] + \
                [(n, ctypes.c_void_p) for n in ("x", "residual", "weight", "post_weight", "gate", "residual_scale")] + \
                [(n, ctypes.c_int64) for n in ("rows", "cols", "x_stride", "residual_stride", "rows_per_gate")] + \
-               [("eps", ctypes.c_float), ("dtype", ctypes.c_int32)]
+               [("eps", ctypes.c_float), ("dtype", ctypes.c_int32), ("rstd", ctypes.c_void_p)]
 
 
 class Q8Epilogue(ctypes.Structure):

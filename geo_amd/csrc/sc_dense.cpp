@@ -267,22 +267,26 @@ std::tuple<at::Tensor, at::Tensor, MaybeTensor> gated_norm(const at::Tensor& x, 
     return {out, total, rstd};
 }
 
-// (q, scale, total, values)
-std::tuple<at::Tensor, at::Tensor, at::Tensor, MaybeTensor> gated_norm_q8(const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight,
-                                                                          const MaybeTensor& post, const MaybeTensor& gate, const MaybeTensor& scale,
-                                                                          double eps, std::optional<at::ScalarType> values_type)
+// (q, scale, total, values, rstd)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, MaybeTensor, MaybeTensor> gated_norm_q8(const at::Tensor& x, const at::Tensor& residual,
+                                                                                     const at::Tensor& weight, const MaybeTensor& post,
+                                                                                     const MaybeTensor& gate, const MaybeTensor& scale, double eps,
+                                                                                     std::optional<at::ScalarType> values_type, bool for_backward)
 {
     not_recorded();
-    const Gated g = as_gated(x, residual, weight, post, gate, scale, eps);
+    Gated g = as_gated(x, residual, weight, post, gate, scale, eps);
     const int vtype = values_type ? dtype_of(*values_type, "values") : 0;
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     const at::Tensor q = empty_q(x.sizes(), x.options()), q_scale = row_scalars(x), total = at::empty(x.sizes(), x.options());
     MaybeTensor values;
     if (values_type) values = at::empty(x.sizes(), x.options().dtype(*values_type));
+    MaybeTensor rstd;
+    if (for_backward) rstd = at::empty({g.x.rows, 2}, x.options().dtype(at::kFloat));
+    g.desc.rstd = (float*)data_of(rstd);
     check_status(geo_sc_gated_norm_q8(&g.desc, q.data_ptr<int8_t>(), (g.x.cols + 15) / 16 * 16, q_scale.data_ptr<float>(), total.data_ptr(),
                                       data_of(values), vtype, stream_of(x)),
                  "gated_norm_q8");
-    return {q, q_scale, total, values};
+    return {q, q_scale, total, values, rstd};
 }
 
 struct GatedGradients {
@@ -812,6 +816,16 @@ struct NormLinearQ8 : torch::autograd::Function<NormLinearQ8> {
     }
 };
 
+// Which of weight (at `at` of the inputs) and of `around`, which follow each other, the gradients are wanted of: inputs are counted
+// without those that are None.
+std::array<bool, 4> wanted_of(AutogradContext* ctx, size_t weight, size_t at, const at::Tensor* around)
+{
+    std::array<bool, 4> wanted = {ctx->needs_input_grad(weight), false, false, false};
+    for (size_t i = 0; i < 3; ++i)
+        if (around[i].defined()) wanted[1 + i] = ctx->needs_input_grad(at++);
+    return wanted;
+}
+
 // (out, total)
 struct GatedNorm : torch::autograd::Function<GatedNorm> {
     static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight,
@@ -826,14 +840,55 @@ struct GatedNorm : torch::autograd::Function<GatedNorm> {
     static variable_list backward(AutogradContext* ctx, variable_list grads)
     {
         const auto s = ctx->get_saved_variables();
-        // (inputs are counted without those that are None)
-        std::array<bool, 4> wanted = {ctx->needs_input_grad(2), false, false, false};
-        for (size_t i = 0, at = 3; i < 3; ++i)
-            if (s[3 + i].defined()) wanted[1 + i] = ctx->needs_input_grad(at++);
+        const auto wanted = wanted_of(ctx, 2, 3, &s[3]);
         const GatedGradients d = gated_norm_backward(grads[0], grads[1], s[0], s[1], s[2], maybe(s[3]), maybe(s[4]), maybe(s[5]),
                                                      ctx->saved_data["eps"].toDouble(), s[6], wanted);
         return {ctx->needs_input_grad(0) ? d.x : at::Tensor(), ctx->needs_input_grad(1) ? d.residual : at::Tensor(), undefined_or(d.weight),
                 undefined_or(d.post), undefined_or(d.gate), undefined_or(d.scale), at::Tensor()};
+    }
+};
+
+// The gated norm with 8-bit output and the product: (y, total)
+struct GatedNormLinearQ8 : torch::autograd::Function<GatedNormLinearQ8> {
+    static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& residual, const at::Tensor& gain, const at::Tensor& weight,
+                                 const MaybeTensor& post, const MaybeTensor& gate, const MaybeTensor& scale, const MaybeTensor& bias, double eps,
+                                 int64_t activation, bool keep_slope)
+    {
+        const auto [q, q_scale, total, none, rstd] = gated_norm_q8(x, residual, gain, post, gate, scale, eps, std::nullopt, true);
+        const auto [wq, wscale, none2] = quantize_rows(weight, std::nullopt);
+        ctx->set_materialize_grads(false);
+        After after;
+        after.bias = bias;
+        after.activation = (int)activation;
+        after.keep_slope = keep_slope;
+        const at::Tensor y = matmul_q8(q, q_scale, wq, wscale, x.scalar_type(), after);
+        ctx->save_for_backward({q, q_scale, wq, wscale, x, residual, gain, undefined_or(post), undefined_or(gate), undefined_or(scale), *rstd, after.slope});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["w"] = weight.scalar_type();
+        if (bias) ctx->saved_data["bias"] = bias->scalar_type();
+        return {y, total};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads)
+    {
+        const auto s = ctx->get_saved_variables();
+        const size_t at_bias = 4 + s[7].defined() + s[8].defined() + s[9].defined();
+        const auto wanted = wanted_of(ctx, 2, 4, &s[7]);
+        const bool through = ctx->needs_input_grad(0) || ctx->needs_input_grad(1) || wanted[0] || wanted[1] || wanted[2] || wanted[3];
+        ProductGradients d;
+        if (grads[0].defined()) {
+            std::optional<at::ScalarType> x, w, bias;
+            if (through) x = s[4].scalar_type();
+            if (ctx->needs_input_grad(3)) w = ctx->saved_data["w"].toScalarType();
+            if (ctx->saved_data.count("bias") && ctx->needs_input_grad(at_bias)) bias = ctx->saved_data["bias"].toScalarType();
+            if (x || w || bias) d = matmul_q8_backward(grads[0], s[0], s[1], s[2], s[3], x, w, s[11], bias);
+        }
+        GatedGradients n;
+        if (through)
+            n = gated_norm_backward(undefined_or(d.x), grads[1], s[4], s[5], s[6], maybe(s[7]), maybe(s[8]), maybe(s[9]),
+                                    ctx->saved_data["eps"].toDouble(), s[10], wanted);
+        return {ctx->needs_input_grad(0) ? n.x : at::Tensor(), ctx->needs_input_grad(1) ? n.residual : at::Tensor(), undefined_or(n.weight),
+                undefined_or(d.w), undefined_or(n.post), undefined_or(n.gate), undefined_or(n.scale), undefined_or(d.bias), at::Tensor(),
+                at::Tensor(), at::Tensor()};
     }
 };
 
@@ -905,7 +960,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
         const auto [out, total, none] = gated_norm(x, residual, weight, post, gate, scale, eps, false);
         return std::make_tuple(out, total);
     }, "norm behind a block, gate, scaled residual and the next norm: (out, total)");
-    m.def("gated_norm_q8", &gated_norm_q8, "the same with 8-bit output: (q, scale, total, values or None)");
+    m.def("gated_norm_q8", [](const at::Tensor& x, const at::Tensor& residual, const at::Tensor& weight, const MaybeTensor& post, const MaybeTensor& gate,
+                              const MaybeTensor& scale, double eps, std::optional<at::ScalarType> values) {
+        const auto [q, q_scale, total, v, none] = gated_norm_q8(x, residual, weight, post, gate, scale, eps, values, false);
+        return std::make_tuple(q, q_scale, total, v);
+    }, "the same with 8-bit output: (q, scale, total, values or None)");
+    m.def("gated_norm_linear_q8", [](const at::Tensor& x, const at::Tensor& residual, const at::Tensor& gain, const at::Tensor& weight, const MaybeTensor& post,
+                                     const MaybeTensor& gate, const MaybeTensor& scale, double eps, const MaybeTensor& bias,
+                                     const std::optional<std::string>& activation) {
+        const int kind = activation_of(activation);
+        const auto wants = [](const MaybeTensor& t) { return t && t->requires_grad(); };
+        const bool keep = kind != GEO_SC_ACT_NONE && at::GradMode::is_enabled() &&
+                          (x.requires_grad() || residual.requires_grad() || gain.requires_grad() || weight.requires_grad() || wants(post) ||
+                           wants(gate) || wants(scale) || wants(bias));
+        const variable_list out = GatedNormLinearQ8::apply(x, residual, gain, weight, post, gate, scale, bias, eps, kind, keep);
+        return std::make_tuple(out[0], out[1]);
+    }, "the gated norm with 8-bit output and the product: (y, total)");
     m.def("adamw_step", &adamw_step, "one AdamW step on lists of tensors");
     m.def("distill_topk", [](const at::Tensor& logits, const at::Tensor& top_logits, const at::Tensor& top_index, double temperature, int64_t reduction) {
         return DistillTopK::apply(logits, top_logits, top_index, temperature, reduction);

@@ -15,6 +15,8 @@
 //   e = dt gate,  dpost = sum of e n1,  s = e post,  dx = r1 (s - n1 mean(s n1))   (without the norm dx = e)
 // n1 and n2 are at most the root of the columns: nothing but the gradients themselves can pass fp32's range.  t is formed again, as
 // its rounding would show in the sums over rows.
+#include <stddef.h>
+
 #include <type_traits>
 
 #include "sc_dense.h"
@@ -867,8 +869,8 @@ int run_back(BackArgs a, int dtype, hipStream_t s)
 // what a description must have, whichever call it is for
 int check(const geo_sc_gated_norm_desc* d, NormArgs* n)
 {
-    if (!d || d->struct_bytes != sizeof *d || !dtype_known(d->dtype) || d->rows < 0 || d->cols < 1 || d->rows > 0x7fffffff || d->cols > 0x7fffffff ||
-        d->x_stride < 0 || d->residual_stride < 0 || !(d->eps >= 0.f) || (d->gate && (d->rows_per_gate < 1 || d->rows % d->rows_per_gate)))
+    if (!d || (d->struct_bytes != sizeof *d && d->struct_bytes != offsetof(geo_sc_gated_norm_desc, rstd)) || !dtype_known(d->dtype) ||
+        d->rows < 0 || d->cols < 1 || d->rows > 0x7fffffff || d->cols > 0x7fffffff || d->x_stride < 0 || d->residual_stride < 0 || !(d->eps >= 0.f) || (d->gate && (d->rows_per_gate < 1 || d->rows % d->rows_per_gate)))
         return GEO_SC_ERR_INVALID_ARGUMENT;
     if (d->rows && (!d->x || !d->residual || !d->weight)) return GEO_SC_ERR_INVALID_ARGUMENT;
     *n = {};
@@ -926,6 +928,7 @@ int geo_sc_gated_norm_q8(const geo_sc_gated_norm_desc* desc, int8_t* q, int64_t 
     n.q = q;
     n.q_stride = q_stride;
     n.q_scale = scale;
+    if (desc->struct_bytes == sizeof *desc) n.rstd = desc->rstd;
     n.values = values;
     n.values_dtype = values_dtype;
     return run_forward<true>(n, desc->dtype, (hipStream_t)stream);

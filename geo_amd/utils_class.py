@@ -310,7 +310,7 @@ class NormLinear_Q8(Linear_Q8):
 
 class GatedNormLinear_Q8(NormLinear_Q8):
     """``NormLinear_Q8`` behind a block whose output ``x`` is normed and gated before it joins the stream ``residual``
-    (``utils_functional.gated_norm``, its 8-bit form once the weight is prepared), then the product.  Parameters: ``gain`` (in front of
+    (``utils_functional.gated_norm_linear_q8``; from a prepared weight the same bits), then the product.  Parameters: ``gain`` (in front of
     the product), ``post_gain`` and ``gate`` (of the block's output, per channel), ``residual_scale``.  Returns (y, the new stream)."""
 
     def __init__(self, in_features, out_features, eps=1e-6, bias=False, activation=None, gate=1.0):
@@ -324,7 +324,6 @@ class GatedNormLinear_Q8(NormLinear_Q8):
         around = dict(post_weight=self.post_gain, gate=self.gate, residual_scale=self.residual_scale, eps=self.eps)
         epilogue = dict(bias=self.bias, activation=self.activation)
         if weight is None:
-            normed, total = utils_functional.gated_norm(x, residual, self.gain, **around)
-            return utils_functional.linear_q8(normed, self.weight, **epilogue), total
+            return utils_functional.gated_norm_linear_q8(x, residual, self.gain, self.weight, **around, **epilogue)
         q, scale, total, _ = utils_functional.gated_norm_q8(x, residual, self.gain, **around)
         return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype, **epilogue), total

@@ -277,11 +277,18 @@ def gated_norm(x, residual, weight, post_weight=None, gate=None, residual_scale=
 
 
 def gated_norm_q8(x, residual, weight, post_weight=None, gate=None, residual_scale=None, eps=1e-6, values=None):
-    """``gated_norm`` with its ``out`` as ``quantize_rows`` has it, for the 8-bit products of a served network: (q, scale, total,
-    values), ``values`` None unless a type is named.  No gradients: train with ``gated_norm`` and ``linear_q8``."""
+    """``gated_norm`` with its ``out``, before it is rounded to a type, as ``quantize_rows`` has it, for the 8-bit products of a served network: (q,
+    scale, total, values), ``values`` None unless a type is named.  No gradients: train with ``gated_norm_linear_q8``."""
     if _wants_grad(x, residual, weight, post_weight, gate, residual_scale):
         raise ValueError("gated_norm_q8 has no gradients: take gated_norm (or torch.no_grad())")
     return _dense().gated_norm_q8(x, residual, weight, post_weight, gate, residual_scale, eps, values)
+
+
+def gated_norm_linear_q8(x, residual, gain, weight, post_weight=None, gate=None, residual_scale=None, eps=1e-6, bias=None, activation=None):
+    """``gated_norm_q8`` (its weight is ``gain``) and the product of its rows with ``weight`` rounded to 8-bit rows, with bias and activation
+    (``matmul_q8``): (y, total), differentiable (once) in all tensors.  The norm's output goes from float32 to 8 bits, as it does in a served
+    network: both give the same bits."""
+    return _dense().gated_norm_linear_q8(x, residual, gain, weight, post_weight, gate, residual_scale, eps, bias, activation)
 
 
 # ---------------------------------------------------------------- optimiser step

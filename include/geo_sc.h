@@ -591,7 +591,9 @@ GEO_SC_API int geo_sc_distill_topk_backward(const float* grad, int reduction, co
  * gate is (rows / rows_per_gate, cols): one for each run of rows_per_gate consecutive rows, which must divide rows.  post_weight, gate and
  * residual_scale may be NULL.  All are of `dtype`.
  * geo_sc_gated_norm: out and total, (rows, cols) of dtype; rstd NULL, or rows * 2 floats for the backward (both norms' factors).
- * geo_sc_gated_norm_q8: instead of out its rows in 8 bits (geo_sc_quantize_rows), values NULL or what they stand for in values_dtype.
+ * geo_sc_gated_norm_q8: instead of out its rows in 8 bits (as geo_sc_quantize_rows has them, of out in fp32, which is not rounded to dtype
+ * on the way), values NULL or what they stand for in values_dtype; desc's rstd is for it alone: NULL, or as above.  (A caller built without that
+ * field passes the smaller struct_bytes.)
  * Backward, from the gradients of out and of total (NULL: none), both of dtype: dx and dresidual (rows, cols), and dweight,
  * dpost, dscale (cols) and dgate (of the gate's shape), each NULL where it is not wanted, summed over rows in an order that does not
  * change from run to run.  Workspace, 4-byte aligned: geo_sc_gated_norm_backward_workspace_size.
@@ -607,6 +609,7 @@ typedef struct geo_sc_gated_norm_desc {
     int64_t rows, cols, x_stride, residual_stride, rows_per_gate;
     float eps;
     int32_t dtype;
+    float* rstd;
 } geo_sc_gated_norm_desc;
 GEO_SC_API int geo_sc_gated_norm(const geo_sc_gated_norm_desc* desc, void* out, void* total, float* rstd, geo_sc_stream_t stream);
 GEO_SC_API int geo_sc_gated_norm_q8(const geo_sc_gated_norm_desc* desc, int8_t* q, int64_t q_stride, float* scale, void* total, void* values,
