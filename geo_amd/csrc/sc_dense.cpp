@@ -43,7 +43,7 @@ void not_recorded()
 {
     TORCH_CHECK(!torch::jit::tracer::isTracing() &&
                     !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
-                "the dense 8-bit layers, the distillation loss and the AdamW step cannot be traced");
+                "the dense 8-bit layers, the gated norm, the distillation loss and the AdamW step cannot be traced");
 }
 
 geo_sc_stream_t stream_of(const at::Tensor& t)
@@ -73,7 +73,7 @@ Rows as_rows(const at::Tensor& t, const char* what)
 struct Once : torch::autograd::Node {
     torch::autograd::variable_list apply(torch::autograd::variable_list&&) override
     {
-        TORCH_CHECK(false, "the dense 8-bit layers and the distillation loss can be differentiated once only");
+        TORCH_CHECK(false, "the dense 8-bit layers, the gated norm and the distillation loss can be differentiated once only");
     }
     std::string name() const override { return "DifferentiableOnce"; }
 };
