@@ -571,6 +571,12 @@ void in_step(const at::Tensor& t, const char* what, const at::Tensor& first, int
         if (t.scalar_type() == type) return;
     TORCH_CHECK(false, what, " must not be ", t.scalar_type());
 }
+// what goes with a parameter element by element
+void beside(const at::Tensor& t, const char* what, const at::Tensor& first, const at::Tensor& param, std::initializer_list<at::ScalarType> types)
+{
+    in_step(t, what, first, param.numel(), types);
+    TORCH_CHECK(t.sizes() == param.sizes(), what, " must have the shape of its parameter, ", param.sizes(), ", got ", t.sizes());
+}
 
 constexpr int64_t kStateBlock = 256;
 
@@ -607,23 +613,23 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
         geo_sc_adamw_tensor t = {};
         t.elements = elements;
         in_step(params[i], "params", first, elements, {at::kFloat, at::kBFloat16, at::kHalf});
-        in_step(grads[i], "grads", first, elements, {at::kFloat, at::kBFloat16, at::kHalf});
+        beside(grads[i], "grads", first, params[i], {at::kFloat, at::kBFloat16, at::kHalf});
         t.param = write(params[i]);
         t.grad = grads[i].const_data_ptr();
         for (const auto& [state, scales, what, codes, scale] : {std::make_tuple(&exp_avg, &avg_scales, "exp_avg", &t.exp_avg, &t.avg_scale),
                                                                 std::make_tuple(&exp_avg_sq, &sq_scales, "exp_avg_sq", &t.exp_avg_sq, &t.sq_scale)}) {
-            in_step((*state)[i], what, first, elements, {eight ? at::kFloat8_e4m3fn : at::kFloat});
+            beside((*state)[i], what, first, params[i], {eight ? at::kFloat8_e4m3fn : at::kFloat});
             *codes = write((*state)[i]);
             if (!eight) continue;
             in_step((**scales)[i], "scales", first, blocks, {at::kFloat8_e8m0fnu});
             *scale = (uint8_t*)write((**scales)[i]);
         }
         if (copies) {
-            in_step((*copies)[i], "copies", first, elements, {at::kFloat, at::kBFloat16, at::kHalf});
+            beside((*copies)[i], "copies", first, params[i], {at::kFloat, at::kBFloat16, at::kHalf});
             t.copy = write((*copies)[i]);
         }
         if (clamped && (*clamped)[i]) {
-            in_step(*(*clamped)[i], "clamped", first, elements, {at::kFloat});
+            beside(*(*clamped)[i], "clamped", first, params[i], {at::kFloat});
             t.clamped = (float*)write(*(*clamped)[i]);
         }
         const Types types = {dtype_of(params[i].scalar_type(), "params"), dtype_of(grads[i].scalar_type(), "grads"),

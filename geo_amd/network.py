@@ -404,7 +404,7 @@ class AdamW(torch.optim.Optimizer):
             for k, v in state_dict["state"][i].items():
                 if k == "step":
                     v = int(v)
-                elif v.dtype != state[k].dtype or v.numel() != state[k].numel():
+                elif v.dtype != state[k].dtype or v.shape != state[k].shape:
                     raise ValueError(f"{k} of a parameter of {tuple(p.shape)} does not fit states of {group['state_bits']} bits")
                 else:
                     v = v.to(p.device, copy=True)

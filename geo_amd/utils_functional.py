@@ -295,8 +295,8 @@ def gated_norm_linear_q8(x, residual, gain, weight, post_weight=None, gate=None,
 
 def adamw_step(params, grads, exp_avg, exp_avg_sq, step, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, grad_scale=1.0, scales=None,
                copies=None, clamped=None, bounds=(-1.0, 0.999)):
-    """One AdamW step on lists of contiguous GPU tensors, in place, in fp32 operations whatever their types: with t = ``step`` and
-    g = ``grads * grad_scale``::
+    """One AdamW step on lists of contiguous GPU tensors (those of a parameter of its shape), in place, in fp32 operations whatever their types: with
+    t = ``step`` and g = ``grads * grad_scale``::
 
         m = beta1 m + (1 - beta1) g;   v = beta2 v + (1 - beta2) g^2
         params = params (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
