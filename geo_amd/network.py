@@ -316,8 +316,12 @@ class AdamW(torch.optim.Optimizer):
     8.  Parameters are contiguous GPU tensors of float32, bfloat16 or float16; gradients of any of these types.
 
     ``capturable=True`` counts the steps on the GPU, for steps that are recorded into a graph (``GraphedTrainStep``), where the learning rate
-    is recorded with them; parameters whose first step was the same are counted together, also in a step that has no gradient for one of
-    them.  ``apply_update`` hands it the unscaling of the gradients and the copies into the parameters as well."""
+    is recorded with them.  Parameters whose first step was the same are counted together until a step has no gradient for some of them:
+    the others are counted apart from there on.  A recorded step cannot part them, nor can any step after one of them all was recorded, whose
+    graph counts them together: both are refused, and a step like it is to be made before.  ``apply_update`` hands it the unscaling of the
+    gradients and the copies into the parameters as well."""
+
+    _in_graph = ()   # counters that recorded steps count
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, capturable=False):
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
@@ -342,6 +346,25 @@ class AdamW(torch.optim.Optimizer):
             state.update(exp_avg=like(p.shape, torch.float32), exp_avg_sq=like(p.shape, torch.float32))
         return state
 
+    def _count_apart(self, group, stepping, recorded):
+        """Of parameters that are counted together and do not all make this step, those that do receive a counter of their own."""
+        together = {}
+        for p in group["params"]:
+            state = self.state.get(p)
+            if state:
+                together.setdefault(id(state["step"]), []).append(p)
+        for params in together.values():
+            those = [p for p in params if id(p) in stepping]
+            if 0 < len(those) < len(params):
+                counter = self.state[those[0]]["step"]
+                if recorded:   # (every replay would part them anew)
+                    raise RuntimeError("a step of some of the parameters that are counted together cannot be recorded: make one like it before")
+                if any(counter is c for c in self._in_graph):
+                    raise RuntimeError("a step of some of the parameters that are counted together, in a recorded step too: make it before that is recorded")
+                counter = counter.clone()
+                for p in those:
+                    self.state[p]["step"] = counter
+
     @torch.no_grad()
     def step(self, closure=None, grad_scale=1.0, grads=None, copies=None, clamped=None, bounds=(-1.0, 0.999)):
         """One step.  ``grads``, ``copies``, ``clamped``: dicts from parameters to tensors; a gradient that is not among them is the
@@ -357,10 +380,10 @@ class AdamW(torch.optim.Optimizer):
         for group in self.param_groups:
             # parameters that have made the same number of steps; those counted on the GPU, that are counted together
             rows, counters = {}, {}
-            for p in group["params"]:
-                g = (grads or {}).get(p, p.grad)
-                if g is None:
-                    continue
+            stepping = [(p, g) for p in group["params"] if (g := (grads or {}).get(p, p.grad)) is not None]
+            if group["capturable"]:
+                self._count_apart(group, {id(p) for p, _ in stepping}, recorded)
+            for p, g in stepping:
                 if g.is_sparse:
                     raise RuntimeError("AdamW takes no sparse gradients")
                 state = self.state[p]
@@ -390,6 +413,8 @@ class AdamW(torch.optim.Optimizer):
                 if not group["capturable"]:
                     for state in states:
                         state["step"] = step
+                elif recorded and not any(step is c for c in self._in_graph):
+                    self._in_graph += (step,)
         return loss
 
     def load_state_dict(self, state_dict):
