@@ -265,8 +265,9 @@ class PatchMLP_q8(nn.Module):
     """Residual network of dense 8-bit layers on image patches: every patch of ``patch`` x ``patch`` pixels is a row; blocks of
     norm, widening, activation and narrowing; the rows' mean through a last norm and layer.  All products are exact 8-bit ones
     (``utils_class.Linear_Q8``), so it serves as the teacher of an SC network (``python -m geo_amd.main_distill``).  ``gated``: each block's
-    output is normed and gated before it joins the stream (``utils_class.GatedNormLinear_Q8``); ``bias``: the blocks' layers have one.  Not in
-    the reference."""
+    output is normed and gated before it joins the stream (``utils_class.GatedNormLinear_Q8``, which the layer behind the block is, behind the last
+    one the head: every row goes through it, and the logits are their rows' mean); ``bias``: the blocks' layers have one.  Not in the
+    reference."""
 
     def __init__(self, num_classes=10, c_in=3, patch=4, width=256, hidden=1024, depth=4, activation="relu", gated=False, bias=False):
         super().__init__()
@@ -277,7 +278,14 @@ class PatchMLP_q8(nn.Module):
         self.up = nn.ModuleList((utils_class.GatedNormLinear_Q8 if gated and i else utils_class.NormLinear_Q8)(width, hidden, **inner)
                                 for i in range(depth))
         self.down = nn.ModuleList(utils_class.Linear_Q8(hidden, width, bias=bias) for _ in range(depth))
-        self.head = utils_class.NormLinear_Q8(width, num_classes)
+        self.head = (utils_class.GatedNormLinear_Q8 if gated and depth else utils_class.NormLinear_Q8)(width, num_classes)
+
+    def _load_from_state_dict(self, state_dict, prefix, *args):
+        head = self.head
+        if isinstance(head, utils_class.GatedNormLinear_Q8) and prefix + "head.gain" in state_dict and prefix + "head.gate" not in state_dict:
+            # saved when the last block was not gated: as it was
+            self.head = utils_class.NormLinear_Q8(head.weight.shape[1], head.weight.shape[0]).to(head.weight).train(head.training)
+        super()._load_from_state_dict(state_dict, prefix, *args)
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -302,6 +310,8 @@ class PatchMLP_q8(nn.Module):
         for up, down in zip(self.up, self.down):
             wide, total = up(y, total)
             y = down(wide)
+        if isinstance(self.head, utils_class.GatedNormLinear_Q8):
+            return self.head(y, total)[0].mean(1)
         logits, _ = self.head((y if total is None else total + y).mean(1))
         return logits
 
