@@ -135,6 +135,7 @@ C_API = {
     "geo_sc_gated_norm_backward_workspace_size": (ctypes.c_int, [_L, _L, _SZ]),
     "geo_sc_gated_norm_backward": (ctypes.c_int, [ctypes.POINTER(GatedNormDesc), _P, _L, _P, _L] + [_P] * 8 + [ctypes.c_size_t, _P]),
     "geo_sc_adamw": (ctypes.c_int, [_I, ctypes.POINTER(AdamWTensor), ctypes.POINTER(AdamWOptions), _P, ctypes.c_size_t, _P]),
+    "geo_sc_adamw_plan": (ctypes.c_int, [_I, ctypes.POINTER(AdamWTensor), ctypes.POINTER(AdamWOptions)] + [ctypes.POINTER(_I)] * 2),
 }
 
 _lib = None

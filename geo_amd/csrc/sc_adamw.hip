@@ -250,13 +250,8 @@ void run(const Share& s, uint32_t groups, int grad_dtype, int bits, hipStream_t 
     else run<P, f16>(s, groups, bits, stream);
 }
 
-}  // namespace
-}  // namespace geo_sc
-
-using namespace geo_sc;
-
-extern "C" int geo_sc_adamw(int count, const geo_sc_adamw_tensor* tensors, const geo_sc_adamw_options* o, void* workspace,
-                            size_t workspace_bytes, geo_sc_stream_t stream)
+// what a call must have, but for the workspace
+int check(int count, const geo_sc_adamw_tensor* tensors, const geo_sc_adamw_options* o)
 {
     if (count < 0 || (count && !tensors) || !o || o->struct_bytes != sizeof *o) return GEO_SC_ERR_INVALID_ARGUMENT;
     if (!dtype_known(o->param_dtype) || !dtype_known(o->grad_dtype) || (o->state_bits != 8 && o->state_bits != 32) || !(o->lr >= 0) ||
@@ -273,10 +268,69 @@ extern "C" int geo_sc_adamw(int count, const geo_sc_adamw_tensor* tensors, const
             return GEO_SC_ERR_INVALID_ARGUMENT;
         if (t.elements > (int64_t)kTile * (0xffffffffll / kThreads)) return GEO_SC_ERR_UNSUPPORTED;   // (one launch's threads)
     }
+    return GEO_SC_OK;
+}
+
+// Past the caches where what is written fills them, and everything that is loaded lies at whole lines' parts.
+bool past_caches(int count, const geo_sc_adamw_tensor* tensors, const geo_sc_adamw_options* o)
+{
+    const bool eight = o->state_bits == 8;
+    int64_t written = 0;
+    uint64_t places = 0;
+    for (int i = 0; i < count; ++i) {
+        const geo_sc_adamw_tensor& t = tensors[i];
+        written += t.elements * (dtype_bytes(o->param_dtype) + (eight ? 2 : 8) + (t.copy ? dtype_bytes(o->copy_dtype) : 0) + (t.clamped ? 4 : 0));
+        if (t.elements) places |= (uintptr_t)t.param | (uintptr_t)t.grad | (eight ? 0 : (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq);
+    }
+    return streams(written) && places % 16 == 0;
+}
+
+// Calls launch(share, groups) with the tensors of one launch after the other: c's constants, `groups` workgroups.
+template <typename F>
+void in_shares(const Constants& c, int count, const geo_sc_adamw_tensor* tensors, F launch)
+{
+    Share s = {};
+    s.c = c;
+    uint32_t groups = 0;
+    const auto flush = [&]() {
+        if (groups) launch(s, groups);
+        s.count = 0;
+        groups = 0;
+    };
+    for (int i = 0; i < count; ++i) {
+        const geo_sc_adamw_tensor& t = tensors[i];
+        if (!t.elements) continue;
+        const uint32_t more = (uint32_t)((t.elements + kTile - 1) / kTile);
+        if (s.count == kTensors || (uint64_t)groups + more > 0xffffffffll / kThreads) flush();
+        s.first[s.count] = groups;
+        s.tensors[s.count++] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.avg_scale, t.sq_scale, t.copy, t.clamped, t.elements};
+        groups += more;
+    }
+    flush();
+}
+
+}  // namespace
+}  // namespace geo_sc
+
+using namespace geo_sc;
+
+extern "C" int geo_sc_adamw_plan(int count, const geo_sc_adamw_tensor* tensors, const geo_sc_adamw_options* o, int* launches, int* uncached)
+{
+    if (!launches || !uncached) return GEO_SC_ERR_INVALID_ARGUMENT;
+    if (const int rc = check(count, tensors, o)) return rc;
+    *launches = 0;
+    in_shares({}, count, tensors, [&](const Share&, uint32_t) { ++*launches; });
+    *uncached = past_caches(count, tensors, o);
+    return GEO_SC_OK;
+}
+
+extern "C" int geo_sc_adamw(int count, const geo_sc_adamw_tensor* tensors, const geo_sc_adamw_options* o, void* workspace,
+                            size_t workspace_bytes, geo_sc_stream_t stream)
+{
+    if (const int rc = check(count, tensors, o)) return rc;
     if (o->device_step && (!workspace || workspace_bytes < sizeof(Steps) || (uintptr_t)workspace % 8)) return GEO_SC_ERR_WORKSPACE;
     hipStream_t st = (hipStream_t)stream;
-    Share s = {};
-    Constants& c = s.c;
+    Constants c = {};
     c.scale = (float)o->grad_scale;
     c.b1 = (float)o->beta1;
     c.c1 = (float)(1 - o->beta1);
@@ -293,36 +347,14 @@ extern "C" int geo_sc_adamw(int count, const geo_sc_adamw_tensor* tensors, const
     } else {
         c.steps = steps_at(o->lr, o->beta1, o->beta2, o->step);
     }
-    // Past the caches where what is written fills them, and everything lies at whole lines' parts.
-    int64_t written = 0;
-    uint64_t places = 0;
-    for (int i = 0; i < count; ++i) {
-        const geo_sc_adamw_tensor& t = tensors[i];
-        written += t.elements * (dtype_bytes(o->param_dtype) + (eight ? 2 : 8) + (t.copy ? dtype_bytes(o->copy_dtype) : 0));
-        if (t.elements) places |= (uintptr_t)t.param | (uintptr_t)t.grad | (eight ? 0 : (uintptr_t)t.exp_avg | (uintptr_t)t.exp_avg_sq);
-    }
-    c.streamed = streams(written) && places % 16 == 0;
-    uint32_t groups = 0;
+    c.streamed = past_caches(count, tensors, o);
     bool launched = o->device_step;
-    const auto launch = [&]() {
-        if (!groups) return;
+    in_shares(c, count, tensors, [&](const Share& s, uint32_t groups) {
         launched = true;
         if (o->param_dtype == GEO_SC_F32) run<f32>(s, groups, o->grad_dtype, o->state_bits, st);
         else if (o->param_dtype == GEO_SC_BF16) run<bf16>(s, groups, o->grad_dtype, o->state_bits, st);
         else run<f16>(s, groups, o->grad_dtype, o->state_bits, st);
-        s.count = 0;
-        groups = 0;
-    };
-    for (int i = 0; i < count; ++i) {
-        const geo_sc_adamw_tensor& t = tensors[i];
-        if (!t.elements) continue;
-        const uint32_t more = (uint32_t)((t.elements + kTile - 1) / kTile);
-        if (s.count == kTensors || (uint64_t)groups + more > 0xffffffffll / kThreads) launch();
-        s.first[s.count] = groups;
-        s.tensors[s.count++] = {t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.avg_scale, t.sq_scale, t.copy, t.clamped, t.elements};
-        groups += more;
-    }
-    launch();
+    });
     if (!launched) return GEO_SC_OK;
     return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
 }

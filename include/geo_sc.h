@@ -661,6 +661,9 @@ typedef struct geo_sc_adamw_options {
 } geo_sc_adamw_options;
 GEO_SC_API int geo_sc_adamw(int count, const geo_sc_adamw_tensor* tensors, const geo_sc_adamw_options* options, void* workspace,
                             size_t workspace_bytes, geo_sc_stream_t stream);
+/* What geo_sc_adamw does with such tensors: its launches on them, and whether (1, else 0) their loads and stores go past the caches. */
+GEO_SC_API int geo_sc_adamw_plan(int count, const geo_sc_adamw_tensor* tensors, const geo_sc_adamw_options* options, int* launches,
+                                 int* uncached);
 
 #ifdef __cplusplus
 }
