@@ -1485,41 +1485,59 @@ int64_t rounds_of(const TileArgs& a, const TileArgs& b, int tile)
     return (tiles(a) + (b.rows ? tiles(b) : 0) + at_once - 1) / at_once;
 }
 
+void set_splits(TwoProducts* both, const Plan& p)
+{
+    both->first.splits = p.splits[0];
+    both->first.stages_per_split = p.stages_per_split[0];
+    both->second.splits = p.splits[1];
+    both->second.stages_per_split = p.stages_per_split[1];
+}
+uint8_t* const kAligned = (uint8_t*)256;   // of a workspace, for a query
+// How k_tiles goes over its products: whether their rows are taken as they lie, and whether strips are cut off them.
+struct Tiles {
+    bool direct, cut;
+    Strips first, second;
+};
+Tiles tiles_of(const TwoProducts& both, const Plan& p, const Epilogue* e)
+{
+    Tiles t = {};
+    t.direct = is_direct(both.first, p.tile) && (!both.second.rows || is_direct(both.second, p.tile));
+    if (!t.direct || p.tile <= 64 || p.splits[0] != 1 || (both.second.rows && p.splits[1] != 1)) return t;
+    t.first = cut_strips(both.first, p.tile, e);
+    t.second = cut_strips(both.second, p.tile, nullptr);
+    t.cut = rounds_of(t.first.main, t.second.main, p.tile) < rounds_of(both.first, both.second, p.tile);
+    return t;
+}
+
 // Runs one product, or two in one launch (second.rows 0: one).  The caller has made the plan and the partial sums' memory.
 // `e`: the epilogue of the one product, or NULL; where the inner dimension is cut, the join has it.
 template <bool INT8>
 int run_products(TwoProducts both, const Epilogue* e, const Plan& p, hipStream_t s)
 {
     const Epilogue* const now = both.first.partial ? nullptr : e;
-    both.first.splits = p.splits[0];
-    both.first.stages_per_split = p.stages_per_split[0];
-    both.second.splits = p.splits[1];
-    both.second.stages_per_split = p.stages_per_split[1];
+    set_splits(&both, p);
     if (p.few) {
         if (p.few == 1) run_few<1>(both.first, now, s);
         else if (p.few == 2) run_few<2>(both.first, now, s);
         else if (p.few == 3) run_few<3>(both.first, now, s);
         else run_few<4>(both.first, now, s);
     } else {
-        const bool direct = is_direct(both.first, p.tile) && (!both.second.rows || is_direct(both.second, p.tile));
-        if (direct && p.tile > 64 && p.splits[0] == 1 && (!both.second.rows || p.splits[1] == 1)) {
-            const Strips first = cut_strips(both.first, p.tile, now), second = cut_strips(both.second, p.tile, nullptr);
-            if (rounds_of(first.main, second.main, p.tile) < rounds_of(both.first, both.second, p.tile)) {
-                const auto strip = [&](const TileArgs& a, const Epilogue& e) {
-                    TwoProducts one = {};
-                    one.first = a;
-                    return !a.rows || run_tiles<64, INT8>(one, now ? &e : nullptr, true, s);
-                };
-                if (!strip(first.down, first.down_epilogue) || !strip(first.right, first.right_epilogue) || !strip(second.down, {}) ||
-                    !strip(second.right, {}))
-                    return GEO_SC_ERR_UNSUPPORTED;
-                both.first = first.main;
-                both.second = second.main;
-            }
+        const Tiles t = tiles_of(both, p, now);
+        if (t.cut) {
+            const auto strip = [&](const TileArgs& a, const Epilogue& e) {
+                TwoProducts one = {};
+                one.first = a;
+                return !a.rows || run_tiles<64, INT8>(one, now ? &e : nullptr, true, s);
+            };
+            if (!strip(t.first.down, t.first.down_epilogue) || !strip(t.first.right, t.first.right_epilogue) || !strip(t.second.down, {}) ||
+                !strip(t.second.right, {}))
+                return GEO_SC_ERR_UNSUPPORTED;
+            both.first = t.first.main;
+            both.second = t.second.main;
         }
-        const bool fits = p.tile == 256   ? run_tiles<256, INT8>(both, now, direct, s)
-                          : p.tile == 128 ? run_tiles<128, INT8>(both, now, direct, s)
-                                          : run_tiles<64, INT8>(both, now, direct, s);
+        const bool fits = p.tile == 256   ? run_tiles<256, INT8>(both, now, t.direct, s)
+                          : p.tile == 128 ? run_tiles<128, INT8>(both, now, t.direct, s)
+                                          : run_tiles<64, INT8>(both, now, t.direct, s);
         if (!fits) return GEO_SC_ERR_UNSUPPORTED;
     }
     const auto joins = [](const TileArgs& a) { return a.partial ? (uint32_t)((a.rows * ((a.cols + 3) / 4) + 255) / 256) : 0u; };
@@ -1915,6 +1933,32 @@ GradLayout grad_layout(int64_t rows, int64_t cols, int64_t inner, int terms, boo
     return l;
 }
 
+// The products of the gradients on a workspace that begins at `base`, without their outputs; the first is dx, or dw where dx is not wanted.
+TwoProducts grad_products(const GradLayout& l, uint8_t* base, int terms, bool need_dx, bool need_dw)
+{
+    const auto product = [&](const Shape& shape, size_t left, size_t right, size_t back, bool cut, size_t partial) {
+        TileArgs a = {};
+        a.x = base + left;
+        a.w = base + right;
+        a.x_stride = shape.inner;
+        a.w_stride = shape.inner / terms;
+        a.rows = shape.rows;
+        a.cols = shape.cols;
+        a.inner = shape.inner;
+        a.w_stages = (int)(a.w_stride / kStage);
+        a.x_scale = (const float*)(base + back);
+        a.y_stride = shape.cols;
+        a.partial = cut ? (uint32_t*)(base + partial) : nullptr;
+        return a;
+    };
+    TwoProducts both = {};
+    if (need_dx) both.first = product(l.dx, l.dx_left, l.dx_right, l.dx_back, l.plan.splits[0] > 1, l.first_partial);
+    if (need_dw)
+        (need_dx ? both.second : both.first) = product(l.dw, l.dw_left, l.dw_right, l.dw_back, l.plan.splits[need_dx ? 1 : 0] > 1,
+                                                       need_dx ? l.second_partial : l.first_partial);
+    return both;
+}
+
 Plan forward_plan(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t cols, int64_t inner, TileArgs* a)
 {
     a->x = (const uint8_t*)x;
@@ -2056,30 +2100,10 @@ int backward(const void* grad, int grad_dtype, int64_t grad_stride, const void* 
     if (terms == 1) k_grad_operands<1><<<grid, dim3(256), 0, s>>>(o);
     else k_grad_operands<2><<<grid, dim3(256), 0, s>>>(o);
     if (!products) return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
-    const auto product = [&](const Shape& shape, size_t left, size_t right, size_t back, bool cut, size_t partial, void* y, int dtype) {
-        TileArgs a = {};
-        a.x = base + left;
-        a.w = base + right;
-        a.x_stride = shape.inner;
-        a.w_stride = shape.inner / terms;
-        a.rows = shape.rows;
-        a.cols = shape.cols;
-        a.inner = shape.inner;
-        a.w_stages = (int)(a.w_stride / kStage);
-        a.x_scale = (const float*)(base + back);
-        a.y = y;
-        a.y_stride = shape.cols;
-        a.dtype = dtype;
-        a.partial = cut ? (uint32_t*)(base + partial) : nullptr;
-        return a;
-    };
-    TwoProducts both = {};
-    if (dx) both.first = product(l.dx, l.dx_left, l.dx_right, l.dx_back, l.plan.splits[0] > 1, l.first_partial, dx, dx_dtype);
-    if (dw) {
-        const int which = dx ? 1 : 0;
-        (dx ? both.second : both.first) =
-            product(l.dw, l.dw_left, l.dw_right, l.dw_back, l.plan.splits[which] > 1, dx ? l.second_partial : l.first_partial, dw, dw_dtype);
-    }
+    TwoProducts both = grad_products(l, base, terms, dx, dw);
+    if (dx) both.first.y = dx, both.first.dtype = dx_dtype;
+    TileArgs& of_w = dx ? both.second : both.first;
+    if (dw) of_w.y = dw, of_w.dtype = dw_dtype;
     return run_products<false>(both, nullptr, l.plan, s);
 }
 
@@ -2114,6 +2138,42 @@ int geo_sc_matmul_q8_plan(const int8_t* x, int64_t x_stride, const int8_t* w, in
     else *kernel = is_direct(a, plan.tile) || copies.x || copies.w ? GEO_SC_Q8_TILES : GEO_SC_Q8_TILES_ANY;
     *tile = plan.few ? 16 * plan.few : plan.tile;
     *splits = plan.splits[0];
+    return GEO_SC_OK;
+}
+
+int geo_sc_matmul_q8_strips(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t cols, int64_t inner,
+                            int64_t* last_rows, int64_t* last_cols)
+{
+    if (!last_rows || !last_cols || !sizes_fit(rows, cols, inner) || x_stride < 0 || w_stride < 0) return GEO_SC_ERR_INVALID_ARGUMENT;
+    TwoProducts both = {};
+    TileArgs& a = both.first;
+    const Plan plan = forward_plan(x, x_stride, w, w_stride, rows, cols, inner, &a);
+    const Copies copies = copies_of(a, plan, rows, cols);
+    if (copies.x) a.x = kAligned, a.x_stride = (inner + 15) / 16 * 16;
+    if (copies.w) a.w = kAligned, a.w_stride = (inner + 15) / 16 * 16;
+    set_splits(&both, plan);
+    *last_rows = *last_cols = 0;
+    if (plan.few) return GEO_SC_OK;
+    const Tiles t = tiles_of(both, plan, nullptr);
+    if (t.cut) *last_rows = t.first.down.rows, *last_cols = t.first.right.cols;
+    return GEO_SC_OK;
+}
+
+int geo_sc_matmul_q8_backward_strips(int64_t rows, int64_t cols, int64_t inner, int grad_dtype, int need_dx, int need_dw, int64_t* dx_rows,
+                                     int64_t* dx_cols, int64_t* dw_rows, int64_t* dw_cols)
+{
+    if (!dx_rows || !dx_cols || !dw_rows || !dw_cols || !sizes_fit(rows, cols, inner) || !dtype_known(grad_dtype)) return GEO_SC_ERR_INVALID_ARGUMENT;
+    *dx_rows = *dx_cols = *dw_rows = *dw_cols = 0;
+    if (!need_dx && !need_dw) return GEO_SC_OK;
+    const int terms = terms_of(grad_dtype);
+    const GradLayout l = grad_layout(rows, cols, inner, terms, need_dx, need_dw, false);
+    TwoProducts both = grad_products(l, kAligned, terms, need_dx, need_dw);
+    set_splits(&both, l.plan);
+    const Tiles t = tiles_of(both, l.plan, nullptr);
+    if (!t.cut) return GEO_SC_OK;
+    const Strips& of_w = need_dx ? t.second : t.first;
+    if (need_dx) *dx_rows = t.first.down.rows, *dx_cols = t.first.right.cols;
+    if (need_dw) *dw_rows = of_w.down.rows, *dw_cols = of_w.right.cols;
     return GEO_SC_OK;
 }
 

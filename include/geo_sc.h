@@ -521,6 +521,14 @@ GEO_SC_API int geo_sc_matmul_q8_workspace_size(const int8_t* x, int64_t x_stride
 enum geo_sc_q8_kernel { GEO_SC_Q8_FEW_ROWS = 0, GEO_SC_Q8_FEW_STREAMED = 1, GEO_SC_Q8_TILES = 2, GEO_SC_Q8_TILES_ANY = 3 };
 GEO_SC_API int geo_sc_matmul_q8_plan(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t cols,
                                      int64_t inner, int* kernel, int* tile, int* splits);
+/*
+ * The last rows and columns that the product (with an epilogue too), or the products of its backward, take as strips of their own in tiles
+ * of 64 rows, where whole tiles would cost another round of the compute units for them; 0: none.
+ */
+GEO_SC_API int geo_sc_matmul_q8_strips(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t cols,
+                                       int64_t inner, int64_t* last_rows, int64_t* last_cols);
+GEO_SC_API int geo_sc_matmul_q8_backward_strips(int64_t rows, int64_t cols, int64_t inner, int grad_dtype, int need_dx, int need_dw,
+                                                int64_t* dx_rows, int64_t* dx_cols, int64_t* dw_rows, int64_t* dw_cols);
 GEO_SC_API int geo_sc_matmul_q8(const int8_t* x, int64_t x_stride, const float* x_scale, const int8_t* w, int64_t w_stride,
                                 const float* w_scale, int64_t rows, int64_t cols, int64_t inner, void* y, int dtype, void* workspace,
                                 size_t workspace_bytes, geo_sc_stream_t stream);
