@@ -213,7 +213,7 @@ def matmul_q8(q, scale, weight_q, weight_scale, dtype=torch.float32, bias=None, 
     """``y[..., n] = act(scale[...] * weight_scale[n] * sum_k q[..., k] * weight_q[n, k] + bias[n]) + residual[..., n]`` for 8-bit rows with a
     scale each (``quantize_rows``, ``rms_norm_q8``, ``gated_norm_q8``); the integer sum is exact (at most 131071 terms), what follows is
     float32, ``y``, rounded once, of ``dtype``.  ``bias``: (columns,) of any of the three types; ``activation``: None, "relu", "gelu" (z times
-    the normal distribution's share below z) or "silu" (z / (1 + exp(-z))); ``residual``: of y's shape and type.  No gradients: see
+    the normal distribution's share below z, to 0.75e-7 of that) or "silu" (z / (1 + exp(-z))); ``residual``: of y's shape and type.  No gradients: see
     ``linear_q8``."""
     if bias is None and activation is None and residual is None:
         return _dense().matmul_q8(q, scale, weight_q, weight_scale, dtype)
