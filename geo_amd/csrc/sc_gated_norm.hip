@@ -423,6 +423,9 @@ __global__ __launch_bounds__(1024) void k_gated_norm_long(NormArgs a)
     }
 }
 
+// Two chunks a thread, in 16 bits two rows at once, where rows are many and more than a wave's: the channels' vectors are read once for
+// both.  One chunk / two, us: bf16 2048 x 1024 9.3 / 11.1, 4096 x 1024 14.1 / 14.5, 16384 x 1024 41.3 / 36.5, 1024 x 4096 14.0 / 15.1, 2048 x 4096
+// 22.3 / 21.0, 8192 x 4096 73.3 / 70.0, 4096 x 8192 87.3 / 76.2; fp32 within a twentieth either way (4096 x 8192 137 / 131, 8192 x 4096 124 / 132).
 template <typename T, bool EIGHT>
 int run_norm(NormArgs a, int dtype, hipStream_t s)
 {
@@ -863,7 +866,10 @@ int run_back(BackArgs a, int dtype, hipStream_t s)
             const dim3 grid((uint32_t)((n.cols + columns() - 1) / columns()), (uint32_t)(kSums + (by_border ? a.units - 1 : runs)));
             k_join<T, columns(), shares()><<<grid, dim3(columns(), shares()), 0, s>>>(a, by_border);
         };
-        if (n.cols <= 1024) join(std::integral_constant<int, 8>(), std::integral_constant<int, 128>());
+        // Few columns by many shares of the units, or whole lines where the columns are workgroups enough.  8 x 128 / 32 x 16, us: 16384 x 256 fp32
+        // 18 / 107, 8192 x 1024 bf16 22 / 54, 1009 x 1111 fp16 17 / 28, 8192 x 2048 22 / 28, 8192 x 3000 16.6 / 18.4, 8192 x 3500 20.1 / 19.2,
+        // 8192 x 4096 22.8 / 16.1 (all four sums).
+        if (n.cols <= 3000) join(std::integral_constant<int, 8>(), std::integral_constant<int, 128>());
         else join(std::integral_constant<int, 32>(), std::integral_constant<int, 16>());
     }
     return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
