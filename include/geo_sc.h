@@ -542,7 +542,7 @@ GEO_SC_API int geo_sc_matmul_q8_backward(const void* grad, int grad_dtype, int64
 /*
  * The same product with an epilogue: with z = x_scale[m] w_scale[n] sum + bias[n] in fp32, y = act(z) + residual, rounded once.
  * Activations: relu (slope 1 above zero and at NaN, else 0); gelu, z times the normal distribution's share below z, which is within 0.75e-7
- * of it (so that gelu(-5) has an error of 0.14 %), its slope likewise; silu, z / (1 + exp(-z)).
+ * of it (gelu(-5) is 0.16 % off), its slope likewise; silu, z / (1 + exp(-z)).
  *   bias, residual   NULL: none; `cols` elements of bias_dtype, (rows, cols) of y's dtype with residual_stride between its rows
  *   slope            NULL, or (rows, cols), without gaps, for the backward: act'(z) in slope_dtype, GEO_SC_F16, GEO_SC_F32 or, of a
  *                    relu (or no activation), GEO_SC_U8
@@ -598,14 +598,14 @@ GEO_SC_API int geo_sc_distill_topk_backward(const float* grad, int reduction, co
  *   t = residual_scale residual + gate m,   out = t / sqrt(mean_j t[j]^2 + eps) weight
  * in fp32; t is rounded for `total` only.  Rows of any finite x and t.  weight, post_weight and residual_scale are `cols` elements,
  * gate is (rows / rows_per_gate, cols): one for each run of rows_per_gate consecutive rows, which must divide rows.  post_weight, gate and
- * residual_scale may be NULL.  All are of `dtype`.
+ * residual_scale may be NULL.  All are of `dtype`.  Outputs overlap nothing that is read.
  * geo_sc_gated_norm: out and total, (rows, cols) of dtype; rstd NULL, or rows * 2 floats for the backward (both norms' factors).
  * geo_sc_gated_norm_q8: instead of out its rows in 8 bits (as geo_sc_quantize_rows has them, of out in fp32, which is not rounded to dtype
  * on the way), values NULL or what they stand for in values_dtype; desc's rstd is for it alone: NULL, or as above.  (A caller built without that
  * field passes the smaller struct_bytes.)
  * Backward, from the gradients of out and of total (NULL: none), both of dtype: dx and dresidual (rows, cols), and dweight,
  * dpost, dscale (cols) and dgate (of the gate's shape), each NULL where it is not wanted, summed over rows in an order that does not
- * change from run to run.  Workspace, 4-byte aligned: geo_sc_gated_norm_backward_workspace_size.
+ * change from run to run.  (With eps 0, rows whose root mean square is below 3e-39 have factors that are no numbers, and such gradients.)  Workspace, 4-byte aligned: geo_sc_gated_norm_backward_workspace_size.
  */
 typedef struct geo_sc_gated_norm_desc {
     size_t struct_bytes; /* sizeof(geo_sc_gated_norm_desc) */

@@ -2,7 +2,7 @@
 
 gelu: the series has 2 Q(x) to 1.5e-7 absolute (Abramowitz and Stegun 7.1.26) for all x >= 0, so z Q(|z|) to 0.75e-7 |z|; the exponential, the
 reciprocal and some ten fp32 operations around them are allowed 16 U of what they give, which is at most the number's tail for z < 0 and z for
-z > 0.  Relative to a negative tail that is much: 0.14 % of gelu(-5).  silu: an exponential of a product (1.5 U of its exponent
+z > 0.  Relative to a negative tail that is much: 0.16 % of gelu(-5).  silu: an exponential of a product (1.5 U of its exponent
 besides), a reciprocal and a product."""
 import pytest
 import torch
