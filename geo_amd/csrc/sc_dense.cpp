@@ -562,20 +562,19 @@ using MaybeTensors = std::optional<Tensors>;
 
 // What one of the lists of a step must be: on the GPU of the first parameter, side by side, of the parameter's element count (of its
 // blocks'), of the type or types named.
-void in_step(const at::Tensor& t, const char* what, const at::Tensor& first, int64_t elements, std::initializer_list<at::ScalarType> types)
+// `param`: or NULL; what goes with it element by element has its shape.
+void in_step(const at::Tensor& t, const char* what, const at::Tensor& first, int64_t elements, std::initializer_list<at::ScalarType> types,
+             const at::Tensor* param = nullptr)
 {
     with(t, what, first, "params");
     TORCH_CHECK(t.is_contiguous(), what, " must be contiguous");
-    TORCH_CHECK(t.numel() == elements, what, " must have ", elements, " elements, got ", t.numel());
+    if (!param || t.sizes() != param->sizes()) {
+        TORCH_CHECK(t.numel() == elements, what, " must have ", elements, " elements, got ", t.numel());
+        TORCH_CHECK(!param, what, " must have the shape of its parameter, ", param->sizes(), ", got ", t.sizes());
+    }
     for (const at::ScalarType type : types)
         if (t.scalar_type() == type) return;
     TORCH_CHECK(false, what, " must not be ", t.scalar_type());
-}
-// what goes with a parameter element by element
-void beside(const at::Tensor& t, const char* what, const at::Tensor& first, const at::Tensor& param, std::initializer_list<at::ScalarType> types)
-{
-    in_step(t, what, first, param.numel(), types);
-    TORCH_CHECK(t.sizes() == param.sizes(), what, " must have the shape of its parameter, ", param.sizes(), ", got ", t.sizes());
 }
 
 constexpr int64_t kStateBlock = 256;
@@ -613,23 +612,23 @@ void adamw_step(const Tensors& params, const Tensors& grads, const Tensors& exp_
         geo_sc_adamw_tensor t = {};
         t.elements = elements;
         in_step(params[i], "params", first, elements, {at::kFloat, at::kBFloat16, at::kHalf});
-        beside(grads[i], "grads", first, params[i], {at::kFloat, at::kBFloat16, at::kHalf});
+        in_step(grads[i], "grads", first, elements, {at::kFloat, at::kBFloat16, at::kHalf}, &params[i]);
         t.param = write(params[i]);
         t.grad = grads[i].const_data_ptr();
         for (const auto& [state, scales, what, codes, scale] : {std::make_tuple(&exp_avg, &avg_scales, "exp_avg", &t.exp_avg, &t.avg_scale),
                                                                 std::make_tuple(&exp_avg_sq, &sq_scales, "exp_avg_sq", &t.exp_avg_sq, &t.sq_scale)}) {
-            beside((*state)[i], what, first, params[i], {eight ? at::kFloat8_e4m3fn : at::kFloat});
+            in_step((*state)[i], what, first, elements, {eight ? at::kFloat8_e4m3fn : at::kFloat}, &params[i]);
             *codes = write((*state)[i]);
             if (!eight) continue;
             in_step((**scales)[i], "scales", first, blocks, {at::kFloat8_e8m0fnu});
             *scale = (uint8_t*)write((**scales)[i]);
         }
         if (copies) {
-            beside((*copies)[i], "copies", first, params[i], {at::kFloat, at::kBFloat16, at::kHalf});
+            in_step((*copies)[i], "copies", first, elements, {at::kFloat, at::kBFloat16, at::kHalf}, &params[i]);
             t.copy = write((*copies)[i]);
         }
         if (clamped && (*clamped)[i]) {
-            beside(*(*clamped)[i], "clamped", first, params[i], {at::kFloat});
+            in_step(*(*clamped)[i], "clamped", first, elements, {at::kFloat}, &params[i]);
             t.clamped = (float*)write(*(*clamped)[i]);
         }
         const Types types = {dtype_of(params[i].scalar_type(), "params"), dtype_of(grads[i].scalar_type(), "grads"),
