@@ -1724,8 +1724,11 @@ __global__ __launch_bounds__(kPeakWaves * 64) void k_grad_peaks(OperandArgs a)
 }
 
 // The maxima and sums of more than kMostJoined blocks of rows, into the first block's place: every tile of k_grad_operands would
-// read them all (16384 x 1024 in 128 blocks: 50 us, so 37 and 4).
+// read the maxima, of kJoinedElements elements or more in as much time as this takes at the least, and its first tiles add up the sums, one after
+// the other.  k_grad_operands alone / both, us: 5579 x 2138 30 / 28 + 5, 16384 x 256 16.4 / 15.7 + 3.8, 16384 x 1024 31.3 / 26.4 + 3.8, 65536 x 1024
+// 134 / 113 + 4.8; with sums 16384 x 1024 52 / 32 + 4.6, 2000 x 2000 30 / 16 + 10, 65536 x 64 44 / 16 + 4.8.
 constexpr uint32_t kMostJoined = 32;
+constexpr int64_t kJoinedElements = (int64_t)1 << 24;
 __global__ __launch_bounds__(256) void k_join_peaks(OperandArgs a)
 {
     const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
@@ -1784,7 +1787,9 @@ __device__ __forceinline__ void widen_tile(const int8_t* q, int64_t stride, int6
     }
 }
 
-template <int TERMS>
+// (SLOPE by itself, and no more loads of maxima at once than eight waves on a SIMD have registers for: bf16 7266 x 13203 without a slope 194 us, 243
+// with the slope's code in it and eight loads, 205 before there was either; 4096 x 4096 43, 44 and 46.)
+template <int TERMS, bool SLOPE>
 __global__ __launch_bounds__(256) void k_grad_operands(OperandArgs a)
 {
     __shared__ float tile[kSide][kSide + 1];
@@ -1807,7 +1812,7 @@ __global__ __launch_bounds__(256) void k_grad_operands(OperandArgs a)
         for (int j = 0; j < kChunk; ++j) v[i][j] = 0.f;
         if (r0 + r < a.rows && c0 + c < a.cols) {
             load_chunk(a.g, a.dtype, (r0 + r) * a.g_stride, c0 + c, a.cols, 0.f, v[i]);
-            if (a.slope) {
+            if constexpr (SLOPE) {
                 float slope[kChunk];
                 if (a.slope_dtype == GEO_SC_U8) load_columns((const uint8_t*)a.slope + (r0 + r) * a.cols + c0 + c, a.cols - c0 - c, slope);
                 else load_chunk(a.slope, a.slope_dtype, (r0 + r) * a.cols, c0 + c, a.cols, 0.f, slope);
@@ -1824,12 +1829,12 @@ __global__ __launch_bounds__(256) void k_grad_operands(OperandArgs a)
         else ((f16*)a.dbias)[c0 + threadIdx.x] = (f16)sum;
     }
     // the blocks' maxima of the tile's rows and columns, a quarter of the blocks per wave
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const uint32_t wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
     uint32_t row_most = 0, col_most = 0;
     if (a.dx_left && r0 + lane < a.rows)
         for (uint32_t k = wave; k < a.col_blocks; k += 4) row_most = max(row_most, a.row_peaks[k * a.rows + r0 + lane]);
     if (a.dw_left && c0 + lane < a.cols)
-#pragma unroll 8
+#pragma unroll 4
         for (uint32_t k = wave; k < a.row_blocks; k += 4) col_most = max(col_most, a.col_peaks[k * a.cols + c0 + lane]);
     most[0][wave][lane] = row_most;
     most[1][wave][lane] = col_most;
@@ -2092,13 +2097,15 @@ int backward(const void* grad, int grad_dtype, int64_t grad_stride, const void* 
     if (grad_dtype == GEO_SC_F32) peaks(f32());
     else if (grad_dtype == GEO_SC_BF16) peaks(bf16());
     else peaks(f16());
-    if (o.row_blocks > kMostJoined && (o.col_peaks || o.col_sums)) {
+    if (o.row_blocks > kMostJoined && (o.col_sums || (o.col_peaks && rows * cols >= kJoinedElements))) {
         k_join_peaks<<<dim3((uint32_t)((cols + 63) / 64)), dim3(256), 0, s>>>(o);
         o.row_blocks = 1;
     }
     const dim3 grid((uint32_t)(g_tiles + w_tiles + x_tiles));
-    if (terms == 1) k_grad_operands<1><<<grid, dim3(256), 0, s>>>(o);
-    else k_grad_operands<2><<<grid, dim3(256), 0, s>>>(o);
+    if (terms == 1 && slope) k_grad_operands<1, true><<<grid, dim3(256), 0, s>>>(o);
+    else if (terms == 1) k_grad_operands<1, false><<<grid, dim3(256), 0, s>>>(o);
+    else if (slope) k_grad_operands<2, true><<<grid, dim3(256), 0, s>>>(o);
+    else k_grad_operands<2, false><<<grid, dim3(256), 0, s>>>(o);
     if (!products) return hipGetLastError() == hipSuccess ? GEO_SC_OK : GEO_SC_ERR_LAUNCH;
     TwoProducts both = grad_products(l, base, terms, dx, dw);
     if (dx) both.first.y = dx, both.first.dtype = dx_dtype;
