@@ -1438,7 +1438,7 @@ bool run_tiles(TwoProducts both, const Epilogue* e, bool direct, hipStream_t s)
 }
 
 // The rows and columns of a product that its last tiles are for, if they are no more than 64 in a direction, as products of their own
-// in tiles of 64: 4096 x 4099 takes 272 tiles of 256, a second round of the compute units for 48 rows of w's.
+// in tiles of 64: 4096 x 4099 takes 272 tiles of 256, a second round of the compute units for 3 rows of w's.
 constexpr int64_t kMostStrip = 64;
 struct Strips {
     TileArgs main, down, right;   // all but the last rows and columns; the last rows; the last columns of the others (rows 0: none)
@@ -1478,11 +1478,28 @@ Strips cut_strips(const TileArgs& a, int tile, const Epilogue* e)
     }
     return s;
 }
-int64_t rounds_of(const TileArgs& a, const TileArgs& b, int tile)
+int64_t rounds_of(const TileArgs& a, const TileArgs& b, const TileCost& cost)
 {
-    const auto tiles = [&](const TileArgs& t) { return ((t.rows + tile - 1) / tile) * ((t.cols + tile - 1) / tile); };
-    const int64_t at_once = kUnits * (tile == 256 ? 1 : 2);
+    const auto tiles = [&](const TileArgs& t) { return ((t.rows + cost.tile - 1) / cost.tile) * ((t.cols + cost.tile - 1) / cost.tile); };
+    const int64_t at_once = kUnits * cost.held;
     return (tiles(a) + (b.rows ? tiles(b) : 0) + at_once - 1) / at_once;
+}
+// Whether strips cost less than the rounds that they save: those last as long as the shorter product's tiles (a compute unit that ends
+// them early goes on with the longer one's), a strip is a launch by itself whose few workgroups walk its whole inner dimension.
+// Of 158 products and pairs of gradients whose strips save a round, on average within half a per cent of the better way by this rule; 11 off it
+// always with strips (1071 x 2974 x 1955, both gradients bf16, four of them: 102 us, 59 without), 5 never (4095 x 4099 x 2047, one: 67 us, 107
+// without).
+constexpr double kStripRest = 4.5, kStripStage = .16;   // us of a strip, and of each of its stages
+bool strips_pay(const TileArgs& a, const TileArgs& b, const Strips& of_a, const Strips& of_b, int tile)
+{
+    const TileCost& cost = tile == 256 ? kTileCosts[0] : kTileCosts[1];
+    const auto stages = [](const TileArgs& t) { return (double)((t.inner + kStage - 1) / kStage); };
+    const double shorter = b.rows && stages(b) < stages(a) ? stages(b) : stages(a);
+    const double saved = (double)(rounds_of(a, b, cost) - rounds_of(of_a.main, of_b.main, cost)) * (cost.alone * shorter + cost.rest);
+    double spent = 0;
+    for (const TileArgs* t : {&of_a.down, &of_a.right, &of_b.down, &of_b.right})
+        if (t->rows) spent += kStripRest + kStripStage * stages(*t);
+    return saved > spent;
 }
 
 void set_splits(TwoProducts* both, const Plan& p)
@@ -1505,7 +1522,7 @@ Tiles tiles_of(const TwoProducts& both, const Plan& p, const Epilogue* e)
     if (!t.direct || p.tile <= 64 || p.splits[0] != 1 || (both.second.rows && p.splits[1] != 1)) return t;
     t.first = cut_strips(both.first, p.tile, e);
     t.second = cut_strips(both.second, p.tile, nullptr);
-    t.cut = rounds_of(t.first.main, t.second.main, p.tile) < rounds_of(both.first, both.second, p.tile);
+    t.cut = strips_pay(both.first, both.second, t.first, t.second, p.tile);
     return t;
 }
 

@@ -11,7 +11,7 @@ from tests.test_gpu_dense_kernels import aligned
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("shape", [s for s in FORWARD if FORWARD[s][0] == 256] + [(7171, 1025, 257)])
+@pytest.mark.parametrize("shape", FORWARD)
 def test_product(uf, shape):
     m, n, k = shape
     assert any(forward(*shape)[1:])
