@@ -281,13 +281,18 @@ class Linear_Q8(nn.Module):
             warnings.warn("the weight has changed since prepare(), whose result this call takes: prepare() again", stacklevel=3)
         return None if torch.is_grad_enabled() else self._q8
 
+    def _epilogue(self):
+        """(bias, activation); a token's call is bound by its host time, and the search for an attribute of a module is part of it."""
+        parameters = self._parameters
+        return parameters["bias"] if "bias" in parameters else self.bias, self.activation
+
     def forward(self, x, residual=None):
         weight = self._prepared()
-        epilogue = dict(bias=self.bias, activation=self.activation)
+        bias, activation = self._epilogue()
         if weight is None:
-            return utils_functional.linear_q8(x, self.weight, residual=residual, **epilogue)
+            return utils_functional.linear_q8(x, self.weight, bias, activation, residual)
         q, scale, _ = utils_functional.quantize_rows(x)
-        return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype, residual=residual, **epilogue)
+        return utils_functional.matmul_q8(q, scale, *weight, x.dtype, bias, activation, residual)
 
 
 class NormLinear_Q8(Linear_Q8):
@@ -301,11 +306,11 @@ class NormLinear_Q8(Linear_Q8):
 
     def forward(self, x, residual=None):
         weight = self._prepared()
-        epilogue = dict(bias=self.bias, activation=self.activation)
+        bias, activation = self._epilogue()
         if weight is None:
-            return utils_functional.norm_linear_q8(x, self.gain, self.weight, residual=residual, eps=self.eps, **epilogue)
-        q, scale, total, _ = utils_functional.rms_norm_q8(x, self.gain, residual=residual, eps=self.eps)
-        return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype, **epilogue), total
+            return utils_functional.norm_linear_q8(x, self.gain, self.weight, residual, self.eps, bias, activation)
+        q, scale, total, _ = utils_functional.rms_norm_q8(x, self.gain, residual, self.eps)
+        return utils_functional.matmul_q8(q, scale, *weight, x.dtype, bias, activation), total
 
 
 class GatedNormLinear_Q8(NormLinear_Q8):
@@ -321,9 +326,9 @@ class GatedNormLinear_Q8(NormLinear_Q8):
 
     def forward(self, x, residual):
         weight = self._prepared()
-        around = dict(post_weight=self.post_gain, gate=self.gate, residual_scale=self.residual_scale, eps=self.eps)
-        epilogue = dict(bias=self.bias, activation=self.activation)
+        around = self.post_gain, self.gate, self.residual_scale, self.eps
+        bias, activation = self._epilogue()
         if weight is None:
-            return utils_functional.gated_norm_linear_q8(x, residual, self.gain, self.weight, **around, **epilogue)
-        q, scale, total, _ = utils_functional.gated_norm_q8(x, residual, self.gain, **around)
-        return utils_functional.matmul_q8(q, scale, *weight, dtype=x.dtype, **epilogue), total
+            return utils_functional.gated_norm_linear_q8(x, residual, self.gain, self.weight, *around, bias, activation)
+        q, scale, total, _ = utils_functional.gated_norm_q8(x, residual, self.gain, *around)
+        return utils_functional.matmul_q8(q, scale, *weight, x.dtype, bias, activation), total
