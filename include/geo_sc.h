@@ -523,7 +523,7 @@ GEO_SC_API int geo_sc_matmul_q8_plan(const int8_t* x, int64_t x_stride, const in
                                      int64_t inner, int* kernel, int* tile, int* splits);
 /*
  * The last rows and columns that the product (with an epilogue too), or the products of its backward, take as strips of their own in tiles
- * of 64 rows, where whole tiles would cost another round of the compute units for them; 0: none.
+ * of 64 rows, where that costs less than the round of the compute units that whole tiles would take for them; 0: none.
  */
 GEO_SC_API int geo_sc_matmul_q8_strips(const int8_t* x, int64_t x_stride, const int8_t* w, int64_t w_stride, int64_t rows, int64_t cols,
                                        int64_t inner, int64_t* last_rows, int64_t* last_cols);
